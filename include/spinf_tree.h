@@ -334,6 +334,53 @@ int spinf_xdecode_attn_fwd(const spinf_xdec_args* args, void* stream);
 int spinf_xdecode_put(const void* k, int64_t k_g, int64_t k_h, int64_t k_q, const void* v, int64_t v_g, int64_t v_h, int64_t v_q,
                       void* gk, void* gv, const int64_t* step, int32_t G, int32_t h, int32_t Q, int32_t S, int32_t d, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ paged cache
+ * Keys and values of contents that stay after their pass, in pages; the reference keeps no such cache (its decoder copies a pass's keys and
+ * values, spinf_serve/decode.py:129-171).  k, v: [pages, page, hkv, d] bf16 with any strides (elements, multiples of 8; the head dims of a row
+ * contiguous; 16-byte aligned), page a multiple of 16, d in {64, 128, 256, 512}.  A request is a list of pages (stored key s lies in entry s % page of
+ * page table[s / page]) and two lengths: kv_len stored keys, the last q_len of which are the call's new tokens.  Requests may share pages.
+ *
+ * Visibility: new token i of a request (stored key c + i, c = kv_len - q_len) sees stored key s when s <= c + i; of a TREE of new tokens (end, pos
+ * given: the tokens of the request's branches in pre-order, end[t] = the exclusive end of row t's subtree in rows of the call, pos[t] = its position) the
+ * new tokens whose subtree it lies in, and all stored keys below c; on a layer with a window only where pos(i) - pos(s) < window, a stored key's
+ * position being its place s.  A row that sees nothing comes out as zeros with a log-sum of -inf.  A key that a row does not see contributes nothing to
+ * it, whatever the cache holds there.
+ *
+ * spinf_paged_plan_*: the work lists of a call, host only, deterministic; from the lengths, the trees and the geometry.  They serve every layer of that
+ * geometry.  How a request is cut depends on nothing but its own lengths and tree: its outputs are the same bits whatever shares the call.
+ *   counts: [0] wave items, [1] block items, [2] runs, [3] joins, [4] partial rows (workspace: d + 2 floats each).
+ *   export: wave and block [12 int32 each], runs [4], joins [8]; host arrays of the caller, to be copied to the device. */
+typedef struct spinf_paged_plan_args {
+    const int32_t* q_lens; const int32_t* kv_lens; int64_t reqs;
+    const int32_t* end; const int32_t* pos;   /* [sum of q_lens] host arrays, or both NULL */
+    int32_t hq, hkv, d, page, window;         /* window 0: global layer */
+    int32_t variant;                          /* 0 = by the request's size; 1 = wave items only, 2 = block items only (tests, measurements) */
+} spinf_paged_plan_args;
+typedef struct spinf_pagedplan spinf_pagedplan;
+int spinf_paged_plan_build(const spinf_paged_plan_args* args, spinf_pagedplan** out);
+int spinf_paged_plan_counts(const spinf_pagedplan* plan, int64_t counts[5]);
+int spinf_paged_plan_export(const spinf_pagedplan* plan, int32_t* wave, int32_t* block, int32_t* runs, int32_t* joins);
+void spinf_paged_plan_free(spinf_pagedplan* plan);
+
+/* out[t] = softmax over the visible keys of scale q.k (softcap > 0: of softcap tanh(scale q.k / softcap)) times v, for every new token and query head.
+ *   q, out [tokens, hq, d] bf16 (token and head strides in elements, multiples of 8); lse [tokens, hq] fp32 natural log of the sum of exponentials, or NULL;
+ *   table: int32 device array, the requests' pages back to back; every entry a page of k and v (the caller checks that: the kernel reads
+ *   what it is told); end, pos: device copies of the plan's arrays, or NULL; wave .. joins: device copies of the exported lists; workspace: 16-byte aligned,
+ *   part_rows * (d + 2) * 4 bytes, the caller's.  One launch per kind of item and one that joins split rows; nothing is allocated. */
+typedef struct spinf_paged_args {
+    const void* q; void* out; float* lse;
+    int64_t q_tok, q_head, o_tok, o_head;
+    const void* k; const void* v;
+    int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    const int32_t* table; const int32_t* end; const int32_t* pos;
+    const int32_t* wave; const int32_t* block; const int32_t* runs; const int32_t* joins;
+    int64_t n_wave, n_block, n_joins, part_rows;
+    void* workspace; int64_t workspace_bytes;
+    int32_t hq, hkv, d, page, window;
+    float scale, softcap;
+} spinf_paged_args;
+int spinf_paged_attn_fwd(const spinf_paged_args* args, void* stream);
+
 /* ------------------------------------------------------------------------------------------------ yardstick
  * No counterpart in the reference: one launch of a pure v_mfma_f32_32x32x16_bf16 loop on every compute unit (one workgroup of eight
  * waves per CU, iters x 8 MFMAs per wave, operands in registers), for the benchmark's "what do the matrix cores sustain on this
@@ -382,6 +429,8 @@ int spinf_diag_attn_stream(const spinf_attn_args* args, int32_t parts, int32_t n
  * spinf_gdn_pre_args, spinf_gdn_gate_args, spinf_lm_args, spinf_lm_head_args, spinf_xdec_args as this library was built (n must be
  * 7): a binding compares them with its own mirrors of the structures before its first call. */
 int spinf_struct_sizes(int64_t* sizes, int32_t n);
+/* The same for the paged cache: spinf_paged_plan_args, spinf_paged_args (n must be 2). */
+int spinf_paged_struct_sizes(int64_t* sizes, int32_t n);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,710 @@
+// Attention of new tokens over a paged cache of keys and values for gfx950 (MI355X): single tokens, chunks, trees of questions below a
+// stored content.  No counterpart in the reference, whose contents are read anew with every request.
+//
+// Mathematics.  Row = new token x query head; out = sum_s p_s v_s / sum_s p_s over the stored keys s that the row sees, p_s = exp(t_s - ref), t_s the
+// (capped) scaled score, ref a running maximum that is raised, and what was summed so far rescaled, only where a tile's maximum exceeds it by more
+// than TAU (exponents in units of log 2).  Sums, maxima and accumulators are fp32; the p_s are rounded to bf16 once, for the matrix product with V
+// (their sum takes the unrounded ones): an error of at most 2^-8 of each term, of either sign, as the output's own rounding.
+//
+// Tiles.  32 keys; S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_bf16 (a lane owns one row; V^T through ds_read_b64_tr_b16), K and V
+// global -> LDS by DMA in the padded layout of attn_tiles.h.  A tile is two halves of 16 keys and a page a multiple of 16, so a half lies in one
+// page: two scalar reads of the page list per tile, no per-key lookup.  Rows behind the stored keys are never read (the last key is read in their place).
+//
+// Two kernels over the items of csrc/pagedplan.cpp:
+//   wave   few rows: the workgroup's waves share 32 rows and divide the tiles, each with a tile buffer of its own and no barrier; joined at the end
+//   block  many rows: four waves with 32 rows each on the same double-buffered tiles, one barrier per tile
+// and paged_join_kernel where an item's keys were cut into pieces.
+//
+// Keys that a row does not see have p = 0 exactly; 0 x inf or NaN in the matrix product would still be NaN.  Nothing is spent on that in the usual
+// case: a workgroup that masked some tile and whose results are not all finite computes its rows again one by one, over the keys that each of them
+// sees (slow_row).
+#include <hip/hip_runtime.h>
+
+#include <climits>
+
+#include "spinf_tree.h"
+#include "common.h"
+#include "paged.h"
+#include "attn_tiles.h"
+
+namespace {
+
+constexpr int TK = PAGED_TILE;
+constexpr float TAU = 8.f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Params {
+    const __bf16* q; __bf16* out; float* lse;
+    long q_tok, q_head, o_tok, o_head;
+    const char* k; const char* v;
+    long k_page, k_row, k_head, v_page, v_row, v_head;   // bytes
+    const int* table; const int* end; const int* pos;
+    const PagedItem* items; const PagedRun* runs; const PagedJoin* joins;
+    float* part_o; float2* part_ml;
+    int n_items, hq, group, window;
+    int page16; unsigned page_mul; int page_shift;   // 16-key pieces of a page, and the multiplier and shift that divide by it (0: divide by 1)
+    float c, cap_in, cap_out;                        // scale log2 e; with a cap: 2 scale log2 e / cap and cap log2 e
+};
+
+typedef const __attribute__((address_space(4))) int* scalar_ints;
+// a value at a wave-uniform address, through the scalar cache
+__device__ __forceinline__ int sload(const int* p, int i) { return ((scalar_ints)(size_t)p)[__builtin_amdgcn_readfirstlane(i)]; }
+
+__device__ __forceinline__ PagedItem load_item(const PagedItem* items, int i) {
+    PagedItem it;
+    const int* p = (const int*)(items + i);
+    it.cu = sload(p, 0); it.T = sload(p, 1); it.L = sload(p, 2); it.tab = sload(p, 3);
+    it.kvh = sload(p, 4); it.row0 = sload(p, 5); it.first = sload(p, 6); it.runs = sload(p, 7);
+    it.tiles = sload(p, 8); it.part = sload(p, 9);
+    return it;
+}
+
+// the tiles of an item, in order
+struct Walk {
+    const int* at;
+    int kt, count, bits, off, tiles;
+    __device__ __forceinline__ void load() {
+        kt = sload(at, 0);
+        count = sload(at, 1);
+        bits = sload(at, 2);
+    }
+    __device__ __forceinline__ Walk(const PagedRun* runs, const PagedItem& it, int start) : at((const int*)(runs + it.first)), kt(0), count(0), bits(0), off(0), tiles(it.tiles) {
+        if (tiles > 0) load();
+        step(start);
+    }
+    __device__ __forceinline__ bool more() const { return tiles > 0; }
+    __device__ __forceinline__ int tile() const { return kt + off; }
+    __device__ __forceinline__ void step(int n) {
+        tiles -= n;
+        if (tiles <= 0) return;
+        off += n;
+        while (off >= count) {   // (tiles are left, so there is a run behind this one)
+            off -= count;
+            at += 4;
+            load();
+        }
+    }
+};
+
+// where the two halves of a tile lie: byte addresses of the key / value head's row 0 and row 16, and the last row that is stored
+struct Place {
+    const char *k0, *k1, *v0, *v1;
+    int last;
+    __device__ __forceinline__ Place(const Params& p, const PagedItem& it, int kt) {
+        const int n = 2 * kt, end = (it.L - 1) >> 4;
+        last = it.L - 1 - kt * TK < TK - 1 ? it.L - 1 - kt * TK : TK - 1;
+        const int n1 = n + 1 < end ? n + 1 : end;
+        const int a = p.page_mul ? (int)(__umulhi((unsigned)n, p.page_mul) >> p.page_shift) : n;
+        const int b = p.page_mul ? (int)(__umulhi((unsigned)n1, p.page_mul) >> p.page_shift) : n1;
+        const long ia = sload(p.table, it.tab + a), ib = sload(p.table, it.tab + b);
+        const long ra = (long)(n - a * p.page16) * 16, rb = (long)(n1 - b * p.page16) * 16;
+        k0 = p.k + ia * p.k_page + ra * p.k_row + it.kvh * p.k_head;
+        v0 = p.v + ia * p.v_page + ra * p.v_row + it.kvh * p.v_head;
+        k1 = p.k + ib * p.k_page + rb * p.k_row + it.kvh * p.k_head;
+        v1 = p.v + ib * p.v_page + rb * p.v_row + it.kvh * p.v_head;
+    }
+};
+
+// DMA of regions reg0 .. reg0 + N - 1 of a tile (32 rows of W dims) into the LDS tile at `lds`; RS: distance of its regions
+template <int W, int N, int RS>
+__device__ __forceinline__ void fetch(const char* b0, const char* b1, long row, int last, int reg0, unsigned lds, int lane) {
+    using G = Geo<W, TK>;
+    const int slot = lane / G::CPR, chunk = lane % G::CPR;
+    if (last == TK - 1 && b1 == b0 + 16 * row) {   // 32 rows, one after the other: a uniform base and a constant per lane
+        const unsigned off = (unsigned)(slot * G::NREG * (int)row + chunk * 16);
+#pragma unroll
+        for (int i = 0; i < N; i++) dma16_uniform(b0 + (reg0 + i) * row, off, lds + (reg0 + i) * RS);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            int r = reg0 + i + G::NREG * slot;
+            r = r < last ? r : last;
+            const char* b = r >= 16 ? b1 : b0;
+            dma16_lane(b + (r & 15) * row + chunk * 16, lds + (reg0 + i) * RS);
+        }
+    }
+}
+
+// subtree ends and positions of a tile's new tokens into 2 x 256 bytes of LDS (the 32 keys twice)
+__device__ __forceinline__ void fetch_meta(const Params& p, const PagedItem& it, int kt, unsigned lds, int lane) {
+    int u = kt * TK + (lane & (TK - 1)) - (it.L - it.T);
+    u = u < 0 ? 0 : u < it.T ? u : it.T - 1;
+    dma4_lane(p.end + it.cu + u, lds);
+    dma4_lane(p.pos + it.cu + u, lds + 256);
+}
+
+constexpr int vmcnt_imm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }   // waits for all but the n youngest vector memory operations
+constexpr int LGKM0 = 0xc07f;                                                     // waits for every LDS operation
+
+// A wave's 32 rows: queries, output accumulators, softmax state
+template <int D, int DV, bool CAP>
+struct Rows {
+    using GK = Geo<D, TK>;
+    using GV = Geo<DV, TK>;
+    static constexpr int NS = D / 16, NDT = DV / 32;
+    bf16x8 qf[NS];
+    f32x16 o[NDT];
+    float M, l;
+    int lane, m, g, tok, head, qpos;
+    bool valid;
+
+    __device__ __forceinline__ void load(const Params& p, const PagedItem& it, int row0) {
+        lane = threadIdx.x & 63;
+        m = lane & 31;
+        g = lane >> 5;
+        const int N = it.T * p.group, row = row0 + m;
+        valid = row < N;
+        const int r = valid ? row : N - 1;
+        tok = r / p.group;
+        head = it.kvh * p.group + (r - tok * p.group);
+        const __bf16* qp = p.q + (long)(it.cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
+        qpos = it.L - it.T + tok;
+        if (p.window && p.pos) qpos = p.pos[it.cu + tok];
+        // (waited for here: left to the compiler, the wait would sit at the first use inside the tile loop, behind the DMAs in flight)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+#pragma unroll
+        for (int s = 0; s < NS; s++) asm volatile("" : "+v"(qf[s]));
+        asm volatile("" : "+v"(qpos));
+    }
+    __device__ __forceinline__ void reset() {
+        M = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[dt][i] = 0.f;
+    }
+    // scores of a tile; register i holds key 8 (i / 4) + 4 g + i % 4
+    __device__ __forceinline__ void scores(const char* kt_lds, f32x16& s) {
+        const char* krow = kt_lds + GK::k_off(m) + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+        for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(krow + 32 * st), qf[st], s, 0, 0, 0);
+    }
+    // (four keys at a time, a scheduling barrier in between: requested all at once, the keys' ends and positions would cost the tile loop its registers)
+    __device__ __forceinline__ void mask(const Params& p, const PagedItem& it, int kt, const int* meta, bool tree, f32x16& s) {
+        const int u0 = kt * TK - (it.L - it.T) + 4 * g;   // key 8 i4 + j of this lane is new token u0 + 8 i4 + j of the request (below 0: stored before)
+        const int sees = p.window ? p.window : INT_MAX, far = p.window ? qpos - (kt * TK + 4 * g) : 0;   // distance to the lane's first key
+        if (!tree) {
+            // keys first .. last of the lane's: the rows' own key last, the window's first
+            const int last = tok - u0, first = far - sees;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int k = 8 * (i >> 2) + (i & 3);
+                s[i] = (k <= last) & (k > first) ? s[i] : -INFINITY;
+            }
+        } else {
+            const int row = it.cu + tok;
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) {
+                __builtin_amdgcn_sched_barrier(0);
+                const int4 e = *(const int4*)(meta + 8 * i4 + 4 * g), ps = *(const int4*)(meta + 64 + 8 * i4 + 4 * g);
+                const int ev[4] = {e.x, e.y, e.z, e.w}, pv[4] = {ps.x, ps.y, ps.z, ps.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int k = 8 * i4 + j;
+                    const bool fresh = u0 + k >= 0;
+                    bool vis = (u0 + k <= tok) & (!fresh | (row < ev[j]));
+                    if (p.window) vis = vis & ((fresh ? qpos - pv[j] : far - k) < sees);
+                    s[4 * i4 + j] = vis ? s[4 * i4 + j] : -INFINITY;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // scores -> probabilities; raises the reference and rescales where it has to
+    __device__ __forceinline__ void softmax(const Params& p, f32x16& s, bf16x8 (&pb)[2]) {
+        if (CAP) {   // cap * tanh(scale s / cap) in units of log 2; a masked score stays -inf
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float e = __builtin_amdgcn_exp2f(s[i] * p.cap_in);
+                const float t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
+                s[i] = s[i] == -INFINITY ? -INFINITY : t;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
+        mx = lane32_max(mx);
+        if (!CAP) mx *= p.c;
+        const bool up = mx > M + TAU;
+        const float mn = up ? mx : M;
+        const float alpha = up ? __builtin_amdgcn_exp2f(M - mn) : 1.0f;
+        if (__builtin_amdgcn_ballot_w64(up && M != -INFINITY) != 0) {   // (rows without a key so far hold zeros)
+#pragma unroll
+            for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
+        }
+        l *= alpha;
+        M = mn;
+        const float ms = M == -INFINITY ? 0.f : M;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float pr = __builtin_amdgcn_exp2f(CAP ? s[i] - ms : __builtin_fmaf(s[i], p.c, -ms));
+            sum += pr;
+            pb[i >> 3][i & 7] = (__bf16)pr;
+        }
+        l += sum;
+    }
+    __device__ __forceinline__ void values(const char* vt_lds, const bf16x8 (&pb)[2]) {
+        const int tr_a = lane & 3, tr_j = (lane >> 2) & 3, tr_mb = (lane >> 4) & 1;
+        const char* vrow = vt_lds + GV::v_off(4 * g + tr_j) + 32 * tr_mb + 8 * tr_a;
+#pragma unroll
+        for (int f = 0; f < 2 * NDT; f++) {
+            const char* vp = vrow + GV::v_off(16 * (f / NDT)) + 64 * (f % NDT);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)vp);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vp + GV::v_off(8)));
+            const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[f % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb[f / NDT], o[f % NDT], 0, 0, 0);
+        }
+    }
+    // is some result of the wave's rows not finite?
+    __device__ __forceinline__ bool spoilt() const {
+        float t = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) t += o[dt][i] * 0.f;
+        return __builtin_amdgcn_ballot_w64(valid && !(t == 0.f)) != 0;
+    }
+};
+
+// 1 / sum; rows that saw nothing come out as zeros
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.0f / sum; }
+__device__ __forceinline__ float log_sum(float M, float sum) { return sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * LN2; }
+
+// One row of an item by a whole wave, from memory: what a workgroup falls back to for all its rows where a result is not finite.  A key's values are
+// touched only where the row sees the key.
+template <int D, int DV, bool CAP>
+__device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol) {
+    constexpr int VEC = DV / 64;   // output dims per lane
+    const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+    const int c = it.L - it.T, tok = (it.row0 + j) / p.group, head = it.kvh * p.group + (it.row0 + j - tok * p.group);
+    const __bf16* q = p.q + (long)(it.cu + tok) * p.q_tok + (long)head * p.q_head + g * (D / 2);
+    const int qpos = p.window && p.pos ? p.pos[it.cu + tok] : c + tok;
+    float o[VEC], M = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int x = 0; x < VEC; x++) o[x] = 0.f;
+#pragma unroll 1
+    for (Walk at(p.runs, it, 0); at.more(); at.step(1)) {
+        const Place pl(p, it, at.tile());
+        const int r = m < pl.last ? m : pl.last, u = at.tile() * TK + m - c;
+        const bool fresh = p.end && u >= 0 && u < it.T;
+        bool vis = u <= tok && m <= pl.last;
+        if (fresh) vis = vis && it.cu + tok < p.end[it.cu + u];
+        if (p.window) vis = vis && qpos - (fresh ? p.pos[it.cu + u] : at.tile() * TK + m) < p.window;
+        // lane (m, g): half g of the dims of key m
+        const __bf16* kr = (const __bf16*)((r >= 16 ? pl.k1 : pl.k0) + (r & 15) * p.k_row) + g * (D / 2);
+        float s = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D / 2; d += 8) {
+            const bf16x8 a = *(const bf16x8*)(q + d), b = *(const bf16x8*)(kr + d);
+#pragma unroll
+            for (int x = 0; x < 8; x++) s = __builtin_fmaf((float)a[x], (float)b[x], s);
+        }
+        s = lane32_sum(s);
+        float t = s * p.c;
+        if (CAP) t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f));
+        t = vis ? t : -INFINITY;
+        float mx = t;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+        const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn, alpha = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - ms);
+        const float pr = __builtin_amdgcn_exp2f(t - ms);
+        M = mn;
+        float sum = pr;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor(sum, d);
+        l = l * alpha + sum;
+#pragma unroll
+        for (int x = 0; x < VEC; x++) o[x] *= alpha;
+        unsigned see = (unsigned)__builtin_amdgcn_ballot_w64(vis);
+#pragma unroll 1
+        while (see) {
+            const int key = __builtin_ctz(see);
+            see &= see - 1;
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pr), key));
+            const __bf16* vr = (const __bf16*)((key >= 16 ? pl.v1 : pl.v0) + (key & 15) * p.v_row) + vcol + VEC * lane;
+#pragma unroll
+            for (int x = 0; x < VEC; x++) o[x] = __builtin_fmaf(w, (float)vr[x], o[x]);
+        }
+    }
+    if (it.part >= 0) {
+        float* dst = p.part_o + (long)(it.part + j) * D + vcol + VEC * lane;
+#pragma unroll
+        for (int x = 0; x < VEC; x++) dst[x] = o[x];
+        if (lane == 0 && vcol == 0) p.part_ml[it.part + j] = make_float2(M, l);
+    } else {
+        __bf16* dst = p.out + (long)(it.cu + tok) * p.o_tok + (long)head * p.o_head + vcol + VEC * lane;
+        const float inv = inverse(l);
+#pragma unroll
+        for (int x = 0; x < VEC; x++) dst[x] = (__bf16)(o[x] * inv);
+        if (p.lse && lane == 0 && vcol == 0) p.lse[(long)(it.cu + tok) * p.hq + head] = log_sum(M, l);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ waves that share rows and divide the keys
+template <int D, int DV, int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(const Params p) {
+    using R = Rows<D, DV, CAP>;
+    using GK = typename R::GK;
+    using GV = typename R::GV;
+    constexpr int TILE = GK::KTILEB + GV::VTILEB + 512;
+    constexpr int OROW = DV + 4;   // floats of a row of the exchange (16 bytes of padding: rows of neighbouring lanes fall on other banks)
+    constexpr int LDS = NW * TILE > NW * 32 * OROW * 4 ? NW * TILE : NW * 32 * OROW * 4;
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    __shared__ float2 ml[NW][32];
+    int b = blockIdx.x;
+    int vcol = 0;
+    if (DV < D) {   // (the workgroups of the two halves run on one XCD, close in time, and read the keys through one L2)
+        vcol = ((b >> 3) & 1) * DV;
+        b = (b >> 4) * 8 + (b & 7);
+        if (b >= p.n_items) return;
+    }
+    const PagedItem it = load_item(p.items, b);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = it.L - it.T;
+    R rows;
+    rows.load(p, it, it.row0);
+    char* const kb = lds + w * TILE;
+    char* const vb = kb + GK::KTILEB;
+    int* const meta = (int*)(vb + GV::VTILEB);
+    const unsigned k_at = lds_addr(kb), v_at = lds_addr(vb), m_at = lds_addr(meta);
+    constexpr int NK = GK::NREG, NV = GV::NREG;
+
+    bool tree = false, seen_mask = false;
+    rows.reset();
+    {
+        Walk at(p.runs, it, w);
+        const auto is_tree = [&](const Walk& x) { return p.end != nullptr && (x.bits & 16) && x.tile() * TK + TK > c; };
+        if (at.more()) {
+            const Place pl(p, it, at.tile());
+            tree = is_tree(at);
+            if (tree) fetch_meta(p, it, at.tile(), m_at, rows.lane);
+            fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
+            fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, 0, v_at, rows.lane);
+        }
+        while (at.more()) {
+            const int kt = at.tile();
+            const bool masked = at.bits & 16;
+            seen_mask |= masked;
+            at.step(NW);
+            const bool next = at.more();
+            const Place pl(p, it, next ? at.tile() : kt);
+            const bool next_tree = next && is_tree(at);
+            f32x16 s;
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(NV));   // the keys (and ends, positions) are there; the values may still be on their way
+            __builtin_amdgcn_sched_barrier(0);
+            rows.scores(kb, s);
+            if (masked) rows.mask(p, it, kt, meta, tree, s);
+            __builtin_amdgcn_s_waitcnt(LGKM0);           // nothing reads the tile's keys any more
+            __builtin_amdgcn_sched_barrier(0);
+            if (next) {
+                if (next_tree) fetch_meta(p, it, at.tile(), m_at, rows.lane);
+                fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
+            }
+            bf16x8 pb[2];
+            rows.softmax(p, s, pb);
+            if (!next) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            else if (next_tree) __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK + 2));
+            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK));
+            __builtin_amdgcn_sched_barrier(0);
+            rows.values(vb, pb);
+            __builtin_amdgcn_s_waitcnt(LGKM0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (next) fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, 0, v_at, rows.lane);
+            tree = next_tree;
+        }
+    }
+    if (__syncthreads_or(seen_mask && rows.spoilt())) {
+        for (int j = w; j < 32 && it.row0 + j < it.T * p.group; j += NW) slow_row<D, DV, CAP>(p, it, j, vcol);
+        return;
+    }
+
+    // ---- join the waves: every wave leaves its references and sums, then its accumulators scaled to the largest reference
+    const float sum = lane32_sum(rows.l);
+    if (rows.g == 0) ml[w][rows.m] = make_float2(rows.M, sum);
+    __syncthreads();   // (and every wave is done with its tiles)
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; x++) top = fmaxf(top, ml[x][rows.m].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < NW; x++) total += ml[x][rows.m].y * (NW == 1 || ml[x][rows.m].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[x][rows.m].x - ref));
+    const float mine = NW == 1 || rows.M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(rows.M - ref);
+    const float f = it.part < 0 ? mine * inverse(total) : mine;
+    float* const stage = (float*)lds;
+#pragma unroll
+    for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++)
+            *(float4*)(stage + (w * 32 + rows.m) * OROW + 32 * dt + 8 * i4 + 4 * rows.g) =
+                make_float4(rows.o[dt][4 * i4] * f, rows.o[dt][4 * i4 + 1] * f, rows.o[dt][4 * i4 + 2] * f, rows.o[dt][4 * i4 + 3] * f);
+    if (w == 0 && rows.g == 0 && rows.valid && vcol == 0) {
+        if (it.part >= 0) p.part_ml[it.part + rows.m] = make_float2(top, total);
+        else if (p.lse) p.lse[(long)(it.cu + rows.tok) * p.hq + rows.head] = log_sum(top, total);
+    }
+    __syncthreads();
+    const int here = it.T * p.group - it.row0 < 32 ? it.T * p.group - it.row0 : 32;
+    constexpr int PIECES = DV / 8;
+    for (int i = threadIdx.x; i < here * PIECES; i += 64 * NW) {
+        const int j = i / PIECES, d = (i - j * PIECES) * 8;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = stage[j * OROW + d + k];
+#pragma unroll
+        for (int y = 1; y < NW; y++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] += stage[(y * 32 + j) * OROW + d + k];
+        if (it.part >= 0) {
+            float* dst = p.part_o + (long)(it.part + j) * D + vcol + d;
+            *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
+            *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            const int row = it.row0 + j, tok = row / p.group, head = it.kvh * p.group + (row - tok * p.group);
+            bf16x8 y;
+#pragma unroll
+            for (int k = 0; k < 8; k++) y[k] = (__bf16)x[k];
+            *(bf16x8*)(p.out + (long)(it.cu + tok) * p.o_tok + (long)head * p.o_head + vcol + d) = y;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ waves with rows of their own on the same tiles
+template <int D, int DV, bool CAP>
+__global__ __launch_bounds__(256, D == 512 ? 1 : 2) void paged_block_kernel(const Params p) {
+    using R = Rows<D, DV, CAP>;
+    using GK = typename R::GK;
+    using GV = typename R::GV;
+    constexpr int BUF = GK::KTILEB + GV::VTILEB + 512;
+    constexpr int OROW = DV * 2 + 16;   // bytes of an output row in LDS
+    constexpr int LDS = 2 * BUF > 4 * 32 * OROW ? 2 * BUF : 4 * 32 * OROW;
+    constexpr int NK = GK::NREG / 4, NV = GV::NREG / 4;
+    static_assert(NK * 4 == GK::NREG && NV * 4 == GV::NREG, "a tile's regions must divide among the four waves");
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    int b = blockIdx.x;
+    int vcol = 0;
+    if (DV < D) {
+        vcol = ((b >> 3) & 1) * DV;
+        b = (b >> 4) * 8 + (b & 7);
+        if (b >= p.n_items) return;
+    }
+    const PagedItem it = load_item(p.items, b);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = it.L - it.T;
+    R rows;
+    rows.load(p, it, it.row0 + 32 * w);
+    const unsigned base = lds_addr(lds);
+    const auto is_tree = [&](const Walk& x) { return p.end != nullptr && (x.bits & 0xf0) && x.tile() * TK + TK > c; };
+    const auto issue = [&](const Walk& x, int buf) {
+        const Place pl(p, it, x.tile());
+        const unsigned at = base + buf * BUF;
+        fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, w * NK, at, rows.lane);
+        fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, w * NV, at + GK::KTILEB, rows.lane);
+        if (w == 0 && is_tree(x)) fetch_meta(p, it, x.tile(), at + GK::KTILEB + GV::VTILEB, rows.lane);
+    };
+
+    bool seen_mask = false;
+    rows.reset();
+    {
+        Walk at(p.runs, it, 0);
+        if (at.more()) issue(at, 0);
+        for (int buf = 0; at.more(); buf ^= 1) {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
+            __syncthreads();                            // ... and everybody's; the other buffer is free
+            const int kt = at.tile(), bits = at.bits >> w;
+            const bool tree = is_tree(at);
+            at.step(1);
+            if (at.more()) issue(at, buf ^ 1);
+            // A row group that sees nothing of the tile is computed all the same (masked): its wave would wait for the others at the barrier anyway,
+            // and a branch around the products makes the compiler keep the accumulators twice (256 dims: 205 registers spilled).
+            const bool masked = (bits & 17) != 1;
+            seen_mask |= masked;
+            const char* kb = lds + buf * BUF;
+            f32x16 s;
+            rows.scores(kb, s);
+            if (masked) rows.mask(p, it, kt, (const int*)(kb + GK::KTILEB + GV::VTILEB), tree, s);
+            bf16x8 pb[2];
+            rows.softmax(p, s, pb);
+            rows.values(kb + GK::KTILEB, pb);
+        }
+    }
+    // (also the barrier behind which the tile buffers are free)
+    if (__syncthreads_or(seen_mask && rows.spoilt())) {
+        for (int j = w; j < 128 && it.row0 + j < it.T * p.group; j += 4) slow_row<D, DV, CAP>(p, it, j, vcol);
+        return;
+    }
+
+    const float sum = lane32_sum(rows.l);
+    const float f = it.part < 0 ? inverse(sum) : 1.f;
+    if (it.part >= 0) {
+        if (!rows.valid) return;
+        const long prow = it.part + 32 * w + rows.m;
+        if (rows.g == 0 && vcol == 0) p.part_ml[prow] = make_float2(rows.M, sum);
+        float* po = p.part_o + prow * D + vcol;
+#pragma unroll
+        for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++)
+                *(float4*)(po + 32 * dt + 8 * i4 + 4 * rows.g) = make_float4(rows.o[dt][4 * i4], rows.o[dt][4 * i4 + 1], rows.o[dt][4 * i4 + 2], rows.o[dt][4 * i4 + 3]);
+        return;
+    }
+    if (p.lse && rows.g == 0 && rows.valid && vcol == 0) p.lse[(long)(it.cu + rows.tok) * p.hq + rows.head] = log_sum(rows.M, sum);
+    // rows through the wave's own slice of LDS, stored as 16-byte pieces
+    char* const stage = lds + w * 32 * OROW;
+#pragma unroll
+    for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++) {
+            bf16x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = (__bf16)(rows.o[dt][4 * i4 + j] * f);
+            *(bf16x4*)(stage + rows.m * OROW + (32 * dt + 8 * i4 + 4 * rows.g) * 2) = x;
+        }
+    const int row0 = it.row0 + 32 * w, here = it.T * p.group - row0;
+    constexpr int PIECES = DV / 8;
+#pragma unroll
+    for (int k = 0; k < 32 * PIECES / 64; k++) {
+        const int i = k * 64 + rows.lane, j = i / PIECES, d = (i - j * PIECES) * 8;
+        if (j < here) {
+            const int row = row0 + j, tok = row / p.group, head = it.kvh * p.group + (row - tok * p.group);
+            *(bf16x8*)(p.out + (long)(it.cu + tok) * p.o_tok + (long)head * p.o_head + vcol + d) = *(const bf16x8*)(stage + j * OROW + d * 2);
+        }
+    }
+}
+
+// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces, in ascending order; a wave per row
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
+    constexpr int VEC = D / 64;
+    typedef __attribute__((ext_vector_type(VEC))) float vec;
+    typedef __attribute__((ext_vector_type(VEC))) __bf16 bvec;
+    const int lane = threadIdx.x & 63;
+    const int i = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int* jp = (const int*)(p.joins + (i >> 5));
+    const int j = i & 31;
+    if (j >= sload(jp, 3)) return;
+    const int cu = sload(jp, 0), kvh = sload(jp, 1), row = sload(jp, 2) + j, n = sload(jp, 5), stride = sload(jp, 6);
+    const long part = (long)sload(jp, 4) + j;
+    const int tok = row / p.group, head = kvh * p.group + (row - tok * p.group);
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 64) top = fmaxf(top, p.part_ml[part + (long)s * stride].x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -INFINITY ? 0.f : top;
+    vec acc = (vec)(0.f);
+    float total = 0.f;
+    for (int s0 = 0; s0 < n; s0 += 4) {   // four pieces requested at a time
+        vec x[4];
+        float2 ml[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const long at = part + (long)(s0 + k < n ? s0 + k : n - 1) * stride;
+            x[k] = *(const vec*)(p.part_o + at * D + VEC * lane);
+            ml[k] = p.part_ml[at];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (s0 + k >= n) break;
+            const float f = ml[k].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[k].x - ref);   // (a piece without a visible key holds zeros, or NaN that stays)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) acc[e] = __builtin_fmaf(f, x[k][e], acc[e]);
+            total = __builtin_fmaf(f, ml[k].y, total);
+        }
+    }
+    const float inv = inverse(total);
+    bvec y;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) y[e] = (__bf16)(acc[e] * inv);
+    *(bvec*)(p.out + (long)(cu + tok) * p.o_tok + (long)head * p.o_head + VEC * lane) = y;
+    if (p.lse && lane == 0) p.lse[(long)(cu + tok) * p.hq + head] = log_sum(top, total);
+}
+
+template <int D, int DV, int NW, bool CAP>
+int launch(Params p, const spinf_paged_args* a, hipStream_t s) {
+    auto grid = [](int64_t n) { return dim3((unsigned)(D / DV == 2 ? (n + 7) / 8 * 16 : n)); };
+    hipError_t e = hipSuccess;
+    if (a->n_block) {
+        p.items = (const PagedItem*)a->block;
+        p.n_items = (int)a->n_block;
+        hipLaunchKernelGGL((paged_block_kernel<D, DV, CAP>), grid(a->n_block), dim3(256), 0, s, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && a->n_wave) {
+        p.items = (const PagedItem*)a->wave;
+        p.n_items = (int)a->n_wave;
+        hipLaunchKernelGGL((paged_wave_kernel<D, DV, NW, CAP>), grid(a->n_wave), dim3(64 * NW), 0, s, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && a->n_joins) {
+        hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a->n_joins * 8)), dim3(256), 0, s, p);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "paged_attn: launch: %s", hipGetErrorString(e));
+}
+
+template <int D, int DV, int NW>
+int launch_cap(const Params& p, const spinf_paged_args* a, hipStream_t s) {
+    return a->softcap > 0.f ? launch<D, DV, NW, true>(p, a, s) : launch<D, DV, NW, false>(p, a, s);
+}
+
+}  // namespace
+
+extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
+    if (!a) return spinf_fail(SPINF_E_ARG, "paged_attn: null args");
+    if (a->n_wave < 0 || a->n_block < 0 || a->n_joins < 0 || a->part_rows < 0 || a->n_wave > (1 << 26) || a->n_block > (1 << 26) || a->n_joins > (1 << 26))
+        return spinf_fail(SPINF_E_ARG, "paged_attn: bad item counts");
+    if (a->n_wave + a->n_block == 0) return SPINF_OK;
+    if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv) return spinf_fail(SPINF_E_ARG, "paged_attn: %d query heads do not group over %d key / value heads", a->hq, a->hkv);
+    if (a->page < 16 || a->page % 16 || a->page > (1 << 20)) return spinf_fail(SPINF_E_ARG, "paged_attn: pages of %d keys (a multiple of 16)", a->page);
+    if (a->window < 0) return spinf_fail(SPINF_E_ARG, "paged_attn: window %d", a->window);
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY) || !(a->softcap >= 0.f) || !(a->softcap < INFINITY))
+        return spinf_fail(SPINF_E_ARG, "paged_attn: scale %g must be positive and finite, softcap %g not negative", (double)a->scale, (double)a->softcap);
+    if (!a->q || !a->out || !a->k || !a->v || !a->table || !a->runs || (a->n_wave && !a->wave) || (a->n_block && !a->block) || (a->n_joins && !a->joins))
+        return spinf_fail(SPINF_E_ARG, "paged_attn: null pointer");
+    if ((a->end == nullptr) != (a->pos == nullptr)) return spinf_fail(SPINF_E_ARG, "paged_attn: a tree needs both end and pos");
+    for (const void* ptr : {a->q, (const void*)a->out, a->k, a->v, (const void*)a->wave, (const void*)a->block, (const void*)a->runs, (const void*)a->joins})
+        if ((uintptr_t)ptr % 16) return spinf_fail(SPINF_E_ARG, "paged_attn: tensors and lists must be 16-byte aligned");
+    for (int64_t st : {a->q_tok, a->q_head, a->o_tok, a->o_head, a->k_page, a->k_row, a->k_head, a->v_page, a->v_row, a->v_head})
+        if (st % 8) return spinf_fail(SPINF_E_ARG, "paged_attn: strides must be multiples of 8 elements");
+    if (a->k_row < 0 || a->v_row < 0 || a->k_row > (1 << 24) || a->v_row > (1 << 24))   // (32 rows are reached by 32-bit byte offsets)
+        return spinf_fail(SPINF_E_ARG, "paged_attn: row strides of the cache must lie in 0 .. 2^24");
+    const int64_t need = a->part_rows * (a->d + 2) * 4;
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
+        return spinf_fail(SPINF_E_ARG, "paged_attn: split rows need a 16-byte aligned workspace of %lld bytes", (long long)need);
+    Params p = {};
+    p.q = (const __bf16*)a->q; p.out = (__bf16*)a->out; p.lse = a->lse;
+    p.q_tok = a->q_tok; p.q_head = a->q_head; p.o_tok = a->o_tok; p.o_head = a->o_head;
+    p.k = (const char*)a->k; p.v = (const char*)a->v;
+    p.k_page = 2 * a->k_page; p.k_row = 2 * a->k_row; p.k_head = 2 * a->k_head;
+    p.v_page = 2 * a->v_page; p.v_row = 2 * a->v_row; p.v_head = 2 * a->v_head;
+    p.table = a->table; p.end = a->end; p.pos = a->pos;
+    p.runs = (const PagedRun*)a->runs; p.joins = (const PagedJoin*)a->joins;
+    p.part_o = (float*)a->workspace;
+    p.part_ml = (float2*)(p.part_o + a->part_rows * a->d);
+    p.hq = a->hq; p.group = a->hq / a->hkv; p.window = a->window;
+    // n / page16 for n < 2^27 as the high word of a product: multiplier ceil(2^(31 + b) / page16), b = ceil(log2 page16), shift b - 1
+    p.page16 = a->page / 16;
+    if (p.page16 > 1) {
+        int b = 0;
+        while ((1 << b) < p.page16) b++;
+        p.page_mul = (unsigned)(((1ull << (31 + b)) + p.page16 - 1) / p.page16);
+        p.page_shift = b - 1;
+    }
+    p.c = a->scale * LOG2E;
+    p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
+    p.cap_out = a->softcap * LOG2E;
+    hipStream_t s = (hipStream_t)stream;
+    switch (a->d) {
+        case 64: return launch_cap<64, 64, 4>(p, a, s);
+        case 128: return launch_cap<128, 128, 4>(p, a, s);
+        case 256: return launch_cap<256, 256, 2>(p, a, s);
+        case 512: return launch_cap<512, 256, 1>(p, a, s);
+        default: return spinf_fail(SPINF_E_ARG, "paged_attn: head dim %d not supported (64, 128, 256, 512)", a->d);
+    }
+}

@@ -100,6 +100,28 @@ class GdnArgs(C.Structure):
     ]
 
 
+class PagedPlanArgs(C.Structure):
+    _fields_ = [
+        ("q_lens", C.c_void_p), ("kv_lens", C.c_void_p), ("reqs", C.c_int64), ("end", C.c_void_p), ("pos", C.c_void_p),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("page", C.c_int32), ("window", C.c_int32), ("variant", C.c_int32),
+    ]
+
+
+class PagedArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_tok", C.c_int64), ("q_head", C.c_int64), ("o_tok", C.c_int64), ("o_head", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("table", C.c_void_p), ("end", C.c_void_p), ("pos", C.c_void_p),
+        ("wave", C.c_void_p), ("block", C.c_void_p), ("runs", C.c_void_p), ("joins", C.c_void_p),
+        ("n_wave", C.c_int64), ("n_block", C.c_int64), ("n_joins", C.c_int64), ("part_rows", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("page", C.c_int32), ("window", C.c_int32),
+        ("scale", C.c_float), ("softcap", C.c_float),
+    ]
+
+
 def library_path() -> str:
     return os.environ.get("SPINF_TREE_LIB", os.path.join(_HERE, "libspinf_tree.so"))
 
@@ -163,13 +185,25 @@ def _bind(lib, path):
     lib.spinf_xdecode_plan_ragged.argtypes = [C.POINTER(XdecArgs), C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]
     lib.spinf_xdecode_put.argtypes = ([C.c_void_p] + [C.c_int64] * 3) * 2 + [C.c_void_p] * 3 + [C.c_int32] * 5 + [C.c_void_p]
     lib.spinf_xdecode_tiles.argtypes = [C.POINTER(XdecArgs), C.POINTER(C.c_int32)]
-    for name in ("spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
+    lib.spinf_paged_plan_build.argtypes = [C.POINTER(PagedPlanArgs), C.POINTER(C.c_void_p)]
+    lib.spinf_paged_plan_counts.argtypes = [C.c_void_p, C.POINTER(C.c_int64)]
+    lib.spinf_paged_plan_export.argtypes = [C.c_void_p] * 5
+    lib.spinf_paged_plan_free.argtypes = [C.c_void_p]
+    lib.spinf_paged_plan_free.restype = None
+    lib.spinf_paged_attn_fwd.argtypes = [C.POINTER(PagedArgs), C.c_void_p]
+    lib.spinf_paged_struct_sizes.argtypes = [C.POINTER(C.c_int64), C.c_int32]
+    for name in ("spinf_paged_plan_build", "spinf_paged_plan_counts", "spinf_paged_plan_export", "spinf_paged_attn_fwd", "spinf_paged_struct_sizes", "spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
         getattr(lib, name).restype = C.c_int
     # the argument blocks above mirror include/spinf_tree.h: a library built from another version of the header would read them wrongly
     mirrors = (AttnArgs, GdnArgs, GdnPreArgs, GdnGateArgs, LmArgs, LmHeadArgs, XdecArgs)
     sizes = (C.c_int64 * len(mirrors))()
     if lib.spinf_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
         raise RuntimeError(f"{path}: argument blocks of {list(sizes)} bytes, this package's are {[C.sizeof(m) for m in mirrors]}: "
+                           "the library and the package are of different versions (rebuild: python __graft_entry__.py); no fallback")
+    mirrors = (PagedPlanArgs, PagedArgs)
+    sizes = (C.c_int64 * len(mirrors))()
+    if lib.spinf_paged_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
+        raise RuntimeError(f"{path}: the paged cache's argument blocks have {list(sizes)} bytes, this package's {[C.sizeof(m) for m in mirrors]}: "
                            "the library and the package are of different versions (rebuild: python __graft_entry__.py); no fallback")
     _LIB = lib
     return lib

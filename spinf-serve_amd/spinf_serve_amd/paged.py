@@ -1,0 +1,306 @@
+"""A paged cache of keys and values: contents that stay after their pass, and the attention of new tokens over them.
+
+  PagedCache     the pages of one layer's keys and values
+  PagedBatch     one call's requests: lengths, page tables, trees of new tokens; the work lists, compiled once per head geometry
+  paged_attn     attention of the new tokens (single tokens, chunks, trees of questions) over what is stored
+  paged_weights  the attention weight that every stored key received, added to what it had
+  cache_evict    the stored keys with the least weight dropped, the others moved together into other pages
+
+The reference keeps no such cache: its contents are read anew with every request, and its decoder copies a pass's keys and values
+(spinf_serve/decode.py:129-171).  All device work goes through libspinf_tree.so; there is no CPU or PyTorch path.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import os
+import threading
+from dataclasses import dataclass
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import _lib
+from .masks import _Shared, _staging
+
+# which kernel the work lists are made for (spinf_paged_plan_args.variant): 0 = the library's choice, 1 = the one whose waves share rows and divide the
+# keys, 2 = the one whose waves have rows of their own.  For tests and measurements: results differ in their last bits.
+VARIANT = int(os.environ.get("SPINF_PAGED_VARIANT", "0"))
+
+
+@dataclass
+class PagedCache:
+    """k, v: [pages, page, hkv, d] bf16 in any memory order whose rows of d are contiguous; page a multiple of 16.  What unused entries hold does not
+    matter."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+
+    def __post_init__(self):
+        for name, t in (("k", self.k), ("v", self.v)):
+            if t.dim() != 4 or t.dtype != torch.bfloat16 or t.stride(3) != 1:
+                raise ValueError(f"{name} must be bf16 [pages, page, key / value heads, head dim] with contiguous head dims")
+            if any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned with strides that are multiples of 8 elements")
+        if self.k.shape != self.v.shape or self.k.device != self.v.device:
+            raise ValueError(f"k {tuple(self.k.shape)} on {self.k.device} and v {tuple(self.v.shape)} on {self.v.device} differ")
+        if self.page < 16 or self.page % 16:
+            raise ValueError(f"pages of {self.page} keys: a multiple of 16 is needed")
+        if self.k.shape[3] not in (64, 128, 256, 512):
+            raise ValueError(f"head dim {self.k.shape[3]} not supported (64, 128, 256, 512)")
+
+    @property
+    def page(self) -> int:
+        return self.k.shape[1]
+
+    @classmethod
+    def empty(cls, pages: int, page: int, hkv: int, d: int, device="cuda") -> "PagedCache":
+        """unwritten pages, each head's rows of a page next to each other in memory"""
+        k, v = (torch.empty((pages, hkv, page, d), dtype=torch.bfloat16, device=device).transpose(1, 2) for _ in range(2))
+        return cls(k, v)
+
+
+def _lengths(x, what):
+    a = np.ascontiguousarray(x, np.int64).reshape(-1)
+    if len(a) and (a.min() < 0 or a.max() > 1 << 30):
+        raise ValueError(f"{what} must lie in 0 .. 2^30")
+    return a.astype(np.int32)
+
+
+class PagedBatch:
+    """The requests of a call, shared by its layers.  Request r has kv_lens[r] stored keys, the last q_lens[r] of them its new tokens; stored key s lies
+    in entry s % page of page tables[r][s // page].  The rows of a call's tensors are the requests' new tokens back to back.
+
+    The new tokens of a request follow each other, or (end, pos given) are trees: the branches in pre-order, end[t] = the exclusive end of row t's
+    subtree in rows of the call, pos[t] = its position (at most its place among the stored keys).  A row sees all keys stored before the new tokens, and
+    of these the ones whose subtree it lies in.
+
+    Host threads and streams may share a batch: what a first call makes is made once, and a call on another stream waits for the copies."""
+
+    def __init__(self, q_lens, kv_lens, table, need, page, device, end, pos):
+        self._lock = threading.RLock()
+        self.q_lens, self.kv_lens, self.page, self.device = q_lens, kv_lens, page, device
+        self._table, self._need = table, need       # the pages back to back, and how many each request has
+        self._end, self._pos = end, pos
+        self.tokens = int(q_lens.sum(dtype=np.int64))
+        self.max_page = int(table.max()) if len(table) else -1
+        self._plans, self._dev, self._rows = {}, None, None
+
+    @classmethod
+    def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None) -> "PagedBatch":
+        """tables: per request its pages (a list or a row of an integer array; entries behind the stored keys are ignored).  Host data only."""
+        q_lens, kv_lens = _lengths(q_lens, "q_lens"), _lengths(kv_lens, "kv_lens")
+        page = int(page)
+        if page < 16 or page % 16:
+            raise ValueError(f"pages of {page} keys: a multiple of 16 is needed")
+        if len(q_lens) != len(kv_lens) or len(tables) != len(kv_lens):
+            raise ValueError(f"{len(q_lens)} q_lens, {len(kv_lens)} kv_lens and {len(tables)} tables")
+        need = -(-kv_lens.astype(np.int64) // page)
+        parts = []
+        for r, n in enumerate(need):
+            t = np.asarray(tables[r])
+            if t.ndim != 1 or len(t) < n or (n and t.dtype.kind not in "iu"):
+                raise ValueError(f"request {r}: {kv_lens[r]} stored keys need {n} pages of {page}, its table has {t.shape}")
+            parts.append(t[:n])
+        table = np.concatenate(parts).astype(np.int64) if parts else np.zeros(0, np.int64)
+        if len(table) and (table.min() < 0 or table.max() >= 1 << 31):
+            raise ValueError("page numbers must lie in 0 .. 2^31 - 1")
+        if (end is None) != (pos is None):
+            raise ValueError("a tree needs both end and pos")
+        if end is not None:
+            end, pos = (np.ascontiguousarray(x, np.int64).reshape(-1) for x in (end, pos))
+            tokens = int(q_lens.sum(dtype=np.int64))
+            if len(end) != tokens or len(pos) != tokens:
+                raise ValueError(f"end and pos hold {len(end)} and {len(pos)} values for {tokens} new tokens")
+            if (q_lens > kv_lens).any():
+                raise ValueError("a tree's new tokens are among the stored keys: q_lens must not exceed kv_lens")
+            if tokens:
+                at = np.arange(tokens) - np.repeat(np.cumsum(q_lens, dtype=np.int64) - kv_lens, q_lens)
+                if end.min() < 0 or end.max() > tokens or pos.min() < 0 or (pos > at).any():
+                    raise ValueError("end must lie in 0 .. tokens, pos in 0 .. the token's place among the stored keys")
+            end, pos = end.astype(np.int32), pos.astype(np.int32)
+        return cls(q_lens, kv_lens, table.astype(np.int32), need, page, torch.device(device), end, pos)
+
+    def __reduce__(self):
+        """copied and saved as what it is built from"""
+        tables = np.split(self._table, np.cumsum(self._need)[:-1]) if len(self._need) else []
+        return PagedBatch.build, (self.q_lens, self.kv_lens, tables, self.page, str(self.device), self._end, self._pos)
+
+    def _reach(self, shared):
+        if shared.device.type == "cuda":
+            shared.reach(_lib.raw_stream(shared.device.index))
+
+    def _upload(self, *arrays):
+        """int32 arrays back to back, each 16-byte aligned, in one copy -> device tensor, where each begins"""
+        at, n = [], 0
+        for a in arrays:
+            at.append(n)
+            n += -(-len(a) // 4) * 4
+        buf = _staging(max(n, 4), self.device)
+        host = buf.numpy()
+        for a, i in zip(arrays, at):
+            host[i : i + len(a)] = a
+        dev = buf.to(self.device, non_blocking=True)
+        return dev, at, _Shared(dev) if dev.is_cuda else None
+
+    def device_data(self):
+        """-> device tensors table, end, pos (the latter None without trees)"""
+        if self._dev is None:
+            with self._lock:
+                if self._dev is None:
+                    tree = self._end is not None
+                    arrays = (self._table, self._end, self._pos) if tree else (self._table,)
+                    dev, at, shared = self._upload(*arrays)
+                    parts = [dev[i : i + len(a)] for a, i in zip(arrays, at)]
+                    self._dev = (*parts, *[None] * (3 - len(parts))), shared
+        (table, end, pos), shared = self._dev
+        if shared is not None:
+            self._reach(shared)
+        return table, end, pos
+
+    def rows(self):
+        """-> (slots, positions) of the new tokens, device tensors int64 and int32: where the rows' keys and values go in the cache (page * page size +
+        entry; -1 where a request has fewer stored keys than new tokens), and the rows' positions"""
+        if self._rows is None:
+            with self._lock:
+                if self._rows is None:
+                    base = np.cumsum(self.q_lens, dtype=np.int64) - self.kv_lens      # row - stored place, by request
+                    at = np.arange(self.tokens) - np.repeat(base, self.q_lens)
+                    page = np.repeat(np.cumsum(self._need) - self._need, self.q_lens) + np.maximum(at, 0) // self.page
+                    inside = at >= 0
+                    slots = np.full(self.tokens, -1, np.int64)
+                    slots[inside] = self._table[page[inside]].astype(np.int64) * self.page + at[inside] % self.page
+                    pos = np.maximum(at, 0).astype(np.int32) if self._pos is None else self._pos
+                    dev, i, shared = self._upload(slots.view(np.int32), pos)
+                    self._rows = dev[: 2 * self.tokens].view(torch.int64), dev[i[1] : i[1] + self.tokens], shared
+        slots, pos, shared = self._rows
+        if shared is not None:
+            self._reach(shared)
+        return slots, pos
+
+    def plan(self, hq: int, hkv: int, d: int, window: int):
+        """the work lists for a head geometry and a window (0: none) -> (lists on the device, counts, where wave, block, runs, joins begin)"""
+        key = (hq, hkv, d, window, VARIANT)
+        got = self._plans.get(key)
+        if got is None:
+            with self._lock:
+                got = self._plans.get(key)
+                if got is None:
+                    got = self._plans[key] = self._compile(*key)
+        if got[3] is not None:
+            self._reach(got[3])
+        return got[:3]
+
+    def _compile(self, hq, hkv, d, window, variant):
+        lib = _lib.load_library()
+        a = _lib.PagedPlanArgs()
+        a.q_lens, a.kv_lens, a.reqs = self.q_lens.ctypes.data, self.kv_lens.ctypes.data, len(self.kv_lens)
+        if self._end is not None:
+            a.end, a.pos = self._end.ctypes.data, self._pos.ctypes.data
+        a.hq, a.hkv, a.d, a.page, a.window, a.variant = hq, hkv, d, self.page, window, variant
+        h = C.c_void_p()
+        _lib.check(lib.spinf_paged_plan_build(C.byref(a), C.byref(h)), "paged_plan")
+        try:
+            counts = (C.c_int64 * 5)()
+            _lib.check(lib.spinf_paged_plan_counts(h, counts), "paged_plan_counts")
+            sizes = [12 * counts[0], 12 * counts[1], 4 * counts[2], 8 * counts[3]]
+            at = [0, sizes[0], sizes[0] + sizes[1], sum(sizes[:3])]
+            buf = _staging(max(sum(sizes), 4), self.device)
+            p = buf.data_ptr()
+            _lib.check(lib.spinf_paged_plan_export(h, *(p + 4 * i for i in at)), "paged_plan_export")
+        finally:
+            lib.spinf_paged_plan_free(h)
+        dev = buf.to(self.device, non_blocking=True)
+        return dev, list(counts), at, _Shared(dev) if dev.is_cuda else None
+
+
+def _check_call(q, k, v, tokens, page, max_page, what):
+    """raises on tensors the kernels do not take"""
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError(f"{what}: q must be bf16 [new tokens, query heads, head dim] with contiguous head dims")
+    if q.shape[0] != tokens:
+        raise ValueError(f"{what}: the batch has {tokens} new tokens, q {q.shape[0]} rows")
+    if q.shape[2] != k.shape[3]:
+        raise ValueError(f"{what}: head dim {q.shape[2]} of q, {k.shape[3]} of the cache")
+    if k.shape[2] <= 0 or q.shape[1] <= 0 or q.shape[1] % k.shape[2]:
+        raise ValueError(f"{what}: {q.shape[1]} query heads do not group over {k.shape[2]} key / value heads")
+    if k.shape[1] != page:
+        raise ValueError(f"{what}: the batch counts pages of {page} keys, the cache has {k.shape[1]}")
+    if max_page >= k.shape[0]:
+        raise ValueError(f"{what}: page {max_page} in a table, the cache has {k.shape[0]}")
+    if not q.is_cuda:
+        raise RuntimeError(f"{what} runs on ROCm device tensors only (no CPU path)")
+    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        raise ValueError(f"{what}: q must be 16-byte aligned with strides that are multiples of 8 elements")
+
+
+def _window(window) -> int:
+    w = int(window) if window is not None else 0
+    if w < 0:
+        raise ValueError(f"window {w}")
+    return w
+
+
+def _fill(a, q, k, v, page, window, scale, softcap):
+    a.q, a.q_tok, a.q_head = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    a.k_page, a.k_row, a.k_head = k.stride()[:3]
+    a.v_page, a.v_row, a.v_head = v.stride()[:3]
+    a.hq, a.hkv, a.d, a.page, a.window = q.shape[1], k.shape[2], q.shape[2], page, window
+    a.scale, a.softcap = scale, softcap
+
+
+def _paged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, end: Optional[torch.Tensor], pos: Optional[torch.Tensor],
+                lists: torch.Tensor, counts: list[int], at: list[int], page: int, max_page: int, tokens: int, scale: float, window: int, softcap: float,
+                want_lse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _check_call(q, k, v, tokens, page, max_page, "paged_attn")
+    _lib.same_device(q.device, k, v, table, end, pos, lists)
+    T, hq, d = q.shape
+    out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((T, hq) if want_lse else (0,), dtype=torch.float32, device=q.device)
+    if T == 0:
+        return out, lse
+    a = _lib.PagedArgs()
+    _fill(a, q, k, v, page, window, scale, softcap)
+    a.out, a.o_tok, a.o_head = out.data_ptr(), hq * d, d
+    a.lse = lse.data_ptr() if want_lse else None
+    a.table = table.data_ptr()
+    if end is not None:
+        a.end, a.pos = end.data_ptr(), pos.data_ptr()
+    base = lists.data_ptr()
+    a.wave, a.block, a.runs, a.joins = (base + 4 * i for i in at)
+    a.n_wave, a.n_block, _, a.n_joins, a.part_rows = counts
+    if a.part_rows:
+        work = torch.empty(a.part_rows * (d + 2), dtype=torch.float32, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel() * 4
+    _lib.launch(_lib.load_library().spinf_paged_attn_fwd, a, q.device, "paged_attn")
+    return out, lse
+
+
+_paged_op = torch.library.custom_op("spinf::paged_attn", _paged_attn, mutates_args=())
+
+
+@_paged_op.register_fake
+def _(q, k, v, table, end, pos, lists, counts, at, page, max_page, tokens, scale, window, softcap, want_lse):
+    return (torch.empty(q.shape, dtype=torch.bfloat16, device=q.device),
+            torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device))
+
+
+def paged_attn(q, cache: PagedCache, batch: PagedBatch, scale=None, window=None, softcap=None, return_lse=False):
+    """q [new tokens, hq, d] bf16 -> [new tokens, hq, d] bf16: softmax over the stored keys that each row sees of scale q.k (with ``softcap``: of softcap
+    tanh(scale q.k / softcap)), times the values.  Row i of a request, stored at place c + i, sees the keys up to its own place (of a tree's new tokens
+    those whose subtree it lies in), with ``window`` those less than ``window`` positions behind it.  A row that sees nothing is zeros.
+    return_lse: also the natural log of each row's sum of exponentials, [new tokens, hq] fp32 (-inf where a row sees nothing).
+    The new tokens' own keys and values have to be in the cache (qk_norm_rope_put).  A request's rows are the same bits whatever else is in the batch."""
+    window = _window(window)
+    k, v = cache.k, cache.v
+    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    softcap = float(softcap) if softcap else 0.0
+    _check_call(q, k, v, batch.tokens, batch.page, batch.max_page, "paged_attn")
+    _lib.same_device(q.device, k, v)
+    table, end, pos = batch.device_data()
+    lists, counts, at = batch.plan(q.shape[1], k.shape[2], q.shape[2], window)
+    run = _paged_attn if _lib.eager(q, k, v) else _paged_op
+    out, lse = run(q, k, v, table, end, pos, lists, counts, at, batch.page, batch.max_page, batch.tokens, scale, window, softcap, bool(return_lse))
+    return (out, lse) if return_lse else out
