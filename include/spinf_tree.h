@@ -381,6 +381,61 @@ typedef struct spinf_paged_args {
 } spinf_paged_args;
 int spinf_paged_attn_fwd(const spinf_paged_args* args, void* stream);
 
+/* The attention weight that every stored key received, added to what it had: out[r, h, s] = acc[r, h, s] + sum over the new tokens that see key s and the
+ * query heads of key / value head h of exp(cap(scale q.k) - lse); s behind the stored keys: acc.  Visibility, q, k, table, end, pos as above;
+ *   lse [tokens, hq] fp32 as spinf_paged_attn_fwd leaves it; reqs [n_reqs, 4] int32 device: {first row, new tokens, stored keys, first page in table} of each
+ *   request; acc (NULL: zeros) and out [n_reqs, hkv, keys] fp32 dense, out may be acc.  keys >= the most stored keys of a request (the caller checks). */
+typedef struct spinf_paged_weights_args {
+    const void* q; const float* lse; const float* acc; float* out;
+    int64_t q_tok, q_head;
+    const void* k; int64_t k_page, k_row, k_head;
+    const int32_t* table; const int32_t* reqs; const int32_t* end; const int32_t* pos;
+    int64_t n_reqs, tokens, keys;
+    int32_t hq, hkv, d, page, window;
+    float scale, softcap;
+} spinf_paged_weights_args;
+int spinf_paged_weights(const spinf_paged_weights_args* args, void* stream);
+
+/* Eviction: of each request's n stored keys and for every key / value head min(n, keep) stay: all where n <= keep, else the first `sink`, the last `recent`, and
+ * of the others those with the largest acc (ties to the lowest index, NaN above everything).  Their keys and values are copied, in order, into the pages that
+ * new_table names for the request (entries 0 .. min(n, keep) - 1); kept [n_reqs, hkv, keep] int32 gets their places (-1 behind), new_acc their acc (0 behind).
+ *   acc [n_reqs, hkv, keys] fp32; reqs, new_reqs as above (of new_reqs the first page is read).  The pages written must be no pages read (the caller checks).
+ *   sink + recent <= keep. */
+typedef struct spinf_evict_args {
+    const float* acc; int64_t keys;
+    const int32_t* reqs; const int32_t* new_reqs; const int32_t* table; const int32_t* new_table;
+    int32_t* kept; float* new_acc;
+    void* k; void* v;
+    int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    int64_t n_reqs;
+    int32_t hkv, d, page, keep, sink, recent;
+} spinf_evict_args;
+int spinf_cache_evict(const spinf_evict_args* args, void* stream);
+
+/* Norms of queries and keys per head and their rotation by position in one pass, before the attention; with `slots` the keys and the values go into
+ * a paged cache.  y = x / sqrt(mean x^2 + eps) * w, then the first `rot` dims rotated in pairs (i, i + rot / 2), or (2 i, 2 i + 1) with `neighbours`:
+ * (a, b) -> (a cos - b sin, b cos + a sin).  fp32 arithmetic, one rounding to bf16.
+ *   q [T, hq, d], k, v [T, hkv, d] bf16 (token and head strides in elements, multiples of 8); wq, wk [d] or NULL (no weight), fp32 (w_f32) or bf16;
+ *   plus_one: the weight is 1 + w; cos, sin [n_pos, >= rot / 2] fp32 (cs_f32) or bf16, rows cos_ld, sin_ld elements apart, 16-byte aligned; pos [T] int64
+ *   (pos_i64) or int32 device: the tables' row of each token, NULL: row t.  A position outside the tables gives a query and a key of NaN.
+ *   slots NULL: q_out [T, hq, d], k_out [T, hkv, d] dense, v is not touched.
+ *   slots [T] int64 device: token t's key and value become entry slots[t] % page of page slots[t] / page of the cache (k_out, v_out with their
+ *   strides, `pages` pages); v_norm: the value is normed too, without weight.  A negative slot stores nothing (a pad); one behind the cache stores nothing
+ *   and makes the token's query NaN.  Two tokens with one slot: either's rows.  d in {64, 128, 256, 512}, rot a multiple of 16. */
+typedef struct spinf_rope_args {
+    const void* q; const void* k; const void* v;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    const void* wq; const void* wk; const void* cos; const void* sin;
+    int64_t cos_ld, sin_ld, n_pos;
+    const void* pos; const int64_t* slots;
+    void* q_out; void* k_out; void* v_out;
+    int64_t k_page, k_row, kh_out, v_page, v_row, vh_out, pages;
+    int64_t T; int32_t hq, hkv, d, rot, page;
+    int32_t neighbours, plus_one, v_norm, w_f32, cs_f32, pos_i64;
+    float eps;
+} spinf_rope_args;
+int spinf_qk_norm_rope(const spinf_rope_args* args, void* stream);
+
 /* ------------------------------------------------------------------------------------------------ yardstick
  * No counterpart in the reference: one launch of a pure v_mfma_f32_32x32x16_bf16 loop on every compute unit (one workgroup of eight
  * waves per CU, iters x 8 MFMAs per wave, operands in registers), for the benchmark's "what do the matrix cores sustain on this
@@ -429,7 +484,8 @@ int spinf_diag_attn_stream(const spinf_attn_args* args, int32_t parts, int32_t n
  * spinf_gdn_pre_args, spinf_gdn_gate_args, spinf_lm_args, spinf_lm_head_args, spinf_xdec_args as this library was built (n must be
  * 7): a binding compares them with its own mirrors of the structures before its first call. */
 int spinf_struct_sizes(int64_t* sizes, int32_t n);
-/* The same for the paged cache: spinf_paged_plan_args, spinf_paged_args (n must be 2). */
+/* The same for the paged cache: spinf_paged_plan_args, spinf_paged_args, spinf_rope_args, spinf_paged_weights_args and
+ * spinf_evict_args, in this order; n must be 5. */
 int spinf_paged_struct_sizes(int64_t* sizes, int32_t n);
 
 #ifdef __cplusplus

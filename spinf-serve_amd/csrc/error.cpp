@@ -27,8 +27,9 @@ extern "C" int spinf_struct_sizes(int64_t* sizes, int32_t n) {
 
 // the same for the blocks of the paged cache
 extern "C" int spinf_paged_struct_sizes(int64_t* sizes, int32_t n) {
-    const int64_t all[2] = {(int64_t)sizeof(spinf_paged_plan_args), (int64_t)sizeof(spinf_paged_args)};
-    if (!sizes || n != 2) return spinf_fail(SPINF_E_ARG, "paged_struct_sizes: 2 sizes (plan, attn)");
+    const int64_t all[5] = {(int64_t)sizeof(spinf_paged_plan_args), (int64_t)sizeof(spinf_paged_args), (int64_t)sizeof(spinf_rope_args),
+                            (int64_t)sizeof(spinf_paged_weights_args), (int64_t)sizeof(spinf_evict_args)};
+    if (!sizes || n != 5) return spinf_fail(SPINF_E_ARG, "paged_struct_sizes: 5 sizes (plan, attn, rope, weights, evict)");
     for (int i = 0; i < n; i++) sizes[i] = all[i];
     return SPINF_OK;
 }

@@ -26,12 +26,12 @@
 #include "common.h"
 #include "paged.h"
 #include "attn_tiles.h"
+#include "paged_dev.h"
 
 namespace {
 
-constexpr int TK = PAGED_TILE;
 constexpr float TAU = 8.f;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LN2 = 0.6931471805599453f;
 
 struct Params {
     const __bf16* q; __bf16* out; float* lse;
@@ -42,13 +42,9 @@ struct Params {
     const PagedItem* items; const PagedRun* runs; const PagedJoin* joins;
     float* part_o; float2* part_ml;
     int n_items, hq, group, window;
-    int page16; unsigned page_mul; int page_shift;   // 16-key pieces of a page, and the multiplier and shift that divide by it (0: divide by 1)
+    PageDiv page;
     float c, cap_in, cap_out;                        // scale log2 e; with a cap: 2 scale log2 e / cap and cap log2 e
 };
-
-typedef const __attribute__((address_space(4))) int* scalar_ints;
-// a value at a wave-uniform address, through the scalar cache
-__device__ __forceinline__ int sload(const int* p, int i) { return ((scalar_ints)(size_t)p)[__builtin_amdgcn_readfirstlane(i)]; }
 
 __device__ __forceinline__ PagedItem load_item(const PagedItem* items, int i) {
     PagedItem it;
@@ -94,36 +90,15 @@ struct Place {
         const int n = 2 * kt, end = (it.L - 1) >> 4;
         last = it.L - 1 - kt * TK < TK - 1 ? it.L - 1 - kt * TK : TK - 1;
         const int n1 = n + 1 < end ? n + 1 : end;
-        const int a = p.page_mul ? (int)(__umulhi((unsigned)n, p.page_mul) >> p.page_shift) : n;
-        const int b = p.page_mul ? (int)(__umulhi((unsigned)n1, p.page_mul) >> p.page_shift) : n1;
+        const int a = p.page.of(n), b = p.page.of(n1);
         const long ia = sload(p.table, it.tab + a), ib = sload(p.table, it.tab + b);
-        const long ra = (long)(n - a * p.page16) * 16, rb = (long)(n1 - b * p.page16) * 16;
+        const long ra = (long)(n - a * p.page.pieces) * 16, rb = (long)(n1 - b * p.page.pieces) * 16;
         k0 = p.k + ia * p.k_page + ra * p.k_row + it.kvh * p.k_head;
         v0 = p.v + ia * p.v_page + ra * p.v_row + it.kvh * p.v_head;
         k1 = p.k + ib * p.k_page + rb * p.k_row + it.kvh * p.k_head;
         v1 = p.v + ib * p.v_page + rb * p.v_row + it.kvh * p.v_head;
     }
 };
-
-// DMA of regions reg0 .. reg0 + N - 1 of a tile (32 rows of W dims) into the LDS tile at `lds`; RS: distance of its regions
-template <int W, int N, int RS>
-__device__ __forceinline__ void fetch(const char* b0, const char* b1, long row, int last, int reg0, unsigned lds, int lane) {
-    using G = Geo<W, TK>;
-    const int slot = lane / G::CPR, chunk = lane % G::CPR;
-    if (last == TK - 1 && b1 == b0 + 16 * row) {   // 32 rows, one after the other: a uniform base and a constant per lane
-        const unsigned off = (unsigned)(slot * G::NREG * (int)row + chunk * 16);
-#pragma unroll
-        for (int i = 0; i < N; i++) dma16_uniform(b0 + (reg0 + i) * row, off, lds + (reg0 + i) * RS);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            int r = reg0 + i + G::NREG * slot;
-            r = r < last ? r : last;
-            const char* b = r >= 16 ? b1 : b0;
-            dma16_lane(b + (r & 15) * row + chunk * 16, lds + (reg0 + i) * RS);
-        }
-    }
-}
 
 // subtree ends and positions of a tile's new tokens into 2 x 256 bytes of LDS (the 32 keys twice)
 __device__ __forceinline__ void fetch_meta(const Params& p, const PagedItem& it, int kt, unsigned lds, int lane) {
@@ -133,7 +108,6 @@ __device__ __forceinline__ void fetch_meta(const Params& p, const PagedItem& it,
     dma4_lane(p.pos + it.cu + u, lds + 256);
 }
 
-constexpr int vmcnt_imm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }   // waits for all but the n youngest vector memory operations
 constexpr int LGKM0 = 0xc07f;                                                     // waits for every LDS operation
 
 // A wave's 32 rows: queries, output accumulators, softmax state
@@ -688,14 +662,7 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     p.part_o = (float*)a->workspace;
     p.part_ml = (float2*)(p.part_o + a->part_rows * a->d);
     p.hq = a->hq; p.group = a->hq / a->hkv; p.window = a->window;
-    // n / page16 for n < 2^27 as the high word of a product: multiplier ceil(2^(31 + b) / page16), b = ceil(log2 page16), shift b - 1
-    p.page16 = a->page / 16;
-    if (p.page16 > 1) {
-        int b = 0;
-        while ((1 << b) < p.page16) b++;
-        p.page_mul = (unsigned)(((1ull << (31 + b)) + p.page16 - 1) / p.page16);
-        p.page_shift = b - 1;
-    }
+    p.page = PageDiv::of_page(a->page);
     p.c = a->scale * LOG2E;
     p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
     p.cap_out = a->softcap * LOG2E;

@@ -1,0 +1,177 @@
+// The attention weight that every stored key of a paged cache received, for gfx950 (MI355X): what cache_evict (paged_evict.hip) decides by.  No
+// counterpart in the reference.
+//
+// Mathematics: W[r, h, s] = acc[r, h, s] + sum over the request's new tokens that see key s and the query heads of key / value head h of
+// exp(cap(scale q.k) - lse), with the log-sums lse that the attention left: the probabilities once more, without their softmax.
+//
+// S = Q K^T the other way round than in the attention: a lane of v_mfma_f32_32x32x16_bf16's result owns one KEY and 16 of the 32 rows, so a key's
+// sum stays in its lane over all rows: no atomics, one order, one lane exchange at the end.  A workgroup's waves take 32 keys each: the keys come once, by
+// DMA through LDS, and stay in registers; the rows come from memory block by block.
+//
+// Bound by HBM where rows are few (a decoding step: the keys' bytes), by the loads of the rows where they are many.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+
+#include "spinf_tree.h"
+#include "common.h"
+#include "paged_dev.h"
+
+namespace {
+
+struct Params {
+    const __bf16* q; const float* lse; const float* acc; float* out;
+    long q_tok, q_head;
+    const char* k;
+    long k_page, k_row, k_head;   // bytes
+    const int* table; const int* reqs; const int* end; const int* pos;
+    long keys;                    // of a row of acc and out
+    int blocks, hq, hkv, group, window;
+    PageDiv page;
+    float c, cap_in, cap_out;
+};
+
+template <int D, int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) {
+    using GK = Geo<D, TK>;
+    constexpr int NS = D / 16;
+    __shared__ __attribute__((aligned(16))) char lds[NW * GK::KTILEB];
+    __shared__ __attribute__((aligned(16))) float row_lse[NW][32];
+    __shared__ __attribute__((aligned(16))) int row_tok[NW][32], row_pos[NW][32];
+    const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rh = blockIdx.x / p.blocks, r = rh / p.hkv, kvh = rh - r * p.hkv;
+    const int kt = (int)(blockIdx.x - (unsigned)rh * p.blocks) * NW + w;
+    const int cu = sload(p.reqs, 4 * r), T = sload(p.reqs, 4 * r + 1), L = sload(p.reqs, 4 * r + 2), tab = sload(p.reqs, 4 * r + 3);
+    const int key = kt * TK + m;
+    float sum = 0.f;
+    if (kt * TK < L && T > 0) {   // (no barrier below: each wave has its own buffers)
+        const int c = L - T, N = T * p.group;
+        char* const kb = lds + w * GK::KTILEB;
+        {
+            const int n = 2 * kt, last16 = (L - 1) >> 4, n1 = n + 1 < last16 ? n + 1 : last16;
+            const int last = L - 1 - kt * TK < TK - 1 ? L - 1 - kt * TK : TK - 1;
+            const int a = p.page.of(n), b = p.page.of(n1);
+            const long ia = sload(p.table, tab + a), ib = sload(p.table, tab + b);
+            const char* k0 = p.k + ia * p.k_page + (long)(n - a * p.page.pieces) * 16 * p.k_row + kvh * p.k_head;
+            const char* k1 = p.k + ib * p.k_page + (long)(n1 - b * p.page.pieces) * 16 * p.k_row + kvh * p.k_head;
+            fetch<D, GK::NREG, GK::KRS>(k0, k1, p.k_row, last, 0, lds_addr(kb), lane);
+        }
+        const int u = key - c;   // this lane's key as a new token of the request (below 0: stored before)
+        const bool fresh = p.end && u >= 0;
+        const int uc = u < T ? u : T - 1;
+        const int end_k = fresh ? p.end[cu + uc] : INT_MAX;
+        const int pos_k = fresh && p.pos ? p.pos[cu + uc] : key;
+        const int u_lo = kt * TK - c, u_hi = u_lo + TK - 1;
+        // row blocks that hold a row which may see a key of the tile
+        const int rb0 = u_lo > 0 ? (int)((long)u_lo * p.group / 32) : 0;
+        long rows = N;
+        if (p.window && !p.end) {   // (without a tree a row's position is its place) tokens from u_hi + window on are too far from the tile's keys
+            const long most = ((long)u_hi + p.window) * p.group;
+            rows = most < rows ? most : rows;
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 kf[NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) kf[s] = *(const bf16x8*)(kb + GK::k_off(m) + 16 * g + 32 * s);
+        for (int row0 = rb0 * 32; row0 < rows; row0 += 32) {
+            const int row = row0 + m, rc = row < N ? row : N - 1;
+            const int tok = rc / p.group, head = kvh * p.group + (rc - tok * p.group);
+            const __bf16* qp = p.q + (long)(cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
+            bf16x8 qf[NS];
+#pragma unroll
+            for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
+            const float lse = p.lse[(long)(cu + tok) * p.hq + head];
+            if (g == 0) {   // a row behind the last, or one that saw nothing, gives no weight
+                row_lse[w][m] = row < N && lse != -INFINITY ? lse * LOG2E : INFINITY;
+                row_tok[w][m] = tok;
+                row_pos[w][m] = p.window ? (p.end ? p.pos[cu + tok] : c + tok) : 0;
+            }
+            f32x16 s;
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+            for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[st], kf[st], s, 0, 0, 0);
+            const bool masked = u_hi > __builtin_amdgcn_readfirstlane(tok) || p.window;   // (lane 0's token is the block's first)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) {
+                const float4 l4 = *(const float4*)&row_lse[w][8 * i4 + 4 * g];
+                const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+                int tv[4] = {0, 0, 0, 0}, pv[4] = {0, 0, 0, 0};
+                if (masked || p.end) {
+                    const int4 t4 = *(const int4*)&row_tok[w][8 * i4 + 4 * g], p4 = *(const int4*)&row_pos[w][8 * i4 + 4 * g];
+                    tv[0] = t4.x; tv[1] = t4.y; tv[2] = t4.z; tv[3] = t4.w;
+                    pv[0] = p4.x; pv[1] = p4.y; pv[2] = p4.z; pv[3] = p4.w;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float t = s[4 * i4 + j];
+                    if (CAP) t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t * p.cap_in) + 1.0f));
+                    const float x = __builtin_amdgcn_exp2f(CAP ? t - lv[j] : __builtin_fmaf(t, p.c, -lv[j]));
+                    bool vis = true;
+                    if (masked || p.end) {
+                        vis = (u <= tv[j]) & (cu + tv[j] < end_k);
+                        if (p.window) vis = vis & (pv[j] - pos_k < p.window);
+                    }
+                    sum += vis ? x : 0.f;
+                }
+            }
+        }
+        sum = lane32_sum(sum);
+    }
+    if (g == 0 && key < p.keys) {
+        const long at = (long)rh * p.keys + key;
+        const float before = p.acc ? p.acc[at] : 0.f;
+        p.out[at] = key < L ? before + sum : before;
+    }
+}
+
+template <int D, int NW>
+int launch(Params p, int64_t reqs, bool cap, hipStream_t s) {
+    const int64_t blocks = (p.keys + 32 * NW - 1) / (32 * NW), grid = blocks * p.hkv * reqs;
+    if (grid > INT32_MAX) return spinf_fail(SPINF_E_ARG, "paged_weights: %lld requests of %ld keys are too many", (long long)reqs, p.keys);
+    p.blocks = (int)blocks;
+    if (cap) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
+    else hipLaunchKernelGGL((paged_weights_kernel<D, NW, false>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "paged_weights: launch: %s", hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" int spinf_paged_weights(const spinf_paged_weights_args* a, void* stream) {
+    if (!a) return spinf_fail(SPINF_E_ARG, "paged_weights: null args");
+    if (a->n_reqs < 0 || a->n_reqs > (1 << 24) || a->keys < 0 || a->keys > (1 << 30)) return spinf_fail(SPINF_E_ARG, "paged_weights: %lld requests, %lld keys", (long long)a->n_reqs, (long long)a->keys);
+    if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv) return spinf_fail(SPINF_E_ARG, "paged_weights: %d query heads do not group over %d key / value heads", a->hq, a->hkv);
+    if (a->d != 64 && a->d != 128 && a->d != 256 && a->d != 512) return spinf_fail(SPINF_E_ARG, "paged_weights: head dim %d not supported (64, 128, 256, 512)", a->d);
+    if (a->page < 16 || a->page % 16 || a->page > (1 << 20)) return spinf_fail(SPINF_E_ARG, "paged_weights: pages of %d keys (a multiple of 16)", a->page);
+    if (a->window < 0) return spinf_fail(SPINF_E_ARG, "paged_weights: window %d", a->window);
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY) || !(a->softcap >= 0.f) || !(a->softcap < INFINITY))
+        return spinf_fail(SPINF_E_ARG, "paged_weights: scale %g must be positive and finite, softcap %g not negative", (double)a->scale, (double)a->softcap);
+    if (a->n_reqs == 0 || a->keys == 0) return SPINF_OK;
+    if (!a->reqs || !a->out || !a->k || !a->table || (a->tokens > 0 && (!a->q || !a->lse))) return spinf_fail(SPINF_E_ARG, "paged_weights: null pointer");
+    if ((a->end == nullptr) != (a->pos == nullptr)) return spinf_fail(SPINF_E_ARG, "paged_weights: a tree needs both end and pos");
+    if ((uintptr_t)a->q % 16 || (uintptr_t)a->k % 16 || (uintptr_t)a->reqs % 16) return spinf_fail(SPINF_E_ARG, "paged_weights: tensors must be 16-byte aligned");
+    for (int64_t st : {a->q_tok, a->q_head, a->k_page, a->k_row, a->k_head})
+        if (st % 8) return spinf_fail(SPINF_E_ARG, "paged_weights: strides must be multiples of 8 elements");
+    if (a->k_row < 0 || a->k_row > (1 << 24)) return spinf_fail(SPINF_E_ARG, "paged_weights: row strides of the cache must lie in 0 .. 2^24");
+    Params p = {};
+    p.q = (const __bf16*)a->q; p.lse = a->lse; p.acc = a->acc; p.out = a->out;
+    p.q_tok = a->q_tok; p.q_head = a->q_head;
+    p.k = (const char*)a->k; p.k_page = 2 * a->k_page; p.k_row = 2 * a->k_row; p.k_head = 2 * a->k_head;
+    p.table = a->table; p.reqs = a->reqs; p.end = a->end; p.pos = a->pos;
+    p.keys = a->keys; p.hq = a->hq; p.hkv = a->hkv; p.group = a->hq / a->hkv; p.window = a->window;
+    p.page = PageDiv::of_page(a->page);
+    p.c = a->scale * LOG2E;
+    p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
+    p.cap_out = a->softcap * LOG2E;
+    hipStream_t s = (hipStream_t)stream;
+    const bool cap = a->softcap > 0.f;
+    switch (a->d) {
+        case 64: return launch<64, 4>(p, a->n_reqs, cap, s);
+        case 128: return launch<128, 4>(p, a->n_reqs, cap, s);
+        case 256: return launch<256, 4>(p, a->n_reqs, cap, s);
+        default: return launch<512, 2>(p, a->n_reqs, cap, s);
+    }
+}

@@ -6,7 +6,9 @@
   gdn         recurrent, chunked (spinf_serve/models/qwen35/gdn.py)
   qwen_plan   tree_plan, gdn_tree (spinf_serve/models/qwen35/qwen.py:158-276, 514-590)
   decode      XCaches, GroupKV, x_attention: the extraction decoder's attention step (spinf_serve/decode.py:35-104)
-  paged       PagedCache, PagedBatch, paged_attn: attention of new tokens over a paged cache of contents read before
+  paged       PagedCache, PagedBatch, paged_attn, paged_weights, cache_evict: a paged cache of contents read before, the attention of new
+              tokens over it, and what keeps it small
+  rope        qk_norm_rope, qk_norm_rope_put: norms and rotation of queries and keys, and their way into the cache
   synth       seeded synthetic workloads of the benchmark configurations
 
 All device work goes through libspinf_tree.so (HIP, gfx950); there is no CPU or PyTorch fallback: importing the
@@ -21,5 +23,6 @@ from .gdn import chunked, recurrent  # noqa: F401
 from .gdn_layer import gdn_gate, gdn_prologue  # noqa: F401
 from .lm_head import lm_head_logprobs, lm_logprobs  # noqa: F401
 from .decode import GroupKV, XCaches, x_attention, xdecode_attn  # noqa: F401
-from .paged import PagedBatch, PagedCache, paged_attn  # noqa: F401
+from .paged import PagedBatch, PagedCache, cache_evict, paged_attn, paged_weights  # noqa: F401
+from .rope import qk_norm_rope, qk_norm_rope_put  # noqa: F401
 from .qwen_plan import Call, TreePlan, gdn_tree, tree_plan  # noqa: F401

@@ -122,6 +122,44 @@ class PagedArgs(C.Structure):
     ]
 
 
+class PagedWeightsArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("lse", C.c_void_p), ("acc", C.c_void_p), ("out", C.c_void_p),
+        ("q_tok", C.c_int64), ("q_head", C.c_int64),
+        ("k", C.c_void_p), ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
+        ("table", C.c_void_p), ("reqs", C.c_void_p), ("end", C.c_void_p), ("pos", C.c_void_p),
+        ("n_reqs", C.c_int64), ("tokens", C.c_int64), ("keys", C.c_int64),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("page", C.c_int32), ("window", C.c_int32),
+        ("scale", C.c_float), ("softcap", C.c_float),
+    ]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [
+        ("acc", C.c_void_p), ("keys", C.c_int64),
+        ("reqs", C.c_void_p), ("new_reqs", C.c_void_p), ("table", C.c_void_p), ("new_table", C.c_void_p),
+        ("kept", C.c_void_p), ("new_acc", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("n_reqs", C.c_int64),
+        ("hkv", C.c_int32), ("d", C.c_int32), ("page", C.c_int32), ("keep", C.c_int32), ("sink", C.c_int32), ("recent", C.c_int32),
+    ]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_tok", C.c_int64), ("q_head", C.c_int64), ("k_tok", C.c_int64), ("k_head", C.c_int64), ("v_tok", C.c_int64), ("v_head", C.c_int64),
+        ("wq", C.c_void_p), ("wk", C.c_void_p), ("cos", C.c_void_p), ("sin", C.c_void_p),
+        ("cos_ld", C.c_int64), ("sin_ld", C.c_int64), ("n_pos", C.c_int64),
+        ("pos", C.c_void_p), ("slots", C.c_void_p),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("k_page", C.c_int64), ("k_row", C.c_int64), ("kh_out", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64), ("vh_out", C.c_int64), ("pages", C.c_int64),
+        ("T", C.c_int64), ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("rot", C.c_int32), ("page", C.c_int32),
+        ("neighbours", C.c_int32), ("plus_one", C.c_int32), ("v_norm", C.c_int32), ("w_f32", C.c_int32), ("cs_f32", C.c_int32), ("pos_i64", C.c_int32),
+        ("eps", C.c_float),
+    ]
+
+
 def library_path() -> str:
     return os.environ.get("SPINF_TREE_LIB", os.path.join(_HERE, "libspinf_tree.so"))
 
@@ -191,8 +229,11 @@ def _bind(lib, path):
     lib.spinf_paged_plan_free.argtypes = [C.c_void_p]
     lib.spinf_paged_plan_free.restype = None
     lib.spinf_paged_attn_fwd.argtypes = [C.POINTER(PagedArgs), C.c_void_p]
+    lib.spinf_paged_weights.argtypes = [C.POINTER(PagedWeightsArgs), C.c_void_p]
+    lib.spinf_cache_evict.argtypes = [C.POINTER(EvictArgs), C.c_void_p]
+    lib.spinf_qk_norm_rope.argtypes = [C.POINTER(RopeArgs), C.c_void_p]
     lib.spinf_paged_struct_sizes.argtypes = [C.POINTER(C.c_int64), C.c_int32]
-    for name in ("spinf_paged_plan_build", "spinf_paged_plan_counts", "spinf_paged_plan_export", "spinf_paged_attn_fwd", "spinf_paged_struct_sizes", "spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
+    for name in ("spinf_paged_plan_build", "spinf_paged_plan_counts", "spinf_paged_plan_export", "spinf_paged_attn_fwd", "spinf_paged_weights", "spinf_cache_evict", "spinf_qk_norm_rope", "spinf_paged_struct_sizes", "spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
         getattr(lib, name).restype = C.c_int
     # the argument blocks above mirror include/spinf_tree.h: a library built from another version of the header would read them wrongly
     mirrors = (AttnArgs, GdnArgs, GdnPreArgs, GdnGateArgs, LmArgs, LmHeadArgs, XdecArgs)
@@ -200,7 +241,7 @@ def _bind(lib, path):
     if lib.spinf_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
         raise RuntimeError(f"{path}: argument blocks of {list(sizes)} bytes, this package's are {[C.sizeof(m) for m in mirrors]}: "
                            "the library and the package are of different versions (rebuild: python __graft_entry__.py); no fallback")
-    mirrors = (PagedPlanArgs, PagedArgs)
+    mirrors = (PagedPlanArgs, PagedArgs, RopeArgs, PagedWeightsArgs, EvictArgs)
     sizes = (C.c_int64 * len(mirrors))()
     if lib.spinf_paged_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
         raise RuntimeError(f"{path}: the paged cache's argument blocks have {list(sizes)} bytes, this package's {[C.sizeof(m) for m in mirrors]}: "

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import threading
+import weakref
 from dataclasses import dataclass
 from typing import Optional
 
@@ -85,7 +86,7 @@ class PagedBatch:
         self._end, self._pos = end, pos
         self.tokens = int(q_lens.sum(dtype=np.int64))
         self.max_page = int(table.max()) if len(table) else -1
-        self._plans, self._dev, self._rows = {}, None, None
+        self._plans, self._moves, self._dev, self._rows = {}, {}, None, None
 
     @classmethod
     def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None) -> "PagedBatch":
@@ -136,7 +137,7 @@ class PagedBatch:
         at, n = [], 0
         for a in arrays:
             at.append(n)
-            n += -(-len(a) // 4) * 4
+            n += -(-max(len(a), 1) // 4) * 4   # (an empty one has a place of its own too: no entry of it is read, but its address is passed)
         buf = _staging(max(n, 4), self.device)
         host = buf.numpy()
         for a, i in zip(arrays, at):
@@ -144,20 +145,46 @@ class PagedBatch:
         dev = buf.to(self.device, non_blocking=True)
         return dev, at, _Shared(dev) if dev.is_cuda else None
 
-    def device_data(self):
-        """-> device tensors table, end, pos (the latter None without trees)"""
+    def _device(self):
         if self._dev is None:
             with self._lock:
                 if self._dev is None:
                     tree = self._end is not None
-                    arrays = (self._table, self._end, self._pos) if tree else (self._table,)
+                    cu, tab = (np.cumsum(x, dtype=np.int64) - x for x in (self.q_lens, self._need))
+                    reqs = np.stack([cu, self.q_lens, self.kv_lens, tab], 1).astype(np.int32).reshape(-1)
+                    arrays = (reqs, self._table, self._end, self._pos) if tree else (reqs, self._table)
                     dev, at, shared = self._upload(*arrays)
-                    parts = [dev[i : i + len(a)] for a, i in zip(arrays, at)]
-                    self._dev = (*parts, *[None] * (3 - len(parts))), shared
-        (table, end, pos), shared = self._dev
+                    parts = [dev[i : i + max(len(a), 1)] for a, i in zip(arrays, at)]
+                    self._dev = (*parts, *[None] * (4 - len(parts))), shared
+        parts, shared = self._dev
         if shared is not None:
             self._reach(shared)
-        return table, end, pos
+        return parts
+
+    def device_data(self):
+        """-> device tensors table, end, pos (the latter None without trees)"""
+        return self._device()[1:]
+
+    def device_requests(self):
+        """-> device tensor [4 requests] int32: first row, new tokens, stored keys, first page in the table"""
+        return self._device()[0]
+
+    def check_move(self, into, keep: int):
+        """raises unless the pages of `into` can take what stays of this batch's requests; settled once for a pair of batches"""
+        got = self._moves.get(keep)
+        if got is not None and got() is into:
+            return
+        if len(into.kv_lens) != len(self.kv_lens):
+            raise ValueError(f"cache_evict: {len(self.kv_lens)} requests into {len(into.kv_lens)}")
+        stay = np.minimum(self.kv_lens, keep)
+        if (into.kv_lens < stay).any():
+            raise ValueError("cache_evict: the trimmed requests have fewer stored keys than stay")
+        need = -(-stay.astype(np.int64) // self.page)
+        first = np.cumsum(into._need) - into._need
+        pages = into._table[np.repeat(first - (np.cumsum(need) - need), need) + np.arange(need.sum())]
+        if len(np.unique(pages)) < len(pages) or np.isin(pages, self._table).any():
+            raise ValueError("cache_evict: a page to be written twice, or one that is read")
+        self._moves[keep] = weakref.ref(into)
 
     def rows(self):
         """-> (slots, positions) of the new tokens, device tensors int64 and int32: where the rows' keys and values go in the cache (page * page size +
@@ -304,3 +331,114 @@ def paged_attn(q, cache: PagedCache, batch: PagedBatch, scale=None, window=None,
     run = _paged_attn if _lib.eager(q, k, v) else _paged_op
     out, lse = run(q, k, v, table, end, pos, lists, counts, at, batch.page, batch.max_page, batch.tokens, scale, window, softcap, bool(return_lse))
     return (out, lse) if return_lse else out
+
+
+def _paged_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, acc: Optional[torch.Tensor], table: torch.Tensor, reqs: torch.Tensor,
+                   end: Optional[torch.Tensor], pos: Optional[torch.Tensor], page: int, max_page: int, tokens: int, longest: int, n_reqs: int, keys: int, scale: float,
+                   window: int, softcap: float) -> torch.Tensor:
+    out = torch.empty((n_reqs, k.shape[2], keys), dtype=torch.float32, device=q.device)
+    _weights_into(out, q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, scale, window, softcap)
+    return out
+
+
+def _weights_into(out, q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, scale, window, softcap):
+    _check_call(q, k, k, tokens, page, max_page, "paged_weights")
+    _lib.same_device(q.device, out, k, lse, acc, table, reqs, end, pos)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
+        raise ValueError(f"paged_weights: lse must be contiguous fp32 {tuple(q.shape[:2])}")
+    n_reqs, _, keys = out.shape
+    if acc is not None and (acc.dtype != torch.float32 or acc.shape != out.shape or not acc.is_contiguous()):
+        raise ValueError(f"paged_weights: acc must be contiguous fp32 {tuple(out.shape)}")
+    if keys < longest:
+        raise ValueError(f"paged_weights: acc holds {keys} keys, a request has {longest}")
+    a = _lib.PagedWeightsArgs()
+    a.q, a.q_tok, a.q_head, a.lse, a.out = q.data_ptr(), q.stride(0), q.stride(1), lse.data_ptr(), out.data_ptr()
+    a.acc = acc.data_ptr() if acc is not None else None
+    a.k, (a.k_page, a.k_row, a.k_head) = k.data_ptr(), k.stride()[:3]
+    a.table, a.reqs = table.data_ptr(), reqs.data_ptr()
+    if end is not None:
+        a.end, a.pos = end.data_ptr(), pos.data_ptr()
+    a.n_reqs, a.tokens, a.keys = n_reqs, tokens, keys
+    a.hq, a.hkv, a.d, a.page, a.window, a.scale, a.softcap = q.shape[1], k.shape[2], q.shape[2], page, window, scale, softcap
+    _lib.launch(_lib.load_library().spinf_paged_weights, a, q.device, "paged_weights")
+
+
+_weights_op = torch.library.custom_op("spinf::paged_weights", _paged_weights, mutates_args=())
+
+
+@_weights_op.register_fake
+def _(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap):
+    return torch.empty((n_reqs, k.shape[2], keys), dtype=torch.float32, device=q.device)
+
+
+def paged_weights(q, cache: PagedCache, batch: PagedBatch, lse, scale=None, window=None, softcap=None, acc=None):
+    """-> [requests, hkv, keys] fp32: acc (None: zeros over the longest request's keys) plus, for every stored key and key / value head, the attention weight that
+    the new tokens' query heads gave it in paged_attn(q, cache, batch, scale, window, softcap, return_lse=True), whose log-sums are ``lse``.  Entries
+    behind a request's stored keys are acc's.  Sums in one fixed order, without atomics."""
+    window = _window(window)
+    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    longest = int(batch.kv_lens.max(initial=0))
+    keys = longest if acc is None else acc.shape[-1]
+    k = cache.k
+    _check_call(q, k, k, batch.tokens, batch.page, batch.max_page, "paged_weights")
+    table, end, pos = batch.device_data()
+    run = _paged_weights if _lib.eager(q, k, lse, acc) else _weights_op
+    return run(q, k, lse, acc, table, batch.device_requests(), end, pos, batch.page, batch.max_page, batch.tokens, longest, len(batch.kv_lens), int(keys), scale, window,
+               float(softcap) if softcap else 0.0)
+
+
+def _cache_evict(k: torch.Tensor, v: torch.Tensor, acc: torch.Tensor, table: torch.Tensor, reqs: torch.Tensor, new_table: torch.Tensor, new_reqs: torch.Tensor,
+                 page: int, keep: int, sink: int, recent: int) -> tuple[torch.Tensor, torch.Tensor]:
+    R, hkv, keys = acc.shape
+    kept = torch.empty((R, hkv, keep), dtype=torch.int32, device=acc.device)
+    new_acc = torch.empty((R, hkv, keep), dtype=torch.float32, device=acc.device)
+    a = _lib.EvictArgs()
+    a.acc, a.keys, a.reqs, a.new_reqs, a.table, a.new_table = acc.data_ptr(), keys, reqs.data_ptr(), new_reqs.data_ptr(), table.data_ptr(), new_table.data_ptr()
+    a.kept, a.new_acc, a.k, a.v = kept.data_ptr(), new_acc.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.k_page, a.k_row, a.k_head = k.stride()[:3]
+    a.v_page, a.v_row, a.v_head = v.stride()[:3]
+    a.n_reqs, a.hkv, a.d, a.page, a.keep, a.sink, a.recent = R, hkv, k.shape[3], page, keep, sink, recent
+    if R and keep and keys:
+        _lib.launch(_lib.load_library().spinf_cache_evict, a, acc.device, "cache_evict")
+    else:   # no stored key at all
+        kept.fill_(-1)
+        new_acc.zero_()
+    return kept, new_acc
+
+
+_evict_op = torch.library.custom_op("spinf::cache_evict", _cache_evict, mutates_args=("k", "v"))
+
+
+@_evict_op.register_fake
+def _(k, v, acc, table, reqs, new_table, new_reqs, page, keep, sink, recent):
+    shape = (*acc.shape[:2], keep)
+    return torch.empty(shape, dtype=torch.int32, device=acc.device), torch.empty(shape, dtype=torch.float32, device=acc.device)
+
+
+def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, keep: int, sink: int = 0, recent: int = 0):
+    """Trims every request of ``batch`` to at most ``keep`` stored keys, per key / value head: all stay where there are no more, else the first ``sink``, the last
+    ``recent``, and of the others those with the largest ``acc`` [requests, hkv, keys] fp32 (ties to the lowest index, NaN above everything).  Their keys
+    and values are copied, in order, into the first entries of the pages that ``into`` (the batch of the trimmed requests) gives them: the old pages stay
+    as they are, since other requests may share them; into's pages must be none of batch's.  Rotated keys keep their positions: a layer with a window, which goes by places,
+    is not trimmed this way.
+    -> kept [requests, hkv, keep] int32 (the places that stayed, ascending, -1 behind them) and their acc (0 behind them): the next paged_weights' acc"""
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError(f"cache_evict: keep {keep}, of these the first {sink} and the last {recent}")
+    k, v = cache.k, cache.v
+    R = len(batch.kv_lens)
+    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (R, k.shape[2]) or not acc.is_contiguous():
+        raise ValueError(f"cache_evict: acc must be contiguous fp32 [{R}, {k.shape[2]}, keys]")
+    if acc.shape[2] < batch.kv_lens.max(initial=0):
+        raise ValueError(f"cache_evict: acc holds {acc.shape[2]} keys, a request has {batch.kv_lens.max()}")
+    if batch.page != cache.page or into.page != cache.page:
+        raise ValueError(f"cache_evict: the batches count pages of {batch.page} and {into.page} keys, the cache has {cache.page}")
+    if max(batch.max_page, into.max_page) >= k.shape[0]:
+        raise ValueError(f"cache_evict: page {max(batch.max_page, into.max_page)} in a table, the cache has {k.shape[0]}")
+    batch.check_move(into, keep)
+    if not acc.is_cuda:
+        raise RuntimeError("cache_evict runs on ROCm device tensors only (no CPU path)")
+    table, new_table, reqs, new_reqs = batch.device_data()[0], into.device_data()[0], batch.device_requests(), into.device_requests()
+    _lib.same_device(acc.device, k, v, table, new_table, reqs, new_reqs)
+    run = _cache_evict if _lib.eager(acc, k, v) else _evict_op
+    return run(k, v, acc, table, reqs, new_table, new_reqs, cache.page, keep, sink, recent)

@@ -208,9 +208,9 @@ def test_plan_and_attention_refuse_bad_arguments_at_the_c_entry(lib):
     assert lib.spinf_paged_attn_fwd(C.byref(b), None) == 0   # nothing to do
     b.n_wave = 1
     assert lib.spinf_paged_attn_fwd(C.byref(b), None) == -1
-    sizes = (C.c_int64 * 2)()
-    assert lib.spinf_paged_struct_sizes(sizes, 2) == 0 and lib.spinf_paged_struct_sizes(sizes, 3) == -1
-    assert list(sizes) == [C.sizeof(_lib.PagedPlanArgs), C.sizeof(_lib.PagedArgs)]
+    sizes = (C.c_int64 * 5)()
+    assert lib.spinf_paged_struct_sizes(sizes, 5) == 0 and lib.spinf_paged_struct_sizes(sizes, 4) == -1
+    assert list(sizes) == [C.sizeof(x) for x in (_lib.PagedPlanArgs, _lib.PagedArgs, _lib.RopeArgs, _lib.PagedWeightsArgs, _lib.EvictArgs)]
 
 
 def test_attention_refuses_tensors_before_any_launch():
@@ -309,3 +309,385 @@ def test_attention_against_the_oracle(dev, q_lens, kv_lens, page, heads, window,
     close(out, want, tol)
     close(lse, wlse, ltol)
     assert torch.equal(out, sa.paged_attn(q, cache, b, scale, window, softcap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("q_lens,kv_lens,page,heads,window,tree", [
+    ([1, 3], [45, 130], 16, (4, 2, 128), 0, None),
+    ([40, 70], [90, 70], 48, (4, 2, 64), 25, None),
+    ([50, 20], [130, 33], 16, (4, 2, 256), 0, (1, 9)),
+    ([9], [40], 32, (2, 1, 512), 0, (2, 5)),
+])
+def test_what_a_row_does_not_see_leaves_no_trace(dev, q_lens, kv_lens, page, heads, window, tree, variant, monkeypatch):
+    """NaN and infinities behind the stored keys, in other requests' pages and in new tokens that some rows do not see: those rows' results stay what they are, and
+    only rows that see such a key are not finite"""
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = make_batch(q_lens, kv_lens, page, dev, tree)
+    cache, q = fill(b, pages, heads, 3, dev)
+    clean = sa.paged_attn(q, cache, b, window=window or None)
+    slots, _ = b.rows()
+    stored = torch.zeros(pages * page, dtype=torch.bool, device=dev)
+    at = 0
+    for n, L in zip(b._need, b.kv_lens):
+        s = np.arange(L)
+        stored[torch.from_numpy(b._table[at : at + n][s // page].astype(np.int64) * page + s % page).to(dev)] = True
+        at += n
+    rubbish = ~stored.view(pages, page)
+    for t, x in ((cache.k, float("nan")), (cache.v, float("inf"))):
+        t[rubbish] = x
+    assert torch.equal(sa.paged_attn(q, cache, b, window=window or None), clean)
+    # one request's last-but-one new token turns into NaN / inf: the rows that do not see it keep their values (to rounding: they may be computed row by row)
+    row = int(b.q_lens[0]) - 2 if b.q_lens[0] > 1 else int(b.tokens) - 2
+    slot = int(slots[row])
+    cache.k[slot // page, slot % page] = float("nan")
+    cache.v[slot // page, slot % page] = float("-inf")
+    out, lse = sa.paged_attn(q, cache, b, window=window or None, return_lse=True)
+    base = np.cumsum(b.q_lens) - b.q_lens
+    touched = np.zeros(b.tokens, bool)
+    for r, see in enumerate(dense(b, window)):
+        T, L = see.shape
+        if base[r] <= row < base[r] + T:
+            touched[base[r] : base[r] + T] = see[:, L - T + row - base[r]]
+    touched = torch.from_numpy(touched).to(dev)
+    assert touched.any() and not touched.all()
+    assert out[touched].isnan().all() and lse[touched].isnan().all()
+    keep = clean[~touched].float()
+    # twice what rounding may cost: probabilities to bf16 in one computation and not in the other, values at most 5 (unit scale, these sizes)
+    assert torch.isfinite(out[~touched]).all() and ((out[~touched].float() - keep).abs() <= 2.0**-8 * (5 + keep.abs())).all()
+
+
+@pytest.mark.gpu
+def test_a_request_has_the_same_bits_whatever_shares_the_call(dev):
+    heads = (8, 2, 128)
+    b, pages = make_batch([1, 300, 37, 2], [4100, 700, 1500, 65], 64, dev)
+    cache, q = fill(b, pages, heads, 5, dev)
+    out = sa.paged_attn(q, cache, b)
+    tables = np.split(b._table, np.cumsum(b._need)[:-1])
+    base = 0
+    for r, (T, L) in enumerate(zip(b.q_lens, b.kv_lens)):
+        one = sa.PagedBatch.build([T], [L], [tables[r]], 64, dev)
+        assert torch.equal(sa.paged_attn(q[base : base + T], cache, one), out[base : base + T])
+        base += T
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 512])
+def test_strided_queries_and_a_single_key(dev, d):
+    b, pages = make_batch([3, 40], [3, 61], 16, dev)
+    heads = (4, 2, d)
+    cache, q = fill(b, pages, heads, 6, dev)
+    wide = torch.zeros((b.tokens, 9, d + 8), dtype=BF16, device=dev)
+    wide[:, 3:7, :d] = q
+    assert torch.equal(sa.paged_attn(wide[:, 3:7, :d], cache, b), sa.paged_attn(q, cache, b))
+    one = sa.PagedBatch.build([1], [1], [[2]], 16, dev)   # a row that sees one key is that key's value
+    assert torch.equal(sa.paged_attn(q[:1], cache, one)[0], cache.v[2, 0].repeat_interleave(2, 0))
+    none = sa.PagedBatch.build([2], [0], [[]], 16, dev)
+    out, lse = sa.paged_attn(q[:2], cache, none, return_lse=True)
+    assert not out.any() and (lse == float("-inf")).all()
+    empty = sa.PagedBatch.build([0, 0], [0, 5], [[], [1]], 16, dev)
+    assert sa.paged_attn(q[:0], cache, empty).shape == (0, 4, d)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+def test_scores_that_range_widely(dev, variant, monkeypatch):
+    """the running maximum rises late and by much, and stays finite where exp alone would not"""
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = make_batch([2, 33], [700, 500], 64, dev)
+    cache, q = fill(b, pages, (4, 2, 128), 8, dev)
+    cache.k.mul_(torch.linspace(0.1, 12, pages, device=dev).to(BF16)[:, None, None, None])
+    q = q * 4
+    out, lse = sa.paged_attn(q, cache, b, return_lse=True)
+    want, wlse, tol, ltol = reference(q, cache, b, 128**-0.5)
+    close(out, want, tol)
+    close(lse, wlse, ltol)
+
+
+# ------------------------------------------------------------------------------------------------ weights
+WEIGHTS = [  # q_lens, kv_lens, page, (hq, hkv, d), window, softcap, tree
+    ([1, 1, 0, 1], [1, 700, 33, 32], 16, (8, 2, 128), 0, 0.0, None),
+    ([1], [2100], 48, (16, 1, 512), 0, 0.0, None),
+    ([64, 5, 40], [457, 5, 2], 80, (4, 2, 256), 0, 30.0, None),
+    ([33, 70], [400, 300], 64, (12, 12, 64), 50, 0.0, None),
+    ([60, 20], [361, 35], 48, (10, 2, 64), 0, 0.0, (1, 9)),
+    ([60, 20], [100, 35], 32, (4, 2, 128), 12, 0.0, (4, 24)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,kv_lens,page,heads,window,softcap,tree", WEIGHTS)
+def test_weights_against_the_oracle(dev, q_lens, kv_lens, page, heads, window, softcap, tree):
+    b, pages = make_batch(q_lens, kv_lens, page, dev, tree)
+    cache, q = fill(b, pages, heads, 11, dev)
+    scale = heads[2] ** -0.5
+    _, lse = sa.paged_attn(q, cache, b, scale, window, softcap, return_lse=True)
+    longest = int(b.kv_lens.max())
+    acc = torch.rand((len(b.kv_lens), heads[1], longest + 5), device=dev)
+    got = sa.paged_weights(q, cache, b, lse, scale, window, softcap, acc=acc)
+    bare = sa.paged_weights(q, cache, b, lse, scale, window, softcap)
+    assert got.shape == acc.shape and bare.shape == (len(b.kv_lens), heads[1], longest)
+    qn, kn, ln = q.double().cpu().numpy(), cache.k.float().cpu().numpy(), lse.double().cpu().numpy()
+    base = 0
+    for r, see in enumerate(dense(b, window)):
+        T, L = see.shape
+        at = int(b._need[:r].sum())
+        k = op.stored(kn, b._table[at : at + b._need[r]], L)
+        rows = slice(base, base + T)
+        want = op.weights(qn[rows], k, see, ln[rows], scale, softcap)
+        # each weight: the score's error (d products in fp32) and exp2's, sums of T x group terms in fp32
+        group = heads[0] // heads[1]
+        size = max([float((np.abs(qn[rows, h]) @ np.abs(k[:, h // group]).T).max(initial=0)) for h in range(heads[0])], default=0) * scale
+        rel = size * (heads[2] + 4) * 2.0**-24 + softcap * 2.0**-21 + (T * group + 40) * 2.0**-24 + 2.0**-20
+        a = acc[r].double().cpu().numpy()
+        close(bare[r, :, :L], want, rel * want + 1e-30)
+        close(got[r, :, :L], a[:, :L] + want, rel * want + 2.0**-23 * (a[:, :L] + want))
+        assert torch.equal(got[r, :, L:], acc[r, :, L:]) and not bare[r, :, L:].any()
+        # what every row gave away sums to one
+        seen = see.any(1)
+        assert abs(float(bare[r].double().sum()) - seen.sum() * heads[0]) <= seen.sum() * heads[0] * (2 * rel + 1e-5)
+        base += T
+
+
+@pytest.mark.gpu
+def test_weights_of_rubbish_that_nobody_sees(dev):
+    b, pages = make_batch([2, 1], [20, 45], 16, dev)
+    cache, q = fill(b, pages, (4, 2, 64), 12, dev)
+    _, lse = sa.paged_attn(q, cache, b, return_lse=True)
+    want = sa.paged_weights(q, cache, b, lse)
+    slot = int(b.rows()[0][1])     # the request's last token: its first row does not see it
+    other = torch.ones(pages, dtype=torch.bool)
+    other[b._table.astype(np.int64)] = False
+    cache.k[other.to(dev)] = float("nan")
+    cache.k[int(b._table[1]), 4:] = float("nan")   # behind the first request's 20 keys
+    assert torch.equal(sa.paged_weights(q, cache, b, lse), want)
+    q0, lse0 = q.clone(), lse.clone()
+    lse0[1] = float("-inf")                        # a row that counts as one that saw nothing
+    cache.k[slot // 16, slot % 16] = float("nan")
+    got = sa.paged_weights(q0, cache, b, lse0)
+    assert torch.isfinite(got[0, :, :19]).all()
+
+
+def test_weights_and_eviction_refuse_bad_arguments():
+    b, pages = make_batch([2, 1], [40, 20], 16)
+    c = sa.PagedCache.empty(pages, 16, 2, 64, "cpu")
+    q, lse = torch.zeros((3, 4, 64), dtype=BF16), torch.zeros((3, 4))
+    with pytest.raises(RuntimeError, match="ROCm"):
+        sa.paged_weights(q, c, b, lse)
+    with pytest.raises(ValueError):
+        sa.paged_weights(q[:2], c, b, lse)
+    free = sorted(set(range(pages)) - set(b._table.tolist()))
+    into = sa.PagedBatch.build([0, 0], [16, 16], [free[:1], free[1:2]], 16, "cpu")
+    acc = torch.zeros((2, 2, 40))
+    with pytest.raises(RuntimeError, match="ROCm"):
+        sa.cache_evict(c, b, into, acc, 16, 4, 4)
+    bad = sa.PagedBatch.build([0, 0], [16, 16], [free[:1], b._table[:1]], 16, "cpu")
+    twice = sa.PagedBatch.build([0, 0], [16, 16], [free[:1], free[:1]], 16, "cpu")
+    short = sa.PagedBatch.build([0, 0], [16, 15], [free[:1], free[1:2]], 16, "cpu")
+    one = sa.PagedBatch.build([0], [16], [free[:1]], 16, "cpu")
+    for x in (bad, twice, short, one):
+        with pytest.raises(ValueError):
+            sa.cache_evict(c, b, x, acc, 16, 4, 4)
+    for args in ((acc[:, :, :39], 16, 4, 4), (acc.double(), 16, 4, 4), (acc[:1], 16, 4, 4), (acc, 16, 14, 4), (acc, 16, -1, 4), (acc, -1, 0, 0)):
+        with pytest.raises(ValueError):
+            sa.cache_evict(c, b, into, *args)
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "wild"])
+@pytest.mark.parametrize("kv_lens,keep,sink,recent,page,hkv,d", [
+    ([900, 40, 33], 40, 4, 7, 16, 2, 64), ([5000, 0, 1], 64, 0, 0, 48, 1, 128), ([130, 129], 128, 4, 64, 64, 3, 256), ([300], 90, 0, 90, 32, 2, 512), ([77, 500], 1, 0, 0, 16, 2, 64),
+    ([20000], 7777, 1, 2, 80, 1, 64),
+])
+def test_eviction_against_the_oracle(dev, kv_lens, keep, sink, recent, page, hkv, d, kind):
+    R, longest = len(kv_lens), max(kv_lens)
+    rng = np.random.default_rng(4)
+    need, new = [-(-n // page) for n in kv_lens], [-(-min(n, keep) // page) for n in kv_lens]
+    pages = sum(need) + sum(new) + 2
+    ids = rng.permutation(pages)
+    cut = np.cumsum(need + new)
+    parts = np.split(ids, cut)[: 2 * R]
+    b = sa.PagedBatch.build([0] * R, kv_lens, parts[:R], page, dev)
+    into = sa.PagedBatch.build([0] * R, [min(n, keep) for n in kv_lens], parts[R:], page, dev)
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn((pages, page, hkv, d), generator=g).to(BF16).to(dev) for _ in range(2))
+    cache = sa.PagedCache(k, v)
+    acc = torch.rand((R, hkv, longest + 3), generator=g) ** 4
+    if kind == "ties":
+        acc = (acc * 6).floor() / 6
+    elif kind == "equal":
+        acc = torch.full_like(acc, 0.25)
+    elif kind == "wild":   # both signs and zeros, infinities, NaN, subnormals
+        acc = torch.randn(acc.shape, generator=g)
+        pick = torch.randint(0, 12, acc.shape, generator=g)
+        for i, x in enumerate((float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 1e-42, -1e-42)):
+            acc[pick == i] = x
+    before = k.clone(), v.clone()
+    accd = acc.to(dev)
+    kept, new_acc = sa.cache_evict(cache, b, into, accd, keep, sink, recent)
+    assert kept.shape == new_acc.shape == (R, hkv, keep)
+    wk, wv = (t.clone() for t in before)
+    for r, n in enumerate(kv_lens):
+        m = min(n, keep)
+        for h in range(hkv):
+            places = op.keep_places(acc[r, h].numpy(), n, keep, sink, recent)
+            assert kept[r, h].tolist() == places.tolist() + [-1] * (keep - m), (r, h)
+            assert np.array_equal(new_acc[r, h].cpu().numpy(), np.concatenate([acc[r, h].numpy()[places], np.zeros(keep - m, np.float32)]), equal_nan=True)
+            src, dst = parts[r][places // page], parts[R + r][np.arange(m) // page]
+            src, dst, e, f = (torch.from_numpy(np.ascontiguousarray(x)).to(dev) for x in (src, dst, places % page, np.arange(m) % page))
+            for t, old in ((wk, before[0]), (wv, before[1])):
+                t[dst, f, h] = old[src, e, h]
+    assert torch.equal(k, wk) and torch.equal(v, wv)   # the kept rows, in order, and nothing else
+
+
+# ------------------------------------------------------------------------------------------------ norms and rotation
+ROPE = [  # tokens, hq, hkv, d, rot, neighbours, plus_one, tables, weights, pos
+    (1, 4, 2, 64, 64, False, False, torch.float32, BF16, torch.int32),
+    (37, 24, 4, 256, 64, False, True, BF16, BF16, torch.int64),
+    (1000, 16, 8, 256, 256, False, False, torch.float32, torch.float32, None),
+    (130, 10, 2, 128, 32, True, True, torch.float32, BF16, torch.int32),
+    (65, 16, 1, 512, 512, True, False, BF16, None, torch.int64),
+    (9, 3, 3, 64, 16, False, False, torch.float32, BF16, None),
+    (5, 5, 1, 128, 0, False, False, torch.float32, BF16, None),
+]
+
+
+def rope_case(dev, T, hq, hkv, d, rot, tables, weights, pos, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    y = torch.randn((T, (hq + 2 * hkv) * d + 8), generator=g).mul_(torch.rand((T, 1), generator=g) * 4).to(BF16).to(dev)
+    q, k, v = (t.unflatten(1, (-1, d)) for t in y[:, 8:].split([hq * d, hkv * d, hkv * d], 1))
+    w = [None, None] if weights is None else [(1 + 0.3 * torch.randn(d, generator=g)).to(weights).to(dev) for _ in range(2)]
+    n = 500 if pos is not None else T
+    ang = torch.rand((n, rot // 2), generator=g) * 6.3
+    full = torch.cat([ang, ang], 1)    # as models hand them over: both halves, of which the first is passed
+    cos, sin = (f(full).to(tables).to(dev)[:, : rot // 2] for f in (torch.cos, torch.sin))
+    p = None if pos is None else torch.randint(0, n, (T,), generator=g).to(pos).to(dev)
+    return q, k, v, *w, cos, sin, p
+
+
+def rope_want(x, w, cos, sin, p, eps, neighbours, plus_one):
+    f = lambda t: None if t is None else t.double().cpu().numpy()  # noqa: E731
+    at = np.arange(x.shape[0]) if p is None else p.cpu().numpy()
+    want = op.norm_rope(f(x), f(w), f(cos)[at], f(sin)[at], eps, neighbours, plus_one)
+    # fp32 arithmetic (a sum of d squares, some ten roundings, of terms no larger than the pair's length), then one rounding to bf16
+    size = np.abs(op.norm_rope(f(x), f(w), np.zeros_like(f(cos)[at]), np.ones_like(f(sin)[at]), eps, neighbours, plus_one)) + np.abs(
+        op.norm_rope(f(x), f(w), np.ones_like(f(cos)[at]), np.zeros_like(f(sin)[at]), eps, neighbours, plus_one))
+    return want, 2.0**-8 * np.abs(want) + (x.shape[2] / 2 + 24) * 2.0**-24 * 1.5 * size + 1e-30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,hq,hkv,d,rot,neighbours,plus_one,tables,weights,pos", ROPE)
+def test_norm_and_rotation_against_the_oracle(dev, T, hq, hkv, d, rot, neighbours, plus_one, tables, weights, pos):
+    q, k, v, wq, wk, cos, sin, p = rope_case(dev, T, hq, hkv, d, rot, tables, weights, pos)
+    got = sa.qk_norm_rope(q, k, wq, wk, cos, sin, 1e-6, p, neighbours, plus_one)
+    for x, w, y in zip((q, k), (wq, wk), got):
+        assert y.is_contiguous() and y.dtype == BF16
+        close(y, *rope_want(x, w, cos, sin, p, 1e-6, neighbours, plus_one))
+    # with the cache: the same queries, the keys and values at their places, everything else as it was
+    page = 16
+    pages = -(-T // page) + 2
+    g = torch.Generator().manual_seed(9)
+    slots = torch.randperm(pages * page, generator=g)[:T].to(dev)
+    if T > 3:
+        slots[1] = -1
+        slots[2] = pages * page
+    for v_norm in (False, True):
+        cache = sa.PagedCache.empty(pages, page, hkv, d, dev)
+        cache.k.fill_(7)
+        cache.v.fill_(5)
+        q2 = sa.qk_norm_rope_put(q, k, v, wq, wk, cos, sin, 1e-6, cache, slots, p, neighbours, plus_one, v_norm)
+        inside = (slots >= 0) & (slots < pages * page)
+        wantk, wantv = torch.full_like(cache.k, 7), torch.full_like(cache.v, 5)
+        s = slots[inside]
+        wantk[s // page, s % page] = got[1][inside]
+        wantv[s // page, s % page] = v[inside]
+        assert torch.equal(cache.k, wantk)
+        if not v_norm:
+            assert torch.equal(cache.v, wantv)
+        else:
+            want, tol = rope_want(v, None, cos[:, :0], sin[:, :0], p, 1e-6, False, False)
+            i = inside.cpu().numpy()
+            close(cache.v[s // page, s % page], want[i], tol[i])
+            rest = torch.ones(pages * page, dtype=torch.bool, device=dev)
+            rest[s] = False
+            assert (cache.v.flatten(0, 1)[rest] == 5).all()
+        known = slots < pages * page
+        assert torch.equal(q2[known], got[0][known]) and q2[~known].isnan().all()
+
+
+@pytest.mark.gpu
+def test_rows_that_say_so_themselves(dev):
+    """a position outside the tables: a query and a key of NaN, the value as it is; a row of zeros, of infinities, of NaN"""
+    q, k, v, wq, wk, cos, sin, _ = rope_case(dev, 5, 4, 2, 64, 32, torch.float32, BF16, torch.int32)
+    pos = torch.tensor([0, -1, 500, 499, 3], device=dev)
+    got = sa.qk_norm_rope(q, k, wq, wk, cos, sin, 1e-6, pos)
+    for y in got:
+        assert y[1:3].isnan().all() and torch.isfinite(y[[0, 3, 4]]).all()
+    q = q.clone()
+    q[0] = 0
+    q[3, 1] = float("inf")
+    q[4, 2, 5] = float("nan")
+    a, b = sa.qk_norm_rope(q, k, wq, wk, cos, sin, 1e-6, pos)
+    assert not a[0].any() and torch.equal(b[[0, 3, 4]], got[1][[0, 3, 4]])
+    assert torch.equal(a[3, [0, 2, 3]], got[0][3, [0, 2, 3]]) and a[4, 2].isnan().all() and torch.equal(a[4, [0, 1, 3]], got[0][4, [0, 1, 3]])
+
+
+def test_norm_and_rotation_refuse_bad_arguments():
+    q, k, w, c = torch.zeros((3, 4, 64), dtype=BF16), torch.zeros((3, 2, 64), dtype=BF16), torch.zeros(64), torch.zeros((3, 16))
+    with pytest.raises(RuntimeError, match="ROCm"):
+        sa.qk_norm_rope(q, k, w, w, c, c, 1e-6)
+
+
+@pytest.mark.gpu
+def test_norm_and_rotation_refuse_tensors_before_any_launch(dev):
+    q, k, w, c = (t.to(dev) for t in (torch.zeros((3, 4, 64), dtype=BF16), torch.zeros((3, 2, 64), dtype=BF16), torch.zeros(64), torch.zeros((3, 16))))
+    good = dict(q=q, k=k, wq=w, wk=w, cos=c, sin=c, eps=1e-6, pos=None)
+    sa.qk_norm_rope(**good)
+    long = torch.zeros((3, 40), device=dev)
+    for bad in (dict(q=q.float()), dict(q=q[:2]), dict(k=k[..., ::2]), dict(wq=w[:32]), dict(wq=w.half()), dict(wq=w.to(BF16)), dict(cos=c.double()), dict(sin=c[:, :8]),
+                dict(cos=c[:2], sin=c[:2]), dict(cos=long, sin=long), dict(cos=c[:, :4], sin=c[:, :4]), dict(pos=torch.zeros(2, dtype=torch.int64, device=dev)),
+                dict(pos=torch.zeros(3, device=dev)), dict(eps=-1.0), dict(eps=float("nan")), dict(wq=w.cpu()), dict(cos=torch.zeros((3, 17), device=dev)[:, 1:], sin=c),
+                dict(q=torch.zeros((3, 4, 96), dtype=BF16, device=dev), k=torch.zeros((3, 2, 96), dtype=BF16, device=dev))):
+        with pytest.raises(ValueError):
+            sa.qk_norm_rope(**{**good, **bad})
+    cache, slots = sa.PagedCache.empty(2, 16, 2, 64, dev), torch.zeros(3, dtype=torch.int64, device=dev)
+    for bad in (dict(slots=slots.int()), dict(slots=slots[:2]), dict(v=k[:2]), dict(cache=sa.PagedCache.empty(2, 16, 2, 128, dev)), dict(cache=sa.PagedCache.empty(2, 16, 1, 64, dev)),
+                dict(cache=sa.PagedCache.empty(0, 16, 2, 64, dev))):
+        with pytest.raises(ValueError):
+            sa.qk_norm_rope_put(**{**good, "v": k, "cache": cache, "slots": slots, **bad})
+
+
+# ------------------------------------------------------------------------------------------------ together
+@pytest.mark.gpu
+def test_streams_compiled_programs_and_recorded_graphs(dev):
+    heads = (8, 2, 128)
+    b, pages = make_batch([1, 70], [900, 300], 64, dev)
+    cache, q = fill(b, pages, heads, 21, dev)
+    acc = torch.rand((2, 2, 900), device=dev)
+    want, lse = sa.paged_attn(q, cache, b, return_lse=True)
+    weight = sa.paged_weights(q, cache, b, lse, acc=acc)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    fresh = pickle.loads(pickle.dumps(b))      # its uploads are made on the default stream, then used on another
+    fresh.device_data()
+    with torch.cuda.stream(side):
+        assert torch.equal(sa.paged_attn(q, cache, fresh), want)
+        assert torch.equal(sa.paged_weights(q, cache, fresh, lse, acc=acc), weight)
+    torch.cuda.synchronize()
+    torch.library.opcheck(torch.ops.spinf.paged_weights.default, (q, cache.k, lse, acc, *[b.device_data()[0], b.device_requests(), None, None], 64, b.max_page, b.tokens, 900, 2, 900, 0.1, 0, 0.0),
+                          test_utils=("test_schema", "test_faketensor"))
+    lists, counts, at = b.plan(8, 2, 128, 0)
+    torch.library.opcheck(torch.ops.spinf.paged_attn.default, (q, cache.k, cache.v, b.device_data()[0], None, None, lists, counts, at, 64, b.max_page, b.tokens, 0.1, 0, 0.0, True),
+                          test_utils=("test_schema", "test_faketensor"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, l2 = sa.paged_attn(q, cache, b, return_lse=True)
+        w2 = sa.paged_weights(q, cache, b, l2, acc=acc)
+    for seed in range(3):
+        q.copy_(fill(b, pages, heads, 30 + seed, dev)[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        e, el = sa.paged_attn(q, cache, b, return_lse=True)
+        assert torch.equal(out, e) and torch.equal(l2, el) and torch.equal(w2, sa.paged_weights(q, cache, b, el, acc=acc))
+        torch.cuda.synchronize()
