@@ -37,7 +37,8 @@ struct Params {
     const __bf16* q; __bf16* out; float* lse;
     long q_tok, q_head, o_tok, o_head;
     const char* k; const char* v;
-    long k_page, k_row, k_head, v_page, v_row, v_head;   // bytes
+    unsigned k_page, k_row, v_page, v_row; long k_head, v_head;   // bytes
+    bool same;                                                    // keys and values have the same strides
     const int* table; const int* end; const int* pos;
     const PagedItem* items; const PagedRun* runs; const PagedJoin* joins;
     float* part_o; float2* part_ml;
@@ -82,21 +83,41 @@ struct Walk {
     }
 };
 
-// where the two halves of a tile lie: byte addresses of the key / value head's row 0 and row 16, and the last row that is stored
+// The pages of a tile's two halves.  Asked for a tile ahead (the scalar loads are on their way while the tile before is computed); pages of a multiple of
+// 32 keys hold both halves, so one is asked for.
+struct Pages {
+    int n, row0, row1, id0, id1;   // the tile's first 16-key piece; rows of the halves inside their pages; the pages
+    __device__ __forceinline__ void ask(const Params& p, const PagedItem& it, int kt) {
+        n = 2 * kt;
+        const int a = p.page.of(n);
+        id0 = sload(p.table, it.tab + a);
+        row0 = (n - a * p.page.pieces) * 16;
+        if (p.page.pieces & 1) {
+            const int end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, b = p.page.of(n1);
+            id1 = sload(p.table, it.tab + b);
+            row1 = (n1 - b * p.page.pieces) * 16;
+        }
+    }
+};
+
+// Where a tile lies: byte addresses of row 0 and row 16 of the key / value head's keys and values, and the tile's last stored row
 struct Place {
     const char *k0, *k1, *v0, *v1;
     int last;
-    __device__ __forceinline__ Place(const Params& p, const PagedItem& it, int kt) {
-        const int n = 2 * kt, end = (it.L - 1) >> 4;
-        last = it.L - 1 - kt * TK < TK - 1 ? it.L - 1 - kt * TK : TK - 1;
-        const int n1 = n + 1 < end ? n + 1 : end;
-        const int a = p.page.of(n), b = p.page.of(n1);
-        const long ia = sload(p.table, it.tab + a), ib = sload(p.table, it.tab + b);
-        const long ra = (long)(n - a * p.page.pieces) * 16, rb = (long)(n1 - b * p.page.pieces) * 16;
-        k0 = p.k + ia * p.k_page + ra * p.k_row + it.kvh * p.k_head;
-        v0 = p.v + ia * p.v_page + ra * p.v_row + it.kvh * p.v_head;
-        k1 = p.k + ib * p.k_page + rb * p.k_row + it.kvh * p.k_head;
-        v1 = p.v + ib * p.v_page + rb * p.v_row + it.kvh * p.v_head;
+    // kb, vb: the cache's keys and values of the key / value head
+    __device__ __forceinline__ Place(const Params& p, const char* kb, const char* vb, int L, const Pages& g) {
+        last = L - 1 - g.n * 16 < TK - 1 ? L - 1 - g.n * 16 : TK - 1;
+        const unsigned long long ko = (unsigned long long)(unsigned)g.id0 * p.k_page + (unsigned long long)(unsigned)g.row0 * p.k_row;
+        k0 = kb + ko;
+        v0 = vb + (p.same ? ko : (unsigned long long)(unsigned)g.id0 * p.v_page + (unsigned long long)(unsigned)g.row0 * p.v_row);
+        if (p.page.pieces & 1) {
+            const unsigned long long k2 = (unsigned long long)(unsigned)g.id1 * p.k_page + (unsigned long long)(unsigned)g.row1 * p.k_row;
+            k1 = kb + k2;
+            v1 = vb + (p.same ? k2 : (unsigned long long)(unsigned)g.id1 * p.v_page + (unsigned long long)(unsigned)g.row1 * p.v_row);
+        } else {
+            k1 = k0 + 16 * (unsigned long long)p.k_row;
+            v1 = v0 + 16 * (unsigned long long)p.v_row;
+        }
     }
 };
 
@@ -116,21 +137,20 @@ struct Rows {
     using GK = Geo<D, TK>;
     using GV = Geo<DV, TK>;
     static constexpr int NS = D / 16, NDT = DV / 32;
+    static constexpr int KAHEAD = D >= 256 ? 3 : 4, VAHEAD = D >= 256 ? 3 : 4;   // fragments read ahead of the products
     bf16x8 qf[NS];
     f32x16 o[NDT];
     float M, l;
-    int lane, m, g, tok, head, qpos;
-    bool valid;
+    int lane, m, g, tok, qpos;
 
     __device__ __forceinline__ void load(const Params& p, const PagedItem& it, int row0) {
         lane = threadIdx.x & 63;
         m = lane & 31;
         g = lane >> 5;
         const int N = it.T * p.group, row = row0 + m;
-        valid = row < N;
-        const int r = valid ? row : N - 1;
+        const int r = row < N ? row : N - 1;
         tok = r / p.group;
-        head = it.kvh * p.group + (r - tok * p.group);
+        const int head = it.kvh * p.group + (r - tok * p.group);
         const __bf16* qp = p.q + (long)(it.cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
@@ -153,10 +173,19 @@ struct Rows {
     // scores of a tile; register i holds key 8 (i / 4) + 4 g + i % 4
     __device__ __forceinline__ void scores(const char* kt_lds, f32x16& s) {
         const char* krow = kt_lds + GK::k_off(m) + 16 * g;
+        constexpr int PF = NS < KAHEAD ? NS : KAHEAD;
+        bf16x8 kf[PF];
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
-        for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(krow + 32 * st), qf[st], s, 0, 0, 0);
+        for (int st = 0; st < PF; st++) kf[st] = *(const bf16x8*)(krow + 32 * st);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < NS; st++) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[st % PF], qf[st], s, 0, 0, 0);
+            if (st + PF < NS) kf[st % PF] = *(const bf16x8*)(krow + 32 * (st + PF));
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     // (four keys at a time, a scheduling barrier in between: requested all at once, the keys' ends and positions would cost the tile loop its registers)
     __device__ __forceinline__ void mask(const Params& p, const PagedItem& it, int kt, const int* meta, bool tree, f32x16& s) {
@@ -228,26 +257,40 @@ struct Rows {
     __device__ __forceinline__ void values(const char* vt_lds, const bf16x8 (&pb)[2]) {
         const int tr_a = lane & 3, tr_j = (lane >> 2) & 3, tr_mb = (lane >> 4) & 1;
         const char* vrow = vt_lds + GV::v_off(4 * g + tr_j) + 32 * tr_mb + 8 * tr_a;
-#pragma unroll
-        for (int f = 0; f < 2 * NDT; f++) {
+        constexpr int NF = 2 * NDT, PF = NF < VAHEAD ? NF : VAHEAD;
+        s16x4 lo[PF], hi[PF];
+        auto ask = [&](const int f) __attribute__((always_inline)) {
             const char* vp = vrow + GV::v_off(16 * (f / NDT)) + 64 * (f % NDT);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)vp);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vp + GV::v_off(8)));
-            const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            lo[f % PF] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)vp);
+            hi[f % PF] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vp + GV::v_off(8)));
+        };
+#pragma unroll
+        for (int f = 0; f < PF; f++) ask(f);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo[f % PF], hi[f % PF], 0, 1, 2, 3, 4, 5, 6, 7));
             o[f % NDT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb[f / NDT], o[f % NDT], 0, 0, 0);
+            if (f + PF < NF) ask(f + PF);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     // is some result of the wave's rows not finite?
-    __device__ __forceinline__ bool spoilt() const {
+    __device__ __forceinline__ bool spoilt(int rows_left) const {
         float t = 0.f;
 #pragma unroll
         for (int dt = 0; dt < NDT; dt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) t += o[dt][i] * 0.f;
-        return __builtin_amdgcn_ballot_w64(valid && !(t == 0.f)) != 0;
+        return __builtin_amdgcn_ballot_w64((lane_now() & 31) < rows_left && !(t == 0.f)) != 0;
     }
 };
 
+// place of a row in lse
+__device__ __forceinline__ long row_head(const Params& p, const PagedItem& it, int row) {
+    const int tok = row / p.group;
+    return (long)(it.cu + tok) * p.hq + it.kvh * p.group + (row - tok * p.group);
+}
 // 1 / sum; rows that saw nothing come out as zeros
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.0f / sum; }
 __device__ __forceinline__ float log_sum(float M, float sum) { return sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * LN2; }
@@ -266,7 +309,9 @@ __device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol) 
     for (int x = 0; x < VEC; x++) o[x] = 0.f;
 #pragma unroll 1
     for (Walk at(p.runs, it, 0); at.more(); at.step(1)) {
-        const Place pl(p, it, at.tile());
+        Pages pages;
+        pages.ask(p, it, at.tile());
+        const Place pl(p, p.k + it.kvh * p.k_head, p.v + it.kvh * p.v_head, it.L, pages);
         const int r = m < pl.last ? m : pl.last, u = at.tile() * TK + m - c;
         const bool fresh = p.end && u >= 0 && u < it.T;
         bool vis = u <= tok && m <= pl.last;
@@ -350,18 +395,22 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
     int* const meta = (int*)(vb + GV::VTILEB);
     const unsigned k_at = lds_addr(kb), v_at = lds_addr(vb), m_at = lds_addr(meta);
     constexpr int NK = GK::NREG, NV = GV::NREG;
+    const char* const k_base = p.k + it.kvh * p.k_head;
+    const char* const v_base = p.v + it.kvh * p.v_head + vcol * 2;
 
     bool tree = false, seen_mask = false;
     rows.reset();
     {
         Walk at(p.runs, it, w);
         const auto is_tree = [&](const Walk& x) { return p.end != nullptr && (x.bits & 16) && x.tile() * TK + TK > c; };
+        Pages pages;
         if (at.more()) {
-            const Place pl(p, it, at.tile());
+            pages.ask(p, it, at.tile());
+            const Place pl(p, k_base, v_base, it.L, pages);
             tree = is_tree(at);
             if (tree) fetch_meta(p, it, at.tile(), m_at, rows.lane);
             fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
-            fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, 0, v_at, rows.lane);
+            fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, rows.lane);
         }
         while (at.more()) {
             const int kt = at.tile();
@@ -369,7 +418,7 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
             seen_mask |= masked;
             at.step(NW);
             const bool next = at.more();
-            const Place pl(p, it, next ? at.tile() : kt);
+            if (next) pages.ask(p, it, at.tile());
             const bool next_tree = next && is_tree(at);
             f32x16 s;
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(NV));   // the keys (and ends, positions) are there; the values may still be on their way
@@ -378,6 +427,7 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
             if (masked) rows.mask(p, it, kt, meta, tree, s);
             __builtin_amdgcn_s_waitcnt(LGKM0);           // nothing reads the tile's keys any more
             __builtin_amdgcn_sched_barrier(0);
+            const Place pl(p, k_base, v_base, it.L, pages);
             if (next) {
                 if (next_tree) fetch_meta(p, it, at.tile(), m_at, rows.lane);
                 fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
@@ -391,11 +441,12 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
             rows.values(vb, pb);
             __builtin_amdgcn_s_waitcnt(LGKM0);
             __builtin_amdgcn_sched_barrier(0);
-            if (next) fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, 0, v_at, rows.lane);
+            if (next) fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, rows.lane);
             tree = next_tree;
         }
     }
-    if (__syncthreads_or(seen_mask && rows.spoilt())) {
+    const int left = it.T * p.group - it.row0;   // rows from this group's first on
+    if (__syncthreads_or(seen_mask && rows.spoilt(left))) {
         for (int j = w; j < 32 && it.row0 + j < it.T * p.group; j += NW) slow_row<D, DV, CAP>(p, it, j, vcol);
         return;
     }
@@ -419,12 +470,12 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
         for (int i4 = 0; i4 < 4; i4++)
             *(float4*)(stage + (w * 32 + rows.m) * OROW + 32 * dt + 8 * i4 + 4 * rows.g) =
                 make_float4(rows.o[dt][4 * i4] * f, rows.o[dt][4 * i4 + 1] * f, rows.o[dt][4 * i4 + 2] * f, rows.o[dt][4 * i4 + 3] * f);
-    if (w == 0 && rows.g == 0 && rows.valid && vcol == 0) {
+    if (w == 0 && rows.g == 0 && rows.m < left && vcol == 0) {
         if (it.part >= 0) p.part_ml[it.part + rows.m] = make_float2(top, total);
-        else if (p.lse) p.lse[(long)(it.cu + rows.tok) * p.hq + rows.head] = log_sum(top, total);
+        else if (p.lse) p.lse[row_head(p, it, it.row0 + rows.m)] = log_sum(top, total);
     }
     __syncthreads();
-    const int here = it.T * p.group - it.row0 < 32 ? it.T * p.group - it.row0 : 32;
+    const int here = left < 32 ? left : 32;
     constexpr int PIECES = DV / 8;
     for (int i = threadIdx.x; i < here * PIECES; i += 64 * NW) {
         const int j = i / PIECES, d = (i - j * PIECES) * 8;
@@ -450,8 +501,40 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------ waves with rows of their own on the same tiles
+// What the tile loop needs of WIN tiles of an item, found by a thread per tile: where their halves lie, which tile it is and its bits.  Found tile by tile
+// with scalar arithmetic, this was 75 of the 110 scalar instructions of a tile, most of them in one wave's way (two documents of 8k new on 8k stored tokens,
+// 32 / 16 x 128: 3,554 us).
+template <int WIN>
+struct Window {
+    unsigned long long k[WIN][2], v[WIN][2];
+    int2 tile[WIN];   // tile, bits
+};
+template <int WIN>
+__device__ __forceinline__ void fill(Window<WIN>& win, const Params& p, const PagedItem& it, int from, const char* kb, const char* vb) {
+    const int i = from + (int)threadIdx.x;
+    int kt = 0, bits = 0;
+    for (int r = 0; r < it.runs; r++) {
+        const int* run = (const int*)(p.runs + it.first + r);
+        const int start = sload(run, 3);
+        if (i >= start) {
+            kt = sload(run, 0) + i - start;
+            bits = sload(run, 2);
+        }
+    }
+    if ((int)threadIdx.x < WIN && i < it.tiles) {
+        const int n = 2 * kt, end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, a = p.page.of(n), b = p.page.of(n1);
+        const unsigned ia = p.table[it.tab + a], ib = p.table[it.tab + b], ra = (n - a * p.page.pieces) * 16, rb = (n1 - b * p.page.pieces) * 16;
+        const int t = threadIdx.x;
+        win.k[t][0] = (unsigned long long)kb + (unsigned long long)ia * p.k_page + (unsigned long long)ra * p.k_row;
+        win.k[t][1] = (unsigned long long)kb + (unsigned long long)ib * p.k_page + (unsigned long long)rb * p.k_row;
+        win.v[t][0] = (unsigned long long)vb + (unsigned long long)ia * p.v_page + (unsigned long long)ra * p.v_row;
+        win.v[t][1] = (unsigned long long)vb + (unsigned long long)ib * p.v_page + (unsigned long long)rb * p.v_row;
+        win.tile[t] = make_int2(kt, bits);
+    }
+}
+
 template <int D, int DV, bool CAP>
-__global__ __launch_bounds__(256, D == 512 ? 1 : 2) void paged_block_kernel(const Params p) {
+__global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_block_kernel(const Params p) {
     using R = Rows<D, DV, CAP>;
     using GK = typename R::GK;
     using GV = typename R::GV;
@@ -459,8 +542,11 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void paged_block_kernel(cons
     constexpr int OROW = DV * 2 + 16;   // bytes of an output row in LDS
     constexpr int LDS = 2 * BUF > 4 * 32 * OROW ? 2 * BUF : 4 * 32 * OROW;
     constexpr int NK = GK::NREG / 4, NV = GV::NREG / 4;
+    constexpr int WIN = 128;
     static_assert(NK * 4 == GK::NREG && NV * 4 == GV::NREG, "a tile's regions must divide among the four waves");
+    static_assert((D == 256 ? 2 : 1) * (LDS + sizeof(Window<WIN>)) <= 160 * 1024, "LDS budget");
     __shared__ __attribute__((aligned(16))) char lds[LDS];
+    __shared__ Window<WIN> win;
     int b = blockIdx.x;
     int vcol = 0;
     if (DV < D) {
@@ -471,64 +557,105 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void paged_block_kernel(cons
     const PagedItem it = load_item(p.items, b);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = it.L - it.T;
+    const char* const k_base = p.k + it.kvh * p.k_head;
+    const char* const v_base = p.v + it.kvh * p.v_head + vcol * 2;
+    fill<WIN>(win, p, it, 0, k_base, v_base);
     R rows;
     rows.load(p, it, it.row0 + 32 * w);
     const unsigned base = lds_addr(lds);
-    const auto is_tree = [&](const Walk& x) { return p.end != nullptr && (x.bits & 0xf0) && x.tile() * TK + TK > c; };
-    const auto issue = [&](const Walk& x, int buf) {
-        const Place pl(p, it, x.tile());
+
+    // This lane's place in the regions that its wave copies: rows r + x (x < NK, NV) of the tile, which lie in one half of it
+    const auto k_row = [&](int lane) { return w * NK + GK::NREG * (lane / GK::CPR); };
+    const auto v_row = [&](int lane) { return w * NV + GV::NREG * (lane / GV::CPR); };
+    const auto issue = [&](int i, int kt, int bits, int buf) __attribute__((always_inline)) {
         const unsigned at = base + buf * BUF;
-        fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, w * NK, at, rows.lane);
-        fetch<DV, NV, GV::VRS>(pl.v0 + vcol * 2, pl.v1 + vcol * 2, p.v_row, pl.last, w * NV, at + GK::KTILEB, rows.lane);
-        if (w == 0 && is_tree(x)) fetch_meta(p, it, x.tile(), at + GK::KTILEB + GV::VTILEB, rows.lane);
+        if (kt * TK + TK <= it.L) {
+            const int lane = D >= 256 ? lane_now() : rows.lane;   // (256 dims: what depends on the lane alone would be spilled, and reloaded in front of every request)
+            const char* ka = (const char*)win.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16);
+            const char* va = (const char*)win.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16);
+#pragma unroll
+            for (int x = 0; x < NK; x++, ka += p.k_row) dma16_lane(ka, at + (w * NK + x) * GK::KRS);
+#pragma unroll
+            for (int x = 0; x < NV; x++, va += p.v_row) dma16_lane(va, at + GK::KTILEB + (w * NV + x) * GV::VRS);
+        } else {   // the request's last tile: rows behind the stored keys are the last key's
+            const int last = it.L - 1 - kt * TK, lane = lane_now();
+#pragma unroll
+            for (int x = 0; x < NK; x++) {
+                const int r = k_row(lane) + x < last ? k_row(lane) + x : last;
+                dma16_lane((const char*)win.k[i][r >> 4] + (r & 15) * (unsigned long long)p.k_row + lane % GK::CPR * 16, at + (w * NK + x) * GK::KRS);
+            }
+#pragma unroll
+            for (int x = 0; x < NV; x++) {
+                const int r = v_row(lane) + x < last ? v_row(lane) + x : last;
+                dma16_lane((const char*)win.v[i][r >> 4] + (r & 15) * (unsigned long long)p.v_row + lane % GV::CPR * 16, at + GK::KTILEB + (w * NV + x) * GV::VRS);
+            }
+        }
+        if (w == 0 && p.end && (bits & 0xf0) && kt * TK + TK > c) fetch_meta(p, it, kt, at + GK::KTILEB + GV::VTILEB, lane_now());
     };
 
     bool seen_mask = false;
     rows.reset();
-    {
-        Walk at(p.runs, it, 0);
-        if (at.more()) issue(at, 0);
-        for (int buf = 0; at.more(); buf ^= 1) {
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
-            __syncthreads();                            // ... and everybody's; the other buffer is free
-            const int kt = at.tile(), bits = at.bits >> w;
-            const bool tree = is_tree(at);
-            at.step(1);
-            if (at.more()) issue(at, buf ^ 1);
-            // A row group that sees nothing of the tile is computed all the same (masked): its wave would wait for the others at the barrier anyway,
-            // and a branch around the products makes the compiler keep the accumulators twice (256 dims: 205 registers spilled).
-            const bool masked = (bits & 17) != 1;
-            seen_mask |= masked;
-            const char* kb = lds + buf * BUF;
-            f32x16 s;
-            rows.scores(kb, s);
-            if (masked) rows.mask(p, it, kt, (const int*)(kb + GK::KTILEB + GV::VTILEB), tree, s);
-            bf16x8 pb[2];
-            rows.softmax(p, s, pb);
-            rows.values(kb + GK::KTILEB, pb);
-        }
+    __syncthreads();
+    int kt = 0, bits = 0;
+    if (it.tiles > 0) {
+        const int2 t = win.tile[0];
+        kt = __builtin_amdgcn_readfirstlane(t.x);
+        bits = __builtin_amdgcn_readfirstlane(t.y);
+        issue(0, kt, bits, 0);
     }
+    for (int i = 0, j = 0, buf = 0; i < it.tiles; i++, buf ^= 1) {   // j: tile i's place in the window
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
+        __syncthreads();                            // ... and everybody's; the other buffer is free
+        if (++j == WIN) {                           // (the window's last tile has been requested)
+            j = 0;
+            fill<WIN>(win, p, it, i + 1, k_base, v_base);
+            __syncthreads();
+        }
+        int kt_next = 0, bits_next = 0;
+        if (i + 1 < it.tiles) {
+            const int2 t = win.tile[j];
+            kt_next = __builtin_amdgcn_readfirstlane(t.x);
+            bits_next = __builtin_amdgcn_readfirstlane(t.y);
+            issue(j, kt_next, bits_next, buf ^ 1);
+        }
+        // A row group that sees nothing of the tile is computed all the same (masked): its wave would wait for the others at the barrier anyway,
+        // and a branch around the products makes the compiler keep the accumulators twice (256 dims: 205 registers spilled).
+        const bool masked = ((bits >> w) & 17) != 1;
+        const bool tree = p.end && (bits & 0xf0) && kt * TK + TK > c;
+        seen_mask |= masked;
+        const char* kb = lds + buf * BUF;
+        f32x16 s;
+        rows.scores(kb, s);
+        if (masked) rows.mask(p, it, kt, (const int*)(kb + GK::KTILEB + GV::VTILEB), tree, s);
+        bf16x8 pb[2];
+        rows.softmax(p, s, pb);
+        rows.values(kb + GK::KTILEB, pb);
+        kt = kt_next;
+        bits = bits_next;
+    }
+    const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
     // (also the barrier behind which the tile buffers are free)
-    if (__syncthreads_or(seen_mask && rows.spoilt())) {
+    if (__syncthreads_or(seen_mask && rows.spoilt(left))) {
         for (int j = w; j < 128 && it.row0 + j < it.T * p.group; j += 4) slow_row<D, DV, CAP>(p, it, j, vcol);
         return;
     }
 
     const float sum = lane32_sum(rows.l);
     const float f = it.part < 0 ? inverse(sum) : 1.f;
+    const int lane = lane_now(), m = lane & 31, g = lane >> 5;
     if (it.part >= 0) {
-        if (!rows.valid) return;
-        const long prow = it.part + 32 * w + rows.m;
-        if (rows.g == 0 && vcol == 0) p.part_ml[prow] = make_float2(rows.M, sum);
+        if (m >= left) return;
+        const long prow = it.part + 32 * w + m;
+        if (g == 0 && vcol == 0) p.part_ml[prow] = make_float2(rows.M, sum);
         float* po = p.part_o + prow * D + vcol;
 #pragma unroll
         for (int dt = 0; dt < R::NDT; dt++)
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++)
-                *(float4*)(po + 32 * dt + 8 * i4 + 4 * rows.g) = make_float4(rows.o[dt][4 * i4], rows.o[dt][4 * i4 + 1], rows.o[dt][4 * i4 + 2], rows.o[dt][4 * i4 + 3]);
+                *(float4*)(po + 32 * dt + 8 * i4 + 4 * g) = make_float4(rows.o[dt][4 * i4], rows.o[dt][4 * i4 + 1], rows.o[dt][4 * i4 + 2], rows.o[dt][4 * i4 + 3]);
         return;
     }
-    if (p.lse && rows.g == 0 && rows.valid && vcol == 0) p.lse[(long)(it.cu + rows.tok) * p.hq + rows.head] = log_sum(rows.M, sum);
+    if (p.lse && g == 0 && m < left && vcol == 0) p.lse[row_head(p, it, it.row0 + 32 * w + m)] = log_sum(rows.M, sum);
     // rows through the wave's own slice of LDS, stored as 16-byte pieces
     char* const stage = lds + w * 32 * OROW;
 #pragma unroll
@@ -538,65 +665,72 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : 2) void paged_block_kernel(cons
             bf16x4 x;
 #pragma unroll
             for (int j = 0; j < 4; j++) x[j] = (__bf16)(rows.o[dt][4 * i4 + j] * f);
-            *(bf16x4*)(stage + rows.m * OROW + (32 * dt + 8 * i4 + 4 * rows.g) * 2) = x;
+            *(bf16x4*)(stage + m * OROW + (32 * dt + 8 * i4 + 4 * g) * 2) = x;
         }
-    const int row0 = it.row0 + 32 * w, here = it.T * p.group - row0;
     constexpr int PIECES = DV / 8;
 #pragma unroll
     for (int k = 0; k < 32 * PIECES / 64; k++) {
-        const int i = k * 64 + rows.lane, j = i / PIECES, d = (i - j * PIECES) * 8;
-        if (j < here) {
-            const int row = row0 + j, tok = row / p.group, head = it.kvh * p.group + (row - tok * p.group);
+        const int i = k * 64 + lane, j = i / PIECES, d = (i - j * PIECES) * 8;
+        if (j < left) {
+            const int row = it.row0 + 32 * w + j, tok = row / p.group, head = it.kvh * p.group + (row - tok * p.group);
             *(bf16x8*)(p.out + (long)(it.cu + tok) * p.o_tok + (long)head * p.o_head + vcol + d) = *(const bf16x8*)(stage + j * OROW + d * 2);
         }
     }
 }
 
-// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces, in ascending order; a wave per row
+// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per row and 64 head dims: 16 lanes per piece, 16 pieces at a time, added up
+// in one fixed order (a wave per row went through a long document's 241 pieces one after the other: 16 rows of 512 dims 73 us).
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
-    constexpr int VEC = D / 64;
-    typedef __attribute__((ext_vector_type(VEC))) float vec;
-    typedef __attribute__((ext_vector_type(VEC))) __bf16 bvec;
-    const int lane = threadIdx.x & 63;
-    const int i = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const int* jp = (const int*)(p.joins + (i >> 5));
-    const int j = i & 31;
+    constexpr int SLICES = D / 64, GROUPS = 16;
+    __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
+    __shared__ float total_sum[GROUPS];
+    const int slice = blockIdx.x % SLICES, i = blockIdx.x / SLICES, j = i % PAGED_JOIN;
+    const int* jp = (const int*)(p.joins + i / PAGED_JOIN);
     if (j >= sload(jp, 3)) return;
     const int cu = sload(jp, 0), kvh = sload(jp, 1), row = sload(jp, 2) + j, n = sload(jp, 5), stride = sload(jp, 6);
     const long part = (long)sload(jp, 4) + j;
-    const int tok = row / p.group, head = kvh * p.group + (row - tok * p.group);
+    const int lane = threadIdx.x & 63, piece = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
     float top = -INFINITY;
     for (int s = lane; s < n; s += 64) top = fmaxf(top, p.part_ml[part + (long)s * stride].x);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.f : top;
-    vec acc = (vec)(0.f);
-    float total = 0.f;
-    for (int s0 = 0; s0 < n; s0 += 4) {   // four pieces requested at a time
-        vec x[4];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
+    for (int s0 = piece; s0 < n; s0 += 4 * GROUPS) {   // four pieces requested at a time
+        float4 x[4];
         float2 ml[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const long at = part + (long)(s0 + k < n ? s0 + k : n - 1) * stride;
-            x[k] = *(const vec*)(p.part_o + at * D + VEC * lane);
+            const int s = s0 + k * GROUPS;
+            const long at = part + (long)(s < n ? s : s0) * stride;
+            x[k] = *(const float4*)(p.part_o + at * D + slice * 64 + d);
             ml[k] = p.part_ml[at];
         }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (s0 + k >= n) break;
+            if (s0 + k * GROUPS >= n) break;
             const float f = ml[k].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[k].x - ref);   // (a piece without a visible key holds zeros, or NaN that stays)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) acc[e] = __builtin_fmaf(f, x[k][e], acc[e]);
+            acc[0] = __builtin_fmaf(f, x[k].x, acc[0]);
+            acc[1] = __builtin_fmaf(f, x[k].y, acc[1]);
+            acc[2] = __builtin_fmaf(f, x[k].z, acc[2]);
+            acc[3] = __builtin_fmaf(f, x[k].w, acc[3]);
             total = __builtin_fmaf(f, ml[k].y, total);
         }
     }
-    const float inv = inverse(total);
-    bvec y;
-#pragma unroll
-    for (int e = 0; e < VEC; e++) y[e] = (__bf16)(acc[e] * inv);
-    *(bvec*)(p.out + (long)(cu + tok) * p.o_tok + (long)head * p.o_head + VEC * lane) = y;
-    if (p.lse && lane == 0) p.lse[(long)(cu + tok) * p.hq + head] = log_sum(top, total);
+    *(float4*)&part_sum[piece][d] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (d == 0) total_sum[piece] = total;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int used = n < GROUPS ? n : GROUPS;
+    float o = 0.f, l = 0.f;
+    for (int s = 0; s < used; s++) {
+        o += part_sum[s][lane];
+        l += total_sum[s];
+    }
+    const int tok = row / p.group, head = kvh * p.group + (row - tok * p.group);
+    p.out[(long)(cu + tok) * p.o_tok + (long)head * p.o_head + slice * 64 + lane] = (__bf16)(o * inverse(l));
+    if (p.lse && slice == 0 && lane == 0) p.lse[(long)(cu + tok) * p.hq + head] = log_sum(top, l);
 }
 
 template <int D, int DV, int NW, bool CAP>
@@ -616,7 +750,7 @@ int launch(Params p, const spinf_paged_args* a, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess && a->n_joins) {
-        hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a->n_joins * 8)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a->n_joins * PAGED_JOIN * (D / 64))), dim3(256), 0, s, p);
         e = hipGetLastError();
     }
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "paged_attn: launch: %s", hipGetErrorString(e));
@@ -631,7 +765,7 @@ int launch_cap(const Params& p, const spinf_paged_args* a, hipStream_t s) {
 
 extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     if (!a) return spinf_fail(SPINF_E_ARG, "paged_attn: null args");
-    if (a->n_wave < 0 || a->n_block < 0 || a->n_joins < 0 || a->part_rows < 0 || a->n_wave > (1 << 26) || a->n_block > (1 << 26) || a->n_joins > (1 << 26))
+    if (a->n_wave < 0 || a->n_block < 0 || a->n_joins < 0 || a->part_rows < 0 || a->n_wave > (1 << 26) || a->n_block > (1 << 26) || a->n_joins > (1 << 24))
         return spinf_fail(SPINF_E_ARG, "paged_attn: bad item counts");
     if (a->n_wave + a->n_block == 0) return SPINF_OK;
     if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv) return spinf_fail(SPINF_E_ARG, "paged_attn: %d query heads do not group over %d key / value heads", a->hq, a->hkv);
@@ -646,8 +780,8 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
         if ((uintptr_t)ptr % 16) return spinf_fail(SPINF_E_ARG, "paged_attn: tensors and lists must be 16-byte aligned");
     for (int64_t st : {a->q_tok, a->q_head, a->o_tok, a->o_head, a->k_page, a->k_row, a->k_head, a->v_page, a->v_row, a->v_head})
         if (st % 8) return spinf_fail(SPINF_E_ARG, "paged_attn: strides must be multiples of 8 elements");
-    if (a->k_row < 0 || a->v_row < 0 || a->k_row > (1 << 24) || a->v_row > (1 << 24))   // (32 rows are reached by 32-bit byte offsets)
-        return spinf_fail(SPINF_E_ARG, "paged_attn: row strides of the cache must lie in 0 .. 2^24");
+    if (a->k_row < 0 || a->v_row < 0 || a->k_row > (1 << 24) || a->v_row > (1 << 24) || a->k_page < 0 || a->v_page < 0 || a->k_page > (1u << 30) || a->v_page > (1u << 30))
+        return spinf_fail(SPINF_E_ARG, "paged_attn: strides of the cache must lie in 0 .. 2^24 elements (rows) and 0 .. 2^30 (pages)");   // (32-bit byte counts; 32 rows by 32-bit offsets)
     const int64_t need = a->part_rows * (a->d + 2) * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
         return spinf_fail(SPINF_E_ARG, "paged_attn: split rows need a 16-byte aligned workspace of %lld bytes", (long long)need);
@@ -655,8 +789,9 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     p.q = (const __bf16*)a->q; p.out = (__bf16*)a->out; p.lse = a->lse;
     p.q_tok = a->q_tok; p.q_head = a->q_head; p.o_tok = a->o_tok; p.o_head = a->o_head;
     p.k = (const char*)a->k; p.v = (const char*)a->v;
-    p.k_page = 2 * a->k_page; p.k_row = 2 * a->k_row; p.k_head = 2 * a->k_head;
-    p.v_page = 2 * a->v_page; p.v_row = 2 * a->v_row; p.v_head = 2 * a->v_head;
+    p.k_page = (unsigned)(2 * a->k_page); p.k_row = (unsigned)(2 * a->k_row); p.k_head = 2 * a->k_head;
+    p.v_page = (unsigned)(2 * a->v_page); p.v_row = (unsigned)(2 * a->v_row); p.v_head = 2 * a->v_head;
+    p.same = a->k_page == a->v_page && a->k_row == a->v_row;
     p.table = a->table; p.end = a->end; p.pos = a->pos;
     p.runs = (const PagedRun*)a->runs; p.joins = (const PagedJoin*)a->joins;
     p.part_o = (float*)a->workspace;

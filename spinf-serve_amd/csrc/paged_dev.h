@@ -12,6 +12,13 @@ typedef const __attribute__((address_space(4))) int* scalar_ints;
 // a value at a wave-uniform address, through the scalar cache
 __device__ __forceinline__ int sload(const int* p, int i) { return ((scalar_ints)(size_t)p)[__builtin_amdgcn_readfirstlane(i)]; }
 
+// The lane's index, found anew (two instructions): for code outside a tile loop, where a value kept in a register across the loop would be spilled.
+__device__ __forceinline__ int lane_now() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+    return lane;
+}
+
 // Division by the page size in pieces of 16 keys: n / pieces for n < 2^27 as the high word of a product, with the multiplier ceil(2^(31 + b) / pieces),
 // b = ceil(log2 pieces), and the shift b - 1 (exact: the multiplier is too large by less than pieces / 2^(31 + b) of itself, times n < 2^31 less than 1 / pieces).
 struct PageDiv {

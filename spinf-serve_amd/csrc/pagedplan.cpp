@@ -178,7 +178,7 @@ class Builder {
                 const int32_t first = (int32_t)p_->runs.size();
                 while (left > 0) {
                     const int64_t take = std::min<int64_t>(left, runs[at].count - off);
-                    p_->runs.push_back({(int32_t)(runs[at].kt + off), (int32_t)take, runs[at].bits, 0});
+                    p_->runs.push_back({(int32_t)(runs[at].kt + off), (int32_t)take, runs[at].bits, cut_tiles.back() - (int32_t)left});
                     left -= take;
                     off += take;
                     if (off == runs[at].count) { at++; off = 0; }
@@ -188,8 +188,8 @@ class Builder {
             for (int h = 0; h < a_->hkv; h++) {
                 const int64_t part = p_->part_rows;
                 if (nsplit > 1) {
-                    for (int64_t j = 0; j < here; j += GROUP)
-                        p_->joins.push_back({r.cu, h, (int32_t)(row0 + j), (int32_t)std::min<int64_t>(GROUP, here - j), (int32_t)(part + j), (int32_t)nsplit, rows, 0});
+                    for (int64_t j = 0; j < here; j += PAGED_JOIN)
+                        p_->joins.push_back({r.cu, h, (int32_t)(row0 + j), (int32_t)std::min<int64_t>(PAGED_JOIN, here - j), (int32_t)(part + j), (int32_t)nsplit, rows, 0});
                     p_->part_rows += nsplit * rows;
                 }
                 for (int64_t s = 0; s < nsplit; s++)
