@@ -30,7 +30,10 @@ from .masks import _Shared, _staging
 VARIANT = int(os.environ.get("SPINF_PAGED_VARIANT", "0"))
 
 
-@dataclass
+BF16 = torch.bfloat16
+
+
+@dataclass(frozen=True)
 class PagedCache:
     """k, v: [pages, page, hkv, d] bf16 in any memory order whose rows of d are contiguous; page a multiple of 16.  What unused entries hold does not
     matter."""
@@ -86,7 +89,9 @@ class PagedBatch:
         self._end, self._pos = end, pos
         self.tokens = int(q_lens.sum(dtype=np.int64))
         self.max_page = int(table.max()) if len(table) else -1
+        self.longest = int(kv_lens.max(initial=0))
         self._plans, self._moves, self._dev, self._rows = {}, {}, None, None
+        self._calls = {}    # argument blocks without their tensors' addresses, by the tensors' shapes and strides and the call's numbers
 
     @classmethod
     def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None) -> "PagedBatch":
@@ -219,6 +224,13 @@ class PagedBatch:
             self._reach(got[3])
         return got[:3]
 
+    def keep(self, key, args, device, *geometry):
+        """notes an argument block with what it points into: the plan of `geometry`, if any, and the batch's own data"""
+        shared = [self._dev[1]] + ([self._plans[(*geometry, VARIANT)][3]] if geometry else [])
+        if len(self._calls) > 256:
+            self._calls.clear()
+        self._calls[key] = bytes(args), device, tuple(x for x in shared if x is not None)
+
     def _compile(self, hq, hkv, d, window, variant):
         lib = _lib.load_library()
         a = _lib.PagedPlanArgs()
@@ -281,27 +293,42 @@ def _fill(a, q, k, v, page, window, scale, softcap):
 def _paged_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, end: Optional[torch.Tensor], pos: Optional[torch.Tensor],
                 lists: torch.Tensor, counts: list[int], at: list[int], page: int, max_page: int, tokens: int, scale: float, window: int, softcap: float,
                 want_lse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    a = _attn_block(q, k, v, table, end, pos, lists, counts, at, page, max_page, tokens, scale, window, softcap)
+    out, lse = _attn_run(a, q, k, v, want_lse)
+    return out, torch.empty((0,), dtype=torch.float32, device=q.device) if lse is None else lse
+
+
+def _attn_block(q, k, v, table, end, pos, lists, counts, at, page, max_page, tokens, scale, window, softcap):
+    """the argument block of a call but for the memory of q, k, v, the outputs and the workspace; raises on tensors the kernels do not take"""
     _check_call(q, k, v, tokens, page, max_page, "paged_attn")
     _lib.same_device(q.device, k, v, table, end, pos, lists)
-    T, hq, d = q.shape
-    out = torch.empty((T, hq, d), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((T, hq) if want_lse else (0,), dtype=torch.float32, device=q.device)
-    if T == 0:
-        return out, lse
     a = _lib.PagedArgs()
     _fill(a, q, k, v, page, window, scale, softcap)
-    a.out, a.o_tok, a.o_head = out.data_ptr(), hq * d, d
-    a.lse = lse.data_ptr() if want_lse else None
+    a.o_tok, a.o_head = q.shape[1] * q.shape[2], q.shape[2]
     a.table = table.data_ptr()
     if end is not None:
         a.end, a.pos = end.data_ptr(), pos.data_ptr()
     base = lists.data_ptr()
     a.wave, a.block, a.runs, a.joins = (base + 4 * i for i in at)
     a.n_wave, a.n_block, _, a.n_joins, a.part_rows = counts
-    if a.part_rows:
-        work = torch.empty(a.part_rows * (d + 2), dtype=torch.float32, device=q.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel() * 4
-    _lib.launch(_lib.load_library().spinf_paged_attn_fwd, a, q.device, "paged_attn")
+    return a
+
+
+def _attn_run(a, q, k, v, want_lse, stream=None):
+    device = q.device
+    T, hq, d = shape = q.shape
+    out = torch.empty(shape, dtype=BF16, device=device)
+    lse = None
+    if want_lse:
+        lse = torch.empty((T, hq), dtype=torch.float32, device=device)
+        a.lse = lse.data_ptr()
+    if T:
+        a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        if a.part_rows:
+            n = a.part_rows * (d + 2)
+            work = torch.empty(n, dtype=torch.float32, device=device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), 4 * n
+        _lib.launch(_lib.load_library().spinf_paged_attn_fwd, a, device, "paged_attn", stream)
     return out, lse
 
 
@@ -320,47 +347,67 @@ def paged_attn(q, cache: PagedCache, batch: PagedBatch, scale=None, window=None,
     those whose subtree it lies in), with ``window`` those less than ``window`` positions behind it.  A row that sees nothing is zeros.
     return_lse: also the natural log of each row's sum of exponentials, [new tokens, hq] fp32 (-inf where a row sees nothing).
     The new tokens' own keys and values have to be in the cache (qk_norm_rope_put).  A request's rows are the same bits whatever else is in the batch."""
-    window = _window(window)
     k, v = cache.k, cache.v
-    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
-    softcap = float(softcap) if softcap else 0.0
+    eager = _lib.eager(q, k, v)
+    if eager:   # a later layer or step of this batch: everything but the tensors' memory was settled by the first
+        key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), v.stride(), scale, window, softcap, VARIANT)
+        got = batch._calls.get(key)
+        if got is not None and q.device == got[1] == k.device == v.device:
+            stream = _lib.raw_stream(got[1].index)
+            for shared in got[2]:
+                if stream not in shared.streams:
+                    shared.reach(stream)
+            out, lse = _attn_run(_lib.PagedArgs.from_buffer_copy(got[0]), q, k, v, return_lse, stream)
+            return (out, lse) if return_lse else out
+    w = _window(window)
+    sc = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    cap = float(softcap) if softcap else 0.0
     _check_call(q, k, v, batch.tokens, batch.page, batch.max_page, "paged_attn")
     _lib.same_device(q.device, k, v)
     table, end, pos = batch.device_data()
-    lists, counts, at = batch.plan(q.shape[1], k.shape[2], q.shape[2], window)
-    run = _paged_attn if _lib.eager(q, k, v) else _paged_op
-    out, lse = run(q, k, v, table, end, pos, lists, counts, at, batch.page, batch.max_page, batch.tokens, scale, window, softcap, bool(return_lse))
+    lists, counts, at = batch.plan(q.shape[1], k.shape[2], q.shape[2], w)
+    args = (q, k, v, table, end, pos, lists, counts, at, batch.page, batch.max_page, batch.tokens, sc, w, cap)
+    if eager:
+        a = _attn_block(*args)
+        batch.keep(key, a, q.device, q.shape[1], k.shape[2], q.shape[2], w)
+        out, lse = _attn_run(a, q, k, v, return_lse)
+    else:
+        out, lse = _paged_op(*args, bool(return_lse))
     return (out, lse) if return_lse else out
 
 
 def _paged_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, acc: Optional[torch.Tensor], table: torch.Tensor, reqs: torch.Tensor,
                    end: Optional[torch.Tensor], pos: Optional[torch.Tensor], page: int, max_page: int, tokens: int, longest: int, n_reqs: int, keys: int, scale: float,
                    window: int, softcap: float) -> torch.Tensor:
-    out = torch.empty((n_reqs, k.shape[2], keys), dtype=torch.float32, device=q.device)
-    _weights_into(out, q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, scale, window, softcap)
-    return out
+    return _weights_run(_weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap), q, k, lse, acc)
 
 
-def _weights_into(out, q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, scale, window, softcap):
+def _weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap):
     _check_call(q, k, k, tokens, page, max_page, "paged_weights")
-    _lib.same_device(q.device, out, k, lse, acc, table, reqs, end, pos)
+    _lib.same_device(q.device, k, lse, acc, table, reqs, end, pos)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
         raise ValueError(f"paged_weights: lse must be contiguous fp32 {tuple(q.shape[:2])}")
-    n_reqs, _, keys = out.shape
-    if acc is not None and (acc.dtype != torch.float32 or acc.shape != out.shape or not acc.is_contiguous()):
-        raise ValueError(f"paged_weights: acc must be contiguous fp32 {tuple(out.shape)}")
+    if acc is not None and (acc.dtype != torch.float32 or acc.shape != (n_reqs, k.shape[2], keys) or not acc.is_contiguous()):
+        raise ValueError(f"paged_weights: acc must be contiguous fp32 [{n_reqs}, {k.shape[2]}, keys]")
     if keys < longest:
         raise ValueError(f"paged_weights: acc holds {keys} keys, a request has {longest}")
     a = _lib.PagedWeightsArgs()
-    a.q, a.q_tok, a.q_head, a.lse, a.out = q.data_ptr(), q.stride(0), q.stride(1), lse.data_ptr(), out.data_ptr()
-    a.acc = acc.data_ptr() if acc is not None else None
-    a.k, (a.k_page, a.k_row, a.k_head) = k.data_ptr(), k.stride()[:3]
+    a.q_tok, a.q_head, (a.k_page, a.k_row, a.k_head) = q.stride(0), q.stride(1), k.stride()[:3]
     a.table, a.reqs = table.data_ptr(), reqs.data_ptr()
     if end is not None:
         a.end, a.pos = end.data_ptr(), pos.data_ptr()
     a.n_reqs, a.tokens, a.keys = n_reqs, tokens, keys
     a.hq, a.hkv, a.d, a.page, a.window, a.scale, a.softcap = q.shape[1], k.shape[2], q.shape[2], page, window, scale, softcap
-    _lib.launch(_lib.load_library().spinf_paged_weights, a, q.device, "paged_weights")
+    return a
+
+
+def _weights_run(a, q, k, lse, acc, stream=None):
+    out = torch.empty((a.n_reqs, a.hkv, a.keys), dtype=torch.float32, device=q.device)
+    a.q, a.k, a.lse, a.out = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
+    if acc is not None:
+        a.acc = acc.data_ptr()
+    _lib.launch(_lib.load_library().spinf_paged_weights, a, q.device, "paged_weights", stream)
+    return out
 
 
 _weights_op = torch.library.custom_op("spinf::paged_weights", _paged_weights, mutates_args=())
@@ -375,34 +422,44 @@ def paged_weights(q, cache: PagedCache, batch: PagedBatch, lse, scale=None, wind
     """-> [requests, hkv, keys] fp32: acc (None: zeros over the longest request's keys) plus, for every stored key and key / value head, the attention weight that
     the new tokens' query heads gave it in paged_attn(q, cache, batch, scale, window, softcap, return_lse=True), whose log-sums are ``lse``.  Entries
     behind a request's stored keys are acc's.  Sums in one fixed order, without atomics."""
-    window = _window(window)
-    scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
-    longest = int(batch.kv_lens.max(initial=0))
-    keys = longest if acc is None else acc.shape[-1]
     k = cache.k
+    eager = _lib.eager(q, k, lse, acc)
+    if eager:
+        key = ("weights", q.shape, q.stride(), q.dtype, k.shape, k.stride(), lse.shape, lse.stride(), lse.dtype, acc if acc is None else (acc.shape, acc.stride(), acc.dtype), scale, window, softcap)
+        got = batch._calls.get(key)
+        if got is not None and q.device == got[1] == k.device == lse.device and (acc is None or acc.device == got[1]):
+            stream = _lib.raw_stream(got[1].index)
+            for shared in got[2]:
+                if stream not in shared.streams:
+                    shared.reach(stream)
+            return _weights_run(_lib.PagedWeightsArgs.from_buffer_copy(got[0]), q, k, lse, acc, stream)
+    w = _window(window)
+    sc = float(scale) if scale is not None else q.shape[-1] ** -0.5
+    longest = batch.longest
+    keys = longest if acc is None else acc.shape[-1]
     _check_call(q, k, k, batch.tokens, batch.page, batch.max_page, "paged_weights")
     table, end, pos = batch.device_data()
-    run = _paged_weights if _lib.eager(q, k, lse, acc) else _weights_op
-    return run(q, k, lse, acc, table, batch.device_requests(), end, pos, batch.page, batch.max_page, batch.tokens, longest, len(batch.kv_lens), int(keys), scale, window,
-               float(softcap) if softcap else 0.0)
+    args = (q, k, lse, acc, table, batch.device_requests(), end, pos, batch.page, batch.max_page, batch.tokens, longest, len(batch.kv_lens), int(keys), sc, w, float(softcap) if softcap else 0.0)
+    if not eager:
+        return _weights_op(*args)
+    a = _weights_block(*args)
+    batch.keep(key, a, q.device)
+    return _weights_run(a, q, k, lse, acc)
 
 
 def _cache_evict(k: torch.Tensor, v: torch.Tensor, acc: torch.Tensor, table: torch.Tensor, reqs: torch.Tensor, new_table: torch.Tensor, new_reqs: torch.Tensor,
                  page: int, keep: int, sink: int, recent: int) -> tuple[torch.Tensor, torch.Tensor]:
+    device = acc.device
+    _lib.same_device(device, k, v, table, new_table, reqs, new_reqs)
+    shape = (*acc.shape[:2], keep)
+    kept, new_acc = torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
     R, hkv, keys = acc.shape
-    kept = torch.empty((R, hkv, keep), dtype=torch.int32, device=acc.device)
-    new_acc = torch.empty((R, hkv, keep), dtype=torch.float32, device=acc.device)
-    a = _lib.EvictArgs()
-    a.acc, a.keys, a.reqs, a.new_reqs, a.table, a.new_table = acc.data_ptr(), keys, reqs.data_ptr(), new_reqs.data_ptr(), table.data_ptr(), new_table.data_ptr()
-    a.kept, a.new_acc, a.k, a.v = kept.data_ptr(), new_acc.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.k_page, a.k_row, a.k_head = k.stride()[:3]
-    a.v_page, a.v_row, a.v_head = v.stride()[:3]
-    a.n_reqs, a.hkv, a.d, a.page, a.keep, a.sink, a.recent = R, hkv, k.shape[3], page, keep, sink, recent
-    if R and keep and keys:
-        _lib.launch(_lib.load_library().spinf_cache_evict, a, acc.device, "cache_evict")
-    else:   # no stored key at all
-        kept.fill_(-1)
-        new_acc.zero_()
+    if not (R and keep and keys):   # no stored key at all
+        return kept.fill_(-1), new_acc.zero_()
+    ks, vs = k.stride(), v.stride()
+    a = _lib.EvictArgs(acc.data_ptr(), keys, reqs.data_ptr(), new_reqs.data_ptr(), table.data_ptr(), new_table.data_ptr(), kept.data_ptr(), new_acc.data_ptr(), k.data_ptr(),
+                       v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], R, hkv, k.shape[3], page, keep, sink, recent)
+    _lib.launch(_lib.load_library().spinf_cache_evict, a, device, "cache_evict")
     return kept, new_acc
 
 
@@ -426,19 +483,18 @@ def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, kee
     if sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError(f"cache_evict: keep {keep}, of these the first {sink} and the last {recent}")
     k, v = cache.k, cache.v
+    pages, page, hkv, _ = k.shape
     R = len(batch.kv_lens)
-    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (R, k.shape[2]) or not acc.is_contiguous():
-        raise ValueError(f"cache_evict: acc must be contiguous fp32 [{R}, {k.shape[2]}, keys]")
-    if acc.shape[2] < batch.kv_lens.max(initial=0):
-        raise ValueError(f"cache_evict: acc holds {acc.shape[2]} keys, a request has {batch.kv_lens.max()}")
-    if batch.page != cache.page or into.page != cache.page:
-        raise ValueError(f"cache_evict: the batches count pages of {batch.page} and {into.page} keys, the cache has {cache.page}")
-    if max(batch.max_page, into.max_page) >= k.shape[0]:
-        raise ValueError(f"cache_evict: page {max(batch.max_page, into.max_page)} in a table, the cache has {k.shape[0]}")
+    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[0] != R or acc.shape[1] != hkv or not acc.is_contiguous():
+        raise ValueError(f"cache_evict: acc must be contiguous fp32 [{R}, {hkv}, keys]")
+    if acc.shape[2] < batch.longest:
+        raise ValueError(f"cache_evict: acc holds {acc.shape[2]} keys, a request has {batch.longest}")
+    if batch.page != page or into.page != page:
+        raise ValueError(f"cache_evict: the batches count pages of {batch.page} and {into.page} keys, the cache has {page}")
+    if max(batch.max_page, into.max_page) >= pages:
+        raise ValueError(f"cache_evict: page {max(batch.max_page, into.max_page)} in a table, the cache has {pages}")
     batch.check_move(into, keep)
     if not acc.is_cuda:
         raise RuntimeError("cache_evict runs on ROCm device tensors only (no CPU path)")
-    table, new_table, reqs, new_reqs = batch.device_data()[0], into.device_data()[0], batch.device_requests(), into.device_requests()
-    _lib.same_device(acc.device, k, v, table, new_table, reqs, new_reqs)
-    run = _cache_evict if _lib.eager(acc, k, v) else _evict_op
-    return run(k, v, acc, table, reqs, new_table, new_reqs, cache.page, keep, sink, recent)
+    old, new = batch._device(), into._device()
+    return (_cache_evict if _lib.eager(acc, k, v) else _evict_op)(k, v, acc, old[1], old[0], new[1], new[0], page, keep, sink, recent)

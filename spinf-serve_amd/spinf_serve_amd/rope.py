@@ -73,13 +73,47 @@ def _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, what):
     return a
 
 
+# Argument blocks without their tensors' addresses, by everything the checks above look at (shapes, strides, types, numbers): a layer's later calls
+# check the devices and the alignment alone.
+_SEEN: dict = {}
+
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _known(key, device, tensors):
+    """the block kept for this key, if the tensors lie on `device` and are aligned as the kernel wants them"""
+    got = _SEEN.get(key)
+    if got is None or device.type != "cuda":
+        return None
+    for t in tensors:
+        if t is not None and (t.device != device or t.data_ptr() % 16):
+            return None   # (the checks say what is wrong)
+    a = _lib.RopeArgs.from_buffer_copy(got)
+    a.q, a.k, a.v, a.wq, a.wk, a.cos, a.sin = (None if t is None else t.data_ptr() for t in tensors[:7])
+    return a
+
+
+def _note(key, a):
+    if len(_SEEN) > 1024:
+        _SEEN.clear()
+    _SEEN[key] = bytes(a)
+
+
 def _rope(q: torch.Tensor, k: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
           pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    a = _rope_args(q, k, None, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope")
-    q_out, k_out = (torch.empty(t.shape, dtype=torch.bfloat16, device=q.device) for t in (q, k))
+    device = q.device
+    key = (_meta(q), _meta(k), _meta(wq), _meta(wk), _meta(cos), _meta(sin), _meta(pos), eps, neighbours, plus_one)
+    a = _known(key, device, (q, k, None, wq, wk, cos, sin))
+    if a is None or (pos is not None and pos.device != device):
+        a = _rope_args(q, k, None, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope")
+        _note(key, a)
+    q_out, k_out = torch.empty(q.shape, dtype=torch.bfloat16, device=device), torch.empty(k.shape, dtype=torch.bfloat16, device=device)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
+    a.pos = pos.data_ptr() if pos is not None else None
     if q.shape[0]:
-        _lib.launch(_lib.load_library().spinf_qk_norm_rope, a, q.device, "spinf_qk_norm_rope")
+        _lib.launch(_lib.load_library().spinf_qk_norm_rope, a, device, "spinf_qk_norm_rope")
     return q_out, k_out
 
 
@@ -101,21 +135,27 @@ def qk_norm_rope(q, k, wq, wk, cos, sin, eps, pos=None, neighbours=False, plus_o
 
 def _put(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
          ck: torch.Tensor, cv: torch.Tensor, slots: torch.Tensor, pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool, v_norm: bool) -> torch.Tensor:
-    a = _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope_put")
-    if ck.shape[2:] != k.shape[1:]:
-        raise ValueError(f"the cache holds {tuple(ck.shape[2:])} a key, the layer makes {tuple(k.shape[1:])}")
-    if slots.dtype != torch.int64 or slots.shape != (q.shape[0],) or not slots.is_contiguous():
-        raise ValueError(f"slots must hold {q.shape[0]} contiguous int64 values")
-    if q.shape[0] and (ck.shape[0] == 0 or ck.shape[0] * ck.shape[1] >= 1 << 31):
-        raise ValueError(f"a cache of {ck.shape[0]} pages of {ck.shape[1]} keys")
-    _lib.same_device(q.device, ck, cv, slots)
-    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    device = q.device
+    key = (_meta(q), _meta(k), _meta(v), _meta(wq), _meta(wk), _meta(cos), _meta(sin), _meta(pos), _meta(ck), cv.stride(), _meta(slots), eps, neighbours, plus_one, v_norm)
+    a = _known(key, device, (q, k, v, wq, wk, cos, sin, ck, cv))
+    if a is None or (pos is not None and pos.device != device) or slots.device != device:
+        a = _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope_put")
+        if ck.shape[2:] != k.shape[1:]:
+            raise ValueError(f"the cache holds {tuple(ck.shape[2:])} a key, the layer makes {tuple(k.shape[1:])}")
+        if slots.dtype != torch.int64 or slots.shape != (q.shape[0],) or not slots.is_contiguous():
+            raise ValueError(f"slots must hold {q.shape[0]} contiguous int64 values")
+        if q.shape[0] and (ck.shape[0] == 0 or ck.shape[0] * ck.shape[1] >= 1 << 31):
+            raise ValueError(f"a cache of {ck.shape[0]} pages of {ck.shape[1]} keys")
+        _lib.same_device(device, ck, cv, slots)
+        a.k_page, a.k_row, a.kh_out = ck.stride()[:3]
+        a.v_page, a.v_row, a.vh_out = cv.stride()[:3]
+        a.pages, a.page, a.v_norm = ck.shape[0], ck.shape[1], int(v_norm)
+        _note(key, a)
+    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
     a.q_out, a.k_out, a.v_out, a.slots = q_out.data_ptr(), ck.data_ptr(), cv.data_ptr(), slots.data_ptr()
-    a.k_page, a.k_row, a.kh_out = ck.stride()[:3]
-    a.v_page, a.v_row, a.vh_out = cv.stride()[:3]
-    a.pages, a.page, a.v_norm = ck.shape[0], ck.shape[1], int(v_norm)
+    a.pos = pos.data_ptr() if pos is not None else None
     if q.shape[0]:
-        _lib.launch(_lib.load_library().spinf_qk_norm_rope, a, q.device, "spinf_qk_norm_rope")
+        _lib.launch(_lib.load_library().spinf_qk_norm_rope, a, device, "spinf_qk_norm_rope")
     return q_out
 
 
