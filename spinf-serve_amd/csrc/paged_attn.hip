@@ -91,11 +91,11 @@ struct Pages {
         n = 2 * kt;
         const int a = p.page.of(n);
         id0 = sload(p.table, it.tab + a);
-        row0 = (n - a * p.page.pieces) * 16;
-        if (p.page.pieces & 1) {
+        row0 = (n - a * p.page.d) * 16;
+        if (p.page.d & 1) {
             const int end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, b = p.page.of(n1);
             id1 = sload(p.table, it.tab + b);
-            row1 = (n1 - b * p.page.pieces) * 16;
+            row1 = (n1 - b * p.page.d) * 16;
         }
     }
 };
@@ -110,7 +110,7 @@ struct Place {
         const unsigned long long ko = (unsigned long long)(unsigned)g.id0 * p.k_page + (unsigned long long)(unsigned)g.row0 * p.k_row;
         k0 = kb + ko;
         v0 = vb + (p.same ? ko : (unsigned long long)(unsigned)g.id0 * p.v_page + (unsigned long long)(unsigned)g.row0 * p.v_row);
-        if (p.page.pieces & 1) {
+        if (p.page.d & 1) {
             const unsigned long long k2 = (unsigned long long)(unsigned)g.id1 * p.k_page + (unsigned long long)(unsigned)g.row1 * p.k_row;
             k1 = kb + k2;
             v1 = vb + (p.same ? k2 : (unsigned long long)(unsigned)g.id1 * p.v_page + (unsigned long long)(unsigned)g.row1 * p.v_row);
@@ -523,7 +523,7 @@ __device__ __forceinline__ void fill(Window<WIN>& win, const Params& p, const Pa
     }
     if ((int)threadIdx.x < WIN && i < it.tiles) {
         const int n = 2 * kt, end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, a = p.page.of(n), b = p.page.of(n1);
-        const unsigned ia = p.table[it.tab + a], ib = p.table[it.tab + b], ra = (n - a * p.page.pieces) * 16, rb = (n1 - b * p.page.pieces) * 16;
+        const unsigned ia = p.table[it.tab + a], ib = p.table[it.tab + b], ra = (n - a * p.page.d) * 16, rb = (n1 - b * p.page.d) * 16;
         const int t = threadIdx.x;
         win.k[t][0] = (unsigned long long)kb + (unsigned long long)ia * p.k_page + (unsigned long long)ra * p.k_row;
         win.k[t][1] = (unsigned long long)kb + (unsigned long long)ib * p.k_page + (unsigned long long)rb * p.k_row;

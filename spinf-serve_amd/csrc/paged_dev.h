@@ -19,21 +19,25 @@ __device__ __forceinline__ int lane_now() {
     return lane;
 }
 
-// Division by the page size in pieces of 16 keys: n / pieces for n < 2^27 as the high word of a product, with the multiplier ceil(2^(31 + b) / pieces),
-// b = ceil(log2 pieces), and the shift b - 1 (exact: the multiplier is too large by less than pieces / 2^(31 + b) of itself, times n < 2^31 less than 1 / pieces).
-struct PageDiv {
-    int pieces; unsigned mul; int shift;   // mul 0: divide by 1
-    static PageDiv of_page(int page) {
-        PageDiv d = {page / 16, 0, 0};
-        if (d.pieces > 1) {
+// Division of n < 2^31 by a number known when the kernel is launched, as the high word of a product: the multiplier ceil(2^(31 + b) / d), b = ceil(log2 d), and the
+// shift b - 1 (exact: the multiplier is too large by less than one, which is less than 2^b / n of a unit of the quotient's last place).
+struct Div {
+    int d; unsigned mul; int shift;   // mul 0: divide by 1
+    static Div by(int d) {
+        Div x = {d, 0, 0};
+        if (d > 1) {
             int b = 0;
-            while ((1 << b) < d.pieces) b++;
-            d.mul = (unsigned)(((1ull << (31 + b)) + d.pieces - 1) / d.pieces);
-            d.shift = b - 1;
+            while ((1 << b) < d) b++;
+            x.mul = (unsigned)(((1ull << (31 + b)) + d - 1) / d);
+            x.shift = b - 1;
         }
-        return d;
+        return x;
     }
     __device__ __forceinline__ int of(int n) const { return mul ? (int)(__umulhi((unsigned)n, mul) >> shift) : n; }
+};
+// of the page size, in pieces of 16 keys
+struct PageDiv : Div {
+    static PageDiv of_page(int page) { return {Div::by(page / 16)}; }
 };
 
 constexpr int vmcnt_imm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }   // waits for all but the n youngest vector memory operations

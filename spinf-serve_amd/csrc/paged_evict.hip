@@ -36,8 +36,11 @@ __device__ __forceinline__ unsigned order(float x) {
 constexpr int KW = 16;          // waves of a workgroup
 constexpr int BINS = 2048;
 
+// J: 64-key pieces of a wave's stretch that stay in registers, loaded once and together; 0: any number, loaded anew for every pass, eight at a time.
+// (One at a time, anew for every pass, the loads' latency was all the time there was: 128 sets of 12,000 keys 45 us.)
+template <int J>
 __global__ __launch_bounds__(64 * KW) void paged_keep_kernel(const Params p) {
-    __shared__ int hist[BINS];
+    __shared__ __attribute__((aligned(16))) int hist[BINS][4];   // four counts a bin, by lane: equal weights queue for one word otherwise
     __shared__ int wave_sum[KW], above[KW], equal[KW];
     __shared__ int found[2];
     const int rh = blockIdx.x, r = rh / p.hkv;
@@ -55,23 +58,52 @@ __global__ __launch_bounds__(64 * KW) void paged_keep_kernel(const Params p) {
     }
     const int c0 = p.sink, c1 = n - p.recent;             // candidates
     const int want = p.keep - p.sink - p.recent;          // of these stay (0 <= want < c1 - c0)
+    const int per = ((n + KW - 1) / KW + 63) / 64 * 64, i0 = w * per, i1 = i0 + per < n ? i0 + per : n;   // this wave's stretch of the keys
+    float mine[J ? J : 8];
+    if (J) {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int i = i0 + j * 64 + lane;
+            mine[j] = j * 64 < per ? x[i < i1 ? i : 0] : 0.f;
+        }
+    }
+    // f(i, weight) for every 64 keys of the stretch, whole waves: i >= i1 is no key
+    const auto each = [&](auto f) __attribute__((always_inline)) {
+        if (J) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (i0 + j * 64 < i1) f(i0 + j * 64 + lane, mine[j]);
+        } else {
+            for (int b = i0; b < i1; b += 8 * 64) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = b + j * 64 + lane;
+                    mine[j] = x[i < i1 ? i : 0];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (b + j * 64 < i1) f(b + j * 64 + lane, mine[j]);
+            }
+        }
+    };
     // the smallest key that stays, digit by digit: `floor` holds the digits found, `left` how many of the keys with these digits stay
     unsigned floor = 0;
     int left = want;
-    const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
     if (want > 0) {
 #pragma unroll 1
         for (int d = 0; d < 3; d++) {
-            const int sh = shifts[d], nb = 1 << bits[d];
-            for (int i = tid; i < BINS; i += 64 * KW) hist[i] = 0;
+            const int sh = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
+            for (int i = tid; i < BINS; i += 64 * KW) *(int4*)hist[i] = make_int4(0, 0, 0, 0);
             __syncthreads();
-            for (int i = c0 + tid; i < c1; i += 64 * KW) {
-                const unsigned o = order(x[i]);
-                if (d == 0 || (o >> (sh + bits[d])) == (floor >> (sh + bits[d]))) atomicAdd(&hist[(o >> sh) & (nb - 1)], 1);
-            }
+            each([&](int i, float xi) __attribute__((always_inline)) {
+                const unsigned o = order(xi);
+                if (i >= c0 && i < c1 && i < i1 && (d == 0 || (o >> (sh + bits)) == (floor >> (sh + bits)))) atomicAdd(&hist[(o >> sh) & ((1 << bits) - 1)][lane & 3], 1);
+            });
             __syncthreads();
             // bins from the highest down, two per thread: a running count over the workgroup, and the bin in which it reaches `left`
-            const int b1 = BINS - 1 - 2 * tid, n1 = hist[b1], n0 = hist[b1 - 1];
+            const int b1 = BINS - 1 - 2 * tid;
+            const int4 h1 = *(const int4*)hist[b1], h0 = *(const int4*)hist[b1 - 1];
+            const int n1 = h1.x + h1.y + h1.z + h1.w, n0 = h0.x + h0.y + h0.z + h0.w;
             int run = n1 + n0;
 #pragma unroll
             for (int k = 1; k < 64; k <<= 1) {
@@ -87,21 +119,16 @@ __global__ __launch_bounds__(64 * KW) void paged_keep_kernel(const Params p) {
             __syncthreads();
             floor |= (unsigned)found[0] << sh;
             left = found[1];
-            __syncthreads();
         }
     }
-    // Each wave counts its stretch of the keys: those above the floor (or kept whatever they weigh), and those equal to it.
-    const int per = ((n + KW - 1) / KW + 63) / 64 * 64, i0 = w * per, i1 = i0 + per < n ? i0 + per : n;
+    // Each wave counts in its stretch the keys above the floor (or kept whatever they weigh), and those equal to it.
     int a = 0, e = 0;
-    for (int i = i0 + lane; i < i1; i += 64) {
-        const bool always = i < c0 || i >= c1;
-        const unsigned o = always ? 0 : order(x[i]);
-        a += __popcll(__builtin_amdgcn_ballot_w64(always || (want > 0 && o > floor)));
-        e += __popcll(__builtin_amdgcn_ballot_w64(!always && want > 0 && o == floor));
-    }
-    // (lanes behind the end have left the loop: lane 0 is in every round)
-    a = __builtin_amdgcn_readfirstlane(a);
-    e = __builtin_amdgcn_readfirstlane(e);
+    each([&](int i, float xi) __attribute__((always_inline)) {
+        const bool in = i < i1, always = in && (i < c0 || i >= c1);
+        const unsigned o = order(xi);
+        a += __popcll(__builtin_amdgcn_ballot_w64(always || (in && want > 0 && o > floor)));
+        e += __popcll(__builtin_amdgcn_ballot_w64(in && !always && want > 0 && o == floor));
+    });
     if (lane == 0) { above[w] = a; equal[w] = e; }
     __syncthreads();
     int at = 0, ties = 0;   // kept keys and ties in front of this wave's stretch
@@ -111,14 +138,12 @@ __global__ __launch_bounds__(64 * KW) void paged_keep_kernel(const Params p) {
         ties += equal[k];
     }
     const unsigned long long below = (1ull << lane) - 1;
-    for (int base = i0; base < i1; base += 64) {
-        const int i = base + lane;
+    each([&](int i, float xi) __attribute__((always_inline)) {
         const bool in = i < i1, always = in && (i < c0 || i >= c1);
-        const float xi = in ? x[i] : 0.f;
         const unsigned o = order(xi);
         const bool tie = in && !always && want > 0 && o == floor;
         const unsigned long long tie_mask = __builtin_amdgcn_ballot_w64(tie);
-        const bool stays = always || (in && want > 0 && !always && o > floor) || (tie && ties + __popcll(tie_mask & below) < left);
+        const bool stays = always || (in && want > 0 && o > floor) || (tie && ties + __popcll(tie_mask & below) < left);
         const unsigned long long mask = __builtin_amdgcn_ballot_w64(stays);
         if (stays) {
             const int j = at + __popcll(mask & below);
@@ -127,7 +152,7 @@ __global__ __launch_bounds__(64 * KW) void paged_keep_kernel(const Params p) {
         }
         at += __popcll(mask);
         ties += __popcll(tie_mask);
-    }
+    });
 }
 
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
@@ -152,7 +177,7 @@ __global__ __launch_bounds__(256) void paged_move_kernel(const Params p) {
             const int s = kept[jc];
             const int a = p.page.of(s >> 4), b = p.page.of(jc >> 4);
             const long from = p.table[tab + a], dst = p.new_table[to + b];
-            const long es = s - a * p.page.pieces * 16, ed = jc - b * p.page.pieces * 16;
+            const long es = s - a * p.page.d * 16, ed = jc - b * p.page.d * 16;
             xk[u] = *(const u32x4*)(p.k + from * p.k_page + es * p.k_row + h * p.k_head + piece * 16);
             xv[u] = *(const u32x4*)(p.v + from * p.v_page + es * p.v_row + h * p.v_head + piece * 16);
             dk[u] = dst * p.k_page + ed * p.k_row + h * p.k_head + piece * 16;
@@ -192,7 +217,11 @@ extern "C" int spinf_cache_evict(const spinf_evict_args* a, void* stream) {
     const int64_t grid = a->n_reqs * a->hkv;
     if (grid * p.chunks > INT32_MAX) return spinf_fail(SPINF_E_ARG, "cache_evict: %lld requests of %d kept keys are too many", (long long)a->n_reqs, a->keep);
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(paged_keep_kernel, dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    // (stretches of up to 4, 16 and 32 pieces of 64 keys: 4,096, 16,384 and 32,768 keys)
+    if (a->keys <= 4 * 64 * KW) hipLaunchKernelGGL(paged_keep_kernel<4>, dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    else if (a->keys <= 16 * 64 * KW) hipLaunchKernelGGL(paged_keep_kernel<16>, dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    else if (a->keys <= 32 * 64 * KW) hipLaunchKernelGGL(paged_keep_kernel<32>, dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    else hipLaunchKernelGGL(paged_keep_kernel<0>, dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
         const dim3 g((unsigned)(grid * p.chunks));

@@ -6,9 +6,9 @@
 //
 // S = Q K^T the other way round than in the attention: a lane of v_mfma_f32_32x32x16_bf16's result owns one KEY and 16 of the 32 rows, so a key's
 // sum stays in its lane over all rows: no atomics, one order, one lane exchange at the end.  A workgroup's waves take 32 keys each: the keys come once, by
-// DMA through LDS, and stay in registers; the rows come from memory block by block.
+// DMA through LDS, and stay in registers; the rows follow into the same place, a block of 32 per wave at a time.
 //
-// Bound by HBM where rows are few (a decoding step: the keys' bytes), by the loads of the rows where they are many.
+// Bound by HBM where rows are few (a decoding step: the keys' bytes).
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -26,81 +26,79 @@ struct Params {
     long k_page, k_row, k_head;   // bytes
     const int* table; const int* reqs; const int* end; const int* pos;
     long keys;                    // of a row of acc and out
-    int blocks, hq, hkv, group, window;
+    int blocks, hq, hkv, window;
+    Div group;   // query heads per key / value head
     PageDiv page;
     float c, cap_in, cap_out;
+};
+
+// Rows of up to NW blocks of 32 as the products need them: log-sums in units of log 2 (infinite: the row gives no weight), tokens, positions
+template <int NW>
+struct RowData {
+    float lse[NW][32];
+    int tok[NW][32], pos[NW][32];
 };
 
 template <int D, int NW, bool CAP>
 __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) {
     using GK = Geo<D, TK>;
     constexpr int NS = D / 16;
-    __shared__ __attribute__((aligned(16))) char lds[NW * GK::KTILEB];
-    __shared__ __attribute__((aligned(16))) float row_lse[NW][32];
-    __shared__ __attribute__((aligned(16))) int row_tok[NW][32], row_pos[NW][32];
+    __shared__ __attribute__((aligned(16))) char lds[NW * GK::KTILEB];   // 32 keys of each wave; behind that NW blocks of 32 queries
+    __shared__ __attribute__((aligned(16))) RowData<NW> rd;
     const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rh = blockIdx.x / p.blocks, r = rh / p.hkv, kvh = rh - r * p.hkv;
-    const int kt = (int)(blockIdx.x - (unsigned)rh * p.blocks) * NW + w;
+    const int kt0 = (int)(blockIdx.x - (unsigned)rh * p.blocks) * NW, kt = kt0 + w;
     const int cu = sload(p.reqs, 4 * r), T = sload(p.reqs, 4 * r + 1), L = sload(p.reqs, 4 * r + 2), tab = sload(p.reqs, 4 * r + 3);
     const int key = kt * TK + m;
     float sum = 0.f;
-    if (kt * TK < L && T > 0) {   // (no barrier below: each wave has its own buffers)
-        const int c = L - T, N = T * p.group;
+    if (kt0 * TK < L && T > 0) {   // (uniform over the workgroup)
+        const bool on = kt * TK < L;
+        const int c = L - T, N = T * p.group.d;
         char* const kb = lds + w * GK::KTILEB;
-        {
+        if (on) {
             const int n = 2 * kt, last16 = (L - 1) >> 4, n1 = n + 1 < last16 ? n + 1 : last16;
             const int last = L - 1 - kt * TK < TK - 1 ? L - 1 - kt * TK : TK - 1;
             const int a = p.page.of(n), b = p.page.of(n1);
             const long ia = sload(p.table, tab + a), ib = sload(p.table, tab + b);
-            const char* k0 = p.k + ia * p.k_page + (long)(n - a * p.page.pieces) * 16 * p.k_row + kvh * p.k_head;
-            const char* k1 = p.k + ib * p.k_page + (long)(n1 - b * p.page.pieces) * 16 * p.k_row + kvh * p.k_head;
+            const char* k0 = p.k + ia * p.k_page + (long)(n - a * p.page.d) * 16 * p.k_row + kvh * p.k_head;
+            const char* k1 = p.k + ib * p.k_page + (long)(n1 - b * p.page.d) * 16 * p.k_row + kvh * p.k_head;
             fetch<D, GK::NREG, GK::KRS>(k0, k1, p.k_row, last, 0, lds_addr(kb), lane);
         }
         const int u = key - c;   // this lane's key as a new token of the request (below 0: stored before)
         const bool fresh = p.end && u >= 0;
         const int uc = u < T ? u : T - 1;
         const int end_k = fresh ? p.end[cu + uc] : INT_MAX;
-        const int pos_k = fresh && p.pos ? p.pos[cu + uc] : key;
+        const int pos_k = fresh ? p.pos[cu + uc] : key;
         const int u_lo = kt * TK - c, u_hi = u_lo + TK - 1;
-        // row blocks that hold a row which may see a key of the tile
-        const int rb0 = u_lo > 0 ? (int)((long)u_lo * p.group / 32) : 0;
-        long rows = N;
-        if (p.window && !p.end) {   // (without a tree a row's position is its place) tokens from u_hi + window on are too far from the tile's keys
-            const long most = ((long)u_hi + p.window) * p.group;
-            rows = most < rows ? most : rows;
-        }
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __builtin_amdgcn_sched_barrier(0);
         bf16x8 kf[NS];
 #pragma unroll
         for (int s = 0; s < NS; s++) kf[s] = *(const bf16x8*)(kb + GK::k_off(m) + 16 * g + 32 * s);
-        for (int row0 = rb0 * 32; row0 < rows; row0 += 32) {
-            const int row = row0 + m, rc = row < N ? row : N - 1;
-            const int tok = rc / p.group, head = kvh * p.group + (rc - tok * p.group);
-            const __bf16* qp = p.q + (long)(cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
-            bf16x8 qf[NS];
-#pragma unroll
-            for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
+
+        // token and head of this lane's row of a block (rows behind the last: the last one)
+        const auto place = [&](int row, int& tok, int& head) __attribute__((always_inline)) {
+            const int rc = row < N ? row : N - 1;
+            tok = p.group.of(rc);
+            head = kvh * p.group.d + (rc - tok * p.group.d);
+        };
+        const auto note = [&](int slot, int row, int tok, int head) __attribute__((always_inline)) {   // (lanes of either half: the same values)
             const float lse = p.lse[(long)(cu + tok) * p.hq + head];
-            if (g == 0) {   // a row behind the last, or one that saw nothing, gives no weight
-                row_lse[w][m] = row < N && lse != -INFINITY ? lse * LOG2E : INFINITY;
-                row_tok[w][m] = tok;
-                row_pos[w][m] = p.window ? (p.end ? p.pos[cu + tok] : c + tok) : 0;
-            }
-            f32x16 s;
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = 0.f;
-#pragma unroll
-            for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[st], kf[st], s, 0, 0, 0);
-            const bool masked = u_hi > __builtin_amdgcn_readfirstlane(tok) || p.window;   // (lane 0's token is the block's first)
+            rd.lse[slot][m] = row < N && lse != -INFINITY ? lse * LOG2E : INFINITY;
+            rd.tok[slot][m] = tok;
+            rd.pos[slot][m] = p.window ? (p.end ? p.pos[cu + tok] : c + tok) : 0;
+        };
+        // weights of a block's rows; s: its scores, register i of which holds row 8 (i / 4) + 4 g + i % 4; first: the block's first token
+        const auto add = [&](const f32x16& s, int slot, int first) __attribute__((always_inline)) {
+            const bool masked = u_hi > first || p.window || p.end;
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++) {
-                const float4 l4 = *(const float4*)&row_lse[w][8 * i4 + 4 * g];
+                const float4 l4 = *(const float4*)&rd.lse[slot][8 * i4 + 4 * g];
                 const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
                 int tv[4] = {0, 0, 0, 0}, pv[4] = {0, 0, 0, 0};
-                if (masked || p.end) {
-                    const int4 t4 = *(const int4*)&row_tok[w][8 * i4 + 4 * g], p4 = *(const int4*)&row_pos[w][8 * i4 + 4 * g];
+                if (masked) {
+                    const int4 t4 = *(const int4*)&rd.tok[slot][8 * i4 + 4 * g], p4 = *(const int4*)&rd.pos[slot][8 * i4 + 4 * g];
                     tv[0] = t4.x; tv[1] = t4.y; tv[2] = t4.z; tv[3] = t4.w;
                     pv[0] = p4.x; pv[1] = p4.y; pv[2] = p4.z; pv[3] = p4.w;
                 }
@@ -110,11 +108,65 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
                     if (CAP) t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t * p.cap_in) + 1.0f));
                     const float x = __builtin_amdgcn_exp2f(CAP ? t - lv[j] : __builtin_fmaf(t, p.c, -lv[j]));
                     bool vis = true;
-                    if (masked || p.end) {
+                    if (masked) {
                         vis = (u <= tv[j]) & (cu + tv[j] < end_k);
                         if (p.window) vis = vis & (pv[j] - pos_k < p.window);
                     }
                     sum += vis ? x : 0.f;
+                }
+            }
+        };
+        if (N <= 32) {   // a decoding step: the few rows straight into registers, no barrier
+            if (on) {
+                int tok, head;
+                place(m, tok, head);
+                const __bf16* qp = p.q + (long)(cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
+                note(w, m, tok, head);
+                f32x16 s;
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+                for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qp + 16 * st), kf[st], s, 0, 0, 0);
+                add(s, w, 0);
+            }
+        } else {
+            // Many rows: the keys' place in LDS is free now; it takes a block of rows per wave at a time, from which all waves compute.  (Each wave
+            // loading every row from memory by itself: 4 x 16k keys, 64 tokens, 32 / 16 x 128, 154 us.)
+            const int top = kt0 * TK - c;   // first key of the workgroup as a new token: earlier rows see none of its keys
+            const int first = top > 0 ? (int)((long)top * p.group.d / 32) : 0;
+            long rows = N;
+            if (p.window && !p.end) {   // (without a tree a row's position is its place) later tokens are too far from the workgroup's keys
+                const long most = ((long)kt0 * TK + NW * TK - 1 - c + p.window) * p.group.d;
+                rows = most < rows ? most : rows;
+            }
+            const int blocks = rows > 0 ? (int)((rows + 31) / 32) : 0;
+            for (int b0 = first; b0 < blocks; b0 += NW) {
+                __syncthreads();   // every wave has its keys in registers, or is through with the blocks before
+                if (b0 + w < blocks) {
+                    const int row0 = (b0 + w) * 32;
+                    int tok, head;
+#pragma unroll
+                    for (int i = 0; i < GK::NREG; i++) {
+                        place(row0 + i + GK::NREG * (lane / GK::CPR), tok, head);
+                        dma16_lane((const char*)(p.q + (long)(cu + tok) * p.q_tok + (long)head * p.q_head) + lane % GK::CPR * 16, lds_addr(kb) + i * GK::KRS);
+                    }
+                    place(row0 + m, tok, head);
+                    note(w, row0 + m, tok, head);
+                }
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+                __syncthreads();
+                if (!on) continue;
+                const int here = blocks - b0 < NW ? blocks - b0 : NW;
+                for (int b = 0; b < here; b++) {
+                    const int last_tok = __builtin_amdgcn_readfirstlane(rd.tok[b][31]);
+                    if (last_tok < u_lo) continue;   // all of the block's tokens lie before the wave's keys
+                    const char* qb = lds + b * GK::KTILEB + GK::k_off(m) + 16 * g;
+                    f32x16 s;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+                    for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + 32 * st), kf[st], s, 0, 0, 0);
+                    add(s, b, __builtin_amdgcn_readfirstlane(rd.tok[b][0]));
                 }
             }
         }
@@ -161,7 +213,7 @@ extern "C" int spinf_paged_weights(const spinf_paged_weights_args* a, void* stre
     p.q_tok = a->q_tok; p.q_head = a->q_head;
     p.k = (const char*)a->k; p.k_page = 2 * a->k_page; p.k_row = 2 * a->k_row; p.k_head = 2 * a->k_head;
     p.table = a->table; p.reqs = a->reqs; p.end = a->end; p.pos = a->pos;
-    p.keys = a->keys; p.hq = a->hq; p.hkv = a->hkv; p.group = a->hq / a->hkv; p.window = a->window;
+    p.keys = a->keys; p.hq = a->hq; p.hkv = a->hkv; p.group = Div::by(a->hq / a->hkv); p.window = a->window;
     p.page = PageDiv::of_page(a->page);
     p.c = a->scale * LOG2E;
     p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
