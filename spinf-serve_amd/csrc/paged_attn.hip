@@ -3,7 +3,7 @@
 //
 // Mathematics.  Row = new token x query head; out = sum_s p_s v_s / sum_s p_s over the stored keys s that the row sees, p_s = exp(t_s - ref), t_s the
 // (capped) scaled score, ref a running maximum that is raised, and what was summed so far rescaled, only where a tile's maximum exceeds it by more
-// than TAU (exponents in units of log 2).  Sums, maxima and accumulators are fp32; the p_s are rounded to bf16 once, for the matrix product with V
+// than TAU (exponents in units of log 2; probabilities stay below 2^TAU).  Sums, maxima and accumulators are fp32; the p_s are rounded to bf16 once, for the matrix product with V
 // (their sum takes the unrounded ones): an error of at most 2^-8 of each term, of either sign, as the output's own rounding.
 //
 // Tiles.  32 keys; S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_32x32x16_bf16 (a lane owns one row; V^T through ds_read_b64_tr_b16), K and V
@@ -16,8 +16,8 @@
 // and paged_join_kernel where an item's keys were cut into pieces.
 //
 // Keys that a row does not see have p = 0 exactly; 0 x inf or NaN in the matrix product would still be NaN.  Nothing is spent on that in the usual
-// case: a workgroup that masked some tile and whose results are not all finite computes its rows again one by one, over the keys that each of them
-// sees (slow_row).
+// case: a workgroup that masked some tile and whose results are not all finite looks whether those tiles hold such values (rubbish), and if so computes its rows again
+// one by one, over the keys that each of them sees (slow_row).
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -140,7 +140,7 @@ struct Rows {
     static constexpr int KAHEAD = D >= 256 ? 3 : 4, VAHEAD = D >= 256 ? 3 : 4;   // fragments read ahead of the products
     bf16x8 qf[NS];
     f32x16 o[NDT];
-    float M, l;
+    float M, l, over;   // reference (0 before a row's first key), sum, score above which the reference is raised (-inf: no key so far)
     int lane, m, g, tok, qpos;
 
     __device__ __forceinline__ void load(const Params& p, const PagedItem& it, int row0) {
@@ -163,8 +163,9 @@ struct Rows {
         asm volatile("" : "+v"(qpos));
     }
     __device__ __forceinline__ void reset() {
-        M = -INFINITY;
+        M = 0.f;
         l = 0.f;
+        over = -INFINITY;
 #pragma unroll
         for (int dt = 0; dt < NDT; dt++)
 #pragma unroll
@@ -187,6 +188,8 @@ struct Rows {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // (a capped score of -inf is minus the cap and has its weight: it must not be taken for a masked one)
+    static __device__ __forceinline__ float seen(float s) { return CAP && s == -INFINITY ? -3.4e38f : s; }
     // (four keys at a time, a scheduling barrier in between: requested all at once, the keys' ends and positions would cost the tile loop its registers)
     __device__ __forceinline__ void mask(const Params& p, const PagedItem& it, int kt, const int* meta, bool tree, f32x16& s) {
         const int u0 = kt * TK - (it.L - it.T) + 4 * g;   // key 8 i4 + j of this lane is new token u0 + 8 i4 + j of the request (below 0: stored before)
@@ -197,7 +200,7 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int k = 8 * (i >> 2) + (i & 3);
-                s[i] = (k <= last) & (k > first) ? s[i] : -INFINITY;
+                s[i] = (k <= last) & (k > first) ? seen(s[i]) : -INFINITY;
             }
         } else {
             const int row = it.cu + tok;
@@ -212,48 +215,55 @@ struct Rows {
                     const bool fresh = u0 + k >= 0;
                     bool vis = (u0 + k <= tok) & (!fresh | (row < ev[j]));
                     if (p.window) vis = vis & ((fresh ? qpos - pv[j] : far - k) < sees);
-                    s[4 * i4 + j] = vis ? s[4 * i4 + j] : -INFINITY;
+                    s[4 * i4 + j] = vis ? seen(s[4 * i4 + j]) : -INFINITY;
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // scores -> probabilities; raises the reference and rescales where it has to
-    __device__ __forceinline__ void softmax(const Params& p, f32x16& s, bf16x8 (&pb)[2]) {
-        if (CAP) {   // cap * tanh(scale s / cap) in units of log 2; a masked score stays -inf
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float e = __builtin_amdgcn_exp2f(s[i] * p.cap_in);
-                const float t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f));
-                s[i] = s[i] == -INFINITY ? -INFINITY : t;
-            }
-        }
+    // scores -> probabilities.  The reference stays while no score lies more than TAU above it, which one comparison per lane with `over` (the score that
+    // far above, in the scores' own units) tells; where one does, or a row meets its first keys, it is raised and what was summed is rescaled.
+    __device__ __forceinline__ void softmax(const Params& p, f32x16& s, bool masked, bf16x8 (&pb)[2]) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
-        mx = lane32_max(mx);
-        if (!CAP) mx *= p.c;
-        const bool up = mx > M + TAU;
-        const float mn = up ? mx : M;
-        const float alpha = up ? __builtin_amdgcn_exp2f(M - mn) : 1.0f;
-        if (__builtin_amdgcn_ballot_w64(up && M != -INFINITY) != 0) {   // (rows without a key so far hold zeros)
+        if (__builtin_amdgcn_ballot_w64(mx > over) != 0) {
+            mx = lane32_max(mx);
+            const float t = CAP ? cap(p, mx) : mx * p.c;
+            const bool fresh = over == -INFINITY, up = mx > -INFINITY && (fresh || t > M + TAU);
+            const float alpha = up && !fresh ? __builtin_amdgcn_exp2f(M - t) : 1.0f;
+            if (__builtin_amdgcn_ballot_w64(up && !fresh) != 0) {   // (rows without a key so far hold zeros)
 #pragma unroll
-            for (int dt = 0; dt < NDT; dt++)
+                for (int dt = 0; dt < NDT; dt++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
+                    for (int i = 0; i < 16; i++) o[dt][i] *= alpha;
+            }
+            l *= alpha;
+            M = up ? t : M;
+            if (CAP) {   // the inverse of the cap: y / cap = tanh(x / cap); nothing lies above the cap itself
+                const float y = (M + TAU) / p.cap_out;
+                over = up ? (y < 1.f ? __builtin_amdgcn_logf((1.f + y) / (1.f - y)) / p.cap_in : INFINITY) : over;
+            } else {
+                over = up ? (M + TAU) / p.c : over;
+            }
         }
-        l *= alpha;
-        M = mn;
-        const float ms = M == -INFINITY ? 0.f : M;
         float sum = 0.f;
+        const float shift = p.cap_out - M;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float pr = __builtin_amdgcn_exp2f(CAP ? s[i] - ms : __builtin_fmaf(s[i], p.c, -ms));
+            float pr;
+            if (CAP) {   // cap_out tanh - M = (cap_out - M) - 2 cap_out / (exp(2 x) + 1)
+                pr = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * p.cap_in) + 1.0f), -2.0f * p.cap_out, shift));
+                if (masked) pr = s[i] == -INFINITY ? 0.f : pr;
+            } else {
+                pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.c, -M));
+            }
             sum += pr;
             pb[i >> 3][i & 7] = (__bf16)pr;
         }
         l += sum;
     }
+    static __device__ __forceinline__ float cap(const Params& p, float s) { return p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f)); }
     __device__ __forceinline__ void values(const char* vt_lds, const bf16x8 (&pb)[2]) {
         const int tr_a = lane & 3, tr_j = (lane >> 2) & 3, tr_mb = (lane >> 4) & 1;
         const char* vrow = vt_lds + GV::v_off(4 * g + tr_j) + 32 * tr_mb + 8 * tr_a;
@@ -294,6 +304,32 @@ __device__ __forceinline__ long row_head(const Params& p, const PagedItem& it, i
 // 1 / sum; rows that saw nothing come out as zeros
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.0f / sum; }
 __device__ __forceinline__ float log_sum(float M, float sum) { return sum == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(sum)) * LN2; }
+
+// Do partly masked tiles of an item hold values that are not finite?  (If not, a result that is not finite came from keys the row sees.)  Every wave looks at its
+// share of the tiles; groups: row groups of the item.
+template <int DV>
+__device__ bool rubbish(const Params& p, const PagedItem& it, int vcol, int w, int nw, int groups) {
+    constexpr int PIECES = DV / 8;
+    const int all = (1 << groups) - 1;
+    const int lane = threadIdx.x & 63;
+    bool found = false;
+#pragma unroll 1
+    for (Walk at(p.runs, it, w); at.more(); at.step(nw)) {
+        if ((at.bits & all) == all && !((at.bits >> 4) & all)) continue;
+        Pages pages;
+        pages.ask(p, it, at.tile());
+        const Place pl(p, p.k + it.kvh * p.k_head, p.v + it.kvh * p.v_head + vcol * 2, it.L, pages);
+#pragma unroll 1
+        for (int i = lane; i < TK * PIECES; i += 64) {
+            int r = i / PIECES;
+            r = r < pl.last ? r : pl.last;
+            const s16x8 x = *(const s16x8*)((r >= 16 ? pl.v1 : pl.v0) + (r & 15) * (unsigned long long)p.v_row + (i % PIECES) * 16);
+#pragma unroll
+            for (int k = 0; k < 8; k++) found |= (x[k] & 0x7f80) == 0x7f80;
+        }
+    }
+    return __builtin_amdgcn_ballot_w64(found) != 0;
+}
 
 // One row of an item by a whole wave, from memory: what a workgroup falls back to for all its rows where a result is not finite.  A key's values are
 // touched only where the row sees the key.
@@ -433,7 +469,7 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
                 fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
             }
             bf16x8 pb[2];
-            rows.softmax(p, s, pb);
+            rows.softmax(p, s, masked, pb);
             if (!next) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
             else if (next_tree) __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK + 2));
             else __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK));
@@ -446,13 +482,14 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
         }
     }
     const int left = it.T * p.group - it.row0;   // rows from this group's first on
-    if (__syncthreads_or(seen_mask && rows.spoilt(left))) {
+    if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, vcol, w, NW, 1))) {
         for (int j = w; j < 32 && it.row0 + j < it.T * p.group; j += NW) slow_row<D, DV, CAP>(p, it, j, vcol);
         return;
     }
 
     // ---- join the waves: every wave leaves its references and sums, then its accumulators scaled to the largest reference
     const float sum = lane32_sum(rows.l);
+    if (sum == 0.f) rows.M = -INFINITY;   // no key seen
     if (rows.g == 0) ml[w][rows.m] = make_float2(rows.M, sum);
     __syncthreads();   // (and every wave is done with its tiles)
     float top = -INFINITY, total = 0.f;
@@ -628,19 +665,20 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
         rows.scores(kb, s);
         if (masked) rows.mask(p, it, kt, (const int*)(kb + GK::KTILEB + GV::VTILEB), tree, s);
         bf16x8 pb[2];
-        rows.softmax(p, s, pb);
+        rows.softmax(p, s, masked, pb);
         rows.values(kb + GK::KTILEB, pb);
         kt = kt_next;
         bits = bits_next;
     }
     const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
     // (also the barrier behind which the tile buffers are free)
-    if (__syncthreads_or(seen_mask && rows.spoilt(left))) {
+    if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, vcol, w, 4, left + 32 * w < 128 ? (left + 32 * w + 31) / 32 : 4))) {
         for (int j = w; j < 128 && it.row0 + j < it.T * p.group; j += 4) slow_row<D, DV, CAP>(p, it, j, vcol);
         return;
     }
 
     const float sum = lane32_sum(rows.l);
+    if (sum == 0.f) rows.M = -INFINITY;   // no key seen
     const float f = it.part < 0 ? inverse(sum) : 1.f;
     const int lane = lane_now(), m = lane & 31, g = lane >> 5;
     if (it.part >= 0) {
