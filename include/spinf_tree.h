@@ -391,6 +391,7 @@ typedef struct spinf_paged_weights_args {
     const void* k; int64_t k_page, k_row, k_head;
     const int32_t* table; const int32_t* reqs; const int32_t* end; const int32_t* pos;
     int64_t n_reqs, tokens, keys;
+    int32_t max_q;                            /* most new tokens of a request */
     int32_t hq, hkv, d, page, window;
     float scale, softcap;
 } spinf_paged_weights_args;

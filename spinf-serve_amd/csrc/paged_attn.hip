@@ -405,7 +405,7 @@ __device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol) 
 
 // ------------------------------------------------------------------------------------------------ waves that share rows and divide the keys
 template <int D, int DV, int NW, bool CAP>
-__global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(const Params p) {
+__global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_wave_kernel(const Params p) {
     using R = Rows<D, DV, CAP>;
     using GK = typename R::GK;
     using GV = typename R::GV;
@@ -424,8 +424,6 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
     const PagedItem it = load_item(p.items, b);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = it.L - it.T;
-    R rows;
-    rows.load(p, it, it.row0);
     char* const kb = lds + w * TILE;
     char* const vb = kb + GK::KTILEB;
     int* const meta = (int*)(vb + GV::VTILEB);
@@ -434,20 +432,23 @@ __global__ __launch_bounds__(64 * NW, D == 512 ? 1 : 2) void paged_wave_kernel(c
     const char* const k_base = p.k + it.kvh * p.k_head;
     const char* const v_base = p.v + it.kvh * p.v_head + vcol * 2;
 
+    R rows;
     bool tree = false, seen_mask = false;
-    rows.reset();
     {
         Walk at(p.runs, it, w);
         const auto is_tree = [&](const Walk& x) { return p.end != nullptr && (x.bits & 16) && x.tile() * TK + TK > c; };
         Pages pages;
-        if (at.more()) {
+        if (at.more()) {   // (the first tile is asked for ahead of the queries: their latencies pass together)
             pages.ask(p, it, at.tile());
             const Place pl(p, k_base, v_base, it.L, pages);
+            const int lane = lane_now();
             tree = is_tree(at);
-            if (tree) fetch_meta(p, it, at.tile(), m_at, rows.lane);
-            fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
-            fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, rows.lane);
+            if (tree) fetch_meta(p, it, at.tile(), m_at, lane);
+            fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, lane);
+            fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, lane);
         }
+        rows.load(p, it, it.row0);
+        rows.reset();
         while (at.more()) {
             const int kt = at.tile();
             const bool masked = at.bits & 16;
@@ -598,7 +599,6 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
     const char* const v_base = p.v + it.kvh * p.v_head + vcol * 2;
     fill<WIN>(win, p, it, 0, k_base, v_base);
     R rows;
-    rows.load(p, it, it.row0 + 32 * w);
     const unsigned base = lds_addr(lds);
 
     // This lane's place in the regions that its wave copies: rows r + x (x < NK, NV) of the tile, which lie in one half of it
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
     const auto issue = [&](int i, int kt, int bits, int buf) __attribute__((always_inline)) {
         const unsigned at = base + buf * BUF;
         if (kt * TK + TK <= it.L) {
-            const int lane = D >= 256 ? lane_now() : rows.lane;   // (256 dims: what depends on the lane alone would be spilled, and reloaded in front of every request)
+            const int lane = D >= 256 ? lane_now() : threadIdx.x & 63;   // (256 dims: what depends on the lane alone would be spilled, and reloaded in front of every request)
             const char* ka = (const char*)win.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16);
             const char* va = (const char*)win.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16);
 #pragma unroll
@@ -631,15 +631,16 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
     };
 
     bool seen_mask = false;
-    rows.reset();
     __syncthreads();
     int kt = 0, bits = 0;
     if (it.tiles > 0) {
         const int2 t = win.tile[0];
         kt = __builtin_amdgcn_readfirstlane(t.x);
         bits = __builtin_amdgcn_readfirstlane(t.y);
-        issue(0, kt, bits, 0);
+        issue(0, kt, bits, 0);   // (ahead of the queries: their latencies pass together)
     }
+    rows.load(p, it, it.row0 + 32 * w);
+    rows.reset();
     for (int i = 0, j = 0, buf = 0; i < it.tiles; i++, buf ^= 1) {   // j: tile i's place in the window
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
         __syncthreads();                            // ... and everybody's; the other buffer is free
@@ -843,8 +844,8 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     switch (a->d) {
         case 64: return launch_cap<64, 64, 4>(p, a, s);
         case 128: return launch_cap<128, 128, 4>(p, a, s);
-        case 256: return launch_cap<256, 256, 2>(p, a, s);
-        case 512: return launch_cap<512, 256, 1>(p, a, s);
+        case 256: return launch_cap<256, 256, 4>(p, a, s);
+        case 512: return launch_cap<512, 256, 3>(p, a, s);
         default: return spinf_fail(SPINF_E_ARG, "paged_attn: head dim %d not supported (64, 128, 256, 512)", a->d);
     }
 }

@@ -39,7 +39,8 @@ struct RowData {
     int tok[NW][32], pos[NW][32];
 };
 
-template <int D, int NW, bool CAP>
+// FEW: every request's rows fit one block (a decoding step)
+template <int D, int NW, bool CAP, bool FEW>
 __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) {
     using GK = Geo<D, TK>;
     constexpr int NS = D / 16;
@@ -71,18 +72,29 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
         const int end_k = fresh ? p.end[cu + uc] : INT_MAX;
         const int pos_k = fresh ? p.pos[cu + uc] : key;
         const int u_lo = kt * TK - c, u_hi = u_lo + TK - 1;
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-        __builtin_amdgcn_sched_barrier(0);
-        bf16x8 kf[NS];
-#pragma unroll
-        for (int s = 0; s < NS; s++) kf[s] = *(const bf16x8*)(kb + GK::k_off(m) + 16 * g + 32 * s);
-
         // token and head of this lane's row of a block (rows behind the last: the last one)
         const auto place = [&](int row, int& tok, int& head) __attribute__((always_inline)) {
             const int rc = row < N ? row : N - 1;
             tok = p.group.of(rc);
             head = kvh * p.group.d + (rc - tok * p.group.d);
         };
+        // few rows go straight into registers; where no request has more, they are asked for while the keys are on their way (their registers would
+        // cost the kernel for many rows a workgroup per compute unit: 91 -> 99 us)
+        const bool few = FEW || N <= 32;
+        bf16x8 qf[FEW ? NS : 1];
+        int tok0 = 0, head0 = 0;
+        place(m, tok0, head0);
+        const __bf16* qp = p.q + (long)(cu + tok0) * p.q_tok + (long)head0 * p.q_head + 8 * g;
+        if (FEW) {
+#pragma unroll
+            for (int st = 0; st < NS; st++) qf[st] = *(const bf16x8*)(qp + 16 * st);
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 kf[NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) kf[s] = *(const bf16x8*)(kb + GK::k_off(m) + 16 * g + 32 * s);
+
         const auto note = [&](int slot, int row, int tok, int head) __attribute__((always_inline)) {   // (lanes of either half: the same values)
             const float lse = p.lse[(long)(cu + tok) * p.hq + head];
             rd.lse[slot][m] = row < N && lse != -INFINITY ? lse * LOG2E : INFINITY;
@@ -116,20 +128,17 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
                 }
             }
         };
-        if (N <= 32) {   // a decoding step: the few rows straight into registers, no barrier
+        if (few) {
             if (on) {
-                int tok, head;
-                place(m, tok, head);
-                const __bf16* qp = p.q + (long)(cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
-                note(w, m, tok, head);
+                note(w, m, tok0, head0);
                 f32x16 s;
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
-                for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qp + 16 * st), kf[st], s, 0, 0, 0);
+                for (int st = 0; st < NS; st++) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FEW ? qf[FEW ? st : 0] : *(const bf16x8*)(qp + 16 * st), kf[st], s, 0, 0, 0);
                 add(s, w, 0);
             }
-        } else {
+        } else if (!FEW) {
             // Many rows: the keys' place in LDS is free now; it takes a block of rows per wave at a time, from which all waves compute.  (Each wave
             // loading every row from memory by itself: 4 x 16k keys, 64 tokens, 32 / 16 x 128, 154 us.)
             const int top = kt0 * TK - c;   // first key of the workgroup as a new token: earlier rows see none of its keys
@@ -180,12 +189,16 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
 }
 
 template <int D, int NW>
-int launch(Params p, int64_t reqs, bool cap, hipStream_t s) {
-    const int64_t blocks = (p.keys + 32 * NW - 1) / (32 * NW), grid = blocks * p.hkv * reqs;
-    if (grid > INT32_MAX) return spinf_fail(SPINF_E_ARG, "paged_weights: %lld requests of %ld keys are too many", (long long)reqs, p.keys);
+int launch(Params p, const spinf_paged_weights_args* a, hipStream_t s) {
+    const int64_t blocks = (p.keys + 32 * NW - 1) / (32 * NW), n = blocks * p.hkv * a->n_reqs;
+    if (n > INT32_MAX) return spinf_fail(SPINF_E_ARG, "paged_weights: %lld requests of %ld keys are too many", (long long)a->n_reqs, p.keys);
     p.blocks = (int)blocks;
-    if (cap) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
-    else hipLaunchKernelGGL((paged_weights_kernel<D, NW, false>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
+    const dim3 grid((unsigned)n), threads(64 * NW);
+    const bool cap = a->softcap > 0.f, few = (int64_t)a->max_q * p.group.d <= 32;
+    if (cap && few) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true, true>), grid, threads, 0, s, p);
+    else if (cap) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true, false>), grid, threads, 0, s, p);
+    else if (few) hipLaunchKernelGGL((paged_weights_kernel<D, NW, false, true>), grid, threads, 0, s, p);
+    else hipLaunchKernelGGL((paged_weights_kernel<D, NW, false, false>), grid, threads, 0, s, p);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "paged_weights: launch: %s", hipGetErrorString(e));
 }
@@ -198,6 +211,7 @@ extern "C" int spinf_paged_weights(const spinf_paged_weights_args* a, void* stre
     if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv) return spinf_fail(SPINF_E_ARG, "paged_weights: %d query heads do not group over %d key / value heads", a->hq, a->hkv);
     if (a->d != 64 && a->d != 128 && a->d != 256 && a->d != 512) return spinf_fail(SPINF_E_ARG, "paged_weights: head dim %d not supported (64, 128, 256, 512)", a->d);
     if (a->page < 16 || a->page % 16 || a->page > (1 << 20)) return spinf_fail(SPINF_E_ARG, "paged_weights: pages of %d keys (a multiple of 16)", a->page);
+    if (a->max_q < 0 || a->max_q > a->tokens) return spinf_fail(SPINF_E_ARG, "paged_weights: %d new tokens of a request of %lld", a->max_q, (long long)a->tokens);
     if (a->window < 0) return spinf_fail(SPINF_E_ARG, "paged_weights: window %d", a->window);
     if (!(a->scale > 0.f) || !(a->scale < INFINITY) || !(a->softcap >= 0.f) || !(a->softcap < INFINITY))
         return spinf_fail(SPINF_E_ARG, "paged_weights: scale %g must be positive and finite, softcap %g not negative", (double)a->scale, (double)a->softcap);
@@ -219,11 +233,10 @@ extern "C" int spinf_paged_weights(const spinf_paged_weights_args* a, void* stre
     p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
     p.cap_out = a->softcap * LOG2E;
     hipStream_t s = (hipStream_t)stream;
-    const bool cap = a->softcap > 0.f;
     switch (a->d) {
-        case 64: return launch<64, 4>(p, a->n_reqs, cap, s);
-        case 128: return launch<128, 4>(p, a->n_reqs, cap, s);
-        case 256: return launch<256, 4>(p, a->n_reqs, cap, s);
-        default: return launch<512, 2>(p, a->n_reqs, cap, s);
+        case 64: return launch<64, 4>(p, a, s);
+        case 128: return launch<128, 4>(p, a, s);
+        case 256: return launch<256, 4>(p, a, s);
+        default: return launch<512, 2>(p, a, s);
     }
 }

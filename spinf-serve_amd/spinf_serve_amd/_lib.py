@@ -128,7 +128,7 @@ class PagedWeightsArgs(C.Structure):
         ("q_tok", C.c_int64), ("q_head", C.c_int64),
         ("k", C.c_void_p), ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
         ("table", C.c_void_p), ("reqs", C.c_void_p), ("end", C.c_void_p), ("pos", C.c_void_p),
-        ("n_reqs", C.c_int64), ("tokens", C.c_int64), ("keys", C.c_int64),
+        ("n_reqs", C.c_int64), ("tokens", C.c_int64), ("keys", C.c_int64), ("max_q", C.c_int32),
         ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("page", C.c_int32), ("window", C.c_int32),
         ("scale", C.c_float), ("softcap", C.c_float),
     ]

@@ -377,12 +377,12 @@ def paged_attn(q, cache: PagedCache, batch: PagedBatch, scale=None, window=None,
 
 
 def _paged_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, acc: Optional[torch.Tensor], table: torch.Tensor, reqs: torch.Tensor,
-                   end: Optional[torch.Tensor], pos: Optional[torch.Tensor], page: int, max_page: int, tokens: int, longest: int, n_reqs: int, keys: int, scale: float,
+                   end: Optional[torch.Tensor], pos: Optional[torch.Tensor], page: int, max_page: int, tokens: int, max_q: int, longest: int, n_reqs: int, keys: int, scale: float,
                    window: int, softcap: float) -> torch.Tensor:
-    return _weights_run(_weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap), q, k, lse, acc)
+    return _weights_run(_weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, max_q, longest, n_reqs, keys, scale, window, softcap), q, k, lse, acc)
 
 
-def _weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap):
+def _weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, max_q, longest, n_reqs, keys, scale, window, softcap):
     _check_call(q, k, k, tokens, page, max_page, "paged_weights")
     _lib.same_device(q.device, k, lse, acc, table, reqs, end, pos)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
@@ -396,7 +396,7 @@ def _weights_block(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens
     a.table, a.reqs = table.data_ptr(), reqs.data_ptr()
     if end is not None:
         a.end, a.pos = end.data_ptr(), pos.data_ptr()
-    a.n_reqs, a.tokens, a.keys = n_reqs, tokens, keys
+    a.n_reqs, a.tokens, a.max_q, a.keys = n_reqs, tokens, max_q, keys
     a.hq, a.hkv, a.d, a.page, a.window, a.scale, a.softcap = q.shape[1], k.shape[2], q.shape[2], page, window, scale, softcap
     return a
 
@@ -414,7 +414,7 @@ _weights_op = torch.library.custom_op("spinf::paged_weights", _paged_weights, mu
 
 
 @_weights_op.register_fake
-def _(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, longest, n_reqs, keys, scale, window, softcap):
+def _(q, k, lse, acc, table, reqs, end, pos, page, max_page, tokens, max_q, longest, n_reqs, keys, scale, window, softcap):
     return torch.empty((n_reqs, k.shape[2], keys), dtype=torch.float32, device=q.device)
 
 
@@ -439,7 +439,7 @@ def paged_weights(q, cache: PagedCache, batch: PagedBatch, lse, scale=None, wind
     keys = longest if acc is None else acc.shape[-1]
     _check_call(q, k, k, batch.tokens, batch.page, batch.max_page, "paged_weights")
     table, end, pos = batch.device_data()
-    args = (q, k, lse, acc, table, batch.device_requests(), end, pos, batch.page, batch.max_page, batch.tokens, longest, len(batch.kv_lens), int(keys), sc, w, float(softcap) if softcap else 0.0)
+    args = (q, k, lse, acc, table, batch.device_requests(), end, pos, batch.page, batch.max_page, batch.tokens, int(batch.q_lens.max(initial=0)), longest, len(batch.kv_lens), int(keys), sc, w, float(softcap) if softcap else 0.0)
     if not eager:
         return _weights_op(*args)
     a = _weights_block(*args)

@@ -675,7 +675,7 @@ def test_streams_compiled_programs_and_recorded_graphs(dev):
         assert torch.equal(sa.paged_attn(q, cache, fresh), want)
         assert torch.equal(sa.paged_weights(q, cache, fresh, lse, acc=acc), weight)
     torch.cuda.synchronize()
-    torch.library.opcheck(torch.ops.spinf.paged_weights.default, (q, cache.k, lse, acc, *[b.device_data()[0], b.device_requests(), None, None], 64, b.max_page, b.tokens, 900, 2, 900, 0.1, 0, 0.0),
+    torch.library.opcheck(torch.ops.spinf.paged_weights.default, (q, cache.k, lse, acc, *[b.device_data()[0], b.device_requests(), None, None], 64, b.max_page, b.tokens, 70, 900, 2, 900, 0.1, 0, 0.0),
                           test_utils=("test_schema", "test_faketensor"))
     lists, counts, at = b.plan(8, 2, 128, 0)
     torch.library.opcheck(torch.ops.spinf.paged_attn.default, (q, cache.k, cache.v, b.device_data()[0], None, None, lists, counts, at, 64, b.max_page, b.tokens, 0.1, 0, 0.0, True),
