@@ -137,8 +137,13 @@ class PagedBatch:
         if shared.device.type == "cuda":
             shared.reach(_lib.raw_stream(shared.device.index))
 
+    def _not_recording(self):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a batch's first call of a kind copies its lists to the device, which cannot be recorded: make that call before the capture")
+
     def _upload(self, *arrays):
         """int32 arrays back to back, each 16-byte aligned, in one copy -> device tensor, where each begins"""
+        self._not_recording()
         at, n = [], 0
         for a in arrays:
             at.append(n)
@@ -232,6 +237,7 @@ class PagedBatch:
         self._calls[key] = bytes(args), device, tuple(x for x in shared if x is not None)
 
     def _compile(self, hq, hkv, d, window, variant):
+        self._not_recording()
         lib = _lib.load_library()
         a = _lib.PagedPlanArgs()
         a.q_lens, a.kv_lens, a.reqs = self.q_lens.ctypes.data, self.kv_lens.ctypes.data, len(self.kv_lens)

@@ -691,3 +691,81 @@ def test_streams_compiled_programs_and_recorded_graphs(dev):
         e, el = sa.paged_attn(q, cache, b, return_lse=True)
         assert torch.equal(out, e) and torch.equal(l2, el) and torch.equal(w2, sa.paged_weights(q, cache, b, el, acc=acc))
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_a_session_equals_reading_anew(dev):
+    """examples/paged_session.py: documents, later questions and tokens over the cache against tree_attn over the whole stream"""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_session.py")
+    spec = importlib.util.spec_from_file_location("paged_session", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    off = module.main(dev)
+    # values of unit scale (at most about 5): two computations' probabilities and outputs, each rounded to bf16 once
+    assert all(off[x] <= 4 * 2.0**-8 * 5 for x in ("documents", "questions", "steps")), off
+    assert off["weights"] <= 1e-4, off
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(dev):
+    """pages whose bytes begin beyond 2^32, read, written and moved"""
+    page, hkv, d = 64, 8, 256
+    pages = (5 << 30) // (page * hkv * d * 2)
+    cache = sa.PagedCache.empty(pages, page, hkv, d, dev)
+    small = sa.PagedCache.empty(12, page, hkv, d, dev)
+    g = torch.Generator().manual_seed(3)
+    for a, b in ((small.k, cache.k), (small.v, cache.v)):
+        a.copy_(torch.randn(a.shape, generator=g).to(BF16))
+        b[-12:] = a
+    far = [pages - 12 + i for i in range(12)]
+    q = torch.randn((70, 16, d), generator=g).to(BF16).to(dev)
+    make = lambda ids: sa.PagedBatch.build([1, 69], [250, 130], [ids[:4], ids[4:7]], page, dev)  # noqa: E731
+    near, there = make(list(range(12))), make(far)
+    want, lse = sa.paged_attn(q, small, near, return_lse=True)
+    assert torch.equal(sa.paged_attn(q, cache, there), want)
+    w = sa.paged_weights(q, small, near, lse)
+    assert torch.equal(sa.paged_weights(q, cache, there, lse), w)
+    outs = []
+    for c, b, ids in ((small, near, list(range(12))), (cache, there, far)):
+        into = sa.PagedBatch.build([0, 0], [100, 100], [ids[7:9], ids[9:11]], page, dev)
+        outs.append((sa.cache_evict(c, b, into, w, 100, 4, 8), c.k[ids].clone(), c.v[ids].clone()))
+    assert all(torch.equal(x, y) for x, y in zip((*outs[0][0], *outs[0][1:]), (*outs[1][0], *outs[1][1:])))
+    ang = torch.rand((3, 32), generator=g).to(dev)
+    k, v = (torch.randn((3, hkv, d), generator=g).to(BF16).to(dev) for _ in range(2))
+    for c, ids in ((small, list(range(12))), (cache, far)):
+        slots = torch.tensor([ids[11] * page, ids[11] * page + 63, ids[0] * page + 5], device=dev)
+        sa.qk_norm_rope_put(q[:3], k, v, None, None, ang.cos(), ang.sin(), 1e-6, c, slots)
+    assert torch.equal(small.k, cache.k[-12:]) and torch.equal(small.v, cache.v[-12:])
+
+
+@pytest.mark.gpu
+def test_calls_refuse_what_the_kernels_do_not_take(dev):
+    b, pages = make_batch([2], [20], 16, dev)
+    cache, q = fill(b, pages, (4, 2, 64), 0, dev)
+    for bad in (dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(softcap=-2.0), dict(window=-1)):
+        with pytest.raises(ValueError):
+            sa.paged_attn(q, cache, b, **bad)
+        with pytest.raises(ValueError):
+            sa.paged_weights(q, cache, b, torch.zeros((2, 4), device=dev), **bad)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        sa.paged_attn(q.cpu(), cache, b)
+    odd = torch.zeros((2, 4, 65), dtype=BF16, device=dev)[..., 1:]
+    with pytest.raises(ValueError, match="aligned"):
+        sa.paged_attn(odd, cache, b)
+    for lse in (torch.zeros((2, 4), device=dev).double(), torch.zeros((2, 3), device=dev), torch.zeros((4, 2), device=dev).t(), torch.zeros((2, 4))):
+        with pytest.raises(ValueError):
+            sa.paged_weights(q, cache, b, lse)
+    for acc in (torch.zeros((1, 2, 19), device=dev), torch.zeros((1, 4, 20), device=dev), torch.zeros((1, 2, 20), device=dev).double()):
+        with pytest.raises(ValueError):
+            sa.paged_weights(q, cache, b, torch.zeros((2, 4), device=dev), acc=acc)
+    fresh = pickle.loads(pickle.dumps(b))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="recorded"):
+        with torch.cuda.graph(graph):
+            sa.paged_attn(q, cache, fresh)
+    torch.cuda.synchronize()
+    assert torch.equal(sa.paged_attn(q, cache, fresh), sa.paged_attn(q, cache, b))
