@@ -11,7 +11,6 @@
 #include <cstdint>
 #include <exception>
 #include <new>
-#include <numeric>
 #include <vector>
 
 #include "spinf_tree.h"
@@ -156,7 +155,7 @@ class Builder {
         const bool by_wave = a_->variant ? a_->variant == 1 : N <= GROUP || blocks <= PAGED_WAVE_MAX;
         const int groups = by_wave ? 1 : BLOCK_GROUPS, rows = groups * GROUP;
         const int64_t row_items = (N + rows - 1) / rows * a_->hkv * halves;
-        std::vector<Run> runs;
+        std::vector<Run>& runs = runs_;
         for (int64_t row0 = 0; row0 < N; row0 += rows) {
             list(r, (int)row0, groups, runs);
             int64_t tiles = 0;
@@ -168,22 +167,20 @@ class Builder {
             const int64_t per = std::max(least, (tiles + want - 1) / want);
             const int64_t nsplit = std::max<int64_t>(1, (tiles + per - 1) / per);
             const int64_t here = std::min<int64_t>(rows, N - row0);
-            std::vector<std::pair<int32_t, int32_t>> cut;   // (first run, runs) of each piece
-            std::vector<int32_t> cut_tiles;
+            cut_.clear();
             size_t at = 0;
             int64_t off = 0;
             for (int64_t s = 0; s < nsplit; s++) {
                 int64_t left = tiles * (s + 1) / nsplit - tiles * s / nsplit;
-                cut_tiles.push_back((int32_t)left);
-                const int32_t first = (int32_t)p_->runs.size();
+                const int32_t here = (int32_t)left, first = (int32_t)p_->runs.size();
                 while (left > 0) {
                     const int64_t take = std::min<int64_t>(left, runs[at].count - off);
-                    p_->runs.push_back({(int32_t)(runs[at].kt + off), (int32_t)take, runs[at].bits, cut_tiles.back() - (int32_t)left});
+                    p_->runs.push_back({(int32_t)(runs[at].kt + off), (int32_t)take, runs[at].bits, here - (int32_t)left});
                     left -= take;
                     off += take;
                     if (off == runs[at].count) { at++; off = 0; }
                 }
-                cut.push_back({first, (int32_t)p_->runs.size() - first});
+                cut_.push_back({first, (int32_t)p_->runs.size() - first, here});
             }
             for (int h = 0; h < a_->hkv; h++) {
                 const int64_t part = p_->part_rows;
@@ -194,7 +191,7 @@ class Builder {
                 }
                 for (int64_t s = 0; s < nsplit; s++)
                     (by_wave ? p_->wave : p_->block)
-                        .push_back({r.cu, r.T, r.L, r.tab, h, (int32_t)row0, cut[s].first, cut[s].second, cut_tiles[s], nsplit > 1 ? (int32_t)(part + s * rows) : -1, index,
+                        .push_back({r.cu, r.T, r.L, r.tab, h, (int32_t)row0, cut_[s].first, cut_[s].runs, cut_[s].tiles, nsplit > 1 ? (int32_t)(part + s * rows) : -1, index,
                                     (int32_t)nsplit});
             }
         }
@@ -202,29 +199,42 @@ class Builder {
 
     // Launch order.  Workgroup i runs on XCD i % 8: the items of one (request, key / value head) go to one XCD, whose L2 then holds what they
     // share, unless there are too few of these sets to fill eight; inside a set the longest items come first, and so do the heaviest sets.
-    static void order(std::vector<Item>& items) {
+    void order(std::vector<Item>& items) const {
         if (items.empty()) return;
-        std::vector<int32_t> idx(items.size());
-        std::iota(idx.begin(), idx.end(), 0);
-        std::stable_sort(idx.begin(), idx.end(), [&](int32_t x, int32_t y) {
-            const Item &a = items[x], &b = items[y];
-            return a.req != b.req ? a.req < b.req : a.kvh != b.kvh ? a.kvh < b.kvh : a.tiles > b.tiles;
-        });
+        const int hkv = a_->hkv;
+        // items by set (they were made request by request, so a set lies inside its request's stretch), longest first
+        std::vector<int32_t> idx(items.size()), at(hkv + 1);
+        int64_t total = 0;
+        for (size_t i = 0; i < items.size();) {
+            size_t j = i;
+            std::fill(at.begin(), at.end(), 0);
+            for (; j < items.size() && items[j].req == items[i].req; j++) at[items[j].kvh + 1]++;
+            for (int h = 0; h < hkv; h++) at[h + 1] += at[h];
+            for (size_t k = i; k < j; k++) {
+                idx[i + at[items[k].kvh]++] = (int32_t)k;
+                total += weight(items[k]);
+            }
+            for (int h = 0; h < hkv; h++) {   // (at[h] is the end of head h's items now)
+                const auto first = idx.begin() + i + (h ? at[h - 1] : 0), last = idx.begin() + i + at[h];
+                const auto longer = [&](int32_t x, int32_t y) { return items[x].tiles > items[y].tiles; };
+                if (!std::is_sorted(first, last, longer)) std::stable_sort(first, last, longer);
+            }
+            i = j;
+        }
         struct Set { size_t at, n; int64_t weight; };
         std::vector<Set> sets;
-        auto weight = [&](int32_t i) { return (int64_t)items[i].tiles + 4; };
-        int64_t total = 0;
-        for (int32_t i : idx) total += weight(i);
         for (size_t i = 0; i < idx.size();) {
             size_t j = i;
             int64_t w = 0;
+            const Item& lead = items[idx[i]];
             // (a set heavier than a sixteenth of the call is dealt out in pieces)
-            while (j < idx.size() && items[idx[j]].req == items[idx[i]].req && items[idx[j]].kvh == items[idx[i]].kvh && (j == i || w * 16 < total)) w += weight(idx[j++]);
+            while (j < idx.size() && items[idx[j]].req == lead.req && items[idx[j]].kvh == lead.kvh && (j == i || w * 16 < total)) w += weight(items[idx[j++]]);
             sets.push_back({i, j - i, w});
             i = j;
         }
         std::stable_sort(sets.begin(), sets.end(), [](const Set& x, const Set& y) { return x.weight > y.weight; });
         std::vector<int32_t> lists[XCDS];
+        for (auto& l : lists) l.reserve(items.size() / 4);
         int64_t load[XCDS] = {};
         for (const Set& s : sets) {
             const int x = (int)(std::min_element(load, load + XCDS) - load);
@@ -240,9 +250,14 @@ class Builder {
                 if (i < l.size()) out.push_back(items[l[i]]);   // (a list that has run out shifts the others by one: placement, not results)
         items.swap(out);
     }
+    static int64_t weight(const Item& x) { return (int64_t)x.tiles + 4; }
+
+    struct Piece { int32_t first, runs, tiles; };
 
     const spinf_paged_plan_args* a_;
     spinf_pagedplan* p_;
+    std::vector<Piece> cut_;   // of the row block in hand
+    std::vector<Run> runs_;
     const int group_, window_;
 };
 

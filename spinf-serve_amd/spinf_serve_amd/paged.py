@@ -103,13 +103,7 @@ class PagedBatch:
         if len(q_lens) != len(kv_lens) or len(tables) != len(kv_lens):
             raise ValueError(f"{len(q_lens)} q_lens, {len(kv_lens)} kv_lens and {len(tables)} tables")
         need = -(-kv_lens.astype(np.int64) // page)
-        parts = []
-        for r, n in enumerate(need):
-            t = np.asarray(tables[r])
-            if t.ndim != 1 or len(t) < n or (n and t.dtype.kind not in "iu"):
-                raise ValueError(f"request {r}: {kv_lens[r]} stored keys need {n} pages of {page}, its table has {t.shape}")
-            parts.append(t[:n])
-        table = np.concatenate(parts).astype(np.int64) if parts else np.zeros(0, np.int64)
+        table = cls._pages(tables, need, kv_lens, page)
         if len(table) and (table.min() < 0 or table.max() >= 1 << 31):
             raise ValueError("page numbers must lie in 0 .. 2^31 - 1")
         if (end is None) != (pos is None):
@@ -127,6 +121,20 @@ class PagedBatch:
                     raise ValueError("end must lie in 0 .. tokens, pos in 0 .. the token's place among the stored keys")
             end, pos = end.astype(np.int32), pos.astype(np.int32)
         return cls(q_lens, kv_lens, table.astype(np.int32), need, page, torch.device(device), end, pos)
+
+    @staticmethod
+    def _pages(tables, need, kv_lens, page):
+        """the requests' pages back to back"""
+        if isinstance(tables, np.ndarray) and tables.ndim == 2 and tables.dtype.kind in "iu" and (not len(need) or need.max() <= tables.shape[1]):
+            return tables[np.arange(tables.shape[1]) < need[:, None]].astype(np.int64)
+        parts = []
+        for r, n in enumerate(need.tolist()):
+            t = tables[r]
+            t = np.array(t[:n]) if type(t) is list else np.asarray(t)[:n]
+            if t.shape != (n,) or (n and t.dtype.kind not in "iu"):
+                raise ValueError(f"request {r}: {kv_lens[r]} stored keys need {n} pages of {page}, whole numbers; its table gives {t.shape} of {t.dtype}")
+            parts.append(t)
+        return np.concatenate(parts).astype(np.int64) if parts else np.zeros(0, np.int64)
 
     def __reduce__(self):
         """copied and saved as what it is built from"""
@@ -455,17 +463,28 @@ def paged_weights(q, cache: PagedCache, batch: PagedBatch, lse, scale=None, wind
 
 def _cache_evict(k: torch.Tensor, v: torch.Tensor, acc: torch.Tensor, table: torch.Tensor, reqs: torch.Tensor, new_table: torch.Tensor, new_reqs: torch.Tensor,
                  page: int, keep: int, sink: int, recent: int) -> tuple[torch.Tensor, torch.Tensor]:
-    device = acc.device
-    _lib.same_device(device, k, v, table, new_table, reqs, new_reqs)
-    shape = (*acc.shape[:2], keep)
-    kept, new_acc = torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
+    _lib.same_device(acc.device, k, v, table, new_table, reqs, new_reqs)
+    return _evict_run(_evict_block(k, v, acc, table, reqs, page, keep, sink, recent), k, v, acc, new_table, new_reqs)
+
+
+def _evict_block(k, v, acc, table, reqs, page, keep, sink, recent):
     R, hkv, keys = acc.shape
-    if not (R and keep and keys):   # no stored key at all
+    a = _lib.EvictArgs()
+    a.keys, a.n_reqs, a.hkv, a.d, a.page, a.keep, a.sink, a.recent = keys, R, hkv, k.shape[3], page, keep, sink, recent
+    a.reqs, a.table = reqs.data_ptr(), table.data_ptr()
+    a.k_page, a.k_row, a.k_head = k.stride()[:3]
+    a.v_page, a.v_row, a.v_head = v.stride()[:3]
+    return a
+
+
+def _evict_run(a, k, v, acc, new_table, new_reqs, stream=None):
+    device, shape = acc.device, (a.n_reqs, a.hkv, a.keep)
+    kept, new_acc = torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
+    if not (a.n_reqs and a.keep and a.keys):   # no stored key at all
         return kept.fill_(-1), new_acc.zero_()
-    ks, vs = k.stride(), v.stride()
-    a = _lib.EvictArgs(acc.data_ptr(), keys, reqs.data_ptr(), new_reqs.data_ptr(), table.data_ptr(), new_table.data_ptr(), kept.data_ptr(), new_acc.data_ptr(), k.data_ptr(),
-                       v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], R, hkv, k.shape[3], page, keep, sink, recent)
-    _lib.launch(_lib.load_library().spinf_cache_evict, a, device, "cache_evict")
+    a.acc, a.k, a.v, a.kept, a.new_acc = acc.data_ptr(), k.data_ptr(), v.data_ptr(), kept.data_ptr(), new_acc.data_ptr()
+    a.new_table, a.new_reqs = new_table.data_ptr(), new_reqs.data_ptr()
+    _lib.launch(_lib.load_library().spinf_cache_evict, a, device, "cache_evict", stream)
     return kept, new_acc
 
 
@@ -485,12 +504,25 @@ def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, kee
     as they are, since other requests may share them; into's pages must be none of batch's.  Rotated keys keep their positions: a layer with a window, which goes by places,
     is not trimmed this way.
     -> kept [requests, hkv, keep] int32 (the places that stayed, ascending, -1 behind them) and their acc (0 behind them): the next paged_weights' acc"""
-    keep, sink, recent = int(keep), int(sink), int(recent)
-    if sink < 0 or recent < 0 or sink + recent > keep:
-        raise ValueError(f"cache_evict: keep {keep}, of these the first {sink} and the last {recent}")
     k, v = cache.k, cache.v
     pages, page, hkv, _ = k.shape
     R = len(batch.kv_lens)
+    eager = _lib.eager(acc, k, v)
+    if eager:
+        key = ("evict", acc.shape, acc.stride(), acc.dtype, k.shape, k.stride(), v.stride(), keep, sink, recent)
+        got = batch._calls.get(key)
+        if got is not None and acc.device == got[1] == k.device == v.device and into.page == page and into.max_page < pages:
+            batch.check_move(into, keep)
+            new = into._device()
+            if new[0].device == got[1]:
+                stream = _lib.raw_stream(got[1].index)
+                for shared in got[2]:
+                    if stream not in shared.streams:
+                        shared.reach(stream)
+                return _evict_run(_lib.EvictArgs.from_buffer_copy(got[0]), k, v, acc, new[1], new[0], stream)
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError(f"cache_evict: keep {keep}, of these the first {sink} and the last {recent}")
     if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[0] != R or acc.shape[1] != hkv or not acc.is_contiguous():
         raise ValueError(f"cache_evict: acc must be contiguous fp32 [{R}, {hkv}, keys]")
     if acc.shape[2] < batch.longest:
@@ -503,4 +535,9 @@ def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, kee
     if not acc.is_cuda:
         raise RuntimeError("cache_evict runs on ROCm device tensors only (no CPU path)")
     old, new = batch._device(), into._device()
-    return (_cache_evict if _lib.eager(acc, k, v) else _evict_op)(k, v, acc, old[1], old[0], new[1], new[0], page, keep, sink, recent)
+    if not eager:
+        return _evict_op(k, v, acc, old[1], old[0], new[1], new[0], page, keep, sink, recent)
+    _lib.same_device(acc.device, k, v, *old[:2], *new[:2])
+    a = _evict_block(k, v, acc, old[1], old[0], page, keep, sink, recent)
+    batch.keep(key, a, acc.device)
+    return _evict_run(a, k, v, acc, new[1], new[0])
