@@ -78,21 +78,32 @@ def _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, what):
 _SEEN: dict = {}
 
 
-def _meta(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype)
-
-
 def _known(key, device, tensors):
-    """the block kept for this key, if the tensors lie on `device` and are aligned as the kernel wants them"""
+    """the block kept for this key with the tensors' addresses, if they lie on `device` and are aligned as the kernel wants them"""
     got = _SEEN.get(key)
     if got is None or device.type != "cuda":
         return None
+    at, bits = [], 0
     for t in tensors:
-        if t is not None and (t.device != device or t.data_ptr() % 16):
+        if t is None:
+            at.append(None)
+            continue
+        if t.device != device:
             return None   # (the checks say what is wrong)
+        x = t.data_ptr()
+        bits |= x
+        at.append(x)
+    if bits % 16:
+        return None
     a = _lib.RopeArgs.from_buffer_copy(got)
-    a.q, a.k, a.v, a.wq, a.wk, a.cos, a.sin = (None if t is None else t.data_ptr() for t in tensors[:7])
+    a.q, a.k, a.v, a.wq, a.wk, a.cos, a.sin = at[:7]
     return a
+
+
+def _table(wq, wk, cos, sin, pos):
+    """what the checks look at of the weights, the tables and the positions"""
+    return (None if wq is None else (wq.shape, wq.stride(), wq.dtype), None if wk is None else (wk.shape, wk.stride(), wk.dtype), cos.shape, cos.stride(), cos.dtype,
+            sin.shape, sin.stride(), sin.dtype, None if pos is None else (pos.shape, pos.stride(), pos.dtype))
 
 
 def _note(key, a):
@@ -104,7 +115,7 @@ def _note(key, a):
 def _rope(q: torch.Tensor, k: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
           pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool) -> tuple[torch.Tensor, torch.Tensor]:
     device = q.device
-    key = (_meta(q), _meta(k), _meta(wq), _meta(wk), _meta(cos), _meta(sin), _meta(pos), eps, neighbours, plus_one)
+    key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, _table(wq, wk, cos, sin, pos), eps, neighbours, plus_one)
     a = _known(key, device, (q, k, None, wq, wk, cos, sin))
     if a is None or (pos is not None and pos.device != device):
         a = _rope_args(q, k, None, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope")
@@ -136,7 +147,8 @@ def qk_norm_rope(q, k, wq, wk, cos, sin, eps, pos=None, neighbours=False, plus_o
 def _put(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
          ck: torch.Tensor, cv: torch.Tensor, slots: torch.Tensor, pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool, v_norm: bool) -> torch.Tensor:
     device = q.device
-    key = (_meta(q), _meta(k), _meta(v), _meta(wq), _meta(wk), _meta(cos), _meta(sin), _meta(pos), _meta(ck), cv.stride(), _meta(slots), eps, neighbours, plus_one, v_norm)
+    key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, ck.shape, ck.stride(), cv.stride(), slots.shape, slots.stride(), slots.dtype,
+           _table(wq, wk, cos, sin, pos), eps, neighbours, plus_one, v_norm)
     a = _known(key, device, (q, k, v, wq, wk, cos, sin, ck, cv))
     if a is None or (pos is not None and pos.device != device) or slots.device != device:
         a = _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope_put")

@@ -644,6 +644,15 @@ def test_norm_and_rotation_refuse_tensors_before_any_launch(dev):
     q, k, w, c = (t.to(dev) for t in (torch.zeros((3, 4, 64), dtype=BF16), torch.zeros((3, 2, 64), dtype=BF16), torch.zeros(64), torch.zeros((3, 16))))
     good = dict(q=q, k=k, wq=w, wk=w, cos=c, sin=c, eps=1e-6, pos=None)
     sa.qk_norm_rope(**good)
+    with pytest.raises(RuntimeError, match="ROCm"):   # (the same call elsewhere is not a known one)
+        sa.qk_norm_rope(**{n: t.cpu() if isinstance(t, torch.Tensor) else t for n, t in good.items()})
+    for one in ("q", "k", "wq", "wk", "cos", "sin"):
+        with pytest.raises((RuntimeError, ValueError)):
+            sa.qk_norm_rope(**{**good, one: good[one].cpu()})
+    for one in ("q", "k"):   # the same strides, another alignment
+        t = torch.zeros(good[one].numel() + 8, dtype=BF16, device=dev)[1 : 1 + good[one].numel()].view(good[one].shape)
+        with pytest.raises(ValueError, match="aligned"):
+            sa.qk_norm_rope(**{**good, one: t})
     long = torch.zeros((3, 40), device=dev)
     for bad in (dict(q=q.float()), dict(q=q[:2]), dict(k=k[..., ::2]), dict(wq=w[:32]), dict(wq=w.half()), dict(wq=w.to(BF16)), dict(cos=c.double()), dict(sin=c[:, :8]),
                 dict(cos=c[:2], sin=c[:2]), dict(cos=long, sin=long), dict(cos=c[:, :4], sin=c[:, :4]), dict(pos=torch.zeros(2, dtype=torch.int64, device=dev)),
