@@ -11,9 +11,9 @@ struct PagedRun { int32_t kt, count; uint32_t bits; int32_t start; };
 // rows row0 .. of key / value head kvh of the request whose new tokens are rows cu .. cu + T - 1 of the call and whose L stored keys lie in the pages
 // tab .. of the page list; runs first .. first + runs - 1 (`tiles` tiles); part: first partial row, -1: the only piece
 struct PagedItem { int32_t cu, T, L, tab, kvh, row0, first, runs, tiles, part, req, nsplit; };
-constexpr int PAGED_JOIN = 8;             // most rows of a join
-// up to PAGED_JOIN rows whose nsplit pieces (partial rows part + s * stride + j) are to be joined
-struct PagedJoin { int32_t cu, kvh, row0, rows, part, nsplit, stride, pad; };
+constexpr int PAGED_JOIN = 16;            // groups of 16 lanes that join rows: up to PAGED_JOIN / share rows, `share` groups to each
+// rows row0 .. row0 + rows - 1, whose nsplit pieces (partial rows part + s * stride + j) are to be joined
+struct PagedJoin { int32_t cu, kvh, row0, rows, part, nsplit, stride, share; };
 static_assert(sizeof(PagedRun) == 16 && sizeof(PagedItem) == 48 && sizeof(PagedJoin) == 32, "read by the kernels as 16-byte pieces");
 
 constexpr int PAGED_PLACES = 512;        // workgroups of either kernel that run at a time (two per compute unit)

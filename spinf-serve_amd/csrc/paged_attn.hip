@@ -717,59 +717,81 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
     }
 }
 
-// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per row and 64 head dims: 16 lanes per piece, 16 pieces at a time, added up
-// in one fixed order (a wave per row went through a long document's 241 pieces one after the other: 16 rows of 512 dims 73 us).
+// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per join and 64 head dims; 16 lanes hold a piece, `share` such groups
+// take a row's pieces in turn, each with a reference of its own, and are added up in one fixed order.  Rows of few pieces share a workgroup, a long document's row has
+// one for itself.  Bound by the pieces' bytes where rows are many, by one round trip to memory where they are few.
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
     constexpr int SLICES = D / 64, GROUPS = 16;
     __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
-    __shared__ float total_sum[GROUPS];
-    const int slice = blockIdx.x % SLICES, i = blockIdx.x / SLICES, j = i % PAGED_JOIN;
-    const int* jp = (const int*)(p.joins + i / PAGED_JOIN);
-    if (j >= sload(jp, 3)) return;
-    const int cu = sload(jp, 0), kvh = sload(jp, 1), row = sload(jp, 2) + j, n = sload(jp, 5), stride = sload(jp, 6);
-    const long part = (long)sload(jp, 4) + j;
-    const int lane = threadIdx.x & 63, piece = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
-    float top = -INFINITY;
-    for (int s = lane; s < n; s += 64) top = fmaxf(top, p.part_ml[part + (long)s * stride].x);
+    __shared__ float2 part_ml[GROUPS];
+    const int slice = blockIdx.x % SLICES;
+    const int* jp = (const int*)(p.joins + blockIdx.x / SLICES);
+    const int cu = sload(jp, 0), kvh = sload(jp, 1), rows = sload(jp, 3), n = sload(jp, 5), stride = sload(jp, 6), share = sload(jp, 7);
+    const int row0 = sload(jp, 2);
+    const long part = sload(jp, 4);
+    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
+    const int j = group / share, piece = group - j * share;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, total = 0.f;
+    // (a piece without a visible key holds zeros, or NaN that stays)
+    auto add = [&](const float4& x, float m, float l, float ref) {
+        const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);
+        acc[0] = __builtin_fmaf(f, x.x, acc[0]);
+        acc[1] = __builtin_fmaf(f, x.y, acc[1]);
+        acc[2] = __builtin_fmaf(f, x.z, acc[2]);
+        acc[3] = __builtin_fmaf(f, x.w, acc[3]);
+        total = __builtin_fmaf(f, l, total);
+    };
+    if (j < rows)
+        for (int s0 = piece; s0 < n; s0 += 4 * share) {   // four pieces requested at a time
+            float4 x[4];
+            float2 ml[4];
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float ref = top == -INFINITY ? 0.f : top;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
-    for (int s0 = piece; s0 < n; s0 += 4 * GROUPS) {   // four pieces requested at a time
-        float4 x[4];
-        float2 ml[4];
+            for (int k = 0; k < 4; k++) {
+                const int s = s0 + k * share;
+                const long at = part + j + (long)(s < n ? s : s0) * stride;
+                x[k] = *(const float4*)(p.part_o + at * D + slice * 64 + d);
+                ml[k] = p.part_ml[at];
+            }
+            float ref = top;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int s = s0 + k * GROUPS;
-            const long at = part + (long)(s < n ? s : s0) * stride;
-            x[k] = *(const float4*)(p.part_o + at * D + slice * 64 + d);
-            ml[k] = p.part_ml[at];
+            for (int k = 0; k < 4; k++) ref = fmaxf(ref, ml[k].x);   // (a piece asked for twice changes no maximum)
+            if (top != -INFINITY) {
+                const float f = __builtin_amdgcn_exp2f(top - ref);
+                total *= f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[k] *= f;
+            }
+            top = ref;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (s0 + k * share < n) add(x[k], ml[k].x, ml[k].y, ref);
         }
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (s0 + k * GROUPS >= n) break;
-            const float f = ml[k].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[k].x - ref);   // (a piece without a visible key holds zeros, or NaN that stays)
-            acc[0] = __builtin_fmaf(f, x[k].x, acc[0]);
-            acc[1] = __builtin_fmaf(f, x[k].y, acc[1]);
-            acc[2] = __builtin_fmaf(f, x[k].z, acc[2]);
-            acc[3] = __builtin_fmaf(f, x[k].w, acc[3]);
-            total = __builtin_fmaf(f, ml[k].y, total);
+    if (share > 1) {
+        *(float4*)&part_sum[group][d] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (d == 0) part_ml[group] = make_float2(top, total);
+        __syncthreads();
+        if (piece) return;
+        const int used = n < share ? n : share;
+        const float m0 = top, l0 = total;
+        for (int s = 1; s < used; s++) top = fmaxf(top, part_ml[group + s].x);
+        total = 0.f;
+        const float4 own = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+        add(own, m0, l0, top);
+        for (int s = 1; s < used; s++) {
+            const float2 ml = part_ml[group + s];
+            add(*(const float4*)&part_sum[group + s][d], ml.x, ml.y, top);
         }
     }
-    *(float4*)&part_sum[piece][d] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (d == 0) total_sum[piece] = total;
-    __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int used = n < GROUPS ? n : GROUPS;
-    float o = 0.f, l = 0.f;
-    for (int s = 0; s < used; s++) {
-        o += part_sum[s][lane];
-        l += total_sum[s];
-    }
-    const int tok = row / p.group, head = kvh * p.group + (row - tok * p.group);
-    p.out[(long)(cu + tok) * p.o_tok + (long)head * p.o_head + slice * 64 + lane] = (__bf16)(o * inverse(l));
-    if (p.lse && slice == 0 && lane == 0) p.lse[(long)(cu + tok) * p.hq + head] = log_sum(top, l);
+    if (j >= rows) return;
+    const int row = row0 + j, tok = row / p.group, head = kvh * p.group + (row - tok * p.group);
+    const float f = inverse(total);
+    bf16x4 y;
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = (__bf16)(acc[k] * f);
+    *(bf16x4*)(p.out + (long)(cu + tok) * p.o_tok + (long)head * p.o_head + slice * 64 + d) = y;
+    if (p.lse && slice == 0 && d == 0) p.lse[(long)(cu + tok) * p.hq + head] = log_sum(top, total);
 }
 
 template <int D, int DV, int NW, bool CAP>
@@ -789,7 +811,7 @@ int launch(Params p, const spinf_paged_args* a, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess && a->n_joins) {
-        hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a->n_joins * PAGED_JOIN * (D / 64))), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a->n_joins * (D / 64))), dim3(256), 0, s, p);
         e = hipGetLastError();
     }
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "paged_attn: launch: %s", hipGetErrorString(e));

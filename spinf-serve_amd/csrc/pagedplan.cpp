@@ -185,8 +185,10 @@ class Builder {
             for (int h = 0; h < a_->hkv; h++) {
                 const int64_t part = p_->part_rows;
                 if (nsplit > 1) {
-                    for (int64_t j = 0; j < here; j += PAGED_JOIN)
-                        p_->joins.push_back({r.cu, h, (int32_t)(row0 + j), (int32_t)std::min<int64_t>(PAGED_JOIN, here - j), (int32_t)(part + j), (int32_t)nsplit, rows, 0});
+                    int share = 1;   // (each group asks for four pieces at a time)
+                    while (share < PAGED_JOIN && share * 4 < nsplit) share *= 2;
+                    for (int64_t j = 0; j < here; j += PAGED_JOIN / share)
+                        p_->joins.push_back({r.cu, h, (int32_t)(row0 + j), (int32_t)std::min<int64_t>(PAGED_JOIN / share, here - j), (int32_t)(part + j), (int32_t)nsplit, rows, share});
                     p_->part_rows += nsplit * rows;
                 }
                 for (int64_t s = 0; s < nsplit; s++)
