@@ -21,9 +21,10 @@ constexpr int PAGED_PLACES = 512;        // workgroups of either kernel that run
 // mostly idle; the shared tiles read them once per 128 rows and are the faster where it, or others like it, fill the GPU (us, 1 / 16 such requests in a call, wave -> shared):
 //   16 heads on 8 of 256 dims, 160 new on 2,000 stored  36 / 378 -> 58 / 187     48 new on 8,000  37 / 438 -> 71 / 257     160 new on 400  20 / 101 -> 34 / 50
 //   32 heads on 16 of 128,     160 new on 2,000         25 / 252 -> 44 / 185     48 new on 8,000  25 / 319 -> 55 / 245     160 new on 400  18 / 76 -> 26 / 43
-// Up to PAGED_WAVE_MAX workgroups of the shared kernel and PAGED_WAVE_WORK tiles of 32 rows x 32 keys x 128 dims the request goes to the waves.
+// Up to PAGED_WAVE_MAX workgroups of the shared kernel and PAGED_WAVE_WORK tiles of 32 rows x 32 keys x 128 dims the request goes to the waves: there the two are
+// even at about four such requests in a call (80 new on 2,000, 8 heads of 256 dims: 56 / 59 us; 16 heads of 128: 43 / 45).
 constexpr int PAGED_WAVE_MAX = 64;
-constexpr int PAGED_WAVE_WORK = 9000;
+constexpr int PAGED_WAVE_WORK = 5000;
 constexpr int PAGED_WAVE_TILES = 16;     // least tiles of a piece there
 // Least tiles of a piece of the shared kernel (us at 32 / 48 / 64; a call of 1 and of 16 requests, 640 rows per key / value head on 8,000 stored keys: 8 heads of
 // 256 dims 79 / 80 / 98 and 963 / 889 / 861, 16 heads of 128 dims 70 / 72 / 84 and 892 / 907 / 882; a window of 1,024 under 512 new tokens 143 / 98 / 98).

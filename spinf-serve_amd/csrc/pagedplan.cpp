@@ -152,9 +152,15 @@ class Builder {
         const int halves = a_->d == 512 ? 2 : 1;
         // The kernel whose waves share their rows and divide the keys takes what the other one would leave the GPU mostly idle with.
         const int64_t blocks = (N + GROUP * BLOCK_GROUPS - 1) / (GROUP * BLOCK_GROUPS) * a_->hkv * halves;
-        const int64_t keys = window_ > 0 ? std::min<int64_t>(r.L, (int64_t)window_ + r.T) : r.L;
-        const int64_t work = (N + GROUP - 1) / GROUP * a_->hkv * ((keys + TK - 1) / TK) * a_->d / 128;
-        const bool by_wave = a_->variant ? a_->variant == 1 : N <= 2 * GROUP || (blocks <= PAGED_WAVE_MAX && work <= PAGED_WAVE_WORK);
+        bool by_wave = a_->variant ? a_->variant == 1 : N <= 2 * GROUP || blocks <= PAGED_WAVE_MAX;
+        if (by_wave && !a_->variant && N > 2 * GROUP) {
+            int64_t work = 0;
+            for (int64_t row0 = 0; row0 < N; row0 += GROUP) {
+                list(r, (int)row0, 1, runs_);
+                for (const Run& x : runs_) work += x.count;
+            }
+            by_wave = work * a_->hkv * a_->d / 128 <= PAGED_WAVE_WORK;
+        }
         const int groups = by_wave ? 1 : BLOCK_GROUPS, rows = groups * GROUP;
         const int64_t row_items = (N + rows - 1) / rows * a_->hkv * halves;
         std::vector<Run>& runs = runs_;
