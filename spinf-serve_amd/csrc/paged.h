@@ -16,7 +16,10 @@ constexpr int PAGED_JOIN = 16;            // groups of 16 lanes that join rows: 
 struct PagedJoin { int32_t cu, kvh, row0, rows, part, nsplit, stride, share; };
 static_assert(sizeof(PagedRun) == 16 && sizeof(PagedItem) == 48 && sizeof(PagedJoin) == 32, "read by the kernels as 16-byte pieces");
 
-constexpr int PAGED_PLACES = 512;        // workgroups of either kernel that run at a time (two per compute unit)
+// Workgroups that run at a time (two per compute unit, one where a workgroup's tiles fill its LDS: 512 dims, and 256 dims in the wave kernel).  A request's keys are cut
+// for that many, and not more: a second round of workgroups costs its start and its share of the join (one token over 131,071 keys of 512 dims, one
+// key / value head: 256 workgroups 45.8 + 4.9 us for the join, 482 52.9 + 6.6).
+constexpr int PAGED_PLACES = 512;
 // Which kernel takes a request, by its own size alone.  The waves that divide the keys read them once per 32 rows and are the faster where the request leaves the GPU
 // mostly idle; the shared tiles read them once per 128 rows and are the faster where it, or others like it, fill the GPU (us, 1 / 16 such requests in a call, wave -> shared):
 //   16 heads on 8 of 256 dims, 160 new on 2,000 stored  36 / 378 -> 58 / 187     48 new on 8,000  37 / 438 -> 71 / 257     160 new on 400  20 / 101 -> 34 / 50
@@ -25,7 +28,8 @@ constexpr int PAGED_PLACES = 512;        // workgroups of either kernel that run
 // even at about four such requests in a call (80 new on 2,000, 8 heads of 256 dims: 56 / 59 us; 16 heads of 128: 43 / 45).
 constexpr int PAGED_WAVE_MAX = 64;
 constexpr int PAGED_WAVE_WORK = 5000;
-constexpr int PAGED_WAVE_TILES = 16;     // least tiles of a piece there
+// Least tiles of a piece there (us at 8 / 16 / 32: one token over 4,000 keys, 8 heads of 256 dims 11 / 14 / 21; 64 such requests of 3,000 keys, 4 heads: 171 / 149 / 140).
+constexpr int PAGED_WAVE_TILES = 16;
 // Least tiles of a piece of the shared kernel (us at 32 / 48 / 64; a call of 1 and of 16 requests, 640 rows per key / value head on 8,000 stored keys: 8 heads of
 // 256 dims 79 / 80 / 98 and 963 / 889 / 861, 16 heads of 128 dims 70 / 72 / 84 and 892 / 907 / 882; a window of 1,024 under 512 new tokens 143 / 98 / 98).
 constexpr int PAGED_BLOCK_TILES = 48;

@@ -11,9 +11,15 @@
 // page: two scalar reads of the page list per tile, no per-key lookup.  Rows behind the stored keys are never read (the last key is read in their place).
 //
 // Two kernels over the items of csrc/pagedplan.cpp:
-//   wave   few rows: the workgroup's waves share 32 rows and divide the tiles, each with a tile buffer of its own and no barrier; joined at the end
-//   block  many rows: four waves with 32 rows each on the same double-buffered tiles, one barrier per tile
+//   wave   few rows: the workgroup's waves share 32 rows and divide the tiles, each with a tile buffer of its own and no barrier; joined at the end.
+//          Bound by HBM where the GPU is full (64 requests of ~3,000 keys, one token, 24 heads on 4 of 256 dims: 863 MB in 164 us, 5.3 TB/s; one of 131,071 keys of
+//          512 dims 46 us, 5.8), by a tile's latency where it is not (a request's 350 questions' tokens on 301 keys, 16 on 8 of 256: 15.5 us).
+//   block  many rows: four waves with 32 rows each on the same double-buffered tiles, one barrier per tile.  Bound by what a wave cannot overlap: products,
+//          softmax and LDS reads of one tile follow each other, and the two or three waves of a SIMD hide only part of it (two documents of 8,192 new on
+//          8,192 stored tokens, 32 on 16 of 128: 3.10 ms, 1.06 PFLOP/s, matrix pipe busy 45 %; 8 of 256 dims: 2.84 ms, 1.16 PFLOP/s).
 // and paged_join_kernel where an item's keys were cut into pieces.
+// 512 dims: an item is two workgroups, each with all of S and half of the output's dims, whose accumulators would not fit one wave's registers otherwise;
+// the scores are computed twice (514 TFLOP/s counted once).
 //
 // Keys that a row does not see have p = 0 exactly; 0 x inf or NaN in the matrix product would still be NaN.  Nothing is spent on that in the usual
 // case: a workgroup that masked some tile and whose results are not all finite looks whether those tiles hold such values (rubbish), and if so computes its rows again
@@ -866,7 +872,7 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     switch (a->d) {
         case 64: return launch_cap<64, 64, 4>(p, a, s);
         case 128: return launch_cap<128, 128, 4>(p, a, s);
-        case 256: return launch_cap<256, 256, 4>(p, a, s);
+        case 256: return launch_cap<256, 256, 4>(p, a, s);   // (as many waves as have tile buffers in 160 KB of LDS; two waves: a request's questions 21.7 us for 15.5)
         case 512: return launch_cap<512, 256, 3>(p, a, s);
         default: return spinf_fail(SPINF_E_ARG, "paged_attn: head dim %d not supported (64, 128, 256, 512)", a->d);
     }

