@@ -18,8 +18,8 @@
 //          softmax and LDS reads of one tile follow each other, and the two or three waves of a SIMD hide only part of it (two documents of 8,192 new on
 //          8,192 stored tokens, 32 on 16 of 128: 3.10 ms, 1.06 PFLOP/s, matrix pipe busy 45 %; 8 of 256 dims: 2.84 ms, 1.16 PFLOP/s).
 // and paged_join_kernel where an item's keys were cut into pieces.
-// 512 dims: an item is two workgroups, each with all of S and half of the output's dims, whose accumulators would not fit one wave's registers otherwise;
-// the scores are computed twice (514 TFLOP/s counted once).
+// 512 dims: a wave's registers hold the accumulators of half of them.  In the wave kernel an item is two workgroups, each with all of S and half of the output's dims
+// (bound by the keys' bytes, which the L2 gives the second one); in the block kernel two waves share their rows, each with half of the products on either side.
 //
 // Keys that a row does not see have p = 0 exactly; 0 x inf or NaN in the matrix product would still be NaN.  Nothing is spent on that in the usual
 // case: a workgroup that masked some tile and whose results are not all finite looks whether those tiles hold such values (rubbish), and if so computes its rows again
@@ -149,7 +149,8 @@ struct Rows {
     float M, l, over;   // reference (0 before a row's first key), sum, score above which the reference is raised (-inf: no key so far)
     int lane, m, g, tok, qpos;
 
-    __device__ __forceinline__ void load(const Params& p, const PagedItem& it, int row0) {
+    // queries of rows row0 + m, dims col ..
+    __device__ __forceinline__ void load(const Params& p, const PagedItem& it, int row0, int col = 0) {
         lane = threadIdx.x & 63;
         m = lane & 31;
         g = lane >> 5;
@@ -157,7 +158,7 @@ struct Rows {
         const int r = row < N ? row : N - 1;
         tok = r / p.group;
         const int head = it.kvh * p.group + (r - tok * p.group);
-        const __bf16* qp = p.q + (long)(it.cu + tok) * p.q_tok + (long)head * p.q_head + 8 * g;
+        const __bf16* qp = p.q + (long)(it.cu + tok) * p.q_tok + (long)head * p.q_head + col + 8 * g;
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
         qpos = it.L - it.T + tok;
@@ -577,35 +578,35 @@ __device__ __forceinline__ void fill(Window<WIN>& win, const Params& p, const Pa
     }
 }
 
+//
+// 512 dims: two waves share 32 rows, each with one half of the dims (H = 2) of queries, keys, values and outputs, as a wave of 256 dims has them.  Their
+// scores are exchanged through the place of the tile's keys, which nobody reads any more, and added: both then hold the same bits and the same softmax.
+// (Two documents of 8,192 new on 8,192 stored, 16 heads on 1: 8.26 ms, 798 TFLOP/s; with all scores in both halves, each a workgroup of its own, 12.99 ms.)
 template <int D, int DV, bool CAP>
-__global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_block_kernel(const Params p) {
-    using R = Rows<D, DV, CAP>;
+__global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void paged_block_kernel(const Params p) {
+    constexpr int H = D / DV;
+    using R = Rows<DV, DV, CAP>;
     using GK = typename R::GK;
     using GV = typename R::GV;
-    constexpr int BUF = GK::KTILEB + GV::VTILEB + 512;
+    constexpr int HALF = GK::KTILEB + GV::VTILEB + 512, BUF = H * HALF;
     constexpr int OROW = DV * 2 + 16;   // bytes of an output row in LDS
-    constexpr int LDS = 2 * BUF > 4 * 32 * OROW ? 2 * BUF : 4 * 32 * OROW;
+    constexpr int LDS = 2 * BUF > H * 4 * 32 * OROW ? 2 * BUF : H * 4 * 32 * OROW;
     constexpr int NK = GK::NREG / 4, NV = GV::NREG / 4;
     constexpr int WIN = 128;
     static_assert(NK * 4 == GK::NREG && NV * 4 == GV::NREG, "a tile's regions must divide among the four waves");
     static_assert((D == 256 ? 2 : 1) * (LDS + sizeof(Window<WIN>)) <= 160 * 1024, "LDS budget");
+    static_assert(H == 1 || 4 * 4096 <= GK::KTILEB, "four waves' scores take the place of a half's keys");
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ Window<WIN> win;
-    int b = blockIdx.x;
-    int vcol = 0;
-    if (DV < D) {
-        vcol = ((b >> 3) & 1) * DV;
-        b = (b >> 4) * 8 + (b & 7);
-        if (b >= p.n_items) return;
-    }
-    const PagedItem it = load_item(p.items, b);
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedItem it = load_item(p.items, blockIdx.x);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = H == 1 ? wave : wave & 3, half = H == 1 ? 0 : wave >> 2, vcol = half * DV;
     const int c = it.L - it.T;
     const char* const k_base = p.k + it.kvh * p.k_head;
-    const char* const v_base = p.v + it.kvh * p.v_head + vcol * 2;
+    const char* const v_base = p.v + it.kvh * p.v_head;
     fill<WIN>(win, p, it, 0, k_base, v_base);
     R rows;
-    const unsigned base = lds_addr(lds);
+    const unsigned base = lds_addr(lds) + half * HALF;
 
     // This lane's place in the regions that its wave copies: rows r + x (x < NK, NV) of the tile, which lie in one half of it
     const auto k_row = [&](int lane) { return w * NK + GK::NREG * (lane / GK::CPR); };
@@ -614,8 +615,8 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
         const unsigned at = base + buf * BUF;
         if (kt * TK + TK <= it.L) {
             const int lane = D >= 256 ? lane_now() : threadIdx.x & 63;   // (256 dims: what depends on the lane alone would be spilled, and reloaded in front of every request)
-            const char* ka = (const char*)win.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16);
-            const char* va = (const char*)win.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16);
+            const char* ka = (const char*)win.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16 + vcol * 2);
+            const char* va = (const char*)win.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16 + vcol * 2);
 #pragma unroll
             for (int x = 0; x < NK; x++, ka += p.k_row) dma16_lane(ka, at + (w * NK + x) * GK::KRS);
 #pragma unroll
@@ -625,15 +626,15 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
 #pragma unroll
             for (int x = 0; x < NK; x++) {
                 const int r = k_row(lane) + x < last ? k_row(lane) + x : last;
-                dma16_lane((const char*)win.k[i][r >> 4] + (r & 15) * (unsigned long long)p.k_row + lane % GK::CPR * 16, at + (w * NK + x) * GK::KRS);
+                dma16_lane((const char*)win.k[i][r >> 4] + (r & 15) * (unsigned long long)p.k_row + lane % GK::CPR * 16 + vcol * 2, at + (w * NK + x) * GK::KRS);
             }
 #pragma unroll
             for (int x = 0; x < NV; x++) {
                 const int r = v_row(lane) + x < last ? v_row(lane) + x : last;
-                dma16_lane((const char*)win.v[i][r >> 4] + (r & 15) * (unsigned long long)p.v_row + lane % GV::CPR * 16, at + GK::KTILEB + (w * NV + x) * GV::VRS);
+                dma16_lane((const char*)win.v[i][r >> 4] + (r & 15) * (unsigned long long)p.v_row + lane % GV::CPR * 16 + vcol * 2, at + GK::KTILEB + (w * NV + x) * GV::VRS);
             }
         }
-        if (w == 0 && p.end && (bits & 0xf0) && kt * TK + TK > c) fetch_meta(p, it, kt, at + GK::KTILEB + GV::VTILEB, lane_now());
+        if (wave == 0 && p.end && (bits & 0xf0) && kt * TK + TK > c) fetch_meta(p, it, kt, at + GK::KTILEB + GV::VTILEB, lane_now());
     };
 
     bool seen_mask = false;
@@ -645,7 +646,7 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
         bits = __builtin_amdgcn_readfirstlane(t.y);
         issue(0, kt, bits, 0);   // (ahead of the queries: their latencies pass together)
     }
-    rows.load(p, it, it.row0 + 32 * w);
+    rows.load(p, it, it.row0 + 32 * w, vcol);
     rows.reset();
     for (int i = 0, j = 0, buf = 0; i < it.tiles; i++, buf ^= 1) {   // j: tile i's place in the window
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
@@ -667,10 +668,26 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
         const bool masked = ((bits >> w) & 17) != 1;
         const bool tree = p.end && (bits & 0xf0) && kt * TK + TK > c;
         seen_mask |= masked;
-        const char* kb = lds + buf * BUF;
+        char* kb = lds + buf * BUF + half * HALF;
         f32x16 s;
         rows.scores(kb, s);
-        if (masked) rows.mask(p, it, kt, (const int*)(kb + GK::KTILEB + GV::VTILEB), tree, s);
+        if (H == 2) {
+            char* const mine = kb + w * 4096 + lane_now() * 16;
+            const char* const other = mine + (half ? -HALF : HALF);
+            __syncthreads();   // every wave is done with the keys
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) *(float4*)(mine + i4 * 1024) = make_float4(s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]);
+            __syncthreads();
+#pragma unroll
+            for (int i4 = 0; i4 < 4; i4++) {
+                const float4 x = *(const float4*)(other + i4 * 1024);
+                s[4 * i4] += x.x;
+                s[4 * i4 + 1] += x.y;
+                s[4 * i4 + 2] += x.z;
+                s[4 * i4 + 3] += x.w;
+            }
+        }
+        if (masked) rows.mask(p, it, kt, (const int*)(lds + buf * BUF + GK::KTILEB + GV::VTILEB), tree, s);
         bf16x8 pb[2];
         rows.softmax(p, s, masked, pb);
         rows.values(kb + GK::KTILEB, pb);
@@ -702,7 +719,7 @@ __global__ __launch_bounds__(256, D == 512 ? 1 : D == 256 ? 2 : 3) void paged_bl
     }
     if (p.lse && g == 0 && m < left && vcol == 0) p.lse[row_head(p, it, it.row0 + 32 * w + m)] = log_sum(rows.M, sum);
     // rows through the wave's own slice of LDS, stored as 16-byte pieces
-    char* const stage = lds + w * 32 * OROW;
+    char* const stage = lds + wave * 32 * OROW;
 #pragma unroll
     for (int dt = 0; dt < R::NDT; dt++)
 #pragma unroll
@@ -802,18 +819,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const Params p) {
 
 template <int D, int DV, int NW, bool CAP>
 int launch(Params p, const spinf_paged_args* a, hipStream_t s) {
-    auto grid = [](int64_t n) { return dim3((unsigned)(D / DV == 2 ? (n + 7) / 8 * 16 : n)); };
     hipError_t e = hipSuccess;
     if (a->n_block) {
         p.items = (const PagedItem*)a->block;
         p.n_items = (int)a->n_block;
-        hipLaunchKernelGGL((paged_block_kernel<D, DV, CAP>), grid(a->n_block), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_block_kernel<D, DV, CAP>), dim3((unsigned)a->n_block), dim3(256 * (D / DV)), 0, s, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a->n_wave) {
         p.items = (const PagedItem*)a->wave;
         p.n_items = (int)a->n_wave;
-        hipLaunchKernelGGL((paged_wave_kernel<D, DV, NW, CAP>), grid(a->n_wave), dim3(64 * NW), 0, s, p);
+        const int64_t n = D / DV == 2 ? (a->n_wave + 7) / 8 * 16 : a->n_wave;
+        hipLaunchKernelGGL((paged_wave_kernel<D, DV, NW, CAP>), dim3((unsigned)n), dim3(64 * NW), 0, s, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess && a->n_joins) {

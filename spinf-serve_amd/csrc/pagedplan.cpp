@@ -149,9 +149,8 @@ class Builder {
 
     void request(const Request& r, int index) {
         const int64_t N = (int64_t)r.T * group_;
-        const int halves = a_->d == 512 ? 2 : 1;
         // The kernel whose waves share their rows and divide the keys takes what the other one would leave the GPU mostly idle with.
-        const int64_t blocks = (N + GROUP * BLOCK_GROUPS - 1) / (GROUP * BLOCK_GROUPS) * a_->hkv * halves;
+        const int64_t blocks = (N + GROUP * BLOCK_GROUPS - 1) / (GROUP * BLOCK_GROUPS) * a_->hkv;
         bool by_wave = a_->variant ? a_->variant == 1 : N <= 2 * GROUP || blocks <= PAGED_WAVE_MAX;
         if (by_wave && !a_->variant && N > 2 * GROUP) {
             int64_t work = 0;
@@ -162,7 +161,7 @@ class Builder {
             by_wave = work * a_->hkv * a_->d / 128 <= PAGED_WAVE_WORK;
         }
         const int groups = by_wave ? 1 : BLOCK_GROUPS, rows = groups * GROUP;
-        const int64_t row_items = (N + rows - 1) / rows * a_->hkv * halves;
+        const int64_t row_items = (N + rows - 1) / rows * a_->hkv * (by_wave && a_->d == 512 ? 2 : 1);   // (the wave kernel has a workgroup per half of 512 dims)
         std::vector<Run>& runs = runs_;
         for (int64_t row0 = 0; row0 < N; row0 += rows) {
             list(r, (int)row0, groups, runs);
