@@ -371,6 +371,52 @@ def test_a_request_has_the_same_bits_whatever_shares_the_call(dev):
         base += T
 
 
+# many rows at 512 dims (halves that exchange their scores): chunks, a window with a cap, trees, keys cut into pieces, two key / value heads
+HALVES = [
+    ([33, 9], [700, 9], 48, (16, 1, 512), 200, 30.0, None),
+    ([70, 1], [70, 40], 16, (4, 2, 512), 0, 0.0, None),
+    ([30, 22], [130, 60], 16, (8, 1, 512), 40, 0.0, (2, 8)),
+    ([40], [3300], 64, (4, 1, 512), 0, 0.0, None),
+]
+# pieces per row: a few up to more than four times the groups that a join's rows may have; few rows and many
+PIECES = [
+    ([3, 1], [1100, 2600], 16, (4, 1, 64), 0, 0.0, None),
+    ([9], [3600], 48, (4, 1, 128), 0, 20.0, None),
+    ([5, 2], [7000, 4400], 64, (3, 1, 64), 0, 0.0, None),
+    ([1], [13000], 16, (6, 1, 64), 0, 0.0, None),
+    ([2], [35000], 64, (1, 1, 64), 0, 0.0, None),
+    ([150], [3300], 64, (2, 1, 128), 0, 0.0, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("q_lens,kv_lens,page,heads,window,softcap,tree", HALVES + PIECES)
+def test_halves_and_pieces_against_the_oracle(dev, q_lens, kv_lens, page, heads, window, softcap, tree, variant, monkeypatch):
+    test_attention_against_the_oracle(dev, q_lens, kv_lens, page, heads, window, softcap, tree, variant, "heads", monkeypatch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,kv_lens,window,tree", [([50, 20], [130, 33], 0, (1, 9)), ([40, 70], [90, 70], 25, None)])
+def test_halves_leave_no_trace_of_unseen_keys(dev, q_lens, kv_lens, window, tree, monkeypatch):
+    test_what_a_row_does_not_see_leaves_no_trace(dev, q_lens, kv_lens, 16, (4, 1, 512), window, tree, 2, monkeypatch)
+
+
+def test_joins_cover_every_row_of_cut_keys():
+    """share: groups of 16 lanes per row, a power of two, the fewest that ask for a row's pieces four at a time (16 at most)"""
+    for n, hq, hkv, d in ((1100, 4, 1, 64), (3600, 8, 2, 128), (9000, 16, 1, 512), (40000, 3, 1, 64), (90000, 24, 4, 256)):
+        b, _ = make_batch([3], [n], 16)
+        lists, counts, at, _ = b._compile(hq, hkv, d, 0, 0)
+        joins = lists[at[3] : at[3] + 8 * counts[3]].reshape(-1, 8)
+        assert len(joins)
+        rows = sorted((int(j[1]), int(j[2]) + x) for j in joins for x in range(j[3]))
+        assert rows == [(h, r) for h in range(hkv) for r in range(3 * hq // hkv)]
+        for _, _, _, count, part, pieces, stride, share in joins.tolist():
+            assert share in (1, 2, 4, 8, 16) and 1 <= count <= 16 // share
+            assert share == 16 or 4 * share >= pieces and (share == 1 or 2 * share < pieces)
+            assert 0 <= part and part + count + (pieces - 1) * stride <= counts[4]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [128, 512])
 def test_strided_queries_and_a_single_key(dev, d):
