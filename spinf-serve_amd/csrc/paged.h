@@ -26,6 +26,7 @@ constexpr int PAGED_PLACES = 512;
 //   32 heads on 16 of 128,     160 new on 2,000         25 / 252 -> 44 / 185     48 new on 8,000  25 / 319 -> 55 / 245     160 new on 400  18 / 76 -> 26 / 43
 // Up to PAGED_WAVE_MAX workgroups of the shared kernel and PAGED_WAVE_WORK tiles of 32 rows x 32 keys x 128 dims the request goes to the waves: there the two are
 // even at about four such requests in a call (80 new on 2,000, 8 heads of 256 dims: 56 / 59 us; 16 heads of 128: 43 / 45).
+// Up to 64 rows per key / value head it always does: half and more of the shared kernel's rows would idle (48 rows on 8,000 keys, 8 heads of 256 dims: 23 / 314 -> 67 / 247).
 constexpr int PAGED_WAVE_MAX = 64;
 constexpr int PAGED_WAVE_WORK = 5000;
 // Least tiles of a piece there (us at 8 / 16 / 32: one token over 4,000 keys, 8 heads of 256 dims 11 / 14 / 21; 64 such requests of 3,000 keys, 4 heads: 171 / 149 / 140).
