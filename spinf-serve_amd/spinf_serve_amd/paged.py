@@ -330,8 +330,8 @@ def _attn_block(q, k, v, table, end, pos, lists, counts, at, page, max_page, tok
 
 def _attn_run(a, q, k, v, want_lse, stream=None):
     device = q.device
-    T, hq, d = shape = q.shape
-    out = torch.empty(shape, dtype=BF16, device=device)
+    T, hq, d = q.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = None
     if want_lse:
         lse = torch.empty((T, hq), dtype=torch.float32, device=device)
@@ -479,7 +479,8 @@ def _evict_block(k, v, acc, table, reqs, page, keep, sink, recent):
 
 def _evict_run(a, k, v, acc, new_table, new_reqs, stream=None):
     device, shape = acc.device, (a.n_reqs, a.hkv, a.keep)
-    kept, new_acc = torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
+    kept = torch.empty(shape, dtype=torch.int32, device=device)
+    new_acc = torch.empty_like(kept, dtype=torch.float32)
     if not (a.n_reqs and a.keep and a.keys):   # no stored key at all
         return kept.fill_(-1), new_acc.zero_()
     a.acc, a.k, a.v, a.kept, a.new_acc = acc.data_ptr(), k.data_ptr(), v.data_ptr(), kept.data_ptr(), new_acc.data_ptr()

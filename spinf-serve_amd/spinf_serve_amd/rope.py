@@ -17,6 +17,7 @@ import torch
 from . import _lib
 
 _TABLE = (torch.float32, torch.bfloat16)
+_DENSE = torch.contiguous_format   # (an output made like its input costs the host half of what one of a given shape does)
 
 
 def _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, what):
@@ -78,17 +79,17 @@ def _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, what):
 _SEEN: dict = {}
 
 
-def _known(key, device, tensors):
-    """the block kept for this key with the tensors' addresses, if they lie on `device` and are aligned as the kernel wants them"""
+def _known(key, index, tensors):
+    """the block kept for this key with the tensors' addresses, if they lie on GPU `index` and are aligned as the kernel wants them"""
     got = _SEEN.get(key)
-    if got is None or device.type != "cuda":
+    if got is None or index < 0:
         return None
     at, bits = [], 0
     for t in tensors:
         if t is None:
             at.append(None)
             continue
-        if t.device != device:
+        if t.get_device() != index:
             return None   # (the checks say what is wrong)
         x = t.data_ptr()
         bits |= x
@@ -114,13 +115,13 @@ def _note(key, a):
 
 def _rope(q: torch.Tensor, k: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
           pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    device = q.device
+    device, index = q.device, q.get_device()
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, _table(wq, wk, cos, sin, pos), eps, neighbours, plus_one)
-    a = _known(key, device, (q, k, None, wq, wk, cos, sin))
-    if a is None or (pos is not None and pos.device != device):
+    a = _known(key, index, (q, k, None, wq, wk, cos, sin))
+    if a is None or (pos is not None and pos.get_device() != index):
         a = _rope_args(q, k, None, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope")
         _note(key, a)
-    q_out, k_out = torch.empty(q.shape, dtype=torch.bfloat16, device=device), torch.empty(k.shape, dtype=torch.bfloat16, device=device)
+    q_out, k_out = torch.empty_like(q, memory_format=_DENSE), torch.empty_like(k, memory_format=_DENSE)
     a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
     a.pos = pos.data_ptr() if pos is not None else None
     if q.shape[0]:
@@ -146,11 +147,11 @@ def qk_norm_rope(q, k, wq, wk, cos, sin, eps, pos=None, neighbours=False, plus_o
 
 def _put(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, eps: float,
          ck: torch.Tensor, cv: torch.Tensor, slots: torch.Tensor, pos: Optional[torch.Tensor], neighbours: bool, plus_one: bool, v_norm: bool) -> torch.Tensor:
-    device = q.device
+    device, index = q.device, q.get_device()
     key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, ck.shape, ck.stride(), cv.stride(), slots.shape, slots.stride(), slots.dtype,
            _table(wq, wk, cos, sin, pos), eps, neighbours, plus_one, v_norm)
-    a = _known(key, device, (q, k, v, wq, wk, cos, sin, ck, cv))
-    if a is None or (pos is not None and pos.device != device) or slots.device != device:
+    a = _known(key, index, (q, k, v, wq, wk, cos, sin, ck, cv))
+    if a is None or (pos is not None and pos.get_device() != index) or slots.get_device() != index:
         a = _rope_args(q, k, v, wq, wk, cos, sin, eps, pos, neighbours, plus_one, "qk_norm_rope_put")
         if ck.shape[2:] != k.shape[1:]:
             raise ValueError(f"the cache holds {tuple(ck.shape[2:])} a key, the layer makes {tuple(k.shape[1:])}")
@@ -163,7 +164,7 @@ def _put(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, wq: Optional[torch.T
         a.v_page, a.v_row, a.vh_out = cv.stride()[:3]
         a.pages, a.page, a.v_norm = ck.shape[0], ck.shape[1], int(v_norm)
         _note(key, a)
-    q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
+    q_out = torch.empty_like(q, memory_format=_DENSE)
     a.q_out, a.k_out, a.v_out, a.slots = q_out.data_ptr(), ck.data_ptr(), cv.data_ptr(), slots.data_ptr()
     a.pos = pos.data_ptr() if pos is not None else None
     if q.shape[0]:
