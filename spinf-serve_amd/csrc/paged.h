@@ -6,7 +6,8 @@ constexpr int PAGED_TILE = 32;           // keys per tile
 constexpr int PAGED_ROWS = 32;           // rows per row group (row = new token * query heads per key / value head + head)
 constexpr int PAGED_BLOCK_GROUPS = 4;    // row groups of a block item
 
-// `count` tiles from kt on, the item's tiles start .. start + count - 1; bits: 1 << g some row of row group g sees a key, 16 << g some pair is masked
+// `count` tiles from kt on, the item's tiles start .. start + count - 1; bits: 1 << g some row of row group g sees a key, 16 << g some pair of it is
+// masked (all of them, where the group sees nothing: the kernel computes the tile for every group of the item)
 struct PagedRun { int32_t kt, count; uint32_t bits; int32_t start; };
 // rows row0 .. of key / value head kvh of the request whose new tokens are rows cu .. cu + T - 1 of the call and whose L stored keys lie in the pages
 // tab .. of the page list; runs first .. first + runs - 1 (`tiles` tiles); part: first partial row, -1: the only piece

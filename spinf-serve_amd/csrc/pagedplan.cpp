@@ -142,7 +142,8 @@ class Builder {
             }
             uint32_t bits = 0;
             for (int i = 0; i < n; i++) bits |= tile_bits(r, window_, (int)kt, g[i].a, g[i].b, g[i].lo, g[i].hi) << i;
-            if (bits & 15u) add(kt, 1, bits);
+            // (a group that sees nothing of a tile that another one sees computes it too: all of its pairs are masked)
+            if (bits & all) add(kt, 1, bits | (all & ~bits) << 4);
             kt++;
         }
     }

@@ -141,6 +141,81 @@ def test_work_lists_are_the_dense_mask(q_lens, kv_lens, page, heads, window, tre
     assert joined == {(int(cu[r]), h, x) for (r, h, row0, g), ps in pieces.items() if len(ps) > 1 for x in range(row0, min(row0 + 32 * g, int(b.q_lens[r]) * group))}
 
 
+def branches(counts, stored, page, device="cpu"):
+    """-> batch, pages in all; request r: branches of counts[r] tokens each below stored[r] keys"""
+    end, pos = [], []
+    for lens, c in zip(counts, stored):
+        for n in lens:
+            end += [len(end) + n] * n
+            pos += range(c, c + n)
+    q_lens = [sum(lens) for lens in counts]
+    kv_lens = [c + n for c, n in zip(stored, q_lens)]
+    need = [-(-n // page) for n in kv_lens]
+    tables = np.split(np.arange(sum(need)), np.cumsum(need)[:-1])
+    return sa.PagedBatch.build(q_lens, kv_lens, [t.tolist() for t in tables], page, device, end=end, pos=pos), sum(need)
+
+
+def by_the_kernels_rule(b, window, it, kt, bits, g, groups, group, N):
+    """[rows, 32] bool: what a kernel lets row group g of an item see of tile kt, from the tile's bits: whole where the group has no masked bit; else the tokens up
+    to a row's own, and where some group is masked and the tile holds new tokens of a tree, of these the ones whose subtree the row lies in"""
+    cu, T, L, row0 = int(it[0]), int(it[1]), int(it[2]), int(it[5])
+    c = L - T
+    tok = np.arange(row0 + 32 * g, min(row0 + 32 * g + 32, N))[:, None] // group
+    s = 32 * kt + np.arange(32)[None]
+    if groups == 1 and not bits & 16 or groups > 1 and (bits >> g) & 17 == 1:
+        return np.ones((len(tok), 32), bool)
+    u = s - c
+    see = u <= tok
+    fresh = np.zeros_like(u, bool)
+    at = s
+    if b._end is not None and bits & 0xf0 and 32 * kt + 32 > c:
+        fresh = u >= 0
+        new = np.clip(u, 0, T - 1)
+        see = see & (~fresh | (cu + tok < b._end[cu + new]))
+        at = np.where(fresh, b._pos[cu + new], s)
+    if window:
+        place = c + tok if b._pos is None else b._pos[cu + tok]
+        see = see & (place - at < window)
+    return see
+
+
+# branches that end on a row group's boundary inside an item, with tiles that lie wholly in an earlier one
+BOUNDARIES = [  # branches, stored, page, (hq, hkv, d), window
+    ([[80, 48]], [64], 64, (16, 8, 256), 0),
+    ([[80, 48] * 5], [64], 64, (16, 8, 256), 0),
+    ([[96] * 3, [48, 80]], [470, 32], 48, (16, 8, 128), 0),
+    ([[80] * 4], [512], 16, (12, 12, 64), 0),
+    ([[96, 64, 96]], [64], 32, (4, 2, 128), 70),
+    ([[40, 24, 40]], [96], 16, (4, 1, 512), 0),
+]
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("q_lens,kv_lens,page,heads,window,tree", [x for x in PLANS if x[5]] + [(c, s, p, h, w, None) for c, s, p, h, w in BOUNDARIES] + [PLANS[5], PLANS[3]])
+def test_what_the_bits_of_a_tile_let_rows_see_is_the_dense_mask(q_lens, kv_lens, page, heads, window, tree, variant, monkeypatch):
+    """every row group of an item computes all of its tiles, those it sees nothing of among them"""
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, _ = branches(q_lens, kv_lens, page) if isinstance(q_lens[0], list) else make_batch(q_lens, kv_lens, page, tree=tree)
+    hq, hkv, d = heads
+    group = hq // hkv
+    lists, (nw, nb, nr, _, _), at = b.plan(hq, hkv, d, window)
+    lists = lists.numpy()
+    runs = lists[at[2] : at[2] + 4 * nr].reshape(-1, 4)
+    see = [np.repeat(x, group, 0) for x in dense(b, window)]
+    for n, off, groups in ((nw, at[0], 1), (nb, at[1], 4)):
+        for it in lists[off : off + 12 * n].reshape(-1, 12):
+            if it[4]:   # (the same runs as head 0's)
+                continue
+            r, L, N = int(it[10]), int(it[2]), int(it[1]) * group
+            for kt, cnt, bits, _ in runs[it[6] : it[6] + it[7]].tolist():
+                for t in range(kt, kt + cnt):
+                    for g in range(groups):
+                        rows = slice(int(it[5]) + 32 * g, min(int(it[5]) + 32 * g + 32, N))
+                        if rows.start < rows.stop:
+                            got = by_the_kernels_rule(b, window, it, t, bits, g, groups, group, N)
+                            assert np.array_equal(got[:, : L - 32 * t], see[r][rows, 32 * t : min(32 * t + 32, L)]) and not got[:, L - 32 * t :].any(), (r, rows, t, bits)
+
+
 def test_a_request_is_cut_the_same_way_whatever_shares_the_call():
     alone, _ = make_batch([1], [5000], 64)
     both, _ = make_batch([300, 1, 1], [2000, 5000, 17], 64)
@@ -355,6 +430,19 @@ def test_what_a_row_does_not_see_leaves_no_trace(dev, q_lens, kv_lens, page, hea
     keep = clean[~touched].float()
     # twice what rounding may cost: probabilities to bf16 in one computation and not in the other, values at most 5 (unit scale, these sizes)
     assert torch.isfinite(out[~touched]).all() and ((out[~touched].float() - keep).abs() <= 2.0**-8 * (5 + keep.abs())).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("counts,stored,page,heads,window", BOUNDARIES)
+def test_branches_that_end_inside_an_item_against_the_oracle(dev, counts, stored, page, heads, window, variant, monkeypatch):
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = branches(counts, stored, page, dev)
+    cache, q = fill(b, pages, heads, 17, dev)
+    out, lse = sa.paged_attn(q, cache, b, window=window or None, return_lse=True)
+    want, wlse, tol, ltol = reference(q, cache, b, heads[2] ** -0.5, window)
+    close(out, want, tol)
+    close(lse, wlse, ltol)
 
 
 @pytest.mark.gpu
