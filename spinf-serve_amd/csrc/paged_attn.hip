@@ -339,9 +339,10 @@ __device__ bool rubbish(const Params& p, const PagedItem& it, int vcol, int w, i
 }
 
 // One row of an item by a whole wave, from memory: what a workgroup falls back to for all its rows where a result is not finite.  A key's values are
-// touched only where the row sees the key.
+// touched only where the row sees the key.  ml: the row's reference and sum as the workgroup of the output's other dims has them, which need not fall back (its
+// values may be finite): a piece of a row has one reference for all dims.  (Values do not go into either: this workgroup's tile loop found the same.)
 template <int D, int DV, bool CAP>
-__device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol) {
+__device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol, const float2* ml = nullptr) {
     constexpr int VEC = DV / 64;   // output dims per lane
     const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
     const int c = it.L - it.T, tok = (it.row0 + j) / p.group, head = it.kvh * p.group + (it.row0 + j - tok * p.group);
@@ -398,9 +399,11 @@ __device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol) 
     }
     if (it.part >= 0) {
         float* dst = p.part_o + (long)(it.part + j) * D + vcol + VEC * lane;
+        const float2 piece = ml ? *ml : make_float2(M, l);
+        const float f = M == -INFINITY || piece.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - piece.x);
 #pragma unroll
-        for (int x = 0; x < VEC; x++) dst[x] = o[x];
-        if (lane == 0 && vcol == 0) p.part_ml[it.part + j] = make_float2(M, l);
+        for (int x = 0; x < VEC; x++) dst[x] = o[x] * f;
+        if (lane == 0 && vcol == 0) p.part_ml[it.part + j] = piece;
     } else {
         __bf16* dst = p.out + (long)(it.cu + tok) * p.o_tok + (long)head * p.o_head + vcol + VEC * lane;
         const float inv = inverse(l);
@@ -489,23 +492,31 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_wave_kernel(c
             tree = next_tree;
         }
     }
-    const int left = it.T * p.group - it.row0;   // rows from this group's first on
-    if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, vcol, w, NW, 1))) {
-        for (int j = w; j < 32 && it.row0 + j < it.T * p.group; j += NW) slow_row<D, DV, CAP>(p, it, j, vcol);
-        return;
-    }
-
     // ---- join the waves: every wave leaves its references and sums, then its accumulators scaled to the largest reference
+    const int left = it.T * p.group - it.row0;   // rows from this group's first on
     const float sum = lane32_sum(rows.l);
     if (sum == 0.f) rows.M = -INFINITY;   // no key seen
     if (rows.g == 0) ml[w][rows.m] = make_float2(rows.M, sum);
+    const bool again = __syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, vcol, w, NW, 1));
     __syncthreads();   // (and every wave is done with its tiles)
-    float top = -INFINITY, total = 0.f;
+    const auto joined = [&](int row) __attribute__((always_inline)) {   // a row's reference and sum
+        float top = -INFINITY, total = 0.f;
 #pragma unroll
-    for (int x = 0; x < NW; x++) top = fmaxf(top, ml[x][rows.m].x);
-    const float ref = top == -INFINITY ? 0.f : top;
+        for (int x = 0; x < NW; x++) top = fmaxf(top, ml[x][row].x);
+        const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int x = 0; x < NW; x++) total += ml[x][rows.m].y * (NW == 1 || ml[x][rows.m].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[x][rows.m].x - ref));
+        for (int x = 0; x < NW; x++) total += ml[x][row].y * (NW == 1 || ml[x][row].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[x][row].x - ref));
+        return make_float2(top, total);
+    };
+    if (again) {
+        for (int j = w; j < 32 && j < left; j += NW) {
+            const float2 state = joined(j);
+            slow_row<D, DV, CAP>(p, it, j, vcol, &state);
+        }
+        return;
+    }
+    const float2 state = joined(rows.m);
+    const float top = state.x, total = state.y, ref = top == -INFINITY ? 0.f : top;
     const float mine = NW == 1 || rows.M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(rows.M - ref);
     const float f = it.part < 0 ? mine * inverse(total) : mine;
     float* const stage = (float*)lds;

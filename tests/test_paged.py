@@ -490,6 +490,35 @@ def test_halves_leave_no_trace_of_unseen_keys(dev, q_lens, kv_lens, window, tree
     test_what_a_row_does_not_see_leaves_no_trace(dev, q_lens, kv_lens, 16, (4, 1, 512), window, tree, 2, monkeypatch)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("q_lens,kv_lens,page,hq,tree,variant", [
+    ([3], [700], 16, 4, None, 1), ([9, 2], [1100, 40], 48, 4, None, 1), ([8], [900], 16, 16, (2, 4), 1), ([60, 2], [3400, 40], 64, 4, None, 2),
+])
+def test_halves_of_pieces_with_rubbish_in_one_of_them(dev, q_lens, kv_lens, page, hq, tree, variant, half, bad, monkeypatch):
+    """keys cut into pieces, and a value that is not finite in one half of 512 dims alone: the rows that do not see it keep both halves"""
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = make_batch(q_lens, kv_lens, page, dev, tree)
+    cache, q = fill(b, pages, (hq, 1, 512), 41, dev)
+    assert b.plan(hq, 1, 512, 0)[1][3]
+    clean = sa.paged_attn(q, cache, b)
+    row = int(b.q_lens[0]) - 1
+    slot = int(b.rows()[0][row])
+    cache.v[slot // page, slot % page, 0, 256 * half : 256 * half + 256] = bad
+    out = sa.paged_attn(q, cache, b)
+    see = dense(b, 0)[0]
+    touched = np.zeros(b.tokens, bool)
+    touched[: see.shape[0]] = see[:, see.shape[1] - see.shape[0] + row]
+    touched = torch.from_numpy(touched).to(dev)
+    assert touched.any() and not touched.all()
+    keep = clean[~touched].float()
+    # as above: probabilities to bf16 in one computation and not in the other, values at most 5
+    assert torch.isfinite(out[~touched]).all() and ((out[~touched].float() - keep).abs() <= 2.0**-8 * (5 + keep.abs())).all()
+    halves = out[touched].unflatten(2, (2, 256))
+    assert not torch.isfinite(halves[:, :, half]).any() and torch.isfinite(halves[:, :, 1 - half]).all()
+
+
 def test_joins_cover_every_row_of_cut_keys():
     """share: groups of 16 lanes per row, a power of two, the fewest that ask for a row's pieces four at a time (16 at most)"""
     for n, hq, hkv, d in ((1100, 4, 1, 64), (3600, 8, 2, 128), (9000, 16, 1, 512), (40000, 3, 1, 64), (90000, 24, 4, 256)):
