@@ -891,7 +891,8 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     p.runs = (const PagedRun*)a->runs; p.joins = (const PagedJoin*)a->joins;
     p.part_o = (float*)a->workspace;
     p.part_ml = (float2*)(p.part_o + a->part_rows * a->d);
-    p.hq = a->hq; p.group = a->hq / a->hkv; p.window = a->window;
+    p.hq = a->hq; p.group = a->hq / a->hkv;
+    p.window = a->window < 1 << 30 ? a->window : 1 << 30;   // (no request is longer; a wider one would leave 32 bits where a tile's first key is subtracted)
     p.page = PageDiv::of_page(a->page);
     p.c = a->scale * LOG2E;
     p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;

@@ -65,6 +65,19 @@ class PagedCache:
         return cls(k, v)
 
 
+LONGEST = 1 << 30   # stored keys of a request
+
+
+def _whole(x, what) -> int:
+    try:
+        n = int(x)
+    except OverflowError:
+        n = None
+    if n is None or n != x:
+        raise ValueError(f"{what} {x}: a whole number is needed")
+    return n
+
+
 def _lengths(x, what):
     a = np.ascontiguousarray(x, np.int64).reshape(-1)
     if len(a) and (a.min() < 0 or a.max() > 1 << 30):
@@ -289,10 +302,11 @@ def _check_call(q, k, v, tokens, page, max_page, what):
 
 
 def _window(window) -> int:
-    w = int(window) if window is not None else 0
+    """(a window as wide as the longest request may be hides nothing: wider ones are that one, and any of them fits the library's 32 bits)"""
+    w = _whole(window, "window") if window is not None else 0
     if w < 0:
         raise ValueError(f"window {w}")
-    return w
+    return min(w, LONGEST)
 
 
 def _fill(a, q, k, v, page, window, scale, softcap):

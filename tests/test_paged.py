@@ -305,6 +305,18 @@ def test_attention_refuses_tensors_before_any_launch():
         sa.paged_attn(q, c, b, window=-3)
 
 
+def test_windows_of_any_width_are_taken_for_what_they_are():
+    b, _ = make_batch([70, 2], [300, 130], 16)
+    none = b.plan(4, 2, 128, paged._window(None))
+    for window in (1 << 30, 2**31 - 1, 2**31, 2**32 + 5, 2**70, np.int64(2**40), float(2**40)):
+        lists, counts, at = b.plan(4, 2, 128, paged._window(window))
+        assert counts == none[1] and torch.equal(lists, none[0]), window
+    assert paged._window(5) == paged._window(np.int32(5)) == paged._window(5.0) == 5 and paged._window(0) == 0
+    for window in (-1, -(2**32) + 5, 2.5, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            paged._window(window)
+
+
 # ------------------------------------------------------------------------------------------------ attention on the GPU
 def fill(batch, pages, heads, seed, device, peaky=True, order="heads"):
     """cache and queries of unit scale; order of the cache's memory: a head's rows of a page together, or a row's heads"""
@@ -565,6 +577,24 @@ def test_scores_that_range_widely(dev, variant, monkeypatch):
     want, wlse, tol, ltol = reference(q, cache, b, 128**-0.5)
     close(out, want, tol)
     close(lse, wlse, ltol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+def test_a_window_wider_than_every_request_is_none(dev, variant, monkeypatch):
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = make_batch([70, 2], [300, 130], 16, dev)
+    cache, q = fill(b, pages, (4, 2, 128), 46, dev)
+    want, lse = sa.paged_attn(q, cache, b, return_lse=True)
+    weight = sa.paged_weights(q, cache, b, lse)
+    for window in (1 << 30, 2**31 - 30, 2**31 - 1, 2**31, 2**32 + 5):
+        assert torch.equal(sa.paged_attn(q, cache, b, window=window), want), window
+        got = sa.paged_weights(q, cache, b, lse, window=window)
+        assert torch.equal(got, weight), window
+    # the C entry by itself, with the widest window that its 32 bits hold
+    lists, counts, at = b.plan(4, 2, 128, 1 << 30)
+    a = paged._attn_block(q, cache.k, cache.v, *b.device_data(), lists, counts, at, 16, b.max_page, b.tokens, 128**-0.5, 2**31 - 1, 0.0)
+    assert torch.equal(paged._attn_run(a, q, cache.k, cache.v, False)[0], want)
 
 
 # ------------------------------------------------------------------------------------------------ weights
