@@ -535,8 +535,8 @@ def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, kee
                     if stream not in shared.streams:
                         shared.reach(stream)
                 return _evict_run(_lib.EvictArgs.from_buffer_copy(got[0]), k, v, acc, new[1], new[0], stream)
-    keep, sink, recent = int(keep), int(sink), int(recent)
-    if sink < 0 or recent < 0 or sink + recent > keep:
+    keep, sink, recent = (_whole(x, f"cache_evict: {name}") for x, name in ((keep, "keep"), (sink, "sink"), (recent, "recent")))
+    if sink < 0 or recent < 0 or sink + recent > keep or keep > LONGEST:
         raise ValueError(f"cache_evict: keep {keep}, of these the first {sink} and the last {recent}")
     if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[0] != R or acc.shape[1] != hkv or not acc.is_contiguous():
         raise ValueError(f"cache_evict: acc must be contiguous fp32 [{R}, {hkv}, keys]")

@@ -686,6 +686,18 @@ def test_weights_and_eviction_refuse_bad_arguments():
             sa.cache_evict(c, b, into, *args)
 
 
+def test_eviction_refuses_counts_that_32_bits_or_whole_numbers_do_not_hold():
+    b, pages = make_batch([2, 1], [40, 20], 16)
+    c = sa.PagedCache.empty(pages + 4, 16, 2, 64, "cpu")
+    into = sa.PagedBatch.build([0, 0], [40, 16], [[pages, pages + 1, pages + 2], [pages + 3]], 16, "cpu")
+    acc = torch.zeros((2, 2, 40))
+    with pytest.raises(RuntimeError, match="ROCm"):   # (all is well but the device)
+        sa.cache_evict(c, b, into, acc, 16.0, np.int64(4), 4)
+    for args in ((2**32 + 16, 4, 4), (2**30 + 1, 4, 4), (16, 2**32 + 4, 4), (16, 4, 2**32), (2**40, 2**32, 2**32), (16.5, 4, 4), (16, 0.5, 4), (16, 4, 3.5), (float("inf"), 0, 0)):
+        with pytest.raises(ValueError):
+            sa.cache_evict(c, b, into, acc, *args)
+
+
 # ------------------------------------------------------------------------------------------------ eviction
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["plain", "ties", "equal", "wild"])
