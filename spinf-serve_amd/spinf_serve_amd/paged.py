@@ -78,9 +78,21 @@ def _whole(x, what) -> int:
     return n
 
 
+def _wholes(x, what):
+    """-> int64 array of these values, which have to be whole numbers"""
+    a = np.asarray(x).reshape(-1)
+    if a.dtype.kind not in "iub":
+        f = np.asarray(a, np.float64)
+        if not (np.abs(f) < 2.0**63).all() or (f != np.floor(f)).any():
+            raise ValueError(f"{what} must be whole numbers")
+    elif a.dtype == np.uint64 and (a >> np.uint64(63)).any():
+        raise ValueError(f"{what} must be whole numbers of 64 bits")
+    return np.ascontiguousarray(a, np.int64)
+
+
 def _lengths(x, what):
-    a = np.ascontiguousarray(x, np.int64).reshape(-1)
-    if len(a) and (a.min() < 0 or a.max() > 1 << 30):
+    a = _wholes(x, what)
+    if len(a) and (a.min() < 0 or a.max() > LONGEST):
         raise ValueError(f"{what} must lie in 0 .. 2^30")
     return a.astype(np.int32)
 
@@ -110,9 +122,9 @@ class PagedBatch:
     def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None) -> "PagedBatch":
         """tables: per request its pages (a list or a row of an integer array; entries behind the stored keys are ignored).  Host data only."""
         q_lens, kv_lens = _lengths(q_lens, "q_lens"), _lengths(kv_lens, "kv_lens")
-        page = int(page)
-        if page < 16 or page % 16:
-            raise ValueError(f"pages of {page} keys: a multiple of 16 is needed")
+        page = _whole(page, "page")
+        if page < 16 or page % 16 or page > 1 << 20:
+            raise ValueError(f"pages of {page} keys: a multiple of 16 is needed, at most 2^20")
         if len(q_lens) != len(kv_lens) or len(tables) != len(kv_lens):
             raise ValueError(f"{len(q_lens)} q_lens, {len(kv_lens)} kv_lens and {len(tables)} tables")
         need = -(-kv_lens.astype(np.int64) // page)
@@ -122,7 +134,7 @@ class PagedBatch:
         if (end is None) != (pos is None):
             raise ValueError("a tree needs both end and pos")
         if end is not None:
-            end, pos = (np.ascontiguousarray(x, np.int64).reshape(-1) for x in (end, pos))
+            end, pos = _wholes(end, "end"), _wholes(pos, "pos")
             tokens = int(q_lens.sum(dtype=np.int64))
             if len(end) != tokens or len(pos) != tokens:
                 raise ValueError(f"end and pos hold {len(end)} and {len(pos)} values for {tokens} new tokens")

@@ -252,6 +252,19 @@ def test_batches_that_make_no_sense_are_refused(bad):
         sa.PagedBatch.build(**{**good, **bad}, device="cpu")
 
 
+@pytest.mark.parametrize("bad", [
+    dict(q_lens=[1.5, 1]), dict(kv_lens=[20, 6.9]), dict(kv_lens=[float("nan"), 6]), dict(kv_lens=[float("inf"), 6]), dict(kv_lens=[2**32 + 20, 6]), dict(q_lens=[2**64 - 1, 1]),
+    dict(kv_lens=np.array([2**63 + 20, 6], np.uint64)), dict(end=[1, 1.5]), dict(pos=[18.5, 5]), dict(page=16.5), dict(page=2**32 + 16), dict(page=(1 << 20) + 16),
+])
+def test_numbers_that_would_be_cut_are_refused(bad):
+    good = dict(q_lens=[1, 1], kv_lens=[20, 6], tables=[[0, 1], [2]], page=16, end=[1, 2], pos=[19, 5])
+    a = sa.PagedBatch.build(**good, device="cpu")
+    b = sa.PagedBatch.build(**{**good, "q_lens": torch.tensor([1, 1]), "kv_lens": np.array([20.0, 6.0]), "page": np.int64(16), "end": np.array([1, 2], np.uint8)}, device="cpu")
+    assert a.rows()[0].tolist() == b.rows()[0].tolist() and b.kv_lens.tolist() == [20, 6]
+    with pytest.raises(ValueError):
+        sa.PagedBatch.build(**{**good, **bad}, device="cpu")
+
+
 def test_caches_that_the_kernels_do_not_take_are_refused():
     k = torch.zeros((4, 16, 2, 64), dtype=BF16)
     sa.PagedCache(k, k)
