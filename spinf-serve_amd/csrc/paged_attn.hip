@@ -50,7 +50,7 @@ struct Params {
     float* part_o; float2* part_ml;
     int n_items, hq, group, window;
     PageDiv page;
-    float c, cap_in, cap_out;                        // scale log2 e; with a cap: 2 scale log2 e / cap and cap log2 e
+    SoftCap cap;
 };
 
 __device__ __forceinline__ PagedItem load_item(const PagedItem* items, int i) {
@@ -195,8 +195,6 @@ struct Rows {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // (a capped score of -inf is minus the cap and has its weight: it must not be taken for a masked one)
-    static __device__ __forceinline__ float seen(float s) { return CAP && s == -INFINITY ? -3.4e38f : s; }
     // (four keys at a time, a scheduling barrier in between: requested all at once, the keys' ends and positions would cost the tile loop its registers)
     __device__ __forceinline__ void mask(const Params& p, const PagedItem& it, int kt, const int* meta, bool tree, f32x16& s) {
         const int u0 = kt * TK - (it.L - it.T) + 4 * g;   // key 8 i4 + j of this lane is new token u0 + 8 i4 + j of the request (below 0: stored before)
@@ -207,7 +205,7 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int k = 8 * (i >> 2) + (i & 3);
-                s[i] = (k <= last) & (k > first) ? seen(s[i]) : -INFINITY;
+                s[i] = (k <= last) & (k > first) ? s[i] : -INFINITY;
             }
         } else {
             const int row = it.cu + tok;
@@ -222,21 +220,21 @@ struct Rows {
                     const bool fresh = u0 + k >= 0;
                     bool vis = (u0 + k <= tok) & (!fresh | (row < ev[j]));
                     if (p.window) vis = vis & ((fresh ? qpos - pv[j] : far - k) < sees);
-                    s[4 * i4 + j] = vis ? seen(s[4 * i4 + j]) : -INFINITY;
+                    s[4 * i4 + j] = vis ? s[4 * i4 + j] : -INFINITY;
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    // scores -> probabilities.  The reference stays while no score lies more than TAU above it, which one comparison per lane with `over` (the score that
+    // scores (with a cap: their tanh) -> probabilities.  The reference stays while no score lies more than TAU above it, which one comparison per lane with `over` (the score that
     // far above, in the scores' own units) tells; where one does, or a row meets its first keys, it is raised and what was summed is rescaled.
-    __device__ __forceinline__ void softmax(const Params& p, f32x16& s, bool masked, bf16x8 (&pb)[2]) {
+    __device__ __forceinline__ void softmax(const Params& p, f32x16& s, bf16x8 (&pb)[2]) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, s[i]);
         if (__builtin_amdgcn_ballot_w64(mx > over) != 0) {
             mx = lane32_max(mx);
-            const float t = CAP ? cap(p, mx) : mx * p.c;
+            const float t = mx * p.cap.unit;
             const bool fresh = over == -INFINITY, up = mx > -INFINITY && (fresh || t > M + TAU);
             const float alpha = up && !fresh ? __builtin_amdgcn_exp2f(M - t) : 1.0f;
             if (__builtin_amdgcn_ballot_w64(up && !fresh) != 0) {   // (rows without a key so far hold zeros)
@@ -247,30 +245,17 @@ struct Rows {
             }
             l *= alpha;
             M = up ? t : M;
-            if (CAP) {   // the inverse of the cap: y / cap = tanh(x / cap); nothing lies above the cap itself
-                const float y = (M + TAU) / p.cap_out;
-                over = up ? (y < 1.f ? __builtin_amdgcn_logf((1.f + y) / (1.f - y)) / p.cap_in : INFINITY) : over;
-            } else {
-                over = up ? (M + TAU) / p.c : over;
-            }
+            over = up ? (M + TAU) / p.cap.unit : over;
         }
         float sum = 0.f;
-        const float shift = p.cap_out - M;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            float pr;
-            if (CAP) {   // cap_out tanh - M = (cap_out - M) - 2 cap_out / (exp(2 x) + 1)
-                pr = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * p.cap_in) + 1.0f), -2.0f * p.cap_out, shift));
-                if (masked) pr = s[i] == -INFINITY ? 0.f : pr;
-            } else {
-                pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.c, -M));
-            }
+            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.cap.unit, -M));
             sum += pr;
             pb[i >> 3][i & 7] = (__bf16)pr;
         }
         l += sum;
     }
-    static __device__ __forceinline__ float cap(const Params& p, float s) { return p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f)); }
     __device__ __forceinline__ void values(const char* vt_lds, const bf16x8 (&pb)[2]) {
         const int tr_a = lane & 3, tr_j = (lane >> 2) & 3, tr_mb = (lane >> 4) & 1;
         const char* vrow = vt_lds + GV::v_off(4 * g + tr_j) + 32 * tr_mb + 8 * tr_a;
@@ -371,9 +356,7 @@ __device__ void slow_row(const Params& p, const PagedItem& it, int j, int vcol, 
             for (int x = 0; x < 8; x++) s = __builtin_fmaf((float)a[x], (float)b[x], s);
         }
         s = lane32_sum(s);
-        float t = s * p.c;
-        if (CAP) t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.cap_in) + 1.0f));
-        t = vis ? t : -INFINITY;
+        const float t = vis ? (CAP ? p.cap.of(s) : s) * p.cap.unit : -INFINITY;
         float mx = t;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
@@ -471,6 +454,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_wave_kernel(c
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(NV));   // the keys (and ends, positions) are there; the values may still be on their way
             __builtin_amdgcn_sched_barrier(0);
             rows.scores(kb, s);
+            if (CAP) p.cap.of(s);
             if (masked) rows.mask(p, it, kt, meta, tree, s);
             __builtin_amdgcn_s_waitcnt(LGKM0);           // nothing reads the tile's keys any more
             __builtin_amdgcn_sched_barrier(0);
@@ -480,7 +464,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_wave_kernel(c
                 fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
             }
             bf16x8 pb[2];
-            rows.softmax(p, s, masked, pb);
+            rows.softmax(p, s, pb);
             if (!next) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
             else if (next_tree) __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK + 2));
             else __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK));
@@ -698,9 +682,10 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void paged_block
                 s[4 * i4 + 3] += x.w;
             }
         }
+        if (CAP) p.cap.of(s);
         if (masked) rows.mask(p, it, kt, (const int*)(lds + buf * BUF + GK::KTILEB + GV::VTILEB), tree, s);
         bf16x8 pb[2];
-        rows.softmax(p, s, masked, pb);
+        rows.softmax(p, s, pb);
         rows.values(kb + GK::KTILEB, pb);
         kt = kt_next;
         bits = bits_next;
@@ -853,7 +838,7 @@ int launch(Params p, const spinf_paged_args* a, hipStream_t s) {
 
 template <int D, int DV, int NW>
 int launch_cap(const Params& p, const spinf_paged_args* a, hipStream_t s) {
-    return a->softcap > 0.f ? launch<D, DV, NW, true>(p, a, s) : launch<D, DV, NW, false>(p, a, s);
+    return p.cap.on ? launch<D, DV, NW, true>(p, a, s) : launch<D, DV, NW, false>(p, a, s);
 }
 
 }  // namespace
@@ -894,9 +879,7 @@ extern "C" int spinf_paged_attn_fwd(const spinf_paged_args* a, void* stream) {
     p.hq = a->hq; p.group = a->hq / a->hkv;
     p.window = a->window < 1 << 30 ? a->window : 1 << 30;   // (no request is longer; a wider one would leave 32 bits where a tile's first key is subtracted)
     p.page = PageDiv::of_page(a->page);
-    p.c = a->scale * LOG2E;
-    p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
-    p.cap_out = a->softcap * LOG2E;
+    if (!SoftCap::of(a->scale, a->softcap, p.cap)) return spinf_fail(SPINF_E_ARG, "paged_attn: scale %g and softcap %g leave fp32's range", (double)a->scale, (double)a->softcap);
     hipStream_t s = (hipStream_t)stream;
     switch (a->d) {
         case 64: return launch_cap<64, 64, 4>(p, a, s);

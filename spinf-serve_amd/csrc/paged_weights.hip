@@ -30,7 +30,7 @@ struct Params {
     int blocks, hq, hkv, window;
     Div group;   // query heads per key / value head
     PageDiv page;
-    float c, cap_in, cap_out;
+    SoftCap cap;
 };
 
 // Rows of up to NW blocks of 32 as the products need them: log-sums in units of log 2 (infinite: the row gives no weight), tokens, positions
@@ -103,7 +103,8 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
             rd.pos[slot][m] = p.window ? (p.end ? p.pos[cu + tok] : c + tok) : 0;
         };
         // weights of a block's rows; s: its scores, register i of which holds row 8 (i / 4) + 4 g + i % 4; first: the block's first token
-        const auto add = [&](const f32x16& s, int slot, int first) __attribute__((always_inline)) {
+        const auto add = [&](f32x16& s, int slot, int first) __attribute__((always_inline)) {
+            if (CAP) p.cap.of(s);
             const bool masked = u_hi > first || p.window || p.end;
 #pragma unroll
             for (int i4 = 0; i4 < 4; i4++) {
@@ -117,9 +118,7 @@ __global__ __launch_bounds__(64 * NW) void paged_weights_kernel(const Params p) 
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    float t = s[4 * i4 + j];
-                    if (CAP) t = p.cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(t * p.cap_in) + 1.0f));
-                    const float x = __builtin_amdgcn_exp2f(CAP ? t - lv[j] : __builtin_fmaf(t, p.c, -lv[j]));
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + j], p.cap.unit, -lv[j]));
                     bool vis = true;
                     if (masked) {
                         vis = (u <= tv[j]) & (cu + tv[j] < end_k);
@@ -195,7 +194,7 @@ int launch(Params p, const spinf_paged_weights_args* a, hipStream_t s) {
     if (n > INT32_MAX) return spinf_fail(SPINF_E_ARG, "paged_weights: %lld requests of %ld keys are too many", (long long)a->n_reqs, p.keys);
     p.blocks = (int)blocks;
     const dim3 grid((unsigned)n), threads(64 * NW);
-    const bool cap = a->softcap > 0.f, few = (int64_t)a->max_q * p.group.d <= 32;
+    const bool cap = p.cap.on, few = (int64_t)a->max_q * p.group.d <= 32;
     if (cap && few) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true, true>), grid, threads, 0, s, p);
     else if (cap) hipLaunchKernelGGL((paged_weights_kernel<D, NW, true, false>), grid, threads, 0, s, p);
     else if (few) hipLaunchKernelGGL((paged_weights_kernel<D, NW, false, true>), grid, threads, 0, s, p);
@@ -230,9 +229,7 @@ extern "C" int spinf_paged_weights(const spinf_paged_weights_args* a, void* stre
     p.table = a->table; p.reqs = a->reqs; p.end = a->end; p.pos = a->pos;
     p.keys = a->keys; p.hq = a->hq; p.hkv = a->hkv; p.group = Div::by(a->hq / a->hkv); p.window = a->window;
     p.page = PageDiv::of_page(a->page);
-    p.c = a->scale * LOG2E;
-    p.cap_in = a->softcap > 0.f ? 2.0f * LOG2E * a->scale / a->softcap : 0.f;
-    p.cap_out = a->softcap * LOG2E;
+    if (!SoftCap::of(a->scale, a->softcap, p.cap)) return spinf_fail(SPINF_E_ARG, "paged_weights: scale %g and softcap %g leave fp32's range", (double)a->scale, (double)a->softcap);
     hipStream_t s = (hipStream_t)stream;
     switch (a->d) {
         case 64: return launch<64, 4>(p, a, s);

@@ -610,6 +610,103 @@ def test_a_window_wider_than_every_request_is_none(dev, variant, monkeypatch):
     assert torch.equal(paged._attn_run(a, q, cache.k, cache.v, False)[0], want)
 
 
+CAPS = [0.5, 3.0, 30.0, 50.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e30, 2e38]
+
+
+def capped(q, cache, batch, scale, softcap):
+    """as `reference`, with no more allowed than the scores' own digits: the cap's tanh is off by some 2^-22 of a score, taken as 2^-20"""
+    qn, kn, vn = (t.float().cpu().numpy() for t in (q, cache.k, cache.v))
+    out, lse, tol, ltol = [], [], [], []
+    base = 0
+    for r, see in enumerate(dense(batch, 0)):
+        T, L = see.shape
+        at = int(batch._need[:r].sum())
+        table = batch._table[at : at + batch._need[r]]
+        o, s, mag, size = op.attention(qn[base : base + T].astype(np.float64), op.stored(kn, table, L), op.stored(vn, table, L), see, scale, softcap)
+        terr = size * ((qn.shape[2] + 4) * 2.0**-24 + 2.0**-20) + 2.0**-20
+        out.append(o)
+        lse.append(s)
+        tol.append(1.02 * (2.0**-8 * (mag + np.abs(o)) + mag * (2 * terr[..., None] + (L + 64) * 2.0**-24)) + 1e-30)
+        ltol.append(terr + (L + 64) * 2.0**-24 + np.where(np.isfinite(s), np.abs(s), 0) * 2.0**-22)
+        base += T
+    return tuple(np.concatenate(x) for x in (out, lse, tol, ltol))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("softcap", CAPS)
+@pytest.mark.parametrize("heads", [(4, 2, 128), (4, 1, 512), (8, 2, 64), (4, 2, 256)])
+def test_caps_of_every_size(dev, softcap, variant, heads, monkeypatch):
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    b, pages = make_batch([1, 40], [900, 130], 64, dev)
+    cache, q = fill(b, pages, heads, 43, dev)
+    out, lse = sa.paged_attn(q, cache, b, softcap=softcap, return_lse=True)
+    want, wlse, tol, ltol = capped(q, cache, b, heads[2] ** -0.5, softcap)
+    close(lse, wlse, ltol)
+    close(out, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softcap", CAPS)
+def test_weights_under_caps_of_every_size(dev, softcap):
+    b, pages = make_batch([3, 40], [900, 130], 64, dev)
+    heads = (4, 2, 128)
+    cache, q = fill(b, pages, heads, 44, dev)
+    scale = heads[2] ** -0.5
+    lse = torch.from_numpy(capped(q, cache, b, scale, softcap)[1].astype(np.float32)).to(dev)
+    got = sa.paged_weights(q, cache, b, lse, softcap=softcap)
+    qn, kn, ln = q.double().cpu().numpy(), cache.k.float().cpu().numpy(), lse.double().cpu().numpy()
+    base = 0
+    for r, see in enumerate(dense(b, 0)):
+        T, L = see.shape
+        at = int(b._need[:r].sum())
+        k = op.stored(kn, b._table[at : at + b._need[r]], L)
+        rows = slice(base, base + T)
+        want = op.weights(qn[rows], k, see, ln[rows], scale, softcap)
+        size = max(float((np.abs(qn[rows, h]) @ np.abs(k[:, h // 2]).T).max()) for h in range(4)) * scale
+        rel = size * ((heads[2] + 4) * 2.0**-24 + 2.0**-20) + (T * 2 + 40) * 2.0**-24 + 2.0**-20
+        close(got[r, :, :L], want, rel * want + 1e-30)
+        base += T
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("softcap", [0.5, 2.0])
+def test_infinite_scores_weigh_what_the_cap_leaves_them(dev, softcap, variant, monkeypatch):
+    """keys of -inf, a request's first page of them: scores of minus the cap, seen like others"""
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    heads = (4, 2, 128)
+    b, pages = make_batch([2, 40], [130, 90], 32, dev)
+    cache, q = fill(b, pages, heads, 45, dev)
+    q = q.abs() + 0.01
+    for r in range(2):
+        cache.k[int(b._table[int(b._need[:r].sum())])] = float("-inf")
+    out, lse = sa.paged_attn(q, cache, b, softcap=softcap, return_lse=True)
+    qn, kn, vn = (t.float().cpu().numpy().astype(np.float64) for t in (q, cache.k, cache.v))
+    base = 0
+    for r, see in enumerate(dense(b, 0)):
+        T, L = see.shape
+        at = int(b._need[:r].sum())
+        table = b._table[at : at + b._need[r]]
+        rows = slice(base, base + T)
+        o, s, mag, _ = op.attention(qn[rows], op.stored(kn, table, L), op.stored(vn, table, L), see, 128**-0.5, softcap)
+        # scores of at most 2: their errors are far below 2^-16
+        close(out[rows], o, 1.02 * 2.0**-8 * (mag + np.abs(o)) + mag * 2.0**-14)
+        close(lse[rows], s, 2.0**-15 + 0 * s)
+        base += T
+
+
+@pytest.mark.gpu
+def test_scales_and_caps_outside_the_range_are_refused(dev):
+    b, pages = make_batch([2], [20], 16, dev)
+    cache, q = fill(b, pages, (4, 2, 64), 0, dev)
+    for bad in (dict(scale=3e38), dict(softcap=1e-39, scale=1.0), dict(softcap=float("inf")), dict(softcap=float("nan"))):
+        with pytest.raises(ValueError):
+            sa.paged_attn(q, cache, b, **bad)
+        with pytest.raises(ValueError):
+            sa.paged_weights(q, cache, b, torch.zeros((2, 4), device=dev), **bad)
+
+
 # ------------------------------------------------------------------------------------------------ weights
 WEIGHTS = [  # q_lens, kv_lens, page, (hq, hkv, d), window, softcap, tree
     ([1, 1, 0, 1], [1, 700, 33, 32], 16, (8, 2, 128), 0, 0.0, None),
