@@ -3,7 +3,8 @@ come later, goes on token by token, and trims what it keeps.
 
     python examples/paged_session.py        (needs an MI355X and the built library)
 
-Every step is checked against tree_attn over the same tokens packed into one stream, i.e. against reading the documents anew.
+Every step is checked: against tree_attn over the same tokens packed into one stream, i.e. against reading the documents anew, and what follows the trimming
+against plain attention over the keys that stayed.
 """
 
 from __future__ import annotations
@@ -47,6 +48,22 @@ class Layer:
         pos = torch.from_numpy(stream.pos.astype(np.int64)).to(x.device)
         q, k = sa.qk_norm_rope(q, k, self.wq, self.wk, self.cos, self.sin, 1e-6, pos)
         return sa.tree_attn(q, k, v, sa.block_masks(stream, None, device=x.device)["full_attention"], D**-0.5)
+
+    def trimmed(self, text, asks, question, stay):
+        """one text's questions (branches of question[i] tokens) over the keys that stayed [kv heads, keys], rotated by the positions they were read at"""
+        q, k, v = self.project(torch.cat([text, asks]))
+        at = [*range(len(text)), *(len(text) + i for b in question for i in range(b))]
+        q, k = sa.qk_norm_rope(q, k, self.wq, self.wk, self.cos, self.sin, 1e-6, torch.tensor(at, device=text.device))
+        out, first = [], len(text)
+        for b in question:
+            new = slice(first, first + b)
+            for h in range(HQ):
+                kk, vv = (torch.cat([t[stay[h // (HQ // HKV)], h // (HQ // HKV)], t[new, h // (HQ // HKV)]]).float() for t in (k, v))
+                s = (q[new, h].float() @ kk.T) * D**-0.5
+                s += torch.full_like(s, float("-inf")).triu(1 + kk.shape[0] - b)
+                out.append(s.softmax(1) @ vv)
+            first += b
+        return torch.cat([torch.stack(out[i : i + HQ], 1) for i in range(0, len(out), HQ)])
 
 
 def main(device="cuda", documents=(700, 333), questions=((7, 12, 9), (5, 16)), steps=3, keep=256):
@@ -107,17 +124,23 @@ def main(device="cuda", documents=(700, 333), questions=((7, 12, 9), (5, 16)), s
         off["steps"] = max(off.get("steps", 0.0), float((layer.anew(padded, stream)[ends] - out).abs().max()))
     off["weights"] = float((weight.sum(2) - steps * HQ / HKV).abs().max())   # each token gave every head's weight away, one in all
 
-    # 4. the documents are trimmed to the keys that were looked at; the old pages are free again
-    fresh = [[free.pop() for _ in range(-(-(min(n, keep) + 1) // PAGE))] for n in lens]
-    into = sa.PagedBatch.build([0] * len(lens), [min(n, keep) for n in lens], fresh, PAGE, device)
+    # 4. the documents are trimmed to the keys that were looked at, and the old pages are free again; questions go on from where the texts are, below what is left of them
+    fresh = [[free.pop() for _ in range(-(-(min(n, keep) + sum(q)) // PAGE))] for n, q in zip(lens, questions)]
+    left = [min(n, keep) for n in lens]
+    into = sa.PagedBatch.build([0] * len(lens), left, fresh, PAGE, device)
     kept, weight = sa.cache_evict(cache, batch, into, weight, keep, sink=4, recent=32)
-    lens = [min(n, keep) + 1 for n in lens]
-    q, k, v = layer.project(rand(len(lens)))
-    batch = sa.PagedBatch.build([1] * len(lens), lens, fresh, PAGE, device)
-    place = torch.tensor([n + steps for n in documents], device=device)        # (a rotated key keeps its position: so does the next token)
-    q = sa.qk_norm_rope_put(q, k, v, layer.wq, layer.wk, layer.cos, layer.sin, 1e-6, cache, batch.rows()[0], pos=place)
-    out = sa.paged_attn(q, cache, batch)
-    assert torch.isfinite(out).all() and int((kept >= 0).sum()) == HKV * sum(n - 1 for n in lens)
+    asks = [rand(sum(q)) for q in questions]
+    end, pos, base = [], [], 0
+    for n, q in zip(lens, questions):
+        for b in q:
+            end += [base + b] * b
+            pos += range(n, n + b)                                             # (positions in the text, of which n - left tokens are gone)
+            base += b
+    batch = sa.PagedBatch.build([sum(q) for q in questions], [n + sum(q) for n, q in zip(left, questions)], fresh, PAGE, device, end=end, pos=pos,
+                                dropped=[n - m for n, m in zip(lens, left)])
+    _, out = layer.paged(torch.cat(asks), cache, batch)
+    want = [layer.trimmed(t, a, q, stay[:, :m]) for t, a, q, stay, m in zip(texts, asks, questions, kept.long(), left)]
+    off["trimmed"] = float((torch.cat(want) - out).abs().max())
     return off
 
 

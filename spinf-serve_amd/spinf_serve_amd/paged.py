@@ -105,13 +105,17 @@ class PagedBatch:
     subtree in rows of the call, pos[t] = its position (at most its place among the stored keys).  A row sees all keys stored before the new tokens, and
     of these the ones whose subtree it lies in.
 
+    A request that cache_evict has trimmed stores fewer keys than its text has tokens, rotated by the positions they had.  dropped[r] says how many are gone: its new tokens'
+    positions are their places plus that (of a tree, what pos says: the same at most).  A window counts places, so a call over such a batch takes none.
+
     Host threads and streams may share a batch: what a first call makes is made once, and a call on another stream waits for the copies."""
 
-    def __init__(self, q_lens, kv_lens, table, need, page, device, end, pos):
+    def __init__(self, q_lens, kv_lens, table, need, page, device, end, pos, dropped=None):
+        """pos: counted in places, without what was dropped"""
         self._lock = threading.RLock()
         self.q_lens, self.kv_lens, self.page, self.device = q_lens, kv_lens, page, device
         self._table, self._need = table, need       # the pages back to back, and how many each request has
-        self._end, self._pos = end, pos
+        self._end, self._pos, self._dropped = end, pos, dropped
         self.tokens = int(q_lens.sum(dtype=np.int64))
         self.max_page = int(table.max()) if len(table) else -1
         self.longest = int(kv_lens.max(initial=0))
@@ -119,7 +123,7 @@ class PagedBatch:
         self._calls = {}    # argument blocks without their tensors' addresses, by the tensors' shapes and strides and the call's numbers
 
     @classmethod
-    def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None) -> "PagedBatch":
+    def build(cls, q_lens, kv_lens, tables, page, device="cuda", end=None, pos=None, dropped=None) -> "PagedBatch":
         """tables: per request its pages (a list or a row of an integer array; entries behind the stored keys are ignored).  Host data only."""
         q_lens, kv_lens = _lengths(q_lens, "q_lens"), _lengths(kv_lens, "kv_lens")
         page = _whole(page, "page")
@@ -131,6 +135,11 @@ class PagedBatch:
         table = cls._pages(tables, need, kv_lens, page)
         if len(table) and (table.min() < 0 or table.max() >= 1 << 31):
             raise ValueError("page numbers must lie in 0 .. 2^31 - 1")
+        if dropped is not None:
+            dropped = _lengths(dropped, "dropped")
+            if len(dropped) != len(kv_lens):
+                raise ValueError(f"{len(dropped)} values of dropped for {len(kv_lens)} requests")
+            dropped = dropped if dropped.any() else None
         if (end is None) != (pos is None):
             raise ValueError("a tree needs both end and pos")
         if end is not None:
@@ -140,12 +149,14 @@ class PagedBatch:
                 raise ValueError(f"end and pos hold {len(end)} and {len(pos)} values for {tokens} new tokens")
             if (q_lens > kv_lens).any():
                 raise ValueError("a tree's new tokens are among the stored keys: q_lens must not exceed kv_lens")
+            if dropped is not None:
+                pos = pos - np.repeat(dropped, q_lens)
             if tokens:
                 at = np.arange(tokens) - np.repeat(np.cumsum(q_lens, dtype=np.int64) - kv_lens, q_lens)
                 if end.min() < 0 or end.max() > tokens or pos.min() < 0 or (pos > at).any():
-                    raise ValueError("end must lie in 0 .. tokens, pos in 0 .. the token's place among the stored keys")
+                    raise ValueError("end must lie in 0 .. tokens, pos (less what was dropped) in 0 .. the token's place among the stored keys")
             end, pos = end.astype(np.int32), pos.astype(np.int32)
-        return cls(q_lens, kv_lens, table.astype(np.int32), need, page, torch.device(device), end, pos)
+        return cls(q_lens, kv_lens, table.astype(np.int32), need, page, torch.device(device), end, pos, dropped)
 
     @staticmethod
     def _pages(tables, need, kv_lens, page):
@@ -164,7 +175,7 @@ class PagedBatch:
     def __reduce__(self):
         """copied and saved as what it is built from"""
         tables = np.split(self._table, np.cumsum(self._need)[:-1]) if len(self._need) else []
-        return PagedBatch.build, (self.q_lens, self.kv_lens, tables, self.page, str(self.device), self._end, self._pos)
+        return PagedBatch.build, (self.q_lens, self.kv_lens, tables, self.page, str(self.device), self._end, self._positions() if self._pos is not None else None, self._dropped)
 
     def _reach(self, shared):
         if shared.device.type == "cuda":
@@ -229,9 +240,18 @@ class PagedBatch:
             raise ValueError("cache_evict: a page to be written twice, or one that is read")
         self._moves[keep] = weakref.ref(into)
 
+    def _positions(self):
+        """of the new tokens, in their texts"""
+        if self._pos is None:
+            base = np.cumsum(self.q_lens, dtype=np.int64) - self.kv_lens
+            pos = np.maximum(np.arange(self.tokens) - np.repeat(base, self.q_lens), 0).astype(np.int32)
+        else:
+            pos = self._pos
+        return pos if self._dropped is None else pos + np.repeat(self._dropped, self.q_lens)
+
     def rows(self):
         """-> (slots, positions) of the new tokens, device tensors int64 and int32: where the rows' keys and values go in the cache (page * page size +
-        entry; -1 where a request has fewer stored keys than new tokens), and the rows' positions"""
+        entry; -1 where a request has fewer stored keys than new tokens), and the rows' positions in their texts (`dropped` counted)"""
         if self._rows is None:
             with self._lock:
                 if self._rows is None:
@@ -241,8 +261,7 @@ class PagedBatch:
                     inside = at >= 0
                     slots = np.full(self.tokens, -1, np.int64)
                     slots[inside] = self._table[page[inside]].astype(np.int64) * self.page + at[inside] % self.page
-                    pos = np.maximum(at, 0).astype(np.int32) if self._pos is None else self._pos
-                    dev, i, shared = self._upload(slots.view(np.int32), pos)
+                    dev, i, shared = self._upload(slots.view(np.int32), self._positions())
                     self._rows = dev[: 2 * self.tokens].view(torch.int64), dev[i[1] : i[1] + self.tokens], shared
         slots, pos, shared = self._rows
         if shared is not None:
@@ -313,11 +332,13 @@ def _check_call(q, k, v, tokens, page, max_page, what):
         raise ValueError(f"{what}: q must be 16-byte aligned with strides that are multiples of 8 elements")
 
 
-def _window(window) -> int:
+def _window(window, batch=None) -> int:
     """(a window as wide as the longest request may be hides nothing: wider ones are that one, and any of them fits the library's 32 bits)"""
     w = _whole(window, "window") if window is not None else 0
     if w < 0:
         raise ValueError(f"window {w}")
+    if w and batch is not None and batch._dropped is not None:
+        raise ValueError(f"window {w}: of a trimmed request's keys the places tell no distances")
     return min(w, LONGEST)
 
 
@@ -399,7 +420,7 @@ def paged_attn(q, cache: PagedCache, batch: PagedBatch, scale=None, window=None,
                     shared.reach(stream)
             out, lse = _attn_run(_lib.PagedArgs.from_buffer_copy(got[0]), q, k, v, return_lse, stream)
             return (out, lse) if return_lse else out
-    w = _window(window)
+    w = _window(window, batch)
     sc = float(scale) if scale is not None else q.shape[-1] ** -0.5
     cap = float(softcap) if softcap else 0.0
     _check_call(q, k, v, batch.tokens, batch.page, batch.max_page, "paged_attn")
@@ -473,7 +494,7 @@ def paged_weights(q, cache: PagedCache, batch: PagedBatch, lse, scale=None, wind
                 if stream not in shared.streams:
                     shared.reach(stream)
             return _weights_run(_lib.PagedWeightsArgs.from_buffer_copy(got[0]), q, k, lse, acc, stream)
-    w = _window(window)
+    w = _window(window, batch)
     sc = float(scale) if scale is not None else q.shape[-1] ** -0.5
     longest = batch.longest
     keys = longest if acc is None else acc.shape[-1]
@@ -528,8 +549,8 @@ def cache_evict(cache: PagedCache, batch: PagedBatch, into: PagedBatch, acc, kee
     """Trims every request of ``batch`` to at most ``keep`` stored keys, per key / value head: all stay where there are no more, else the first ``sink``, the last
     ``recent``, and of the others those with the largest ``acc`` [requests, hkv, keys] fp32 (ties to the lowest index, NaN above everything).  Their keys
     and values are copied, in order, into the first entries of the pages that ``into`` (the batch of the trimmed requests) gives them: the old pages stay
-    as they are, since other requests may share them; into's pages must be none of batch's.  Rotated keys keep their positions: a layer with a window, which goes by places,
-    is not trimmed this way.
+    as they are, since other requests may share them; into's pages must be none of batch's.  Rotated keys keep their positions: later batches of these requests are built with
+    ``dropped``, and a layer with a window, which goes by places, is not trimmed this way.
     -> kept [requests, hkv, keep] int32 (the places that stayed, ascending, -1 behind them) and their acc (0 behind them): the next paged_weights' acc"""
     k, v = cache.k, cache.v
     pages, page, hkv, _ = k.shape
