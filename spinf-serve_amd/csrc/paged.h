@@ -30,8 +30,9 @@ constexpr int PAGED_PLACES = 512;
 // Up to 64 rows per key / value head it always does: half and more of the shared kernel's rows would idle (48 rows on 8,000 keys, 8 heads of 256 dims: 23 / 314 -> 67 / 247).
 constexpr int PAGED_WAVE_MAX = 64;
 constexpr int PAGED_WAVE_WORK = 5000;
-// Least tiles of a piece there (us at 8 / 16 / 32: one token over 4,000 keys, 8 heads of 256 dims 11 / 14 / 21; 64 such requests of 3,000 keys, 4 heads: 171 / 149 / 140).
+// Tiles of a piece there: a row group's keys are cut into as many equal pieces as pieces of this size would be begun, so one holds at least half of it (17 tiles: 8 and 9), where
+// the request's places allow that many (us at 8 / 16 / 32: one token over 4,000 keys, 8 heads of 256 dims 11 / 14 / 21; 64 such requests of 3,000 keys, 4 heads: 171 / 149 / 140).
 constexpr int PAGED_WAVE_TILES = 16;
-// Least tiles of a piece of the shared kernel (us at 32 / 48 / 64; a call of 1 and of 16 requests, 640 rows per key / value head on 8,000 stored keys: 8 heads of
+// The same for the shared kernel (us at 32 / 48 / 64; a call of 1 and of 16 requests, 640 rows per key / value head on 8,000 stored keys: 8 heads of
 // 256 dims 79 / 80 / 98 and 963 / 889 / 861, 16 heads of 128 dims 70 / 72 / 84 and 892 / 907 / 882; a window of 1,024 under 512 new tokens 143 / 98 / 98).
 constexpr int PAGED_BLOCK_TILES = 48;

@@ -168,11 +168,11 @@ class Builder {
             list(r, (int)row0, groups, runs);
             int64_t tiles = 0;
             for (const Run& x : runs) tiles += x.count;
-            // Keys are divided where the request's own items leave places free.  A piece keeps so many tiles
-            // that its partial results, written and read back in 32 bits, stay below an eighth of the bytes of its keys and values.
-            const int64_t places = a_->d == 512 || (by_wave && a_->d == 256) ? PAGED_PLACES / 2 : PAGED_PLACES, least = by_wave ? PAGED_WAVE_TILES : PAGED_BLOCK_TILES;
+            // Keys are divided where the request's own items leave places free, into pieces of about `size` tiles or more (at least half of it): there the partial results, written
+            // and read back in 32 bits, are an eighth of the bytes of a piece's keys and values in the wave kernel and a sixth in the shared one, at most twice that.
+            const int64_t places = a_->d == 512 || (by_wave && a_->d == 256) ? PAGED_PLACES / 2 : PAGED_PLACES, size = by_wave ? PAGED_WAVE_TILES : PAGED_BLOCK_TILES;
             int64_t want = std::max<int64_t>(1, places / row_items);
-            const int64_t per = std::max(least, (tiles + want - 1) / want);
+            const int64_t per = std::max(size, (tiles + want - 1) / want);
             const int64_t nsplit = std::max<int64_t>(1, (tiles + per - 1) / per);
             const int64_t here = std::min<int64_t>(rows, N - row0);
             cut_.clear();

@@ -229,6 +229,17 @@ def test_a_request_is_cut_the_same_way_whatever_shares_the_call():
     assert cuts(alone, 5000) == cuts(both, 5000) and len(cuts(alone, 5000)) > 2
 
 
+@pytest.mark.parametrize("variant,size", [(1, 16), (2, 48)])
+def test_pieces_hold_at_least_half_of_their_size(variant, size, monkeypatch):
+    monkeypatch.setattr(paged, "VARIANT", variant)
+    for tiles in (1, size - 1, size, size + 1, 2 * size - 1, 2 * size + 1, 5 * size + 3):
+        b, _ = make_batch([1], [32 * tiles], 16)
+        lists, counts, at = b.plan(4, 1, 128, 0)
+        n = counts[variant - 1]
+        pieces = lists.numpy()[at[variant - 1] :][: 12 * n].reshape(-1, 12)[:, 8]
+        assert n == -(-tiles // size) and pieces.sum() == tiles and pieces.max() - pieces.min() <= 1 and (n == 1 or pieces.min() >= size // 2)
+
+
 def test_rows_slots_and_positions():
     b = sa.PagedBatch.build([2, 3, 2], [18, 1, 16], [[5, 2], [7], [9]], 16, "cpu")
     slots, pos = b.rows()
