@@ -108,7 +108,8 @@ class PagedBatch:
     A request that cache_evict has trimmed stores fewer keys than its text has tokens, rotated by the positions they had.  dropped[r] says how many are gone: its new tokens'
     positions are their places plus that (of a tree, what pos says: the same at most).  A window counts places, so a call over such a batch takes none.
 
-    Host threads and streams may share a batch: what a first call makes is made once, and a call on another stream waits for the copies."""
+    Host threads and streams may share a batch: what a first call makes is made once, and a call on another stream waits for the copies.  A recorded graph reads the batch's
+    lists on the device, as it reads the call's tensors: both have to live as long as the graph is replayed."""
 
     def __init__(self, q_lens, kv_lens, table, need, page, device, end, pos, dropped=None):
         """pos: counted in places, without what was dropped"""

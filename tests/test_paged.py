@@ -1054,6 +1054,117 @@ def test_streams_compiled_programs_and_recorded_graphs(dev):
         torch.cuda.synchronize()
 
 
+class Layer:
+    """one pass through all of the operators, over a cache that `fresh` puts back"""
+
+    def __init__(self, dev):
+        g = torch.Generator().manual_seed(7)
+        self.heads = (8, 2, 128)
+        self.b, pages = make_batch([1, 70], [900, 300], 64, dev, spare=12)
+        self.cache, self.q = fill(self.b, pages, self.heads, 21, dev)
+        self.k, self.v = (torch.randn((71, 2, 128), generator=g).to(BF16).to(dev) for _ in range(2))
+        self.w = torch.rand(128, generator=g).to(dev)
+        ang = torch.rand((1000, 32), generator=g).to(dev)
+        self.cos, self.sin = ang.cos(), ang.sin()
+        self.slots, self.pos = self.b.rows()
+        free = sorted(set(range(pages)) - set(self.b._table.tolist()))
+        self.into = sa.PagedBatch.build([0, 0], [200, 200], [free[:4], free[4:8]], 64, dev)
+        self.acc = torch.rand((2, 2, 900), generator=g).to(dev)
+        self.kept = self.cache.k.clone(), self.cache.v.clone()
+        self.want = self.run(self.q, self.k, self.v, self.acc)
+        self.left = self.cache.k.clone(), self.cache.v.clone()
+        self.fresh()
+
+    def fresh(self):
+        self.cache.k.copy_(self.kept[0])
+        self.cache.v.copy_(self.kept[1])
+
+    def run(self, q, k, v, acc):
+        a, c = sa.qk_norm_rope(q, k, self.w, self.w, self.cos, self.sin, 1e-6, self.pos)
+        y = sa.qk_norm_rope_put(q, k, v, self.w, self.w, self.cos, self.sin, 1e-6, self.cache, self.slots, self.pos)
+        out, lse = sa.paged_attn(y, self.cache, self.b, return_lse=True)
+        weight = sa.paged_weights(y, self.cache, self.b, lse, acc=acc)
+        return (a, c, y, out, lse, weight, *sa.cache_evict(self.cache, self.b, self.into, weight, 200, 4, 8))
+
+    def check(self, got):
+        assert all(torch.equal(x, y) for x, y in zip((*got, self.cache.k, self.cache.v), (*self.want, *self.left)))
+
+
+@pytest.mark.gpu
+def test_the_registered_operators_of_the_cache(dev):
+    """schemas (what they write among it) and shapes without memory"""
+    x, tests, ops = Layer(dev), ("test_schema", "test_faketensor"), torch.ops.spinf
+    table = (x.w, x.w, x.cos, x.sin, 1e-6)
+    torch.library.opcheck(ops.qk_norm_rope.default, (x.q, x.k, *table, x.pos, False, False), test_utils=tests)
+    torch.library.opcheck(ops.qk_norm_rope_put.default, (x.q, x.k, x.v, *table, x.cache.k, x.cache.v, x.slots, x.pos, False, False, False), test_utils=tests)
+    old, new = x.b._device(), x.into._device()
+    torch.library.opcheck(ops.cache_evict.default, (x.cache.k, x.cache.v, x.acc, old[1], old[0], new[1], new[0], 64, 200, 4, 8), test_utils=tests)
+
+
+@pytest.mark.gpu
+def test_a_compiled_pass_over_the_cache(dev):
+    x = Layer(dev)
+    torch._dynamo.reset()
+    try:
+        compiled = torch.compile(x.run, backend="aot_eager")
+        for _ in range(2):
+            x.check(compiled(x.q, x.k, x.v, x.acc))
+            x.fresh()
+    finally:
+        torch._dynamo.reset()
+    x.check(x.run(x.q, x.k, x.v, x.acc))
+
+
+@pytest.mark.gpu
+def test_a_recorded_pass_over_the_cache(dev):
+    x = Layer(dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = x.run(x.q, x.k, x.v, x.acc)
+    for seed in range(3):
+        x.q.copy_(fill(x.b, x.cache.k.shape[0], x.heads, 50 + seed, dev)[1])
+        x.fresh()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (*out, x.cache.k, x.cache.v)]
+        x.fresh()
+        assert all(torch.equal(a, b) for a, b in zip(got, (*x.run(x.q, x.k, x.v, x.acc), x.cache.k, x.cache.v)))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_host_threads_share_a_batch(dev):
+    """first calls of four threads, each on a stream of its own"""
+    import threading
+
+    x = Layer(dev)
+    want, lse = sa.paged_attn(x.q, x.cache, x.b, return_lse=True)
+    weight = sa.paged_weights(x.q, x.cache, x.b, lse)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(10):
+        b, start, got = pickle.loads(pickle.dumps(x.b)), threading.Barrier(4), [None] * 4
+
+        def run(i):
+            with torch.cuda.stream(streams[i]):
+                start.wait(60)
+                for _ in range(3):
+                    out, l2 = sa.paged_attn(x.q, x.cache, b, return_lse=True)
+                    w2 = sa.paged_weights(x.q, x.cache, b, l2)
+                streams[i].synchronize()
+            got[i] = out, l2, w2, b.rows()[0]
+
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for t in got for a, c in zip(t, (want, lse, weight, x.slots)))
+
+
 @pytest.mark.gpu
 def test_a_session_equals_reading_anew(dev):
     """examples/paged_session.py: documents, later questions and tokens over the cache against tree_attn over the whole stream"""
