@@ -41,6 +41,13 @@ __device__ __forceinline__ void load8(const void* p, long i, int f32, float (&x)
     }
 }
 
+// 1 / sqrt(x); the instruction by itself takes a subnormal x for zero (rows of some 1e-19 with eps 0)
+__device__ __forceinline__ float inverse_root(float x) {
+    const bool tiny = x < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x);
+    return tiny ? r * 0x1p50f : r;
+}
+
 template <int D, int U>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const Params p) {
     constexpr int LANES = D / 16;       // lanes of a row
@@ -90,7 +97,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const Params p) {
         }
 #pragma unroll
         for (int d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d);
-        float r = __builtin_amdgcn_rsqf(sum * (1.0f / D) + p.eps);
+        float r = inverse_root(sum * (1.0f / D) + p.eps);
         if (kind[u] == 2 && !p.v_norm) r = 1.0f;
         if (kind[u] < 2) {
             // A position outside the tables, or a place outside the cache, cannot be refused here: the row says so itself.

@@ -985,6 +985,21 @@ def test_rows_that_say_so_themselves(dev):
     assert torch.equal(a[3, [0, 2, 3]], got[0][3, [0, 2, 3]]) and a[4, 2].isnan().all() and torch.equal(a[4, [0, 1, 3]], got[0][4, [0, 1, 3]])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 256])
+def test_rows_whose_mean_square_is_subnormal(dev, d):
+    q, k, v, wq, wk, cos, sin, p = rope_case(dev, 9, 4, 2, d, 32, torch.float32, BF16, torch.int32, seed=3)
+    q, k = q.clone(), k.clone()
+    for t in (q, k):
+        t.mul_(2.0**-64)
+    got = sa.qk_norm_rope(q, k, wq, wk, cos, sin, 0.0, p)
+    for x, w, y in zip((q, k), (wq, wk), got):
+        want, tol = rope_want(x, w, cos, sin, p, 0.0, False, False)
+        # squares of up to 2^-124 in steps of 2^-149: their mean, of 2^-132 and more here, is off by 2^-17 at most
+        assert float((x.double() ** 2).mean(-1).min()) > 2.0**-132
+        close(y, want, tol + 2.0**-17 * np.abs(want) + 2.0**-17 * np.abs(want).max(-1, keepdims=True))
+
+
 def test_norm_and_rotation_refuse_bad_arguments():
     q, k, w, c = torch.zeros((3, 4, 64), dtype=BF16), torch.zeros((3, 2, 64), dtype=BF16), torch.zeros(64), torch.zeros((3, 16))
     with pytest.raises(RuntimeError, match="ROCm"):
