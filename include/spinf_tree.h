@@ -344,7 +344,8 @@ int spinf_xdecode_put(const void* k, int64_t k_g, int64_t k_h, int64_t k_q, cons
  * given: the tokens of the request's branches in pre-order, end[t] = the exclusive end of row t's subtree in rows of the call, pos[t] = its position) the
  * new tokens whose subtree it lies in, and all stored keys below c; on a layer with a window only where pos(i) - pos(s) < window, a stored key's
  * position being its place s.  A row that sees nothing comes out as zeros with a log-sum of -inf.  A key that a row does not see contributes nothing to
- * it, whatever the cache holds there.
+ * it, whatever the cache holds there.  Scores, sums and outputs are accumulated in fp32; a key's probability is rounded to bf16 once for its product with the value (the sum of
+ * the probabilities takes the unrounded ones).  A soft cap above 2^100 is none.
  *
  * spinf_paged_plan_*: the work lists of a call, host only, deterministic; from the lengths, the trees and the geometry.  They serve every layer of that
  * geometry.  How a request is cut depends on nothing but its own lengths and tree: its outputs are the same bits whatever shares the call.
@@ -422,7 +423,7 @@ int spinf_cache_evict(const spinf_evict_args* args, void* stream);
  *   slots NULL: q_out [T, hq, d], k_out [T, hkv, d] dense, v is not touched.
  *   slots [T] int64 device: token t's key and value become entry slots[t] % page of page slots[t] / page of the cache (k_out, v_out with their
  *   strides, `pages` pages); v_norm: the value is normed too, without weight.  A negative slot stores nothing (a pad); one behind the cache stores nothing
- *   and makes the token's query NaN.  Two tokens with one slot: either's rows.  d in {64, 128, 256, 512}, rot a multiple of 16. */
+ *   and makes the token's query NaN.  Two tokens with one slot: every 16 bytes are either's.  d in {64, 128, 256, 512}, rot a multiple of 16. */
 typedef struct spinf_rope_args {
     const void* q; const void* k; const void* v;
     int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;

@@ -183,6 +183,6 @@ def _(q, k, v, wq, wk, cos, sin, eps, ck, cv, slots, pos, neighbours, plus_one, 
 def qk_norm_rope_put(q, k, v, wq, wk, cos, sin, eps, cache, slots, pos=None, neighbours=False, plus_one=False, v_norm=False):
     """as qk_norm_rope, but the keys and the values (``v_norm``: normed too, without weight) go into ``cache`` (a PagedCache): token t's become entry
     slots[t] % page of page slots[t] // page (slots int64; PagedBatch.rows() has them).  -> the queries.  A negative slot stores nothing (a pad); a slot
-    behind the cache stores nothing either, and that token's query comes out as NaN."""
+    behind the cache stores nothing either, and that token's query comes out as NaN.  Slots should differ: of two tokens with one, every 16 bytes are either's."""
     run = _put if _lib.eager(q, k, v, wq, wk, cos, sin, cache.k, cache.v) else _put_op
     return run(q, k, v, wq, wk, cos, sin, float(eps), cache.k, cache.v, slots, pos, bool(neighbours), bool(plus_one), bool(v_norm))
