@@ -178,7 +178,7 @@ def _book(s, pool, tables, lens, keys, rows, page, content, stored):
     s["book"] = dict(lens=_i32(lens), table=_i32(table), free=_i32(pool), left=_i32([left]), first=_i32(np.zeros(R + 1)), slots=torch.full((rows,), -1, dtype=torch.int64, device=DEV),
                      pos=torch.zeros(rows, dtype=torch.int32, device=DEV), content=_i32(content), text=_i32(np.append(stored, 0)))
     if own:
-        seats = _package().PagedSeats.build(seats=R, rows=rows, page=page, keys=keys, pool=pool, contents=(stored, tables), stored=lens, heads=s.get("heads", ()), device=DEV)
+        seats = _package().PagedSeats.build(seats=R, rows=rows, page=page, keys=keys, pool=pool, contents=(stored, tables[: len(stored)]), stored=lens, heads=s.get("heads", ()), device=DEV)
         seats.content.copy_(s["book"]["content"])
         s["seats"] = seats
 
