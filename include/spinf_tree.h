@@ -438,6 +438,77 @@ typedef struct spinf_rope_args {
 } spinf_rope_args;
 int spinf_qk_norm_rope(const spinf_rope_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ seats
+ * A decoding step whose lengths and pages stay on the GPU, so that a recorded one can be replayed for the next; no counterpart in the reference.  `seats` requests go on
+ * at a time: seat r has keys of its own (at most `keys`), in pages out of a pool that the seats share, behind those of content content[r] (-1, or any number outside 0 ..
+ * contents - 1: of none), which other seats may share.  Own key s lies in entry s % page of page lists[table_at + r * ceil(keys / page) + s / page].
+ *
+ * spinf_seats_step: first the last min(drop[r], lens[r]) own keys of every seat go (drop NULL: none), and the pages that hold none any more go back on the stack `free` (left[0] of
+ * its `pool` entries are pages to be had, the last goes first), in the reverse of the order they were taken in; then come[r] new tokens (below 1: none) come to seat r, with as
+ * many pages as that needs.  A seat gets its tokens or none of them: none where they would pass `keys`, where the tokens asked for by the seats up to it are more than `rows`, or where it needs
+ * a page and the pages asked for by the seats up to it are more than there are.  Afterwards
+ *   lens, left, lists: as they are then; took [seats], first [seats + 1]: each seat's new tokens, and the row its first one is; stay [seats]: its keys before them;
+ *   slots [rows] int64, pos [rows]: where the rows' keys and values go (page * page size + entry) and their positions, text positions of the content counted; -1 and 0 behind
+ *   the last row; and for each of the `kinds` head geometries (window 0: none) the work lists of spinf_seats_attn.
+ * shared [contents, 3]: stored keys (at most `longest`), positions of the text, first page in `lists`.  Lists, as long as
+ * spinf_seats_rooms says ([0 .. 2] items of 12 int32 each, [3] partial rows of the attention's workspace), 16-byte aligned; counts [4]; parts [rows + 1]; seat_parts [2 seats + 1].  One launch
+ * (two where rows > 8,192); nothing is allocated.  At most 2,048 seats and 8 geometries. */
+typedef struct spinf_seats_kind {
+    int32_t* wave; int32_t* single; int32_t* block; int32_t* counts; int32_t* parts; int32_t* seat_parts;
+    int32_t hq, hkv, d, window;
+} spinf_seats_kind;
+typedef struct spinf_seats_args {
+    const int32_t* come; const int32_t* drop; const int32_t* content;
+    int32_t* lens; int32_t* lists; int32_t* free; int32_t* left; int32_t* first; int32_t* took; int32_t* stay;
+    int64_t* slots; int32_t* pos;
+    const int32_t* shared;
+    int64_t rows, keys, pool, table_at, longest;
+    int32_t seats, page, contents, kinds;
+    spinf_seats_kind kind[8];
+} spinf_seats_args;
+int spinf_seats_rooms(const spinf_seats_args* args, int32_t kind, int64_t rooms[4]);
+int spinf_seats_step(const spinf_seats_args* args, void* stream);
+
+/* Attention of a step's new tokens: out[t] = softmax over the keys that row t sees of scale q.k (softcap > 0: of softcap tanh(scale q.k / softcap)) times v, for every row and query head.  A
+ * row sees its content's stored keys and its seat's own keys up to its own, with a window those less than `window` places behind it.  The rows of seats one after the other below one
+ * content read its keys together.  Rows behind the step's last come out as zeros (lse: -inf).
+ *   q, out [rows, hq, d] bf16 (strides in elements, multiples of 8); lse [rows, hq] fp32 or NULL; k, v the cache as above, every page in `lists` one of its;
+ *   lists, first, pos as spinf_seats_step leaves them; kind: the lists of this geometry and window; rooms: what spinf_seats_rooms says of it; workspace: 16-byte aligned,
+ *   rooms[3] * hq * (d + 2) * 4 bytes, the caller's.  Three launches; nothing is allocated. */
+typedef struct spinf_seats_attn_args {
+    const void* q; void* out; float* lse;
+    int64_t q_tok, q_head, o_tok, o_head;
+    const void* k; const void* v;
+    int64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    const int32_t* lists; const int32_t* first; const int32_t* pos;
+    spinf_seats_kind kind;
+    int64_t rooms[4];
+    void* workspace; int64_t workspace_bytes;
+    int64_t rows;
+    int32_t seats, page;
+    float scale, softcap;
+} spinf_seats_attn_args;
+int spinf_seats_attn_fwd(const spinf_seats_attn_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ draws
+ * Tokens drawn from logits [rows, vocab] (fp32: dtype 0, bf16: 1; rows ld elements apart) by given random numbers u [rows] in 0 .. 1 (fp32, or fp64 with u_f64); the reference draws
+ * none.  Of each row: temperature T, top-k, top-p and min-p, [rows] device arrays or (NULL) one number for all.  Order: larger logits first, of equal ones the lower index; weight w = exp((x -
+ * max) / T).  Kept are the first top_k of the order (below 1, or vocab and more: all), of these the shortest beginning with at least top_p of their weight (1 and more: all; the first in any
+ * case), of these the tokens with w >= min_p of the largest weight.  token [rows] int64: the first by index up to which the kept weights add up to more than u times their sum (u at or
+ * above 1: the last kept one; below 0 or NaN: the first); prob [rows] fp32 or NULL: its share of the kept weights.  T 0: the first of the order.  Logits of -inf and NaN are never drawn; where one
+ * is +inf, those that are share the weight.  token -1 and prob 0 where no logit is left, or T, top_p or min_p of the row is negative or NaN.
+ * Weights are 64-bit, their sums exact to 2^-49 of a weight.  Two launches, four where a filter is given; the workspace is the caller's, nothing is allocated. */
+typedef struct spinf_sample_args {
+    const void* logits; int64_t ld, rows, vocab;
+    const void* u; const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;
+    int64_t* token; float* prob;
+    void* workspace; int64_t workspace_bytes;
+    float all_temperature, all_top_p, all_min_p; int32_t all_top_k;
+    int32_t dtype, u_f64;
+} spinf_sample_args;
+int spinf_sample_workspace(const spinf_sample_args* args, int64_t* bytes);
+int spinf_sample(const spinf_sample_args* args, void* stream);
+
 /* ------------------------------------------------------------------------------------------------ yardstick
  * No counterpart in the reference: one launch of a pure v_mfma_f32_32x32x16_bf16 loop on every compute unit (one workgroup of eight
  * waves per CU, iters x 8 MFMAs per wave, operands in registers), for the benchmark's "what do the matrix cores sustain on this
@@ -489,6 +560,8 @@ int spinf_struct_sizes(int64_t* sizes, int32_t n);
 /* The same for the paged cache: spinf_paged_plan_args, spinf_paged_args, spinf_rope_args, spinf_paged_weights_args and
  * spinf_evict_args, in this order; n must be 5. */
 int spinf_paged_struct_sizes(int64_t* sizes, int32_t n);
+/* The same for spinf_seats_kind, spinf_seats_args, spinf_seats_attn_args and spinf_sample_args, in this order; n must be 4. */
+int spinf_seats_struct_sizes(int64_t* sizes, int32_t n);
 
 #ifdef __cplusplus
 }

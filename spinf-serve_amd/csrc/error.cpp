@@ -33,3 +33,11 @@ extern "C" int spinf_paged_struct_sizes(int64_t* sizes, int32_t n) {
     for (int i = 0; i < n; i++) sizes[i] = all[i];
     return SPINF_OK;
 }
+
+// the same for the blocks of the seats and the sampler
+extern "C" int spinf_seats_struct_sizes(int64_t* sizes, int32_t n) {
+    const int64_t all[4] = {(int64_t)sizeof(spinf_seats_kind), (int64_t)sizeof(spinf_seats_args), (int64_t)sizeof(spinf_seats_attn_args), (int64_t)sizeof(spinf_sample_args)};
+    if (!sizes || n != 4) return spinf_fail(SPINF_E_ARG, "seats_struct_sizes: 4 sizes (kind, step, attn, sample)");
+    for (int i = 0; i < n; i++) sizes[i] = all[i];
+    return SPINF_OK;
+}

@@ -1,0 +1,657 @@
+// Tokens drawn from logits by given random numbers, for gfx950 (MI355X): temperature, top-k, top-p and min-p of every row.  The reference reads log-probs of given options
+// and takes the best tokens of its extraction decoder (spinf_serve/decode.py:246-300); it draws none.
+//
+// Mathematics.  Order: larger logits first, of equal ones the lower index: as one number per token (the complement of its ordered bits above its index), ascending.  Weight of a
+// token w = exp((x - max) / T).  Kept are the first k of the order, of these the shortest beginning that holds p of their weight, of these the tokens with w >= min_p.  The token
+// drawn is the first, by index, up to which the kept weights add up to more than u times their sum.
+//
+// Where a border falls decides which token comes out, so weights are taken in 64 bits, and sums of them are sums of whole numbers: units of 2^-49 of the largest weight of a chunk
+// (16,384 logits), the same in any order.
+//
+// Kernels.  chunks: a chunk's largest logit, its weight, and how many logits and how much weight lie in each of 255 bins, a twelfth of T wide, below its largest one (bins at whole
+// multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
+// of the bins in question.  draw: those few are put in order by digits of their numbers, the chunk is found by the chunks' weights and the token in it.  Rows without a filter need the first and
+// the last.  Where bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself, digit by digit.
+// Bound by HBM: the logits once; the second reading comes out of the last-level cache.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "spinf_tree.h"
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef unsigned long long u64;
+
+namespace {
+
+constexpr int LANES = 1024, EACH = 16, CHUNK = LANES * EACH;
+constexpr int BINS = 256;              // the last one: all below
+constexpr int SEGMENT = 1024;          // tokens of a chunk that lie in the bins in question
+constexpr int LISTED = 8192;           // ... of a row
+constexpr int MOST_CHUNKS = 256;
+constexpr float BINS_PER_UNIT = 12.f;
+
+struct Stat { float top; unsigned at; u64 sum; };       // of a chunk: largest logit (-inf: none), where, weight
+// of a row: largest logit; what to do; bins [from, to] and `kth` in question; of all: weight, kept tokens before the kth bin, weight before it and before `from`
+struct Row { float top; int grid, how, from, to, kth, before_k, unused; double sum, mass_k, mass_from; };
+static_assert(sizeof(Stat) == 16 && sizeof(Row) == 56, "workspace layout");
+enum { PLAIN = 0, LIST = 1, SEARCH = 2, NOTHING = 3, BEST = 4 };
+
+struct Params {
+    const void* logits; long ld; int vocab, rows, chunks; bool aligned;
+    const void* u; bool u_f64;
+    const float *temperature, *top_p, *min_p; const int* top_k;
+    float all_temperature, all_top_p, all_min_p; int all_top_k;
+    long* token; float* prob;
+    Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
+};
+
+struct How { double inv; float scale, p, least; int k; bool best, wrong, filtered; };
+__device__ __forceinline__ How settings(const Params& p, int row) {
+    How h;
+    const float T = p.temperature ? p.temperature[row] : p.all_temperature;
+    h.p = p.top_p ? p.top_p[row] : p.all_top_p;
+    h.least = p.min_p ? p.min_p[row] : p.all_min_p;
+    h.k = p.top_k ? p.top_k[row] : p.all_top_k;
+    h.wrong = !(T >= 0.f) || !(h.p >= 0.f) || !(h.least >= 0.f);
+    h.best = T == 0.f;
+    h.inv = 1.0 / (double)T;
+    h.scale = fminf(BINS_PER_UNIT / T, 3e38f);
+    if (h.k <= 0 || h.k >= p.vocab) h.k = 0;
+    if (h.p == 0.f) {   // the first alone
+        h.p = 1.f;
+        h.k = 1;
+    }
+    if (h.k == 1) h.best = true;
+    h.filtered = h.k || h.p < 1.f || h.least > 0.f;
+    return h;
+}
+
+__device__ __forceinline__ unsigned ordered(float x) {   // larger for larger x
+    const unsigned b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~ordered(x) << 32 | at; }   // smaller: earlier in the order
+__device__ __forceinline__ float clean(float x) { return x == x ? (x == 0.f ? 0.f : x) : -INFINITY; }   // (zeros are equal whatever their sign)
+
+// a token's place on the grid of bins; never falls as x grows
+__device__ __forceinline__ int place(float x, float scale) { return (int)floorf(fminf(fmaxf(x * scale, -1e9f), 1e9f)); }
+
+// exp((x - top) / T), 1 for the largest ones also where they are infinite
+__device__ __forceinline__ double weight(float x, float top, double inv) { return x == top ? 1.0 : top == INFINITY ? 0.0 : exp(((double)x - (double)top) * inv); }
+// in units of 2^-49: the last bits of w + 8, rounded there
+__device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 8.0) - __double_as_longlong(8.0)); }
+constexpr double UNIT = 0x1p-49;
+
+template <bool BF16>
+__device__ __forceinline__ float load1(const Params& p, int row, int i) {
+    const long at = (long)row * p.ld + i;
+    return BF16 ? (float)((const __bf16*)p.logits)[at] : ((const float*)p.logits)[at];
+}
+template <bool BF16>
+constexpr int VEC = BF16 ? 8 : 4;
+// index of a lane's e-th logit
+template <bool BF16>
+__device__ __forceinline__ int index_of(int chunk, int e) { return chunk * CHUNK + (e / VEC<BF16> * LANES + (int)threadIdx.x) * VEC<BF16> + e % VEC<BF16>; }
+template <bool BF16>
+__device__ __forceinline__ void load(const Params& p, int row, int chunk, float (&x)[EACH]) {
+    constexpr int V = VEC<BF16>;
+#pragma unroll
+    for (int i = 0; i < EACH / V; i++) {
+        const int at = index_of<BF16>(chunk, i * V);
+        if (p.aligned && at + V <= p.vocab) {
+            if (BF16) {
+                const bf16x8 y = *(const bf16x8*)((const __bf16*)p.logits + (long)row * p.ld + at);
+#pragma unroll
+                for (int j = 0; j < V; j++) x[i * V + j] = (float)y[j];
+            } else {
+                const float4 y = *(const float4*)((const float*)p.logits + (long)row * p.ld + at);
+                x[i * V] = y.x; x[i * V + 1] = y.y; x[i * V + 2] = y.z; x[i * V + 3] = y.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) x[i * V + j] = at + j < p.vocab ? load1<BF16>(p, row, at + j) : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) x[e] = clean(x[e]);
+}
+
+template <class T, class F>
+__device__ __forceinline__ T over_all(T x, T* room, F f) {   // room: one place per wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x = f(x, __shfl_xor(x, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = room[0];
+    for (int w = 1; w < (int)blockDim.x / 64; w++) x = f(x, room[w]);
+    return x;
+}
+__device__ __forceinline__ u64 sum_all(u64 x, u64* room) { return over_all(x, room, [](u64 a, u64 b) { return a + b; }); }
+
+template <bool BF16>
+__global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
+    __shared__ u64 room[LANES / 64];
+    __shared__ u64 weights[BINS];
+    __shared__ int numbers[BINS];
+    const int chunk = blockIdx.x, row = blockIdx.y;
+    const How h = settings(p, row);
+    if (h.wrong) return;
+    float x[EACH];
+    load<BF16>(p, row, chunk, x);
+    u64 first = ~0ull;   // the least number of the chunk
+#pragma unroll
+    for (int e = 0; e < EACH; e++) first = std::min(first, number(x[e], index_of<BF16>(chunk, e)));
+    first = over_all(first, room, [](u64 a, u64 b) { return a < b ? a : b; });
+    const float top = unordered(~(unsigned)(first >> 32));
+    Stat s = {top, (unsigned)first, 0};
+    const long at = (long)row * p.chunks + chunk;
+    if (h.best || top == -INFINITY) {   // (an empty chunk's bins are not looked at)
+        if (threadIdx.x == 0) p.stat[at] = s;
+        return;
+    }
+    if (h.filtered) {
+        if (threadIdx.x < BINS) {
+            weights[threadIdx.x] = 0;
+            numbers[threadIdx.x] = 0;
+        }
+        __syncthreads();
+    }
+    const int grid = place(top, h.scale);
+    int there = 0;   // logits that can be drawn
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        there += x[e] > -INFINITY;
+        const u64 w = x[e] == -INFINITY ? 0 : units(weight(x[e], top, h.inv));
+        s.sum += w;
+        const int b = grid - place(x[e], h.scale);
+        if (h.filtered && x[e] > -INFINITY && b < BINS - 1) {
+            atomicAdd(&weights[b], w);
+            atomicAdd(&numbers[b], 1);
+        }
+    }
+    if (h.filtered) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) there += __shfl_xor(there, d);
+        if ((threadIdx.x & 63) == 0) atomicAdd(&numbers[BINS - 1], there);   // (of all bins and below)
+    }
+    s.sum = sum_all(s.sum, room);   // (its barriers are behind the bins' last addition)
+    if (threadIdx.x == 0) p.stat[at] = s;
+    if (h.filtered && threadIdx.x < BINS) {
+        p.hist_w[at * BINS + threadIdx.x] = weights[threadIdx.x];
+        p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
+    }
+}
+
+// a row's largest logit and its weight in all
+__device__ __forceinline__ float row_top(const Params& p, int row) {
+    float top = -INFINITY;
+    for (int c = 0; c < p.chunks; c++) top = fmaxf(top, p.stat[(long)row * p.chunks + c].top);
+    return top;
+}
+
+__global__ __launch_bounds__(BINS) void sample_rows_kernel(const Params p) {
+    __shared__ double masses[BINS];
+    __shared__ int counts[BINS];
+    __shared__ int found[3];
+    const int row = blockIdx.x, b = threadIdx.x;
+    const How h = settings(p, row);
+    Row r = {};
+    r.top = h.wrong ? -INFINITY : row_top(p, row);
+    r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
+    if (r.how != PLAIN || !h.filtered) {
+        if (b == 0) p.row[row] = r;
+        return;
+    }
+    r.grid = place(r.top, h.scale);
+    double mass = 0.0, sum = 0.0;
+    int n = 0, there = 0;
+    for (int c = 0; c < p.chunks; c++) {
+        const long at = (long)row * p.chunks + c;
+        const Stat s = p.stat[at];
+        if (s.top == -INFINITY) continue;
+        there += p.hist_n[at * BINS + BINS - 1];
+        const double f = weight(s.top, r.top, h.inv) * UNIT;
+        sum += f * (double)s.sum;
+        const int mine = b - (r.grid - place(s.top, h.scale));
+        if (mine >= 0 && mine < BINS - 1 && b < BINS - 1) {
+            mass += f * (double)p.hist_w[at * BINS + mine];
+            n += p.hist_n[at * BINS + mine];
+        }
+    }
+    r.sum = sum;
+    const int own_n = n, k = h.k < there ? h.k : 0;
+    for (int d = 1; d < BINS; d <<= 1) {   // sums up to the bin
+        masses[b] = mass;
+        counts[b] = n;
+        __syncthreads();
+        if (b >= d) {
+            mass += masses[b - d];
+            n += counts[b - d];
+        }
+        __syncthreads();
+    }
+    masses[b] = mass;
+    counts[b] = n;
+    if (b < 3) found[b] = BINS;
+    __syncthreads();
+    const bool in = b < BINS - 1;
+    if (k && in && n >= k && n - own_n < k) found[2] = b;
+    __syncthreads();
+    r.kth = found[2];
+    double low = sum, high = sum;   // the weight of the first k lies between
+    if (r.kth < BINS) {
+        high = masses[r.kth];
+        low = r.kth ? masses[r.kth - 1] : 0.0;
+    }
+    if (h.p < 1.f && in) {   // (what the sums' rounding could move across a border is in question too)
+        if (mass >= (double)h.p * low * (1.0 - 1e-10)) atomicMin(&found[0], b);
+        if (mass >= (double)h.p * high * (1.0 + 1e-10)) atomicMin(&found[1], b);
+    }
+    __syncthreads();
+    if (b) return;
+    r.how = k && r.kth == BINS ? SEARCH : LIST;   // (the k-th lies below the bins)
+    if (h.p < 1.f) {
+        r.to = std::min(found[1], r.kth);
+        r.from = std::min(found[0], r.to);
+        if (r.to == BINS) r.how = SEARCH;
+    } else {
+        r.from = r.to = k ? r.kth : INT_MAX;   // (no bin in question: all are kept that min-p leaves)
+    }
+    if (r.how == LIST) {
+        if (r.kth < BINS) {
+            r.before_k = r.kth ? counts[r.kth - 1] : 0;
+            r.mass_k = low;
+        }
+        r.mass_from = r.from > 0 && r.from < BINS ? masses[r.from - 1] : 0.0;
+    }
+    p.row[row] = r;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
+    __shared__ u64 room[LANES / 64];
+    __shared__ int n;
+    const int chunk = blockIdx.x, row = blockIdx.y;
+    const Row r = p.row[row];
+    if (r.how != LIST) return;
+    const long at = (long)row * p.chunks + chunk;
+    const Stat s = p.stat[at];
+    if (threadIdx.x == 0) n = 0;
+    __syncthreads();
+    u64 kept = 0;
+    const How h = settings(p, row);
+    // (a chunk whose largest logit lies behind the bins in question has nothing that matters)
+    const int begin = s.top == -INFINITY ? INT_MAX : r.grid - place(s.top, h.scale);
+    if (begin <= r.to || begin <= r.kth) {
+        const double least = log((double)h.least);
+        float x[EACH];
+        load<BF16>(p, row, chunk, x);
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            if (x[e] == -INFINITY) continue;
+            const int b = r.grid - place(x[e], h.scale);
+            if (b < r.from) {
+                if (x[e] == r.top || ((double)x[e] - (double)r.top) * h.inv >= least) kept += units(weight(x[e], s.top, h.inv));
+            } else if (b <= r.to || b == r.kth) {
+                const int i = atomicAdd(&n, 1);
+                if (i < SEGMENT) p.list[at * SEGMENT + i] = make_uint2(ordered(x[e]), index_of<BF16>(chunk, e));
+            }
+        }
+    }
+    kept = sum_all(kept, room);
+    if (threadIdx.x == 0) {
+        p.kept[at] = kept;
+        p.count[at] = n;
+    }
+}
+
+// The least number up to which (it counted in) those of `each` hold at least `need` in all; ~0: all of them hold less.  each(f) calls f(number, worth) for every one in question,
+// each lane for its share.  Eight bits at a time, from the top.
+template <class E>
+__device__ u64 search(u64 need, u64* sums, int* counts, u64* found, E each) {
+    u64 prefix = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            sums[threadIdx.x] = 0;
+            counts[threadIdx.x] = 0;
+        }
+        if (threadIdx.x == 0) found[0] = found[1] = ~0ull;
+        __syncthreads();
+        each([&](u64 c, u64 worth) __attribute__((always_inline)) {
+            if (shift == 56 || c >> (shift + 8) == prefix >> (shift + 8)) {
+                const int digit = (int)(c >> shift) & 255;
+                atomicAdd(&sums[digit], worth);
+                atomicAdd(&counts[digit], 1);
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {   // four digits a lane
+            const int d0 = 4 * threadIdx.x;
+            const u64 mine = sums[d0] + sums[d0 + 1] + sums[d0 + 2] + sums[d0 + 3];
+            u64 upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const u64 y = __shfl_up(upto, d);
+                if ((int)threadIdx.x >= d) upto += y;
+            }
+            u64 before = upto - mine;
+            if (before < need && upto >= need) {
+                int d = d0;
+                while (before + sums[d] < need) before += sums[d++];
+                found[0] = d;
+                found[1] = need - before;
+            }
+        }
+        __syncthreads();
+        if (found[0] == ~0ull) return ~0ull;   // (of the first digit alone)
+        prefix |= found[0] << shift;
+        need = found[1];
+        const bool only = counts[found[0]] == 1;
+        if (only && shift) {   // the rest of its digits
+            __syncthreads();
+            if (threadIdx.x == 0) found[0] = 0;
+            __syncthreads();
+            each([&](u64 c, u64) __attribute__((always_inline)) {
+                if (c >> shift == prefix >> shift) found[0] = c;
+            });
+            __syncthreads();
+            prefix = found[0];
+            break;
+        }
+    }
+    __syncthreads();
+    return prefix;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, const bool filters) {
+    __shared__ u64 room[LANES / 64];
+    __shared__ u64 listed[LISTED];
+    __shared__ u64 chunks[MOST_CHUNKS];
+    __shared__ u64 sums[256], found[2];
+    __shared__ int counts[256], begins[MOST_CHUNKS + 1];
+    __shared__ double target[2];
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const How h = settings(p, row);
+    const Stat* stat = p.stat + (long)row * p.chunks;
+    Row r = {};
+    if (filters) r = p.row[row];
+    else {
+        r.top = h.wrong ? -INFINITY : row_top(p, row);
+        r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
+    }
+    if (r.how == NOTHING || r.how == BEST) {
+        if (tid == 0) {
+            long token = -1;
+            if (r.how == BEST)
+                for (int c = 0; c < p.chunks && token < 0; c++)
+                    if (stat[c].top == r.top) token = stat[c].at;
+            p.token[row] = token;
+            if (p.prob) p.prob[row] = token < 0 ? 0.f : 1.f;
+        }
+        return;
+    }
+    const double least = log((double)h.least);
+    const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
+    u64 last = ~0ull;   // the last number that is kept
+    if (r.how == LIST) {
+        int n = 0;
+        for (int c = 0; c < p.chunks; c++) {
+            const int m = p.count[(long)row * p.chunks + c];
+            if (tid == 0) begins[c] = n;
+            n = m > SEGMENT || n + m > LISTED ? LISTED + 1 : n + m;
+        }
+        if (tid == 0) begins[p.chunks] = n;
+        __syncthreads();
+        if (n > LISTED) r.how = SEARCH;
+        else {
+            for (int c = tid >> 6; c < p.chunks; c += LANES / 64)
+                for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
+                    const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
+                    listed[i] = (u64)~y.x << 32 | y.y;
+                }
+            __syncthreads();
+            const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
+            double all = r.sum;   // weight of the first k
+            if (r.kth < BINS) {
+                last = search(h.k - r.before_k, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                    for (int i = tid; i < n; i += LANES)
+                        if (r.grid - place(value(listed[i]), h.scale) == r.kth) f(listed[i], 1);
+                });
+                if (h.p < 1.f) {
+                    u64 w = 0;
+                    for (int i = tid; i < n; i += LANES) {
+                        const float x = value(listed[i]);
+                        if (listed[i] <= last && r.grid - place(x, h.scale) == r.kth) w += units(weight(x, r.top, h.inv));
+                    }
+                    all = r.mass_k + UNIT * (double)sum_all(w, room);
+                }
+            }
+            if (h.p < 1.f) {
+                const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p49);
+                const u64 border = search(need < 1.0 ? 1 : (u64)need, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                    for (int i = tid; i < n; i += LANES) {
+                        const float x = value(listed[i]);
+                        if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to) f(listed[i], units(weight(x, r.top, h.inv)));
+                    }
+                });
+                last = std::min(last, border);
+            }
+            // what is kept of them, by chunk
+            for (int c = tid; c < p.chunks; c += LANES) chunks[c] = p.kept[(long)row * p.chunks + c];
+            __syncthreads();
+            for (int i = tid; i < n; i += LANES) {
+                const float x = value(listed[i]);
+                const int c = (int)((unsigned)listed[i] / CHUNK);
+                if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to && stays(x)) atomicAdd(&chunks[c], units(weight(x, stat[c].top, h.inv)));
+            }
+        }
+    }
+    if (r.how == SEARCH) {
+        last = ~0ull;
+        const auto each = [&](auto f) __attribute__((always_inline)) {
+            for (int c = 0; c < p.chunks; c++) {
+                if (stat[c].top == -INFINITY) continue;
+                float x[EACH];
+                load<BF16>(p, row, c, x);
+#pragma unroll
+                for (int e = 0; e < EACH; e++)
+                    if (x[e] > -INFINITY) f(x[e], number(x[e], index_of<BF16>(c, e)));
+            }
+        };
+        // (up to 2^22 of them: units of 2^-40 leave room for the sum)
+        const auto worth = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.inv)) + 256) >> 9; };
+        if (h.k) last = search(h.k, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
+        if (h.p < 1.f) {
+            u64 w = 0;
+            each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) w += worth(x); });
+            w = sum_all(w, room);
+            const double need = ceil((double)h.p * (double)w);
+            const u64 border = search(need < 1.0 ? 1 : (u64)need, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) f(c, worth(x)); });
+            });
+            last = std::min(last, border);
+        }
+        for (int c = 0; c < p.chunks; c++) {
+            u64 w = 0;
+            if (stat[c].top > -INFINITY) {
+                float x[EACH];
+                load<BF16>(p, row, c, x);
+#pragma unroll
+                for (int e = 0; e < EACH; e++)
+                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += units(weight(x[e], stat[c].top, h.inv));
+            }
+            w = sum_all(w, room);
+            if (tid == 0) chunks[c] = w;
+        }
+    } else if (r.how == PLAIN) {
+        for (int c = tid; c < p.chunks; c += LANES) chunks[c] = stat[c].top == -INFINITY ? 0 : stat[c].sum;
+    }
+    __syncthreads();
+    if (tid == 0) {   // the chunk, and how much of it lies before the token
+        double all = 0.0;
+        for (int c = 0; c < p.chunks; c++)
+            if (chunks[c]) all += weight(stat[c].top, r.top, h.inv) * UNIT * (double)chunks[c];
+        double u = p.u_f64 ? ((const double*)p.u)[row] : (double)((const float*)p.u)[row];
+        u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
+        const double want = u * all;
+        double before = 0.0;
+        int at = -1;
+        target[0] = 0.0;
+        for (int c = 0; c < p.chunks; c++) {
+            if (!chunks[c]) continue;
+            const double f = weight(stat[c].top, r.top, h.inv) * UNIT, mine = f * (double)chunks[c];
+            at = c;
+            target[0] = (want - before) / f;
+            if (before + mine > want) break;
+            before += mine;
+        }
+        begins[0] = at;
+        target[1] = all;
+        found[0] = found[1] = ~0ull;
+    }
+    __syncthreads();
+    const int chunk = begins[0];
+    if (chunk < 0) {   // (no row comes here: its largest logit is kept)
+        if (tid == 0) {
+            p.token[row] = -1;
+            if (p.prob) p.prob[row] = 0.f;
+        }
+        return;
+    }
+    const u64 want = target[0] > 0.0 ? (u64)target[0] : 0;
+    const float top = stat[chunk].top;
+    // a lane's 16 logits one after the other
+    u64 w[EACH], mine = 0;
+    const int first = chunk * CHUNK + tid * EACH;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const float x = first + e < p.vocab ? clean(load1<BF16>(p, row, first + e)) : -INFINITY;
+        const bool in = x > -INFINITY && (r.how == PLAIN || (number(x, first + e) <= last && stays(x) && (r.how == SEARCH || r.grid - place(x, h.scale) <= r.to)));
+        w[e] = in ? units(weight(x, top, h.inv)) : 0;
+        mine += w[e];
+    }
+    u64 before = mine;   // sums up to the lane
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 y = __shfl_up(before, d);
+        if ((tid & 63) >= d) before += y;
+    }
+    if ((tid & 63) == 63) room[tid >> 6] = before;
+    __syncthreads();
+    u64 ahead = 0;
+    for (int y = 0; y < (tid >> 6); y++) ahead += room[y];
+    before += ahead - mine;
+    int hit = -1, some = -1;
+    u64 hit_w = 0, some_w = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        before += w[e];
+        if (w[e]) {
+            some = first + e;
+            some_w = w[e];
+        }
+        if (hit < 0 && w[e] && before > want) {
+            hit = first + e;
+            hit_w = w[e];
+        }
+    }
+    // the first hit; where rounding left none, the last token that is kept
+    const u64 best = over_all(hit < 0 ? ~0ull : (u64)hit, room, [](u64 a, u64 b) { return a < b ? a : b; });
+    const u64 end = over_all((u64)(some + 1), room, [](u64 a, u64 b) { return a > b ? a : b; });
+    const bool is = best != ~0ull ? hit == (int)best : some + 1 == (int)end && some >= 0;
+    if (is) {
+        p.token[row] = best != ~0ull ? hit : some;
+        if (p.prob) p.prob[row] = (float)((double)(best != ~0ull ? hit_w : some_w) * UNIT * weight(top, r.top, h.inv) / target[1]);
+    }
+}
+
+struct Sizes { int64_t stat, row, hist_n, hist_w, kept, count, list, all; int chunks; };
+Sizes sizes(const spinf_sample_args* a, bool filters) {
+    Sizes s;
+    s.chunks = (int)((a->vocab + CHUNK - 1) / CHUNK);
+    const int64_t n = a->rows * s.chunks;
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) { const int64_t x = at; at += (bytes + 15) / 16 * 16; return x; };
+    s.stat = take(n * (int64_t)sizeof(Stat));
+    s.row = take(filters ? a->rows * (int64_t)sizeof(Row) : 0);
+    s.hist_w = take(filters ? n * BINS * 8 : 0);
+    s.hist_n = take(filters ? n * BINS * 4 : 0);
+    s.kept = take(filters ? n * 8 : 0);
+    s.count = take(filters ? n * 4 : 0);
+    s.list = take(filters ? n * SEGMENT * 8 : 0);
+    s.all = at;
+    return s;
+}
+
+bool any_filter(const spinf_sample_args* a) { return a->top_k || a->top_p || a->min_p || a->all_top_k > 0 || a->all_top_p < 1.f || a->all_min_p > 0.f; }
+
+int check(const spinf_sample_args* a, const char* what) {
+    if (!a) return spinf_fail(SPINF_E_ARG, "%s: null args", what);
+    if (a->rows < 0 || a->rows > 65535 || a->vocab < 1 || a->vocab > (int64_t)CHUNK * MOST_CHUNKS) return spinf_fail(SPINF_E_ARG, "%s: %lld rows (at most 65,535) of %lld logits (1 .. 2^22)", what, (long long)a->rows, (long long)a->vocab);
+    if (a->dtype != 0 && a->dtype != 1) return spinf_fail(SPINF_E_ARG, "%s: dtype %d (0 = fp32, 1 = bf16)", what, a->dtype);
+    if (a->ld < a->vocab) return spinf_fail(SPINF_E_ARG, "%s: rows %lld apart of %lld logits", what, (long long)a->ld, (long long)a->vocab);
+    if ((!a->temperature && !(a->all_temperature >= 0.f)) || (!a->top_p && !(a->all_top_p >= 0.f)) || (!a->min_p && !(a->all_min_p >= 0.f)))
+        return spinf_fail(SPINF_E_ARG, "%s: temperature %g, top-p %g, min-p %g must not be negative", what, (double)a->all_temperature, (double)a->all_top_p, (double)a->all_min_p);
+    return SPINF_OK;
+}
+
+template <bool BF16>
+hipError_t launch(const Params& p, bool filters, hipStream_t s) {
+    hipLaunchKernelGGL(sample_chunks_kernel<BF16>, dim3(p.chunks, p.rows), dim3(LANES), 0, s, p);
+    hipError_t e = hipGetLastError();
+    if (filters) {
+        if (e == hipSuccess) {
+            hipLaunchKernelGGL(sample_rows_kernel, dim3(p.rows), dim3(BINS), 0, s, p);
+            e = hipGetLastError();
+        }
+        if (e == hipSuccess) {
+            hipLaunchKernelGGL(sample_gather_kernel<BF16>, dim3(p.chunks, p.rows), dim3(LANES), 0, s, p);
+            e = hipGetLastError();
+        }
+    }
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(sample_draw_kernel<BF16>, dim3(p.rows), dim3(LANES), 0, s, p, filters);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // namespace
+
+extern "C" int spinf_sample_workspace(const spinf_sample_args* a, int64_t* bytes) {
+    const int rc = check(a, "sample_workspace");
+    if (rc) return rc;
+    if (!bytes) return spinf_fail(SPINF_E_ARG, "sample_workspace: null pointer");
+    *bytes = sizes(a, any_filter(a)).all;
+    return SPINF_OK;
+}
+
+extern "C" int spinf_sample(const spinf_sample_args* a, void* stream) {
+    const int rc = check(a, "sample");
+    if (rc) return rc;
+    if (a->rows == 0) return SPINF_OK;
+    if (!a->logits || !a->u || !a->token) return spinf_fail(SPINF_E_ARG, "sample: null pointer");
+    const bool filters = any_filter(a);
+    const Sizes z = sizes(a, filters);
+    if (!a->workspace || a->workspace_bytes < z.all || (uintptr_t)a->workspace % 16) return spinf_fail(SPINF_E_ARG, "sample: needs a 16-byte aligned workspace of %lld bytes", (long long)z.all);
+    Params p = {};
+    p.logits = a->logits; p.ld = a->ld; p.vocab = (int)a->vocab; p.rows = (int)a->rows; p.chunks = z.chunks;
+    p.aligned = (uintptr_t)a->logits % 16 == 0 && a->ld % (a->dtype ? 8 : 4) == 0;
+    p.u = a->u; p.u_f64 = a->u_f64 != 0;
+    p.temperature = a->temperature; p.top_k = a->top_k; p.top_p = a->top_p; p.min_p = a->min_p;
+    p.all_temperature = a->all_temperature; p.all_top_k = a->all_top_k; p.all_top_p = a->all_top_p; p.all_min_p = a->all_min_p;
+    p.token = (long*)a->token; p.prob = a->prob;
+    char* w = (char*)a->workspace;
+    p.stat = (Stat*)(w + z.stat); p.row = (Row*)(w + z.row); p.hist_n = (int*)(w + z.hist_n); p.hist_w = (u64*)(w + z.hist_w);
+    p.kept = (u64*)(w + z.kept); p.count = (int*)(w + z.count); p.list = (uint2*)(w + z.list);
+    const hipError_t e = a->dtype ? launch<true>(p, filters, (hipStream_t)stream) : launch<false>(p, filters, (hipStream_t)stream);
+    return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "sample: launch: %s", hipGetErrorString(e));
+}

@@ -1,0 +1,747 @@
+// Attention of a decoding step over contents that seats share and over their own keys, for gfx950 (MI355X), from work lists that seats_step.hip leaves in device memory.  No
+// counterpart in the reference, whose contents are read anew with every request.
+//
+// Mathematics.  Row = new token x query head; it sees its content's P stored keys and its seat's own up to its own place: out = (sum_A p v + sum_B p v) / (sum_A p + sum_B p), p =
+// exp(t - ref).  The sums over a content's keys are one product per key / value head for all rows that go on below it, so its keys are read once per 128 rows and not once
+// per seat; the sums over own keys are made seat by seat; a piece leaves its reference, its sum and its weighted values in 32 bits, and seats_join_kernel puts a row's pieces together.
+// Tiles, products and the softmax of a tile are those of paged_rows.h; a row sees one interval of a span's keys, so a mask is two comparisons.
+//
+// Kernels (lists of csrc/seats.h):
+//   wave   a seat's own keys: four (three at 512 dims) waves share 32 rows and divide the tiles, or, where the keys are few, take an item each.
+//   block  contents, and own keys of many new tokens: four waves with 32 rows each on shared double-buffered tiles.
+//   join   the pieces of every row; rows behind the step's last become zeros.
+// The lists' lengths are known on the GPU alone: grids have a bounded size and walk the lists.
+//
+// Keys that a row does not see leave no trace: as in paged_attn.hip, a workgroup that masked some tile and holds a result that is not finite looks whether masked tiles hold such
+// values, and if so computes its rows one by one over the keys they see.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "spinf_tree.h"
+#include "common.h"
+#include "seats.h"
+#include "attn_tiles.h"
+#include "paged_dev.h"
+#include "paged_rows.h"
+
+namespace {
+
+struct Params {
+    const __bf16* q; __bf16* out; float* lse;
+    long q_tok, q_head, o_tok, o_head;
+    const char* k; const char* v;
+    unsigned k_page, k_row, v_page, v_row; long k_head, v_head;   // bytes
+    bool same;                                                    // keys and values have the same strides
+    const int* lists; const int* first; const int* pos; const int* counts; const int* parts;
+    const SeatItem* wave; const SeatItem* single; const SeatItem* block;
+    float* part_o; float2* part_ml;
+    int hq, hkv, group, window, rows, seats;
+    int room[3];   // (the lists hold no more than they have room for, whatever their counts say)
+    PageDiv page;
+    Div by_group, by_heads;
+    SoftCap cap;
+};
+
+__device__ __forceinline__ SeatItem load_item(const SeatItem* items, int i) {
+    SeatItem it;
+    const int* p = (const int*)(items + i);
+    it.tok0 = sload(p, 0); it.T = sload(p, 1); it.L = sload(p, 2); it.tab = sload(p, 3);
+    it.row0 = sload(p, 4); it.kt0 = sload(p, 5); it.tiles = sload(p, 6); it.piece = sload(p, 7);
+    it.flo = sload(p, 8); it.fhi = sload(p, 9); it.flags = sload(p, 10);
+    return it;
+}
+__device__ __forceinline__ bool is_masked(const SeatItem& it, int kt) { return kt * TK < it.flo || kt * TK + TK - 1 > it.fhi; }
+
+// Where a tile lies: byte addresses of row 0 and row 16 of the key / value head's keys and values, and the tile's last stored row.  The pages are asked for a tile ahead.
+struct Pages {
+    int n, row0, row1, id0, id1;
+    __device__ __forceinline__ void ask(const Params& p, const SeatItem& it, int kt) {
+        n = 2 * kt;
+        const int a = p.page.of(n);
+        id0 = sload(p.lists, it.tab + a);
+        row0 = (n - a * p.page.d) * 16;
+        if (p.page.d & 1) {
+            const int end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, b = p.page.of(n1);
+            id1 = sload(p.lists, it.tab + b);
+            row1 = (n1 - b * p.page.d) * 16;
+        }
+    }
+};
+struct Place {
+    const char *k0, *k1, *v0, *v1;
+    int last;
+    __device__ __forceinline__ Place(const Params& p, const char* kb, const char* vb, int L, const Pages& g) {
+        last = L - 1 - g.n * 16 < TK - 1 ? L - 1 - g.n * 16 : TK - 1;
+        const unsigned long long ko = (unsigned long long)(unsigned)g.id0 * p.k_page + (unsigned long long)(unsigned)g.row0 * p.k_row;
+        k0 = kb + ko;
+        v0 = vb + (p.same ? ko : (unsigned long long)(unsigned)g.id0 * p.v_page + (unsigned long long)(unsigned)g.row0 * p.v_row);
+        if (p.page.d & 1) {
+            const unsigned long long k2 = (unsigned long long)(unsigned)g.id1 * p.k_page + (unsigned long long)(unsigned)g.row1 * p.k_row;
+            k1 = kb + k2;
+            v1 = vb + (p.same ? k2 : (unsigned long long)(unsigned)g.id1 * p.v_page + (unsigned long long)(unsigned)g.row1 * p.v_row);
+        } else {
+            k1 = k0 + 16 * (unsigned long long)p.k_row;
+            v1 = v0 + 16 * (unsigned long long)p.v_row;
+        }
+    }
+};
+
+// the keys lo .. hi of the span that token t of the item's set sees
+__device__ __forceinline__ void interval(const Params& p, const SeatItem& it, int t, int& lo, int& hi) {
+    const bool own = it.flags & SEAT_OWN;
+    const int at = it.L - it.T + t;   // its own place (of a seat's own keys)
+    hi = own ? at : it.L - 1;
+    lo = p.window ? (own ? at : p.pos[it.tok0 + t]) - p.window + 1 : INT_MIN;
+}
+
+// A wave's 32 rows, and the keys that they see
+template <int D, int DV, bool CAP>
+struct Rows : RowTile<D, DV, CAP> {
+    using B = RowTile<D, DV, CAP>;
+    using B::qf, B::lane, B::m, B::g, B::NS;
+    int lo, hi;
+
+    // queries of rows row0 + m, dims col ..
+    __device__ __forceinline__ void load(const Params& p, const SeatItem& it, int kvh, int row0, int col = 0) {
+        lane = threadIdx.x & 63;
+        m = lane & 31;
+        g = lane >> 5;
+        const int N = it.T * p.group, row = row0 + m, r = row < N ? row : N - 1;
+        const int tok = p.by_group.of(r), head = kvh * p.group + (r - tok * p.group);
+        const __bf16* qp = p.q + (long)(it.tok0 + tok) * p.q_tok + (long)head * p.q_head + col + 8 * g;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
+        interval(p, it, tok, lo, hi);
+        // (waited for here: left to the compiler, the wait would sit at the first use inside the tile loop, behind the DMAs in flight)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+#pragma unroll
+        for (int s = 0; s < NS; s++) asm volatile("" : "+v"(qf[s]));
+        asm volatile("" : "+v"(lo), "+v"(hi));
+    }
+    __device__ __forceinline__ void mask(int kt, f32x16& s) {
+        const int key = kt * TK + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int x = key + 8 * (i >> 2) + (i & 3);
+            s[i] = (x >= lo) & (x <= hi) ? s[i] : -INFINITY;
+        }
+    }
+};
+
+__device__ __forceinline__ void token_head(const Params& p, const SeatItem& it, int kvh, int row, int& tok, int& head) {
+    const int t = p.by_group.of(row);
+    tok = it.tok0 + t;
+    head = kvh * p.group + (row - t * p.group);
+}
+__device__ __forceinline__ long part_of(const Params& p, const SeatItem& it, int tok, int head) { return (long)(p.parts[tok] + it.piece) * p.hq + head; }
+
+// Do masked tiles of an item hold values that are not finite?  A wave looks at tiles w, w + nw ..
+template <int DV>
+__device__ bool rubbish(const Params& p, const SeatItem& it, int kvh, int vcol, int w, int nw) {
+    constexpr int PIECES = DV / 8;
+    const int lane = threadIdx.x & 63;
+    bool found = false;
+#pragma unroll 1
+    for (int i = w; i < it.tiles; i += nw) {
+        if (!is_masked(it, it.kt0 + i)) continue;
+        Pages pages;
+        pages.ask(p, it, it.kt0 + i);
+        const Place pl(p, p.k + kvh * p.k_head, p.v + kvh * p.v_head + vcol * 2, it.L, pages);
+#pragma unroll 1
+        for (int j = lane; j < TK * PIECES; j += 64) {
+            int r = j / PIECES;
+            r = r < pl.last ? r : pl.last;
+            const s16x8 x = *(const s16x8*)((r >= 16 ? pl.v1 : pl.v0) + (r & 15) * (unsigned long long)p.v_row + (j % PIECES) * 16);
+#pragma unroll
+            for (int k = 0; k < 8; k++) found |= (x[k] & 0x7f80) == 0x7f80;
+        }
+    }
+    return __builtin_amdgcn_ballot_w64(found) != 0;
+}
+
+// One row of an item by a whole wave, from memory, values touched only where the row sees the key.  state: the row's reference and sum as the tile loop found them: a
+// piece has one reference for all dims, also where the workgroup of the others does not come here (its values may be finite).
+template <int D, int DV, bool CAP>
+__device__ void slow_row(const Params& p, const SeatItem& it, int kvh, int j, int vcol, const float2 state) {
+    constexpr int VEC = DV / 64;   // output dims per lane
+    const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+    int tok, head, lo, hi;
+    token_head(p, it, kvh, it.row0 + j, tok, head);
+    interval(p, it, tok - it.tok0, lo, hi);
+    const __bf16* q = p.q + (long)tok * p.q_tok + (long)head * p.q_head + g * (D / 2);
+    const float ref = state.x == -INFINITY ? 0.f : state.x;
+    float o[VEC];
+#pragma unroll
+    for (int x = 0; x < VEC; x++) o[x] = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < it.tiles; i++) {
+        const int kt = it.kt0 + i;
+        Pages pages;
+        pages.ask(p, it, kt);
+        const Place pl(p, p.k + kvh * p.k_head, p.v + kvh * p.v_head, it.L, pages);
+        const int r = m < pl.last ? m : pl.last;
+        const bool vis = kt * TK + m >= lo && kt * TK + m <= hi;
+        // lane (m, g): half g of the dims of key m
+        const __bf16* kr = (const __bf16*)((r >= 16 ? pl.k1 : pl.k0) + (r & 15) * (unsigned long long)p.k_row) + g * (D / 2);
+        float s = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D / 2; d += 8) {
+            const bf16x8 a = *(const bf16x8*)(q + d), b = *(const bf16x8*)(kr + d);
+#pragma unroll
+            for (int x = 0; x < 8; x++) s = __builtin_fmaf((float)a[x], (float)b[x], s);
+        }
+        s = lane32_sum(s);
+        const float pr = vis ? __builtin_amdgcn_exp2f(__builtin_fmaf(CAP ? p.cap.of(s) : s, p.cap.unit, -ref)) : 0.f;
+        unsigned see = (unsigned)__builtin_amdgcn_ballot_w64(vis);
+#pragma unroll 1
+        while (see) {
+            const int key = __builtin_ctz(see);
+            see &= see - 1;
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pr), key));
+            const __bf16* vr = (const __bf16*)((key >= 16 ? pl.v1 : pl.v0) + (key & 15) * (unsigned long long)p.v_row) + vcol + VEC * lane;
+#pragma unroll
+            for (int x = 0; x < VEC; x++) o[x] = __builtin_fmaf(w, (float)vr[x], o[x]);
+        }
+    }
+    if (it.flags & SEAT_ONLY) {
+        __bf16* dst = p.out + (long)tok * p.o_tok + (long)head * p.o_head + vcol + VEC * lane;
+        const float inv = inverse(state.y);
+#pragma unroll
+        for (int x = 0; x < VEC; x++) dst[x] = (__bf16)(o[x] * inv);
+        if (p.lse && lane == 0 && vcol == 0) p.lse[(long)tok * p.hq + head] = log_sum(state.x, state.y);
+    } else {
+        const long part = part_of(p, it, tok, head);
+        float* dst = p.part_o + part * D + vcol + VEC * lane;
+#pragma unroll
+        for (int x = 0; x < VEC; x++) dst[x] = o[x];
+        if (lane == 0 && vcol == 0) p.part_ml[part] = state;
+    }
+}
+
+// eight dims of a row, as the last word or as a piece
+template <int D>
+__device__ __forceinline__ void put8(const Params& p, const SeatItem& it, int tok, int head, int d, const float (&x)[8]) {
+    if (it.flags & SEAT_ONLY) {
+        bf16x8 y;
+#pragma unroll
+        for (int k = 0; k < 8; k++) y[k] = (__bf16)x[k];
+        *(bf16x8*)(p.out + (long)tok * p.o_tok + (long)head * p.o_head + d) = y;
+    } else {
+        float* dst = p.part_o + part_of(p, it, tok, head) * D + d;
+        *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+__device__ __forceinline__ void put_sum(const Params& p, const SeatItem& it, int tok, int head, float M, float sum) {
+    if (!(it.flags & SEAT_ONLY)) p.part_ml[part_of(p, it, tok, head)] = make_float2(M, sum);
+    else if (p.lse) p.lse[(long)tok * p.hq + head] = log_sum(M, sum);
+}
+
+// ------------------------------------------------------------------------------------------------ a seat's own keys
+template <int D, int DV, int NW, bool CAP>
+__global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(const Params p) {
+    using R = Rows<D, DV, CAP>;
+    using GK = typename R::GK;
+    using GV = typename R::GV;
+    constexpr int OROW = DV + 4;   // floats of a row of the exchange (16 bytes of padding: rows of neighbouring lanes fall on other banks)
+    constexpr int TILE = GK::KTILEB + GV::VTILEB > 32 * OROW * 4 ? GK::KTILEB + GV::VTILEB : 32 * OROW * 4;   // a wave's rows take the place of its tile
+    __shared__ __attribute__((aligned(16))) char lds[NW * TILE];
+    __shared__ float2 ml[NW][32];
+    constexpr int NK = GK::NREG, NV = GV::NREG;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* const kb = lds + w * TILE;
+    char* const vb = kb + GK::KTILEB;
+    const unsigned k_at = lds_addr(kb), v_at = lds_addr(vb);
+    const int shared = seats_least(sload(p.counts, 0), p.room[0]) * p.hkv, alone = seats_least(sload(p.counts, 1), p.room[1]) * p.hkv;
+    const int units = shared + (alone + NW - 1) / NW;
+    const int last_unit = DV < D ? (units + 7) / 8 * 16 : units;
+    for (int u = blockIdx.x; u < last_unit; u += gridDim.x) {
+        int unit = u, vcol = 0;
+        if (DV < D) {   // (the workgroups of the two halves run on one XCD, close in time, and read the keys through one L2)
+            vcol = ((u >> 3) & 1) * DV;
+            unit = (u >> 4) * 8 + (u & 7);
+            if (unit >= units) continue;
+        }
+        const bool single = unit >= shared;
+        const int x = single ? (unit - shared) * NW + w : unit;
+        if (single && x >= alone) continue;   // (waves of these items meet nowhere: only the last unit of a workgroup's walk has idle ones)
+        const int item = p.by_heads.of(x), kvh = x - item * p.hkv;
+        const SeatItem it = load_item(single ? p.single : p.wave, item);
+        const char* const k_base = p.k + kvh * p.k_head;
+        const char* const v_base = p.v + kvh * p.v_head + vcol * 2;
+        const int step = single ? 1 : NW;
+        R rows;
+        bool seen_mask = false;
+        int kt = it.kt0 + (single ? 0 : w);
+        const int end = it.kt0 + it.tiles;
+        {
+            Pages pages;
+            if (kt < end) {   // (the first tile is asked for ahead of the queries: their latencies pass together)
+                pages.ask(p, it, kt);
+                const Place pl(p, k_base, v_base, it.L, pages);
+                const int lane = lane_now();
+                fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, lane);
+                fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, lane);
+            }
+            rows.load(p, it, kvh, it.row0);
+            rows.reset();
+            while (kt < end) {
+                const bool masked = is_masked(it, kt), next = kt + step < end;
+                seen_mask |= masked;
+                if (next) pages.ask(p, it, kt + step);
+                f32x16 s;
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(NV));   // the keys are there; the values may still be on their way
+                __builtin_amdgcn_sched_barrier(0);
+                rows.scores(kb, s);
+                if (CAP) p.cap.of(s);
+                if (masked) rows.mask(kt, s);
+                __builtin_amdgcn_s_waitcnt(LGKM0);           // nothing reads the tile's keys any more
+                __builtin_amdgcn_sched_barrier(0);
+                const Place pl(p, k_base, v_base, it.L, pages);
+                if (next) fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
+                bf16x8 pb[2];
+                rows.softmax(p.cap, s, pb);
+                if (!next) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+                else __builtin_amdgcn_s_waitcnt(vmcnt_imm(NK));
+                __builtin_amdgcn_sched_barrier(0);
+                rows.values(vb, pb);
+                __builtin_amdgcn_s_waitcnt(LGKM0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (next) fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, rows.lane);
+                kt += step;
+            }
+        }
+        const int left = it.T * p.group - it.row0, here = left < 32 ? left : 32;
+        const float sum = lane32_sum(rows.l);
+        if (sum == 0.f) rows.M = -INFINITY;   // no key seen
+        constexpr int PIECES = DV / 8;
+        float* const stage = (float*)lds;
+        if (single) {
+            if (seen_mask && rows.spoilt(left) && rubbish<DV>(p, it, kvh, vcol, 0, 1)) {
+                for (int j = 0; j < here; j++) {
+                    const float2 state = make_float2(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rows.M), j)), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), j)));
+                    slow_row<D, DV, CAP>(p, it, kvh, j, vcol, state);
+                }
+                continue;
+            }
+            const float f = it.flags & SEAT_ONLY ? inverse(sum) : 1.f;
+            float* const mine = (float*)kb;
+            if (rows.m < left) {
+#pragma unroll
+                for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; i4++)
+                        *(float4*)(mine + rows.m * OROW + 32 * dt + 8 * i4 + 4 * rows.g) =
+                            make_float4(rows.o[dt][4 * i4] * f, rows.o[dt][4 * i4 + 1] * f, rows.o[dt][4 * i4 + 2] * f, rows.o[dt][4 * i4 + 3] * f);
+                if (rows.g == 0 && vcol == 0) {
+                    int tok, head;
+                    token_head(p, it, kvh, it.row0 + rows.m, tok, head);
+                    put_sum(p, it, tok, head, rows.M, sum);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();   // (LDS operations of a wave are done in order)
+            for (int i = rows.lane; i < here * PIECES; i += 64) {
+                const int j = i / PIECES, d = (i - j * PIECES) * 8;
+                int tok, head;
+                token_head(p, it, kvh, it.row0 + j, tok, head);
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] = mine[j * OROW + d + k];
+                put8<D>(p, it, tok, head, vcol + d, y);
+            }
+            __builtin_amdgcn_s_waitcnt(LGKM0);   // (the next item's tile comes here)
+            __builtin_amdgcn_sched_barrier(0);
+            continue;
+        }
+        // ---- join the waves: every wave leaves its references and sums, then its accumulators scaled to the largest reference
+        if (rows.g == 0) ml[w][rows.m] = make_float2(rows.M, sum);
+        const bool again = __syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, kvh, vcol, w, NW));
+        __syncthreads();   // (and every wave is done with its tiles)
+        const auto joined = [&](int row) __attribute__((always_inline)) {   // a row's reference and sum
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int y = 0; y < NW; y++) top = fmaxf(top, ml[y][row].x);
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int y = 0; y < NW; y++) total += ml[y][row].y * (ml[y][row].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[y][row].x - ref));
+            return make_float2(top, total);
+        };
+        if (again) {
+            for (int j = w; j < here; j += NW) slow_row<D, DV, CAP>(p, it, kvh, j, vcol, joined(j));
+            __syncthreads();
+            continue;
+        }
+        const float2 state = joined(rows.m);
+        const float ref = state.x == -INFINITY ? 0.f : state.x;
+        const float f = (rows.M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(rows.M - ref)) * (it.flags & SEAT_ONLY ? inverse(state.y) : 1.f);
+        if (rows.m < left) {
+#pragma unroll
+            for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++)
+                    *(float4*)(stage + (w * 32 + rows.m) * OROW + 32 * dt + 8 * i4 + 4 * rows.g) =
+                        make_float4(rows.o[dt][4 * i4] * f, rows.o[dt][4 * i4 + 1] * f, rows.o[dt][4 * i4 + 2] * f, rows.o[dt][4 * i4 + 3] * f);
+            if (w == 0 && rows.g == 0 && vcol == 0) {
+                int tok, head;
+                token_head(p, it, kvh, it.row0 + rows.m, tok, head);
+                put_sum(p, it, tok, head, state.x, state.y);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < here * PIECES; i += 64 * NW) {
+            const int j = i / PIECES, d = (i - j * PIECES) * 8;
+            int tok, head;
+            token_head(p, it, kvh, it.row0 + j, tok, head);
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) y[k] = stage[j * OROW + d + k];
+#pragma unroll
+            for (int z = 1; z < NW; z++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] += stage[(z * 32 + j) * OROW + d + k];
+            put8<D>(p, it, tok, head, vcol + d, y);
+        }
+        __syncthreads();   // (the next item's tiles come here)
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ contents, and own keys of many new tokens
+// A tile's halves, found by a thread per tile, SPAN tiles at a time
+template <int SPAN>
+struct Halves { unsigned long long k[SPAN][2], v[SPAN][2]; };
+template <int SPAN>
+__device__ __forceinline__ void fill(Halves<SPAN>& h, const Params& p, const SeatItem& it, int from, const char* kb, const char* vb) {
+    const int t = threadIdx.x, i = from + t;
+    if (t < SPAN && i < it.tiles) {
+        const int n = 2 * (it.kt0 + i), end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, a = p.page.of(n), b = p.page.of(n1);
+        const unsigned ia = p.lists[it.tab + a], ib = p.lists[it.tab + b], ra = (n - a * p.page.d) * 16, rb = (n1 - b * p.page.d) * 16;
+        h.k[t][0] = (unsigned long long)kb + (unsigned long long)ia * p.k_page + (unsigned long long)ra * p.k_row;
+        h.k[t][1] = (unsigned long long)kb + (unsigned long long)ib * p.k_page + (unsigned long long)rb * p.k_row;
+        h.v[t][0] = (unsigned long long)vb + (unsigned long long)ia * p.v_page + (unsigned long long)ra * p.v_row;
+        h.v[t][1] = (unsigned long long)vb + (unsigned long long)ib * p.v_page + (unsigned long long)rb * p.v_row;
+    }
+}
+
+// 512 dims: two waves share 32 rows, each with one half of the dims of queries, keys, values and outputs; their scores are exchanged through the place of the tile's keys,
+// which nobody reads any more, and added: both then hold the same bits and the same softmax.
+template <int D, int DV, bool CAP>
+__global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block_kernel(const Params p) {
+    constexpr int H = D / DV;
+    using R = Rows<DV, DV, CAP>;
+    using GK = typename R::GK;
+    using GV = typename R::GV;
+    constexpr int HALF = GK::KTILEB + GV::VTILEB, BUF = H * HALF;
+    constexpr int OROW = DV * 2 + 16;   // bytes of an output row in LDS
+    constexpr int LDS = 2 * BUF > H * 4 * 32 * OROW ? 2 * BUF : H * 4 * 32 * OROW;
+    constexpr int NK = GK::NREG / 4, NV = GV::NREG / 4;
+    constexpr int SPAN = 128;
+    static_assert(NK * 4 == GK::NREG && NV * 4 == GV::NREG, "a tile's regions must divide among the four waves");
+    static_assert((D == 256 ? 2 : 1) * (LDS + sizeof(Halves<SPAN>)) <= 160 * 1024, "LDS budget");
+    static_assert(H == 1 || 4 * 4096 <= GK::KTILEB, "four waves' scores take the place of a half's keys");
+    __shared__ __attribute__((aligned(16))) char lds[LDS];
+    __shared__ Halves<SPAN> at;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = H == 1 ? wave : wave & 3, half = H == 1 ? 0 : wave >> 2, vcol = half * DV;
+    const unsigned base = lds_addr(lds) + half * HALF;
+    const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
+        const SeatItem it = load_item(p.block, item);
+        const char* const k_base = p.k + kvh * p.k_head;
+        const char* const v_base = p.v + kvh * p.v_head;
+        fill<SPAN>(at, p, it, 0, k_base, v_base);
+        R rows;
+
+        // This lane's place in the regions that its wave copies: rows r + x (x < NK, NV) of the tile, which lie in one half of it
+        const auto k_row = [&](int lane) { return w * NK + GK::NREG * (lane / GK::CPR); };
+        const auto v_row = [&](int lane) { return w * NV + GV::NREG * (lane / GV::CPR); };
+        const auto issue = [&](int i, int kt, int buf) __attribute__((always_inline)) {
+            const unsigned to = base + buf * BUF;
+            const int lane = lane_now(), last = it.L - 1 - kt * TK;
+            if (last >= TK - 1) {
+                const char* ka = (const char*)at.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16 + vcol * 2);
+                const char* va = (const char*)at.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16 + vcol * 2);
+#pragma unroll
+                for (int x = 0; x < NK; x++, ka += p.k_row) dma16_lane(ka, to + (w * NK + x) * GK::KRS);
+#pragma unroll
+                for (int x = 0; x < NV; x++, va += p.v_row) dma16_lane(va, to + GK::KTILEB + (w * NV + x) * GV::VRS);
+            } else {   // the span's last tile: rows behind the stored keys are the last key's
+#pragma unroll
+                for (int x = 0; x < NK; x++) {
+                    const int r = k_row(lane) + x < last ? k_row(lane) + x : last;
+                    dma16_lane((const char*)at.k[i][r >> 4] + (r & 15) * (unsigned long long)p.k_row + lane % GK::CPR * 16 + vcol * 2, to + (w * NK + x) * GK::KRS);
+                }
+#pragma unroll
+                for (int x = 0; x < NV; x++) {
+                    const int r = v_row(lane) + x < last ? v_row(lane) + x : last;
+                    dma16_lane((const char*)at.v[i][r >> 4] + (r & 15) * (unsigned long long)p.v_row + lane % GV::CPR * 16 + vcol * 2, to + GK::KTILEB + (w * NV + x) * GV::VRS);
+                }
+            }
+        };
+
+        bool seen_mask = false;
+        __syncthreads();
+        if (it.tiles > 0) issue(0, it.kt0, 0);   // (ahead of the queries: their latencies pass together)
+        rows.load(p, it, kvh, it.row0 + 32 * w, vcol);
+        rows.reset();
+        for (int i = 0, j = 0, buf = 0; i < it.tiles; i++, buf ^= 1) {   // j: tile i's place among the halves
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
+            __syncthreads();                            // ... and everybody's; the other buffer is free
+            if (++j == SPAN) {                          // (the last tile of the span in hand has been requested)
+                j = 0;
+                fill<SPAN>(at, p, it, i + 1, k_base, v_base);
+                __syncthreads();
+            }
+            const int kt = it.kt0 + i;
+            if (i + 1 < it.tiles) issue(j, kt + 1, buf ^ 1);
+            const bool masked = is_masked(it, kt);
+            seen_mask |= masked;
+            char* kb = lds + buf * BUF + half * HALF;
+            f32x16 s;
+            rows.scores(kb, s);
+            if (H == 2) {
+                char* const mine = kb + w * 4096 + lane_now() * 16;
+                const char* const other = mine + (half ? -HALF : HALF);
+                __syncthreads();   // every wave is done with the keys
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++) *(float4*)(mine + i4 * 1024) = make_float4(s[4 * i4], s[4 * i4 + 1], s[4 * i4 + 2], s[4 * i4 + 3]);
+                __syncthreads();
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++) {
+                    const float4 x = *(const float4*)(other + i4 * 1024);
+                    s[4 * i4] += x.x;
+                    s[4 * i4 + 1] += x.y;
+                    s[4 * i4 + 2] += x.z;
+                    s[4 * i4 + 3] += x.w;
+                }
+            }
+            if (CAP) p.cap.of(s);
+            if (masked) rows.mask(kt, s);
+            bf16x8 pb[2];
+            rows.softmax(p.cap, s, pb);
+            rows.values(kb + GK::KTILEB, pb);
+        }
+        const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
+        const float sum = lane32_sum(rows.l);
+        if (sum == 0.f) rows.M = -INFINITY;   // no key seen
+        // (also the barrier behind which the tile buffers are free)
+        if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, kvh, vcol, w, 4))) {
+            for (int j = 0; j < 32 && j < left; j++) {
+                const float2 state = make_float2(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rows.M), j)), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), j)));
+                slow_row<D, DV, CAP>(p, it, kvh, 32 * w + j, vcol, state);
+            }
+            __syncthreads();
+            continue;
+        }
+        const float f = it.flags & SEAT_ONLY ? inverse(sum) : 1.f;
+        const int lane = lane_now(), m = lane & 31, g = lane >> 5;
+        if (it.flags & SEAT_ONLY) {   // rows through the wave's own slice of LDS, stored as 16-byte pieces
+            char* const stage = lds + wave * 32 * OROW;
+#pragma unroll
+            for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++) {
+                    bf16x4 x;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[j] = (__bf16)(rows.o[dt][4 * i4 + j] * f);
+                    *(bf16x4*)(stage + m * OROW + (32 * dt + 8 * i4 + 4 * g) * 2) = x;
+                }
+            if (p.lse && g == 0 && m < left && vcol == 0) {
+                int tok, head;
+                token_head(p, it, kvh, it.row0 + 32 * w + m, tok, head);
+                p.lse[(long)tok * p.hq + head] = log_sum(rows.M, sum);
+            }
+            constexpr int PIECES = DV / 8;
+#pragma unroll
+            for (int k = 0; k < 32 * PIECES / 64; k++) {
+                const int i = k * 64 + lane, j = i / PIECES, d = (i - j * PIECES) * 8;
+                if (j < left) {
+                    int tok, head;
+                    token_head(p, it, kvh, it.row0 + 32 * w + j, tok, head);
+                    *(bf16x8*)(p.out + (long)tok * p.o_tok + (long)head * p.o_head + vcol + d) = *(const bf16x8*)(stage + j * OROW + d * 2);
+                }
+            }
+        } else if (m < left) {
+            int tok, head;
+            token_head(p, it, kvh, it.row0 + 32 * w + m, tok, head);
+            const long part = part_of(p, it, tok, head);
+            if (g == 0 && vcol == 0) p.part_ml[part] = make_float2(rows.M, sum);
+            float* po = p.part_o + part * D + vcol;
+#pragma unroll
+            for (int dt = 0; dt < R::NDT; dt++)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++)
+                    *(float4*)(po + 32 * dt + 8 * i4 + 4 * g) = make_float4(rows.o[dt][4 * i4], rows.o[dt][4 * i4 + 1], rows.o[dt][4 * i4 + 2], rows.o[dt][4 * i4 + 3]);
+        }
+        __syncthreads();   // (the next item's tiles and halves come here)
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ pieces joined
+// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per token and 64 dims of its heads (or some of them: blockIdx.y); 16 lanes hold a piece of
+// a head, `share` such groups take a head's pieces in turn, each with a reference of its own, and are added up in one fixed order.
+template <int D>
+__global__ __launch_bounds__(256) void seats_join_kernel(const Params p) {
+    constexpr int SLICES = D / 64, GROUPS = 16;
+    __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
+    __shared__ float2 part_ml[GROUPS];
+    const int tok = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
+    const int first = sload(p.parts, tok), n = sload(p.parts, tok + 1) - first;
+    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
+    if (n == 0) {
+        if (tok < sload(p.first, p.seats)) return;   // its only piece is the last word
+        for (int h = blockIdx.y * GROUPS + group; h < p.hq; h += gridDim.y * GROUPS) {
+            *(uint2*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = make_uint2(0, 0);
+            if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = -INFINITY;
+        }
+        return;
+    }
+    int share = 1;   // (each group asks for four pieces at a time)
+    while (share < GROUPS && share * 4 < n) share *= 2;
+    const int heads = GROUPS / share, piece = group % share;
+    for (int h0 = blockIdx.y * heads; h0 < p.hq; h0 += gridDim.y * heads) {
+        const int h = h0 + group / share;
+        const bool on = h < p.hq;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, total = 0.f;
+        // (a piece without a visible key holds zeros, or NaN that stays)
+        auto add = [&](const float4& x, float m, float l, float ref) {
+            const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);
+            acc[0] = __builtin_fmaf(f, x.x, acc[0]);
+            acc[1] = __builtin_fmaf(f, x.y, acc[1]);
+            acc[2] = __builtin_fmaf(f, x.z, acc[2]);
+            acc[3] = __builtin_fmaf(f, x.w, acc[3]);
+            total = __builtin_fmaf(f, l, total);
+        };
+        if (on)
+            for (int s0 = piece; s0 < n; s0 += 4 * share) {   // four pieces requested at a time
+                float4 x[4];
+                float2 ml[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int s = s0 + k * share;
+                    const long at = (long)(first + (s < n ? s : s0)) * p.hq + h;
+                    x[k] = *(const float4*)(p.part_o + at * D + slice * 64 + d);
+                    ml[k] = p.part_ml[at];
+                }
+                float ref = top;
+#pragma unroll
+                for (int k = 0; k < 4; k++) ref = fmaxf(ref, ml[k].x);   // (a piece asked for twice changes no maximum)
+                if (top != -INFINITY) {
+                    const float f = __builtin_amdgcn_exp2f(top - ref);
+                    total *= f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[k] *= f;
+                }
+                top = ref;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (s0 + k * share < n) add(x[k], ml[k].x, ml[k].y, ref);
+            }
+        if (share > 1) {
+            __syncthreads();   // (the room is free)
+            *(float4*)&part_sum[group][d] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (d == 0) part_ml[group] = make_float2(top, total);
+            __syncthreads();
+            if (piece == 0) {
+                const int used = n < share ? n : share;
+                const float m0 = top, l0 = total;
+                for (int s = 1; s < used; s++) top = fmaxf(top, part_ml[group + s].x);
+                total = 0.f;
+                const float4 own = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+                add(own, m0, l0, top);
+                for (int s = 1; s < used; s++) {
+                    const float2 ml = part_ml[group + s];
+                    add(*(const float4*)&part_sum[group + s][d], ml.x, ml.y, top);
+                }
+            }
+        }
+        if (on && piece == 0) {
+            const float f = inverse(total);
+            bf16x4 y;
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = (__bf16)(acc[k] * f);
+            *(bf16x4*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = y;
+            if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = log_sum(top, total);
+        }
+    }
+}
+
+constexpr int AT_ONCE = 2048;   // workgroups of a launch that walk a list
+
+template <int D, int DV, int NW, bool CAP>
+int launch(const Params& p, const spinf_seats_attn_args* a, hipStream_t s) {
+    const auto grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>(n, AT_ONCE)); };
+    hipLaunchKernelGGL((seats_block_kernel<D, DV, CAP>), grid(a->rooms[2] * p.hkv), dim3(256 * (D / DV)), 0, s, p);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+        const int64_t units = a->rooms[0] * p.hkv + (a->rooms[1] * p.hkv + NW - 1) / NW;
+        hipLaunchKernelGGL((seats_wave_kernel<D, DV, NW, CAP>), grid(DV < D ? (units + 7) / 8 * 16 : units), dim3(64 * NW), 0, s, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) {
+        const int y = p.rows * (D / 64) >= 1024 ? 1 : std::min(p.hq, (1024 + p.rows * (D / 64) - 1) / (p.rows * (D / 64)));
+        hipLaunchKernelGGL((seats_join_kernel<D>), dim3((unsigned)(p.rows * (D / 64)), (unsigned)y), dim3(256), 0, s, p);
+        e = hipGetLastError();
+    }
+    return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "seats_attn: launch: %s", hipGetErrorString(e));
+}
+
+template <int D, int DV, int NW>
+int launch_cap(const Params& p, const spinf_seats_attn_args* a, hipStream_t s) {
+    return p.cap.on ? launch<D, DV, NW, true>(p, a, s) : launch<D, DV, NW, false>(p, a, s);
+}
+
+}  // namespace
+
+extern "C" int spinf_seats_attn_fwd(const spinf_seats_attn_args* a, void* stream) {
+    if (!a) return spinf_fail(SPINF_E_ARG, "seats_attn: null args");
+    const spinf_seats_kind& kd = a->kind;
+    if (a->rows < 1 || a->rows > (1 << 22) || a->seats < 1 || a->seats > SEATS_MOST) return spinf_fail(SPINF_E_ARG, "seats_attn: %lld rows of %d seats", (long long)a->rows, a->seats);
+    if (kd.hq <= 0 || kd.hkv <= 0 || kd.hq % kd.hkv || a->rows * kd.hq > (1 << 30)) return spinf_fail(SPINF_E_ARG, "seats_attn: %d query heads do not group over %d key / value heads", kd.hq, kd.hkv);
+    if (a->page < 16 || a->page % 16 || a->page > (1 << 20)) return spinf_fail(SPINF_E_ARG, "seats_attn: pages of %d keys (a multiple of 16)", a->page);
+    if (kd.window < 0) return spinf_fail(SPINF_E_ARG, "seats_attn: window %d", kd.window);
+    if (!(a->scale > 0.f) || !(a->scale < INFINITY) || !(a->softcap >= 0.f) || !(a->softcap < INFINITY))
+        return spinf_fail(SPINF_E_ARG, "seats_attn: scale %g must be positive and finite, softcap %g not negative", (double)a->scale, (double)a->softcap);
+    if (!a->q || !a->out || !a->k || !a->v || !a->lists || !a->first || !a->pos || !kd.wave || !kd.single || !kd.block || !kd.counts || !kd.parts)
+        return spinf_fail(SPINF_E_ARG, "seats_attn: null pointer");
+    for (const void* ptr : {a->q, (const void*)a->out, a->k, a->v, (const void*)kd.wave, (const void*)kd.single, (const void*)kd.block})
+        if ((uintptr_t)ptr % 16) return spinf_fail(SPINF_E_ARG, "seats_attn: tensors and lists must be 16-byte aligned");
+    for (int64_t st : {a->q_tok, a->q_head, a->o_tok, a->o_head, a->k_page, a->k_row, a->k_head, a->v_page, a->v_row, a->v_head})
+        if (st % 8) return spinf_fail(SPINF_E_ARG, "seats_attn: strides must be multiples of 8 elements");
+    if (a->k_row < 0 || a->v_row < 0 || a->k_row > (1 << 24) || a->v_row > (1 << 24) || a->k_page < 0 || a->v_page < 0 || a->k_page > (1u << 30) || a->v_page > (1u << 30))
+        return spinf_fail(SPINF_E_ARG, "seats_attn: strides of the cache must lie in 0 .. 2^24 elements (rows) and 0 .. 2^30 (pages)");   // (32-bit byte counts; 32 rows by 32-bit offsets)
+    for (int i = 0; i < 4; i++)
+        if (a->rooms[i] < (i < 3) || a->rooms[i] > (1 << 30) || (i < 3 && a->rooms[i] * kd.hkv > (1 << 30))) return spinf_fail(SPINF_E_ARG, "seats_attn: bad lengths of lists");
+    const int64_t parts = a->rooms[3] * kd.hq, need = parts * (kd.d + 2) * 4;
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
+        return spinf_fail(SPINF_E_ARG, "seats_attn: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    Params p = {};
+    p.q = (const __bf16*)a->q; p.out = (__bf16*)a->out; p.lse = a->lse;
+    p.q_tok = a->q_tok; p.q_head = a->q_head; p.o_tok = a->o_tok; p.o_head = a->o_head;
+    p.k = (const char*)a->k; p.v = (const char*)a->v;
+    p.k_page = (unsigned)(2 * a->k_page); p.k_row = (unsigned)(2 * a->k_row); p.k_head = 2 * a->k_head;
+    p.v_page = (unsigned)(2 * a->v_page); p.v_row = (unsigned)(2 * a->v_row); p.v_head = 2 * a->v_head;
+    p.same = a->k_page == a->v_page && a->k_row == a->v_row;
+    p.lists = a->lists; p.first = a->first; p.pos = a->pos; p.counts = kd.counts; p.parts = kd.parts;
+    p.wave = (const SeatItem*)kd.wave; p.single = (const SeatItem*)kd.single; p.block = (const SeatItem*)kd.block;
+    p.part_o = (float*)a->workspace;
+    p.part_ml = (float2*)(p.part_o + parts * kd.d);
+    p.hq = kd.hq; p.hkv = kd.hkv; p.group = kd.hq / kd.hkv; p.rows = (int)a->rows; p.seats = a->seats;
+    p.window = kd.window < 1 << 30 ? kd.window : 1 << 30;
+    for (int i = 0; i < 3; i++) p.room[i] = (int)a->rooms[i];
+    p.page = PageDiv::of_page(a->page);
+    p.by_group = Div::by(p.group);
+    p.by_heads = Div::by(p.hkv);
+    if (!SoftCap::of(a->scale, a->softcap, p.cap)) return spinf_fail(SPINF_E_ARG, "seats_attn: scale %g and softcap %g leave fp32's range", (double)a->scale, (double)a->softcap);
+    hipStream_t s = (hipStream_t)stream;
+    switch (kd.d) {
+        case 64: return launch_cap<64, 64, 4>(p, a, s);
+        case 128: return launch_cap<128, 128, 4>(p, a, s);
+        case 256: return launch_cap<256, 256, 4>(p, a, s);
+        case 512: return launch_cap<512, 256, 3>(p, a, s);
+        default: return spinf_fail(SPINF_E_ARG, "seats_attn: head dim %d not supported (64, 128, 256, 512)", kd.d);
+    }
+}

@@ -8,6 +8,8 @@
   decode      XCaches, GroupKV, x_attention: the extraction decoder's attention step (spinf_serve/decode.py:35-104)
   paged       PagedCache, PagedBatch, paged_attn, paged_weights, cache_evict: a paged cache of contents read before, the attention of new
               tokens over it, and what keeps it small
+  seats       PagedSeats, seats_attn: requests that go on token by token below shared contents, lengths and pages on the GPU
+  sample      sample_tokens: tokens drawn from logits by given random numbers
   rope        qk_norm_rope, qk_norm_rope_put: norms and rotation of queries and keys, and their way into the cache
   synth       seeded synthetic workloads of the benchmark configurations
 
@@ -24,5 +26,7 @@ from .gdn_layer import gdn_gate, gdn_prologue  # noqa: F401
 from .lm_head import lm_head_logprobs, lm_logprobs  # noqa: F401
 from .decode import GroupKV, XCaches, x_attention, xdecode_attn  # noqa: F401
 from .paged import PagedBatch, PagedCache, cache_evict, paged_attn, paged_weights  # noqa: F401
+from .seats import PagedSeats, seats_attn  # noqa: F401
+from .sample import sample_tokens  # noqa: F401
 from .rope import qk_norm_rope, qk_norm_rope_put  # noqa: F401
 from .qwen_plan import Call, TreePlan, gdn_tree, tree_plan  # noqa: F401

@@ -160,6 +160,51 @@ class RopeArgs(C.Structure):
     ]
 
 
+class SeatsKind(C.Structure):
+    _fields_ = [
+        ("wave", C.c_void_p), ("single", C.c_void_p), ("block", C.c_void_p), ("counts", C.c_void_p), ("parts", C.c_void_p), ("seat_parts", C.c_void_p),
+        ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("window", C.c_int32),
+    ]
+
+
+class SeatsArgs(C.Structure):
+    _fields_ = [
+        ("come", C.c_void_p), ("drop", C.c_void_p), ("content", C.c_void_p),
+        ("lens", C.c_void_p), ("lists", C.c_void_p), ("free", C.c_void_p), ("left", C.c_void_p), ("first", C.c_void_p), ("took", C.c_void_p), ("stay", C.c_void_p),
+        ("slots", C.c_void_p), ("pos", C.c_void_p),
+        ("shared", C.c_void_p),
+        ("rows", C.c_int64), ("keys", C.c_int64), ("pool", C.c_int64), ("table_at", C.c_int64), ("longest", C.c_int64),
+        ("seats", C.c_int32), ("page", C.c_int32), ("contents", C.c_int32), ("kinds", C.c_int32),
+        ("kind", SeatsKind * 8),
+    ]
+
+
+class SeatsAttnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_tok", C.c_int64), ("q_head", C.c_int64), ("o_tok", C.c_int64), ("o_head", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("lists", C.c_void_p), ("first", C.c_void_p), ("pos", C.c_void_p),
+        ("kind", SeatsKind), ("rooms", C.c_int64 * 4),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("rows", C.c_int64),
+        ("seats", C.c_int32), ("page", C.c_int32),
+        ("scale", C.c_float), ("softcap", C.c_float),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("ld", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64),
+        ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+        ("token", C.c_void_p), ("prob", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("all_temperature", C.c_float), ("all_top_p", C.c_float), ("all_min_p", C.c_float), ("all_top_k", C.c_int32),
+        ("dtype", C.c_int32), ("u_f64", C.c_int32),
+    ]
+
+
 def library_path() -> str:
     return os.environ.get("SPINF_TREE_LIB", os.path.join(_HERE, "libspinf_tree.so"))
 
@@ -233,7 +278,13 @@ def _bind(lib, path):
     lib.spinf_cache_evict.argtypes = [C.POINTER(EvictArgs), C.c_void_p]
     lib.spinf_qk_norm_rope.argtypes = [C.POINTER(RopeArgs), C.c_void_p]
     lib.spinf_paged_struct_sizes.argtypes = [C.POINTER(C.c_int64), C.c_int32]
-    for name in ("spinf_paged_plan_build", "spinf_paged_plan_counts", "spinf_paged_plan_export", "spinf_paged_attn_fwd", "spinf_paged_weights", "spinf_cache_evict", "spinf_qk_norm_rope", "spinf_paged_struct_sizes", "spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
+    lib.spinf_seats_rooms.argtypes = [C.POINTER(SeatsArgs), C.c_int32, C.POINTER(C.c_int64)]
+    lib.spinf_seats_step.argtypes = [C.POINTER(SeatsArgs), C.c_void_p]
+    lib.spinf_seats_attn_fwd.argtypes = [C.POINTER(SeatsAttnArgs), C.c_void_p]
+    lib.spinf_sample_workspace.argtypes = [C.POINTER(SampleArgs), C.POINTER(C.c_int64)]
+    lib.spinf_sample.argtypes = [C.POINTER(SampleArgs), C.c_void_p]
+    lib.spinf_seats_struct_sizes.argtypes = [C.POINTER(C.c_int64), C.c_int32]
+    for name in ("spinf_seats_rooms", "spinf_seats_step", "spinf_seats_attn_fwd", "spinf_sample_workspace", "spinf_sample", "spinf_seats_struct_sizes", "spinf_paged_plan_build", "spinf_paged_plan_counts", "spinf_paged_plan_export", "spinf_paged_attn_fwd", "spinf_paged_weights", "spinf_cache_evict", "spinf_qk_norm_rope", "spinf_paged_struct_sizes", "spinf_struct_sizes", "spinf_diag_attn_stream", "spinf_diag_lds_order", "spinf_diag_mfma_hazard", "spinf_diag_mfma_valu", "spinf_diag_lds_rate", "spinf_diag_mfma_rate", "spinf_lm_head_workspace", "spinf_lm_head_fwd", "spinf_gdn_plan_build", "spinf_gdn_plan_counts", "spinf_gdn_plan_export", "spinf_gdn_plan_program", "spinf_tileplan_schedule_static", "spinf_attn_ring_aborts", "spinf_tileplan_build", "spinf_tileplan_build_groups", "spinf_tileplan_build_ktile", "spinf_tileplan_counts", "spinf_tileplan_export", "spinf_tileplan_schedule", "spinf_tileplan_row0", "spinf_tree_attn_fwd", "spinf_tree_attn_fwd_noalloc", "spinf_attn_exact_items", "spinf_gdn_fwd", "spinf_gdn_prologue", "spinf_gdn_gate", "spinf_lm_logprobs", "spinf_xdecode_plan", "spinf_xdecode_tiles", "spinf_xdecode_put", "spinf_xdecode_plan_ragged", "spinf_xdecode_attn_fwd"):
         getattr(lib, name).restype = C.c_int
     # the argument blocks above mirror include/spinf_tree.h: a library built from another version of the header would read them wrongly
     mirrors = (AttnArgs, GdnArgs, GdnPreArgs, GdnGateArgs, LmArgs, LmHeadArgs, XdecArgs)
@@ -245,6 +296,11 @@ def _bind(lib, path):
     sizes = (C.c_int64 * len(mirrors))()
     if lib.spinf_paged_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
         raise RuntimeError(f"{path}: the paged cache's argument blocks have {list(sizes)} bytes, this package's {[C.sizeof(m) for m in mirrors]}: "
+                           "the library and the package are of different versions (rebuild: python __graft_entry__.py); no fallback")
+    mirrors = (SeatsKind, SeatsArgs, SeatsAttnArgs, SampleArgs)
+    sizes = (C.c_int64 * len(mirrors))()
+    if lib.spinf_seats_struct_sizes(sizes, len(mirrors)) != 0 or list(sizes) != [C.sizeof(m) for m in mirrors]:
+        raise RuntimeError(f"{path}: the seats' and the sampler's argument blocks have {list(sizes)} bytes, this package's {[C.sizeof(m) for m in mirrors]}: "
                            "the library and the package are of different versions (rebuild: python __graft_entry__.py); no fallback")
     _LIB = lib
     return lib

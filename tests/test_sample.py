@@ -1,0 +1,211 @@
+"""Draws: tokens by given random numbers against the float64 oracle (gpu), refusals (CPU)."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import spinf_serve_amd as sa
+from oracle import sample as oracle_sample
+from spinf_serve_amd import _lib
+
+
+# ------------------------------------------------------------------------------------------------ refusals (CPU)
+def test_draws_refuse_what_they_do_not_take(lib):
+    x, u = torch.zeros((2, 8)), torch.zeros(2)
+    with pytest.raises(RuntimeError):
+        sa.sample_tokens(x, u)   # no CPU path
+    for how in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_p=-0.1), dict(min_p=float("nan")), dict(top_k=-3), dict(top_k=2.5)):
+        with pytest.raises(ValueError):
+            sa.sample_tokens(x, u, **how)
+
+
+def test_the_c_entry_refuses_bad_arguments(lib):
+    x = torch.zeros(64)
+    need = C.c_int64()
+
+    def args():
+        a = _lib.SampleArgs()
+        a.logits, a.ld, a.rows, a.vocab, a.u, a.token = x.data_ptr(), 8, 2, 8, x.data_ptr(), x.data_ptr()
+        a.all_temperature, a.all_top_p = 1.0, 1.0
+        a.workspace, a.workspace_bytes = x.data_ptr() // 16 * 16, 1 << 40
+        return a
+
+    assert lib.spinf_sample_workspace(C.byref(args()), C.byref(need)) == 0 and need.value > 0
+    assert lib.spinf_sample_workspace(C.byref(args()), None) == -1
+    for name, v in (("logits", None), ("u", None), ("token", None), ("workspace", None), ("workspace_bytes", 8), ("rows", -1), ("rows", 65536), ("vocab", 0), ("vocab", (1 << 22) + 1), ("ld", 7), ("dtype", 2),
+                    ("all_temperature", -1.0), ("all_top_p", float("nan")), ("all_min_p", -0.5)):
+        a = args()
+        setattr(a, name, v)
+        assert lib.spinf_sample(C.byref(a), None) == -1, name
+    a = args()
+    a.rows = 0
+    assert lib.spinf_sample(None, None) == -1 and lib.spinf_sample(C.byref(a), None) == 0
+
+
+@pytest.mark.gpu
+def test_draws_refuse_tensors_before_any_launch(dev):
+    x, u = torch.zeros((3, 40), device=dev), torch.zeros(3, device=dev)
+    t = torch.ones(3, device=dev)
+    for bad in (x.double(), x[0], x.t(), x[:, ::2], x.half()):
+        with pytest.raises(ValueError):
+            sa.sample_tokens(bad, u)
+    for bad in (u[:2], u.half(), u.cpu(), torch.zeros(6, device=dev)[::2], u[:, None]):
+        with pytest.raises(ValueError):
+            sa.sample_tokens(x, bad)
+    for bad in (dict(temperature=t.double()), dict(top_k=t), dict(top_p=t[:2]), dict(min_p=t.cpu()), dict(top_k=t.long())):
+        with pytest.raises(ValueError):
+            sa.sample_tokens(x, u, **bad)
+    with pytest.raises(ValueError):
+        sa.sample_tokens(torch.zeros((1, 40), device=dev).expand(3, 40), u)
+    assert sa.sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------------ against the oracle
+def logits(kind, rows, vocab, seed):
+    g = np.random.default_rng(seed)
+    x = 2.2 * g.standard_normal((rows, vocab))
+    if kind == "peaked":
+        for r in range(rows):
+            at = g.integers(0, vocab, min(200, vocab))
+            x[r, at] = 4 + 9 * g.random(len(at)) ** 2
+    elif kind == "ties":
+        x = np.floor(2 * x) / 2
+    elif kind == "equal":
+        x[:] = -3.25
+    elif kind == "masked":
+        x[g.random((rows, vocab)) < 0.95] = -np.inf
+        x[0] = -np.inf
+        x[-1] = -np.inf
+        x[-1, vocab // 2] = 1.5
+        if rows > 2:
+            x[1, g.random(vocab) < 0.5] = np.nan
+    elif kind == "wide":
+        x *= 1000
+    elif kind == "narrow":
+        x *= 1e-4
+    elif kind == "infinite":
+        x[:, g.integers(0, vocab, 3)] = np.inf
+        x[0] = -np.inf
+    elif kind == "signs":   # zeros of either sign are equal
+        x = np.where(g.random((rows, vocab)) < 0.5, -0.0, 0.0)
+    elif kind == "largest":
+        x[:] = np.where(x > 2, np.finfo(np.float32).max, np.where(x < -2, np.finfo(np.float32).min, x))
+    return x
+
+
+def check(dev, x, dtype, u, how, pad=0, u_dtype=torch.float64):
+    rows, vocab = x.shape
+    t = torch.from_numpy(x.astype(np.float32)).to(dtype)
+    wide = torch.full((rows, vocab + pad), 99.0, dtype=dtype, device=dev)
+    wide[:, :vocab] = t.to(dev)
+    given = {k: torch.from_numpy(v).to(dev) if isinstance(v, np.ndarray) else v for k, v in how.items()}
+    ud = torch.from_numpy(u).to(u_dtype).to(dev)
+    token, prob = sa.sample_tokens(wide[:, :vocab], ud, **given, return_prob=True)
+    values, un = t.double().numpy(), ud.double().cpu().numpy()
+    bad = 0
+    for r in range(rows):
+        one = {k: float(np.float32(v[r] if isinstance(v, np.ndarray) else v)) for k, v in how.items()}
+        one["top_k"] = int(one.get("top_k", 0))
+        want, p, near = oracle_sample.draw(values[r], un[r], **one)
+        if near > 1e-10:   # (nearer, the two orders of summing may fall on either side of a border)
+            assert int(token[r]) == want, (r, one, un[r], int(token[r]), want)
+            assert abs(float(prob[r]) - p) <= p * 2.0**-22 + 1e-30
+        bad += near <= 1e-10
+    assert bad <= 1 + rows // 20
+    assert torch.equal(token, sa.sample_tokens(wide[:, :vocab], ud, **given))
+    return token
+
+
+HOW = [
+    dict(), dict(temperature=0.7), dict(temperature=0.0), dict(top_k=1), dict(top_k=40, temperature=0.8), dict(top_p=0.9), dict(min_p=0.05), dict(top_p=0.999, temperature=1.5), dict(top_k=300, top_p=0.8, min_p=0.02),
+    dict(top_k=1000, top_p=0.97), dict(min_p=1.0), dict(top_p=0.0), dict(top_p=1e-6), dict(min_p=1e-12), dict(top_k=1 << 29), dict(temperature=20.0, top_p=0.5), dict(temperature=0.01, top_k=3), dict(min_p=2.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind,rows,vocab,pad", [("peaked", 5, 32000, 0), ("flat", 3, 16385, 3), ("ties", 4, 5000, 1), ("masked", 6, 20000, 0), ("flat", 2, 262144, 0), ("peaked", 40, 97, 0), ("flat", 3, 1, 0)])
+def test_draws_against_the_oracle(dev, kind, rows, vocab, pad, dtype):
+    g = np.random.default_rng(vocab)
+    x = logits(kind, rows, vocab, vocab + 1)
+    for how in HOW:
+        check(dev, x, dtype, g.random(rows), how, pad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["equal", "wide", "narrow", "infinite", "signs", "largest"])
+def test_draws_from_extreme_logits(dev, kind):
+    g = np.random.default_rng(3)
+    x = logits(kind, 3, 20011, 9)
+    for how in HOW:
+        check(dev, x, torch.float32, g.random(3), how)
+
+
+@pytest.mark.gpu
+def test_settings_of_every_row(dev):
+    g = np.random.default_rng(8)
+    rows = 96
+    x = logits("peaked", rows, 50000, 4)
+    x[7] = np.nan
+    f = lambda *v: g.choice(np.array(v, np.float32), rows)  # noqa: E731
+    how = dict(temperature=f(0, 0.5, 1, 1.4), top_k=g.choice(np.array([0, 1, 20, 50, 200, -1, 70000], np.int32), rows), top_p=f(1, 0.9, 0.3, 0.0, 2.0), min_p=f(0, 0, 0.1, 0.01))
+    how["temperature"][3] = -1
+    how["top_p"][4] = np.nan
+    how["min_p"][5] = -0.1
+    token = check(dev, x, torch.float32, g.random(rows), how)
+    assert token[[3, 4, 5, 7]].tolist() == [-1] * 4
+
+
+@pytest.mark.gpu
+def test_random_numbers_at_the_ends(dev):
+    x = logits("peaked", 6, 40000, 2)
+    x[:, 0] = -np.inf
+    u = np.array([0.0, 1.0, 1.5, -0.5, np.nan, 1 - 2.0**-53])
+    for how in (dict(), dict(top_k=7), dict(top_p=0.6), dict(min_p=0.1)):
+        for dt in (torch.float64, torch.float32):
+            token = check(dev, x, torch.float32, u, how, u_dtype=dt)
+            assert (token > 0).all()
+
+
+@pytest.mark.gpu
+def test_how_often_tokens_come(dev):
+    """20,000 draws of one row: counts within 6 standard deviations of what the probabilities say"""
+    x = torch.tensor([[1.0, 0.0, 2.0, -1.0, 0.5, -float("inf"), 1.5, 0.0]], device=dev)
+    n = 20000
+    u = torch.rand(n, generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+    got = sa.sample_tokens(x.repeat(n, 1), u, temperature=0.9, top_k=6, min_p=0.05)
+    p = torch.softmax(x[0].double() / 0.9, 0)
+    keep = torch.zeros(8, dtype=torch.bool, device=dev)
+    keep[torch.sort(x[0], descending=True, stable=True)[1][:6]] = True
+    p = torch.where(keep & (p >= 0.05 * p.max()), p, 0)
+    p /= p.sum()
+    count = torch.bincount(got, minlength=8).double()
+    assert ((count - n * p).abs() <= 6 * (n * p * (1 - p)).sqrt() + 1e-9).all()
+
+
+@pytest.mark.gpu
+def test_graphs_streams_and_the_registered_operator(dev):
+    x = torch.from_numpy(logits("peaked", 8, 40000, 2)).float().to(dev)
+    u = torch.rand(8, device=dev)
+    k = torch.full((8,), 30, dtype=torch.int32, device=dev)
+    how = dict(temperature=0.9, top_k=k, top_p=0.95, return_prob=True)
+    want = sa.sample_tokens(x, u, **how)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a, b) for a, b in zip(sa.sample_tokens(x, u, **how), want))
+    torch.cuda.synchronize()
+    torch.library.opcheck(torch.ops.spinf.sample_tokens.default, (x, u, None, k, None, None, [0.9, 0, 0.95, 0.0], True), test_utils=("test_schema", "test_faketensor"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        token, prob = sa.sample_tokens(x, u, **how)
+    for i in range(3):
+        u.copy_(torch.rand(8, generator=torch.Generator().manual_seed(i)))
+        k.fill_(5 + 50 * i)
+        graph.replay()
+        torch.cuda.synchronize()
+        e = sa.sample_tokens(x, u, **how)
+        assert torch.equal(token, e[0]) and torch.equal(prob, e[1])
+        torch.cuda.synchronize()

@@ -1,0 +1,345 @@
+"""Seats: the books against going seat by seat, the work lists against the dense mask, the attention against the float64 oracle (gpu), refusals (CPU)."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import spinf_serve_amd as sa
+from oracle import paged as op
+from oracle.seats import Books
+from spinf_serve_amd import _lib
+from spinf_serve_amd import seats as ss
+
+BF16 = torch.bfloat16
+
+
+def make(device, stored, own, new, page, heads, content=None, seed=0, spare=3, rows=None, keys=None, window=0, dropped=None):
+    """seats with `own` keys each, `new` of them the last step's; content: of each seat (None: dealt out in turn, one after the other) -> seats, pages in all"""
+    rng = np.random.default_rng(seed)
+    need = [-(-n // page) for n in stored]
+    own_pages = sum(-(-n // page) for n in own)
+    ids = rng.permutation(sum(need) + own_pages + spare)
+    tables = np.split(ids[: sum(need)], np.cumsum(need)[:-1]) if stored else []
+    pool = ids[sum(need) :]
+    rows = rows if rows is not None else sum(new) + 2
+    s = sa.PagedSeats.build(len(own), rows, page, keys or max(own), pool, contents=(stored, tables), stored=[n - m for n, m in zip(own, new)],
+                            heads=[(*heads, window)] if heads else [], dropped=dropped, device=device)
+    s.tables = tables
+    s.content.copy_(torch.tensor(content if content is not None else [-1] * len(own), dtype=torch.int32))
+    if s.device.type == "cuda":
+        s.step(torch.tensor(new, dtype=torch.int32, device=device))
+        torch.cuda.synchronize()
+        assert s.lens.tolist() == list(own) and s.took.tolist() == list(new)
+    return s, len(ids)
+
+
+# ------------------------------------------------------------------------------------------------ refusals (CPU)
+GOOD = dict(seats=2, rows=4, page=16, keys=40, pool=[5, 6, 7, 8], contents=([20], [[0, 1]]), heads=[(4, 2, 64)], device="cpu")
+
+
+@pytest.mark.parametrize("bad", [
+    dict(seats=0), dict(seats=2049), dict(seats=1.5), dict(rows=0), dict(rows=1 << 23), dict(page=8), dict(page=24), dict(keys=0), dict(keys=1 << 29),
+    dict(pool=[5, 5]), dict(pool=[1, 7]), dict(pool=[-1]), dict(pool=[1 << 31]), dict(pool=[2.5]), dict(contents=([20], [])), dict(contents=([40], [[0, 1]])), dict(contents=([-1], [[0]])),
+    dict(heads=[(4, 3, 64)]), dict(heads=[(4, 2, 96)]), dict(heads=[(4, 2, 64, -1)]), dict(heads=[(4, 2, 64), (4, 2, 64, 0)]), dict(heads=[(4, 2, 64, w) for w in range(9)]),
+    dict(heads=[(1 << 40, 1, 64)]), dict(heads=[(0, 0, 64)]), dict(stored=[1]), dict(stored=[41, 0]), dict(stored=[40, 40]), dict(dropped=[1, 2]), dict(dropped=[3], heads=[(4, 2, 64, 8)]), dict(dropped=[-3]),
+])
+def test_seats_that_make_no_sense_are_refused(lib, bad):
+    sa.PagedSeats.build(**GOOD)
+    with pytest.raises(ValueError):
+        sa.PagedSeats.build(**{**GOOD, **bad})
+
+
+def test_steps_and_attention_refuse_what_they_do_not_take(lib):
+    s = sa.PagedSeats.build(**GOOD)
+    new = torch.zeros(2, dtype=torch.int32)
+    for bad in (new.long(), new[:1], torch.zeros(4, dtype=torch.int32)[::2], new.float()):
+        with pytest.raises(ValueError):
+            s.step(bad)
+        with pytest.raises(ValueError):
+            s.step(new, bad)
+    with pytest.raises(RuntimeError):
+        s.step(new)   # no CPU path
+    q, cache = torch.zeros((4, 4, 64), dtype=BF16), sa.PagedCache(*(torch.zeros((9, 16, 2, 64), dtype=BF16) for _ in range(2)))
+    with pytest.raises(RuntimeError):
+        sa.seats_attn(q, cache, s)
+    for x in (q.float(), q[:3], q[:, :2], torch.zeros((4, 4, 128), dtype=BF16), torch.zeros((4, 64, 4), dtype=BF16).transpose(1, 2)):
+        with pytest.raises(ValueError):
+            sa.seats_attn(x, cache, s)
+    for shape in ((8, 16, 2, 64), (9, 32, 2, 64), (9, 16, 4, 64)):   # too few pages, other pages, other heads
+        with pytest.raises(ValueError):
+            sa.seats_attn(q, sa.PagedCache(*(torch.zeros(shape, dtype=BF16) for _ in range(2))), s)
+    for w in (-1, 1.5, 7):   # (7: not among the seats' geometries)
+        with pytest.raises(ValueError):
+            sa.seats_attn(q, cache, s, window=w)
+
+
+def test_the_c_entries_refuse_bad_arguments(lib):
+    s = sa.PagedSeats.build(**GOOD)
+    one = torch.zeros(64, dtype=torch.int32)
+
+    def args():
+        a = ss._step_args(s._state, s._work, s.slots, s.pos, s.content, s._geo)
+        a.come = one.data_ptr()
+        return a
+
+    def refused(a):
+        assert lib.spinf_seats_step(C.byref(a), None) == -1, lib.spinf_last_error()
+
+    for name in ("come", "content", "lens", "lists", "free", "left", "first", "took", "stay", "slots", "pos", "shared"):
+        a = args()
+        setattr(a, name, None)
+        refused(a)
+    for name, x in (("seats", 0), ("seats", 2049), ("rows", 0), ("page", 17), ("keys", 0), ("pool", -1), ("contents", -1), ("kinds", 9), ("longest", -1), ("table_at", -4), ("table_at", 2)):
+        a = args()
+        setattr(a, name, x)
+        refused(a)
+    for name in ("wave", "single", "block", "counts", "parts", "seat_parts"):
+        a = args()
+        setattr(a.kind[0], name, None)
+        refused(a)
+    assert lib.spinf_seats_step(None, None) == -1 and lib.spinf_seats_attn_fwd(None, None) == -1
+    rooms = (C.c_int64 * 4)()
+    assert lib.spinf_seats_rooms(C.byref(args()), 1, rooms) == -1 and lib.spinf_seats_rooms(C.byref(args()), 0, None) == -1
+
+    q = torch.zeros((4, 4, 64), dtype=BF16)
+    cache = [torch.zeros((9, 16, 2, 64), dtype=BF16) for _ in range(2)]
+
+    def attn():
+        b = ss._attn_block(q, *cache, s._state, s._work, s.pos, s._geo, 0, 0.1, 0.0)
+        b.q = b.out = b.k = b.v = b.workspace = q.data_ptr()
+        b.workspace_bytes = b.rooms[3] * 4 * 66 * 4
+        return b
+
+    for name, x in (("q", None), ("out", None), ("k", None), ("v", None), ("lists", None), ("first", None), ("pos", None), ("workspace", None), ("workspace_bytes", 16), ("rows", 0), ("seats", 0),
+                    ("page", 20), ("scale", 0.0), ("scale", float("nan")), ("softcap", -1.0), ("q_tok", 4), ("k_row", -8), ("v_page", (1 << 30) + 8)):
+        b = attn()
+        setattr(b, name, x)
+        assert lib.spinf_seats_attn_fwd(C.byref(b), None) == -1, name
+    for name, x in (("hq", 3), ("d", 96), ("window", -1), ("wave", None), ("counts", None)):
+        b = attn()
+        setattr(b.kind, name, x)
+        assert lib.spinf_seats_attn_fwd(C.byref(b), None) == -1, name
+
+
+# ------------------------------------------------------------------------------------------------ the books
+def books_of(s, text):
+    return Books(s.lens.tolist(), s.table.tolist(), s.free.tolist(), int(s.left), s.keys, s.page, s.rows, text)
+
+
+def same_books(s, b, got):
+    slots, pos, first, took = got
+    assert s.slots.tolist() == slots and s.pos.tolist() == pos and s.first.tolist() == first and s.took.tolist() == took
+    assert s.lens.tolist() == b.lens and int(s.left) == len(b.stack) and s.free[: len(b.stack)].tolist() == b.stack
+    for r, n in enumerate(b.lens):
+        m = -(-n // s.page)
+        assert s.table[r, :m].tolist() == b.table[r][:m]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,page,keys,rows,pages,most", [
+    (1, 16, 40, 8, 4, 20), (3, 16, 100, 30, 12, 40), (64, 64, 700, 300, 90, 60), (70, 48, 50, 40, 71, 3), (300, 16, 90, 500, 700, 9), (1030, 32, 64, 1200, 1100, 4), (2048, 16, 33, 3000, 2500, 5), (9, 16, 4000, 20000, 2000, 3500)])
+def test_steps_against_going_seat_by_seat(dev, R, page, keys, rows, pages, most):
+    """steps at random, seats that ask for more than there is among them: rows, pages, keys"""
+    rng = np.random.default_rng(R)
+    lens = [37, 0, 101]
+    s = sa.PagedSeats.build(R, rows, page, keys, rng.permutation(pages) + 40, contents=(lens, [[0, 1, 2], [], list(range(3, 10))]), dropped=[0, 0, 5], heads=[(8, 2, 64), (4, 4, 512)], device=dev)
+    text = [37, 0, 106]
+    b = books_of(s, text)
+    refused = 0
+    for i in range(8):
+        content = rng.integers(-3, 6, R)
+        content[rng.random(R) < 0.05] = np.iinfo(np.int32).min
+        s.content.copy_(torch.from_numpy(content.astype(np.int32)))
+        new = rng.integers(-2, most + 1, R) * (rng.random(R) < 0.7)
+        drop = rng.integers(-1, most, R) * (rng.random(R) < 0.4)
+        drop[rng.random(R) < 0.1] = np.iinfo(np.int32).max
+        if i == 6:
+            new[rng.integers(0, R)] = np.iinfo(np.int32).max
+        got = b.step(new, drop if i % 3 else np.zeros(R), content)
+        to = lambda x: torch.from_numpy(x.astype(np.int32)).to(dev)  # noqa: E731
+        slots, pos = s.step(to(new), to(drop) if i % 3 else None)
+        assert slots is s.slots and pos is s.pos
+        same_books(s, b, got)
+        refused += sum(m > 0 and t == 0 for m, t in zip(new, got[3]))
+        used = [x for r, n in enumerate(b.lens) for x in b.table[r][: -(-n // page)]] + b.stack
+        assert sorted(used) == sorted(set(used)) and len(used) == pages
+    assert refused or R < 4
+
+
+@pytest.mark.gpu
+def test_a_step_taken_back_leaves_everything_as_it_was(dev):
+    s, _ = make(dev, [40], [17, 3, 64, 1], [1, 1, 1, 1], 16, (4, 2, 64), content=[0, 0, -1, 0], rows=80, keys=100, spare=20)
+    s.step(torch.zeros(4, dtype=torch.int32, device=dev))
+    before = s.lens.clone(), s.left.clone(), s.free.clone()
+    new = torch.tensor([20, 1, 17, 31], dtype=torch.int32, device=dev)
+    s.step(new)
+    one = s.slots.clone(), s.table.clone()
+    s.step(torch.zeros_like(new), new)
+    assert torch.equal(s.lens, before[0]) and torch.equal(s.left, before[1]) and torch.equal(s.free, before[2])
+    s.step(new)
+    assert torch.equal(s.slots, one[0]) and torch.equal(s.table, one[1])
+
+
+# ------------------------------------------------------------------------------------------------ the work lists
+# content lengths, content of each seat, own keys with the new ones, new ones, page, (hq, hkv, d), window
+SHAPES = [
+    ([], [-1], [1], [1], 16, (4, 4, 64), 0),
+    ([33], [0], [1], [1], 16, (4, 2, 128), 0),
+    ([33, 0], [0, 0, -1, 1, 0], [1, 17, 40, 3, 130], [1, 1, 1, 1, 1], 16, (8, 2, 64), 0),
+    ([301], [0] * 24, [5 + i for i in range(24)], [1] * 24, 64, (16, 8, 256), 0),
+    ([470, 130], [0] * 9 + [1] * 8, [1 + 3 * i for i in range(17)], [1] * 17, 48, (24, 4, 256), 0),
+    ([2100], [0, 0, 0], [700, 40, 2], [2, 4, 1], 32, (16, 1, 512), 0),
+    ([1500], [0] * 40, [9] * 40, [4] * 40, 16, (10, 2, 128), 0),
+    ([700, 64], [0, 0, 0, 1, 1, -1], [211, 150, 300, 90, 70, 200], [150, 70, 40, 90, 1, 33], 48, (4, 2, 128), 0),
+    ([700, 64], [0, 0, 0, 1, 1, -1], [211, 150, 300, 90, 70, 200], [150, 70, 40, 90, 1, 33], 16, (6, 2, 64), 100),
+    ([900, 900], [0, 1, 1, 1], [1, 600, 90, 5], [1, 3, 2, 5], 80, (8, 4, 256), 256),
+    ([100], [0, 0], [40, 1], [2, 1], 16, (4, 2, 64), 1),
+    ([5000], [0] * 3, [2500, 30, 130], [1, 1, 2], 64, (12, 12, 64), 0),
+    ([200, 90], [0, -1, 0, 1, 0], [300, 200, 70, 150, 66], [300, 200, 0, 140, 66], 32, (4, 1, 512), 0),
+    ([64], [0, 0, 0], [5, 9, 20], [0, 0, 0], 16, (4, 2, 64), 0),
+]
+
+
+def dense(s, stored, content, own, new, window):
+    """per seat [new, content keys + own keys]"""
+    out = []
+    for c, n, m in zip(content, own, new):
+        P = stored[c] if c >= 0 else 0
+        out.append(op.visible(m, P + n, window=window))
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stored,content,own,new,page,heads,window", SHAPES)
+def test_work_lists_are_the_dense_mask(dev, stored, content, own, new, page, heads, window):
+    s, _ = make(dev, stored, own, new, page, heads, content, window=window)
+    hq, hkv, d = heads
+    group = hq // hkv
+    work = s._work.cpu().numpy()
+    lists = ss._layout(s._geo)["lists"][0]
+    rooms = ss._rooms(s._geo, 0)
+    counts = work[lists[3] : lists[3] + 4]
+    assert all(n <= room for n, room in zip(counts, rooms))
+    parts = work[lists[4] : lists[4] + s.rows + 1]
+    first = s.first.cpu().numpy()
+    see = dense(s, stored, content, own, new, window)
+    seen = [np.zeros((m * group, x.shape[1]), np.int8) for m, x in zip(new, see)]
+    seat_of = np.repeat(np.arange(len(own)), new)
+    span_at = {}   # where a span's page list begins -> its seat or content
+    at = 0
+    for c, n in enumerate(stored):
+        span_at[at] = c
+        at += -(-n // page) if n else 0
+    own_at = {ss._layout(s._geo)["table"] + r * s.table.shape[1]: r for r in range(len(own))}
+    used = set()
+    for kind in range(3):
+        size = 128 if kind == 2 else 32
+        for tok0, T, L, tab, row0, kt0, tiles, piece, flo, fhi, flags, _ in work[lists[kind] : lists[kind] + 12 * counts[kind]].reshape(-1, 12).tolist():
+            rows = range(row0, min(row0 + size, T * group))
+            assert len(rows) and row0 % size == 0 and kt0 >= 0 and tiles >= 0 and (not tiles or 32 * (kt0 + tiles - 1) < L)
+            keys = np.arange(32 * kt0, min(32 * (kt0 + tiles), L))
+            for x in rows:
+                tok = tok0 + x // group
+                r = int(seat_of[tok])
+                c = content[r]
+                P = stored[c] if c >= 0 else 0
+                if flags & 1:
+                    assert own_at[tab] == r and (L, T, tok0) == (own[r], new[r], first[r])
+                    at = P
+                else:
+                    assert span_at[tab] == c and L == P
+                    at = 0
+                assert (flags >> 1 & 1) == (parts[tok + 1] == parts[tok])
+                if not flags & 2:
+                    assert 0 <= piece < parts[tok + 1] - parts[tok] and (tok, x % group, piece) not in used
+                    used.add((tok, x % group, piece))
+                row = (tok - first[r]) * group + x % group
+                line = see[r][tok - first[r]]
+                inside = keys[(keys >= flo) & (keys <= fhi)]
+                assert line[at + inside].all()
+                seen[r][row, at + keys] += line[at + keys].astype(np.int8)
+    for x, y in zip(seen, see):
+        assert (x == np.repeat(y, group, 0)).all()   # every visible pair once
+    total = int(first[-1])
+    assert len(used) == int(parts[total] * group) and (parts[total:] == counts[3]).all() and counts[3] <= rooms[3]
+
+
+@pytest.mark.gpu
+def test_lists_never_outgrow_their_rooms(dev):
+    rng = np.random.default_rng(5)
+    for i in range(40):
+        R, page, keys = int(rng.integers(1, 200)), int(rng.choice([16, 48, 64])), int(rng.choice([20, 300, 3000]))
+        rows = int(rng.integers(1, 900))
+        stored = [int(rng.choice([1, 50, 5000]))] * int(rng.integers(0, 3))
+        at = np.cumsum([0] + [-(-n // page) for n in stored])
+        pool = np.arange(int(rng.integers(1, 4)) * R * -(-keys // page) // 3 + 1) + at[-1]
+        heads = [(16, 8, 256), (16, 1, 512), (8, 8, 64), (32, 2, 128, 100)]
+        s = sa.PagedSeats.build(R, rows, page, keys, pool, contents=(stored, [np.arange(a, b) for a, b in zip(at[:-1], at[1:])]), heads=heads, device=dev)
+        for most in (2, 40, keys):
+            s.content.copy_(torch.from_numpy(rng.integers(-1, 2, R).astype(np.int32)))
+            new = torch.from_numpy(rng.integers(0, most + 1, R).astype(np.int32)).to(dev)
+            s.step(new, torch.from_numpy((rng.integers(0, 2, R) * 10000).astype(np.int32)).to(dev))
+            for k in range(len(heads)):
+                lists = ss._layout(s._geo)["lists"][k]
+                counts = s._work[lists[3] : lists[3] + 4].tolist()
+                assert all(n <= room for n, room in zip(counts, ss._rooms(s._geo, k)))
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def fill(s, pages, heads, seed, device, order="heads", peaky=True):
+    hq, hkv, d = heads
+    g = torch.Generator().manual_seed(seed)
+    shape = (pages, hkv, s.page, d) if order == "heads" else (pages, s.page, hkv, d)
+    k, v = (torch.randn(shape, generator=g).to(BF16).to(device) for _ in range(2))
+    if order == "heads":
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+    q = torch.randn((s.rows, hq, d), generator=g)
+    if peaky:
+        q *= 1 + 3 * (torch.rand(s.rows, hq, 1, generator=g) < 0.2)
+    return sa.PagedCache(k, v), q.to(BF16).to(device)
+
+
+def reference(q, cache, s, stored, content, own, new, scale, window=0, softcap=0.0):
+    """out, lse of the rows in use, and what the kernel's results may be off by"""
+    qn, kn, vn = (t.float().cpu().numpy() for t in (q, cache.k, cache.v))
+    d, table, base = qn.shape[2], s.table.cpu().numpy(), 0
+    out, lse, tol, ltol = [], [], [], []
+    for r, (c, n, m) in enumerate(zip(content, own, new)):
+        P = stored[c] if c >= 0 else 0
+        kk, vv = (np.concatenate([op.stored(x, s.tables[c], P) if P else np.zeros((0, *x.shape[2:])), op.stored(x, table[r], n)]) for x in (kn, vn))
+        o, l, mag, size = op.attention(qn[base : base + m].astype(np.float64), kk, vv, op.visible(m, P + n, window=window), scale, softcap)
+        # scores: d products summed in fp32, then scaled (and capped: the cap's slope is at most 1, its own error 2^-22 of the cap)
+        terr = size * (d + 4) * 2.0**-24 + softcap * 2.0**-21 + 2.0**-20
+        # probabilities: exp of the score's error, rounded to bf16 (half a step: 2^-8 at most, relative); sums in fp32; the output's own rounding to bf16
+        out.append(o)
+        lse.append(l)
+        tol.append(1.02 * (2.0**-8 * (mag + np.abs(o)) + mag * (2 * terr[..., None] + (P + n + 64) * 2.0**-24)) + 1e-30)
+        ltol.append(terr + (P + n + 64) * 2.0**-24 + np.abs(l) * 2.0**-22)
+        base += m
+    return tuple(np.concatenate(x) for x in (out, lse, tol, ltol))
+
+
+def close(got, want, tol):
+    got = got.float().cpu().numpy().astype(np.float64)
+    assert got.shape == want.shape
+    off = np.abs(got - want)
+    worst = float((off / np.maximum(tol, 1e-300)).max(initial=0))
+    assert (off <= tol).all(), f"worst {worst} of the bound, {int((~(off <= tol)).sum())} values"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order,softcap", [("heads", 0.0), ("rows", 20.0)])
+@pytest.mark.parametrize("stored,content,own,new,page,heads,window", SHAPES)
+def test_attention_against_the_oracle(dev, stored, content, own, new, page, heads, window, order, softcap):
+    s, pages = make(dev, stored, own, new, page, heads, content, window=window)
+    cache, q = fill(s, pages, heads, 1, dev, order)
+    out, lse = sa.seats_attn(q, cache, s, window=window or None, softcap=softcap or None, return_lse=True)
+    n = sum(new)
+    assert (out[n:] == 0).all() and (lse[n:] == float("-inf")).all() and len(out) == n + 2
+    if n:
+        want, wlse, tol, ltol = reference(q, cache, s, stored, content, own, new, heads[2] ** -0.5, window, softcap)
+        close(out[:n], want, tol)
+        close(lse[:n], wlse, ltol)
+    assert torch.equal(out, sa.seats_attn(q, cache, s, heads[2] ** -0.5, window or None, softcap or None))
