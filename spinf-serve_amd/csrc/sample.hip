@@ -5,8 +5,8 @@
 // token w = exp((x - max) / T).  Kept are the first k of the order, of these the shortest beginning that holds p of their weight, of these the tokens with w >= min_p.  The token
 // drawn is the first, by index, up to which the kept weights add up to more than u times their sum.
 //
-// Where a border falls decides which token comes out, so weights are taken in 64 bits, and sums of them are sums of whole numbers: units of 2^-49 of the largest weight of a chunk
-// (16,384 logits), the same in any order.
+// Where a border falls decides which token comes out, so weights are taken in 64 bits, and sums of them are sums of whole numbers: units of 2^-47 of the largest weight of a chunk
+// (8,192 logits), the same in any order.
 //
 // Kernels.  chunks: a chunk's largest logit, its weight, and how many logits and how much weight lie in each of 255 bins, a twelfth of T wide, below its largest one (bins at whole
 // multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
@@ -27,11 +27,11 @@ typedef unsigned long long u64;
 
 namespace {
 
-constexpr int LANES = 1024, EACH = 16, CHUNK = LANES * EACH;
+constexpr int LANES = 512, WAVES = LANES / 64, EACH = 16, CHUNK = LANES * EACH;
 constexpr int BINS = 256;              // the last one: all below
 constexpr int SEGMENT = 1024;          // tokens of a chunk that lie in the bins in question
 constexpr int LISTED = 8192;           // ... of a row
-constexpr int MOST_CHUNKS = 256;
+constexpr int MOST_CHUNKS = 512;
 constexpr float BINS_PER_UNIT = 12.f;
 
 struct Stat { float top; unsigned at; u64 sum; };       // of a chunk: largest logit (-inf: none), where, weight
@@ -49,7 +49,7 @@ struct Params {
     Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
 };
 
-struct How { double inv; float scale, p, least; int k; bool best, wrong, filtered; };
+struct How { double inv, by_two; float scale, p, least; int k; bool best, wrong, filtered; };
 __device__ __forceinline__ How settings(const Params& p, int row) {
     How h;
     const float T = p.temperature ? p.temperature[row] : p.all_temperature;
@@ -59,6 +59,7 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
     h.wrong = !(T >= 0.f) || !(h.p >= 0.f) || !(h.least >= 0.f);
     h.best = T == 0.f;
     h.inv = 1.0 / (double)T;
+    h.by_two = h.inv * 1.4426950408889634;
     h.scale = fminf(BINS_PER_UNIT / T, 3e38f);
     if (h.k <= 0 || h.k >= p.vocab) h.k = 0;
     if (h.p == 0.f) {   // the first alone
@@ -75,17 +76,34 @@ __device__ __forceinline__ unsigned ordered(float x) {   // larger for larger x
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-__device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~ordered(x) << 32 | at; }   // smaller: earlier in the order
-__device__ __forceinline__ float clean(float x) { return x == x ? (x == 0.f ? 0.f : x) : -INFINITY; }   // (zeros are equal whatever their sign)
+__device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~ordered(x + 0.f) << 32 | at; }   // smaller: earlier in the order (zeros are equal whatever their sign)
 
 // a token's place on the grid of bins; never falls as x grows
 __device__ __forceinline__ int place(float x, float scale) { return (int)floorf(fminf(fmaxf(x * scale, -1e9f), 1e9f)); }
 
-// exp((x - top) / T), 1 for the largest ones also where they are infinite
-__device__ __forceinline__ double weight(float x, float top, double inv) { return x == top ? 1.0 : top == INFINITY ? 0.0 : exp(((double)x - (double)top) * inv); }
-// in units of 2^-49: the last bits of w + 8, rounded there
-__device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 8.0) - __double_as_longlong(8.0)); }
-constexpr double UNIT = 0x1p-49;
+// 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum.  (19 instructions of 64 bits, which run at the rate of
+// 32-bit ones here; with the library's exp the chunks of 320 rows of 262,144 took 195 us.)
+constexpr double series(int k) {
+    double c = 1.0;
+    for (int i = 1; i <= k; i++) c *= 0.69314718055994530942 / i;
+    return c;
+}
+__device__ __forceinline__ double power(double t) {
+    t = fmax(t, -1000.0);
+    const double n = __builtin_rint(t), f = t - n;
+    double y = series(12);
+#pragma unroll
+    for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, k == 11 ? series(11) : k == 10 ? series(10) : k == 9 ? series(9) : k == 8 ? series(8) : k == 7 ? series(7) : k == 6 ? series(6) : k == 5 ? series(5)
+                                                       : k == 4 ? series(4) : k == 3 ? series(3) : k == 2 ? series(2) : k == 1 ? series(1) : 1.0);
+    return __builtin_ldexp(y, (int)n);
+}
+// exp((x - top) / T) of finite numbers (x may be -inf: nothing), 1 for the largest
+__device__ __forceinline__ double weight_of(float x, float top, double by_two) { return power(((double)x - (double)top) * by_two); }
+// ... of any: where the largest are infinite, only they have a weight
+__device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : weight_of(x, top, by_two); }
+// in units of 2^-47: the last bits of w + 32, rounded there
+__device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 32.0) - __double_as_longlong(32.0)); }
+constexpr double UNIT = 0x1p-47;
 
 template <bool BF16>
 __device__ __forceinline__ float load1(const Params& p, int row, int i) {
@@ -98,27 +116,31 @@ constexpr int VEC = BF16 ? 8 : 4;
 template <bool BF16>
 __device__ __forceinline__ int index_of(int chunk, int e) { return chunk * CHUNK + (e / VEC<BF16> * LANES + (int)threadIdx.x) * VEC<BF16> + e % VEC<BF16>; }
 template <bool BF16>
+__device__ __forceinline__ void load_vec(const Params& p, int row, int at, float* x) {   // 16 bytes, aligned
+    if (BF16) {
+        const bf16x8 y = *(const bf16x8*)((const __bf16*)p.logits + (long)row * p.ld + at);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = (float)y[j];
+    } else {
+        const float4 y = *(const float4*)((const float*)p.logits + (long)row * p.ld + at);
+        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+    }
+}
+template <bool BF16>
 __device__ __forceinline__ void load(const Params& p, int row, int chunk, float (&x)[EACH]) {
     constexpr int V = VEC<BF16>;
 #pragma unroll
     for (int i = 0; i < EACH / V; i++) {
         const int at = index_of<BF16>(chunk, i * V);
         if (p.aligned && at + V <= p.vocab) {
-            if (BF16) {
-                const bf16x8 y = *(const bf16x8*)((const __bf16*)p.logits + (long)row * p.ld + at);
-#pragma unroll
-                for (int j = 0; j < V; j++) x[i * V + j] = (float)y[j];
-            } else {
-                const float4 y = *(const float4*)((const float*)p.logits + (long)row * p.ld + at);
-                x[i * V] = y.x; x[i * V + 1] = y.y; x[i * V + 2] = y.z; x[i * V + 3] = y.w;
-            }
+            load_vec<BF16>(p, row, at, x + i * V);
         } else {
 #pragma unroll
             for (int j = 0; j < V; j++) x[i * V + j] = at + j < p.vocab ? load1<BF16>(p, row, at + j) : -INFINITY;
         }
     }
 #pragma unroll
-    for (int e = 0; e < EACH; e++) x[e] = clean(x[e]);
+    for (int e = 0; e < EACH; e++) x[e] = fmaxf(x[e], -INFINITY);   // (NaN: never drawn)
 }
 
 template <class T, class F>
@@ -129,14 +151,37 @@ __device__ __forceinline__ T over_all(T x, T* room, F f) {   // room: one place 
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
     __syncthreads();
     x = room[0];
-    for (int w = 1; w < (int)blockDim.x / 64; w++) x = f(x, room[w]);
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) x = f(x, room[w]);
     return x;
 }
 __device__ __forceinline__ u64 sum_all(u64 x, u64* room) { return over_all(x, room, [](u64 a, u64 b) { return a + b; }); }
+__device__ __forceinline__ float top_all(float x, float* room) { return over_all(x, room, [](float a, float b) { return fmaxf(a, b); }); }
+// what the lanes up to this one hold, itself counted in, always added in the same order; total: of all
+template <class T>
+__device__ __forceinline__ T scan_all(T x, T* room, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) room[wave] = x;
+    __syncthreads();
+    T before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w == wave) before = total;
+        total += room[w];
+    }
+    return before + x;
+}
 
 template <bool BF16>
 __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
-    __shared__ u64 room[LANES / 64];
+    __shared__ u64 room[WAVES];
     __shared__ u64 weights[BINS];
     __shared__ int numbers[BINS];
     const int chunk = blockIdx.x, row = blockIdx.y;
@@ -144,30 +189,43 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
     if (h.wrong) return;
     float x[EACH];
     load<BF16>(p, row, chunk, x);
-    u64 first = ~0ull;   // the least number of the chunk
-#pragma unroll
-    for (int e = 0; e < EACH; e++) first = std::min(first, number(x[e], index_of<BF16>(chunk, e)));
-    first = over_all(first, room, [](u64 a, u64 b) { return a < b ? a : b; });
-    const float top = unordered(~(unsigned)(first >> 32));
-    Stat s = {top, (unsigned)first, 0};
     const long at = (long)row * p.chunks + chunk;
-    if (h.best || top == -INFINITY) {   // (an empty chunk's bins are not looked at)
+    if (h.best) {
+        u64 first = ~0ull;   // the least number of the chunk
+#pragma unroll
+        for (int e = 0; e < EACH; e++) first = std::min(first, number(x[e], index_of<BF16>(chunk, e)));
+        first = over_all(first, (u64*)room, [](u64 a, u64 b) { return a < b ? a : b; });
+        if (threadIdx.x == 0) p.stat[at] = {unordered(~(unsigned)(first >> 32)), (unsigned)first, 0};
+        return;
+    }
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < EACH; e++) top = fmaxf(top, x[e]);
+    top = top_all(top, (float*)room);
+    Stat s = {top, 0, 0};
+    if (top == -INFINITY) {   // (an empty chunk's bins are not looked at)
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
     }
-    if (h.filtered) {
-        if (threadIdx.x < BINS) {
-            weights[threadIdx.x] = 0;
-            numbers[threadIdx.x] = 0;
-        }
-        __syncthreads();
+    if (!h.filtered && top < INFINITY) {
+        double sum = 32.0;   // (16 weights of at most 1 leave it below 64: it counts in units of 2^-47)
+#pragma unroll
+        for (int e = 0; e < EACH; e++) sum += weight_of(x[e], top, h.by_two);
+        s.sum = sum_all((u64)(__double_as_longlong(sum) - __double_as_longlong(32.0)), room);
+        if (threadIdx.x == 0) p.stat[at] = s;
+        return;
     }
+    if (threadIdx.x < BINS) {
+        weights[threadIdx.x] = 0;
+        numbers[threadIdx.x] = 0;
+    }
+    __syncthreads();
     const int grid = place(top, h.scale);
     int there = 0;   // logits that can be drawn
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         there += x[e] > -INFINITY;
-        const u64 w = x[e] == -INFINITY ? 0 : units(weight(x[e], top, h.inv));
+        const u64 w = units(weight(x[e], top, h.by_two));
         s.sum += w;
         const int b = grid - place(x[e], h.scale);
         if (h.filtered && x[e] > -INFINITY && b < BINS - 1) {
@@ -175,11 +233,9 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
             atomicAdd(&numbers[b], 1);
         }
     }
-    if (h.filtered) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) there += __shfl_xor(there, d);
-        if ((threadIdx.x & 63) == 0) atomicAdd(&numbers[BINS - 1], there);   // (of all bins and below)
-    }
+    for (int d = 1; d < 64; d <<= 1) there += __shfl_xor(there, d);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&numbers[BINS - 1], there);   // (of all bins and below)
     s.sum = sum_all(s.sum, room);   // (its barriers are behind the bins' last addition)
     if (threadIdx.x == 0) p.stat[at] = s;
     if (h.filtered && threadIdx.x < BINS) {
@@ -188,59 +244,75 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
     }
 }
 
-// a row's largest logit and its weight in all
-__device__ __forceinline__ float row_top(const Params& p, int row) {
-    float top = -INFINITY;
-    for (int c = 0; c < p.chunks; c++) top = fmaxf(top, p.stat[(long)row * p.chunks + c].top);
+// A row's chunks, one per lane: the largest logit of all; factor: what a unit of a chunk's weights is worth of the row's largest weight
+__device__ __forceinline__ float stage(const Params& p, int row, const How& h, Stat& s, float* tops, double* factor, float* room) {
+    s = {-INFINITY, 0, 0};
+    if ((int)threadIdx.x < p.chunks && !h.wrong) s = p.stat[(long)row * p.chunks + threadIdx.x];
+    const float top = top_all(s.top, room);
+    if ((int)threadIdx.x < p.chunks) {
+        tops[threadIdx.x] = s.top;
+        factor[threadIdx.x] = s.top == -INFINITY || h.best ? 0.0 : weight(s.top, top, h.by_two) * UNIT;
+    }
+    __syncthreads();
     return top;
 }
 
-__global__ __launch_bounds__(BINS) void sample_rows_kernel(const Params p) {
-    __shared__ double masses[BINS];
-    __shared__ int counts[BINS];
-    __shared__ int found[3];
-    const int row = blockIdx.x, b = threadIdx.x;
+__global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
+    static_assert(LANES == 2 * BINS && LANES >= MOST_CHUNKS, "two lanes a bin, one a chunk");
+    __shared__ double masses[BINS], room[WAVES];
+    __shared__ int counts[BINS], room_n[WAVES];
+    __shared__ int found[4];
+    __shared__ float tops[MOST_CHUNKS];
+    __shared__ double factor[MOST_CHUNKS];
+    const int row = blockIdx.x, tid = threadIdx.x, b = tid & (BINS - 1), half = tid / BINS;
     const How h = settings(p, row);
     Row r = {};
-    r.top = h.wrong ? -INFINITY : row_top(p, row);
+    Stat mine;
+    r.top = stage(p, row, h, mine, tops, factor, (float*)room);
     r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
     if (r.how != PLAIN || !h.filtered) {
-        if (b == 0) p.row[row] = r;
+        if (tid == 0) p.row[row] = r;
         return;
     }
     r.grid = place(r.top, h.scale);
-    double mass = 0.0, sum = 0.0;
-    int n = 0, there = 0;
-    for (int c = 0; c < p.chunks; c++) {
-        const long at = (long)row * p.chunks + c;
-        const Stat s = p.stat[at];
-        if (s.top == -INFINITY) continue;
-        there += p.hist_n[at * BINS + BINS - 1];
-        const double f = weight(s.top, r.top, h.inv) * UNIT;
-        sum += f * (double)s.sum;
-        const int mine = b - (r.grid - place(s.top, h.scale));
-        if (mine >= 0 && mine < BINS - 1 && b < BINS - 1) {
-            mass += f * (double)p.hist_w[at * BINS + mine];
-            n += p.hist_n[at * BINS + mine];
-        }
+    if (tid < 4) found[tid] = tid < 3 ? BINS : 0;
+    __syncthreads();
+    double sum;
+    scan_all(tid < p.chunks ? factor[tid] * (double)mine.sum : 0.0, room, sum);
+    if (mine.top > -INFINITY) atomicAdd(&found[3], p.hist_n[((long)row * p.chunks + tid) * BINS + BINS - 1]);
+    double mass = 0.0;
+    int n = 0;
+#pragma unroll 4
+    for (int c = half; c < p.chunks; c += 2) {   // (the halves' chunks and their order are always the same)
+        const long at = ((long)row * p.chunks + c) * BINS;
+        const int x = b - (tops[c] == -INFINITY ? BINS : r.grid - place(tops[c], h.scale));
+        const bool on = x >= 0 && x < BINS - 1 && b < BINS - 1;
+        const u64 w = on ? p.hist_w[at + x] : 0;
+        n += on ? p.hist_n[at + x] : 0;
+        mass += factor[c] * (double)w;
     }
     r.sum = sum;
-    const int own_n = n, k = h.k < there ? h.k : 0;
-    for (int d = 1; d < BINS; d <<= 1) {   // sums up to the bin
+    if (half) {
         masses[b] = mass;
         counts[b] = n;
-        __syncthreads();
-        if (b >= d) {
-            mass += masses[b - d];
-            n += counts[b - d];
-        }
-        __syncthreads();
     }
-    masses[b] = mass;
-    counts[b] = n;
-    if (b < 3) found[b] = BINS;
     __syncthreads();
-    const bool in = b < BINS - 1;
+    if (!half) {
+        mass += masses[b];
+        n += counts[b];
+    }
+    const int there = found[3];
+    const int own_n = n, k = h.k < there ? h.k : 0;
+    double all_mass;
+    int all_n;
+    mass = scan_all(half ? 0.0 : mass, room, all_mass);   // sums up to the bin
+    n = scan_all(half ? 0 : n, room_n, all_n);
+    if (!half) {
+        masses[b] = mass;
+        counts[b] = n;
+    }
+    __syncthreads();
+    const bool in = !half && b < BINS - 1;
     if (k && in && n >= k && n - own_n < k) found[2] = b;
     __syncthreads();
     r.kth = found[2];
@@ -254,7 +326,7 @@ __global__ __launch_bounds__(BINS) void sample_rows_kernel(const Params p) {
         if (mass >= (double)h.p * high * (1.0 + 1e-10)) atomicMin(&found[1], b);
     }
     __syncthreads();
-    if (b) return;
+    if (tid) return;
     r.how = k && r.kth == BINS ? SEARCH : LIST;   // (the k-th lies below the bins)
     if (h.p < 1.f) {
         r.to = std::min(found[1], r.kth);
@@ -275,7 +347,7 @@ __global__ __launch_bounds__(BINS) void sample_rows_kernel(const Params p) {
 
 template <bool BF16>
 __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
-    __shared__ u64 room[LANES / 64];
+    __shared__ u64 room[WAVES];
     __shared__ int n;
     const int chunk = blockIdx.x, row = blockIdx.y;
     const Row r = p.row[row];
@@ -297,7 +369,7 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
             if (x[e] == -INFINITY) continue;
             const int b = r.grid - place(x[e], h.scale);
             if (b < r.from) {
-                if (x[e] == r.top || ((double)x[e] - (double)r.top) * h.inv >= least) kept += units(weight(x[e], s.top, h.inv));
+                if (x[e] == r.top || ((double)x[e] - (double)r.top) * h.inv >= least) kept += units(weight(x[e], s.top, h.by_two));
             } else if (b <= r.to || b == r.kth) {
                 const int i = atomicAdd(&n, 1);
                 if (i < SEGMENT) p.list[at * SEGMENT + i] = make_uint2(ordered(x[e]), index_of<BF16>(chunk, e));
@@ -372,29 +444,25 @@ __device__ u64 search(u64 need, u64* sums, int* counts, u64* found, E each) {
 
 template <bool BF16>
 __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, const bool filters) {
-    __shared__ u64 room[LANES / 64];
+    __shared__ u64 room[WAVES];
     __shared__ u64 listed[LISTED];
     __shared__ u64 chunks[MOST_CHUNKS];
     __shared__ u64 sums[256], found[2];
-    __shared__ int counts[256], begins[MOST_CHUNKS + 1];
-    __shared__ double target[2];
+    __shared__ int counts[256], begins[MOST_CHUNKS + 1], room_n[WAVES];
+    __shared__ float tops[MOST_CHUNKS];
+    __shared__ double factor[MOST_CHUNKS], target[2];
     const int row = blockIdx.x, tid = threadIdx.x;
     const How h = settings(p, row);
-    const Stat* stat = p.stat + (long)row * p.chunks;
     Row r = {};
     if (filters) r = p.row[row];
-    else {
-        r.top = h.wrong ? -INFINITY : row_top(p, row);
-        r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
-    }
-    if (r.how == NOTHING || r.how == BEST) {
+    Stat own;
+    r.top = stage(p, row, h, own, tops, factor, (float*)room);
+    if (!filters) r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
+    if (r.how == NOTHING || r.how == BEST) {   // (chunks lie in the order of their indices)
+        const u64 first = r.how == BEST ? over_all(own.top == r.top ? (u64)own.at : ~0ull, room, [](u64 a, u64 b) { return a < b ? a : b; }) : ~0ull;
         if (tid == 0) {
-            long token = -1;
-            if (r.how == BEST)
-                for (int c = 0; c < p.chunks && token < 0; c++)
-                    if (stat[c].top == r.top) token = stat[c].at;
-            p.token[row] = token;
-            if (p.prob) p.prob[row] = token < 0 ? 0.f : 1.f;
+            p.token[row] = (long)first;
+            if (p.prob) p.prob[row] = r.how == BEST ? 1.f : 0.f;
         }
         return;
     }
@@ -402,17 +470,14 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
     const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
     u64 last = ~0ull;   // the last number that is kept
     if (r.how == LIST) {
-        int n = 0;
-        for (int c = 0; c < p.chunks; c++) {
-            const int m = p.count[(long)row * p.chunks + c];
-            if (tid == 0) begins[c] = n;
-            n = m > SEGMENT || n + m > LISTED ? LISTED + 1 : n + m;
-        }
-        if (tid == 0) begins[p.chunks] = n;
-        __syncthreads();
-        if (n > LISTED) r.how = SEARCH;
+        const int m = tid < p.chunks ? p.count[(long)row * p.chunks + tid] : 0;
+        int n;
+        const int upto = scan_all(m, room_n, n);
+        if (tid < p.chunks) begins[tid + 1] = upto;
+        if (tid == 0) begins[0] = 0;
+        if (__syncthreads_or(m > SEGMENT) || n > LISTED) r.how = SEARCH;
         else {
-            for (int c = tid >> 6; c < p.chunks; c += LANES / 64)
+            for (int c = tid >> 6; c < p.chunks; c += WAVES)
                 for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
                     const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
                     listed[i] = (u64)~y.x << 32 | y.y;
@@ -429,17 +494,17 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
                     u64 w = 0;
                     for (int i = tid; i < n; i += LANES) {
                         const float x = value(listed[i]);
-                        if (listed[i] <= last && r.grid - place(x, h.scale) == r.kth) w += units(weight(x, r.top, h.inv));
+                        if (listed[i] <= last && r.grid - place(x, h.scale) == r.kth) w += units(weight(x, r.top, h.by_two));
                     }
                     all = r.mass_k + UNIT * (double)sum_all(w, room);
                 }
             }
             if (h.p < 1.f) {
-                const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p49);
+                const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
                 const u64 border = search(need < 1.0 ? 1 : (u64)need, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
                     for (int i = tid; i < n; i += LANES) {
                         const float x = value(listed[i]);
-                        if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to) f(listed[i], units(weight(x, r.top, h.inv)));
+                        if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to) f(listed[i], units(weight(x, r.top, h.by_two)));
                     }
                 });
                 last = std::min(last, border);
@@ -450,7 +515,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
             for (int i = tid; i < n; i += LANES) {
                 const float x = value(listed[i]);
                 const int c = (int)((unsigned)listed[i] / CHUNK);
-                if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to && stays(x)) atomicAdd(&chunks[c], units(weight(x, stat[c].top, h.inv)));
+                if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to && stays(x)) atomicAdd(&chunks[c], units(weight(x, tops[c], h.by_two)));
             }
         }
     }
@@ -458,7 +523,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
         last = ~0ull;
         const auto each = [&](auto f) __attribute__((always_inline)) {
             for (int c = 0; c < p.chunks; c++) {
-                if (stat[c].top == -INFINITY) continue;
+                if (tops[c] == -INFINITY) continue;
                 float x[EACH];
                 load<BF16>(p, row, c, x);
 #pragma unroll
@@ -466,8 +531,8 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
                     if (x[e] > -INFINITY) f(x[e], number(x[e], index_of<BF16>(c, e)));
             }
         };
-        // (up to 2^22 of them: units of 2^-40 leave room for the sum)
-        const auto worth = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.inv)) + 256) >> 9; };
+        // (up to 2^22 of them: units of 2^-38 leave room for the sum)
+        const auto worth = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.by_two)) + 256) >> 9; };
         if (h.k) last = search(h.k, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
         if (h.p < 1.f) {
             u64 w = 0;
@@ -481,41 +546,37 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
         }
         for (int c = 0; c < p.chunks; c++) {
             u64 w = 0;
-            if (stat[c].top > -INFINITY) {
+            if (tops[c] > -INFINITY) {
                 float x[EACH];
                 load<BF16>(p, row, c, x);
 #pragma unroll
                 for (int e = 0; e < EACH; e++)
-                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += units(weight(x[e], stat[c].top, h.inv));
+                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += units(weight(x[e], tops[c], h.by_two));
             }
             w = sum_all(w, room);
             if (tid == 0) chunks[c] = w;
         }
     } else if (r.how == PLAIN) {
-        for (int c = tid; c < p.chunks; c += LANES) chunks[c] = stat[c].top == -INFINITY ? 0 : stat[c].sum;
+        if (tid < p.chunks) chunks[tid] = own.sum;
     }
     __syncthreads();
-    if (tid == 0) {   // the chunk, and how much of it lies before the token
-        double all = 0.0;
-        for (int c = 0; c < p.chunks; c++)
-            if (chunks[c]) all += weight(stat[c].top, r.top, h.inv) * UNIT * (double)chunks[c];
+    {   // the chunk, and how much of it lies before the token
+        const double mine = tid < p.chunks ? factor[tid] * (double)chunks[tid] : 0.0;
+        double all;
+        const double upto = scan_all(mine, (double*)room, all);
         double u = p.u_f64 ? ((const double*)p.u)[row] : (double)((const float*)p.u)[row];
         u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
         const double want = u * all;
-        double before = 0.0;
-        int at = -1;
-        target[0] = 0.0;
-        for (int c = 0; c < p.chunks; c++) {
-            if (!chunks[c]) continue;
-            const double f = weight(stat[c].top, r.top, h.inv) * UNIT, mine = f * (double)chunks[c];
-            at = c;
-            target[0] = (want - before) / f;
-            if (before + mine > want) break;
-            before += mine;
+        const bool some = mine > 0.0;
+        const int hit = over_all(some && upto > want ? tid : LANES, room_n, [](int a, int b) { return a < b ? a : b; });
+        const int end = over_all(some ? tid : -1, room_n, [](int a, int b) { return a > b ? a : b; });
+        if (tid == 0) begins[0] = -1;
+        __syncthreads();
+        if (tid == (hit < LANES ? hit : end)) {   // (where rounding left no chunk: the last that has any)
+            begins[0] = tid;
+            target[0] = (want - (upto - mine)) / factor[tid];
+            target[1] = all;
         }
-        begins[0] = at;
-        target[1] = all;
-        found[0] = found[1] = ~0ull;
     }
     __syncthreads();
     const int chunk = begins[0];
@@ -527,28 +588,28 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
         return;
     }
     const u64 want = target[0] > 0.0 ? (u64)target[0] : 0;
-    const float top = stat[chunk].top;
+    const float top = tops[chunk];
     // a lane's 16 logits one after the other
     u64 w[EACH], mine = 0;
     const int first = chunk * CHUNK + tid * EACH;
+    float x[EACH];
+    if (p.aligned && first + EACH <= p.vocab) {
+        constexpr int V = VEC<BF16>;
+#pragma unroll
+        for (int i = 0; i < EACH; i += V) load_vec<BF16>(p, row, first + i, x + i);
+    } else {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) x[e] = first + e < p.vocab ? load1<BF16>(p, row, first + e) : -INFINITY;
+    }
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        const float x = first + e < p.vocab ? clean(load1<BF16>(p, row, first + e)) : -INFINITY;
-        const bool in = x > -INFINITY && (r.how == PLAIN || (number(x, first + e) <= last && stays(x) && (r.how == SEARCH || r.grid - place(x, h.scale) <= r.to)));
-        w[e] = in ? units(weight(x, top, h.inv)) : 0;
+        x[e] = fmaxf(x[e], -INFINITY);
+        const bool in = x[e] > -INFINITY && (r.how == PLAIN || (number(x[e], first + e) <= last && stays(x[e]) && (r.how == SEARCH || r.grid - place(x[e], h.scale) <= r.to)));
+        w[e] = in ? units(weight(x[e], top, h.by_two)) : 0;
         mine += w[e];
     }
-    u64 before = mine;   // sums up to the lane
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 y = __shfl_up(before, d);
-        if ((tid & 63) >= d) before += y;
-    }
-    if ((tid & 63) == 63) room[tid >> 6] = before;
-    __syncthreads();
-    u64 ahead = 0;
-    for (int y = 0; y < (tid >> 6); y++) ahead += room[y];
-    before += ahead - mine;
+    u64 total;
+    u64 before = scan_all(mine, room, total) - mine;   // sums ahead of the lane
     int hit = -1, some = -1;
     u64 hit_w = 0, some_w = 0;
 #pragma unroll
@@ -564,12 +625,13 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
         }
     }
     // the first hit; where rounding left none, the last token that is kept
+    (void)total;
     const u64 best = over_all(hit < 0 ? ~0ull : (u64)hit, room, [](u64 a, u64 b) { return a < b ? a : b; });
     const u64 end = over_all((u64)(some + 1), room, [](u64 a, u64 b) { return a > b ? a : b; });
     const bool is = best != ~0ull ? hit == (int)best : some + 1 == (int)end && some >= 0;
     if (is) {
         p.token[row] = best != ~0ull ? hit : some;
-        if (p.prob) p.prob[row] = (float)((double)(best != ~0ull ? hit_w : some_w) * UNIT * weight(top, r.top, h.inv) / target[1]);
+        if (p.prob) p.prob[row] = (float)((double)(best != ~0ull ? hit_w : some_w) * factor[chunk] / target[1]);
     }
 }
 
@@ -609,7 +671,7 @@ hipError_t launch(const Params& p, bool filters, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (filters) {
         if (e == hipSuccess) {
-            hipLaunchKernelGGL(sample_rows_kernel, dim3(p.rows), dim3(BINS), 0, s, p);
+            hipLaunchKernelGGL(sample_rows_kernel, dim3(p.rows), dim3(LANES), 0, s, p);
             e = hipGetLastError();
         }
         if (e == hipSuccess) {
