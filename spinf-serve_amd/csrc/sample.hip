@@ -31,12 +31,13 @@ constexpr int LANES = 512, WAVES = LANES / 64, EACH = 16, CHUNK = LANES * EACH;
 constexpr int BINS = 256;              // the last one: all below
 constexpr int SEGMENT = 1024;          // tokens of a chunk that lie in the bins in question
 constexpr int LISTED = 8192;           // ... of a row
+constexpr int FEW = 4096;              // up to so many the first k are listed whole: their weights are taken one by one and nobody else's
 constexpr int MOST_CHUNKS = 512;
 constexpr float BINS_PER_UNIT = 12.f;
 
-struct Stat { float top; unsigned at; u64 sum; };       // of a chunk: largest logit (-inf: none), where, weight
-// of a row: largest logit; what to do; bins [from, to] and `kth` in question; of all: weight, kept tokens before the kth bin, weight before it and before `from`
-struct Row { float top; int grid, how, from, to, kth, before_k, unused; double sum, mass_k, mass_from; };
+struct Stat { float top; unsigned at; u64 sum; };       // of a chunk: largest logit (-inf: none), where (of a row with a filter: how many can be drawn), weight
+// of a row: largest logit; what to do; bins [from, to] and `kth` in question (none: BINS); tokens before the kth bin; of all and before `from` and the kth: weight; does top-p have a say
+struct Row { float top; int grid, how, from, to, kth, before_k, by_mass; double sum, mass_k, mass_from; };
 static_assert(sizeof(Stat) == 16 && sizeof(Row) == 56, "workspace layout");
 enum { PLAIN = 0, LIST = 1, SEARCH = 2, NOTHING = 3, BEST = 4 };
 
@@ -49,7 +50,7 @@ struct Params {
     Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
 };
 
-struct How { double inv, by_two; float scale, p, least; int k; bool best, wrong, filtered; };
+struct How { double inv, by_two; float scale, p, least; int k; bool best, wrong, filtered, few; };
 __device__ __forceinline__ How settings(const Params& p, int row) {
     How h;
     const float T = p.temperature ? p.temperature[row] : p.all_temperature;
@@ -68,6 +69,7 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
     }
     if (h.k == 1) h.best = true;
     h.filtered = h.k || h.p < 1.f || h.least > 0.f;
+    h.few = h.k && h.k <= FEW;
     return h;
 }
 
@@ -81,26 +83,31 @@ __device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~order
 // a token's place on the grid of bins; never falls as x grows
 __device__ __forceinline__ int place(float x, float scale) { return (int)floorf(fminf(fmaxf(x * scale, -1e9f), 1e9f)); }
 
-// 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum.  (19 instructions of 64 bits, which run at the rate of
-// 32-bit ones here; with the library's exp the chunks of 320 rows of 262,144 took 195 us.)
-constexpr double series(int k) {
-    double c = 1.0;
-    for (int i = 1; i <= k; i++) c *= 0.69314718055994530942 / i;
-    return c;
-}
-__device__ __forceinline__ double power(double t) {
-    t = fmax(t, -1000.0);
-    const double n = __builtin_rint(t), f = t - n;
-    double y = series(12);
+// 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum.  (Some 20 instructions of 64 bits, which run at the rate of
+// 32-bit ones here; with the library's exp the chunks of 320 rows of 262,144 took 195 us.)  The coefficients are pinned to scalar registers: left alone, the compiler moves each into
+// vector registers in front of every product.
+struct Powers {
+    double c[13];
+    __device__ __forceinline__ Powers() {
+        c[0] = 1.0;
 #pragma unroll
-    for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, k == 11 ? series(11) : k == 10 ? series(10) : k == 9 ? series(9) : k == 8 ? series(8) : k == 7 ? series(7) : k == 6 ? series(6) : k == 5 ? series(5)
-                                                       : k == 4 ? series(4) : k == 3 ? series(3) : k == 2 ? series(2) : k == 1 ? series(1) : 1.0);
-    return __builtin_ldexp(y, (int)n);
-}
+        for (int k = 1; k <= 12; k++) c[k] = c[k - 1] * (0.69314718055994530942 / k);
+#pragma unroll
+        for (int k = 1; k <= 12; k++) asm("" : "+s"(c[k]));
+    }
+    __device__ __forceinline__ double of(double t) const {
+        t = fmax(t, -1000.0);
+        const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);   // (the nearest whole number, in the last bits)
+        double y = c[12];
+#pragma unroll
+        for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, c[k]);
+        return __longlong_as_double(__double_as_longlong(y) + ((long long)(int)__double_as_longlong(whole) << 52));
+    }
+};
 // exp((x - top) / T) of finite numbers (x may be -inf: nothing), 1 for the largest
-__device__ __forceinline__ double weight_of(float x, float top, double by_two) { return power(((double)x - (double)top) * by_two); }
+__device__ __forceinline__ double weight_of(const Powers& two, float x, float top, double by_two) { return two.of(((double)x - (double)top) * by_two); }
 // ... of any: where the largest are infinite, only they have a weight
-__device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : weight_of(x, top, by_two); }
+__device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : weight_of(Powers(), x, top, by_two); }
 // in units of 2^-47: the last bits of w + 32, rounded there
 __device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 32.0) - __double_as_longlong(32.0)); }
 constexpr double UNIT = 0x1p-47;
@@ -208,9 +215,10 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
         return;
     }
     if (!h.filtered && top < INFINITY) {
+        const Powers two;
         double sum = 32.0;   // (16 weights of at most 1 leave it below 64: it counts in units of 2^-47)
 #pragma unroll
-        for (int e = 0; e < EACH; e++) sum += weight_of(x[e], top, h.by_two);
+        for (int e = 0; e < EACH; e++) sum += weight_of(two, x[e], top, h.by_two);
         s.sum = sum_all((u64)(__double_as_longlong(sum) - __double_as_longlong(32.0)), room);
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
@@ -221,26 +229,38 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
     }
     __syncthreads();
     const int grid = place(top, h.scale);
-    int there = 0;   // logits that can be drawn
+    if (h.few) {   // counts alone
+        int there = 0;   // logits that can be drawn
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            there += x[e] > -INFINITY;
+            const int b = grid - place(x[e], h.scale);
+            if (x[e] > -INFINITY && b < BINS - 1) atomicAdd(&numbers[b], 1);
+        }
+        there = over_all(there, (int*)room, [](int a, int b) { return a + b; });   // (its barriers are behind the bins' last addition)
+        if (threadIdx.x == 0) p.stat[at] = {top, (unsigned)there, 0};
+        if (threadIdx.x < BINS) p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
+        return;
+    }
+    const Powers two;
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        there += x[e] > -INFINITY;
-        const u64 w = units(weight(x[e], top, h.by_two));
+        const bool on = x[e] > -INFINITY;
+        const u64 w = on ? units(x[e] == top ? 1.0 : top == INFINITY ? 0.0 : weight_of(two, x[e], top, h.by_two)) : 0;
         s.sum += w;
+        s.at += on;
         const int b = grid - place(x[e], h.scale);
-        if (h.filtered && x[e] > -INFINITY && b < BINS - 1) {
+        if (h.filtered && on && b < BINS - 1) {
             atomicAdd(&weights[b], w);
-            atomicAdd(&numbers[b], 1);
+            if (h.k) atomicAdd(&numbers[b], 1);
         }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) there += __shfl_xor(there, d);
-    if ((threadIdx.x & 63) == 0) atomicAdd(&numbers[BINS - 1], there);   // (of all bins and below)
-    s.sum = sum_all(s.sum, room);   // (its barriers are behind the bins' last addition)
+    s.sum = sum_all(s.sum, room);
+    s.at = over_all((int)s.at, (int*)room, [](int a, int b) { return a + b; });
     if (threadIdx.x == 0) p.stat[at] = s;
     if (h.filtered && threadIdx.x < BINS) {
         p.hist_w[at * BINS + threadIdx.x] = weights[threadIdx.x];
-        p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
+        if (h.k) p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
     }
 }
 
@@ -277,21 +297,31 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
     r.grid = place(r.top, h.scale);
     if (tid < 4) found[tid] = tid < 3 ? BINS : 0;
     __syncthreads();
-    double sum;
-    scan_all(tid < p.chunks ? factor[tid] * (double)mine.sum : 0.0, room, sum);
-    if (mine.top > -INFINITY) atomicAdd(&found[3], p.hist_n[((long)row * p.chunks + tid) * BINS + BINS - 1]);
+    if (mine.top > -INFINITY) atomicAdd(&found[3], (int)mine.at);
     double mass = 0.0;
     int n = 0;
-#pragma unroll 4
-    for (int c = half; c < p.chunks; c += 2) {   // (the halves' chunks and their order are always the same)
-        const long at = ((long)row * p.chunks + c) * BINS;
-        const int x = b - (tops[c] == -INFINITY ? BINS : r.grid - place(tops[c], h.scale));
-        const bool on = x >= 0 && x < BINS - 1 && b < BINS - 1;
-        const u64 w = on ? p.hist_w[at + x] : 0;
-        n += on ? p.hist_n[at + x] : 0;
-        mass += factor[c] * (double)w;
+    {   // (the halves' chunks and their order are always the same)
+        constexpr int AHEAD = 8;
+        for (int c0 = half; c0 < p.chunks; c0 += 2 * AHEAD) {
+            u64 w[AHEAD];
+            int m[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int c = c0 + 2 * i;
+                int x = BINS;
+                if (c < p.chunks && tops[c] > -INFINITY) x = b - (r.grid - place(tops[c], h.scale));
+                const long at = ((long)row * p.chunks + c) * BINS + x;
+                const bool on = x >= 0 && x < BINS - 1 && b < BINS - 1;
+                w[i] = on && !h.few ? p.hist_w[at] : 0;
+                m[i] = on && h.k ? p.hist_n[at] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                n += m[i];
+                if (w[i]) mass += factor[c0 + 2 * i] * (double)w[i];
+            }
+        }
     }
-    r.sum = sum;
     if (half) {
         masses[b] = mass;
         counts[b] = n;
@@ -301,22 +331,33 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
         mass += masses[b];
         n += counts[b];
     }
-    const int there = found[3];
-    const int own_n = n, k = h.k < there ? h.k : 0;
-    double all_mass;
-    int all_n;
-    mass = scan_all(half ? 0.0 : mass, room, all_mass);   // sums up to the bin
-    n = scan_all(half ? 0 : n, room_n, all_n);
-    if (!half) {
-        masses[b] = mass;
-        counts[b] = n;
-    }
-    __syncthreads();
+    const int there = found[3], k = h.k < there ? h.k : 0;
     const bool in = !half && b < BINS - 1;
-    if (k && in && n >= k && n - own_n < k) found[2] = b;
+    r.kth = BINS;
+    if (h.k) {
+        const int own = n;
+        int all;
+        n = scan_all(half ? 0 : n, room_n, all);   // tokens up to the bin
+        if (!half) counts[b] = n;
+        if (in && n >= k && n - own < k) found[2] = b;
+        __syncthreads();
+        r.kth = found[2];
+    }
+    if (h.few) {
+        r.how = k && r.kth == BINS ? SEARCH : LIST;   // (the k-th lies below the bins)
+        r.to = k ? r.kth : INT_MAX;                   // (all that can be drawn are the first k)
+        r.kth = k ? r.kth : BINS;
+        r.before_k = k && r.kth < BINS && r.kth ? counts[r.kth - 1] : 0;
+        r.by_mass = h.p < 1.f;
+        if (tid == 0) p.row[row] = r;
+        return;
+    }
+    scan_all(tid < p.chunks ? factor[tid] * (double)mine.sum : 0.0, room, r.sum);
+    double all;
+    mass = scan_all(half ? 0.0 : mass, room, all);   // weight up to the bin
+    if (!half) masses[b] = mass;
     __syncthreads();
-    r.kth = found[2];
-    double low = sum, high = sum;   // the weight of the first k lies between
+    double low = r.sum, high = r.sum;   // the weight of the first k lies between
     if (r.kth < BINS) {
         high = masses[r.kth];
         low = r.kth ? masses[r.kth - 1] : 0.0;
@@ -327,20 +368,44 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
     }
     __syncthreads();
     if (tid) return;
-    r.how = k && r.kth == BINS ? SEARCH : LIST;   // (the k-th lies below the bins)
-    if (h.p < 1.f) {
+    r.how = k && r.kth == BINS ? SEARCH : LIST;
+    r.by_mass = h.p < 1.f;
+    r.from = r.to = r.kth;
+    if (r.by_mass) {
         r.to = std::min(found[1], r.kth);
         r.from = std::min(found[0], r.to);
         if (r.to == BINS) r.how = SEARCH;
-    } else {
-        r.from = r.to = k ? r.kth : INT_MAX;   // (no bin in question: all are kept that min-p leaves)
     }
+    if (h.least > 0.f && r.how == LIST) {
+        // min-p's border and two numbers to either side of it
+        const double border = (double)r.top + log((double)h.least) / h.inv;
+        int above = 0, below = BINS;
+        if (border == border && r.top < INFINITY) {
+            float x = (float)fmin(fmax(border, -3e38), 3e38), up = x, down = x;
+            for (int i = 0; i < 2; i++) {
+                up = nextafterf(up, INFINITY);
+                down = nextafterf(down, -INFINITY);
+            }
+            above = std::max(0, r.grid - place(up, h.scale));
+            below = std::max(0, r.grid - place(down, h.scale));
+        }
+        if (below < r.from) {   // it decides alone
+            r.from = above;
+            r.to = below;
+            r.kth = BINS;
+            r.by_mass = 0;
+        } else {
+            r.from = std::min(r.from, above);
+            if (r.from < BINS && r.to >= BINS - 1 && r.kth == BINS) r.how = SEARCH;   // (it lies below the bins, and nothing else decides)
+        }
+    }
+    if (r.from >= BINS - 1) r.how = SEARCH;
     if (r.how == LIST) {
         if (r.kth < BINS) {
             r.before_k = r.kth ? counts[r.kth - 1] : 0;
             r.mass_k = low;
         }
-        r.mass_from = r.from > 0 && r.from < BINS ? masses[r.from - 1] : 0.0;
+        r.mass_from = r.from > 0 ? masses[r.from - 1] : 0.0;
     }
     p.row[row] = r;
 }
@@ -353,30 +418,25 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
     const Row r = p.row[row];
     if (r.how != LIST) return;
     const long at = (long)row * p.chunks + chunk;
-    const Stat s = p.stat[at];
+    const float top = p.stat[at].top;
     if (threadIdx.x == 0) n = 0;
     __syncthreads();
-    u64 kept = 0;
     const How h = settings(p, row);
-    // (a chunk whose largest logit lies behind the bins in question has nothing that matters)
-    const int begin = s.top == -INFINITY ? INT_MAX : r.grid - place(s.top, h.scale);
-    if (begin <= r.to || begin <= r.kth) {
-        const double least = log((double)h.least);
+    const int begin = top == -INFINITY ? INT_MAX : r.grid - place(top, h.scale);   // its first bin
+    u64 kept = begin < r.from && (int)threadIdx.x < std::min(r.from - begin, BINS - 1) ? p.hist_w[at * BINS + threadIdx.x] : 0;   // all of the bins ahead of those in question
+    if (begin <= r.to || begin == r.kth || (begin < r.kth && r.kth < BINS)) {
         float x[EACH];
         load<BF16>(p, row, chunk, x);
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            if (x[e] == -INFINITY) continue;
             const int b = r.grid - place(x[e], h.scale);
-            if (b < r.from) {
-                if (x[e] == r.top || ((double)x[e] - (double)r.top) * h.inv >= least) kept += units(weight(x[e], s.top, h.by_two));
-            } else if (b <= r.to || b == r.kth) {
+            if (x[e] > -INFINITY && b >= r.from && (b <= r.to || b == r.kth)) {
                 const int i = atomicAdd(&n, 1);
-                if (i < SEGMENT) p.list[at * SEGMENT + i] = make_uint2(ordered(x[e]), index_of<BF16>(chunk, e));
+                if (i < SEGMENT) p.list[at * SEGMENT + i] = make_uint2(ordered(x[e] + 0.f), index_of<BF16>(chunk, e));
             }
         }
     }
-    kept = sum_all(kept, room);
+    kept = sum_all(kept, room);   // (its barriers are behind the last count)
     if (threadIdx.x == 0) {
         p.kept[at] = kept;
         p.count[at] = n;
@@ -384,21 +444,25 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
 }
 
 // The least number up to which (it counted in) those of `each` hold at least `need` in all; ~0: all of them hold less.  each(f) calls f(number, worth) for every one in question,
-// each lane for its share.  Eight bits at a time, from the top.
+// each lane for its share; all of them lie in low .. high.  Eight bits at a time, from the first that differs.
 template <class E>
-__device__ u64 search(u64 need, u64* sums, int* counts, u64* found, E each) {
-    u64 prefix = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
+__device__ u64 search(u64 need, u64 low, u64 high, u64* sums, int* counts, u64* found, E each) {
+    int above = low == high ? 0 : 64 - __builtin_clzll(low ^ high);   // bits in question
+    u64 prefix = low;
+    bool first = true;
+    while (above > 0 || first) {
+        const int shift = above > 8 ? above - 8 : 0;
         __syncthreads();
         if (threadIdx.x < 256) {
             sums[threadIdx.x] = 0;
             counts[threadIdx.x] = 0;
         }
-        if (threadIdx.x == 0) found[0] = found[1] = ~0ull;
+        if (threadIdx.x == 0) found[0] = found[1] = found[2] = ~0ull;
         __syncthreads();
+        const u64 mask = above < 64 ? ~0ull << above : 0;
         each([&](u64 c, u64 worth) __attribute__((always_inline)) {
-            if (shift == 56 || c >> (shift + 8) == prefix >> (shift + 8)) {
-                const int digit = (int)(c >> shift) & 255;
+            if (((c ^ prefix) & mask) == 0) {
+                const int digit = (int)(c >> shift) & 255 & ((1 << (above - shift)) - 1);
                 atomicAdd(&sums[digit], worth);
                 atomicAdd(&counts[digit], 1);
             }
@@ -422,19 +486,19 @@ __device__ u64 search(u64 need, u64* sums, int* counts, u64* found, E each) {
             }
         }
         __syncthreads();
-        if (found[0] == ~0ull) return ~0ull;   // (of the first digit alone)
-        prefix |= found[0] << shift;
+        const u64 digit = found[0];
+        if (digit == ~0ull) return ~0ull;   // (of the first digit alone)
         need = found[1];
-        const bool only = counts[found[0]] == 1;
-        if (only && shift) {   // the rest of its digits
-            __syncthreads();
-            if (threadIdx.x == 0) found[0] = 0;
-            __syncthreads();
+        prefix = (prefix & mask) | digit << shift;
+        above = shift;
+        first = false;
+        if (shift && counts[digit] == 1) {   // the rest of its digits
+            const u64 here = ~0ull << shift;
             each([&](u64 c, u64) __attribute__((always_inline)) {
-                if (c >> shift == prefix >> shift) found[0] = c;
+                if (((c ^ prefix) & here) == 0) found[2] = c;
             });
             __syncthreads();
-            prefix = found[0];
+            prefix = found[2];
             break;
         }
     }
@@ -442,22 +506,22 @@ __device__ u64 search(u64 need, u64* sums, int* counts, u64* found, E each) {
     return prefix;
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, const bool filters) {
+template <bool BF16, bool FILTERS>
+__global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     __shared__ u64 room[WAVES];
-    __shared__ u64 listed[LISTED];
+    __shared__ u64 listed[FILTERS ? LISTED : 1], worth[FILTERS ? LISTED : 1];   // numbers of the tokens in question, and their weights
     __shared__ u64 chunks[MOST_CHUNKS];
-    __shared__ u64 sums[256], found[2];
+    __shared__ u64 sums[256], found[3];
     __shared__ int counts[256], begins[MOST_CHUNKS + 1], room_n[WAVES];
     __shared__ float tops[MOST_CHUNKS];
     __shared__ double factor[MOST_CHUNKS], target[2];
     const int row = blockIdx.x, tid = threadIdx.x;
     const How h = settings(p, row);
     Row r = {};
-    if (filters) r = p.row[row];
+    if (FILTERS) r = p.row[row];
     Stat own;
     r.top = stage(p, row, h, own, tops, factor, (float*)room);
-    if (!filters) r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
+    if (!FILTERS) r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
     if (r.how == NOTHING || r.how == BEST) {   // (chunks lie in the order of their indices)
         const u64 first = r.how == BEST ? over_all(own.top == r.top ? (u64)own.at : ~0ull, room, [](u64 a, u64 b) { return a < b ? a : b; }) : ~0ull;
         if (tid == 0) {
@@ -469,7 +533,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
     const double least = log((double)h.least);
     const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
     u64 last = ~0ull;   // the last number that is kept
-    if (r.how == LIST) {
+    if (FILTERS && r.how == LIST) {
         const int m = tid < p.chunks ? p.count[(long)row * p.chunks + tid] : 0;
         int n;
         const int upto = scan_all(m, room_n, n);
@@ -477,50 +541,52 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
         if (tid == 0) begins[0] = 0;
         if (__syncthreads_or(m > SEGMENT) || n > LISTED) r.how = SEARCH;
         else {
+            const Powers two;
+            const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
+            const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
+            u64 low = ~0ull, high = 0;
             for (int c = tid >> 6; c < p.chunks; c += WAVES)
                 for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
                     const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
-                    listed[i] = (u64)~y.x << 32 | y.y;
+                    const u64 x = (u64)~y.x << 32 | y.y;
+                    const float v = unordered(y.x);
+                    listed[i] = x;
+                    worth[i] = units(v == r.top ? 1.0 : r.top == INFINITY ? 0.0 : weight_of(two, v, r.top, h.by_two));
+                    low = std::min(low, x);
+                    high = std::max(high, x);
                 }
-            __syncthreads();
-            const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
-            double all = r.sum;   // weight of the first k
-            if (r.kth < BINS) {
-                last = search(h.k - r.before_k, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+            low = over_all(low, room, [](u64 a, u64 b) { return a < b ? a : b; });
+            high = over_all(high, room, [](u64 a, u64 b) { return a > b ? a : b; });
+            if (r.kth < BINS)
+                last = search(h.k - r.before_k, low, high, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
                     for (int i = tid; i < n; i += LANES)
-                        if (r.grid - place(value(listed[i]), h.scale) == r.kth) f(listed[i], 1);
+                        if (bin(listed[i]) == r.kth) f(listed[i], 1);
                 });
-                if (h.p < 1.f) {
+            if (r.by_mass) {
+                double all = r.sum;   // weight of the first k
+                if (r.kth < BINS || h.few) {
                     u64 w = 0;
-                    for (int i = tid; i < n; i += LANES) {
-                        const float x = value(listed[i]);
-                        if (listed[i] <= last && r.grid - place(x, h.scale) == r.kth) w += units(weight(x, r.top, h.by_two));
-                    }
-                    all = r.mass_k + UNIT * (double)sum_all(w, room);
+                    for (int i = tid; i < n; i += LANES)
+                        if (listed[i] <= last && (h.few || bin(listed[i]) == r.kth)) w += worth[i];
+                    all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(w, room);
                 }
-            }
-            if (h.p < 1.f) {
                 const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
-                const u64 border = search(need < 1.0 ? 1 : (u64)need, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
-                    for (int i = tid; i < n; i += LANES) {
-                        const float x = value(listed[i]);
-                        if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to) f(listed[i], units(weight(x, r.top, h.by_two)));
-                    }
-                });
-                last = std::min(last, border);
+                last = std::min(last, search(need < 1.0 ? 1 : (u64)need, low, high, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                    for (int i = tid; i < n; i += LANES)
+                        if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to)) f(listed[i], worth[i]);
+                }));
             }
-            // what is kept of them, by chunk
-            for (int c = tid; c < p.chunks; c += LANES) chunks[c] = p.kept[(long)row * p.chunks + c];
+            // what is kept, by chunk
+            if (tid < p.chunks) chunks[tid] = p.kept[(long)row * p.chunks + tid];
             __syncthreads();
             for (int i = tid; i < n; i += LANES) {
                 const float x = value(listed[i]);
                 const int c = (int)((unsigned)listed[i] / CHUNK);
-                if (listed[i] <= last && r.grid - place(x, h.scale) <= r.to && stays(x)) atomicAdd(&chunks[c], units(weight(x, tops[c], h.by_two)));
+                if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to) && stays(x)) atomicAdd(&chunks[c], units(weight(x, tops[c], h.by_two)));
             }
         }
     }
-    if (r.how == SEARCH) {
-        last = ~0ull;
+    if (FILTERS && r.how == SEARCH) {
         const auto each = [&](auto f) __attribute__((always_inline)) {
             for (int c = 0; c < p.chunks; c++) {
                 if (tops[c] == -INFINITY) continue;
@@ -532,15 +598,15 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
             }
         };
         // (up to 2^22 of them: units of 2^-38 leave room for the sum)
-        const auto worth = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.by_two)) + 256) >> 9; };
-        if (h.k) last = search(h.k, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
+        const auto coarse = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.by_two)) + 256) >> 9; };
+        if (h.k) last = search(h.k, 0, ~0ull, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
         if (h.p < 1.f) {
             u64 w = 0;
-            each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) w += worth(x); });
+            each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) w += coarse(x); });
             w = sum_all(w, room);
             const double need = ceil((double)h.p * (double)w);
-            const u64 border = search(need < 1.0 ? 1 : (u64)need, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
-                each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) f(c, worth(x)); });
+            const u64 border = search(need < 1.0 ? 1 : (u64)need, 0, ~0ull, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) f(c, coarse(x)); });
             });
             last = std::min(last, border);
         }
@@ -604,7 +670,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p, cons
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         x[e] = fmaxf(x[e], -INFINITY);
-        const bool in = x[e] > -INFINITY && (r.how == PLAIN || (number(x[e], first + e) <= last && stays(x[e]) && (r.how == SEARCH || r.grid - place(x[e], h.scale) <= r.to)));
+        const bool in = x[e] > -INFINITY && (r.how == PLAIN || (number(x[e], first + e) <= last && stays(x[e]) && (r.how == SEARCH || h.few || r.grid - place(x[e], h.scale) <= r.to)));
         w[e] = in ? units(weight(x[e], top, h.by_two)) : 0;
         mine += w[e];
     }
@@ -680,7 +746,8 @@ hipError_t launch(const Params& p, bool filters, hipStream_t s) {
         }
     }
     if (e == hipSuccess) {
-        hipLaunchKernelGGL(sample_draw_kernel<BF16>, dim3(p.rows), dim3(LANES), 0, s, p, filters);
+        if (filters) hipLaunchKernelGGL((sample_draw_kernel<BF16, true>), dim3(p.rows), dim3(LANES), 0, s, p);
+        else hipLaunchKernelGGL((sample_draw_kernel<BF16, false>), dim3(p.rows), dim3(LANES), 0, s, p);
         e = hipGetLastError();
     }
     return e;
