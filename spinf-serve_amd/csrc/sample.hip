@@ -50,7 +50,7 @@ struct Params {
     Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
 };
 
-struct How { double inv, by_two; float scale, p, least; int k; bool best, wrong, filtered, few; };
+struct How { double inv, by_two; float scale, far, p, least; int k; bool best, wrong, filtered, few, plain; };
 __device__ __forceinline__ How settings(const Params& p, int row) {
     How h;
     const float T = p.temperature ? p.temperature[row] : p.all_temperature;
@@ -62,6 +62,8 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
     h.inv = 1.0 / (double)T;
     h.by_two = h.inv * 1.4426950408889634;
     h.scale = fminf(BINS_PER_UNIT / T, 3e38f);
+    h.far = 60.f * T;
+    h.plain = T < 1e36f;   // (far is finite)
     if (h.k <= 0 || h.k >= p.vocab) h.k = 0;
     if (h.p == 0.f) {   // the first alone
         h.p = 1.f;
@@ -83,31 +85,47 @@ __device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~order
 // a token's place on the grid of bins; never falls as x grows
 __device__ __forceinline__ int place(float x, float scale) { return (int)floorf(fminf(fmaxf(x * scale, -1e9f), 1e9f)); }
 
-// 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum.  (Some 20 instructions of 64 bits, which run at the rate of
-// 32-bit ones here; with the library's exp the chunks of 320 rows of 262,144 took 195 us.)  The coefficients are pinned to scalar registers: left alone, the compiler moves each into
-// vector registers in front of every product.
-struct Powers {
-    double c[13];
-    __device__ __forceinline__ Powers() {
-        c[0] = 1.0;
+// 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum
+__device__ __forceinline__ double power(double t) {
+    t = fmax(t, -1000.0);
+    const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);   // (the nearest whole number, in the last bits)
+    double c[13] = {1.0};
 #pragma unroll
-        for (int k = 1; k <= 12; k++) c[k] = c[k - 1] * (0.69314718055994530942 / k);
+    for (int k = 1; k <= 12; k++) c[k] = c[k - 1] * (0.69314718055994530942 / k);
+    double y = c[12];
 #pragma unroll
-        for (int k = 1; k <= 12; k++) asm("" : "+s"(c[k]));
+    for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, c[k]);
+    return __longlong_as_double(__double_as_longlong(y) + ((long long)(int)__double_as_longlong(whole) << 52));
+}
+// The same for a chunk's logits, where instructions of 64 bits are what bounds the kernel (each takes two of 32 bits): t in 32nds, the whole ones by a table of 2^(j / 32) in LDS and the
+// exponent, the rest by a polynomial of degree 4 through the Chebyshev points of -1/2 .. 1/2: off by 2^-43 of the weight at most, either way.  (With the series above 320 rows of
+// 262,144 logits took 120 us, with the library's exp 195.)
+constexpr int STEPS = 32;
+__device__ __forceinline__ void fill_steps(double* steps) {
+    if (threadIdx.x < STEPS) steps[threadIdx.x] = 2.0 * power(threadIdx.x / (double)STEPS - 1.0);
+}
+struct Weights {   // of a chunk, by its largest logit
+    const double* steps; double top, by_step; float low;
+    double c1, c2, c3, c4;
+    __device__ __forceinline__ Weights(const double* steps, float top, const How& h) : steps(steps), top(top), by_step(h.by_two * STEPS), low(fminf(top - h.far, nextafterf(top, -INFINITY))), c1(0.02166084939172217), c2(0.0002345961981994449), c3(1.6938633903155644e-06), c4(9.172607532092245e-09) {
+        asm("" : "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4));   // (pinned to scalar registers: left alone, the compiler moves each into vector registers in front of every product)
     }
-    __device__ __forceinline__ double of(double t) const {
-        t = fmax(t, -1000.0);
-        const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);   // (the nearest whole number, in the last bits)
-        double y = c[12];
-#pragma unroll
-        for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, c[k]);
-        return __longlong_as_double(__double_as_longlong(y) + ((long long)(int)__double_as_longlong(whole) << 52));
+    // (where the next number below the largest lies hundreds of T away, the exponent would not hold its weight)
+    static __device__ __forceinline__ bool fits(float top, const How& h) { return top < INFINITY && h.plain && top - nextafterf(top, -INFINITY) <= 8.f * h.far; }
+    // exp((x - top) / T) to 2^-43 of it; of what lies some 60 T and more below, and of NaN: less than 2^-70
+    __device__ __forceinline__ double of(float x) const {
+        const double t = ((double)fmaxf(x, low) - top) * by_step;
+        const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);
+        const int n = (int)__double_as_longlong(whole);
+        double y = __builtin_fma(c4, f, c3);
+        y = __builtin_fma(y, f, c2);
+        y = __builtin_fma(y, f, c1);
+        y = __builtin_fma(y, f, 1.0) * steps[n & (STEPS - 1)];
+        return __hiloint2double(__double2hiint(y) + ((n & ~(STEPS - 1)) << 15), __double2loint(y));   // (n / 32 into the exponent)
     }
 };
-// exp((x - top) / T) of finite numbers (x may be -inf: nothing), 1 for the largest
-__device__ __forceinline__ double weight_of(const Powers& two, float x, float top, double by_two) { return two.of(((double)x - (double)top) * by_two); }
-// ... of any: where the largest are infinite, only they have a weight
-__device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : weight_of(Powers(), x, top, by_two); }
+// exp((x - top) / T); where the largest are infinite, only they have a weight
+__device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : power(((double)x - (double)top) * by_two); }
 // in units of 2^-47: the last bits of w + 32, rounded there
 __device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 32.0) - __double_as_longlong(32.0)); }
 constexpr double UNIT = 0x1p-47;
@@ -122,6 +140,8 @@ constexpr int VEC = BF16 ? 8 : 4;
 // index of a lane's e-th logit
 template <bool BF16>
 __device__ __forceinline__ int index_of(int chunk, int e) { return chunk * CHUNK + (e / VEC<BF16> * LANES + (int)threadIdx.x) * VEC<BF16> + e % VEC<BF16>; }
+template <bool BF16>
+__device__ __forceinline__ float load_one(const Params& p, int row, int i) { return i < p.vocab ? fmaxf(load1<BF16>(p, row, i), -INFINITY) : -INFINITY; }
 template <bool BF16>
 __device__ __forceinline__ void load_vec(const Params& p, int row, int at, float* x) {   // 16 bytes, aligned
     if (BF16) {
@@ -150,10 +170,31 @@ __device__ __forceinline__ void load(const Params& p, int row, int chunk, float 
     for (int e = 0; e < EACH; e++) x[e] = fmaxf(x[e], -INFINITY);   // (NaN: never drawn)
 }
 
+// f over the lanes of a wave (whatever their order and grouping): neighbours, pairs, quads and eights by permutations within a row of 16 lanes, then the rows
+template <int CTRL>
+__device__ __forceinline__ unsigned permuted(unsigned x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false); }
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T x, F f) {
+    constexpr int WORDS = sizeof(T) / 4;
+    struct Words { unsigned w[WORDS]; };
+    const auto step = [&](auto move) __attribute__((always_inline)) {
+        const Words a = __builtin_bit_cast(Words, x);
+        Words b, c;
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) move(a.w[i], b.w[i], c.w[i]);
+        x = f(__builtin_bit_cast(T, b), __builtin_bit_cast(T, c));
+    };
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0xb1>(a); });
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x4e>(a); });
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x141>(a); });
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x140>(a); });
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { const auto y = __builtin_amdgcn_permlane16_swap(a, a, false, false); b = y[0]; c = y[1]; });
+    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false); b = y[0]; c = y[1]; });
+    return x;
+}
 template <class T, class F>
 __device__ __forceinline__ T over_all(T x, T* room, F f) {   // room: one place per wave
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = f(x, __shfl_xor(x, d));
+    x = over_wave(x, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
     __syncthreads();
@@ -191,12 +232,14 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
     __shared__ u64 room[WAVES];
     __shared__ u64 weights[BINS];
     __shared__ int numbers[BINS];
+    __shared__ double steps[STEPS];
     const int chunk = blockIdx.x, row = blockIdx.y;
     const How h = settings(p, row);
     if (h.wrong) return;
     float x[EACH];
     load<BF16>(p, row, chunk, x);
     const long at = (long)row * p.chunks + chunk;
+    fill_steps(steps);   // (read behind the barriers of top_all)
     if (h.best) {
         u64 first = ~0ull;   // the least number of the chunk
 #pragma unroll
@@ -214,11 +257,16 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
     }
-    if (!h.filtered && top < INFINITY) {
-        const Powers two;
+    if (!h.filtered) {
         double sum = 32.0;   // (16 weights of at most 1 leave it below 64: it counts in units of 2^-47)
+        if (Weights::fits(top, h)) {
+            const Weights w(steps, top, h);
 #pragma unroll
-        for (int e = 0; e < EACH; e++) sum += weight_of(two, x[e], top, h.by_two);
+            for (int e = 0; e < EACH; e++) sum += w.of(x[e]);
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < EACH; e++) sum += weight(load_one<BF16>(p, row, index_of<BF16>(chunk, e)), top, h.by_two);
+        }
         s.sum = sum_all((u64)(__double_as_longlong(sum) - __double_as_longlong(32.0)), room);
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
@@ -242,23 +290,31 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
         if (threadIdx.x < BINS) p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
         return;
     }
-    const Powers two;
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        const bool on = x[e] > -INFINITY;
-        const u64 w = on ? units(x[e] == top ? 1.0 : top == INFINITY ? 0.0 : weight_of(two, x[e], top, h.by_two)) : 0;
+    const auto take = [&](float x, u64 w) __attribute__((always_inline)) {
+        const bool on = x > -INFINITY;
         s.sum += w;
         s.at += on;
-        const int b = grid - place(x[e], h.scale);
-        if (h.filtered && on && b < BINS - 1) {
+        const int b = grid - place(x, h.scale);
+        if (on && b < BINS - 1) {
             atomicAdd(&weights[b], w);
             if (h.k) atomicAdd(&numbers[b], 1);
+        }
+    };
+    if (Weights::fits(top, h)) {
+        const Weights w(steps, top, h);
+#pragma unroll
+        for (int e = 0; e < EACH; e++) take(x[e], units(w.of(x[e])));
+    } else {
+#pragma unroll 1
+        for (int e = 0; e < EACH; e++) {
+            const float y = load_one<BF16>(p, row, index_of<BF16>(chunk, e));
+            take(y, units(weight(y, top, h.by_two)));
         }
     }
     s.sum = sum_all(s.sum, room);
     s.at = over_all((int)s.at, (int*)room, [](int a, int b) { return a + b; });
     if (threadIdx.x == 0) p.stat[at] = s;
-    if (h.filtered && threadIdx.x < BINS) {
+    if (threadIdx.x < BINS) {
         p.hist_w[at * BINS + threadIdx.x] = weights[threadIdx.x];
         if (h.k) p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
     }
@@ -519,6 +575,11 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     const How h = settings(p, row);
     Row r = {};
     if (FILTERS) r = p.row[row];
+    // (what does not depend on anything is asked for at once: every wait for memory is a microsecond of a row's time)
+    const long mine_at = (long)row * p.chunks + tid;
+    const int own_count = FILTERS && tid < p.chunks ? p.count[mine_at] : 0;
+    const u64 own_kept = FILTERS && tid < p.chunks ? p.kept[mine_at] : 0;
+    const double given = p.u_f64 ? ((const double*)p.u)[row] : (double)((const float*)p.u)[row];
     Stat own;
     r.top = stage(p, row, h, own, tops, factor, (float*)room);
     if (!FILTERS) r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
@@ -534,14 +595,13 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
     u64 last = ~0ull;   // the last number that is kept
     if (FILTERS && r.how == LIST) {
-        const int m = tid < p.chunks ? p.count[(long)row * p.chunks + tid] : 0;
+        const int m = own_count;
         int n;
         const int upto = scan_all(m, room_n, n);
         if (tid < p.chunks) begins[tid + 1] = upto;
         if (tid == 0) begins[0] = 0;
         if (__syncthreads_or(m > SEGMENT) || n > LISTED) r.how = SEARCH;
         else {
-            const Powers two;
             const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
             const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
             u64 low = ~0ull, high = 0;
@@ -551,7 +611,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                     const u64 x = (u64)~y.x << 32 | y.y;
                     const float v = unordered(y.x);
                     listed[i] = x;
-                    worth[i] = units(v == r.top ? 1.0 : r.top == INFINITY ? 0.0 : weight_of(two, v, r.top, h.by_two));
+                    worth[i] = units(v == r.top ? 1.0 : r.top == INFINITY ? 0.0 : power(((double)v - (double)r.top) * h.by_two));
                     low = std::min(low, x);
                     high = std::max(high, x);
                 }
@@ -577,7 +637,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                 }));
             }
             // what is kept, by chunk
-            if (tid < p.chunks) chunks[tid] = p.kept[(long)row * p.chunks + tid];
+            if (tid < p.chunks) chunks[tid] = own_kept;
             __syncthreads();
             for (int i = tid; i < n; i += LANES) {
                 const float x = value(listed[i]);
@@ -630,8 +690,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         const double mine = tid < p.chunks ? factor[tid] * (double)chunks[tid] : 0.0;
         double all;
         const double upto = scan_all(mine, (double*)room, all);
-        double u = p.u_f64 ? ((const double*)p.u)[row] : (double)((const float*)p.u)[row];
-        u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
+        const double u = given > 0.0 ? (given < 1.0 ? given : 1.0) : 0.0;
         const double want = u * all;
         const bool some = mine > 0.0;
         const int hit = over_all(some && upto > want ? tid : LANES, room_n, [](int a, int b) { return a < b ? a : b; });

@@ -209,3 +209,18 @@ def test_graphs_streams_and_the_registered_operator(dev):
         e = sa.sample_tokens(x, u, **how)
         assert torch.equal(token, e[0]) and torch.equal(prob, e[1])
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("base", [1e4, 1e7, 1e9, -1e9, 3e38])
+def test_logits_whose_neighbours_lie_far_apart(dev, base):
+    """numbers of 24 bits next to a large one: steps of 2^-10 to more than any temperature"""
+    g = np.random.default_rng(6)
+    x = np.full(9000, np.float32(base))
+    for i in range(3):
+        x[i::3] = np.nextafter(x[i::3], -np.inf) if i else x[i::3]
+    x[2::3] = np.nextafter(x[2::3], np.float32(-np.inf))
+    x[g.integers(0, 9000, 50)] = np.float32(base) - np.float32(abs(base) * 1e-3)
+    x = x.astype(np.float64)[None].repeat(3, 0)
+    for how in (dict(), dict(temperature=50.0), dict(top_p=0.4), dict(min_p=0.3), dict(top_k=4500, top_p=0.9)):
+        check(dev, x, torch.float32, g.random(3), how)
