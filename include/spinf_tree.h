@@ -451,10 +451,11 @@ int spinf_qk_norm_rope(const spinf_rope_args* args, void* stream);
  *   slots [rows] int64, pos [rows]: where the rows' keys and values go (page * page size + entry) and their positions, text positions of the content counted; -1 and 0 behind
  *   the last row; and for each of the `kinds` head geometries (window 0: none) the work lists of spinf_seats_attn.
  * shared [contents, 3]: stored keys (at most `longest`), positions of the text, first page in `lists`.  Lists, as long as
- * spinf_seats_rooms says ([0 .. 2] items of 12 int32 each, [3] partial rows of the attention's workspace), 16-byte aligned; counts [4]; parts [rows + 1]; seat_parts [2 seats + 1].  One launch
+ * spinf_seats_rooms says ([0 .. 2] items of wave, single and block, 24 int32 each, [3] of last, 12 each; [4] partial rows of the attention's workspace), 16-byte aligned; counts [5]; parts
+ * [rows + 1]; seat_parts [2 seats + 1].  One launch
  * (two where rows > 8,192); nothing is allocated.  At most 2,048 seats and 8 geometries. */
 typedef struct spinf_seats_kind {
-    int32_t* wave; int32_t* single; int32_t* block; int32_t* counts; int32_t* parts; int32_t* seat_parts;
+    int32_t* wave; int32_t* single; int32_t* block; int32_t* last; int32_t* counts; int32_t* parts; int32_t* seat_parts;
     int32_t hq, hkv, d, window;
 } spinf_seats_kind;
 typedef struct spinf_seats_args {
@@ -466,7 +467,7 @@ typedef struct spinf_seats_args {
     int32_t seats, page, contents, kinds;
     spinf_seats_kind kind[8];
 } spinf_seats_args;
-int spinf_seats_rooms(const spinf_seats_args* args, int32_t kind, int64_t rooms[4]);
+int spinf_seats_rooms(const spinf_seats_args* args, int32_t kind, int64_t rooms[5]);
 int spinf_seats_step(const spinf_seats_args* args, void* stream);
 
 /* Attention of a step's new tokens: out[t] = softmax over the keys that row t sees of scale q.k (softcap > 0: of softcap tanh(scale q.k / softcap)) times v, for every row and query head.  A
@@ -474,7 +475,7 @@ int spinf_seats_step(const spinf_seats_args* args, void* stream);
  * content read its keys together.  Rows behind the step's last come out as zeros (lse: -inf).
  *   q, out [rows, hq, d] bf16 (strides in elements, multiples of 8); lse [rows, hq] fp32 or NULL; k, v the cache as above, every page in `lists` one of its;
  *   lists, first, pos as spinf_seats_step leaves them; kind: the lists of this geometry and window; rooms: what spinf_seats_rooms says of it; workspace: 16-byte aligned,
- *   rooms[3] * hq * (d + 2) * 4 bytes, the caller's.  Three launches; nothing is allocated. */
+ *   rooms[4] * hq * (d + 2) * 4 bytes, the caller's.  Up to four launches; nothing is allocated. */
 typedef struct spinf_seats_attn_args {
     const void* q; void* out; float* lse;
     int64_t q_tok, q_head, o_tok, o_head;
@@ -482,7 +483,7 @@ typedef struct spinf_seats_attn_args {
     int64_t k_page, k_row, k_head, v_page, v_row, v_head;
     const int32_t* lists; const int32_t* first; const int32_t* pos;
     spinf_seats_kind kind;
-    int64_t rooms[4];
+    int64_t rooms[5];
     void* workspace; int64_t workspace_bytes;
     int64_t rows;
     int32_t seats, page;

@@ -21,6 +21,7 @@
 
 #include "spinf_tree.h"
 #include "common.h"
+#include "lanes.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef unsigned long long u64;
@@ -170,31 +171,9 @@ __device__ __forceinline__ void load(const Params& p, int row, int chunk, float 
     for (int e = 0; e < EACH; e++) x[e] = fmaxf(x[e], -INFINITY);   // (NaN: never drawn)
 }
 
-// f over the lanes of a wave (whatever their order and grouping): neighbours, pairs, quads and eights by permutations within a row of 16 lanes, then the rows
-template <int CTRL>
-__device__ __forceinline__ unsigned permuted(unsigned x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false); }
-template <class T, class F>
-__device__ __forceinline__ T over_wave(T x, F f) {
-    constexpr int WORDS = sizeof(T) / 4;
-    struct Words { unsigned w[WORDS]; };
-    const auto step = [&](auto move) __attribute__((always_inline)) {
-        const Words a = __builtin_bit_cast(Words, x);
-        Words b, c;
-#pragma unroll
-        for (int i = 0; i < WORDS; i++) move(a.w[i], b.w[i], c.w[i]);
-        x = f(__builtin_bit_cast(T, b), __builtin_bit_cast(T, c));
-    };
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0xb1>(a); });
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x4e>(a); });
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x141>(a); });
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { b = a; c = permuted<0x140>(a); });
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { const auto y = __builtin_amdgcn_permlane16_swap(a, a, false, false); b = y[0]; c = y[1]; });
-    step([](unsigned a, unsigned& b, unsigned& c) __attribute__((always_inline)) { const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false); b = y[0]; c = y[1]; });
-    return x;
-}
 template <class T, class F>
 __device__ __forceinline__ T over_all(T x, T* room, F f) {   // room: one place per wave
-    x = over_wave(x, f);
+    x = over_lanes(x, f);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
     __syncthreads();

@@ -15,26 +15,40 @@ constexpr int SEATS_MOST = 2048;      // seats: their lengths and running sums l
 constexpr int SEATS_KINDS = 8;        // head geometries
 constexpr int SEATS_ROWS_AT_ONCE = 8192;   // rows that the workgroup of the books places itself; more get a launch of their own
 
-// Rows row0 .. of a set of new tokens (tokens tok0 .. tok0 + T - 1 of the call, `group` rows each) over tiles kt0 .. kt0 + tiles - 1 of a span of L keys whose pages begin
-// at `tab` of the page lists.  A span is a content, shared by the set's seats, or a seat's own keys (SEAT_OWN: row t sees them up to L - T + t).  Every row of the item sees the
-// keys flo .. fhi; piece: which of its rows' partial results this is (SEAT_ONLY: there is no other).
-struct SeatItem { int32_t tok0, T, L, tab, row0, kt0, tiles, piece, flo, fhi, flags, unused; };
-static_assert(sizeof(SeatItem) == 48, "written and read as 16-byte pieces");
-constexpr int SEAT_OWN = 1, SEAT_ONLY = 2;
+// Tiles kt0 .. kt0 + tiles - 1 of L keys whose pages begin at `tab` of the page lists: a content's, or (own) a seat's, of which row t of T sees those up to L - T + t.  Every row
+// of the item sees the keys flo .. fhi.
+struct SeatSpan { int32_t tab, L, kt0, tiles, flo, fhi, own, unused; };
+// Rows row0 .. of a set of new tokens (tokens tok0 .. tok0 + T - 1 of the call, `group` rows each) over one span, or over a content and then the seat's own keys; piece: which of
+// its rows' partial results this is (only: there is no other).
+struct SeatItem { int32_t tok0, T, row0, piece, only, unused[3]; SeatSpan span[2]; };
+// One token of a seat whose own keys lo .. L - 1 are few: their pages (more than SEAT_PAGES are looked up from `tab` on), and the partial results that its content left
+constexpr int SEAT_PAGES = 6;
+struct SeatLast { int32_t tok, L, lo, tab, part, parts, page[SEAT_PAGES]; };
+static_assert(sizeof(SeatSpan) == 32 && sizeof(SeatItem) == 96 && sizeof(SeatLast) == 48, "written and read as 16-byte pieces");
 
-// A seat's own keys, few rows: one wave takes up to SEAT_SINGLE_TILES tiles by itself (no join of waves, four such items per workgroup); more are divided among the waves
-// of a workgroup, and from SEAT_WAVE_TILES on among workgroups.  Many rows, and contents, go to four waves of 32 rows each on shared tiles.
+// Who takes what, by a seat's rows (new tokens x query heads per key / value head) and the keys of its own that they see:
+//   a token of at most 8 heads on at most SEAT_LAST_KEYS keys      a wave, without LDS, that also joins what the content's pieces left
+//   up to SEAT_SHARED_ROWS rows on at most SEAT_SINGLE_TILES tiles  a wave to 32 rows
+//   up to 32 rows                                                   four waves that divide the tiles
+//   up to SEAT_SHARED_ROWS rows                                     four waves of 32 rows each on shared tiles
+//   more                                                            the same, over the content's keys and then its own: such a seat gains nothing by sharing its content's reading, and this way its
+//                                                                   results need no joining (150 tokens of 2 heads on 1,024 + 211 keys, 35 seats: 260 us with the content shared and all pieces joined)
+// The other seats' contents go to four waves of 32 rows each, or up to SEAT_WAVE_ROWS rows below one content to waves that divide the tiles.
+constexpr int SEAT_LAST_HEADS = 8, SEAT_LAST_KEYS = 128;
 constexpr int SEAT_SINGLE_TILES = 4;
 constexpr int SEAT_WAVE_ROWS = 64;
-constexpr int SEAT_WAVE_TILES = 16;
-constexpr int SEAT_BLOCK_TILES = 48;
-constexpr int SEAT_SHARED_TILES = 16;
+constexpr int SEAT_SHARED_ROWS = 96;
+// Keys are cut so that the items of a step fill the places that run at a time, and into pieces of no less than these; which piece size that is goes by all of a step's lengths.
+constexpr int SEAT_WAVE_TILES = 8, SEAT_BLOCK_TILES = 4;
+
+#if defined(__HIPCC__)
+#define SEATS_BOTH __host__ __device__ __forceinline__
+#else
+#define SEATS_BOTH inline
+#endif
 SEATS_BOTH int seats_least(int a, int b) { return a < b ? a : b; }
 SEATS_BOTH int seats_most(int a, int b) { return a > b ? a : b; }
 SEATS_BOTH int seats_up(int a, int b) { return (a + b - 1) / b; }
-// pieces of `tiles` tiles: as many as pieces of `size` would be begun, where `items` workgroups each leave places for that many
-SEATS_BOTH int seats_pieces(int tiles, int size, int places, int items) { return seats_most(1, seats_least(seats_up(tiles, size), places / seats_most(items, 1))); }
-SEATS_BOTH int seats_wave_pieces(int tiles, int d, int hkv, int blocks) { return seats_pieces(tiles, SEAT_WAVE_TILES, d >= 256 ? PAGED_PLACES / 2 : PAGED_PLACES, blocks * hkv * (d == 512 ? 2 : 1)); }
-SEATS_BOTH int seats_block_pieces(int tiles, int d, int hkv, int blocks, bool shared) {
-    return seats_pieces(tiles, shared ? SEAT_SHARED_TILES : SEAT_BLOCK_TILES, d == 512 ? PAGED_PLACES / 2 : PAGED_PLACES, blocks * hkv);
-}
+// workgroups that run at a time: of waves that divide the tiles (512 dims: two to an item), of waves on shared tiles
+SEATS_BOTH int seats_wave_places(int d) { return d == 512 ? PAGED_PLACES / 4 : d == 256 ? PAGED_PLACES / 2 : PAGED_PLACES; }
+SEATS_BOTH int seats_block_places(int d) { return d == 512 ? PAGED_PLACES / 2 : PAGED_PLACES; }

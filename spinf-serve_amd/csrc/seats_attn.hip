@@ -25,6 +25,7 @@
 #include "attn_tiles.h"
 #include "paged_dev.h"
 #include "paged_rows.h"
+#include "lanes.h"
 
 namespace {
 
@@ -35,36 +36,38 @@ struct Params {
     unsigned k_page, k_row, v_page, v_row; long k_head, v_head;   // bytes
     bool same;                                                    // keys and values have the same strides
     const int* lists; const int* first; const int* pos; const int* counts; const int* parts;
-    const SeatItem* wave; const SeatItem* single; const SeatItem* block;
+    const SeatItem* wave; const SeatItem* single; const SeatItem* block; const SeatLast* last;
     float* part_o; float2* part_ml;
     int hq, hkv, group, window, rows, seats;
-    int room[3];   // (the lists hold no more than they have room for, whatever their counts say)
+    int room[4];   // (the lists hold no more than they have room for, whatever their counts say)
     PageDiv page;
     Div by_group, by_heads;
     SoftCap cap;
 };
 
-__device__ __forceinline__ SeatItem load_item(const SeatItem* items, int i) {
-    SeatItem it;
+struct Item { int tok0, T, row0, piece, only; };
+struct Span { int tab, L, kt0, tiles, flo, fhi, own; };
+__device__ __forceinline__ Item load_item(const SeatItem* items, int i) {
     const int* p = (const int*)(items + i);
-    it.tok0 = sload(p, 0); it.T = sload(p, 1); it.L = sload(p, 2); it.tab = sload(p, 3);
-    it.row0 = sload(p, 4); it.kt0 = sload(p, 5); it.tiles = sload(p, 6); it.piece = sload(p, 7);
-    it.flo = sload(p, 8); it.fhi = sload(p, 9); it.flags = sload(p, 10);
-    return it;
+    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4)};
 }
-__device__ __forceinline__ bool is_masked(const SeatItem& it, int kt) { return kt * TK < it.flo || kt * TK + TK - 1 > it.fhi; }
+__device__ __forceinline__ Span load_span(const SeatItem* items, int i, int which) {
+    const int* p = (const int*)(items + i) + 8 + 8 * which;
+    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4), sload(p, 5), sload(p, 6)};
+}
+__device__ __forceinline__ bool is_masked(const Span& s, int kt) { return kt * TK < s.flo || kt * TK + TK - 1 > s.fhi; }
 
 // Where a tile lies: byte addresses of row 0 and row 16 of the key / value head's keys and values, and the tile's last stored row.  The pages are asked for a tile ahead.
 struct Pages {
     int n, row0, row1, id0, id1;
-    __device__ __forceinline__ void ask(const Params& p, const SeatItem& it, int kt) {
+    __device__ __forceinline__ void ask(const Params& p, const Span& s, int kt) {
         n = 2 * kt;
         const int a = p.page.of(n);
-        id0 = sload(p.lists, it.tab + a);
+        id0 = sload(p.lists, s.tab + a);
         row0 = (n - a * p.page.d) * 16;
         if (p.page.d & 1) {
-            const int end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, b = p.page.of(n1);
-            id1 = sload(p.lists, it.tab + b);
+            const int end = (s.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, b = p.page.of(n1);
+            id1 = sload(p.lists, s.tab + b);
             row1 = (n1 - b * p.page.d) * 16;
         }
     }
@@ -89,11 +92,10 @@ struct Place {
 };
 
 // the keys lo .. hi of the span that token t of the item's set sees
-__device__ __forceinline__ void interval(const Params& p, const SeatItem& it, int t, int& lo, int& hi) {
-    const bool own = it.flags & SEAT_OWN;
-    const int at = it.L - it.T + t;   // its own place (of a seat's own keys)
-    hi = own ? at : it.L - 1;
-    lo = p.window ? (own ? at : p.pos[it.tok0 + t]) - p.window + 1 : INT_MIN;
+__device__ __forceinline__ void interval(const Params& p, const Item& it, const Span& s, int t, int& lo, int& hi) {
+    const int at = s.L - it.T + t;   // its own place (of a seat's own keys)
+    hi = s.own ? at : s.L - 1;
+    lo = p.window ? (s.own ? at : p.pos[it.tok0 + t]) - p.window + 1 : INT_MIN;
 }
 
 // A wave's 32 rows, and the keys that they see
@@ -103,8 +105,12 @@ struct Rows : RowTile<D, DV, CAP> {
     using B::qf, B::lane, B::m, B::g, B::NS;
     int lo, hi;
 
+    __device__ __forceinline__ void see(const Params& p, const Item& it, const Span& s, int row0) {
+        const int N = it.T * p.group, row = row0 + (lane_now() & 31), r = row < N ? row : N - 1;
+        interval(p, it, s, p.by_group.of(r), lo, hi);
+    }
     // queries of rows row0 + m, dims col ..
-    __device__ __forceinline__ void load(const Params& p, const SeatItem& it, int kvh, int row0, int col = 0) {
+    __device__ __forceinline__ void load(const Params& p, const Item& it, const Span& s, int kvh, int row0, int col = 0) {
         lane = threadIdx.x & 63;
         m = lane & 31;
         g = lane >> 5;
@@ -113,7 +119,7 @@ struct Rows : RowTile<D, DV, CAP> {
         const __bf16* qp = p.q + (long)(it.tok0 + tok) * p.q_tok + (long)head * p.q_head + col + 8 * g;
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *(const bf16x8*)(qp + 16 * s);
-        interval(p, it, tok, lo, hi);
+        interval(p, it, s, tok, lo, hi);
         // (waited for here: left to the compiler, the wait would sit at the first use inside the tile loop, behind the DMAs in flight)
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 #pragma unroll
@@ -125,21 +131,21 @@ struct Rows : RowTile<D, DV, CAP> {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int x = key + 8 * (i >> 2) + (i & 3);
-            s[i] = (x >= lo) & (x <= hi) ? s[i] : -INFINITY;
+            s[i] = ((x >= lo) & (x <= hi)) ? s[i] : -INFINITY;
         }
     }
 };
 
-__device__ __forceinline__ void token_head(const Params& p, const SeatItem& it, int kvh, int row, int& tok, int& head) {
+__device__ __forceinline__ void token_head(const Params& p, const Item& it, int kvh, int row, int& tok, int& head) {
     const int t = p.by_group.of(row);
     tok = it.tok0 + t;
     head = kvh * p.group + (row - t * p.group);
 }
-__device__ __forceinline__ long part_of(const Params& p, const SeatItem& it, int tok, int head) { return (long)(p.parts[tok] + it.piece) * p.hq + head; }
+__device__ __forceinline__ long part_of(const Params& p, const Item& it, int tok, int head) { return (long)((p.parts[tok] & INT_MAX) + it.piece) * p.hq + head; }
 
 // Do masked tiles of an item hold values that are not finite?  A wave looks at tiles w, w + nw ..
 template <int DV>
-__device__ bool rubbish(const Params& p, const SeatItem& it, int kvh, int vcol, int w, int nw) {
+__device__ bool rubbish(const Params& p, const Span& it, int kvh, int vcol, int w, int nw) {
     constexpr int PIECES = DV / 8;
     const int lane = threadIdx.x & 63;
     bool found = false;
@@ -164,23 +170,26 @@ __device__ bool rubbish(const Params& p, const SeatItem& it, int kvh, int vcol, 
 // One row of an item by a whole wave, from memory, values touched only where the row sees the key.  state: the row's reference and sum as the tile loop found them: a
 // piece has one reference for all dims, also where the workgroup of the others does not come here (its values may be finite).
 template <int D, int DV, bool CAP>
-__device__ void slow_row(const Params& p, const SeatItem& it, int kvh, int j, int vcol, const float2 state) {
+__device__ void slow_row(const Params& p, const Item& it, const Span* spans, int n_spans, int kvh, int j, int vcol, const float2 state) {
     constexpr int VEC = DV / 64;   // output dims per lane
     const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
     int tok, head, lo, hi;
     token_head(p, it, kvh, it.row0 + j, tok, head);
-    interval(p, it, tok - it.tok0, lo, hi);
     const __bf16* q = p.q + (long)tok * p.q_tok + (long)head * p.q_head + g * (D / 2);
     const float ref = state.x == -INFINITY ? 0.f : state.x;
     float o[VEC];
 #pragma unroll
     for (int x = 0; x < VEC; x++) o[x] = 0.f;
 #pragma unroll 1
-    for (int i = 0; i < it.tiles; i++) {
-        const int kt = it.kt0 + i;
+    for (int x = 0; x < n_spans; x++) {
+    const Span& sp = spans[x];
+    interval(p, it, sp, tok - it.tok0, lo, hi);
+#pragma unroll 1
+    for (int i = 0; i < sp.tiles; i++) {
+        const int kt = sp.kt0 + i;
         Pages pages;
-        pages.ask(p, it, kt);
-        const Place pl(p, p.k + kvh * p.k_head, p.v + kvh * p.v_head, it.L, pages);
+        pages.ask(p, sp, kt);
+        const Place pl(p, p.k + kvh * p.k_head, p.v + kvh * p.v_head, sp.L, pages);
         const int r = m < pl.last ? m : pl.last;
         const bool vis = kt * TK + m >= lo && kt * TK + m <= hi;
         // lane (m, g): half g of the dims of key m
@@ -205,7 +214,8 @@ __device__ void slow_row(const Params& p, const SeatItem& it, int kvh, int j, in
             for (int x = 0; x < VEC; x++) o[x] = __builtin_fmaf(w, (float)vr[x], o[x]);
         }
     }
-    if (it.flags & SEAT_ONLY) {
+    }
+    if (it.only) {
         __bf16* dst = p.out + (long)tok * p.o_tok + (long)head * p.o_head + vcol + VEC * lane;
         const float inv = inverse(state.y);
 #pragma unroll
@@ -222,8 +232,8 @@ __device__ void slow_row(const Params& p, const SeatItem& it, int kvh, int j, in
 
 // eight dims of a row, as the last word or as a piece
 template <int D>
-__device__ __forceinline__ void put8(const Params& p, const SeatItem& it, int tok, int head, int d, const float (&x)[8]) {
-    if (it.flags & SEAT_ONLY) {
+__device__ __forceinline__ void put8(const Params& p, const Item& it, int tok, int head, int d, const float (&x)[8]) {
+    if (it.only) {
         bf16x8 y;
 #pragma unroll
         for (int k = 0; k < 8; k++) y[k] = (__bf16)x[k];
@@ -234,8 +244,8 @@ __device__ __forceinline__ void put8(const Params& p, const SeatItem& it, int to
         *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
 }
-__device__ __forceinline__ void put_sum(const Params& p, const SeatItem& it, int tok, int head, float M, float sum) {
-    if (!(it.flags & SEAT_ONLY)) p.part_ml[part_of(p, it, tok, head)] = make_float2(M, sum);
+__device__ __forceinline__ void put_sum(const Params& p, const Item& it, int tok, int head, float M, float sum) {
+    if (!(it.only)) p.part_ml[part_of(p, it, tok, head)] = make_float2(M, sum);
     else if (p.lse) p.lse[(long)tok * p.hq + head] = log_sum(M, sum);
 }
 
@@ -268,29 +278,31 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         const int x = single ? (unit - shared) * NW + w : unit;
         if (single && x >= alone) continue;   // (waves of these items meet nowhere: only the last unit of a workgroup's walk has idle ones)
         const int item = p.by_heads.of(x), kvh = x - item * p.hkv;
-        const SeatItem it = load_item(single ? p.single : p.wave, item);
+        const SeatItem* const list = single ? p.single : p.wave;
+        const Item it = load_item(list, item);
+        const Span span = load_span(list, item, 0);
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head + vcol * 2;
         const int step = single ? 1 : NW;
         R rows;
         bool seen_mask = false;
-        int kt = it.kt0 + (single ? 0 : w);
-        const int end = it.kt0 + it.tiles;
+        int kt = span.kt0 + (single ? 0 : w);
+        const int end = span.kt0 + span.tiles;
         {
             Pages pages;
             if (kt < end) {   // (the first tile is asked for ahead of the queries: their latencies pass together)
-                pages.ask(p, it, kt);
-                const Place pl(p, k_base, v_base, it.L, pages);
+                pages.ask(p, span, kt);
+                const Place pl(p, k_base, v_base, span.L, pages);
                 const int lane = lane_now();
                 fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, lane);
                 fetch<DV, NV, GV::VRS>(pl.v0, pl.v1, p.v_row, pl.last, 0, v_at, lane);
             }
-            rows.load(p, it, kvh, it.row0);
+            rows.load(p, it, span, kvh, it.row0);
             rows.reset();
             while (kt < end) {
-                const bool masked = is_masked(it, kt), next = kt + step < end;
+                const bool masked = is_masked(span, kt), next = kt + step < end;
                 seen_mask |= masked;
-                if (next) pages.ask(p, it, kt + step);
+                if (next) pages.ask(p, span, kt + step);
                 f32x16 s;
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(NV));   // the keys are there; the values may still be on their way
                 __builtin_amdgcn_sched_barrier(0);
@@ -299,7 +311,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
                 if (masked) rows.mask(kt, s);
                 __builtin_amdgcn_s_waitcnt(LGKM0);           // nothing reads the tile's keys any more
                 __builtin_amdgcn_sched_barrier(0);
-                const Place pl(p, k_base, v_base, it.L, pages);
+                const Place pl(p, k_base, v_base, span.L, pages);
                 if (next) fetch<D, NK, GK::KRS>(pl.k0, pl.k1, p.k_row, pl.last, 0, k_at, rows.lane);
                 bf16x8 pb[2];
                 rows.softmax(p.cap, s, pb);
@@ -319,14 +331,14 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         constexpr int PIECES = DV / 8;
         float* const stage = (float*)lds;
         if (single) {
-            if (seen_mask && rows.spoilt(left) && rubbish<DV>(p, it, kvh, vcol, 0, 1)) {
+            if (seen_mask && rows.spoilt(left) && rubbish<DV>(p, span, kvh, vcol, 0, 1)) {
                 for (int j = 0; j < here; j++) {
                     const float2 state = make_float2(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rows.M), j)), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), j)));
-                    slow_row<D, DV, CAP>(p, it, kvh, j, vcol, state);
+                    slow_row<D, DV, CAP>(p, it, &span, 1, kvh, j, vcol, state);
                 }
                 continue;
             }
-            const float f = it.flags & SEAT_ONLY ? inverse(sum) : 1.f;
+            const float f = it.only ? inverse(sum) : 1.f;
             float* const mine = (float*)kb;
             if (rows.m < left) {
 #pragma unroll
@@ -357,7 +369,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         }
         // ---- join the waves: every wave leaves its references and sums, then its accumulators scaled to the largest reference
         if (rows.g == 0) ml[w][rows.m] = make_float2(rows.M, sum);
-        const bool again = __syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, kvh, vcol, w, NW));
+        const bool again = __syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, span, kvh, vcol, w, NW));
         __syncthreads();   // (and every wave is done with its tiles)
         const auto joined = [&](int row) __attribute__((always_inline)) {   // a row's reference and sum
             float top = -INFINITY, total = 0.f;
@@ -369,13 +381,13 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             return make_float2(top, total);
         };
         if (again) {
-            for (int j = w; j < here; j += NW) slow_row<D, DV, CAP>(p, it, kvh, j, vcol, joined(j));
+            for (int j = w; j < here; j += NW) slow_row<D, DV, CAP>(p, it, &span, 1, kvh, j, vcol, joined(j));
             __syncthreads();
             continue;
         }
         const float2 state = joined(rows.m);
         const float ref = state.x == -INFINITY ? 0.f : state.x;
-        const float f = (rows.M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(rows.M - ref)) * (it.flags & SEAT_ONLY ? inverse(state.y) : 1.f);
+        const float f = (rows.M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(rows.M - ref)) * (it.only ? inverse(state.y) : 1.f);
         if (rows.m < left) {
 #pragma unroll
             for (int dt = 0; dt < R::NDT; dt++)
@@ -412,11 +424,13 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
 template <int SPAN>
 struct Halves { unsigned long long k[SPAN][2], v[SPAN][2]; };
 template <int SPAN>
-__device__ __forceinline__ void fill(Halves<SPAN>& h, const Params& p, const SeatItem& it, int from, const char* kb, const char* vb) {
+__device__ __forceinline__ void fill(Halves<SPAN>& h, const Params& p, const Span (&span)[2], int from, const char* kb, const char* vb) {
     const int t = threadIdx.x, i = from + t;
-    if (t < SPAN && i < it.tiles) {
-        const int n = 2 * (it.kt0 + i), end = (it.L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, a = p.page.of(n), b = p.page.of(n1);
-        const unsigned ia = p.lists[it.tab + a], ib = p.lists[it.tab + b], ra = (n - a * p.page.d) * 16, rb = (n1 - b * p.page.d) * 16;
+    if (t < SPAN && i < span[0].tiles + span[1].tiles) {
+        const bool second = i >= span[0].tiles;
+        const int kt = second ? span[1].kt0 + i - span[0].tiles : span[0].kt0 + i, L = second ? span[1].L : span[0].L, tab = second ? span[1].tab : span[0].tab;
+        const int n = 2 * kt, end = (L - 1) >> 4, n1 = n + 1 < end ? n + 1 : end, a = p.page.of(n), b = p.page.of(n1);
+        const unsigned ia = p.lists[tab + a], ib = p.lists[tab + b], ra = (n - a * p.page.d) * 16, rb = (n1 - b * p.page.d) * 16;
         h.k[t][0] = (unsigned long long)kb + (unsigned long long)ia * p.k_page + (unsigned long long)ra * p.k_row;
         h.k[t][1] = (unsigned long long)kb + (unsigned long long)ib * p.k_page + (unsigned long long)rb * p.k_row;
         h.v[t][0] = (unsigned long long)vb + (unsigned long long)ia * p.v_page + (unsigned long long)ra * p.v_row;
@@ -448,18 +462,20 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
-        const SeatItem it = load_item(p.block, item);
+        const Item it = load_item(p.block, item);
+        const Span span[2] = {load_span(p.block, item, 0), load_span(p.block, item, 1)};
+        const int tiles = span[0].tiles + span[1].tiles;
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head;
-        fill<SPAN>(at, p, it, 0, k_base, v_base);
+        fill<SPAN>(at, p, span, 0, k_base, v_base);
         R rows;
 
         // This lane's place in the regions that its wave copies: rows r + x (x < NK, NV) of the tile, which lie in one half of it
         const auto k_row = [&](int lane) { return w * NK + GK::NREG * (lane / GK::CPR); };
         const auto v_row = [&](int lane) { return w * NV + GV::NREG * (lane / GV::CPR); };
-        const auto issue = [&](int i, int kt, int buf) __attribute__((always_inline)) {
+        const auto issue = [&](int i, int last, int buf) __attribute__((always_inline)) {
             const unsigned to = base + buf * BUF;
-            const int lane = lane_now(), last = it.L - 1 - kt * TK;
+            const int lane = lane_now();
             if (last >= TK - 1) {
                 const char* ka = (const char*)at.k[i][k_row(lane) >> 4] + ((unsigned)(k_row(lane) & 15) * p.k_row + lane % GK::CPR * 16 + vcol * 2);
                 const char* va = (const char*)at.v[i][v_row(lane) >> 4] + ((unsigned)(v_row(lane) & 15) * p.v_row + lane % GV::CPR * 16 + vcol * 2);
@@ -483,20 +499,43 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
 
         bool seen_mask = false;
         __syncthreads();
-        if (it.tiles > 0) issue(0, it.kt0, 0);   // (ahead of the queries: their latencies pass together)
-        rows.load(p, it, kvh, it.row0 + 32 * w, vcol);
+        // keys of tile i behind its first one
+        const auto behind = [&](int i) __attribute__((always_inline)) { return i < span[0].tiles ? span[0].L - 1 - (span[0].kt0 + i) * TK : span[1].L - 1 - (span[1].kt0 + i - span[0].tiles) * TK; };
+        if (tiles > 0) issue(0, behind(0), 0);   // (ahead of the queries: their latencies pass together)
+        if (it.row0 + 32 * w >= it.T * p.group) {   // a wave without rows brings its share of the tiles
+            for (int i = 0, j = 0, buf = 0; i < tiles; i++, buf ^= 1) {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+                __syncthreads();
+                if (++j == SPAN) {
+                    j = 0;
+                    fill<SPAN>(at, p, span, i + 1, k_base, v_base);
+                    __syncthreads();
+                }
+                if (i + 1 < tiles) issue(j, behind(i + 1), buf ^ 1);
+                if (H == 2) {
+                    __syncthreads();
+                    __syncthreads();
+                }
+            }
+            if (__syncthreads_or(0)) __syncthreads_or(0);
+            __syncthreads();
+            continue;
+        }
+        rows.load(p, it, span[0], kvh, it.row0 + 32 * w, vcol);
         rows.reset();
-        for (int i = 0, j = 0, buf = 0; i < it.tiles; i++, buf ^= 1) {   // j: tile i's place among the halves
+        for (int i = 0, j = 0, buf = 0; i < tiles; i++, buf ^= 1) {   // j: tile i's place among the halves
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));   // this wave's share of the tile has landed
             __syncthreads();                            // ... and everybody's; the other buffer is free
             if (++j == SPAN) {                          // (the last tile of the span in hand has been requested)
                 j = 0;
-                fill<SPAN>(at, p, it, i + 1, k_base, v_base);
+                fill<SPAN>(at, p, span, i + 1, k_base, v_base);
                 __syncthreads();
             }
-            const int kt = it.kt0 + i;
-            if (i + 1 < it.tiles) issue(j, kt + 1, buf ^ 1);
-            const bool masked = is_masked(it, kt);
+            if (i + 1 < tiles) issue(j, behind(i + 1), buf ^ 1);
+            if (i == span[0].tiles) rows.see(p, it, span[1], it.row0 + 32 * w);   // (from here on it is the seat's own keys)
+            const bool second = i >= span[0].tiles;
+            const int kt = second ? span[1].kt0 + i - span[0].tiles : span[0].kt0 + i;
+            const bool masked = second ? is_masked(span[1], kt) : is_masked(span[0], kt);
             seen_mask |= masked;
             char* kb = lds + buf * BUF + half * HALF;
             f32x16 s;
@@ -524,20 +563,21 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
             rows.values(kb + GK::KTILEB, pb);
         }
         const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
+        const int live = seats_least(4, seats_up(left + 32 * w, 32));   // waves that have rows
         const float sum = lane32_sum(rows.l);
         if (sum == 0.f) rows.M = -INFINITY;   // no key seen
         // (also the barrier behind which the tile buffers are free)
-        if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, it, kvh, vcol, w, 4))) {
+        if (__syncthreads_or(seen_mask && rows.spoilt(left)) && __syncthreads_or(rubbish<DV>(p, span[0], kvh, vcol, w, live) | rubbish<DV>(p, span[1], kvh, vcol, w, live))) {
             for (int j = 0; j < 32 && j < left; j++) {
                 const float2 state = make_float2(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rows.M), j)), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum), j)));
-                slow_row<D, DV, CAP>(p, it, kvh, 32 * w + j, vcol, state);
+                slow_row<D, DV, CAP>(p, it, span, 2, kvh, 32 * w + j, vcol, state);
             }
             __syncthreads();
             continue;
         }
-        const float f = it.flags & SEAT_ONLY ? inverse(sum) : 1.f;
+        const float f = it.only ? inverse(sum) : 1.f;
         const int lane = lane_now(), m = lane & 31, g = lane >> 5;
-        if (it.flags & SEAT_ONLY) {   // rows through the wave's own slice of LDS, stored as 16-byte pieces
+        if (it.only) {   // rows through the wave's own slice of LDS, stored as 16-byte pieces
             char* const stage = lds + wave * 32 * OROW;
 #pragma unroll
             for (int dt = 0; dt < R::NDT; dt++)
@@ -579,6 +619,129 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     }
 }
 
+// ------------------------------------------------------------------------------------------------ one token on few keys of its own: the last word
+// A wave per (seat, key / value head), D / 8 lanes to a key, its dot products in the vector unit: as few keys as these would leave the matrix unit's tiles mostly empty, and without LDS
+// four times as many waves run at a time, which is what hides the latency of so little (10,752 items of some nine keys of 256 dims: 95 us as tiles).
+// Probabilities stay 32-bit.  Then the pieces that the content's items left are added, and the row is written.
+template <int D, int RM, bool CAP>
+__global__ __launch_bounds__(256) void seats_last_kernel(const Params p) {
+    constexpr int LPK = D / 8, G = 64 / LPK, U = 8;   // lanes of a key, keys of a load, loads ahead
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, mine = lane / LPK, col = lane % LPK * 8;
+    const int units = seats_least(sload(p.counts, 3), p.room[3]) * p.hkv;
+    for (int unit = blockIdx.x * 4 + w; unit < units; unit += gridDim.x * 4) {
+        const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
+        const int* ip = (const int*)(p.last + item);
+        const int tok = sload(ip, 0), L = sload(ip, 1), lo = sload(ip, 2), tab = sload(ip, 3), part = sload(ip, 4), parts = sload(ip, 5);
+        const int page[SEAT_PAGES] = {sload(ip, 6), sload(ip, 7), sload(ip, 8), sload(ip, 9), sload(ip, 10), sload(ip, 11)};
+        const int n = L - lo, page0 = p.page.of(lo >> 4), many = p.page.of((L - 1) >> 4) - page0 + 1;
+        const char* const kb = p.k + kvh * p.k_head + col * 2;
+        const char* const vb = p.v + kvh * p.v_head + col * 2;
+        bf16x8 q[RM];
+#pragma unroll
+        for (int r = 0; r < RM; r++) q[r] = *(const bf16x8*)(p.q + (long)tok * p.q_tok + (long)(kvh * p.group + (r < p.group ? r : p.group - 1)) * p.q_head + col);
+        float M[RM], l[RM], o[RM][8];
+#pragma unroll
+        for (int r = 0; r < RM; r++) {
+            M[r] = -INFINITY;
+            l[r] = 0.f;
+#pragma unroll
+            for (int d = 0; d < 8; d++) o[r][d] = 0.f;
+        }
+        for (int k0 = 0; k0 < n; k0 += U * G) {
+            bf16x8 kx[U], vx[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (k0 + u * G >= n) break;
+                const int j = k0 + u * G + mine, key = lo + (j < n ? j : n - 1);   // (behind the last key: that one again)
+                const int a = p.page.of(key >> 4), x = a - page0;
+                int id = page[0];
+                if (many <= SEAT_PAGES) {
+#pragma unroll
+                    for (int y = 1; y < SEAT_PAGES; y++) id = x == y ? page[y] : id;
+                } else id = p.lists[tab + a];
+                const unsigned row = key - a * p.page.d * 16;
+                kx[u] = *(const bf16x8*)(kb + (unsigned long long)(unsigned)id * p.k_page + (unsigned long long)row * p.k_row);
+                vx[u] = *(const bf16x8*)(vb + (unsigned long long)(unsigned)id * p.v_page + (unsigned long long)row * p.v_row);
+            }
+            float s[U][RM];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int r = 0; r < RM; r++) {
+                    s[u][r] = -INFINITY;
+                    if (k0 + u * G < n) {
+                        float x = 0.f;
+#pragma unroll
+                        for (int d = 0; d < 8; d++) x = __builtin_fmaf((float)q[r][d], (float)kx[u][d], x);
+                        x = over_lanes<LPK>(x, [](float a, float b) { return a + b; });
+                        if (CAP) x = p.cap.of(x);
+                        s[u][r] = k0 + u * G + mine < n ? x * p.cap.unit : -INFINITY;
+                    }
+                }
+#pragma unroll
+            for (int r = 0; r < RM; r++) {
+                float top = M[r];
+#pragma unroll
+                for (int u = 0; u < U; u++) top = fmaxf(top, s[u][r]);
+                const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(M[r] - ref);
+                M[r] = top;
+                l[r] *= f;
+#pragma unroll
+                for (int d = 0; d < 8; d++) o[r][d] *= f;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (k0 + u * G >= n) break;
+                    const float y = __builtin_amdgcn_exp2f(s[u][r] - ref);
+                    l[r] += y;
+                    if (k0 + u * G + mine < n) {
+#pragma unroll
+                        for (int d = 0; d < 8; d++) o[r][d] = __builtin_fmaf(y, (float)vx[u][d], o[r][d]);
+                    }
+                }
+            }
+        }
+        // (rescaled to each other: nothing seen weighs nothing, and leaves NaN where it is)
+        const auto add = [&](int r, float m, float sum, const float (&x)[8]) __attribute__((always_inline)) {
+            const float top = fmaxf(M[r], m), ref = top == -INFINITY ? 0.f : top;
+            const float f = M[r] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M[r] - ref), g = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);
+            M[r] = top;
+            l[r] = f * l[r] + g * sum;
+#pragma unroll
+            for (int d = 0; d < 8; d++) o[r][d] = f * o[r][d] + g * x[d];
+        };
+        for (int s = mine; s < parts; s += G)
+#pragma unroll
+            for (int r = 0; r < RM; r++) {
+                const long at = (long)(part + s) * p.hq + kvh * p.group + (r < p.group ? r : p.group - 1);
+                const float4 a = *(const float4*)(p.part_o + at * D + col), b = *(const float4*)(p.part_o + at * D + col + 4);
+                const float2 ml = p.part_ml[at];
+                const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                add(r, ml.x, ml.y, x);
+            }
+#pragma unroll
+        for (int d = LPK; d < 64; d <<= 1)
+#pragma unroll
+            for (int r = 0; r < RM; r++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = __shfl_xor(o[r][i], d);
+                const float m = __shfl_xor(M[r], d), sum = __shfl_xor(l[r], d);
+                add(r, m, sum, x);
+            }
+#pragma unroll
+        for (int r = 0; r < RM; r++)
+            if (mine == 0 && r < p.group) {
+                const float f = inverse(l[r]);
+                bf16x8 y;
+#pragma unroll
+                for (int d = 0; d < 8; d++) y[d] = (__bf16)(o[r][d] * f);
+                *(bf16x8*)(p.out + (long)tok * p.o_tok + (long)(kvh * p.group + r) * p.o_head + col) = y;
+                if (p.lse && lane == 0) p.lse[(long)tok * p.hq + kvh * p.group + r] = log_sum(M[r], l[r]);
+            }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ pieces joined
 // out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per token and 64 dims of its heads (or some of them: blockIdx.y); 16 lanes hold a piece of
 // a head, `share` such groups take a head's pieces in turn, each with a reference of its own, and are added up in one fixed order.
@@ -588,10 +751,10 @@ __global__ __launch_bounds__(256) void seats_join_kernel(const Params p) {
     __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
     __shared__ float2 part_ml[GROUPS];
     const int tok = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
-    const int first = sload(p.parts, tok), n = sload(p.parts, tok + 1) - first;
+    const int begin = sload(p.parts, tok), first = begin & INT_MAX, n = begin < 0 ? 0 : (sload(p.parts, tok + 1) & INT_MAX) - first;
     const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
     if (n == 0) {
-        if (tok < sload(p.first, p.seats)) return;   // its only piece is the last word
+        if (tok < sload(p.first, p.seats)) return;   // the last word is spoken
         for (int h = blockIdx.y * GROUPS + group; h < p.hq; h += gridDim.y * GROUPS) {
             *(uint2*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = make_uint2(0, 0);
             if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = -INFINITY;
@@ -674,11 +837,21 @@ constexpr int AT_ONCE = 2048;   // workgroups of a launch that walk a list
 template <int D, int DV, int NW, bool CAP>
 int launch(const Params& p, const spinf_seats_attn_args* a, hipStream_t s) {
     const auto grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>(n, AT_ONCE)); };
-    hipLaunchKernelGGL((seats_block_kernel<D, DV, CAP>), grid(a->rooms[2] * p.hkv), dim3(256 * (D / DV)), 0, s, p);
-    hipError_t e = hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (a->rooms[2]) {
+        hipLaunchKernelGGL((seats_block_kernel<D, DV, CAP>), grid(a->rooms[2] * p.hkv), dim3(256 * (D / DV)), 0, s, p);
+        e = hipGetLastError();
+    }
     if (e == hipSuccess) {
         const int64_t units = a->rooms[0] * p.hkv + (a->rooms[1] * p.hkv + NW - 1) / NW;
         hipLaunchKernelGGL((seats_wave_kernel<D, DV, NW, CAP>), grid(DV < D ? (units + 7) / 8 * 16 : units), dim3(64 * NW), 0, s, p);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && a->rooms[3]) {   // (behind the contents' pieces, which it joins)
+        const dim3 n((unsigned)std::min<int64_t>((a->rooms[3] * p.hkv + 3) / 4, 2 * AT_ONCE));
+        if (p.group <= 2) hipLaunchKernelGGL((seats_last_kernel<D, 2, CAP>), n, dim3(256), 0, s, p);
+        else if (p.group <= 4) hipLaunchKernelGGL((seats_last_kernel<D, 4, CAP>), n, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((seats_last_kernel<D, 8, CAP>), n, dim3(256), 0, s, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
@@ -705,17 +878,17 @@ extern "C" int spinf_seats_attn_fwd(const spinf_seats_attn_args* a, void* stream
     if (kd.window < 0) return spinf_fail(SPINF_E_ARG, "seats_attn: window %d", kd.window);
     if (!(a->scale > 0.f) || !(a->scale < INFINITY) || !(a->softcap >= 0.f) || !(a->softcap < INFINITY))
         return spinf_fail(SPINF_E_ARG, "seats_attn: scale %g must be positive and finite, softcap %g not negative", (double)a->scale, (double)a->softcap);
-    if (!a->q || !a->out || !a->k || !a->v || !a->lists || !a->first || !a->pos || !kd.wave || !kd.single || !kd.block || !kd.counts || !kd.parts)
+    if (!a->q || !a->out || !a->k || !a->v || !a->lists || !a->first || !a->pos || !kd.wave || !kd.single || !kd.block || !kd.last || !kd.counts || !kd.parts)
         return spinf_fail(SPINF_E_ARG, "seats_attn: null pointer");
-    for (const void* ptr : {a->q, (const void*)a->out, a->k, a->v, (const void*)kd.wave, (const void*)kd.single, (const void*)kd.block})
+    for (const void* ptr : {a->q, (const void*)a->out, a->k, a->v, (const void*)kd.wave, (const void*)kd.single, (const void*)kd.block, (const void*)kd.last})
         if ((uintptr_t)ptr % 16) return spinf_fail(SPINF_E_ARG, "seats_attn: tensors and lists must be 16-byte aligned");
     for (int64_t st : {a->q_tok, a->q_head, a->o_tok, a->o_head, a->k_page, a->k_row, a->k_head, a->v_page, a->v_row, a->v_head})
         if (st % 8) return spinf_fail(SPINF_E_ARG, "seats_attn: strides must be multiples of 8 elements");
     if (a->k_row < 0 || a->v_row < 0 || a->k_row > (1 << 24) || a->v_row > (1 << 24) || a->k_page < 0 || a->v_page < 0 || a->k_page > (1u << 30) || a->v_page > (1u << 30))
         return spinf_fail(SPINF_E_ARG, "seats_attn: strides of the cache must lie in 0 .. 2^24 elements (rows) and 0 .. 2^30 (pages)");   // (32-bit byte counts; 32 rows by 32-bit offsets)
-    for (int i = 0; i < 4; i++)
-        if (a->rooms[i] < (i < 3) || a->rooms[i] > (1 << 30) || (i < 3 && a->rooms[i] * kd.hkv > (1 << 30))) return spinf_fail(SPINF_E_ARG, "seats_attn: bad lengths of lists");
-    const int64_t parts = a->rooms[3] * kd.hq, need = parts * (kd.d + 2) * 4;
+    for (int i = 0; i < 5; i++)
+        if (a->rooms[i] < (i < 2) || a->rooms[i] > (1 << 26) || (i < 4 && a->rooms[i] * kd.hkv > (1 << 30))) return spinf_fail(SPINF_E_ARG, "seats_attn: bad lengths of lists");
+    const int64_t parts = a->rooms[4] * kd.hq, need = parts * (kd.d + 2) * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
         return spinf_fail(SPINF_E_ARG, "seats_attn: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
     Params p = {};
@@ -726,12 +899,12 @@ extern "C" int spinf_seats_attn_fwd(const spinf_seats_attn_args* a, void* stream
     p.v_page = (unsigned)(2 * a->v_page); p.v_row = (unsigned)(2 * a->v_row); p.v_head = 2 * a->v_head;
     p.same = a->k_page == a->v_page && a->k_row == a->v_row;
     p.lists = a->lists; p.first = a->first; p.pos = a->pos; p.counts = kd.counts; p.parts = kd.parts;
-    p.wave = (const SeatItem*)kd.wave; p.single = (const SeatItem*)kd.single; p.block = (const SeatItem*)kd.block;
+    p.wave = (const SeatItem*)kd.wave; p.single = (const SeatItem*)kd.single; p.block = (const SeatItem*)kd.block; p.last = (const SeatLast*)kd.last;
     p.part_o = (float*)a->workspace;
     p.part_ml = (float2*)(p.part_o + parts * kd.d);
     p.hq = kd.hq; p.hkv = kd.hkv; p.group = kd.hq / kd.hkv; p.rows = (int)a->rows; p.seats = a->seats;
     p.window = kd.window < 1 << 30 ? kd.window : 1 << 30;
-    for (int i = 0; i < 3; i++) p.room[i] = (int)a->rooms[i];
+    for (int i = 0; i < 4; i++) p.room[i] = (int)a->rooms[i];
     p.page = PageDiv::of_page(a->page);
     p.by_group = Div::by(p.group);
     p.by_heads = Div::by(p.hkv);

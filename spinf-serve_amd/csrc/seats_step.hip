@@ -22,7 +22,7 @@ namespace {
 constexpr int LANES = 1024, WAVES = LANES / 64;
 constexpr int LOTS = 1 << 30;   // sums stop there
 
-struct Kind { int* wave; int* single; int* block; int* counts; int* parts; int* seat_parts; int hq, hkv, d, window, wave_room, single_room, block_room; };
+struct Kind { int* wave; int* single; int* block; int* last; int* counts; int* parts; int* seat_parts; int hq, hkv, d, window, room[4]; };
 struct Params {
     const int* come; const int* drop; const int* content;
     int* lens; int* table; int* free; int* left; int* first; int* took; int* stay;
@@ -39,17 +39,17 @@ __device__ __forceinline__ int add(int a, int b) {   // of numbers in 0 .. LOTS
 __device__ __forceinline__ int most(int a, int b) { return a > b ? a : b; }
 
 // Running sums over the workgroup: N values per lane -> what the lanes before hold in all, and the total
-template <int N, class F>
-__device__ __forceinline__ void scan(int (&x)[N], int (&total)[N], int (*room)[WAVES], int none, F f) {
+template <int N, class T, class F>
+__device__ __forceinline__ void scan(T (&x)[N], T (&total)[N], long (*room)[WAVES], T none, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int y[N];
+    T y[N];
 #pragma unroll
     for (int i = 0; i < N; i++) y[i] = x[i];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1)
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int z = __shfl_up(y[i], d);
+            const T z = __shfl_up(y[i], d);
             if (lane >= d) y[i] = f(z, y[i]);
         }
     __syncthreads();   // (the room is free)
@@ -59,12 +59,13 @@ __device__ __forceinline__ void scan(int (&x)[N], int (&total)[N], int (*room)[W
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        int before = none, all = none;
+        T before = none, all = none;
+#pragma unroll
         for (int w = 0; w < WAVES; w++) {
             if (w == wave) before = all;
-            all = f(all, room[i][w]);
+            all = f(all, (T)room[i][w]);
         }
-        const int z = __shfl_up(y[i], 1);
+        const T z = __shfl_up(y[i], 1);
         x[i] = lane ? f(before, z) : before;
         total[i] = all;
     }
@@ -81,10 +82,15 @@ __device__ __forceinline__ int find(const int* sums, int n, int i) {
 }
 
 __device__ __forceinline__ void store(int* items, int at, const SeatItem& it) {
-    int4* p = (int4*)(items + 12 * (long)at);
-    p[0] = make_int4(it.tok0, it.T, it.L, it.tab);
-    p[1] = make_int4(it.row0, it.kt0, it.tiles, it.piece);
-    p[2] = make_int4(it.flo, it.fhi, it.flags, 0);
+    int4* p = (int4*)(items + sizeof(SeatItem) / 4 * (long)at);
+    p[0] = make_int4(it.tok0, it.T, it.row0, it.piece);
+    p[1] = make_int4(it.only, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const SeatSpan& s = it.span[i];
+        p[2 + 2 * i] = make_int4(s.tab, s.L, s.kt0, s.tiles);
+        p[3 + 2 * i] = make_int4(s.flo, s.fhi, s.own, 0);
+    }
 }
 
 // Places and positions of rows, and where their partial results begin
@@ -101,7 +107,8 @@ __device__ __forceinline__ void place_row(const Params& p, int row, int total, i
     p.pos[row] = pos;
     for (int k = 0; k < p.kinds; k++) {
         const int* sp = p.kind[k].seat_parts;
-        p.kind[k].parts[row] = row < total ? sp[2 * seat] + (row - first) * sp[2 * seat + 1] : sp[2 * p.seats];
+        const int base = sp[2 * (row < total ? seat : p.seats)];   // (the sign: no piece is left to be joined)
+        p.kind[k].parts[row] = row < total ? ((base & INT_MAX) + (row - first) * sp[2 * seat + 1]) | (base & INT_MIN) : base;
         if (row == p.rows - 1) p.kind[k].parts[p.rows] = sp[2 * p.seats];
     }
 }
@@ -117,10 +124,11 @@ __global__ __launch_bounds__(256) void seats_rows_kernel(const Params p) {
 template <int SPT>   // seats per lane
 __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
     constexpr int MOST = SPT * LANES;
-    __shared__ int room[4][WAVES];
+    __shared__ long room[6][WAVES];
     __shared__ int stay[MOST], took[MOST], content[MOST], first[MOST + 1];
-    __shared__ int sums[3][MOST + 1];
-    __shared__ int heads[MOST + 1], low[MOST], high[MOST], of_group[MOST], cut[MOST];   // by group of seats in a row below one content; cut: pieces of the content's keys
+    __shared__ int sums[4][MOST + 1];
+    __shared__ int heads[MOST + 1], low[MOST], high[MOST], of_group[MOST], cut[MOST];   // by group of seats in a row that share their content; cut: pieces of its keys
+    __shared__ int best[2];
     const int R = p.seats, tid = threadIdx.x;
     const auto plus = [](int a, int b) __attribute__((always_inline)) { return add(a, b); };
     const auto larger = [](int a, int b) __attribute__((always_inline)) { return most(a, b); };
@@ -212,163 +220,277 @@ __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
         p.table[p.table_at + (long)r * p.width + pages(stay[r]) + i - sums[1][r]] = p.free[left - 1 - i];
     }
 
-    // ---- groups: seats with new tokens, one after the other below the same content (seats without any in between do not part them)
-    int last[1] = {-1}, none[1];
+    // ---- the last seat with new tokens ahead of each
+    int last[1] = {-1}, whole[1];
 #pragma unroll
     for (int i = 0; i < SPT; i++) {
         const int r = tid * SPT + i;
         if (r < R && want[i]) last[0] = r;
     }
-    scan(last, none, room, -1, larger);
-    int head[1] = {0}, groups[1];
-    bool begins[SPT];
-#pragma unroll
-    for (int i = 0; i < SPT; i++) {
-        const int r = tid * SPT + i;
-        begins[i] = r < R && want[i] && (last[0] < 0 || content[last[0]] != content[r]);
-        head[0] += begins[i];
-        if (r < R && want[i]) last[0] = r;
-    }
-    scan(head, groups, room, 0, plus);
-    const int G = groups[0];
-#pragma unroll
-    for (int i = 0; i < SPT; i++) {
-        const int r = tid * SPT + i;
-        if (r < R) {
-            if (begins[i]) {
-                heads[head[0]] = r;
-                low[head[0]] = INT_MAX;
-                high[head[0]] = 0;
-            }
-            head[0] += begins[i];
-            of_group[r] = head[0] - 1;   // (means something only where the seat has new tokens)
-        }
-    }
-    if (tid == 0) heads[G] = R;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < SPT; i++) {   // the least and the largest place among the seats' own keys of a group's new tokens
-        const int r = tid * SPT + i;
-        if (want[i]) {
-            atomicMin(&low[of_group[r]], here[i]);
-            atomicMax(&high[of_group[r]], here[i] + want[i] - 1);
-        }
-    }
+    scan(last, whole, room, -1, larger);
 
     // ---- the lists of every head geometry
     for (int k = 0; k < p.kinds; k++) {
         const Kind& kd = p.kind[k];
         const int group = kd.hq / kd.hkv, W = kd.window;
         const int far = W ? W : LOTS;
+        const auto alone = [&](int r) __attribute__((always_inline)) { return took[r] * group > SEAT_SHARED_ROWS; };   // (such a seat reads its content for itself)
         __syncthreads();
-        // contents: sums[0] over groups
-        int n0[1] = {0}, all0[1];
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int g = tid * SPT + i;
-            if (g < G) {
-                const int r = heads[g], c = content[r];
-                int pieces = 0, count = 0;
-                if (c >= 0) {
-                    const int P = p.shared[3 * c], T = first[heads[g + 1]] - first[r], blocks = seats_up(T * group, 128);
-                    const int lo = most(0, P + low[g] - far + 1), tiles = lo < P ? seats_up(P, PAGED_TILE) - lo / PAGED_TILE : 0;
-                    if (tiles > 0) {
-                        pieces = seats_block_pieces(tiles, kd.d, kd.hkv, blocks, true);
-                        count = pieces * blocks;
-                    }
-                }
-                cut[g] = pieces;
-                n0[0] += count;
-                sums[0][g] = count;
-            }
-        }
-        scan(n0, all0, room, 0, plus);
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int g = tid * SPT + i;
-            if (g < G) {
-                const int count = sums[0][g];
-                sums[0][g] = n0[0];
-                n0[0] += count;
-            }
-        }
-        if (tid == 0) sums[0][G] = all0[0];
-        __syncthreads();
-        for (int i = tid; i < all0[0]; i += LANES) {
-            const int g = find(sums[0], G, i), r = heads[g], c = content[r], j = i - sums[0][g];
-            const int P = p.shared[3 * c], tok0 = first[r], T = first[heads[g + 1]] - tok0, blocks = seats_up(T * group, 128);
-            const int lo = most(0, P + low[g] - far + 1), kt = lo / PAGED_TILE, tiles = seats_up(P, PAGED_TILE) - kt;
-            const int s = j / blocks, b = j - s * blocks, n = cut[g];
-            const int from = (int)((long)tiles * s / n), to = (int)((long)tiles * (s + 1) / n);
-            if (i < kd.block_room)
-                store(kd.block, i, {tok0, T, P, p.shared[3 * c + 2], 128 * b, kt + from, to - from, s, most(0, P + high[g] - far + 1), P - 1, 0, 0});
-        }
-        // seats: how many items of each sort, and partial results
-        __syncthreads();
-        int n1[4] = {0, 0, 0, 0}, all1[4];
-        int c1[SPT][3], parts[SPT];
-        const auto plan = [&](int r, int n, int& blocks, int& tiles, int& sort, int& pieces) __attribute__((always_inline)) {
-            const int rows = n * group, L = stay[r] + n, lo = most(0, stay[r] - far + 1);
-            tiles = seats_up(L, PAGED_TILE) - lo / PAGED_TILE;
-            const bool few = rows <= SEAT_WAVE_ROWS;
-            blocks = seats_up(rows, few ? 32 : 128);
-            sort = !few ? 2 : tiles <= SEAT_SINGLE_TILES ? 1 : 0;
-            pieces = sort == 0 ? seats_wave_pieces(tiles, kd.d, kd.hkv, blocks) : sort == 1 ? 1 : seats_block_pieces(tiles, kd.d, kd.hkv, blocks, false);
-        };
+        // groups: seats that share a content, one after the other (seats without new tokens do not part them)
+        int head[1] = {0}, groups[1], ahead = last[0];
+        bool begins[SPT];
 #pragma unroll
         for (int i = 0; i < SPT; i++) {
             const int r = tid * SPT + i;
-            c1[i][0] = c1[i][1] = c1[i][2] = parts[i] = 0;
-            if (want[i]) {
-                int blocks, tiles, sort, pieces;
-                plan(r, want[i], blocks, tiles, sort, pieces);
-                c1[i][sort] = blocks * pieces;
-                parts[i] = cut[of_group[r]] + pieces;
-            }
-#pragma unroll
-            for (int x = 0; x < 3; x++) n1[x] += c1[i][x];
-            n1[3] = add(n1[3], parts[i] > 1 ? want[i] * parts[i] : 0);
+            begins[i] = r < R && want[i] && (ahead < 0 || content[ahead] != content[r] || alone(r) || alone(ahead));
+            head[0] += begins[i];
+            if (r < R && want[i]) ahead = r;
         }
-        scan(n1, all1, room, 0, plus);
+        scan(head, groups, room, 0, plus);
+        const int G = groups[0];
 #pragma unroll
         for (int i = 0; i < SPT; i++) {
             const int r = tid * SPT + i;
             if (r < R) {
-#pragma unroll
-                for (int x = 0; x < 3; x++) {
-                    sums[x][r] = n1[x];
-                    n1[x] += c1[i][x];
+                if (begins[i]) {
+                    heads[head[0]] = r;
+                    low[head[0]] = INT_MAX;
+                    high[head[0]] = 0;
                 }
-                kd.seat_parts[2 * r] = n1[3];
-                kd.seat_parts[2 * r + 1] = parts[i] > 1 ? parts[i] : 0;
-                n1[3] = add(n1[3], parts[i] > 1 ? want[i] * parts[i] : 0);
+                head[0] += begins[i];
+                of_group[r] = head[0] - 1;   // (means something only where the seat has new tokens)
+            }
+        }
+        if (tid == 0) heads[G] = R;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {   // the least and the largest place among the seats' own keys of a group's new tokens
+            const int r = tid * SPT + i;
+            if (want[i]) {
+                atomicMin(&low[of_group[r]], here[i]);
+                atomicMax(&high[of_group[r]], here[i] + want[i] - 1);
+            }
+        }
+        __syncthreads();
+        // what there is to do: sets of rows (blocks) on tiles; a group's content in the first half, a seat's own keys in the second
+        const auto group_set = [&](int g, int& blocks, int& tiles) __attribute__((always_inline)) {   // -> waves divide the tiles
+            const int r = heads[g], c = content[r];
+            blocks = tiles = 0;
+            if (c < 0 || alone(r)) return false;
+            const int P = p.shared[3 * c], rows = (first[heads[g + 1]] - first[r]) * group;
+            const int lo = most(0, P + low[g] - far + 1);
+            const bool few = rows <= SEAT_WAVE_ROWS;
+            if (lo < P) {
+                tiles = seats_up(P, PAGED_TILE) - lo / PAGED_TILE;
+                blocks = seats_up(rows, few ? 32 : 128);
+            }
+            return few;
+        };
+        // sorts: 0 waves that divide the tiles, 1 a wave to 32 rows, 2 shared tiles, 3 the last word; shared: its content's tiles, where it reads them itself
+        const auto seat_set = [&](int r, int& blocks, int& tiles, int& shared) __attribute__((always_inline)) {
+            const int n = took[r], rows = n * group, L = stay[r] + n, lo = most(0, stay[r] - far + 1);
+            tiles = seats_up(L, PAGED_TILE) - lo / PAGED_TILE;
+            shared = 0;
+            if (n == 1 && group <= SEAT_LAST_HEADS && L - lo <= SEAT_LAST_KEYS) {
+                blocks = 1;
+                return 3;
+            }
+            if (alone(r)) {
+                const int c = content[r], P = c >= 0 ? p.shared[3 * c] : 0, from = most(0, P + stay[r] - far + 1);
+                shared = from < P ? seats_up(P, PAGED_TILE) - from / PAGED_TILE : 0;
+                blocks = seats_up(rows, 128);
+                return 2;
+            }
+            const int sort = tiles <= SEAT_SINGLE_TILES ? 1 : rows <= 32 ? 0 : 2;
+            blocks = seats_up(rows, sort == 2 ? 128 : 32);
+            return sort;
+        };
+        int set[SPT][2][2], sort[SPT][2];   // blocks, tiles; sort (-1: nothing): of group i and of seat i
+        long work[2] = {0, 0}, all_work[2];   // by waves that divide the tiles, on shared tiles
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int r = tid * SPT + i;
+            sort[i][0] = sort[i][1] = -1;
+            if (r < G) {
+                const bool few = group_set(r, set[i][0][0], set[i][0][1]);
+                if (set[i][0][0]) sort[i][0] = few ? 0 : 2;
+            }
+            if (want[i]) {
+                int shared;
+                sort[i][1] = seat_set(r, set[i][1][0], set[i][1][1], shared);
+                set[i][1][1] += shared;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+            {
+                const long n = (long)set[i][x][0] * set[i][x][1];
+                work[0] += sort[i][x] == 0 ? n : 0;
+                work[1] += sort[i][x] == 2 ? n : 0;
+            }
+        }
+        scan(work, all_work, room, 0l, [](long a, long b) { return a + b; });
+        // Tiles of a piece: of some sizes at and above those that make as many pieces as there are places, the one whose rounds of workgroups end first
+        constexpr int SIZES = 6;
+        int size[2][SIZES], items[2][SIZES] = {}, all_items[SIZES];
+        const int places[2] = {seats_wave_places(kd.d), seats_block_places(kd.d)};
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int j = 0; j < SIZES; j++) {
+                const long tiles = (all_work[x] * kd.hkv * (8 + j * (j + 1) / 2) / 8 + places[x] - 1) / places[x];   // 1, 1 1/8, 1 3/8, 1 3/4, 2 1/4, 2 7/8
+                size[x][j] = most(x ? SEAT_BLOCK_TILES : SEAT_WAVE_TILES, (int)(tiles < LOTS ? tiles : LOTS));
+            }
+#pragma unroll
+        for (int i = 0; i < SPT; i++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+                    if (sort[i][x] == 2 * y)
+#pragma unroll
+                        for (int j = 0; j < SIZES; j++) items[y][j] += set[i][x][0] * seats_up(set[i][x][1], size[y][j]);
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            if (all_work[y] == 0) continue;
+            scan(items[y], all_items, room, 0, plus);
+            if (tid == 0) {
+                long cost = LONG_MAX;
+#pragma unroll
+                for (int j = 0; j < SIZES; j++) {
+                    const long rounds = ((long)all_items[j] * kd.hkv + places[y] - 1) / places[y];
+                    const long here = rounds * (size[y][j] + (y ? 4 : 12));   // (a workgroup's start and end are worth some tiles)
+                    if (here < cost) {
+                        cost = here;
+                        best[y] = size[y][j];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const int by_wave = best[0], by_block = best[1];
+        // how many items of each sort, where each set's begin, partial results of each seat
+        int n1[4] = {0, 0, 0, 0}, all1[4];   // sort 0, 1, 3; sort 2: groups, then seats, as one sum each
+        int g0[2] = {0, 0}, all0[2];
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int g = tid * SPT + i;
+            if (g < G) {
+                const int y = sort[i][0], n = y < 0 ? 0 : seats_up(set[i][0][1], y ? by_block : by_wave);
+                cut[g] = n;
+                g0[0] += y == 0 ? n * set[i][0][0] : 0;
+                g0[1] += y == 2 ? n * set[i][0][0] : 0;
+            }
+        }
+        scan(g0, all0, room, 0, plus);
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int g = tid * SPT + i;
+            if (g < G) {
+                sums[0][g] = g0[0];
+                sums[1][g] = g0[1];
+                const int y = sort[i][0], n = y < 0 ? 0 : cut[g] * set[i][0][0];
+                g0[0] += y == 0 ? n : 0;
+                g0[1] += y == 2 ? n : 0;
+            }
+        }
+        if (tid < 2) sums[tid][G] = tid ? all0[1] : all0[0];
+        __syncthreads();
+        // items of contents
+        for (int i = tid; i < all0[0] + all0[1]; i += LANES) {
+            const int y = i >= all0[0], x = y ? i - all0[0] : i, size = y ? 128 : 32;
+            const int g = find(sums[y], G, x), r = heads[g], c = content[r], j = x - sums[y][g];
+            int blocks, tiles;
+            group_set(g, blocks, tiles);
+            const int P = p.shared[3 * c], tok0 = first[r], T = first[heads[g + 1]] - tok0, kt = seats_up(P, PAGED_TILE) - tiles;
+            const int s = j / blocks, b = j - s * blocks, n = cut[g];
+            const int from = (int)((long)tiles * s / n), to = (int)((long)tiles * (s + 1) / n);
+            SeatItem it = {tok0, T, size * b, s, 0, {}, {{p.shared[3 * c + 2], P, kt + from, to - from, most(0, P + high[g] - far + 1), P - 1, 0, 0}, {}}};
+            if (x < (y ? kd.room[2] : kd.room[0])) store(y ? kd.block : kd.wave, x, it);
+        }
+        __syncthreads();
+        int parts[SPT], part0 = 0;
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int r = tid * SPT + i;
+            parts[i] = 0;
+            if (want[i]) {
+                const int y = sort[i][1], n = y == 0 ? seats_up(set[i][1][1], by_wave) : y == 2 ? seats_up(set[i][1][1], by_block) : 1;
+                if (y == 0) n1[0] += n * set[i][1][0];
+                if (y == 1) n1[1] += set[i][1][0];
+                if (y == 2) n1[2] += n * set[i][1][0];
+                if (y == 3) n1[3] += 1;
+                const int theirs = cut[of_group[r]];   // (of a seat that reads its content itself: none)
+                parts[i] = y == 3 ? theirs : theirs + n > 1 ? theirs + n : 0;
+                part0 = add(part0, seats_least(LOTS / 2, want[i] * parts[i]));
+            }
+        }
+        int n2[5] = {n1[0], n1[1], n1[2], n1[3], part0}, all2[5];
+        scan(n2, all2, room, 0, plus);
+#pragma unroll
+        for (int i = 0; i < 4; i++) all1[i] = all2[i];
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int r = tid * SPT + i;
+            if (r < R) {
+                const int y = want[i] ? sort[i][1] : -1, n = y == 0 ? seats_up(set[i][1][1], by_wave) : y == 2 ? seats_up(set[i][1][1], by_block) : 1;
+                sums[0][r] = n2[0];
+                sums[1][r] = n2[1];
+                sums[2][r] = n2[2];
+                kd.seat_parts[2 * r] = n2[4] | (y == 3 || parts[i] == 0 ? INT_MIN : 0);
+                kd.seat_parts[2 * r + 1] = parts[i];
+                if (y == 0) n2[0] += n * set[i][1][0];
+                if (y == 1) n2[1] += set[i][1][0];
+                if (y == 2) n2[2] += n * set[i][1][0];
+                if (y == 3) {
+                    if (n2[3] < kd.room[3]) {
+                        const int L = here[i] + 1, lo = most(0, here[i] - far + 1), at = p.table_at + r * p.width;
+                        int4* to = (int4*)(kd.last + sizeof(SeatLast) / 4 * (long)n2[3]);
+                        int ids[SEAT_PAGES];
+#pragma unroll
+                        for (int x = 0; x < SEAT_PAGES; x++) ids[x] = p.table[at + seats_least(lo / p.page + x, (L - 1) / p.page)];
+                        to[0] = make_int4(first[r], L, lo, at);
+                        to[1] = make_int4(n2[4], parts[i], ids[0], ids[1]);
+                        to[2] = make_int4(ids[2], ids[3], ids[4], ids[5]);
+                    }
+                    n2[3] += 1;
+                }
+                n2[4] = add(n2[4], seats_least(LOTS / 2, want[i] * parts[i]));
             }
         }
         if (tid < 3) sums[tid][R] = tid == 0 ? all1[0] : tid == 1 ? all1[1] : all1[2];
         if (tid == 0) {
-            kd.seat_parts[2 * R] = all1[3];
-            kd.counts[0] = all1[0];
+            kd.seat_parts[2 * R] = all2[4];
+            kd.counts[0] = all0[0] + all1[0];
             kd.counts[1] = all1[1];
-            kd.counts[2] = add(all0[0], all1[2]);
+            kd.counts[2] = all0[1] + all1[2];
             kd.counts[3] = all1[3];
+            kd.counts[4] = all2[4];
         }
         __syncthreads();
+        // items of the seats' own keys
         const int counts = all1[0] + all1[1] + all1[2];
         for (int i = tid; i < counts; i += LANES) {
-            const int sort = i < all1[0] ? 0 : i < all1[0] + all1[1] ? 1 : 2, j = sort == 0 ? i : sort == 1 ? i - all1[0] : i - all1[0] - all1[1];
-            const int r = find(sums[sort], R, j), x = j - sums[sort][r], n = took[r], L = stay[r] + n;
-            int blocks, tiles, is, pieces;
-            plan(r, n, blocks, tiles, is, pieces);
-            const int s = x / blocks, b = x - s * blocks, size = sort == 2 ? 128 : 32;
+            const int y = i < all1[0] ? 0 : i < all1[0] + all1[1] ? 1 : 2, j = y == 0 ? i : y == 1 ? i - all1[0] : i - all1[0] - all1[1];
+            const int r = find(sums[y], R, j), x = j - sums[y][r], n = took[r], L = stay[r] + n;
+            int blocks, tiles, shared;
+            seat_set(r, blocks, tiles, shared);
+            const int pieces = y == 1 ? 1 : seats_up(tiles + shared, y ? by_block : by_wave);
+            const int s = x / blocks, b = x - s * blocks, size = y == 2 ? 128 : 32;
             const int t0 = b * size / group, t1 = seats_least(n - 1, (b * size + size - 1) / group);   // its first and its last token
-            const int lo = most(0, stay[r] + t0 - far + 1), kt = lo / PAGED_TILE, mine = seats_up(stay[r] + t1 + 1, PAGED_TILE) - kt;
-            const int from = (int)((long)mine * s / pieces), to = (int)((long)mine * (s + 1) / pieces);
+            // tiles of the content, then of its own keys, that this block's rows see; the piece's share of them
+            const int c = content[r], P = shared ? p.shared[3 * c] : 0;
+            const int lo = most(0, stay[r] + t0 - far + 1), kt = lo / PAGED_TILE, own = seats_up(stay[r] + t1 + 1, PAGED_TILE) - kt;
+            const int lo2 = most(0, P + stay[r] + t0 - far + 1), kt2 = lo2 / PAGED_TILE, theirs = lo2 < P ? seats_up(P, PAGED_TILE) - kt2 : 0;
+            const int from = (int)((long)(own + theirs) * s / pieces), to = (int)((long)(own + theirs) * (s + 1) / pieces);
+            const SeatSpan mine = {p.table_at + r * p.width, L, kt + most(0, from - theirs), most(0, to - most(from, theirs)), most(0, stay[r] + t1 - far + 1), stay[r] + t0, 1, 0};
             const int ahead = cut[of_group[r]];
-            const SeatItem it = {first[r], n, L, p.table_at + r * p.width, b * size, kt + from, to - from, ahead + s, most(0, stay[r] + t1 - far + 1), stay[r] + t0,
-                                 SEAT_OWN | (ahead + pieces == 1 ? SEAT_ONLY : 0), 0};
-            if (sort == 0) { if (j < kd.wave_room) store(kd.wave, j, it); }
-            else if (sort == 1) { if (j < kd.single_room) store(kd.single, j, it); }
-            else if (all0[0] + j < kd.block_room) store(kd.block, all0[0] + j, it);
+            SeatItem it = {first[r], n, b * size, ahead + s, ahead + pieces == 1, {}, {mine, {}}};
+            if (theirs > 0 && from < theirs) {
+                it.span[0] = {p.shared[3 * c + 2], P, kt2 + from, seats_least(to, theirs) - from, most(0, P + stay[r] + t1 - far + 1), P - 1, 0, 0};
+                it.span[1] = mine;
+            }
+            const int at = y == 0 ? all0[0] + j : y == 1 ? j : all0[1] + j;
+            if (at < (y == 0 ? kd.room[0] : y == 1 ? kd.room[1] : kd.room[2])) store(y == 0 ? kd.wave : y == 1 ? kd.single : kd.block, at, it);
         }
     }
     __syncthreads();
@@ -379,27 +501,18 @@ __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
     }
 }
 
-// How long the lists of a head geometry may get: [0 .. 2] items, [3] partial rows (per query head)
-void rooms(const spinf_seats_args* a, const spinf_seats_kind& k, int64_t out[4]) {
-    const int64_t R = a->seats, rows = a->rows, group = k.hq / k.hkv, A = std::min(R, rows);   // at most A seats have new tokens
-    const int64_t tiles = (a->keys + PAGED_TILE - 1) / PAGED_TILE, in_all = a->pool * a->page / PAGED_TILE + R;
-    const int64_t waves = seats_wave_pieces((int)tiles, k.d, k.hkv, 1), pieces = std::min(A * waves, in_all / SEAT_WAVE_TILES + A);
-    out[0] = 2 * pieces;   // (at most 64 rows: two blocks)
-    out[1] = 2 * A;
-    // blocks x pieces of a set is its blocks, or at most places / hkv; tokens x pieces its tokens, or at most those of 128 rows per place
-    const int64_t places = (k.d == 512 ? PAGED_PLACES / 2 : PAGED_PLACES) / k.hkv + 1;
-    const int64_t big = std::min(A, rows * group / (SEAT_WAVE_ROWS + 1));
-    const auto items = [&](int64_t sets, int64_t most) { return std::min((rows * group / 128 + sets) * most, rows * group / 128 + sets + sets * places); };
-    const auto parts = [&](int64_t sets, int64_t most) { return std::min(rows * most, rows + sets * (128 / group + 1) * places); };
-    const int64_t own = seats_block_pieces((int)tiles, k.d, k.hkv, 1, false);
-    out[2] = big ? items(big, own) : 0;
-    out[3] = rows + std::min(rows * waves, std::max<int64_t>(1, SEAT_WAVE_ROWS / group) * pieces) + (big ? parts(big, own) : 0);
-    if (a->longest) {
-        const int64_t shared = seats_block_pieces((int)((a->longest + PAGED_TILE - 1) / PAGED_TILE), k.d, k.hkv, 1, true);
-        out[2] += items(A, shared);
-        out[3] += parts(A, shared);
-    }
-    for (int i = 0; i < 3; i++) out[i] = std::max<int64_t>(out[i], 1);
+// How long the lists of a head geometry may get: [0 .. 3] items (waves that divide tiles, a wave to 32 rows, shared tiles, the last word), [4] partial rows (per query head).  A set of `blocks`
+// blocks on `tiles` tiles is blocks x ceil(tiles / size) items, size at least the work of all sets over the places: in all no more than the places and a block each.
+void rooms(const spinf_seats_args* a, const spinf_seats_kind& k, int64_t out[5]) {
+    const int64_t group = k.hq / k.hkv, rows = a->rows, A = std::min<int64_t>(a->seats, rows);   // at most A seats have new tokens, below at most A contents
+    const int64_t by_wave = seats_wave_places(k.d) / k.hkv + 1, by_block = seats_block_places(k.d) / k.hkv + 1;
+    const bool block = rows * group > 32;
+    out[0] = by_wave + 3 * A;                                   // (a content's rows: two blocks at most)
+    out[1] = (SEAT_SHARED_ROWS + 31) / 32 * A;
+    out[2] = block ? by_block + 2 * (rows * group / 128 + A) : 0;
+    out[3] = group <= SEAT_LAST_HEADS ? A : 0;
+    // tokens x pieces: those of a set's blocks share the places; a token is in two sets at most
+    out[4] = 2 * rows + (32 / group + 1) * by_wave + (block ? (128 / group + 1) * by_block : 0);
 }
 
 int check(const spinf_seats_args* a, const char* what) {
@@ -419,16 +532,14 @@ int check(const spinf_seats_args* a, const char* what) {
         if (k.hq <= 0 || k.hkv <= 0 || k.hq % k.hkv || k.hq > 4096) return spinf_fail(SPINF_E_ARG, "%s: %d query heads do not group over %d key / value heads", what, k.hq, k.hkv);
         if (k.d != 64 && k.d != 128 && k.d != 256 && k.d != 512) return spinf_fail(SPINF_E_ARG, "%s: head dim %d not supported (64, 128, 256, 512)", what, k.d);
         if (k.window < 0) return spinf_fail(SPINF_E_ARG, "%s: window %d", what, k.window);
-        int64_t n[4];
-        rooms(a, k, n);
-        if (a->rows * k.hq > (1 << 30) || n[0] > (1 << 26) || n[2] > (1 << 26) || n[3] > (1 << 30)) return spinf_fail(SPINF_E_ARG, "%s: %lld rows of %d heads are too many", what, (long long)a->rows, k.hq);
+        if (a->rows * k.hq > (1 << 28)) return spinf_fail(SPINF_E_ARG, "%s: %lld rows of %d heads are too many", what, (long long)a->rows, k.hq);
     }
     return SPINF_OK;
 }
 
 }  // namespace
 
-extern "C" int spinf_seats_rooms(const spinf_seats_args* a, int32_t kind, int64_t out[4]) {
+extern "C" int spinf_seats_rooms(const spinf_seats_args* a, int32_t kind, int64_t out[5]) {
     const int rc = check(a, "seats_rooms");
     if (rc) return rc;
     if (kind < 0 || kind >= a->kinds || !out) return spinf_fail(SPINF_E_ARG, "seats_rooms: head geometry %d of %d", kind, a->kinds);
@@ -450,11 +561,11 @@ extern "C" int spinf_seats_step(const spinf_seats_args* a, void* stream) {
     p.contents = a->contents; p.table_at = (int)a->table_at; p.kinds = a->kinds;
     for (int i = 0; i < a->kinds; i++) {
         const spinf_seats_kind& k = a->kind[i];
-        int64_t n[4];
+        int64_t n[5];
         rooms(a, k, n);
-        if (!k.wave || !k.single || !k.block || !k.counts || !k.parts || !k.seat_parts) return spinf_fail(SPINF_E_ARG, "seats_step: null lists of head geometry %d", i);
-        if ((uintptr_t)k.wave % 16 || (uintptr_t)k.single % 16 || (uintptr_t)k.block % 16) return spinf_fail(SPINF_E_ARG, "seats_step: lists must be 16-byte aligned");
-        p.kind[i] = {k.wave, k.single, k.block, k.counts, k.parts, k.seat_parts, k.hq, k.hkv, k.d, k.window < LOTS ? k.window : LOTS, (int)n[0], (int)n[1], (int)n[2]};
+        if (!k.wave || !k.single || !k.block || !k.last || !k.counts || !k.parts || !k.seat_parts) return spinf_fail(SPINF_E_ARG, "seats_step: null lists of head geometry %d", i);
+        if ((uintptr_t)k.wave % 16 || (uintptr_t)k.single % 16 || (uintptr_t)k.block % 16 || (uintptr_t)k.last % 16) return spinf_fail(SPINF_E_ARG, "seats_step: lists must be 16-byte aligned");
+        p.kind[i] = {k.wave, k.single, k.block, k.last, k.counts, k.parts, k.seat_parts, k.hq, k.hkv, k.d, k.window < LOTS ? k.window : LOTS, {(int)n[0], (int)n[1], (int)n[2], (int)n[3]}};
     }
     hipStream_t s = (hipStream_t)stream;
     if (a->seats <= LANES) hipLaunchKernelGGL(seats_step_kernel<1>, dim3(1), dim3(LANES), 0, s, p);

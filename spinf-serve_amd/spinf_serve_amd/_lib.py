@@ -162,7 +162,7 @@ class RopeArgs(C.Structure):
 
 class SeatsKind(C.Structure):
     _fields_ = [
-        ("wave", C.c_void_p), ("single", C.c_void_p), ("block", C.c_void_p), ("counts", C.c_void_p), ("parts", C.c_void_p), ("seat_parts", C.c_void_p),
+        ("wave", C.c_void_p), ("single", C.c_void_p), ("block", C.c_void_p), ("last", C.c_void_p), ("counts", C.c_void_p), ("parts", C.c_void_p), ("seat_parts", C.c_void_p),
         ("hq", C.c_int32), ("hkv", C.c_int32), ("d", C.c_int32), ("window", C.c_int32),
     ]
 
@@ -186,7 +186,7 @@ class SeatsAttnArgs(C.Structure):
         ("k", C.c_void_p), ("v", C.c_void_p),
         ("k_page", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_page", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
         ("lists", C.c_void_p), ("first", C.c_void_p), ("pos", C.c_void_p),
-        ("kind", SeatsKind), ("rooms", C.c_int64 * 4),
+        ("kind", SeatsKind), ("rooms", C.c_int64 * 5),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
         ("rows", C.c_int64),
         ("seats", C.c_int32), ("page", C.c_int32),

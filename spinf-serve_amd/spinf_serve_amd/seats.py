@@ -108,7 +108,7 @@ class PagedSeats:
             raise ValueError("PagedSeats: numbers out of range")
         geo = [R, rows, page, keys, len(pool), len(c_lens), int(c_lens.max(initial=0)), int(need.sum()), len(kinds), *(x for k in kinds for x in k)]
         a = _numbers(geo)
-        rooms = (C.c_int64 * 4)()
+        rooms = (C.c_int64 * 5)()
         for i in range(len(kinds)):
             _lib.check(lib.spinf_seats_rooms(C.byref(a), i, rooms), "PagedSeats")
             geo += list(rooms)
@@ -175,8 +175,8 @@ def _kinds(geo):
 
 
 def _rooms(geo, i):
-    at = 9 + 4 * (geo[8] + i)
-    return geo[at : at + 4]
+    at = 9 + 4 * geo[8] + 5 * i
+    return geo[at : at + 5]
 
 
 def _layout(geo):
@@ -189,9 +189,9 @@ def _layout(geo):
     lay["all"] = at
     at, lists = 0, []
     for i in range(n):
-        wave, single, block, _ = _rooms(geo, i)
+        wave, single, block, last, _ = _rooms(geo, i)
         begins = []
-        for size in (12 * wave, 12 * single, 12 * block, 4, rows + 1, 2 * R + 1):
+        for size in (24 * wave, 24 * single, 24 * block, 12 * last, 5, rows + 1, 2 * R + 1):
             begins.append(at)
             at += _up4(size)
         lists.append(begins)
@@ -210,7 +210,7 @@ def _numbers(geo):
 
 def _point(kind, work, begins):
     base = work.data_ptr()
-    kind.wave, kind.single, kind.block, kind.counts, kind.parts, kind.seat_parts = (base + 4 * i for i in begins)
+    kind.wave, kind.single, kind.block, kind.last, kind.counts, kind.parts, kind.seat_parts = (base + 4 * i for i in begins)
 
 
 def _step_args(state, work, slots, pos, content, geo):
@@ -261,7 +261,7 @@ def _attn_run(a, q, k, v, want_lse, stream=None):
     if want_lse:
         lse = torch.empty((rows, hq), dtype=torch.float32, device=q.device)
         a.lse = lse.data_ptr()
-    n = a.rooms[3] * hq * (d + 2)
+    n = a.rooms[4] * hq * (d + 2)
     work = torch.empty(n, dtype=torch.float32, device=q.device)
     a.workspace, a.workspace_bytes = work.data_ptr(), 4 * n
     a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()

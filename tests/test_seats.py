@@ -95,12 +95,12 @@ def test_the_c_entries_refuse_bad_arguments(lib):
         a = args()
         setattr(a, name, x)
         refused(a)
-    for name in ("wave", "single", "block", "counts", "parts", "seat_parts"):
+    for name in ("wave", "single", "block", "last", "counts", "parts", "seat_parts"):
         a = args()
         setattr(a.kind[0], name, None)
         refused(a)
     assert lib.spinf_seats_step(None, None) == -1 and lib.spinf_seats_attn_fwd(None, None) == -1
-    rooms = (C.c_int64 * 4)()
+    rooms = (C.c_int64 * 5)()
     assert lib.spinf_seats_rooms(C.byref(args()), 1, rooms) == -1 and lib.spinf_seats_rooms(C.byref(args()), 0, None) == -1
 
     q = torch.zeros((4, 4, 64), dtype=BF16)
@@ -109,7 +109,7 @@ def test_the_c_entries_refuse_bad_arguments(lib):
     def attn():
         b = ss._attn_block(q, *cache, s._state, s._work, s.pos, s._geo, 0, 0.1, 0.0)
         b.q = b.out = b.k = b.v = b.workspace = q.data_ptr()
-        b.workspace_bytes = b.rooms[3] * 4 * 66 * 4
+        b.workspace_bytes = b.rooms[4] * 4 * 66 * 4
         return b
 
     for name, x in (("q", None), ("out", None), ("k", None), ("v", None), ("lists", None), ("first", None), ("pos", None), ("workspace", None), ("workspace_bytes", 16), ("rows", 0), ("seats", 0),
@@ -199,6 +199,9 @@ SHAPES = [
     ([5000], [0] * 3, [2500, 30, 130], [1, 1, 2], 64, (12, 12, 64), 0),
     ([200, 90], [0, -1, 0, 1, 0], [300, 200, 70, 150, 66], [300, 200, 0, 140, 66], 32, (4, 1, 512), 0),
     ([64], [0, 0, 0], [5, 9, 20], [0, 0, 0], 16, (4, 2, 64), 0),
+    ([90, 2000], [0, 0, 1, 1, 1, -1, 1, 1], [128, 129, 100, 7, 300, 64, 97, 500], [1, 1, 1, 2, 97, 1, 1, 49], 16, (16, 8, 128), 0),
+    ([800], [0] * 70 + [-1], [90 + i for i in range(71)], [1] * 71, 16, (8, 1, 64), 120),
+    ([3000], [0] * 20, [40] * 20, [7] * 20, 64, (16, 2, 256), 0),
 ]
 
 
@@ -220,9 +223,10 @@ def test_work_lists_are_the_dense_mask(dev, stored, content, own, new, page, hea
     work = s._work.cpu().numpy()
     lists = ss._layout(s._geo)["lists"][0]
     rooms = ss._rooms(s._geo, 0)
-    counts = work[lists[3] : lists[3] + 4]
+    counts = work[lists[4] : lists[4] + 5]
     assert all(n <= room for n, room in zip(counts, rooms))
-    parts = work[lists[4] : lists[4] + s.rows + 1]
+    begins = work[lists[5] : lists[5] + s.rows + 1]
+    parts, done = begins & 0x7FFFFFFF, begins < 0
     first = s.first.cpu().numpy()
     see = dense(s, stored, content, own, new, window)
     seen = [np.zeros((m * group, x.shape[1]), np.int8) for m, x in zip(new, see)]
@@ -230,40 +234,63 @@ def test_work_lists_are_the_dense_mask(dev, stored, content, own, new, page, hea
     span_at = {}   # where a span's page list begins -> its seat or content
     at = 0
     for c, n in enumerate(stored):
-        span_at[at] = c
-        at += -(-n // page) if n else 0
+        if n:
+            span_at[at] = c
+        at += -(-n // page)
     own_at = {ss._layout(s._geo)["table"] + r * s.table.shape[1]: r for r in range(len(own))}
-    used = set()
+    used, spoken = set(), set()
+
+    def keep(tok, head, piece, only):
+        if only:
+            assert done[tok] and parts[tok + 1] == parts[tok] and (tok, head) not in spoken
+            spoken.add((tok, head))
+        else:
+            assert 0 <= piece < parts[tok + 1] - parts[tok] and (tok, head, piece) not in used
+            used.add((tok, head, piece))
+
     for kind in range(3):
         size = 128 if kind == 2 else 32
-        for tok0, T, L, tab, row0, kt0, tiles, piece, flo, fhi, flags, _ in work[lists[kind] : lists[kind] + 12 * counts[kind]].reshape(-1, 12).tolist():
+        for tok0, T, row0, piece, only, _, _, _, *spans in work[lists[kind] : lists[kind] + 24 * counts[kind]].reshape(-1, 24).tolist():
             rows = range(row0, min(row0 + size, T * group))
-            assert len(rows) and row0 % size == 0 and kt0 >= 0 and tiles >= 0 and (not tiles or 32 * (kt0 + tiles - 1) < L)
-            keys = np.arange(32 * kt0, min(32 * (kt0 + tiles), L))
+            assert len(rows) and row0 % size == 0 and (kind == 2 or spans[11] == 0)
             for x in rows:
                 tok = tok0 + x // group
                 r = int(seat_of[tok])
-                c = content[r]
-                P = stored[c] if c >= 0 else 0
-                if flags & 1:
-                    assert own_at[tab] == r and (L, T, tok0) == (own[r], new[r], first[r])
-                    at = P
-                else:
-                    assert span_at[tab] == c and L == P
-                    at = 0
-                assert (flags >> 1 & 1) == (parts[tok + 1] == parts[tok])
-                if not flags & 2:
-                    assert 0 <= piece < parts[tok + 1] - parts[tok] and (tok, x % group, piece) not in used
-                    used.add((tok, x % group, piece))
-                row = (tok - first[r]) * group + x % group
-                line = see[r][tok - first[r]]
-                inside = keys[(keys >= flo) & (keys <= fhi)]
-                assert line[at + inside].all()
-                seen[r][row, at + keys] += line[at + keys].astype(np.int8)
+                keep(tok, x % group, piece, only)
+                for tab, L, kt0, tiles, flo, fhi, mine, _ in (spans[:8], spans[8:]):
+                    if tiles == 0:
+                        continue
+                    assert kt0 >= 0 and tiles > 0 and 32 * (kt0 + tiles - 1) < L
+                    keys = np.arange(32 * kt0, min(32 * (kt0 + tiles), L))
+                    c = content[r]
+                    P = stored[c] if c >= 0 else 0
+                    if mine:
+                        assert own_at[tab] == r and (L, T, tok0) == (own[r], new[r], first[r])
+                    else:
+                        assert span_at[tab] == c and L == P
+                    at = P if mine else 0
+                    line = see[r][tok - first[r]]
+                    assert line[at + keys[(keys >= flo) & (keys <= fhi)]].all()
+                    seen[r][(tok - first[r]) * group + x % group, at + keys] += line[at + keys].astype(np.int8)
+    for tok, L, lo, tab, part, n, *ids in work[lists[3] : lists[3] + 12 * counts[3]].reshape(-1, 12).tolist():
+        r = int(seat_of[tok])
+        c = content[r]
+        P = stored[c] if c >= 0 else 0
+        table = s.table[r].tolist()
+        assert own_at[tab] == r and (L, part, n) == (own[r], parts[tok], parts[tok + 1] - parts[tok]) and new[r] == 1 and group <= 8 and 0 < L - lo <= 128 and done[tok]
+        many = (L - 1) // page - lo // page + 1
+        assert ids[: min(many, 6)] == table[lo // page : lo // page + min(many, 6)] and set(ids) <= set(table)
+        line = see[r][0]
+        assert line[P + lo : P + L].all()
+        for h in range(group):
+            seen[r][h, P + lo : P + L] += 1
+            assert (tok, h) not in spoken
+            spoken.add((tok, h))
     for x, y in zip(seen, see):
         assert (x == np.repeat(y, group, 0)).all()   # every visible pair once
     total = int(first[-1])
-    assert len(used) == int(parts[total] * group) and (parts[total:] == counts[3]).all() and counts[3] <= rooms[3]
+    assert len(used) == int(parts[total] * group) and (parts[total:] == counts[4]).all() and counts[4] <= rooms[4] and not done[total:].any()
+    assert {t for t, _ in spoken} == set(np.flatnonzero(done).tolist()) and len(spoken) == done.sum() * group
 
 
 @pytest.mark.gpu
@@ -283,7 +310,7 @@ def test_lists_never_outgrow_their_rooms(dev):
             s.step(new, torch.from_numpy((rng.integers(0, 2, R) * 10000).astype(np.int32)).to(dev))
             for k in range(len(heads)):
                 lists = ss._layout(s._geo)["lists"][k]
-                counts = s._work[lists[3] : lists[3] + 4].tolist()
+                counts = s._work[lists[4] : lists[4] + 5].tolist()
                 assert all(n <= room for n, room in zip(counts, ss._rooms(s._geo, k)))
 
 
