@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int LANES = 1024, WAVES = LANES / 64;
+constexpr int LANES = 512, WAVES = LANES / 64;
 constexpr int LOTS = 1 << 30;   // sums stop there
 
 struct Kind { int* wave; int* single; int* block; int* last; int* counts; int* parts; int* seat_parts; int hq, hkv, d, window, room[4]; };
@@ -93,7 +93,7 @@ __device__ __forceinline__ void store(int* items, int at, const SeatItem& it) {
     }
 }
 
-// Places and positions of rows, and where their partial results begin
+// Places and positions of rows
 __device__ __forceinline__ void place_row(const Params& p, int row, int total, int seat, int first, int stay, int content) {
     long slot = -1;
     int pos = 0;
@@ -105,33 +105,31 @@ __device__ __forceinline__ void place_row(const Params& p, int row, int total, i
     }
     p.slots[row] = slot;
     p.pos[row] = pos;
-    for (int k = 0; k < p.kinds; k++) {
-        const int* sp = p.kind[k].seat_parts;
-        const int base = sp[2 * (row < total ? seat : p.seats)];   // (the sign: no piece is left to be joined)
-        p.kind[k].parts[row] = row < total ? ((base & INT_MAX) + (row - first) * sp[2 * seat + 1]) | (base & INT_MIN) : base;
-        if (row == p.rows - 1) p.kind[k].parts[p.rows] = sp[2 * p.seats];
-    }
+}
+// where a row's partial results begin
+__device__ __forceinline__ void place_parts(const Params& p, const Kind& kd, int row, int total, int seat, int first) {
+    const int* sp = kd.seat_parts;
+    const int base = sp[2 * (row < total ? seat : p.seats)];
+    kd.parts[row] = row < total ? ((base & INT_MAX) + (row - first) * sp[2 * seat + 1]) | (base & INT_MIN) : base;
 }
 
 __global__ __launch_bounds__(256) void seats_rows_kernel(const Params p) {
     const int row = blockIdx.x * 256 + threadIdx.x;
-    if (row >= p.rows) return;
+    if (row > p.rows) return;
     const int total = p.first[p.seats];
     const int seat = row < total ? find(p.first, p.seats, row) : 0;
-    place_row(p, row, total, seat, p.first[seat], p.stay[seat], p.content[seat]);
+    if (row < p.rows) place_row(p, row, total, seat, p.first[seat], p.stay[seat], p.content[seat]);
+    for (int k = 0; k < p.kinds; k++) place_parts(p, p.kind[k], row, total, seat, p.first[seat]);
 }
 
 template <int SPT>   // seats per lane
 __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
     constexpr int MOST = SPT * LANES;
-    __shared__ long room[6][WAVES];
+    __shared__ long room[2][WAVES];
     __shared__ int stay[MOST], took[MOST], content[MOST], first[MOST + 1];
-    __shared__ int sums[4][MOST + 1];
-    __shared__ int heads[MOST + 1], low[MOST], high[MOST], of_group[MOST], cut[MOST];   // by group of seats in a row that share their content; cut: pieces of its keys
-    __shared__ int best[2];
+    __shared__ int sums[2][MOST + 1];
     const int R = p.seats, tid = threadIdx.x;
     const auto plus = [](int a, int b) __attribute__((always_inline)) { return add(a, b); };
-    const auto larger = [](int a, int b) __attribute__((always_inline)) { return most(a, b); };
     const auto pages = [&](int n) __attribute__((always_inline)) { return (n + p.page - 1) / p.page; };
 
     // ---- what goes: pages back on the stack, the first of the order last
@@ -220,284 +218,279 @@ __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
         p.table[p.table_at + (long)r * p.width + pages(stay[r]) + i - sums[1][r]] = p.free[left - 1 - i];
     }
 
-    // ---- the last seat with new tokens ahead of each
-    int last[1] = {-1}, whole[1];
-#pragma unroll
-    for (int i = 0; i < SPT; i++) {
-        const int r = tid * SPT + i;
-        if (r < R && want[i]) last[0] = r;
-    }
-    scan(last, whole, room, -1, larger);
-
-    // ---- the lists of every head geometry
-    for (int k = 0; k < p.kinds; k++) {
-        const Kind& kd = p.kind[k];
-        const int group = kd.hq / kd.hkv, W = kd.window;
-        const int far = W ? W : LOTS;
-        const auto alone = [&](int r) __attribute__((always_inline)) { return took[r] * group > SEAT_SHARED_ROWS; };   // (such a seat reads its content for itself)
-        __syncthreads();
-        // groups: seats that share a content, one after the other (seats without new tokens do not part them)
-        int head[1] = {0}, groups[1], ahead = last[0];
-        bool begins[SPT];
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int r = tid * SPT + i;
-            begins[i] = r < R && want[i] && (ahead < 0 || content[ahead] != content[r] || alone(r) || alone(ahead));
-            head[0] += begins[i];
-            if (r < R && want[i]) ahead = r;
-        }
-        scan(head, groups, room, 0, plus);
-        const int G = groups[0];
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int r = tid * SPT + i;
-            if (r < R) {
-                if (begins[i]) {
-                    heads[head[0]] = r;
-                    low[head[0]] = INT_MAX;
-                    high[head[0]] = 0;
-                }
-                head[0] += begins[i];
-                of_group[r] = head[0] - 1;   // (means something only where the seat has new tokens)
-            }
-        }
-        if (tid == 0) heads[G] = R;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {   // the least and the largest place among the seats' own keys of a group's new tokens
-            const int r = tid * SPT + i;
-            if (want[i]) {
-                atomicMin(&low[of_group[r]], here[i]);
-                atomicMax(&high[of_group[r]], here[i] + want[i] - 1);
-            }
-        }
-        __syncthreads();
-        // what there is to do: sets of rows (blocks) on tiles; a group's content in the first half, a seat's own keys in the second
-        const auto group_set = [&](int g, int& blocks, int& tiles) __attribute__((always_inline)) {   // -> waves divide the tiles
-            const int r = heads[g], c = content[r];
-            blocks = tiles = 0;
-            if (c < 0 || alone(r)) return false;
-            const int P = p.shared[3 * c], rows = (first[heads[g + 1]] - first[r]) * group;
-            const int lo = most(0, P + low[g] - far + 1);
-            const bool few = rows <= SEAT_WAVE_ROWS;
-            if (lo < P) {
-                tiles = seats_up(P, PAGED_TILE) - lo / PAGED_TILE;
-                blocks = seats_up(rows, few ? 32 : 128);
-            }
-            return few;
-        };
-        // sorts: 0 waves that divide the tiles, 1 a wave to 32 rows, 2 shared tiles, 3 the last word; shared: its content's tiles, where it reads them itself
-        const auto seat_set = [&](int r, int& blocks, int& tiles, int& shared) __attribute__((always_inline)) {
-            const int n = took[r], rows = n * group, L = stay[r] + n, lo = most(0, stay[r] - far + 1);
-            tiles = seats_up(L, PAGED_TILE) - lo / PAGED_TILE;
-            shared = 0;
-            if (n == 1 && group <= SEAT_LAST_HEADS && L - lo <= SEAT_LAST_KEYS) {
-                blocks = 1;
-                return 3;
-            }
-            if (alone(r)) {
-                const int c = content[r], P = c >= 0 ? p.shared[3 * c] : 0, from = most(0, P + stay[r] - far + 1);
-                shared = from < P ? seats_up(P, PAGED_TILE) - from / PAGED_TILE : 0;
-                blocks = seats_up(rows, 128);
-                return 2;
-            }
-            const int sort = tiles <= SEAT_SINGLE_TILES ? 1 : rows <= 32 ? 0 : 2;
-            blocks = seats_up(rows, sort == 2 ? 128 : 32);
-            return sort;
-        };
-        int set[SPT][2][2], sort[SPT][2];   // blocks, tiles; sort (-1: nothing): of group i and of seat i
-        long work[2] = {0, 0}, all_work[2];   // by waves that divide the tiles, on shared tiles
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int r = tid * SPT + i;
-            sort[i][0] = sort[i][1] = -1;
-            if (r < G) {
-                const bool few = group_set(r, set[i][0][0], set[i][0][1]);
-                if (set[i][0][0]) sort[i][0] = few ? 0 : 2;
-            }
-            if (want[i]) {
-                int shared;
-                sort[i][1] = seat_set(r, set[i][1][0], set[i][1][1], shared);
-                set[i][1][1] += shared;
-            }
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-            {
-                const long n = (long)set[i][x][0] * set[i][x][1];
-                work[0] += sort[i][x] == 0 ? n : 0;
-                work[1] += sort[i][x] == 2 ? n : 0;
-            }
-        }
-        scan(work, all_work, room, 0l, [](long a, long b) { return a + b; });
-        // Tiles of a piece: of some sizes at and above those that make as many pieces as there are places, the one whose rounds of workgroups end first
-        constexpr int SIZES = 6;
-        int size[2][SIZES], items[2][SIZES] = {}, all_items[SIZES];
-        const int places[2] = {seats_wave_places(kd.d), seats_block_places(kd.d)};
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int j = 0; j < SIZES; j++) {
-                const long tiles = (all_work[x] * kd.hkv * (8 + j * (j + 1) / 2) / 8 + places[x] - 1) / places[x];   // 1, 1 1/8, 1 3/8, 1 3/4, 2 1/4, 2 7/8
-                size[x][j] = most(x ? SEAT_BLOCK_TILES : SEAT_WAVE_TILES, (int)(tiles < LOTS ? tiles : LOTS));
-            }
-#pragma unroll
-        for (int i = 0; i < SPT; i++)
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int y = 0; y < 2; y++)
-                    if (sort[i][x] == 2 * y)
-#pragma unroll
-                        for (int j = 0; j < SIZES; j++) items[y][j] += set[i][x][0] * seats_up(set[i][x][1], size[y][j]);
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            if (all_work[y] == 0) continue;
-            scan(items[y], all_items, room, 0, plus);
-            if (tid == 0) {
-                long cost = LONG_MAX;
-#pragma unroll
-                for (int j = 0; j < SIZES; j++) {
-                    const long rounds = ((long)all_items[j] * kd.hkv + places[y] - 1) / places[y];
-                    const long here = rounds * (size[y][j] + (y ? 4 : 12));   // (a workgroup's start and end are worth some tiles)
-                    if (here < cost) {
-                        cost = here;
-                        best[y] = size[y][j];
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        const int by_wave = best[0], by_block = best[1];
-        // how many items of each sort, where each set's begin, partial results of each seat
-        int n1[4] = {0, 0, 0, 0}, all1[4];   // sort 0, 1, 3; sort 2: groups, then seats, as one sum each
-        int g0[2] = {0, 0}, all0[2];
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int g = tid * SPT + i;
-            if (g < G) {
-                const int y = sort[i][0], n = y < 0 ? 0 : seats_up(set[i][0][1], y ? by_block : by_wave);
-                cut[g] = n;
-                g0[0] += y == 0 ? n * set[i][0][0] : 0;
-                g0[1] += y == 2 ? n * set[i][0][0] : 0;
-            }
-        }
-        scan(g0, all0, room, 0, plus);
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int g = tid * SPT + i;
-            if (g < G) {
-                sums[0][g] = g0[0];
-                sums[1][g] = g0[1];
-                const int y = sort[i][0], n = y < 0 ? 0 : cut[g] * set[i][0][0];
-                g0[0] += y == 0 ? n : 0;
-                g0[1] += y == 2 ? n : 0;
-            }
-        }
-        if (tid < 2) sums[tid][G] = tid ? all0[1] : all0[0];
-        __syncthreads();
-        // items of contents
-        for (int i = tid; i < all0[0] + all0[1]; i += LANES) {
-            const int y = i >= all0[0], x = y ? i - all0[0] : i, size = y ? 128 : 32;
-            const int g = find(sums[y], G, x), r = heads[g], c = content[r], j = x - sums[y][g];
-            int blocks, tiles;
-            group_set(g, blocks, tiles);
-            const int P = p.shared[3 * c], tok0 = first[r], T = first[heads[g + 1]] - tok0, kt = seats_up(P, PAGED_TILE) - tiles;
-            const int s = j / blocks, b = j - s * blocks, n = cut[g];
-            const int from = (int)((long)tiles * s / n), to = (int)((long)tiles * (s + 1) / n);
-            SeatItem it = {tok0, T, size * b, s, 0, {}, {{p.shared[3 * c + 2], P, kt + from, to - from, most(0, P + high[g] - far + 1), P - 1, 0, 0}, {}}};
-            if (x < (y ? kd.room[2] : kd.room[0])) store(y ? kd.block : kd.wave, x, it);
-        }
-        __syncthreads();
-        int parts[SPT], part0 = 0;
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int r = tid * SPT + i;
-            parts[i] = 0;
-            if (want[i]) {
-                const int y = sort[i][1], n = y == 0 ? seats_up(set[i][1][1], by_wave) : y == 2 ? seats_up(set[i][1][1], by_block) : 1;
-                if (y == 0) n1[0] += n * set[i][1][0];
-                if (y == 1) n1[1] += set[i][1][0];
-                if (y == 2) n1[2] += n * set[i][1][0];
-                if (y == 3) n1[3] += 1;
-                const int theirs = cut[of_group[r]];   // (of a seat that reads its content itself: none)
-                parts[i] = y == 3 ? theirs : theirs + n > 1 ? theirs + n : 0;
-                part0 = add(part0, seats_least(LOTS / 2, want[i] * parts[i]));
-            }
-        }
-        int n2[5] = {n1[0], n1[1], n1[2], n1[3], part0}, all2[5];
-        scan(n2, all2, room, 0, plus);
-#pragma unroll
-        for (int i = 0; i < 4; i++) all1[i] = all2[i];
-#pragma unroll
-        for (int i = 0; i < SPT; i++) {
-            const int r = tid * SPT + i;
-            if (r < R) {
-                const int y = want[i] ? sort[i][1] : -1, n = y == 0 ? seats_up(set[i][1][1], by_wave) : y == 2 ? seats_up(set[i][1][1], by_block) : 1;
-                sums[0][r] = n2[0];
-                sums[1][r] = n2[1];
-                sums[2][r] = n2[2];
-                kd.seat_parts[2 * r] = n2[4] | (y == 3 || parts[i] == 0 ? INT_MIN : 0);
-                kd.seat_parts[2 * r + 1] = parts[i];
-                if (y == 0) n2[0] += n * set[i][1][0];
-                if (y == 1) n2[1] += set[i][1][0];
-                if (y == 2) n2[2] += n * set[i][1][0];
-                if (y == 3) {
-                    if (n2[3] < kd.room[3]) {
-                        const int L = here[i] + 1, lo = most(0, here[i] - far + 1), at = p.table_at + r * p.width;
-                        int4* to = (int4*)(kd.last + sizeof(SeatLast) / 4 * (long)n2[3]);
-                        int ids[SEAT_PAGES];
-#pragma unroll
-                        for (int x = 0; x < SEAT_PAGES; x++) ids[x] = p.table[at + seats_least(lo / p.page + x, (L - 1) / p.page)];
-                        to[0] = make_int4(first[r], L, lo, at);
-                        to[1] = make_int4(n2[4], parts[i], ids[0], ids[1]);
-                        to[2] = make_int4(ids[2], ids[3], ids[4], ids[5]);
-                    }
-                    n2[3] += 1;
-                }
-                n2[4] = add(n2[4], seats_least(LOTS / 2, want[i] * parts[i]));
-            }
-        }
-        if (tid < 3) sums[tid][R] = tid == 0 ? all1[0] : tid == 1 ? all1[1] : all1[2];
-        if (tid == 0) {
-            kd.seat_parts[2 * R] = all2[4];
-            kd.counts[0] = all0[0] + all1[0];
-            kd.counts[1] = all1[1];
-            kd.counts[2] = all0[1] + all1[2];
-            kd.counts[3] = all1[3];
-            kd.counts[4] = all2[4];
-        }
-        __syncthreads();
-        // items of the seats' own keys
-        const int counts = all1[0] + all1[1] + all1[2];
-        for (int i = tid; i < counts; i += LANES) {
-            const int y = i < all1[0] ? 0 : i < all1[0] + all1[1] ? 1 : 2, j = y == 0 ? i : y == 1 ? i - all1[0] : i - all1[0] - all1[1];
-            const int r = find(sums[y], R, j), x = j - sums[y][r], n = took[r], L = stay[r] + n;
-            int blocks, tiles, shared;
-            seat_set(r, blocks, tiles, shared);
-            const int pieces = y == 1 ? 1 : seats_up(tiles + shared, y ? by_block : by_wave);
-            const int s = x / blocks, b = x - s * blocks, size = y == 2 ? 128 : 32;
-            const int t0 = b * size / group, t1 = seats_least(n - 1, (b * size + size - 1) / group);   // its first and its last token
-            // tiles of the content, then of its own keys, that this block's rows see; the piece's share of them
-            const int c = content[r], P = shared ? p.shared[3 * c] : 0;
-            const int lo = most(0, stay[r] + t0 - far + 1), kt = lo / PAGED_TILE, own = seats_up(stay[r] + t1 + 1, PAGED_TILE) - kt;
-            const int lo2 = most(0, P + stay[r] + t0 - far + 1), kt2 = lo2 / PAGED_TILE, theirs = lo2 < P ? seats_up(P, PAGED_TILE) - kt2 : 0;
-            const int from = (int)((long)(own + theirs) * s / pieces), to = (int)((long)(own + theirs) * (s + 1) / pieces);
-            const SeatSpan mine = {p.table_at + r * p.width, L, kt + most(0, from - theirs), most(0, to - most(from, theirs)), most(0, stay[r] + t1 - far + 1), stay[r] + t0, 1, 0};
-            const int ahead = cut[of_group[r]];
-            SeatItem it = {first[r], n, b * size, ahead + s, ahead + pieces == 1, {}, {mine, {}}};
-            if (theirs > 0 && from < theirs) {
-                it.span[0] = {p.shared[3 * c + 2], P, kt2 + from, seats_least(to, theirs) - from, most(0, P + stay[r] + t1 - far + 1), P - 1, 0, 0};
-                it.span[1] = mine;
-            }
-            const int at = y == 0 ? all0[0] + j : y == 1 ? j : all0[1] + j;
-            if (at < (y == 0 ? kd.room[0] : y == 1 ? kd.room[1] : kd.room[2])) store(y == 0 ? kd.wave : y == 1 ? kd.single : kd.block, at, it);
-        }
-    }
     __syncthreads();
     if (p.rows > SEATS_ROWS_AT_ONCE) return;
     for (int row = tid; row < p.rows; row += LANES) {
         const int seat = row < total ? find(first, R, row) : 0;
         place_row(p, row, total, seat, first[seat], stay[seat], content[seat]);
+    }
+}
+
+// Running sums in place, of N arrays of n numbers in LDS at a time: a[i] becomes the sum of those before it, a[n] of all
+template <int N>
+__device__ __forceinline__ void running(int* const (&a)[N], int n, long (*room)[WAVES]) {
+    const int per = (n + LANES - 1) / LANES, from = seats_least(n, (int)threadIdx.x * per), to = seats_least(n, from + per);
+    int sum[N], all[N];
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        sum[x] = 0;
+        for (int i = from; i < to; i++) sum[x] += a[x][i];
+    }
+    scan(sum, all, room, 0, [](int a, int b) { return a + b; });
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        for (int i = from; i < to; i++) {
+            const int y = a[x][i];
+            a[x][i] = sum[x];
+            sum[x] += y;
+        }
+        if (threadIdx.x == 0) a[x][n] = all[x];
+    }
+    __syncthreads();
+}
+
+// The work lists of a head geometry, a workgroup each.
+template <int MOST>
+__global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
+    __shared__ long room[7][WAVES];
+    __shared__ int stay[MOST], took[MOST], content[MOST], first[MOST + 1];
+    __shared__ int heads[MOST + 1], low[MOST], high[MOST], of_group[MOST + 1], cut[MOST];   // of groups: seats one after the other that share their content; cut: pieces of its keys
+    __shared__ int sums[5][MOST + 1];
+    __shared__ int best[2];
+    const int R = p.seats, tid = threadIdx.x;
+    const Kind& kd = p.kind[blockIdx.x];
+    const int group = kd.hq / kd.hkv, W = kd.window;
+    const int far = W ? W : LOTS, deep = 128;   // rows of an item on shared tiles
+    const auto each_seat = [&](auto f) __attribute__((always_inline)) {
+        for (int r = tid; r < R; r += LANES) f(r);
+    };
+    each_seat([&](int r) __attribute__((always_inline)) {
+        stay[r] = p.stay[r];
+        took[r] = p.took[r];
+        first[r] = p.first[r];
+        const int c = p.content[r];
+        content[r] = c < 0 || c >= p.contents ? -1 : c;
+        heads[r] = took[r] ? r + 1 : 0;
+        low[r] = INT_MAX;
+        high[r] = 0;
+    });
+    const int total = p.first[R];
+    if (tid == 0) first[R] = total;
+    // (a seat of many rows reads its content for itself)
+    const auto alone = [&](int r) __attribute__((always_inline)) { return took[r] * group > SEAT_SHARED_ROWS; };
+    // ---- groups: seats with new tokens below one content, one after the other (seats without any in between do not part them)
+    {   // the last seat with new tokens ahead of each: one more than its index
+        const int per = (R + LANES - 1) / LANES, from = seats_least(R, tid * per), to = seats_least(R, from + per);
+        int last[1] = {0}, all[1];
+        __syncthreads();
+        for (int r = from; r < to; r++) last[0] = most(last[0], heads[r]);
+        scan(last, all, room, 0, [](int a, int b) { return a > b ? a : b; });
+        for (int r = from; r < to; r++) {
+            const int ahead = last[0] - 1;
+            last[0] = most(last[0], heads[r]);
+            of_group[r] = took[r] && (ahead < 0 || content[ahead] != content[r] || alone(r) || alone(ahead));
+        }
+    }
+    __syncthreads();
+    each_seat([&](int r) __attribute__((always_inline)) { sums[0][r] = of_group[r]; });   // (does one begin here?)
+    {
+        int* const a[1] = {of_group};
+        running(a, R, room);   // groups that begin before the seat
+    }
+    const int G = of_group[R];
+    __syncthreads();
+    each_seat([&](int r) __attribute__((always_inline)) {
+        const int begins = sums[0][r], g = of_group[r] + begins - 1;
+        if (begins) heads[g] = r;   // (of a group and a seat: no seat's place in `heads` is read any more)
+        of_group[r] = g;            // (means something only where the seat has new tokens)
+    });
+    if (tid == 0) heads[G] = R;
+    __syncthreads();
+    each_seat([&](int r) __attribute__((always_inline)) {   // the least and the largest place among the seats' own keys of a group's new tokens
+        if (took[r]) {
+            atomicMin(&low[of_group[r]], stay[r]);
+            atomicMax(&high[of_group[r]], stay[r] + took[r] - 1);
+        }
+    });
+    __syncthreads();
+    // ---- what there is to do, as sets of `blocks` blocks of rows on `tiles` tiles.  Sorts: 0 waves that divide the tiles, 1 a wave to 32 rows, 2 shared tiles, 3 the last word, -1 nothing
+    const auto group_set = [&](int g, int& blocks, int& tiles) __attribute__((always_inline)) {
+        const int r = heads[g], c = content[r];
+        blocks = tiles = 0;
+        if (c < 0 || alone(r)) return -1;
+        const int P = p.shared[3 * c], rows = (first[heads[g + 1]] - first[r]) * group, lo = most(0, P + low[g] - far + 1);
+        if (lo >= P) return -1;
+        const bool few = rows <= SEAT_WAVE_ROWS;
+        tiles = seats_up(P, PAGED_TILE) - lo / PAGED_TILE;
+        blocks = seats_up(rows, few ? 32 : deep);
+        return few ? 0 : 2;
+    };
+    // tiles: of its own keys; shared: of its content's, where it reads them itself
+    const auto seat_set = [&](int r, int& blocks, int& tiles, int& shared) __attribute__((always_inline)) {
+        const int n = took[r], rows = n * group, L = stay[r] + n, lo = most(0, stay[r] - far + 1);
+        blocks = tiles = shared = 0;
+        if (n == 0) return -1;
+        tiles = seats_up(L, PAGED_TILE) - lo / PAGED_TILE;
+        blocks = 1;
+        if (n == 1 && group <= SEAT_LAST_HEADS && L - lo <= SEAT_LAST_KEYS) return 3;
+        if (alone(r)) {
+            const int c = content[r], P = c >= 0 ? p.shared[3 * c] : 0, from = most(0, P + stay[r] - far + 1);
+            shared = from < P ? seats_up(P, PAGED_TILE) - from / PAGED_TILE : 0;
+            blocks = seats_up(rows, deep);
+            return 2;
+        }
+        const int sort = tiles <= SEAT_SINGLE_TILES ? 1 : rows <= 32 ? 0 : 2;
+        blocks = seats_up(rows, sort == 2 ? deep : 32);
+        return sort;
+    };
+    const auto each_set = [&](auto f) __attribute__((always_inline)) {   // f(sort, blocks, tiles)
+        for (int i = tid; i < R; i += LANES) {
+            int blocks, tiles, shared;
+            if (i < G) {
+                const int sort = group_set(i, blocks, tiles);
+                f(sort, blocks, tiles);
+            }
+            const int sort = seat_set(i, blocks, tiles, shared);
+            f(sort, blocks, tiles + shared);
+        }
+    };
+    // ---- tiles of a piece: of some sizes at and above those that make as many pieces as there are places, the one whose rounds of workgroups end first
+    long work[2] = {0, 0}, all_work[2];   // by waves that divide the tiles, on shared tiles
+    each_set([&](int sort, int blocks, int tiles) __attribute__((always_inline)) {
+        const long n = (long)blocks * tiles;
+        work[0] += sort == 0 ? n : 0;
+        work[1] += sort == 2 ? n : 0;
+    });
+    scan(work, all_work, room, 0l, [](long a, long b) { return a + b; });
+    if (tid < 2) best[tid] = 1;
+    constexpr int SIZES = 6;
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+        if (all_work[y] == 0) continue;
+        const int places = y ? seats_block_places(kd.d) : seats_wave_places(kd.d);
+        int size[SIZES], items[SIZES], all[SIZES];
+#pragma unroll
+        for (int j = 0; j < SIZES; j++) {
+            const long tiles = (all_work[y] * kd.hkv * (8 + j * (j + 1) / 2) / 8 + places - 1) / places;   // 1, 1 1/8, 1 3/8, 1 3/4, 2 1/4, 2 7/8
+            size[j] = most(y ? SEAT_BLOCK_TILES : SEAT_WAVE_TILES, (int)(tiles < LOTS ? tiles : LOTS));
+            items[j] = 0;
+        }
+        each_set([&](int sort, int blocks, int tiles) __attribute__((always_inline)) {
+            if (sort == 2 * y)
+#pragma unroll
+                for (int j = 0; j < SIZES; j++) items[j] += blocks * seats_up(tiles, size[j]);
+        });
+        scan(items, all, room, 0, [](int a, int b) { return a + b; });
+        if (tid == 0) {
+            long cost = LONG_MAX;
+#pragma unroll
+            for (int j = 0; j < SIZES; j++) {
+                const long rounds = ((long)all[j] * kd.hkv + places - 1) / places, here = rounds * (size[j] + (y ? 4 : 12));   // (a workgroup's start and end are worth some tiles)
+                if (here < cost) {
+                    cost = here;
+                    best[y] = size[j];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int by_wave = best[0], by_block = best[1];
+    // ---- items of contents
+    for (int g = tid; g < G; g += LANES) {
+        int blocks, tiles;
+        const int sort = group_set(g, blocks, tiles), n = sort < 0 ? 0 : seats_up(tiles, sort ? by_block : by_wave);
+        cut[g] = n;
+        sums[0][g] = sort == 0 ? n * blocks : 0;
+        sums[1][g] = sort == 2 ? n * blocks : 0;
+    }
+    {
+        int* const a[2] = {sums[0], sums[1]};
+        running(a, G, room);
+    }
+    const int waves = sums[0][G], blocks_in_all = sums[1][G];
+    for (int i = tid; i < waves + blocks_in_all; i += LANES) {
+        const int y = i >= waves, x = y ? i - waves : i, size = y ? deep : 32;
+        const int g = find(sums[y], G, x), r = heads[g], c = content[r], j = x - sums[y][g];
+        int blocks, tiles;
+        group_set(g, blocks, tiles);
+        const int P = p.shared[3 * c], tok0 = first[r], T = first[heads[g + 1]] - tok0, kt = seats_up(P, PAGED_TILE) - tiles;
+        const int s = j / blocks, b = j - s * blocks, n = cut[g];
+        const int from = (int)((long)tiles * s / n), to = (int)((long)tiles * (s + 1) / n);
+        const SeatItem it = {tok0, T, size * b, s, 0, {}, {{p.shared[3 * c + 2], P, kt + from, to - from, most(0, P + high[g] - far + 1), P - 1, 0, 0}, {}}};
+        if (x < (y ? kd.room[2] : kd.room[0])) store(y ? kd.block : kd.wave, x, it);
+    }
+    __syncthreads();
+    // ---- of the seats' own keys; partial results
+    const auto pieces_of = [&](int r, int sort, int tiles) __attribute__((always_inline)) { return sort == 0 ? seats_up(tiles, by_wave) : sort == 2 ? seats_up(tiles, by_block) : 1; };
+    const auto parts_of = [&](int r, int sort, int pieces) __attribute__((always_inline)) {   // of each of its tokens
+        const int theirs = cut[of_group[r]];                                                  // (of a seat that reads its content itself: none)
+        return sort == 3 ? theirs : theirs + pieces > 1 ? theirs + pieces : 0;
+    };
+    each_seat([&](int r) __attribute__((always_inline)) {
+        int blocks, tiles, shared;
+        const int sort = seat_set(r, blocks, tiles, shared), n = sort < 0 ? 0 : pieces_of(r, sort, tiles + shared);
+#pragma unroll
+        for (int x = 0; x < 4; x++) sums[x][r] = sort == x ? n * blocks : 0;
+        sums[4][r] = sort < 0 ? 0 : seats_least(LOTS / 2, took[r] * parts_of(r, sort, n));
+    });
+    {
+        int* const a[5] = {sums[0], sums[1], sums[2], sums[3], sums[4]};
+        running(a, R, room);
+    }
+    each_seat([&](int r) __attribute__((always_inline)) {
+        int blocks, tiles, shared;
+        const int sort = seat_set(r, blocks, tiles, shared), parts = sort < 0 ? 0 : parts_of(r, sort, pieces_of(r, sort, tiles + shared));
+        kd.seat_parts[2 * r] = sums[4][r] | (sort == 3 || parts == 0 ? INT_MIN : 0);   // (the sign: no piece is left to be joined)
+        kd.seat_parts[2 * r + 1] = parts;
+        if (sort == 3 && sums[3][r] < kd.room[3]) {
+            const int L = stay[r] + 1, lo = most(0, stay[r] - far + 1), at = p.table_at + r * p.width, a = lo / p.page, b = (L - 1) / p.page;
+            int4* to = (int4*)(kd.last + sizeof(SeatLast) / 4 * (long)sums[3][r]);
+            int ids[SEAT_PAGES];
+#pragma unroll
+            for (int x = 0; x < SEAT_PAGES; x++) ids[x] = p.table[at + seats_least(a + x, b)];
+            to[0] = make_int4(first[r], L, lo, at);
+            to[1] = make_int4(sums[4][r], parts, ids[0], ids[1]);
+            to[2] = make_int4(ids[2], ids[3], ids[4], ids[5]);
+        }
+    });
+    if (tid == 0) {
+        kd.seat_parts[2 * R] = sums[4][R];
+        kd.counts[0] = waves + sums[0][R];
+        kd.counts[1] = sums[1][R];
+        kd.counts[2] = blocks_in_all + sums[2][R];
+        kd.counts[3] = sums[3][R];
+        kd.counts[4] = sums[4][R];
+    }
+    const int n0 = sums[0][R], n1 = sums[1][R], items = n0 + n1 + sums[2][R];
+    for (int i = tid; i < items; i += LANES) {
+        const int y = i < n0 ? 0 : i < n0 + n1 ? 1 : 2, j = y == 0 ? i : y == 1 ? i - n0 : i - n0 - n1;
+        const int r = find(sums[y], R, j), x = j - sums[y][r], n = took[r], L = stay[r] + n;
+        int blocks, tiles, shared;
+        seat_set(r, blocks, tiles, shared);
+        const int pieces = pieces_of(r, y, tiles + shared);
+        const int s = x / blocks, b = x - s * blocks, size = y == 2 ? deep : 32;
+        const int t0 = b * size / group, t1 = seats_least(n - 1, (b * size + size - 1) / group);   // its first and its last token
+        // tiles of the content, then of its own keys, that this block's rows see; the piece's share of them
+        const int c = content[r], P = shared ? p.shared[3 * c] : 0;
+        const int lo = most(0, stay[r] + t0 - far + 1), kt = lo / PAGED_TILE, own = seats_up(stay[r] + t1 + 1, PAGED_TILE) - kt;
+        const int lo2 = most(0, P + stay[r] + t0 - far + 1), kt2 = lo2 / PAGED_TILE, theirs = lo2 < P ? seats_up(P, PAGED_TILE) - kt2 : 0;
+        const int from = (int)((long)(own + theirs) * s / pieces), to = (int)((long)(own + theirs) * (s + 1) / pieces);
+        const SeatSpan mine = {p.table_at + r * p.width, L, kt + most(0, from - theirs), most(0, to - most(from, theirs)), most(0, stay[r] + t1 - far + 1), stay[r] + t0, 1, 0};
+        const int ahead = cut[of_group[r]];
+        SeatItem it = {first[r], n, b * size, ahead + s, ahead + pieces == 1, {}, {mine, {}}};
+        if (theirs > 0 && from < theirs) {
+            it.span[0] = {p.shared[3 * c + 2], P, kt2 + from, seats_least(to, theirs) - from, most(0, P + stay[r] + t1 - far + 1), P - 1, 0, 0};
+            it.span[1] = mine;
+        }
+        const int at = y == 0 ? waves + j : y == 1 ? j : blocks_in_all + j;
+        if (at < (y == 0 ? kd.room[0] : y == 1 ? kd.room[1] : kd.room[2])) store(y == 0 ? kd.wave : y == 1 ? kd.single : kd.block, at, it);
+    }
+    if (p.rows > SEATS_ROWS_AT_ONCE) return;
+    __syncthreads();
+    for (int row = tid; row <= p.rows; row += LANES) {
+        const int seat = row < total ? find(first, R, row) : 0;
+        place_parts(p, kd, row, total, seat, first[seat]);
     }
 }
 
@@ -571,8 +564,13 @@ extern "C" int spinf_seats_step(const spinf_seats_args* a, void* stream) {
     if (a->seats <= LANES) hipLaunchKernelGGL(seats_step_kernel<1>, dim3(1), dim3(LANES), 0, s, p);
     else hipLaunchKernelGGL(seats_step_kernel<SEATS_MOST / LANES>, dim3(1), dim3(LANES), 0, s, p);
     hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a->kinds) {
+        if (a->seats <= LANES) hipLaunchKernelGGL(seats_lists_kernel<LANES>, dim3(a->kinds), dim3(LANES), 0, s, p);
+        else hipLaunchKernelGGL(seats_lists_kernel<SEATS_MOST>, dim3(a->kinds), dim3(LANES), 0, s, p);
+        e = hipGetLastError();
+    }
     if (e == hipSuccess && a->rows > SEATS_ROWS_AT_ONCE) {
-        hipLaunchKernelGGL(seats_rows_kernel, dim3((unsigned)((a->rows + 255) / 256)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(seats_rows_kernel, dim3((unsigned)(a->rows / 256 + 1)), dim3(256), 0, s, p);
         e = hipGetLastError();
     }
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "seats_step: launch: %s", hipGetErrorString(e));

@@ -202,6 +202,8 @@ SHAPES = [
     ([90, 2000], [0, 0, 1, 1, 1, -1, 1, 1], [128, 129, 100, 7, 300, 64, 97, 500], [1, 1, 1, 2, 97, 1, 1, 49], 16, (16, 8, 128), 0),
     ([800], [0] * 70 + [-1], [90 + i for i in range(71)], [1] * 71, 16, (8, 1, 64), 120),
     ([3000], [0] * 20, [40] * 20, [7] * 20, 64, (16, 2, 256), 0),
+    ([64, 30], [0] * 600 + [1] * 450 + [-1] * 50, [1 + i % 37 for i in range(1100)], [int(i % 9 > 0) for i in range(1100)], 16, (2, 1, 64), 0),
+    ([97], [0] * 1050, [1 + i % 5 * 40 for i in range(1050)], [1] * 1050, 16, (12, 1, 64), 64),
 ]
 
 
