@@ -38,7 +38,7 @@ struct Params {
     const int* lists; const int* first; const int* pos; const int* counts; const int* parts;
     const SeatItem* wave; const SeatItem* single; const SeatItem* block; const SeatLast* last;
     float* part_o; float2* part_ml;
-    int hq, hkv, group, window, rows, seats;
+    int hq, hkv, group, window, rows, seats, last_blocks, join_x, join_y;
     int room[4];   // (the lists hold no more than they have room for, whatever their counts say)
     PageDiv page;
     Div by_group, by_heads;
@@ -54,6 +54,10 @@ __device__ __forceinline__ Item load_item(const SeatItem* items, int i) {
 __device__ __forceinline__ Span load_span(const SeatItem* items, int i, int which) {
     const int* p = (const int*)(items + i) + 8 + 8 * which;
     return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4), sload(p, 5), sload(p, 6)};
+}
+// (pins an item's loads where they are asked for: beside the list's count and not behind it.  There is room for an item of that index, whatever it holds.)
+__device__ __forceinline__ void asked(int count, const Item& a, const Span& b) {
+    asm volatile("" ::"s"(count), "s"(a.tok0), "s"(a.T), "s"(a.row0), "s"(a.piece), "s"(a.only), "s"(b.tab), "s"(b.L), "s"(b.kt0), "s"(b.tiles), "s"(b.flo), "s"(b.fhi), "s"(b.own));
 }
 __device__ __forceinline__ bool is_masked(const Span& s, int kt) { return kt * TK < s.flo || kt * TK + TK - 1 > s.fhi; }
 
@@ -264,7 +268,13 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
     char* const kb = lds + w * TILE;
     char* const vb = kb + GK::KTILEB;
     const unsigned k_at = lds_addr(kb), v_at = lds_addr(vb);
-    const int shared = seats_least(sload(p.counts, 0), p.room[0]) * p.hkv, alone = seats_least(sload(p.counts, 1), p.room[1]) * p.hkv;
+    // (the first item, if it is one for all waves)
+    const int first_unit = DV < D ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x, first_item = seats_least(p.by_heads.of(first_unit), p.room[0] - 1);
+    const int count = sload(p.counts, 0), singles = sload(p.counts, 1);
+    const Item item0 = load_item(p.wave, first_item);
+    const Span span0 = load_span(p.wave, first_item, 0);
+    asked(count, item0, span0);
+    const int shared = seats_least(count, p.room[0]) * p.hkv, alone = seats_least(singles, p.room[1]) * p.hkv;
     const int units = shared + (alone + NW - 1) / NW;
     const int last_unit = DV < D ? (units + 7) / 8 * 16 : units;
     for (int u = blockIdx.x; u < last_unit; u += gridDim.x) {
@@ -279,8 +289,9 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         if (single && x >= alone) continue;   // (waves of these items meet nowhere: only the last unit of a workgroup's walk has idle ones)
         const int item = p.by_heads.of(x), kvh = x - item * p.hkv;
         const SeatItem* const list = single ? p.single : p.wave;
-        const Item it = load_item(list, item);
-        const Span span = load_span(list, item, 0);
+        const bool known = !single && u == (int)blockIdx.x;
+        const Item it = known ? item0 : load_item(list, item);
+        const Span span = known ? span0 : load_span(list, item, 0);
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head + vcol * 2;
         const int step = single ? 1 : NW;
@@ -459,11 +470,14 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = H == 1 ? wave : wave & 3, half = H == 1 ? 0 : wave >> 2, vcol = half * DV;
     const unsigned base = lds_addr(lds) + half * HALF;
-    const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
-    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int most = p.room[2] * p.hkv;
+    for (int unit = blockIdx.x; unit < most; unit += gridDim.x) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
+        const int count = sload(p.counts, 2);
         const Item it = load_item(p.block, item);
         const Span span[2] = {load_span(p.block, item, 0), load_span(p.block, item, 1)};
+        asked(count, it, span[0]);
+        if (item >= count) return;
         const int tiles = span[0].tiles + span[1].tiles;
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head;
@@ -624,16 +638,29 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
 // four times as many waves run at a time, which is what hides the latency of so little (10,752 items of some nine keys of 256 dims: 95 us as tiles).
 // Probabilities stay 32-bit.  Then the pieces that the content's items left are added, and the row is written.
 template <int D, int RM, bool CAP>
-__global__ __launch_bounds__(256) void seats_last_kernel(const Params p) {
-    constexpr int LPK = D / 8, G = 64 / LPK, U = 8;   // lanes of a key, keys of a load, loads ahead
+__device__ __forceinline__ void last_words(const Params& p) {
+    constexpr int LPK = D / 8, G = 64 / LPK, U = 4;   // lanes of a key, keys of a load, loads ahead
     typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, mine = lane / LPK, col = lane % LPK * 8;
-    const int units = seats_least(sload(p.counts, 3), p.room[3]) * p.hkv;
-    for (int unit = blockIdx.x * 4 + w; unit < units; unit += gridDim.x * 4) {
+    // (an item is read a round ahead, the first one beside the count: there is room for it, whatever it holds)
+    struct Words { int w[12]; };
+    const auto load = [&](int unit) __attribute__((always_inline)) {
+        const int* ip = (const int*)(p.last + seats_least(p.by_heads.of(unit), p.room[3] - 1));
+        Words x;
+#pragma unroll
+        for (int i = 0; i < 12; i++) x.w[i] = sload(ip, i);
+        return x;
+    };
+    const int count = sload(p.counts, 3);
+    Words next = load(blockIdx.x * 4 + w);
+    asm volatile("" ::"s"(count), "s"(next.w[0]), "s"(next.w[4]), "s"(next.w[8]));
+    const int most = seats_least(count, p.room[3]) * p.hkv, stride = p.last_blocks * 4;
+    for (int unit = blockIdx.x * 4 + w; unit < most; unit += stride) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
-        const int* ip = (const int*)(p.last + item);
-        const int tok = sload(ip, 0), L = sload(ip, 1), lo = sload(ip, 2), tab = sload(ip, 3), part = sload(ip, 4), parts = sload(ip, 5);
-        const int page[SEAT_PAGES] = {sload(ip, 6), sload(ip, 7), sload(ip, 8), sload(ip, 9), sload(ip, 10), sload(ip, 11)};
+        const Words now = next;
+        if (unit + stride < most) next = load(unit + stride);
+        const int tok = now.w[0], L = now.w[1], lo = now.w[2], tab = now.w[3], part = now.w[4], parts = now.w[5];
+        const int page[SEAT_PAGES] = {now.w[6], now.w[7], now.w[8], now.w[9], now.w[10], now.w[11]};
         const int n = L - lo, page0 = p.page.of(lo >> 4), many = p.page.of((L - 1) >> 4) - page0 + 1;
         const char* const kb = p.k + kvh * p.k_head + col * 2;
         const char* const vb = p.v + kvh * p.v_head + col * 2;
@@ -743,28 +770,35 @@ __global__ __launch_bounds__(256) void seats_last_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------------------------------------ pieces joined
-// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per token and 64 dims of its heads (or some of them: blockIdx.y); 16 lanes hold a piece of
+// out = sum_s 2^(M_s - M*) O_s / sum_s 2^(M_s - M*) l_s over a row's pieces.  A workgroup per token and 64 dims of its heads (or some of them: y0); 16 lanes hold a piece of
 // a head, `share` such groups take a head's pieces in turn, each with a reference of its own, and are added up in one fixed order.
 template <int D>
-__global__ __launch_bounds__(256) void seats_join_kernel(const Params p) {
+__device__ __forceinline__ void join(const Params& p, int block) {
     constexpr int SLICES = D / 64, GROUPS = 16;
     __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
     __shared__ float2 part_ml[GROUPS];
-    const int tok = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
-    const int begin = sload(p.parts, tok), first = begin & INT_MAX, n = begin < 0 ? 0 : (sload(p.parts, tok + 1) & INT_MAX) - first;
-    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
+    const int sets = p.join_x * SLICES, y0 = block / sets, x0 = block - y0 * sets, slice = x0 % SLICES;
+    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, lane = threadIdx.x & 63, used = sload(p.first, p.seats);
+    for (int tok0 = x0 / SLICES; tok0 < p.rows; tok0 += 64 * p.join_x) {
+    // of 64 tokens of this workgroup: where their pieces begin, and how many there are (0: the last word is spoken)
+    const int at = tok0 + lane * p.join_x, begins = at < p.rows ? p.parts[at] : 0, ends = at < p.rows ? p.parts[at + 1] : 0;
+    const int number = at >= p.rows || begins < 0 ? 0 : (ends & INT_MAX) - begins;
+    unsigned long long left = __builtin_amdgcn_ballot_w64(number > 0 || (at >= used && at < p.rows));
+    while (left) {
+    const int which = __builtin_ctzll(left), tok = tok0 + which * p.join_x;
+    left &= left - 1;
+    const int first = __builtin_amdgcn_readlane(begins, which), n = __builtin_amdgcn_readlane(number, which);
     if (n == 0) {
-        if (tok < sload(p.first, p.seats)) return;   // the last word is spoken
-        for (int h = blockIdx.y * GROUPS + group; h < p.hq; h += gridDim.y * GROUPS) {
+        for (int h = y0 * GROUPS + group; h < p.hq; h += p.join_y * GROUPS) {
             *(uint2*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = make_uint2(0, 0);
             if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = -INFINITY;
         }
-        return;
+        continue;
     }
     int share = 1;   // (each group asks for four pieces at a time)
     while (share < GROUPS && share * 4 < n) share *= 2;
     const int heads = GROUPS / share, piece = group % share;
-    for (int h0 = blockIdx.y * heads; h0 < p.hq; h0 += gridDim.y * heads) {
+    for (int h0 = y0 * heads; h0 < p.hq; h0 += p.join_y * heads) {
         const int h = h0 + group / share;
         const bool on = h < p.hq;
         float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, total = 0.f;
@@ -808,14 +842,14 @@ __global__ __launch_bounds__(256) void seats_join_kernel(const Params p) {
             if (d == 0) part_ml[group] = make_float2(top, total);
             __syncthreads();
             if (piece == 0) {
-                const int used = n < share ? n : share;
+                const int shares = n < share ? n : share;
                 const float m0 = top, l0 = total;
-                for (int s = 1; s < used; s++) top = fmaxf(top, part_ml[group + s].x);
+                for (int s = 1; s < shares; s++) top = fmaxf(top, part_ml[group + s].x);
                 total = 0.f;
                 const float4 own = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
                 add(own, m0, l0, top);
-                for (int s = 1; s < used; s++) {
+                for (int s = 1; s < shares; s++) {
                     const float2 ml = part_ml[group + s];
                     add(*(const float4*)&part_sum[group + s][d], ml.x, ml.y, top);
                 }
@@ -830,33 +864,49 @@ __global__ __launch_bounds__(256) void seats_join_kernel(const Params p) {
             if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = log_sum(top, total);
         }
     }
+    }
+    }
 }
 
-constexpr int AT_ONCE = 2048;   // workgroups of a launch that walk a list
+// What comes behind the contents' and the own keys' pieces: workgroups ahead of `last_blocks` speak last words, the others join pieces (RM 0: only these).  One launch up to two heads; with
+// more the last words' registers would leave the others too few waves.
+template <int D, int RM, bool CAP>
+__global__ __launch_bounds__(256, RM == 0 ? 8 : RM == 2 ? 4 : 2) void seats_finish_kernel(const Params p) {
+    if constexpr (RM > 0) {
+        if (RM > 2 || (int)blockIdx.x < p.last_blocks) {
+            last_words<D, RM, CAP>(p);
+            return;
+        }
+    }
+    if constexpr (RM <= 2) join<D>(p, blockIdx.x - p.last_blocks);
+}
 
+// Workgroups that walk a list: two rounds of those that run at a time (one that finds nothing still takes a microsecond of a place)
 template <int D, int DV, int NW, bool CAP>
-int launch(const Params& p, const spinf_seats_attn_args* a, hipStream_t s) {
-    const auto grid = [](int64_t n) { return dim3((unsigned)std::min<int64_t>(n, AT_ONCE)); };
+int launch(Params p, const spinf_seats_attn_args* a, hipStream_t s) {
     hipError_t e = hipSuccess;
     if (a->rooms[2]) {
-        hipLaunchKernelGGL((seats_block_kernel<D, DV, CAP>), grid(a->rooms[2] * p.hkv), dim3(256 * (D / DV)), 0, s, p);
+        const int64_t units = std::min<int64_t>(a->rooms[2] * p.hkv, 2 * seats_block_places(D));
+        hipLaunchKernelGGL((seats_block_kernel<D, DV, CAP>), dim3((unsigned)units), dim3(256 * (D / DV)), 0, s, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
-        const int64_t units = a->rooms[0] * p.hkv + (a->rooms[1] * p.hkv + NW - 1) / NW;
-        hipLaunchKernelGGL((seats_wave_kernel<D, DV, NW, CAP>), grid(DV < D ? (units + 7) / 8 * 16 : units), dim3(64 * NW), 0, s, p);
-        e = hipGetLastError();
-    }
-    if (e == hipSuccess && a->rooms[3]) {   // (behind the contents' pieces, which it joins)
-        const dim3 n((unsigned)std::min<int64_t>((a->rooms[3] * p.hkv + 3) / 4, 2 * AT_ONCE));
-        if (p.group <= 2) hipLaunchKernelGGL((seats_last_kernel<D, 2, CAP>), n, dim3(256), 0, s, p);
-        else if (p.group <= 4) hipLaunchKernelGGL((seats_last_kernel<D, 4, CAP>), n, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((seats_last_kernel<D, 8, CAP>), n, dim3(256), 0, s, p);
+        const int64_t units = std::min<int64_t>(a->rooms[0] * p.hkv + (a->rooms[1] * p.hkv + NW - 1) / NW, 2 * seats_wave_places(D));
+        hipLaunchKernelGGL((seats_wave_kernel<D, DV, NW, CAP>), dim3((unsigned)(DV < D ? (units + 7) / 8 * 16 : units)), dim3(64 * NW), 0, s, p);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
-        const int y = p.rows * (D / 64) >= 1024 ? 1 : std::min(p.hq, (1024 + p.rows * (D / 64) - 1) / (p.rows * (D / 64)));
-        hipLaunchKernelGGL((seats_join_kernel<D>), dim3((unsigned)(p.rows * (D / 64)), (unsigned)y), dim3(256), 0, s, p);
+        p.last_blocks = (int)std::min<int64_t>((a->rooms[3] * p.hkv + 3) / 4, p.group <= 2 ? 1024 : 512);   // (as many waves as run at a time)
+        p.join_x = std::min(p.rows, 4096 / (D / 64));
+        const int x = p.join_x * (D / 64);
+        p.join_y = x >= 1024 ? 1 : std::min(p.hq, (1024 + x - 1) / x);
+        if (p.last_blocks && p.group <= 2) hipLaunchKernelGGL((seats_finish_kernel<D, 2, CAP>), dim3((unsigned)(p.last_blocks + x * p.join_y)), dim3(256), 0, s, p);
+        else {
+            if (p.last_blocks && p.group <= 4) hipLaunchKernelGGL((seats_finish_kernel<D, 4, CAP>), dim3((unsigned)p.last_blocks), dim3(256), 0, s, p);
+            else if (p.last_blocks) hipLaunchKernelGGL((seats_finish_kernel<D, 8, CAP>), dim3((unsigned)p.last_blocks), dim3(256), 0, s, p);
+            p.last_blocks = 0;
+            hipLaunchKernelGGL((seats_finish_kernel<D, 0, CAP>), dim3((unsigned)(x * p.join_y)), dim3(256), 0, s, p);
+        }
         e = hipGetLastError();
     }
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "seats_attn: launch: %s", hipGetErrorString(e));

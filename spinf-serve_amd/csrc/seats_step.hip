@@ -386,7 +386,8 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
             long cost = LONG_MAX;
 #pragma unroll
             for (int j = 0; j < SIZES; j++) {
-                const long rounds = ((long)all[j] * kd.hkv + places - 1) / places, here = rounds * (size[j] + (y ? 4 : 12));   // (a workgroup's start and end are worth some tiles)
+                // (a workgroup's start and end are worth some tiles; what a piece leaves, written and read again, a 24th of a tile's time over the whole GPU)
+                const long n = (long)all[j] * kd.hkv, rounds = (n + places - 1) / places, here = 24 * rounds * (size[j] + (y ? 4 : 12)) + (y ? n : n / 4);
                 if (here < cost) {
                     cost = here;
                     best[y] = size[j];
