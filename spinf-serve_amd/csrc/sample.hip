@@ -479,13 +479,16 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
 }
 
 // The least number up to which (it counted in) those of `each` hold at least `need` in all; ~0: all of them hold less.  each(f) calls f(number, worth) for every one in question,
-// each lane for its share; all of them lie in low .. high.  Eight bits at a time, from the first that differs.
+// each lane for its share; all of them are `some` but for bits of `mask`.  Eight bits at a time, from the first that differs; bits that never do are passed over.
 template <class E>
-__device__ u64 search(u64 need, u64 low, u64 high, u64* sums, int* counts, u64* found, E each) {
-    int above = low == high ? 0 : 64 - __builtin_clzll(low ^ high);   // bits in question
-    u64 prefix = low;
+__device__ u64 search(u64 need, u64 some, u64 mask_all, u64* sums, int* counts, u64* found, E each) {
+    int above = 64;
+    u64 prefix = some;
     bool first = true;
-    while (above > 0 || first) {
+    while (true) {
+        const u64 open = above < 64 ? mask_all & ((1ull << above) - 1) : mask_all;
+        if (open == 0 && !first) break;
+        above = open ? 64 - __builtin_clzll(open) : 0;
         const int shift = above > 8 ? above - 8 : 0;
         __syncthreads();
         if (threadIdx.x < 256) {
@@ -524,7 +527,7 @@ __device__ u64 search(u64 need, u64 low, u64 high, u64* sums, int* counts, u64* 
         const u64 digit = found[0];
         if (digit == ~0ull) return ~0ull;   // (of the first digit alone)
         need = found[1];
-        prefix = (prefix & mask) | digit << shift;
+        prefix = (prefix & ~(((1ull << (above - shift)) - 1) << shift)) | digit << shift;
         above = shift;
         first = false;
         if (shift && counts[digit] == 1) {   // the rest of its digits
@@ -583,7 +586,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         else {
             const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
             const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
-            u64 low = ~0ull, high = 0;
+            u64 some = 0, differ = 0;
             for (int c = tid >> 6; c < p.chunks; c += WAVES)
                 for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
                     const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
@@ -591,13 +594,44 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                     const float v = unordered(y.x);
                     listed[i] = x;
                     worth[i] = units(v == r.top ? 1.0 : r.top == INFINITY ? 0.0 : power(((double)v - (double)r.top) * h.by_two));
-                    low = std::min(low, x);
-                    high = std::max(high, x);
                 }
-            low = over_all(low, room, [](u64 a, u64 b) { return a < b ? a : b; });
-            high = over_all(high, room, [](u64 a, u64 b) { return a > b ? a : b; });
+            __syncthreads();
+            if (n > 128) {
+                some = listed[0];
+                for (int i = tid; i < n; i += LANES) differ |= listed[i] ^ some;
+                differ = over_all(differ, room, [](u64 a, u64 b) { return a | b; });
+            }
+            if (n <= 128) {   // each token counted against all
+                const u64 x = tid < n ? listed[tid] : ~0ull, w = tid < n ? worth[tid] : 0;
+                if (tid == 0) found[0] = found[1] = ~0ull;
+                __syncthreads();
+                if (r.kth < BINS) {
+                    const bool on = tid < n && bin(x) == r.kth;
+                    int before = 0;
+                    if (tid < n)
+                        for (int i = 0; i < n; i++) before += listed[i] < x;
+                    // (those of other bins come before or behind all of the kth)
+                    const int ahead = over_all(on ? before : INT_MAX, room_n, [](int a, int b) { return a < b ? a : b; });
+                    if (on && before - ahead == h.k - r.before_k - 1) found[0] = x;
+                    __syncthreads();
+                    last = found[0];
+                }
+                if (r.by_mass) {
+                    u64 before = 0;
+                    const bool on = tid < n && x <= last && (h.few || bin(x) <= r.to);
+                    if (tid < n)
+                        for (int i = 0; i < n; i++) before += listed[i] < x ? worth[i] : 0;
+                    double all = r.sum;   // weight of the first k
+                    if (r.kth < BINS || h.few) all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(tid < n && x <= last && (h.few || bin(x) == r.kth) ? w : 0, room);
+                    const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
+                    const u64 least_of = need < 1.0 ? 1 : (u64)need;
+                    if (on && before < least_of && before + w >= least_of) found[1] = x;
+                    __syncthreads();
+                    last = std::min(last, found[1]);
+                }
+            } else {
             if (r.kth < BINS)
-                last = search(h.k - r.before_k, low, high, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                last = search(h.k - r.before_k, some, differ, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
                     for (int i = tid; i < n; i += LANES)
                         if (bin(listed[i]) == r.kth) f(listed[i], 1);
                 });
@@ -610,10 +644,11 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                     all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(w, room);
                 }
                 const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
-                last = std::min(last, search(need < 1.0 ? 1 : (u64)need, low, high, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
+                last = std::min(last, search(need < 1.0 ? 1 : (u64)need, some, differ, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
                     for (int i = tid; i < n; i += LANES)
                         if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to)) f(listed[i], worth[i]);
                 }));
+            }
             }
             // what is kept, by chunk
             if (tid < p.chunks) chunks[tid] = own_kept;

@@ -236,20 +236,20 @@ __device__ void slow_row(const Params& p, const Item& it, const Span* spans, int
 
 // eight dims of a row, as the last word or as a piece
 template <int D>
-__device__ __forceinline__ void put8(const Params& p, const Item& it, int tok, int head, int d, const float (&x)[8]) {
+__device__ __forceinline__ void put8(const Params& p, const Item& it, int tok, int head, int begin, int d, const float (&x)[8]) {
     if (it.only) {
         bf16x8 y;
 #pragma unroll
         for (int k = 0; k < 8; k++) y[k] = (__bf16)x[k];
         *(bf16x8*)(p.out + (long)tok * p.o_tok + (long)head * p.o_head + d) = y;
     } else {
-        float* dst = p.part_o + part_of(p, it, tok, head) * D + d;
+        float* dst = p.part_o + ((long)(begin + it.piece) * p.hq + head) * D + d;
         *(float4*)dst = make_float4(x[0], x[1], x[2], x[3]);
         *(float4*)(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
 }
-__device__ __forceinline__ void put_sum(const Params& p, const Item& it, int tok, int head, float M, float sum) {
-    if (!(it.only)) p.part_ml[part_of(p, it, tok, head)] = make_float2(M, sum);
+__device__ __forceinline__ void put_sum(const Params& p, const Item& it, int tok, int head, int begin, float M, float sum) {
+    if (!it.only) p.part_ml[(long)(begin + it.piece) * p.hq + head] = make_float2(M, sum);
     else if (p.lse) p.lse[(long)tok * p.hq + head] = log_sum(M, sum);
 }
 
@@ -263,6 +263,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
     constexpr int TILE = GK::KTILEB + GV::VTILEB > 32 * OROW * 4 ? GK::KTILEB + GV::VTILEB : 32 * OROW * 4;   // a wave's rows take the place of its tile
     __shared__ __attribute__((aligned(16))) char lds[NW * TILE];
     __shared__ float2 ml[NW][32];
+    __shared__ int part_of_row[NW][32];   // where the rows' pieces begin
     constexpr int NK = GK::NREG, NV = GV::NREG;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* const kb = lds + w * TILE;
@@ -310,6 +311,10 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             }
             rows.load(p, it, span, kvh, it.row0);
             rows.reset();
+            if (rows.g == 0 && !it.only) {   // (asked for here: at the end they would be one more wait for memory)
+                const int N = it.T * p.group, row = it.row0 + rows.m;
+                part_of_row[w][rows.m] = p.parts[it.tok0 + p.by_group.of(row < N ? row : N - 1)] & INT_MAX;
+            }
             while (kt < end) {
                 const bool masked = is_masked(span, kt), next = kt + step < end;
                 seen_mask |= masked;
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
                 if (rows.g == 0 && vcol == 0) {
                     int tok, head;
                     token_head(p, it, kvh, it.row0 + rows.m, tok, head);
-                    put_sum(p, it, tok, head, rows.M, sum);
+                    put_sum(p, it, tok, head, part_of_row[w][rows.m], rows.M, sum);
                 }
             }
             __builtin_amdgcn_wave_barrier();   // (LDS operations of a wave are done in order)
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
                 float y[8];
 #pragma unroll
                 for (int k = 0; k < 8; k++) y[k] = mine[j * OROW + d + k];
-                put8<D>(p, it, tok, head, vcol + d, y);
+                put8<D>(p, it, tok, head, part_of_row[w][j], vcol + d, y);
             }
             __builtin_amdgcn_s_waitcnt(LGKM0);   // (the next item's tile comes here)
             __builtin_amdgcn_sched_barrier(0);
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             if (w == 0 && rows.g == 0 && vcol == 0) {
                 int tok, head;
                 token_head(p, it, kvh, it.row0 + rows.m, tok, head);
-                put_sum(p, it, tok, head, state.x, state.y);
+                put_sum(p, it, tok, head, part_of_row[w][rows.m], state.x, state.y);
             }
         }
         __syncthreads();
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             for (int z = 1; z < NW; z++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) y[k] += stage[(z * 32 + j) * OROW + d + k];
-            put8<D>(p, it, tok, head, vcol + d, y);
+            put8<D>(p, it, tok, head, part_of_row[w][j], vcol + d, y);
         }
         __syncthreads();   // (the next item's tiles come here)
     }
@@ -470,14 +475,11 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = H == 1 ? wave : wave & 3, half = H == 1 ? 0 : wave >> 2, vcol = half * DV;
     const unsigned base = lds_addr(lds) + half * HALF;
-    const int most = p.room[2] * p.hkv;
-    for (int unit = blockIdx.x; unit < most; unit += gridDim.x) {
+    const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
-        const int count = sload(p.counts, 2);
         const Item it = load_item(p.block, item);
         const Span span[2] = {load_span(p.block, item, 0), load_span(p.block, item, 1)};
-        asked(count, it, span[0]);
-        if (item >= count) return;
         const int tiles = span[0].tiles + span[1].tiles;
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head;
