@@ -45,11 +45,16 @@ struct Params {
     SoftCap cap;
 };
 
-struct Item { int tok0, T, row0, piece, only; };
+struct Item { int tok0, T, row0, piece, only, N; };   // N: rows of the set that lie in the call's tensors
 struct Span { int tab, L, kt0, tiles, flo, fhi, own; };
 __device__ __forceinline__ Item load_item(const SeatItem* items, int i) {
     const int* p = (const int*)(items + i);
-    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4)};
+    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4), 0};
+}
+// (a step of more rows than the call's tensors have does not go with them: whatever it left, no row outside them is touched)
+__device__ __forceinline__ bool bound(Item& it, int rows, int group) {
+    it.N = seats_least(it.T, rows - it.tok0) * group;
+    return it.row0 < it.N;
 }
 __device__ __forceinline__ Span load_span(const SeatItem* items, int i, int which) {
     const int* p = (const int*)(items + i) + 8 + 8 * which;
@@ -110,7 +115,7 @@ struct Rows : RowTile<D, DV, CAP> {
     int lo, hi;
 
     __device__ __forceinline__ void see(const Params& p, const Item& it, const Span& s, int row0) {
-        const int N = it.T * p.group, row = row0 + (lane_now() & 31), r = row < N ? row : N - 1;
+        const int row = row0 + (lane_now() & 31), r = row < it.N ? row : it.N - 1;
         interval(p, it, s, p.by_group.of(r), lo, hi);
     }
     // queries of rows row0 + m, dims col ..
@@ -118,7 +123,7 @@ struct Rows : RowTile<D, DV, CAP> {
         lane = threadIdx.x & 63;
         m = lane & 31;
         g = lane >> 5;
-        const int N = it.T * p.group, row = row0 + m, r = row < N ? row : N - 1;
+        const int row = row0 + m, r = row < it.N ? row : it.N - 1;
         const int tok = p.by_group.of(r), head = kvh * p.group + (r - tok * p.group);
         const __bf16* qp = p.q + (long)(it.tok0 + tok) * p.q_tok + (long)head * p.q_head + col + 8 * g;
 #pragma unroll
@@ -291,7 +296,8 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         const int item = p.by_heads.of(x), kvh = x - item * p.hkv;
         const SeatItem* const list = single ? p.single : p.wave;
         const bool known = !single && u == (int)blockIdx.x;
-        const Item it = known ? item0 : load_item(list, item);
+        Item it = known ? item0 : load_item(list, item);
+        if (!bound(it, p.rows, p.group)) continue;
         const Span span = known ? span0 : load_span(list, item, 0);
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head + vcol * 2;
@@ -312,8 +318,8 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             rows.load(p, it, span, kvh, it.row0);
             rows.reset();
             if (rows.g == 0 && !it.only) {   // (asked for here: at the end they would be one more wait for memory)
-                const int N = it.T * p.group, row = it.row0 + rows.m;
-                part_of_row[w][rows.m] = p.parts[it.tok0 + p.by_group.of(row < N ? row : N - 1)] & INT_MAX;
+                const int row = it.row0 + rows.m;
+                part_of_row[w][rows.m] = p.parts[it.tok0 + p.by_group.of(row < it.N ? row : it.N - 1)] & INT_MAX;
             }
             while (kt < end) {
                 const bool masked = is_masked(span, kt), next = kt + step < end;
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
                 kt += step;
             }
         }
-        const int left = it.T * p.group - it.row0, here = left < 32 ? left : 32;
+        const int left = it.N - it.row0, here = left < 32 ? left : 32;
         const float sum = lane32_sum(rows.l);
         if (sum == 0.f) rows.M = -INFINITY;   // no key seen
         constexpr int PIECES = DV / 8;
@@ -478,7 +484,8 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
-        const Item it = load_item(p.block, item);
+        Item it = load_item(p.block, item);
+        if (!bound(it, p.rows, p.group)) continue;
         const Span span[2] = {load_span(p.block, item, 0), load_span(p.block, item, 1)};
         const int tiles = span[0].tiles + span[1].tiles;
         const char* const k_base = p.k + kvh * p.k_head;
@@ -518,7 +525,7 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
         // keys of tile i behind its first one
         const auto behind = [&](int i) __attribute__((always_inline)) { return i < span[0].tiles ? span[0].L - 1 - (span[0].kt0 + i) * TK : span[1].L - 1 - (span[1].kt0 + i - span[0].tiles) * TK; };
         if (tiles > 0) issue(0, behind(0), 0);   // (ahead of the queries: their latencies pass together)
-        if (it.row0 + 32 * w >= it.T * p.group) {   // a wave without rows brings its share of the tiles
+        if (it.row0 + 32 * w >= it.N) {   // a wave without rows brings its share of the tiles
             for (int i = 0, j = 0, buf = 0; i < tiles; i++, buf ^= 1) {
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
                 __syncthreads();
@@ -578,7 +585,7 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
             rows.softmax(p.cap, s, pb);
             rows.values(kb + GK::KTILEB, pb);
         }
-        const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
+        const int left = it.N - it.row0 - 32 * w;   // rows from this wave's first on
         const int live = seats_least(4, seats_up(left + 32 * w, 32));   // waves that have rows
         const float sum = lane32_sum(rows.l);
         if (sum == 0.f) rows.M = -INFINITY;   // no key seen
@@ -663,6 +670,7 @@ __device__ __forceinline__ void last_words(const Params& p) {
         if (unit + stride < most) next = load(unit + stride);
         const int tok = now.w[0], L = now.w[1], lo = now.w[2], tab = now.w[3], part = now.w[4], parts = now.w[5];
         const int page[SEAT_PAGES] = {now.w[6], now.w[7], now.w[8], now.w[9], now.w[10], now.w[11]};
+        if (tok >= p.rows) continue;
         const int n = L - lo, page0 = p.page.of(lo >> 4), many = p.page.of((L - 1) >> 4) - page0 + 1;
         const char* const kb = p.k + kvh * p.k_head + col * 2;
         const char* const vb = p.v + kvh * p.v_head + col * 2;

@@ -50,6 +50,7 @@ class PagedSeats:
         self.lens, self.took, self.first, self.left, self.free = part("lens", R), part("took", R), part("first", R + 1), part("left", 1), part("free", pool)
         self.table = part("table", R * -(-keys // page)).view(R, -1)
         self.seats, self.rows, self.page, self.keys = R, rows, page, keys
+        self._now = rows    # rows of the last step
         self._calls = {}
         self._shared = None
         if state.is_cuda:
@@ -143,10 +144,14 @@ class PagedSeats:
             self._shared.reach(on)
         return on
 
-    def step(self, new, drop=None):
+    def step(self, new, drop=None, rows=None):
         """First the last drop[r] own keys of every seat go (drop None: none; as many as there are at most: a large number empties the seat) and pages that hold none any more are free
         again; then new[r] tokens come to seat r (below 1: none), with the pages they need.  A seat gets all of its tokens or none: none where they would pass ``keys``, where what the seats up to it
-        ask for is more than ``rows`` rows, or more pages than are free (`took` says).  new, drop: [seats] int32 on the device.  -> slots, pos (the seats' own tensors)"""
+        ask for is more than ``rows`` rows, or more pages than are free (`took` says).  new, drop: [seats] int32 on the device.  rows: of this step's tensors, at most the seats' (None: as many).
+        -> slots, pos [rows] (of the seats' own tensors)"""
+        n = self.rows if rows is None else _whole(rows, "PagedSeats.step: rows")
+        if not 1 <= n <= self.rows:
+            raise ValueError(f"PagedSeats.step: {n} rows, the seats were built for up to {self.rows}")
         self._check(new, "new")
         if drop is not None:
             self._check(drop, "drop")
@@ -154,12 +159,13 @@ class PagedSeats:
             raise RuntimeError("PagedSeats.step runs on ROCm device tensors only (no CPU path)")
         if _lib.eager(self._state, new, drop):
             a = _lib.SeatsArgs.from_buffer_copy(self._args)
-            a.come, a.drop = new.data_ptr(), drop.data_ptr() if drop is not None else None
+            a.come, a.drop, a.rows = new.data_ptr(), drop.data_ptr() if drop is not None else None, n
             _lib.launch(_lib.load_library().spinf_seats_step, a, self.device, "seats_step", self._reach())
         else:
             self._reach()
-            _step_op(self._state, self._work, self.slots, self.pos, self.content, new, drop, self._geo)
-        return self.slots, self.pos
+            _step_op(self._state, self._work, self.slots, self.pos, self.content, new, drop, self._geo, n)
+        self._now = n
+        return (self.slots, self.pos) if n == self.rows else (self.slots[:n], self.pos[:n])
 
     def _check(self, t, what):
         if t.dtype != torch.int32 or t.shape != (self.seats,) or not t.is_contiguous():
@@ -222,10 +228,11 @@ def _step_args(state, work, slots, pos, content, geo):
     return a
 
 
-def _step(state: torch.Tensor, work: torch.Tensor, slots: torch.Tensor, pos: torch.Tensor, content: torch.Tensor, new: torch.Tensor, drop: Optional[torch.Tensor], geo: list[int]) -> None:
+def _step(state: torch.Tensor, work: torch.Tensor, slots: torch.Tensor, pos: torch.Tensor, content: torch.Tensor, new: torch.Tensor, drop: Optional[torch.Tensor], geo: list[int],
+          rows: int) -> None:
     _lib.same_device(state.device, work, slots, pos, content, new, drop)
     a = _step_args(state, work, slots, pos, content, geo)
-    a.come, a.drop = new.data_ptr(), drop.data_ptr() if drop is not None else None
+    a.come, a.drop, a.rows = new.data_ptr(), drop.data_ptr() if drop is not None else None, rows
     _lib.launch(_lib.load_library().spinf_seats_step, a, state.device, "seats_step")
 
 
@@ -233,7 +240,7 @@ _step_op = torch.library.custom_op("spinf::seats_step", _step, mutates_args=("st
 
 
 @_step_op.register_fake
-def _(state, work, slots, pos, content, new, drop, geo):
+def _(state, work, slots, pos, content, new, drop, geo, rows):
     return None
 
 
@@ -250,7 +257,7 @@ def _attn_block(q, k, v, state, work, pos, geo, index, scale, softcap):
     _point(a.kind, work, lay["lists"][index])
     for i, n in enumerate(_rooms(geo, index)):
         a.rooms[i] = n
-    a.rows, a.seats, a.page, a.scale, a.softcap = geo[1], geo[0], geo[2], scale, softcap
+    a.rows, a.seats, a.page, a.scale, a.softcap = q.shape[0], geo[0], geo[2], scale, softcap
     return a
 
 
@@ -296,7 +303,7 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     if eager:   # a later layer or step: everything but the tensors' memory was settled by the first
         key = (q.shape, q.stride(), q.dtype, k.shape, k.stride(), v.stride(), scale, window, softcap)
         got = seats._calls.get(key)
-        if got is not None and q.device == seats.device == k.device and not q.data_ptr() % 16:
+        if got is not None and q.shape[0] == seats._now and q.device == seats.device == k.device and not q.data_ptr() % 16:
             out, lse = _attn_run(_lib.SeatsAttnArgs.from_buffer_copy(got), q, k, v, return_lse, seats._reach())
             return (out, lse) if return_lse else out
     w = _whole(window, "window") if window is not None else 0
@@ -305,8 +312,8 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     w = min(w, LONGEST)
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("seats_attn: q must be bf16 [rows, query heads, head dim] with contiguous head dims")
-    if q.shape[0] != seats.rows:
-        raise ValueError(f"seats_attn: a step has {seats.rows} rows, q {q.shape[0]}")
+    if q.shape[0] != seats._now:
+        raise ValueError(f"seats_attn: the last step has {seats._now} rows, q {q.shape[0]}")
     if (q.shape[1], k.shape[2], q.shape[2], w) not in seats.heads or q.shape[2] != k.shape[3]:
         raise ValueError(f"seats_attn: {q.shape[1]} query heads on {k.shape[2]} of {q.shape[2]} dims (the cache: {k.shape[3]}), window {w}: the seats were built for {seats.heads}")
     if k.shape[1] != seats.page:
