@@ -46,7 +46,7 @@ struct Params {
     const void* logits; long ld; int vocab, rows, chunks; bool aligned;
     const void* u; bool u_f64;
     const float *temperature, *top_p, *min_p; const int* top_k;
-    float all_temperature, all_top_p, all_min_p; int all_top_k;
+    float all_temperature, all_top_p, all_min_p; int all_top_k; double all_inv;   // (1 / T of all: a division of 64 bits is a tenth of a chunk's work)
     long* token; float* prob;
     Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
 };
@@ -60,7 +60,7 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
     h.k = p.top_k ? p.top_k[row] : p.all_top_k;
     h.wrong = !(T >= 0.f) || !(h.p >= 0.f) || !(h.least >= 0.f);
     h.best = T == 0.f;
-    h.inv = 1.0 / (double)T;
+    h.inv = p.temperature ? 1.0 / (double)T : p.all_inv;
     h.by_two = h.inv * 1.4426950408889634;
     h.scale = fminf(BINS_PER_UNIT / T, 3e38f);
     h.far = 60.f * T;
@@ -98,32 +98,46 @@ __device__ __forceinline__ double power(double t) {
     for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, c[k]);
     return __longlong_as_double(__double_as_longlong(y) + ((long long)(int)__double_as_longlong(whole) << 52));
 }
-// The same for a chunk's logits, where instructions of 64 bits are what bounds the kernel (each takes two of 32 bits): t in 32nds, the whole ones by a table of 2^(j / 32) in LDS and the
-// exponent, the rest by a polynomial of degree 4 through the Chebyshev points of -1/2 .. 1/2: off by 2^-43 of the weight at most, either way.  (With the series above 320 rows of
-// 262,144 logits took 120 us, with the library's exp 195.)
-constexpr int STEPS = 32;
+// The same for a chunk's logits, where instructions of 64 bits are what bounds the kernel (each takes two of 32 bits).  With t = x / (T ln 2) in 256ths and B the whole number next to the
+// largest logit's t: n = round(t) - B and what is left of t come of one product-and-sum each, exact but for the last bits; 2^(n / 256) by a table in LDS and the exponent, the rest by a
+// polynomial of degree 3 through the Chebyshev points of -1/2 .. 1/2 (off by 2^-45.7 at most), whose coefficients hold what the largest logit's own t is off from B: it weighs 1 to
+// 2^-44.  (320 rows of 262,144 logits: 90 us in all.  With differences from the largest logit, 32nds and degree 4 99, with the series above 120, with the library's exp 195.)
+constexpr int STEPS = 256;
+struct Steps { double of[STEPS]; };
+constexpr Steps make_steps() {   // 2^(j / 256) by its series, the smallest terms first
+    Steps s = {};
+    for (int j = 0; j < STEPS; j++) {
+        double term[18] = {1.0}, y = 0.0;
+        for (int k = 1; k < 18; k++) term[k] = term[k - 1] * (j * (0.69314718055994530942 / STEPS) / k);
+        for (int k = 17; k >= 0; k--) y += term[k];
+        s.of[j] = y;
+    }
+    return s;
+}
+__constant__ const Steps all_steps = make_steps();
 __device__ __forceinline__ void fill_steps(double* steps) {
-    if (threadIdx.x < STEPS) steps[threadIdx.x] = 2.0 * power(threadIdx.x / (double)STEPS - 1.0);
+    static_assert(STEPS <= LANES, "one a lane");
+    if (threadIdx.x < STEPS) steps[threadIdx.x] = all_steps.of[threadIdx.x];
 }
 struct Weights {   // of a chunk, by its largest logit
-    const double* steps; double top, by_step; float low;
-    double c1, c2, c3, c4;
-    __device__ __forceinline__ Weights(const double* steps, float top, const How& h) : steps(steps), top(top), by_step(h.by_two * STEPS), low(fminf(top - h.far, nextafterf(top, -INFINITY))), c1(0.02166084939172217), c2(0.0002345961981994449), c3(1.6938633903155644e-06), c4(9.172607532092245e-09) {
-        asm("" : "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4));   // (pinned to scalar registers: left alone, the compiler moves each into vector registers in front of every product)
+    const double* steps; double by_step, magic; float low;
+    double c0, c1, c2, c3;
+    __device__ __forceinline__ Weights(const double* steps, float top, const How& h) : steps(steps), by_step(h.by_two * STEPS), low(fminf(top - h.far, nextafterf(top, -INFINITY))) {
+        const double B = __builtin_rint(top * by_step), g = part(__builtin_fma(-(double)top, by_step, B), C0, C1, C2, C3);
+        magic = 0x1.8p52 - B;
+        c0 = g * C0; c1 = g * C1; c2 = g * C2; c3 = g * C3;
     }
-    // (where the next number below the largest lies hundreds of T away, the exponent would not hold its weight)
-    static __device__ __forceinline__ bool fits(float top, const How& h) { return top < INFINITY && h.plain && top - nextafterf(top, -INFINITY) <= 8.f * h.far; }
-    // exp((x - top) / T) to 2^-43 of it; of what lies some 60 T and more below, and of NaN: less than 2^-70
+    // (where the next number below the largest lies hundreds of T away, the exponent would not hold its weight; beyond 2^30 steps the whole number its place)
+    static __device__ __forceinline__ bool fits(float top, const How& h) { return h.plain && fabs(top * (h.by_two * STEPS)) < 0x1p30 && top - nextafterf(top, -INFINITY) <= 8.f * h.far; }
+    // exp((x - top) / T) to 2^-44 of it; of what lies some 60 T and more below, and of NaN: less than 2^-70
     __device__ __forceinline__ double of(float x) const {
-        const double t = ((double)fmaxf(x, low) - top) * by_step;
-        const double whole = t + 0x1.8p52, f = t - (whole - 0x1.8p52);
+        const double t = fmaxf(x, low), whole = __builtin_fma(t, by_step, magic), f = __builtin_fma(t, by_step, magic - whole);
         const int n = (int)__double_as_longlong(whole);
-        double y = __builtin_fma(c4, f, c3);
-        y = __builtin_fma(y, f, c2);
-        y = __builtin_fma(y, f, c1);
-        y = __builtin_fma(y, f, 1.0) * steps[n & (STEPS - 1)];
-        return __hiloint2double(__double2hiint(y) + ((n & ~(STEPS - 1)) << 15), __double2loint(y));   // (n / 32 into the exponent)
+        const double y = part(f, c0, c1, c2, c3) * steps[n & (STEPS - 1)];
+        return __hiloint2double(__double2hiint(y) + ((n & ~(STEPS - 1)) << 12), __double2loint(y));   // (n / 256 into the exponent)
     }
+    static __device__ __forceinline__ double part(double f, double c0, double c1, double c2, double c3) { return __builtin_fma(__builtin_fma(__builtin_fma(c3, f, c2), f, c1), f, c0); }
+    static constexpr double C0 = 0.9999999999999825, C1 = 0.0027076061740622767, C2 = 3.6655661567589336e-06, C3 = 3.308302983711395e-09;
 };
 // exp((x - top) / T); where the largest are infinite, only they have a weight
 __device__ __forceinline__ double weight(float x, float top, double by_two) { return x == top ? 1.0 : top == INFINITY || x == -INFINITY ? 0.0 : power(((double)x - (double)top) * by_two); }
@@ -206,11 +220,11 @@ __device__ __forceinline__ T scan_all(T x, T* room, T& total) {
     return before + x;
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
+template <bool BF16, bool FILTERS>   // FILTERS: some row may have one (without, fewer registers: 4 workgroups to a CU where it would be 3)
+__global__ __launch_bounds__(LANES, FILTERS ? 6 : 8) void sample_chunks_kernel(const Params p) {
     __shared__ u64 room[WAVES];
-    __shared__ u64 weights[BINS];
-    __shared__ int numbers[BINS];
+    __shared__ u64 weights[FILTERS ? BINS : 1];
+    __shared__ int numbers[FILTERS ? BINS : 1];
     __shared__ double steps[STEPS];
     const int chunk = blockIdx.x, row = blockIdx.y;
     const How h = settings(p, row);
@@ -236,7 +250,7 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
     }
-    if (!h.filtered) {
+    if (!FILTERS || !h.filtered) {
         double sum = 32.0;   // (16 weights of at most 1 leave it below 64: it counts in units of 2^-47)
         if (Weights::fits(top, h)) {
             const Weights w(steps, top, h);
@@ -250,6 +264,7 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
         if (threadIdx.x == 0) p.stat[at] = s;
         return;
     }
+    if constexpr (FILTERS) {
     if (threadIdx.x < BINS) {
         weights[threadIdx.x] = 0;
         numbers[threadIdx.x] = 0;
@@ -296,6 +311,7 @@ __global__ __launch_bounds__(LANES) void sample_chunks_kernel(const Params p) {
     if (threadIdx.x < BINS) {
         p.hist_w[at * BINS + threadIdx.x] = weights[threadIdx.x];
         if (h.k) p.hist_n[at * BINS + threadIdx.x] = numbers[threadIdx.x];
+    }
     }
 }
 
@@ -806,7 +822,8 @@ int check(const spinf_sample_args* a, const char* what) {
 
 template <bool BF16>
 hipError_t launch(const Params& p, bool filters, hipStream_t s) {
-    hipLaunchKernelGGL(sample_chunks_kernel<BF16>, dim3(p.chunks, p.rows), dim3(LANES), 0, s, p);
+    if (filters) hipLaunchKernelGGL((sample_chunks_kernel<BF16, true>), dim3(p.chunks, p.rows), dim3(LANES), 0, s, p);
+    else hipLaunchKernelGGL((sample_chunks_kernel<BF16, false>), dim3(p.chunks, p.rows), dim3(LANES), 0, s, p);
     hipError_t e = hipGetLastError();
     if (filters) {
         if (e == hipSuccess) {
@@ -849,7 +866,7 @@ extern "C" int spinf_sample(const spinf_sample_args* a, void* stream) {
     p.aligned = (uintptr_t)a->logits % 16 == 0 && a->ld % (a->dtype ? 8 : 4) == 0;
     p.u = a->u; p.u_f64 = a->u_f64 != 0;
     p.temperature = a->temperature; p.top_k = a->top_k; p.top_p = a->top_p; p.min_p = a->min_p;
-    p.all_temperature = a->all_temperature; p.all_top_k = a->all_top_k; p.all_top_p = a->all_top_p; p.all_min_p = a->all_min_p;
+    p.all_temperature = a->all_temperature; p.all_inv = 1.0 / (double)a->all_temperature; p.all_top_k = a->all_top_k; p.all_top_p = a->all_top_p; p.all_min_p = a->all_min_p;
     p.token = (long*)a->token; p.prob = a->prob;
     char* w = (char*)a->workspace;
     p.stat = (Stat*)(w + z.stat); p.row = (Row*)(w + z.row); p.hist_n = (int*)(w + z.hist_n); p.hist_w = (u64*)(w + z.hist_w);

@@ -41,11 +41,6 @@ constexpr int SEAT_SHARED_ROWS = 96;
 // Keys are cut so that the items of a step fill the places that run at a time, and into pieces of no less than these; which piece size that is goes by all of a step's lengths.
 constexpr int SEAT_WAVE_TILES = 8, SEAT_BLOCK_TILES = 4;
 
-#if defined(__HIPCC__)
-#define SEATS_BOTH __host__ __device__ __forceinline__
-#else
-#define SEATS_BOTH inline
-#endif
 SEATS_BOTH int seats_least(int a, int b) { return a < b ? a : b; }
 SEATS_BOTH int seats_most(int a, int b) { return a > b ? a : b; }
 SEATS_BOTH int seats_up(int a, int b) { return (a + b - 1) / b; }
