@@ -452,8 +452,8 @@ int spinf_qk_norm_rope(const spinf_rope_args* args, void* stream);
  *   the last row; and for each of the `kinds` head geometries (window 0: none) the work lists of spinf_seats_attn.
  * shared [contents, 3]: stored keys (at most `longest`), positions of the text, first page in `lists`.  Lists, as long as
  * spinf_seats_rooms says ([0 .. 2] items of wave, single and block, 24 int32 each, [3] of last, 12 each; [4] partial rows of the attention's workspace), 16-byte aligned; counts [5]; parts
- * [rows + 1]; seat_parts [2 seats + 1].  One launch
- * (two where rows > 8,192); nothing is allocated.  At most 2,048 seats and 8 geometries. */
+ * [rows + 1]; seat_parts [2 seats + 1].  A call may have fewer rows than the lists were made for.  One launch, one more where there are geometries, one more where rows > 8,192; nothing is
+ * allocated.  At most 2,048 seats and 8 geometries. */
 typedef struct spinf_seats_kind {
     int32_t* wave; int32_t* single; int32_t* block; int32_t* last; int32_t* counts; int32_t* parts; int32_t* seat_parts;
     int32_t hq, hkv, d, window;
@@ -475,7 +475,7 @@ int spinf_seats_step(const spinf_seats_args* args, void* stream);
  * content read its keys together.  Rows behind the step's last come out as zeros (lse: -inf).
  *   q, out [rows, hq, d] bf16 (rows as the step was given; strides in elements, multiples of 8); lse [rows, hq] fp32 or NULL; k, v the cache as above, every page in `lists` one of its;
  *   lists, first, pos as spinf_seats_step leaves them; kind: the lists of this geometry and window; rooms: what spinf_seats_rooms says of it; workspace: 16-byte aligned,
- *   rooms[4] * hq * (d + 2) * 4 bytes, the caller's.  Up to four launches; nothing is allocated. */
+ *   rooms[4] * hq * (d + 2) * 4 bytes, the caller's.  Two to four launches; nothing is allocated. */
 typedef struct spinf_seats_attn_args {
     const void* q; void* out; float* lse;
     int64_t q_tok, q_head, o_tok, o_head;

@@ -3,14 +3,19 @@
 //
 // Mathematics.  Row = new token x query head; it sees its content's P stored keys and its seat's own up to its own place: out = (sum_A p v + sum_B p v) / (sum_A p + sum_B p), p =
 // exp(t - ref).  The sums over a content's keys are one product per key / value head for all rows that go on below it, so its keys are read once per 128 rows and not once
-// per seat; the sums over own keys are made seat by seat; a piece leaves its reference, its sum and its weighted values in 32 bits, and seats_join_kernel puts a row's pieces together.
+// per seat; the sums over own keys are made seat by seat; a piece leaves its reference, its sum and its weighted values in 32 bits, and a row's pieces are put together at the end.
 // Tiles, products and the softmax of a tile are those of paged_rows.h; a row sees one interval of a span's keys, so a mask is two comparisons.
 //
 // Kernels (lists of csrc/seats.h):
-//   wave   a seat's own keys: four (three at 512 dims) waves share 32 rows and divide the tiles, or, where the keys are few, take an item each.
-//   block  contents, and own keys of many new tokens: four waves with 32 rows each on shared double-buffered tiles.
-//   join   the pieces of every row; rows behind the step's last become zeros.
-// The lists' lengths are known on the GPU alone: grids have a bounded size and walk the lists.
+//   wave    few rows (up to 64 below one content, up to 32 of a seat): four waves (three at 512 dims) divide the tiles, or, where a seat's keys are few, take an item each.
+//   block   many rows: four waves with 32 rows each on shared double-buffered tiles.
+//   finish  one token on few keys of its own, which then adds what its content's pieces left; the pieces of all other rows; rows behind the step's last become zeros.
+// The lists' lengths are known on the GPU alone: grids have a bounded size and walk the lists.  A list without items costs 3 to 5 us of a launch.
+//
+// What bounds it.  24 answers below 301 tokens, 24 us: latency, three launches of one short item to a place each.  24 x 56 branches of one token on 470 + 9 keys, 79 us: latency, the keys
+// alone would be 40 us.  48 answers below 65,536 tokens, 161 us (0.48 PFLOP/s), and 35 questions of 150 tokens in a window of 1,024, 169 us (0.52): the turns of a tile's products and its
+// softmax; the matrix unit is busy a third of the time, and at 256 dims two waves to a SIMD are all that fit: with 64 rows to a wave the accumulators spill, and eight waves
+// on the same tiles (four buffers) go in step, with nothing beside the softmax to feed the matrix unit: 146 for 129 us of the block kernel, 279 for 191.
 //
 // Keys that a row does not see leave no trace: as in paged_attn.hip, a workgroup that masked some tile and holds a result that is not finite looks whether masked tiles hold such
 // values, and if so computes its rows one by one over the keys they see.

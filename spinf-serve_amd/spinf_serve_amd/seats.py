@@ -31,7 +31,7 @@ class PagedSeats:
     the stored keys of content content[r] (-1: of none); own key s lies in entry s % page of page table[r, s // page].
 
     Device tensors, int32, kept by `step` and to be read only, but for ``content``, which the program writes (before the step that brings the seat's first token):
-      content [seats]    which content a seat's request goes on below; a number that is none of them is as -1
+      content [seats]    which content a seat's request goes on below; a number that is none of them is as -1 (written in place: the seats keep this tensor)
       lens [seats]       own keys, the last step's new ones with them
       took, first        [seats] and [seats + 1]: the new tokens the last step gave each seat, and the row its first one is; first[-1]: rows in use
       table [seats, ceil(keys / page)], free [pool], left [1]: the seats' pages (behind a seat's keys: anything), the stack of free ones (its first left[0] entries)
@@ -296,7 +296,8 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     softcap)), times the values.  A row sees the stored keys of its seat's content and its seat's own keys up to its own, with ``window`` those less than ``window`` places behind it.  Rows behind
     the step's last (seats.first[-1] of them are in use) come out as zeros, with a log-sum of -inf.  return_lse: also the natural log of each row's sum of exponentials, [rows, hq] fp32.
     Seats one after the other below the same content share its reading: put them next to each other.  fp32 throughout, but for the probabilities, each rounded to bf16 once for the
-    product with its value, as in paged_attn.  A row's last bits depend on its own lengths and on how many 128-row blocks the seats beside it below its content make, and on nothing else in the step.
+    product with its value, as in paged_attn (one token on few keys of its own: not rounded).  How keys are cut into pieces goes by all lengths of the step: the same step gives the same bits, a
+    row beside other seats differs in the rounding of its sums.  What a row does not see may be anything, NaN and infinities too.
     (hq, key / value heads, d) and the window have to be among the seats' ``heads``.  The new tokens' own keys and values have to be in the cache (qk_norm_rope_put)."""
     k, v = cache.k, cache.v
     eager = _lib.eager(q, k, v)
