@@ -473,8 +473,8 @@ int spinf_seats_step(const spinf_seats_args* args, void* stream);
 /* Attention of a step's new tokens: out[t] = softmax over the keys that row t sees of scale q.k (softcap > 0: of softcap tanh(scale q.k / softcap)) times v, for every row and query head.  A
  * row sees its content's stored keys and its seat's own keys up to its own, with a window those less than `window` places behind it.  The rows of seats one after the other below one
  * content read its keys together.  Rows behind the step's last come out as zeros (lse: -inf).
- *   q, out [rows, hq, d] bf16 (rows as the step was given; strides in elements, multiples of 8); lse [rows, hq] fp32 or NULL; k, v the cache as above, every page in `lists` one of its;
- *   lists, first, pos as spinf_seats_step leaves them; kind: the lists of this geometry and window; rooms: what spinf_seats_rooms says of it; workspace: 16-byte aligned,
+ *   q, out [rows, hq, d] bf16 (rows as the step was given: where its tokens are more than they hold, all come out as NaN; strides in elements, multiples of 8); lse [rows, hq] fp32 or NULL; k, v the cache as above, every page in `lists` one of its;
+ *   lists, first, pos as spinf_seats_step leaves them; kind: the lists of this geometry and window; rooms: what spinf_seats_rooms says of it for as many rows; workspace: 16-byte aligned,
  *   rooms[4] * hq * (d + 2) * 4 bytes, the caller's.  Two to four launches; nothing is allocated. */
 typedef struct spinf_seats_attn_args {
     const void* q; void* out; float* lse;

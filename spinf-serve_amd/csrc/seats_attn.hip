@@ -50,24 +50,21 @@ struct Params {
     SoftCap cap;
 };
 
-struct Item { int tok0, T, row0, piece, only, N; };   // N: rows of the set that lie in the call's tensors
+struct Item { int tok0, T, row0, piece, only; };
 struct Span { int tab, L, kt0, tiles, flo, fhi, own; };
 __device__ __forceinline__ Item load_item(const SeatItem* items, int i) {
     const int* p = (const int*)(items + i);
-    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4), 0};
+    return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4)};
 }
-// (a step of more rows than the call's tensors have does not go with them: whatever it left, no row outside them is touched)
-__device__ __forceinline__ bool bound(Item& it, int rows, int group) {
-    it.N = seats_least(it.T, rows - it.tok0) * group;
-    return it.row0 < it.N;
-}
+// (a step of more rows than the call's tensors have does not go with them: its lists are not walked, and all rows become NaN)
+__device__ __forceinline__ int tokens_of(const Params& p) { return sload(p.first, p.seats); }
 __device__ __forceinline__ Span load_span(const SeatItem* items, int i, int which) {
     const int* p = (const int*)(items + i) + 8 + 8 * which;
     return {sload(p, 0), sload(p, 1), sload(p, 2), sload(p, 3), sload(p, 4), sload(p, 5), sload(p, 6)};
 }
 // (pins an item's loads where they are asked for: beside the list's count and not behind it.  There is room for an item of that index, whatever it holds.)
-__device__ __forceinline__ void asked(int count, const Item& a, const Span& b) {
-    asm volatile("" ::"s"(count), "s"(a.tok0), "s"(a.T), "s"(a.row0), "s"(a.piece), "s"(a.only), "s"(b.tab), "s"(b.L), "s"(b.kt0), "s"(b.tiles), "s"(b.flo), "s"(b.fhi), "s"(b.own));
+__device__ __forceinline__ void asked(int count, int tokens, const Item& a, const Span& b) {
+    asm volatile("" ::"s"(count), "s"(tokens), "s"(a.tok0), "s"(a.T), "s"(a.row0), "s"(a.piece), "s"(a.only), "s"(b.tab), "s"(b.L), "s"(b.kt0), "s"(b.tiles), "s"(b.flo), "s"(b.fhi), "s"(b.own));
 }
 __device__ __forceinline__ bool is_masked(const Span& s, int kt) { return kt * TK < s.flo || kt * TK + TK - 1 > s.fhi; }
 
@@ -120,7 +117,7 @@ struct Rows : RowTile<D, DV, CAP> {
     int lo, hi;
 
     __device__ __forceinline__ void see(const Params& p, const Item& it, const Span& s, int row0) {
-        const int row = row0 + (lane_now() & 31), r = row < it.N ? row : it.N - 1;
+        const int N = it.T * p.group, row = row0 + (lane_now() & 31), r = row < N ? row : N - 1;
         interval(p, it, s, p.by_group.of(r), lo, hi);
     }
     // queries of rows row0 + m, dims col ..
@@ -128,7 +125,7 @@ struct Rows : RowTile<D, DV, CAP> {
         lane = threadIdx.x & 63;
         m = lane & 31;
         g = lane >> 5;
-        const int row = row0 + m, r = row < it.N ? row : it.N - 1;
+        const int N = it.T * p.group, row = row0 + m, r = row < N ? row : N - 1;
         const int tok = p.by_group.of(r), head = kvh * p.group + (r - tok * p.group);
         const __bf16* qp = p.q + (long)(it.tok0 + tok) * p.q_tok + (long)head * p.q_head + col + 8 * g;
 #pragma unroll
@@ -281,11 +278,12 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
     const unsigned k_at = lds_addr(kb), v_at = lds_addr(vb);
     // (the first item, if it is one for all waves)
     const int first_unit = DV < D ? (blockIdx.x >> 4) * 8 + (blockIdx.x & 7) : blockIdx.x, first_item = seats_least(p.by_heads.of(first_unit), p.room[0] - 1);
-    const int count = sload(p.counts, 0), singles = sload(p.counts, 1);
+    const int count = sload(p.counts, 0), singles = sload(p.counts, 1), tokens = tokens_of(p);
     const Item item0 = load_item(p.wave, first_item);
     const Span span0 = load_span(p.wave, first_item, 0);
-    asked(count, item0, span0);
-    const int shared = seats_least(count, p.room[0]) * p.hkv, alone = seats_least(singles, p.room[1]) * p.hkv;
+    asked(count, tokens, item0, span0);
+    const bool right = tokens <= p.rows;
+    const int shared = right ? seats_least(count, p.room[0]) * p.hkv : 0, alone = right ? seats_least(singles, p.room[1]) * p.hkv : 0;
     const int units = shared + (alone + NW - 1) / NW;
     const int last_unit = DV < D ? (units + 7) / 8 * 16 : units;
     for (int u = blockIdx.x; u < last_unit; u += gridDim.x) {
@@ -301,8 +299,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
         const int item = p.by_heads.of(x), kvh = x - item * p.hkv;
         const SeatItem* const list = single ? p.single : p.wave;
         const bool known = !single && u == (int)blockIdx.x;
-        Item it = known ? item0 : load_item(list, item);
-        if (!bound(it, p.rows, p.group)) continue;
+        const Item it = known ? item0 : load_item(list, item);
         const Span span = known ? span0 : load_span(list, item, 0);
         const char* const k_base = p.k + kvh * p.k_head;
         const char* const v_base = p.v + kvh * p.v_head + vcol * 2;
@@ -323,8 +320,8 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
             rows.load(p, it, span, kvh, it.row0);
             rows.reset();
             if (rows.g == 0 && !it.only) {   // (asked for here: at the end they would be one more wait for memory)
-                const int row = it.row0 + rows.m;
-                part_of_row[w][rows.m] = p.parts[it.tok0 + p.by_group.of(row < it.N ? row : it.N - 1)] & INT_MAX;
+                const int N = it.T * p.group, row = it.row0 + rows.m;
+                part_of_row[w][rows.m] = p.parts[it.tok0 + p.by_group.of(row < N ? row : N - 1)] & INT_MAX;
             }
             while (kt < end) {
                 const bool masked = is_masked(span, kt), next = kt + step < end;
@@ -352,7 +349,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void seats_wave_kernel(c
                 kt += step;
             }
         }
-        const int left = it.N - it.row0, here = left < 32 ? left : 32;
+        const int left = it.T * p.group - it.row0, here = left < 32 ? left : 32;
         const float sum = lane32_sum(rows.l);
         if (sum == 0.f) rows.M = -INFINITY;   // no key seen
         constexpr int PIECES = DV / 8;
@@ -486,11 +483,10 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int w = H == 1 ? wave : wave & 3, half = H == 1 ? 0 : wave >> 2, vcol = half * DV;
     const unsigned base = lds_addr(lds) + half * HALF;
-    const int units = seats_least(sload(p.counts, 2), p.room[2]) * p.hkv;
+    const int units = tokens_of(p) <= p.rows ? seats_least(sload(p.counts, 2), p.room[2]) * p.hkv : 0;
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
-        Item it = load_item(p.block, item);
-        if (!bound(it, p.rows, p.group)) continue;
+        const Item it = load_item(p.block, item);
         const Span span[2] = {load_span(p.block, item, 0), load_span(p.block, item, 1)};
         const int tiles = span[0].tiles + span[1].tiles;
         const char* const k_base = p.k + kvh * p.k_head;
@@ -530,7 +526,7 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
         // keys of tile i behind its first one
         const auto behind = [&](int i) __attribute__((always_inline)) { return i < span[0].tiles ? span[0].L - 1 - (span[0].kt0 + i) * TK : span[1].L - 1 - (span[1].kt0 + i - span[0].tiles) * TK; };
         if (tiles > 0) issue(0, behind(0), 0);   // (ahead of the queries: their latencies pass together)
-        if (it.row0 + 32 * w >= it.N) {   // a wave without rows brings its share of the tiles
+        if (it.row0 + 32 * w >= it.T * p.group) {   // a wave without rows brings its share of the tiles
             for (int i = 0, j = 0, buf = 0; i < tiles; i++, buf ^= 1) {
                 __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
                 __syncthreads();
@@ -590,7 +586,7 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
             rows.softmax(p.cap, s, pb);
             rows.values(kb + GK::KTILEB, pb);
         }
-        const int left = it.N - it.row0 - 32 * w;   // rows from this wave's first on
+        const int left = it.T * p.group - it.row0 - 32 * w;   // rows from this wave's first on
         const int live = seats_least(4, seats_up(left + 32 * w, 32));   // waves that have rows
         const float sum = lane32_sum(rows.l);
         if (sum == 0.f) rows.M = -INFINITY;   // no key seen
@@ -665,17 +661,16 @@ __device__ __forceinline__ void last_words(const Params& p) {
         for (int i = 0; i < 12; i++) x.w[i] = sload(ip, i);
         return x;
     };
-    const int count = sload(p.counts, 3);
+    const int count = sload(p.counts, 3), tokens = tokens_of(p);
     Words next = load(blockIdx.x * 4 + w);
-    asm volatile("" ::"s"(count), "s"(next.w[0]), "s"(next.w[4]), "s"(next.w[8]));
-    const int most = seats_least(count, p.room[3]) * p.hkv, stride = p.last_blocks * 4;
+    asm volatile("" ::"s"(count), "s"(tokens), "s"(next.w[0]), "s"(next.w[4]), "s"(next.w[8]));
+    const int most = tokens <= p.rows ? seats_least(count, p.room[3]) * p.hkv : 0, stride = p.last_blocks * 4;
     for (int unit = blockIdx.x * 4 + w; unit < most; unit += stride) {
         const int item = p.by_heads.of(unit), kvh = unit - item * p.hkv;
         const Words now = next;
         if (unit + stride < most) next = load(unit + stride);
         const int tok = now.w[0], L = now.w[1], lo = now.w[2], tab = now.w[3], part = now.w[4], parts = now.w[5];
         const int page[SEAT_PAGES] = {now.w[6], now.w[7], now.w[8], now.w[9], now.w[10], now.w[11]};
-        if (tok >= p.rows) continue;
         const int n = L - lo, page0 = p.page.of(lo >> 4), many = p.page.of((L - 1) >> 4) - page0 + 1;
         const char* const kb = p.k + kvh * p.k_head + col * 2;
         const char* const vb = p.v + kvh * p.v_head + col * 2;
@@ -793,20 +788,21 @@ __device__ __forceinline__ void join(const Params& p, int block) {
     __shared__ __attribute__((aligned(16))) float part_sum[GROUPS][64];
     __shared__ float2 part_ml[GROUPS];
     const int sets = p.join_x * SLICES, y0 = block / sets, x0 = block - y0 * sets, slice = x0 % SLICES;
-    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, lane = threadIdx.x & 63, used = sload(p.first, p.seats);
+    const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, lane = threadIdx.x & 63, used = tokens_of(p);
     for (int tok0 = x0 / SLICES; tok0 < p.rows; tok0 += 64 * p.join_x) {
     // of 64 tokens of this workgroup: where their pieces begin, and how many there are (0: the last word is spoken)
     const int at = tok0 + lane * p.join_x, begins = at < p.rows ? p.parts[at] : 0, ends = at < p.rows ? p.parts[at + 1] : 0;
-    const int number = at >= p.rows || begins < 0 ? 0 : (ends & INT_MAX) - begins;
-    unsigned long long left = __builtin_amdgcn_ballot_w64(number > 0 || (at >= used && at < p.rows));
+    const int number = at >= p.rows || begins < 0 || used > p.rows ? 0 : (ends & INT_MAX) - begins;
+    unsigned long long left = __builtin_amdgcn_ballot_w64(number > 0 || ((at >= used || used > p.rows) && at < p.rows));
     while (left) {
     const int which = __builtin_ctzll(left), tok = tok0 + which * p.join_x;
     left &= left - 1;
     const int first = __builtin_amdgcn_readlane(begins, which), n = __builtin_amdgcn_readlane(number, which);
     if (n == 0) {
+        const unsigned nothing = used > p.rows ? 0x7fc07fc0u : 0;
         for (int h = y0 * GROUPS + group; h < p.hq; h += p.join_y * GROUPS) {
-            *(uint2*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = make_uint2(0, 0);
-            if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = -INFINITY;
+            *(uint2*)(p.out + (long)tok * p.o_tok + (long)h * p.o_head + slice * 64 + d) = make_uint2(nothing, nothing);
+            if (p.lse && slice == 0 && d == 0) p.lse[(long)tok * p.hq + h] = nothing ? NAN : -INFINITY;
         }
         continue;
     }

@@ -255,8 +255,12 @@ def _attn_block(q, k, v, state, work, pos, geo, index, scale, softcap):
     a.lists, a.first, a.pos = base, base + 4 * lay["first"], pos.data_ptr()
     a.kind.hq, a.kind.hkv, a.kind.d, a.kind.window = _kinds(geo)[index]
     _point(a.kind, work, lay["lists"][index])
-    for i, n in enumerate(_rooms(geo, index)):
-        a.rooms[i] = n
+    n = _numbers(geo)   # (room for as many rows as these: a step of few needs little of what the seats' most would)
+    n.rows = q.shape[0]
+    rooms = (C.c_int64 * 5)()
+    _lib.check(_lib.load_library().spinf_seats_rooms(C.byref(n), index, rooms), "seats_attn")
+    for i in range(5):
+        a.rooms[i] = rooms[i]
     a.rows, a.seats, a.page, a.scale, a.softcap = q.shape[0], geo[0], geo[2], scale, softcap
     return a
 
@@ -298,6 +302,7 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     Seats one after the other below the same content share its reading: put them next to each other.  fp32 throughout, but for the probabilities, each rounded to bf16 once for the
     product with its value, as in paged_attn (one token on few keys of its own: not rounded).  How keys are cut into pieces goes by all lengths of the step: the same step gives the same bits, a
     row beside other seats differs in the rounding of its sums.  What a row does not see may be anything, NaN and infinities too.
+    The rows are the last step's (its ``rows``); replayed behind a step of more tokens than q has rows, all of them are NaN.
     (hq, key / value heads, d) and the window have to be among the seats' ``heads``.  The new tokens' own keys and values have to be in the cache (qk_norm_rope_put)."""
     k, v = cache.k, cache.v
     eager = _lib.eager(q, k, v)

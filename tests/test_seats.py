@@ -511,6 +511,77 @@ def test_steps_of_fewer_rows(dev):
 
 
 @pytest.mark.gpu
+def test_rows_of_another_step_become_nan(dev):
+    """attention recorded for a step of few rows and replayed behind one of more tokens: nothing of it is written"""
+    heads = (8, 4, 64)
+    s, pages = make(dev, [300], [40, 1, 90], [1, 1, 1], 16, heads, [0, 0, 0], rows=60, keys=400, spare=30)
+    cache, q = fill(s, pages, heads, 6, dev)
+    new = torch.tensor([1, 0, 0], dtype=torch.int32, device=dev)
+    s.step(new, rows=2)
+    sa.seats_attn(q[:2], cache, s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = sa.seats_attn(q[:2], cache, s, return_lse=True)
+    s.step(new, rows=2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, sa.seats_attn(q[:2], cache, s)) and out[0].isfinite().all() and (out[1] == 0).all()
+    for many in ([30, 1, 1], [1, 1, 1]):
+        s.step(torch.tensor(many, dtype=torch.int32, device=dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out.isnan().all() and lse.isnan().all()
+    s.step(torch.tensor([1, 1, 0], dtype=torch.int32, device=dev))   # (as many tokens as there are rows: these are them)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, sa.seats_attn(q, cache, s)[:2])
+
+
+@pytest.mark.gpu
+def test_several_head_geometries_in_one(dev):
+    """a model's kinds of layers: what each gets is what seats of that kind alone give"""
+    kinds = [((16, 8, 64), 0), ((16, 8, 64), 50), ((16, 8, 64), 1000), ((8, 1, 512), 0), ((40, 8, 128), 0), ((64, 1, 64), 0), ((128, 1, 64), 30), ((1, 1, 256), 0)]
+    stored, content, own, new = [90, 300, 2000], [0, 0, 1, 1, 1, 2, 2, -1], [20, 1, 9, 133, 70, 130, 3, 6], [1, 1, 3, 1, 70, 2, 1, 6]
+    rng = np.random.default_rng(3)
+    need, mine = [-(-n // 16) for n in stored], [-(-n // 16) for n in own]
+    ids = rng.permutation(sum(need) + sum(mine) + 3)
+    tables = np.split(ids[: sum(need)], np.cumsum(need)[:-1])
+
+    def built(heads):
+        s = sa.PagedSeats.build(len(own), sum(new) + 2, 16, max(own), ids[sum(need) :], contents=(stored, tables), stored=[n - m for n, m in zip(own, new)], heads=heads, device=dev)
+        s.tables = tables
+        s.content.copy_(torch.tensor(content, dtype=torch.int32))
+        s.step(torch.tensor(new, dtype=torch.int32, device=dev))
+        return s
+
+    every = built([(*h, w) for h, w in kinds])
+    assert every.took.tolist() == new
+    for h, w in kinds:
+        one = built([(*h, w)])
+        cache, q = fill(one, len(ids), h, 4, dev)
+        got = sa.seats_attn(q, cache, every, window=w or None)
+        assert torch.equal(got, sa.seats_attn(q, cache, one, window=w or None))
+        want, _, tol, _ = reference(q, cache, one, stored, content, own, new, h[2] ** -0.5, w)
+        close(got[: sum(new)], want, tol)
+
+
+@pytest.mark.gpu
+def test_a_step_given_the_seats_own_numbers(dev):
+    """what the last step added taken back, and seats emptied, by the tensors the seats keep themselves"""
+    s, _ = make(dev, [40], [17, 3, 64, 1], [1, 1, 1, 1], 16, (4, 2, 64), content=[0, 0, -1, 0], rows=80, keys=100, spare=20)
+    new = torch.tensor([20, 1, 17, 31], dtype=torch.int32, device=dev)
+    before = s.lens.clone(), s.left.clone(), s.free.clone()
+    s.step(new)
+    s.step(torch.zeros_like(new), s.took)
+    assert torch.equal(s.lens, before[0]) and torch.equal(s.left, before[1]) and torch.equal(s.free, before[2])
+    s.step(new)
+    s.step(s.took, s.took)   # the same tokens again
+    assert s.took.tolist() == new.tolist() and (s.lens - before[0]).tolist() == new.tolist()
+    s.step(new, s.lens)
+    assert s.lens.tolist() == new.tolist()
+
+
+@pytest.mark.gpu
 def test_below_trimmed_contents_positions_go_on(dev):
     heads, stored, gone = (4, 2, 64), [100, 30], [57, 0]
     s, pages = make(dev, stored, [20, 1, 8], [1, 1, 3], 16, heads, [0, 1, 0], dropped=gone)
