@@ -144,6 +144,12 @@ __device__ __forceinline__ double weight(float x, float top, double by_two) { re
 // in units of 2^-47: the last bits of w + 32, rounded there
 __device__ __forceinline__ u64 units(double w) { return (u64)(__double_as_longlong(w + 32.0) - __double_as_longlong(32.0)); }
 constexpr double UNIT = 0x1p-47;
+// units of a chunk's (or, by a row's largest logit, a row's) logits, the same in every kernel
+struct Units {
+    Weights w; float top; double by_two; bool fits;
+    __device__ __forceinline__ Units(const double* steps, float top, const How& h) : w(steps, top, h), top(top), by_two(h.by_two), fits(Weights::fits(top, h)) {}
+    __device__ __forceinline__ u64 of(float x) const { return fits ? units(w.of(x)) : units(weight(x, top, by_two)); }
+};
 
 template <bool BF16>
 __device__ __forceinline__ float load1(const Params& p, int row, int i) {
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
     double mass = 0.0;
     int n = 0;
     {   // (the halves' chunks and their order are always the same)
-        constexpr int AHEAD = 8;
+        constexpr int AHEAD = 16;
         for (int c0 = half; c0 < p.chunks; c0 += 2 * AHEAD) {
             u64 w[AHEAD];
             int m[AHEAD];
@@ -568,7 +574,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     __shared__ u64 sums[256], found[3];
     __shared__ int counts[256], begins[MOST_CHUNKS + 1], room_n[WAVES];
     __shared__ float tops[MOST_CHUNKS];
-    __shared__ double factor[MOST_CHUNKS], target[2];
+    __shared__ double factor[MOST_CHUNKS], target[2], steps[STEPS];
     const int row = blockIdx.x, tid = threadIdx.x;
     const How h = settings(p, row);
     Row r = {};
@@ -578,6 +584,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     const int own_count = FILTERS && tid < p.chunks ? p.count[mine_at] : 0;
     const u64 own_kept = FILTERS && tid < p.chunks ? p.kept[mine_at] : 0;
     const double given = p.u_f64 ? ((const double*)p.u)[row] : (double)((const float*)p.u)[row];
+    fill_steps(steps);   // (read behind the barriers of stage)
     Stat own;
     r.top = stage(p, row, h, own, tops, factor, (float*)room);
     if (!FILTERS) r.how = r.top == -INFINITY ? NOTHING : h.best ? BEST : PLAIN;
@@ -589,9 +596,11 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         }
         return;
     }
-    const double least = log((double)h.least);
+    const double least = h.least > 0.f ? log((double)h.least) : -INFINITY;
     const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
     u64 last = ~0ull;   // the last number that is kept
+    int direct = 0;     // so many tokens in question, one a lane, are all that are kept
+    u64 mine_w = 0;     // ... and this lane's weight, by its chunk
     if (FILTERS && r.how == LIST) {
         const int m = own_count;
         int n;
@@ -603,13 +612,13 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
             const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
             const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
             u64 some = 0, differ = 0;
+            const Units by_row(steps, r.top, h);
             for (int c = tid >> 6; c < p.chunks; c += WAVES)
                 for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
                     const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
                     const u64 x = (u64)~y.x << 32 | y.y;
-                    const float v = unordered(y.x);
                     listed[i] = x;
-                    worth[i] = units(v == r.top ? 1.0 : r.top == INFINITY ? 0.0 : power(((double)v - (double)r.top) * h.by_two));
+                    worth[i] = by_row.of(unordered(y.x));
                 }
             __syncthreads();
             if (n > 128) {
@@ -672,8 +681,12 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
             for (int i = tid; i < n; i += LANES) {
                 const float x = value(listed[i]);
                 const int c = (int)((unsigned)listed[i] / CHUNK);
-                if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to) && stays(x)) atomicAdd(&chunks[c], units(weight(x, tops[c], h.by_two)));
+                if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to) && stays(x)) {
+                    mine_w = Units(steps, tops[c], h).of(x);
+                    atomicAdd(&chunks[c], mine_w);
+                }
             }
+            if (h.few && n <= 128) direct = n;
         }
     }
     if (FILTERS && r.how == SEARCH) {
@@ -687,8 +700,9 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                     if (x[e] > -INFINITY) f(x[e], number(x[e], index_of<BF16>(c, e)));
             }
         };
+        const Units by_top(steps, r.top, h);
         // (up to 2^22 of them: units of 2^-38 leave room for the sum)
-        const auto coarse = [&](float x) __attribute__((always_inline)) { return (units(weight(x, r.top, h.by_two)) + 256) >> 9; };
+        const auto coarse = [&](float x) __attribute__((always_inline)) { return (by_top.of(x) + 256) >> 9; };
         if (h.k) last = search(h.k, 0, ~0ull, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
         if (h.p < 1.f) {
             u64 w = 0;
@@ -705,9 +719,10 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
             if (tops[c] > -INFINITY) {
                 float x[EACH];
                 load<BF16>(p, row, c, x);
+                const Units by_chunk(steps, tops[c], h);
 #pragma unroll
                 for (int e = 0; e < EACH; e++)
-                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += units(weight(x[e], tops[c], h.by_two));
+                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += by_chunk.of(x[e]);
             }
             w = sum_all(w, room);
             if (tid == 0) chunks[c] = w;
@@ -744,7 +759,27 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     }
     const u64 want = target[0] > 0.0 ? (u64)target[0] : 0;
     const float top = tops[chunk];
+    if (FILTERS && direct) {   // the token among those that are listed: each adds up what lies before it
+        const unsigned at = tid < direct ? (unsigned)listed[tid] : 0;
+        const bool here = tid < direct && mine_w && (int)(at / CHUNK) == chunk;
+        if (tid < direct) worth[tid] = here ? mine_w : 0;
+        __syncthreads();
+        u64 before = 0;
+        if (here)
+            for (int i = 0; i < direct; i++) before += (unsigned)listed[i] < at ? worth[i] : 0;
+        bool hit = here && before <= want && before + mine_w > want;
+        if (!__syncthreads_or(hit)) {   // (where rounding left none, the last token that is kept)
+            const unsigned end = over_all(here ? at + 1 : 0u, (unsigned*)room_n, [](unsigned a, unsigned b) { return a > b ? a : b; });
+            hit = here && at + 1 == end;
+        }
+        if (hit) {
+            p.token[row] = at;
+            if (p.prob) p.prob[row] = (float)((double)mine_w * factor[chunk] / target[1]);
+        }
+        return;
+    }
     // a lane's 16 logits one after the other
+    const Units by_chunk(steps, top, h);
     u64 w[EACH], mine = 0;
     const int first = chunk * CHUNK + tid * EACH;
     float x[EACH];
@@ -760,7 +795,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     for (int e = 0; e < EACH; e++) {
         x[e] = fmaxf(x[e], -INFINITY);
         const bool in = x[e] > -INFINITY && (r.how == PLAIN || (number(x[e], first + e) <= last && stays(x[e]) && (r.how == SEARCH || h.few || r.grid - place(x[e], h.scale) <= r.to)));
-        w[e] = in ? units(weight(x[e], top, h.by_two)) : 0;
+        w[e] = in ? by_chunk.of(x[e]) : 0;
         mine += w[e];
     }
     u64 total;
