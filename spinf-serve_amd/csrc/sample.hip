@@ -10,9 +10,9 @@
 //
 // Kernels.  chunks: a chunk's largest logit, its weight, and how many logits and how much weight lie in each of 255 bins, a twelfth of T wide, below its largest one (bins at whole
 // multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
-// of the bins in question.  draw: those few are put in order by digits of their numbers, the chunk is found by the chunks' weights and the token in it.  Rows without a filter need the first and
-// the last.  Where bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself, digit by digit.
-// Bound by HBM: the logits once; the second reading comes out of the last-level cache.
+// of the bins in question.  draw: the borders among those few, then the chunk by the chunks' weights and the token in it.  Rows without a filter need the first and the last.  Where
+// bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself: 8 rows of 262,144 equal logits, top-p: 1.2 ms.
+// Bound by instructions of 64 bits beside HBM (320 rows of 262,144: 88 us, 61 at the rate of a copy) where rows are many, by the four launches' latencies where they are few (one row: 27 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -81,10 +81,11 @@ __device__ __forceinline__ unsigned ordered(float x) {   // larger for larger x
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ float value(u64 number) { return unordered(~(unsigned)(number >> 32)); }
 __device__ __forceinline__ u64 number(float x, unsigned at) { return (u64)~ordered(x + 0.f) << 32 | at; }   // smaller: earlier in the order (zeros are equal whatever their sign)
 
 // a token's place on the grid of bins; never falls as x grows
-__device__ __forceinline__ int place(float x, float scale) { return (int)floorf(fminf(fmaxf(x * scale, -1e9f), 1e9f)); }
+__device__ __forceinline__ int place(float x, float scale) { return (int)floorf(__builtin_amdgcn_fmed3f(x * scale, -1e9f, 1e9f)); }
 
 // 2^t, t <= 0: the whole part by the exponent, the rest (at most a half) by the series of exp, whose 13th term is 2^-52 of the sum
 __device__ __forceinline__ double power(double t) {
@@ -292,13 +293,12 @@ __global__ __launch_bounds__(LANES, FILTERS ? 6 : 8) void sample_chunks_kernel(c
     }
     const auto take = [&](float x, u64 w) __attribute__((always_inline)) {
         const bool on = x > -INFINITY;
-        s.sum += w;
-        s.at += on;
+        if (h.k) s.at += on;
         const int b = grid - place(x, h.scale);
         if (on && b < BINS - 1) {
             atomicAdd(&weights[b], w);
             if (h.k) atomicAdd(&numbers[b], 1);
-        }
+        } else s.sum += w;   // (what lies in bins is added up from these)
     };
     if (Weights::fits(top, h)) {
         const Weights w(steps, top, h);
@@ -311,8 +311,9 @@ __global__ __launch_bounds__(LANES, FILTERS ? 6 : 8) void sample_chunks_kernel(c
             take(y, units(weight(y, top, h.by_two)));
         }
     }
-    s.sum = sum_all(s.sum, room);
-    s.at = over_all((int)s.at, (int*)room, [](int a, int b) { return a + b; });
+    __syncthreads();
+    s.sum = sum_all(s.sum + (threadIdx.x < BINS ? weights[threadIdx.x] : 0), room);
+    if (h.k) s.at = over_all((int)s.at, (int*)room, [](int a, int b) { return a + b; });
     if (threadIdx.x == 0) p.stat[at] = s;
     if (threadIdx.x < BINS) {
         p.hist_w[at * BINS + threadIdx.x] = weights[threadIdx.x];
@@ -501,31 +502,44 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
 }
 
 // The least number up to which (it counted in) those of `each` hold at least `need` in all; ~0: all of them hold less.  each(f) calls f(number, worth) for every one in question,
-// each lane for its share; all of them are `some` but for bits of `mask`.  Eight bits at a time, from the first that differs; bits that never do are passed over.
-template <class E>
-__device__ u64 search(u64 need, u64 some, u64 mask_all, u64* sums, int* counts, u64* found, E each) {
-    int above = 64;
-    u64 prefix = some;
-    bool first = true;
+// each lane for its share; `some`: a number next to them.  By 256 stretches of them (`stretch`, where there is one, never falls from one number to a later one: floats near zero differ in all of their bits, and lie
+// close together), then by eight bits from the first that differs among those that are left (bf16 has few values to a bin: what is left may differ in its index alone), until they
+// are few and counted against each other.
+constexpr int LEFT = 64;
+template <class E, class S>
+__device__ __forceinline__ u64 search(u64 need, u64 some, bool stretches, u64* sums, u64* one, int* counts, u64* found, u64* room, E each, S stretch) {
+    u64 known = 0, prefix = some;
+    int line = -1;   // the stretch, once it is known
+#pragma unroll 1
     while (true) {
-        const u64 open = above < 64 ? mask_all & ((1ull << above) - 1) : mask_all;
-        if (open == 0 && !first) break;
-        above = open ? 64 - __builtin_clzll(open) : 0;
-        const int shift = above > 8 ? above - 8 : 0;
+        const bool by_stretch = stretches && line < 0;
+        const auto in = [&](u64 c) __attribute__((always_inline)) { return ((c ^ prefix) & known) == 0 && (line < 0 || stretch(c) == line); };
+        u64 bits = 0;
+        int low = 0;
+        if (!by_stretch) {
+            u64 open = 0;
+            each([&](u64 c, u64) __attribute__((always_inline)) { open |= in(c) ? c ^ prefix : 0; });
+            open = over_all(open, room, [](u64 a, u64 b) { return a | b; });
+            const int top = 63 - __builtin_clzll(open | 1);
+            low = top > 7 ? top - 7 : 0;
+            bits = ~0ull << low & (~0ull >> (63 - top));
+        }
         __syncthreads();
         if (threadIdx.x < 256) {
             sums[threadIdx.x] = 0;
             counts[threadIdx.x] = 0;
         }
-        if (threadIdx.x == 0) found[0] = found[1] = found[2] = ~0ull;
+        if (threadIdx.x == 0) {
+            found[0] = found[1] = ~0ull;
+            found[2] = 0;
+        }
         __syncthreads();
-        const u64 mask = above < 64 ? ~0ull << above : 0;
         each([&](u64 c, u64 worth) __attribute__((always_inline)) {
-            if (((c ^ prefix) & mask) == 0) {
-                const int digit = (int)(c >> shift) & 255 & ((1 << (above - shift)) - 1);
-                atomicAdd(&sums[digit], worth);
-                atomicAdd(&counts[digit], 1);
-            }
+            if (!in(c)) return;
+            const int digit = by_stretch ? stretch(c) : (int)((c & bits) >> low);
+            atomicAdd(&sums[digit], worth);
+            atomicAdd(&counts[digit], 1);
+            one[digit] = c;   // (any of them)
         });
         __syncthreads();
         if (threadIdx.x < 64) {   // four digits a lane
@@ -547,23 +561,33 @@ __device__ u64 search(u64 need, u64 some, u64 mask_all, u64* sums, int* counts, 
         }
         __syncthreads();
         const u64 digit = found[0];
-        if (digit == ~0ull) return ~0ull;   // (of the first digit alone)
+        if (digit == ~0ull) return ~0ull;   // (of the first pass alone)
         need = found[1];
-        prefix = (prefix & ~(((1ull << (above - shift)) - 1) << shift)) | digit << shift;
-        above = shift;
-        first = false;
-        if (shift && counts[digit] == 1) {   // the rest of its digits
-            const u64 here = ~0ull << shift;
-            each([&](u64 c, u64) __attribute__((always_inline)) {
-                if (((c ^ prefix) & here) == 0) found[2] = c;
-            });
-            __syncthreads();
-            prefix = found[2];
-            break;
+        const int left = counts[digit];
+        if (left > LEFT) {   // (no two numbers are equal: it ends)
+            prefix = one[digit];   // (its bits up to here are the number's)
+            if (by_stretch) line = (int)digit;
+            else known |= bits;
+            continue;
         }
+        __syncthreads();   // (`one` and `sums` take the few)
+        each([&](u64 c, u64 worth) __attribute__((always_inline)) {
+            if (!in(c) || digit != (u64)(by_stretch ? stretch(c) : (int)((c & bits) >> low))) return;
+            const int i = (int)atomicAdd(&found[2], 1);
+            one[i] = c;
+            sums[i] = worth;
+        });
+        __syncthreads();
+        if ((int)threadIdx.x < left) {
+            const u64 c = one[threadIdx.x];
+            u64 before = 0;
+#pragma unroll 4
+            for (int i = 0; i < left; i++) before += one[i] < c ? sums[i] : 0;
+            if (before < need && before + sums[threadIdx.x] >= need) found[0] = c;
+        }
+        __syncthreads();
+        return found[0];
     }
-    __syncthreads();
-    return prefix;
 }
 
 template <bool BF16, bool FILTERS>
@@ -571,7 +595,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     __shared__ u64 room[WAVES];
     __shared__ u64 listed[FILTERS ? LISTED : 1], worth[FILTERS ? LISTED : 1];   // numbers of the tokens in question, and their weights
     __shared__ u64 chunks[MOST_CHUNKS];
-    __shared__ u64 sums[256], found[3];
+    __shared__ u64 sums[256], one[256], found[3];
     __shared__ int counts[256], begins[MOST_CHUNKS + 1], room_n[WAVES];
     __shared__ float tops[MOST_CHUNKS];
     __shared__ double factor[MOST_CHUNKS], target[2], steps[STEPS];
@@ -597,85 +621,117 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         return;
     }
     const double least = h.least > 0.f ? log((double)h.least) : -INFINITY;
-    const auto stays = [&](float x) __attribute__((always_inline)) { return x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
+    const auto stays = [&](float x) __attribute__((always_inline)) { return !(h.least > 0.f) || x == r.top || ((double)x - (double)r.top) * h.inv >= least; };   // min-p
     u64 last = ~0ull;   // the last number that is kept
     int direct = 0;     // so many tokens in question, one a lane, are all that are kept
     u64 mine_w = 0;     // ... and this lane's weight, by its chunk
+    int n = 0;          // tokens in question
     if (FILTERS && r.how == LIST) {
-        const int m = own_count;
-        int n;
-        const int upto = scan_all(m, room_n, n);
+        const int m = own_count, upto = scan_all(m, room_n, n);
         if (tid < p.chunks) begins[tid + 1] = upto;
         if (tid == 0) begins[0] = 0;
         if (__syncthreads_or(m > SEGMENT) || n > LISTED) r.how = SEARCH;
-        else {
-            const auto value = [](u64 c) __attribute__((always_inline)) { return unordered(~(unsigned)(c >> 32)); };
-            const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
-            u64 some = 0, differ = 0;
-            const Units by_row(steps, r.top, h);
+    }
+    if (FILTERS && r.how != PLAIN) {
+        const bool list = r.how == LIST;
+        const auto bin = [&](u64 c) __attribute__((always_inline)) { return r.grid - place(value(c), h.scale); };
+        const Units by_row(steps, r.top, h);
+        if (list) {
             for (int c = tid >> 6; c < p.chunks; c += WAVES)
                 for (int i = begins[c] + (tid & 63); i < begins[c + 1]; i += 64) {
                     const uint2 y = p.list[((long)row * p.chunks + c) * SEGMENT + i - begins[c]];
-                    const u64 x = (u64)~y.x << 32 | y.y;
-                    listed[i] = x;
+                    listed[i] = (u64)~y.x << 32 | y.y;
                     worth[i] = by_row.of(unordered(y.x));
                 }
             __syncthreads();
-            if (n > 128) {
-                some = listed[0];
-                for (int i = tid; i < n; i += LANES) differ |= listed[i] ^ some;
-                differ = over_all(differ, room, [](u64 a, u64 b) { return a | b; });
-            }
-            if (n <= 128) {   // each token counted against all
-                const u64 x = tid < n ? listed[tid] : ~0ull, w = tid < n ? worth[tid] : 0;
-                if (tid == 0) found[0] = found[1] = ~0ull;
+        }
+        const bool by_number = list ? r.kth < BINS : h.k > 0, by_mass = list ? r.by_mass : h.p < 1.f;
+        if (list && n <= 128) {   // each token counted against all
+            const u64 x = tid < n ? listed[tid] : ~0ull, w = tid < n ? worth[tid] : 0;
+            if (tid == 0) found[0] = found[1] = ~0ull;
+            __syncthreads();
+            if (by_number) {
+                const bool on = tid < n && bin(x) == r.kth;
+                int before = 0;
+                if (tid < n)
+                    for (int i = 0; i < n; i++) before += listed[i] < x;
+                // (those of other bins come before or behind all of the kth)
+                const int ahead = over_all(on ? before : INT_MAX, room_n, [](int a, int b) { return a < b ? a : b; });
+                if (on && before - ahead == h.k - r.before_k - 1) found[0] = x;
                 __syncthreads();
-                if (r.kth < BINS) {
-                    const bool on = tid < n && bin(x) == r.kth;
-                    int before = 0;
-                    if (tid < n)
-                        for (int i = 0; i < n; i++) before += listed[i] < x;
-                    // (those of other bins come before or behind all of the kth)
-                    const int ahead = over_all(on ? before : INT_MAX, room_n, [](int a, int b) { return a < b ? a : b; });
-                    if (on && before - ahead == h.k - r.before_k - 1) found[0] = x;
-                    __syncthreads();
-                    last = found[0];
-                }
-                if (r.by_mass) {
-                    u64 before = 0;
-                    const bool on = tid < n && x <= last && (h.few || bin(x) <= r.to);
-                    if (tid < n)
-                        for (int i = 0; i < n; i++) before += listed[i] < x ? worth[i] : 0;
-                    double all = r.sum;   // weight of the first k
-                    if (r.kth < BINS || h.few) all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(tid < n && x <= last && (h.few || bin(x) == r.kth) ? w : 0, room);
-                    const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
-                    const u64 least_of = need < 1.0 ? 1 : (u64)need;
-                    if (on && before < least_of && before + w >= least_of) found[1] = x;
-                    __syncthreads();
-                    last = std::min(last, found[1]);
-                }
-            } else {
-            if (r.kth < BINS)
-                last = search(h.k - r.before_k, some, differ, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
-                    for (int i = tid; i < n; i += LANES)
-                        if (bin(listed[i]) == r.kth) f(listed[i], 1);
-                });
-            if (r.by_mass) {
+                last = found[0];
+            }
+            if (by_mass) {
+                u64 before = 0;
+                const bool on = tid < n && x <= last && (h.few || bin(x) <= r.to);
+                if (tid < n)
+                    for (int i = 0; i < n; i++) before += listed[i] < x ? worth[i] : 0;
                 double all = r.sum;   // weight of the first k
-                if (r.kth < BINS || h.few) {
-                    u64 w = 0;
-                    for (int i = tid; i < n; i += LANES)
-                        if (listed[i] <= last && (h.few || bin(listed[i]) == r.kth)) w += worth[i];
-                    all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(w, room);
-                }
+                if (r.kth < BINS || h.few) all = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(tid < n && x <= last && (h.few || bin(x) == r.kth) ? w : 0, room);
                 const double need = ceil(((double)h.p * all - r.mass_from) * 0x1p47);
-                last = std::min(last, search(need < 1.0 ? 1 : (u64)need, some, differ, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
-                    for (int i = tid; i < n; i += LANES)
-                        if (listed[i] <= last && (h.few || bin(listed[i]) <= r.to)) f(listed[i], worth[i]);
-                }));
+                const u64 least_of = need < 1.0 ? 1 : (u64)need;
+                if (on && before < least_of && before + w >= least_of) found[1] = x;
+                __syncthreads();
+                last = std::min(last, found[1]);
             }
+        } else {
+            const auto of_row = [&](auto f) __attribute__((always_inline)) {   // f(logit, index) of all that can be drawn
+                constexpr int AHEAD = 4;
+#pragma unroll 1
+                for (int i0 = tid; i0 < p.vocab; i0 += AHEAD * LANES) {
+                    float x[AHEAD];
+#pragma unroll
+                    for (int a = 0; a < AHEAD; a++) x[a] = load_one<BF16>(p, row, i0 + a * LANES);
+#pragma unroll
+                    for (int a = 0; a < AHEAD; a++)
+                        if (x[a] > -INFINITY) f(x[a], i0 + a * LANES);
+                }
+            };
+            // (of a whole row up to 2^22 tokens: units of 2^-38 leave room for the sum)
+            const auto coarse = [&](float x) __attribute__((always_inline)) { return (by_row.of(x) + 256) >> 9; };
+#pragma unroll 1
+            for (int mass = 0; mass < 2; mass++) {
+                if (mass ? !by_mass : !by_number) continue;
+                const auto each = [&](auto f) __attribute__((always_inline)) {
+                    if (list) {
+#pragma unroll 1
+                        for (int i = tid; i < n; i += LANES) {
+                            const u64 c = listed[i];
+                            if (mass ? c <= last && (h.few || bin(c) <= r.to) : bin(c) == r.kth) f(c, mass ? worth[i] : 1);
+                        }
+                    } else
+                        of_row([&](float x, int i) __attribute__((always_inline)) {
+                            const u64 c = number(x, i);
+                            if (c <= last) f(c, mass ? coarse(x) : 1);
+                        });
+                };
+                u64 need = list ? h.k - r.before_k : h.k;
+                if (mass) {
+                    u64 w = 0;
+                    double mine = r.sum;   // weight of the first k
+                    if (!list || r.kth < BINS || h.few) {
+                        if (list) {
+#pragma unroll 1
+                            for (int i = tid; i < n; i += LANES)
+                                if (listed[i] <= last && (h.few || bin(listed[i]) == r.kth)) w += worth[i];
+                        } else
+                            of_row([&](float x, int i) __attribute__((always_inline)) {
+                                if (number(x, i) <= last) w += coarse(x);
+                            });
+                        mine = (double)sum_all(w, room);
+                        if (list) mine = (h.few ? 0.0 : r.mass_k) + UNIT * mine;
+                    }
+                    const double least_of = list ? ceil(((double)h.p * mine - r.mass_from) * 0x1p47) : ceil((double)h.p * mine);
+                    need = least_of < 1.0 ? 1 : (u64)least_of;
+                }
+                // (a list's stretches: of the bins that it comes from)
+                const float begin = (float)(r.grid + 1 - (h.few ? 0 : mass ? r.from : r.kth)), wide = 256.f / (h.few ? std::min(r.kth, BINS) + 1 : mass ? r.to - r.from + 1 : 1);
+                const auto stretch = [&](u64 c) __attribute__((always_inline)) { return (int)__builtin_amdgcn_fmed3f((begin - value(c) * h.scale) * wide, 0.f, 255.f); };
+                last = std::min(last, search(need, number(r.top, 0), list, sums, one, counts, found, room, each, stretch));
             }
-            // what is kept, by chunk
+        }
+        // what is kept, by chunk
+        if (list) {
             if (tid < p.chunks) chunks[tid] = own_kept;
             __syncthreads();
             for (int i = tid; i < n; i += LANES) {
@@ -687,45 +743,20 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                 }
             }
             if (h.few && n <= 128) direct = n;
-        }
-    }
-    if (FILTERS && r.how == SEARCH) {
-        const auto each = [&](auto f) __attribute__((always_inline)) {
+        } else {
             for (int c = 0; c < p.chunks; c++) {
-                if (tops[c] == -INFINITY) continue;
-                float x[EACH];
-                load<BF16>(p, row, c, x);
+                u64 w = 0;
+                if (tops[c] > -INFINITY) {
+                    const Units by_chunk(steps, tops[c], h);
+                    float x[EACH];
+                    load<BF16>(p, row, c, x);
 #pragma unroll
-                for (int e = 0; e < EACH; e++)
-                    if (x[e] > -INFINITY) f(x[e], number(x[e], index_of<BF16>(c, e)));
+                    for (int e = 0; e < EACH; e++)
+                        if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += by_chunk.of(x[e]);
+                }
+                w = sum_all(w, room);
+                if (tid == 0) chunks[c] = w;
             }
-        };
-        const Units by_top(steps, r.top, h);
-        // (up to 2^22 of them: units of 2^-38 leave room for the sum)
-        const auto coarse = [&](float x) __attribute__((always_inline)) { return (by_top.of(x) + 256) >> 9; };
-        if (h.k) last = search(h.k, 0, ~0ull, sums, counts, found, [&](auto f) __attribute__((always_inline)) { each([&](float, u64 c) __attribute__((always_inline)) { f(c, 1); }); });
-        if (h.p < 1.f) {
-            u64 w = 0;
-            each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) w += coarse(x); });
-            w = sum_all(w, room);
-            const double need = ceil((double)h.p * (double)w);
-            const u64 border = search(need < 1.0 ? 1 : (u64)need, 0, ~0ull, sums, counts, found, [&](auto f) __attribute__((always_inline)) {
-                each([&](float x, u64 c) __attribute__((always_inline)) { if (c <= last) f(c, coarse(x)); });
-            });
-            last = std::min(last, border);
-        }
-        for (int c = 0; c < p.chunks; c++) {
-            u64 w = 0;
-            if (tops[c] > -INFINITY) {
-                float x[EACH];
-                load<BF16>(p, row, c, x);
-                const Units by_chunk(steps, tops[c], h);
-#pragma unroll
-                for (int e = 0; e < EACH; e++)
-                    if (x[e] > -INFINITY && number(x[e], index_of<BF16>(c, e)) <= last && stays(x[e])) w += by_chunk.of(x[e]);
-            }
-            w = sum_all(w, room);
-            if (tid == 0) chunks[c] = w;
         }
     } else if (r.how == PLAIN) {
         if (tid < p.chunks) chunks[tid] = own.sum;
@@ -779,49 +810,69 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         return;
     }
     // a lane's 16 logits one after the other
-    const Units by_chunk(steps, top, h);
-    u64 w[EACH], mine = 0;
     const int first = chunk * CHUNK + tid * EACH;
-    float x[EACH];
-    if (p.aligned && first + EACH <= p.vocab) {
-        constexpr int V = VEC<BF16>;
-#pragma unroll
-        for (int i = 0; i < EACH; i += V) load_vec<BF16>(p, row, first + i, x + i);
-    } else {
-#pragma unroll
-        for (int e = 0; e < EACH; e++) x[e] = first + e < p.vocab ? load1<BF16>(p, row, first + e) : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        x[e] = fmaxf(x[e], -INFINITY);
-        const bool in = x[e] > -INFINITY && (r.how == PLAIN || (number(x[e], first + e) <= last && stays(x[e]) && (r.how == SEARCH || h.few || r.grid - place(x[e], h.scale) <= r.to)));
-        w[e] = in ? by_chunk.of(x[e]) : 0;
-        mine += w[e];
-    }
-    u64 total;
-    u64 before = scan_all(mine, room, total) - mine;   // sums ahead of the lane
+    const auto kept = [&](float x, int i) __attribute__((always_inline)) {
+        return x > -INFINITY && (r.how == PLAIN || (number(x, i) <= last && stays(x) && (r.how == SEARCH || h.few || r.grid - place(x, h.scale) <= r.to)));
+    };
+    u64 total, mine = 0, before = 0;
     int hit = -1, some = -1;
     u64 hit_w = 0, some_w = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        before += w[e];
-        if (w[e]) {
-            some = first + e;
-            some_w = w[e];
+    const auto look = [&](int i, u64 w) __attribute__((always_inline)) {
+        const u64 ahead = before;
+        before += w;
+        if (w) {
+            some = i;
+            some_w = w;
         }
-        if (hit < 0 && w[e] && before > want) {
-            hit = first + e;
-            hit_w = w[e];
+        if (ahead <= want && before > want) {   // (of all lanes' tokens one, or none)
+            hit = i;
+            hit_w = w;
+        }
+    };
+    if (Weights::fits(top, h)) {
+        const Weights by_chunk(steps, top, h);
+        float x[EACH];
+        u64 w[EACH];
+        if (p.aligned && first + EACH <= p.vocab) {
+            constexpr int V = VEC<BF16>;
+#pragma unroll
+            for (int i = 0; i < EACH; i += V) load_vec<BF16>(p, row, first + i, x + i);
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; e++) x[e] = first + e < p.vocab ? load1<BF16>(p, row, first + e) : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            x[e] = fmaxf(x[e], -INFINITY);
+            w[e] = kept(x[e], first + e) ? units(by_chunk.of(x[e])) : 0;
+            mine += w[e];
+        }
+        before = scan_all(mine, room, total) - mine;   // sums ahead of the lane
+#pragma unroll
+        for (int e = 0; e < EACH; e++) look(first + e, w[e]);
+    } else {   // (rare: not unrolled, what is not fetched costs nothing)
+        const auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll 1
+            for (int i = first; i < first + EACH; i++) {
+                const float x = load_one<BF16>(p, row, i);
+                f(i, kept(x, i) ? units(weight(x, top, h.by_two)) : 0);
+            }
+        };
+        each([&](int, u64 w) __attribute__((always_inline)) { mine += w; });
+        before = scan_all(mine, room, total) - mine;
+        each(look);
+    }
+    (void)total;
+    if (!__syncthreads_or(hit >= 0)) {   // (where rounding left none, the last token that is kept)
+        const int end = over_all(some, room_n, [](int a, int b) { return a > b ? a : b; });
+        if (some == end) {
+            hit = some;
+            hit_w = some_w;
         }
     }
-    // the first hit; where rounding left none, the last token that is kept
-    (void)total;
-    const u64 best = over_all(hit < 0 ? ~0ull : (u64)hit, room, [](u64 a, u64 b) { return a < b ? a : b; });
-    const u64 end = over_all((u64)(some + 1), room, [](u64 a, u64 b) { return a > b ? a : b; });
-    const bool is = best != ~0ull ? hit == (int)best : some + 1 == (int)end && some >= 0;
-    if (is) {
-        p.token[row] = best != ~0ull ? hit : some;
-        if (p.prob) p.prob[row] = (float)((double)(best != ~0ull ? hit_w : some_w) * factor[chunk] / target[1]);
+    if (hit >= 0) {
+        p.token[row] = hit;
+        if (p.prob) p.prob[row] = (float)((double)hit_w * factor[chunk] / target[1]);
     }
 }
 
