@@ -647,9 +647,9 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
 // A wave per (seat, key / value head), D / 8 lanes to a key, its dot products in the vector unit: as few keys as these would leave the matrix unit's tiles mostly empty, and without LDS
 // four times as many waves run at a time, which is what hides the latency of so little (10,752 items of some nine keys of 256 dims: 95 us as tiles).
 // Probabilities stay 32-bit.  Then the pieces that the content's items left are added, and the row is written.
-template <int D, int RM, bool CAP>
+template <int D, bool CAP>
 __device__ __forceinline__ void last_words(const Params& p) {
-    constexpr int LPK = D / 8, G = 64 / LPK, U = 4;   // lanes of a key, keys of a load, loads ahead
+    constexpr int RM = SEAT_LAST_HEADS, LPK = D / 8, G = 64 / LPK, U = 4;   // heads, lanes of a key, keys of a load, loads ahead
     typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, mine = lane / LPK, col = lane % LPK * 8;
     // (an item is read a round ahead, the first one beside the count: there is room for it, whatever it holds)
@@ -879,17 +879,16 @@ __device__ __forceinline__ void join(const Params& p, int block) {
     }
 }
 
-// What comes behind the contents' and the own keys' pieces: workgroups ahead of `last_blocks` speak last words, the others join pieces (RM 0: only these).  One launch up to two heads; with
-// more the last words' registers would leave the others too few waves.
-template <int D, int RM, bool CAP>
-__global__ __launch_bounds__(256, RM == 0 ? 8 : RM == 2 ? 4 : 2) void seats_finish_kernel(const Params p) {
-    if constexpr (RM > 0) {
-        if (RM > 2 || (int)blockIdx.x < p.last_blocks) {
-            last_words<D, RM, CAP>(p);
+// What comes behind the contents' and the own keys' pieces: workgroups ahead of `last_blocks` speak last words (WORDS: there may be some), the others join pieces.
+template <int D, bool WORDS, bool CAP>
+__global__ __launch_bounds__(256, WORDS ? 4 : 8) void seats_finish_kernel(const Params p) {
+    if constexpr (WORDS) {
+        if ((int)blockIdx.x < p.last_blocks) {
+            last_words<D, CAP>(p);
             return;
         }
     }
-    if constexpr (RM <= 2) join<D>(p, blockIdx.x - p.last_blocks);
+    join<D>(p, blockIdx.x - p.last_blocks);
 }
 
 // Workgroups that walk a list: two rounds of those that run at a time (one that finds nothing still takes a microsecond of a place)
@@ -907,17 +906,13 @@ int launch(Params p, const spinf_seats_attn_args* a, hipStream_t s) {
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
-        p.last_blocks = (int)std::min<int64_t>((a->rooms[3] * p.hkv + 3) / 4, p.group <= 2 ? 1024 : 512);   // (as many waves as run at a time)
+        p.last_blocks = (int)std::min<int64_t>((a->rooms[3] * p.hkv + 3) / 4, 1024);   // (as many waves as run at a time)
         p.join_x = std::min(p.rows, 4096 / (D / 64));
         const int x = p.join_x * (D / 64);
         p.join_y = x >= 1024 ? 1 : std::min(p.hq, (1024 + x - 1) / x);
-        if (p.last_blocks && p.group <= 2) hipLaunchKernelGGL((seats_finish_kernel<D, 2, CAP>), dim3((unsigned)(p.last_blocks + x * p.join_y)), dim3(256), 0, s, p);
-        else {
-            if (p.last_blocks && p.group <= 4) hipLaunchKernelGGL((seats_finish_kernel<D, 4, CAP>), dim3((unsigned)p.last_blocks), dim3(256), 0, s, p);
-            else if (p.last_blocks) hipLaunchKernelGGL((seats_finish_kernel<D, 8, CAP>), dim3((unsigned)p.last_blocks), dim3(256), 0, s, p);
-            p.last_blocks = 0;
-            hipLaunchKernelGGL((seats_finish_kernel<D, 0, CAP>), dim3((unsigned)(x * p.join_y)), dim3(256), 0, s, p);
-        }
+        const dim3 grid((unsigned)(p.last_blocks + x * p.join_y));
+        if (D >= 128 && p.last_blocks) hipLaunchKernelGGL((seats_finish_kernel<D, D >= 128, CAP>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((seats_finish_kernel<D, false, CAP>), grid, dim3(256), 0, s, p);
         e = hipGetLastError();
     }
     return e == hipSuccess ? SPINF_OK : spinf_fail(SPINF_E_HIP, "seats_attn: launch: %s", hipGetErrorString(e));

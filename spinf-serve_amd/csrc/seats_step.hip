@@ -280,8 +280,23 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
     });
     const int total = p.first[R];
     if (tid == 0) first[R] = total;
+    const int most_rows = (long)total * kd.hq > 32 * seats_wave_places(kd.d) ? 32 : SEAT_WAVE_ROWS;   // below a content, for waves that divide the tiles
     // (a seat of many rows reads its content for itself)
     const auto alone = [&](int r) __attribute__((always_inline)) { return took[r] * group > SEAT_SHARED_ROWS; };
+    // ---- tokens on few keys of their own
+    const auto few_keys = [&](int r) __attribute__((always_inline)) { const int L = stay[r] + 1; return took[r] == 1 && (L < far ? L : far) <= SEAT_LAST_KEYS; };
+    bool by_vector = false;
+    if (seats_last(group, kd.d)) {
+        long of[2] = {0, 0}, in_all[2];   // tokens, keys
+        each_seat([&](int r) __attribute__((always_inline)) {
+            if (few_keys(r)) {
+                of[0]++;
+                of[1] += seats_least(stay[r] + 1, far);
+            }
+        });
+        scan(of, in_all, room, 0l, [](long a, long b) { return a + b; });
+        by_vector = seats_last_pays(in_all[0], in_all[1], kd.hkv);
+    }
     // ---- groups: seats with new tokens below one content, one after the other (seats without any in between do not part them)
     {   // the last seat with new tokens ahead of each: one more than its index
         const int per = (R + LANES - 1) / LANES, from = seats_least(R, tid * per), to = seats_least(R, from + per);
@@ -324,7 +339,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         if (c < 0 || alone(r)) return -1;
         const int P = p.shared[3 * c], rows = (first[heads[g + 1]] - first[r]) * group, lo = most(0, P + low[g] - far + 1);
         if (lo >= P) return -1;
-        const bool few = rows <= SEAT_WAVE_ROWS;
+        const bool few = rows <= most_rows;
         tiles = seats_up(P, PAGED_TILE) - lo / PAGED_TILE;
         blocks = seats_up(rows, few ? 32 : deep);
         return few ? 0 : 2;
@@ -336,7 +351,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         if (n == 0) return -1;
         tiles = seats_up(L, PAGED_TILE) - lo / PAGED_TILE;
         blocks = 1;
-        if (n == 1 && group <= SEAT_LAST_HEADS && L - lo <= SEAT_LAST_KEYS) return 3;
+        if (by_vector && few_keys(r)) return 3;
         if (alone(r)) {
             const int c = content[r], P = c >= 0 ? p.shared[3 * c] : 0, from = most(0, P + stay[r] - far + 1);
             shared = from < P ? seats_up(P, PAGED_TILE) - from / PAGED_TILE : 0;
@@ -389,8 +404,8 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
             long cost = LONG_MAX;
 #pragma unroll
             for (int j = 0; j < SIZES; j++) {
-                // (a workgroup's start and end are worth some tiles; what a piece leaves, written and read again, a 24th of a tile's time over the whole GPU)
-                const long n = (long)all[j] * kd.hkv, rounds = (n + places - 1) / places, here = 24 * rounds * (size[j] + (y ? 4 : 12)) + (y ? n : n / 4);
+                // (a workgroup's start and end are worth some tiles; what a piece leaves, written and read again, a 12th of a tile's time over the whole GPU: a 24th made pieces of eight tiles of 24 contents with 112 rows each, 76 us for 69)
+                const long n = (long)all[j] * kd.hkv, rounds = (n + places - 1) / places, here = 24 * rounds * (size[j] + (y ? 4 : 12)) + (y ? 2 * n : n / 4);
                 if (here < cost) {
                     cost = here;
                     best[y] = size[j];
@@ -507,7 +522,7 @@ void rooms(const spinf_seats_args* a, const spinf_seats_kind& k, int64_t out[5])
     out[0] = by_wave + 3 * A;                                   // (a content's rows: two blocks at most)
     out[1] = (SEAT_SHARED_ROWS + 31) / 32 * A;
     out[2] = block ? by_block + 2 * (rows * group / 128 + A) : 0;
-    out[3] = group <= SEAT_LAST_HEADS ? A : 0;
+    out[3] = seats_last((int)group, k.d) && seats_last_pays(A, 0, k.hkv) ? A : 0;
     // tokens x pieces: those of a set's blocks share the places; a token is in two sets at most
     out[4] = 2 * rows + (32 / group + 1) * by_wave + (block ? (128 / group + 1) * by_block : 0);
 }

@@ -612,6 +612,32 @@ def test_caches_past_32_bits(dev):
     assert all(torch.equal(x, y) for x, y in zip(*got))
 
 
+# many tokens on few keys of their own: as SHAPES; whether they are the vector unit's
+MANY = [
+    ([301, 0, 77], [0] * 30 + [1] * 10 + [2] * 35 + [-1] * 5, [1 + i % 23 for i in range(80)], [1] * 80, 16, (16, 8, 256), 0, True),
+    ([470, 90], [0] * 60 + [1] * 60, [3 + i % 40 for i in range(120)], [1] * 120, 48, (16, 16, 128), 0, True),
+    ([470, 90], [0] * 60 + [1] * 60, [3 + i % 120 for i in range(120)], [1] * 120, 48, (16, 16, 128), 0, False),
+    ([200], [0] * 90, [120 + i for i in range(90)], [1] * 90, 16, (16, 8, 128), 20, False),   # (50 x 20 keys are more than 90 x 8)
+    ([64], [0] * 170, [1 + i % 9 for i in range(170)], [int(i % 8 > 0) for i in range(170)], 16, (8, 4, 512), 0, False),
+    ([64], [0] * 190, [1 + i % 9 for i in range(190)], [int(i % 8 > 0) for i in range(190)], 16, (8, 4, 512), 0, True),
+    ([500], [0] * 70, [4 + i % 20 + (200 if i % 9 == 0 else 0) for i in range(70)], [1 + 2 * (i % 6 == 5) for i in range(70)], 80, (32, 16, 128), 0, True),
+    ([], [-1] * 700, [1 + i % 3 for i in range(700)], [1] * 700, 16, (1, 1, 256), 0, True),
+    ([300], [0] * 300, [5] * 300, [1] * 300, 16, (8, 8, 64), 0, False),
+    ([300] * 12, [i // 14 for i in range(168)], [20] * 168, [1] * 168, 16, (24, 8, 128), 0, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stored,content,own,new,page,heads,window,vector", MANY)
+def test_many_tokens_on_few_keys(dev, stored, content, own, new, page, heads, window, vector):
+    test_work_lists_are_the_dense_mask(dev, stored, content, own, new, page, heads, window)
+    for order, softcap in (("heads", 0.0), ("rows", 20.0)):
+        test_attention_against_the_oracle(dev, stored, content, own, new, page, heads, window, order, softcap)
+    s, _ = make(dev, stored, own, new, page, heads, content, window=window)
+    at = ss._layout(s._geo)["lists"][0][4]
+    assert (int(s._work[at + 3]) > 0) == vector
+
+
 # ------------------------------------------------------------------------------------------------ together
 class Loop:
     """the tokens of three contents' seats, drawn and read: step, rotation into the cache, attention, head, draw"""
