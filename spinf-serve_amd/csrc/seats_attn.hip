@@ -9,11 +9,11 @@
 // Kernels (lists of csrc/seats.h):
 //   wave    few rows (up to 64 below one content, up to 32 of a seat): four waves (three at 512 dims) divide the tiles, or, where a seat's keys are few, take an item each.
 //   block   many rows: four waves with 32 rows each on shared double-buffered tiles.
-//   finish  one token on few keys of its own, which then adds what its content's pieces left; the pieces of all other rows; rows behind the step's last become zeros.
+//   finish  in steps of many such: one token on few keys of its own, which then adds what its content's pieces left; the pieces of all other rows; rows behind the step's last become zeros.
 // The lists' lengths are known on the GPU alone: grids have a bounded size and walk the lists.  A list without items costs 3 to 5 us of a launch.
 //
-// What bounds it.  24 answers below 301 tokens, 24 us: latency, three launches of one short item to a place each.  24 x 56 branches of one token on 470 + 9 keys, 79 us: latency, the keys
-// alone would be 40 us.  48 answers below 65,536 tokens, 161 us (0.48 PFLOP/s), and 35 questions of 150 tokens in a window of 1,024, 169 us (0.52): the turns of a tile's products and its
+// What bounds it.  24 answers below 301 tokens, 18 us: latency, three launches of one short item to a place each.  24 x 56 branches of one token on 470 + 9 keys, 77 us: the keys
+// alone would be 40 us, pieces written and read again are half as much.  48 answers below 65,536 tokens, 161 us (0.48 PFLOP/s), and 35 questions of 150 tokens in a window of 1,024, 169 us (0.52): the turns of a tile's products and its
 // softmax; the matrix unit is busy a third of the time, and at 256 dims two waves to a SIMD are all that fit: with 64 rows to a wave the accumulators spill, and eight waves
 // on the same tiles (four buffers) go in step, with nothing beside the softmax to feed the matrix unit: 146 for 129 us of the block kernel, 279 for 191.
 //
@@ -645,7 +645,8 @@ __global__ __launch_bounds__(256 * (D / DV), DV == 256 ? 2 : 3) void seats_block
 
 // ------------------------------------------------------------------------------------------------ one token on few keys of its own: the last word
 // A wave per (seat, key / value head), D / 8 lanes to a key, its dot products in the vector unit: as few keys as these would leave the matrix unit's tiles mostly empty, and without LDS
-// four times as many waves run at a time, which is what hides the latency of so little (10,752 items of some nine keys of 256 dims: 95 us as tiles).
+// four times as many waves run at a time, which is what hides the latency of so little (10,752 items of some nine keys of 256 dims: 95 us as tiles, half of it so; csrc/seats.h has both
+// sides' times).
 // Probabilities stay 32-bit.  Then the pieces that the content's items left are added, and the row is written.
 template <int D, bool CAP>
 __device__ __forceinline__ void last_words(const Params& p) {
