@@ -789,6 +789,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         return;
     }
     const u64 want = target[0] > 0.0 ? (u64)target[0] : 0;
+    const auto chance = [&](float x) __attribute__((always_inline)) { return (float)(weight(x, r.top, h.by_two) / target[1]); };   // (units would round a small one)
     const float top = tops[chunk];
     if (FILTERS && direct) {   // the token among those that are listed: each adds up what lies before it
         const unsigned at = tid < direct ? (unsigned)listed[tid] : 0;
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
         }
         if (hit) {
             p.token[row] = at;
-            if (p.prob) p.prob[row] = (float)((double)mine_w * factor[chunk] / target[1]);
+            if (p.prob) p.prob[row] = chance(value(listed[tid]));
         }
         return;
     }
@@ -816,18 +817,11 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     };
     u64 total, mine = 0, before = 0;
     int hit = -1, some = -1;
-    u64 hit_w = 0, some_w = 0;
     const auto look = [&](int i, u64 w) __attribute__((always_inline)) {
         const u64 ahead = before;
         before += w;
-        if (w) {
-            some = i;
-            some_w = w;
-        }
-        if (ahead <= want && before > want) {   // (of all lanes' tokens one, or none)
-            hit = i;
-            hit_w = w;
-        }
+        if (w) some = i;
+        if (ahead <= want && before > want) hit = i;   // (of all lanes' tokens one, or none)
     };
     if (Weights::fits(top, h)) {
         const Weights by_chunk(steps, top, h);
@@ -865,14 +859,11 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     (void)total;
     if (!__syncthreads_or(hit >= 0)) {   // (where rounding left none, the last token that is kept)
         const int end = over_all(some, room_n, [](int a, int b) { return a > b ? a : b; });
-        if (some == end) {
-            hit = some;
-            hit_w = some_w;
-        }
+        if (some == end) hit = some;
     }
     if (hit >= 0) {
         p.token[row] = hit;
-        if (p.prob) p.prob[row] = (float)((double)hit_w * factor[chunk] / target[1]);
+        if (p.prob) p.prob[row] = chance(load1<BF16>(p, row, hit));
     }
 }
 

@@ -68,8 +68,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     likely as the likeliest.  The token drawn is the first, in the vocabulary's order, up to which the kept probabilities add up to more than u of their sum.  return_prob: also its
     probability among the kept ones, [rows] fp32.
     temperature, top_k, top_p, min_p: numbers (taken as 32 bits hold them), or [rows] device tensors (fp32; top_k int32).  Temperature 0: the largest logit.  Logits of -inf and NaN are never
-    drawn; a row without any other, or with a setting that is negative or NaN, gives -1 (probability 0).  Probabilities and their sums are 64-bit: the same call gives the same
-    tokens whatever rows share it."""
+    drawn; a row without any other, or with a setting that is negative or NaN, gives -1 (probability 0).  Probabilities and their sums are 64-bit, in steps of 2^-47 of the largest
+    of 8,192 neighbours (one of less than half a step is none): the same call gives the same tokens whatever rows share it."""
     given, numbers = [], []
     for (name, _), x in zip(_SETTINGS, (temperature, top_k, top_p, min_p)):
         given.append(x if isinstance(x, torch.Tensor) else None)

@@ -245,3 +245,15 @@ def test_borders_among_many_tokens(dev, kind, dtype):
             values = torch.from_numpy(x.astype(np.float32)).to(dtype).double().numpy()
             for r in range(rows):
                 assert int(token[r]) in [oracle_sample.draw(values[r], u[r], top_k=900, top_p=0.5 + off)[0] for off in (-1e-9, 1e-9)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_chance_of_an_unlikely_token(dev, dtype):
+    """the first token kept, drawn by u = 0, where it is some 10^-8 and 10^-12 of the whole"""
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((6, 20000))
+    x[:, 3] = x.max(1) - np.array([10, 17, 18.5, 20, 25, 28])
+    x[:, :3] = -np.inf
+    for how in (dict(), dict(top_k=20000 - 3), dict(top_p=1.0, min_p=1e-14), dict(top_k=19000, temperature=1.1)):
+        check(dev, x, dtype, np.zeros(6), how)
