@@ -8,7 +8,7 @@
 //
 // Bound by latency: kernels of one workgroup of 8 waves, whose lanes hold a share of the at most 2,048 seats; pages, items and rows are dealt out to lanes by a search in the sums.
 //   books   three running sums over the seats; 64 seats 6 us, 1,344 seats 12
-//   lists   of each head geometry in a workgroup of its own: 17 us for 24 seats below one content, 30 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
+//   lists   of each head geometry in a workgroup of its own: 14 us for 24 seats below one content, 27 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
 //           more registers than there are.
 //   rows    over the whole GPU, where a step has more than SEATS_ROWS_AT_ONCE rows (prompts of 100,800 rows: 5 us, 12 with the books)
 #include <hip/hip_runtime.h>
@@ -19,6 +19,7 @@
 #include "spinf_tree.h"
 #include "common.h"
 #include "seats.h"
+#include "lanes.h"
 
 namespace {
 
@@ -93,6 +94,25 @@ __device__ __forceinline__ void store(int* items, int at, const SeatItem& it) {
         const SeatSpan& s = it.span[i];
         p[2 + 2 * i] = make_int4(s.tab, s.L, s.kt0, s.tiles);
         p[3 + 2 * i] = make_int4(s.flo, s.fhi, s.own, 0);
+    }
+}
+
+// Sums over the workgroup alone
+template <int N, class T>
+__device__ __forceinline__ void add_up(const T (&x)[N], T (&all)[N], long (*room)[WAVES]) {
+    T y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = over_lanes<64>(x[i], [](T a, T b) { return a + b; });
+    __syncthreads();   // (the room may be read still)
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) room[i][threadIdx.x >> 6] = (long)y[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        all[i] = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) all[i] += (T)room[i][w];
     }
 }
 
@@ -257,7 +277,7 @@ __device__ __forceinline__ void running(int* const (&a)[N], int n, long (*room)[
 template <int MOST>
 __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
     __shared__ long room[7][WAVES];
-    __shared__ int stay[MOST], took[MOST], content[MOST], first[MOST + 1];
+    __shared__ int stay[MOST], took[MOST], content[MOST], first[MOST + 1], stored[MOST], listed[MOST];   // stored, listed: keys of the seat's content, where its page list begins
     __shared__ int heads[MOST + 1], low[MOST], high[MOST], of_group[MOST + 1], cut[MOST];   // of groups: seats one after the other that share their content; cut: pieces of its keys
     __shared__ int sums[5][MOST + 1];
     __shared__ int best[2];
@@ -273,7 +293,10 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         took[r] = p.took[r];
         first[r] = p.first[r];
         const int c = p.content[r];
-        content[r] = c < 0 || c >= p.contents ? -1 : c;
+        const bool below = c >= 0 && c < p.contents;
+        content[r] = below ? c : -1;
+        stored[r] = below ? p.shared[3 * c] : 0;
+        listed[r] = below ? p.shared[3 * c + 2] : 0;
         heads[r] = took[r] ? r + 1 : 0;
         low[r] = INT_MAX;
         high[r] = 0;
@@ -294,7 +317,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
                 of[1] += seats_least(stay[r] + 1, far);
             }
         });
-        scan(of, in_all, room, 0l, [](long a, long b) { return a + b; });
+        add_up(of, in_all, room);
         by_vector = seats_last_pays(in_all[0], in_all[1], kd.hkv);
     }
     // ---- groups: seats with new tokens below one content, one after the other (seats without any in between do not part them)
@@ -337,7 +360,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         const int r = heads[g], c = content[r];
         blocks = tiles = 0;
         if (c < 0 || alone(r)) return -1;
-        const int P = p.shared[3 * c], rows = (first[heads[g + 1]] - first[r]) * group, lo = most(0, P + low[g] - far + 1);
+        const int P = stored[r], rows = (first[heads[g + 1]] - first[r]) * group, lo = most(0, P + low[g] - far + 1);
         if (lo >= P) return -1;
         const bool few = rows <= most_rows;
         tiles = seats_up(P, PAGED_TILE) - lo / PAGED_TILE;
@@ -353,7 +376,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         blocks = 1;
         if (by_vector && few_keys(r)) return 3;
         if (alone(r)) {
-            const int c = content[r], P = c >= 0 ? p.shared[3 * c] : 0, from = most(0, P + stay[r] - far + 1);
+            const int P = stored[r], from = most(0, P + stay[r] - far + 1);
             shared = from < P ? seats_up(P, PAGED_TILE) - from / PAGED_TILE : 0;
             blocks = seats_up(rows, deep);
             return 2;
@@ -380,17 +403,18 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         work[0] += sort == 0 ? n : 0;
         work[1] += sort == 2 ? n : 0;
     });
-    scan(work, all_work, room, 0l, [](long a, long b) { return a + b; });
+    add_up(work, all_work, room);
     if (tid < 2) best[tid] = 1;
     constexpr int SIZES = 6;
 #pragma unroll
     for (int y = 0; y < 2; y++) {
         if (all_work[y] == 0) continue;
-        const int places = y ? seats_block_places(kd.d) : seats_wave_places(kd.d);
+        static_assert((PAGED_PLACES & (PAGED_PLACES - 1)) == 0, "divisions by places are shifts");
+        const int places = y ? seats_block_places(kd.d) : seats_wave_places(kd.d), shift = __builtin_ctz(places);
         int size[SIZES], items[SIZES], all[SIZES];
 #pragma unroll
         for (int j = 0; j < SIZES; j++) {
-            const long tiles = (all_work[y] * kd.hkv * (8 + j * (j + 1) / 2) / 8 + places - 1) / places;   // 1, 1 1/8, 1 3/8, 1 3/4, 2 1/4, 2 7/8
+            const long tiles = ((all_work[y] * kd.hkv * (8 + j * (j + 1) / 2) >> 3) + places - 1) >> shift;   // 1, 1 1/8, 1 3/8, 1 3/4, 2 1/4, 2 7/8
             size[j] = most(y ? SEAT_BLOCK_TILES : SEAT_WAVE_TILES, (int)(tiles < LOTS ? tiles : LOTS));
             items[j] = 0;
         }
@@ -399,13 +423,13 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
 #pragma unroll
                 for (int j = 0; j < SIZES; j++) items[j] += blocks * seats_up(tiles, size[j]);
         });
-        scan(items, all, room, 0, [](int a, int b) { return a + b; });
+        add_up(items, all, room);
         if (tid == 0) {
             long cost = LONG_MAX;
 #pragma unroll
             for (int j = 0; j < SIZES; j++) {
                 // (a workgroup's start and end are worth some tiles; what a piece leaves, written and read again, a 12th of a tile's time over the whole GPU: a 24th made pieces of eight tiles of 24 contents with 112 rows each, 76 us for 69)
-                const long n = (long)all[j] * kd.hkv, rounds = (n + places - 1) / places, here = 24 * rounds * (size[j] + (y ? 4 : 12)) + (y ? 2 * n : n / 4);
+                const long n = (long)all[j] * kd.hkv, rounds = (n + places - 1) >> shift, here = 24 * rounds * (size[j] + (y ? 4 : 12)) + (y ? 2 * n : n / 4);
                 if (here < cost) {
                     cost = here;
                     best[y] = size[j];
@@ -430,13 +454,13 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
     const int waves = sums[0][G], blocks_in_all = sums[1][G];
     for (int i = tid; i < waves + blocks_in_all; i += LANES) {
         const int y = i >= waves, x = y ? i - waves : i, size = y ? deep : 32;
-        const int g = find(sums[y], G, x), r = heads[g], c = content[r], j = x - sums[y][g];
+        const int g = find(sums[y], G, x), r = heads[g], j = x - sums[y][g];
         int blocks, tiles;
         group_set(g, blocks, tiles);
-        const int P = p.shared[3 * c], tok0 = first[r], T = first[heads[g + 1]] - tok0, kt = seats_up(P, PAGED_TILE) - tiles;
+        const int P = stored[r], tok0 = first[r], T = first[heads[g + 1]] - tok0, kt = seats_up(P, PAGED_TILE) - tiles;
         const int s = j / blocks, b = j - s * blocks, n = cut[g];
         const int from = (int)((long)tiles * s / n), to = (int)((long)tiles * (s + 1) / n);
-        const SeatItem it = {tok0, T, size * b, s, 0, {}, {{p.shared[3 * c + 2], P, kt + from, to - from, most(0, P + high[g] - far + 1), P - 1, 0, 0}, {}}};
+        const SeatItem it = {tok0, T, size * b, s, 0, {}, {{listed[r], P, kt + from, to - from, most(0, P + high[g] - far + 1), P - 1, 0, 0}, {}}};
         if (x < (y ? kd.room[2] : kd.room[0])) store(y ? kd.block : kd.wave, x, it);
     }
     __syncthreads();
@@ -491,7 +515,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         const int s = x / blocks, b = x - s * blocks, size = y == 2 ? deep : 32;
         const int t0 = b * size / group, t1 = seats_least(n - 1, (b * size + size - 1) / group);   // its first and its last token
         // tiles of the content, then of its own keys, that this block's rows see; the piece's share of them
-        const int c = content[r], P = shared ? p.shared[3 * c] : 0;
+        const int P = shared ? stored[r] : 0;
         const int lo = most(0, stay[r] + t0 - far + 1), kt = lo / PAGED_TILE, own = seats_up(stay[r] + t1 + 1, PAGED_TILE) - kt;
         const int lo2 = most(0, P + stay[r] + t0 - far + 1), kt2 = lo2 / PAGED_TILE, theirs = lo2 < P ? seats_up(P, PAGED_TILE) - kt2 : 0;
         const int from = (int)((long)(own + theirs) * s / pieces), to = (int)((long)(own + theirs) * (s + 1) / pieces);
@@ -499,7 +523,7 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
         const int ahead = cut[of_group[r]];
         SeatItem it = {first[r], n, b * size, ahead + s, ahead + pieces == 1, {}, {mine, {}}};
         if (theirs > 0 && from < theirs) {
-            it.span[0] = {p.shared[3 * c + 2], P, kt2 + from, seats_least(to, theirs) - from, most(0, P + stay[r] + t1 - far + 1), P - 1, 0, 0};
+            it.span[0] = {listed[r], P, kt2 + from, seats_least(to, theirs) - from, most(0, P + stay[r] + t1 - far + 1), P - 1, 0, 0};
             it.span[1] = mine;
         }
         const int at = y == 0 ? waves + j : y == 1 ? j : blocks_in_all + j;
