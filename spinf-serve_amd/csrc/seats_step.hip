@@ -8,7 +8,7 @@
 //
 // Bound by latency: kernels of one workgroup of 8 waves, whose lanes hold a share of the at most 2,048 seats; pages, items and rows are dealt out to lanes by a search in the sums.
 //   books   three running sums over the seats; 64 seats 6 us, 1,344 seats 12
-//   lists   of each head geometry in a workgroup of its own: 14 us for 24 seats below one content, 27 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
+//   lists   of each head geometry in a workgroup of its own: 16 us for 24 seats below one content, 27 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
 //           more registers than there are.
 //   rows    over the whole GPU, where a step has more than SEATS_ROWS_AT_ONCE rows (prompts of 100,800 rows: 5 us, 12 with the books)
 #include <hip/hip_runtime.h>
