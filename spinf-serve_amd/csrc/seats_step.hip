@@ -7,8 +7,8 @@
 // seat, whatever order the lanes run in.  Pushed in the reverse of the order they are popped in: a step that takes back what the last one added leaves stack and tables as they were.
 //
 // Bound by latency: kernels of one workgroup of 8 waves, whose lanes hold a share of the at most 2,048 seats; pages, items and rows are dealt out to lanes by a search in the sums.
-//   books   three running sums over the seats; 64 seats 6 us, 1,344 seats 12
-//   lists   of each head geometry in a workgroup of its own: 16 us for 24 seats below one content, 27 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
+//   books   three running sums over the seats; 64 seats 6 us, 1,344 seats 11
+//   lists   of each head geometry in a workgroup of its own: 16 us for 24 seats below one content, 25 us for 24 x 56 (once a step for all layers).  In one kernel with the books they need
 //           more registers than there are.
 //   rows    over the whole GPU, where a step has more than SEATS_ROWS_AT_ONCE rows (prompts of 100,800 rows: 5 us, 12 with the books)
 #include <hip/hip_runtime.h>
@@ -116,7 +116,9 @@ __device__ __forceinline__ void add_up(const T (&x)[N], T (&all)[N], long (*room
     }
 }
 
-// Places and positions of rows
+// Places and positions of rows.  Of more than 512 seats the first rows of each are its lane's own, later ones are searched for (1,344 seats of one row: 11 us, by search alone 12; 64 seats of
+// four 6.6, by search 5.8)
+constexpr int FIRST_ROWS = 4;
 __device__ __forceinline__ void place_row(const Params& p, int row, int total, int seat, int first, int stay, int content) {
     long slot = -1;
     int pos = 0;
@@ -243,9 +245,24 @@ __global__ __launch_bounds__(LANES) void seats_step_kernel(const Params p) {
 
     __syncthreads();
     if (p.rows > SEATS_ROWS_AT_ONCE) return;
-    for (int row = tid; row < p.rows; row += LANES) {
+    constexpr int BY_SEAT = SPT > 1 ? FIRST_ROWS : 0;
+    bool more = SPT == 1;
+    if (BY_SEAT) {
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int r = tid * SPT + i;
+            if (r < R) {
+#pragma unroll
+                for (int j = 0; j < BY_SEAT; j++)
+                    if (j < want[i]) place_row(p, first[r] + j, total, r, first[r], stay[r], content[r]);
+                more |= want[i] > BY_SEAT;
+            }
+        }
+        more = __syncthreads_or(more);
+    }
+    for (int row = more ? tid : total + tid; row < p.rows; row += LANES) {
         const int seat = row < total ? find(first, R, row) : 0;
-        place_row(p, row, total, seat, first[seat], stay[seat], content[seat]);
+        if (row >= total || row - first[seat] >= BY_SEAT) place_row(p, row, total, seat, first[seat], stay[seat], content[seat]);
     }
 }
 
@@ -531,9 +548,18 @@ __global__ __launch_bounds__(LANES) void seats_lists_kernel(const Params p) {
     }
     if (p.rows > SEATS_ROWS_AT_ONCE) return;
     __syncthreads();
-    for (int row = tid; row <= p.rows; row += LANES) {
+    constexpr int BY_SEAT = MOST > LANES ? FIRST_ROWS : 0;
+    bool more = !BY_SEAT;
+    if (BY_SEAT) {
+        each_seat([&](int r) __attribute__((always_inline)) {
+            for (int j = 0; j < seats_least(took[r], BY_SEAT); j++) place_parts(p, kd, first[r] + j, total, r, first[r]);
+            more |= took[r] > BY_SEAT;
+        });
+        more = __syncthreads_or(more);
+    }
+    for (int row = more ? tid : total + tid; row <= p.rows; row += LANES) {
         const int seat = row < total ? find(first, R, row) : 0;
-        place_parts(p, kd, row, total, seat, first[seat]);
+        if (row >= total || row - first[seat] >= BY_SEAT) place_parts(p, kd, row, total, seat, first[seat]);
     }
 }
 
