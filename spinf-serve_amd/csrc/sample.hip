@@ -357,7 +357,7 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
     __syncthreads();
     if (mine.top > -INFINITY) atomicAdd(&found[3], (int)mine.at);
     double mass = 0.0;
-    int n = 0;
+    int n = 0, above = 0, below = BINS;   // bins of min-p's border, and of two numbers to either side of it
     {   // (the halves' chunks and their order are always the same)
         constexpr int AHEAD = 16;
         for (int c0 = half; c0 < p.chunks; c0 += 2 * AHEAD) {
@@ -372,6 +372,18 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
                 const bool on = x >= 0 && x < BINS - 1 && b < BINS - 1;
                 w[i] = on && !h.few ? p.hist_w[at] : 0;
                 m[i] = on && h.k ? p.hist_n[at] : 0;
+            }
+            if (c0 == half && h.least > 0.f && !h.few) {   // (while the bins are on their way)
+                const double border = (double)r.top + log((double)h.least) / h.inv;
+                if (border == border && r.top < INFINITY) {
+                    float x = (float)fmin(fmax(border, -3e38), 3e38), up = x, down = x;
+                    for (int i = 0; i < 2; i++) {
+                        up = nextafterf(up, INFINITY);
+                        down = nextafterf(down, -INFINITY);
+                    }
+                    above = std::max(0, r.grid - place(up, h.scale));
+                    below = std::max(0, r.grid - place(down, h.scale));
+                }
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
@@ -410,7 +422,7 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
         if (tid == 0) p.row[row] = r;
         return;
     }
-    scan_all(tid < p.chunks ? factor[tid] * (double)mine.sum : 0.0, room, r.sum);
+    r.sum = over_all(tid < p.chunks ? factor[tid] * (double)mine.sum : 0.0, room, [](double a, double b) { return a + b; });
     double all;
     mass = scan_all(half ? 0.0 : mass, room, all);   // weight up to the bin
     if (!half) masses[b] = mass;
@@ -435,18 +447,6 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
         if (r.to == BINS) r.how = SEARCH;
     }
     if (h.least > 0.f && r.how == LIST) {
-        // min-p's border and two numbers to either side of it
-        const double border = (double)r.top + log((double)h.least) / h.inv;
-        int above = 0, below = BINS;
-        if (border == border && r.top < INFINITY) {
-            float x = (float)fmin(fmax(border, -3e38), 3e38), up = x, down = x;
-            for (int i = 0; i < 2; i++) {
-                up = nextafterf(up, INFINITY);
-                down = nextafterf(down, -INFINITY);
-            }
-            above = std::max(0, r.grid - place(up, h.scale));
-            below = std::max(0, r.grid - place(down, h.scale));
-        }
         if (below < r.from) {   // it decides alone
             r.from = above;
             r.to = below;
