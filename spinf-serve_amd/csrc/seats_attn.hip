@@ -791,9 +791,10 @@ __device__ __forceinline__ void join(const Params& p, int block) {
     const int sets = p.join_x * SLICES, y0 = block / sets, x0 = block - y0 * sets, slice = x0 % SLICES;
     const int group = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4, lane = threadIdx.x & 63, used = tokens_of(p);
     for (int tok0 = x0 / SLICES; tok0 < p.rows; tok0 += 64 * p.join_x) {
-    // of 64 tokens of this workgroup: where their pieces begin, and how many there are (0: the last word is spoken)
+    // of 64 tokens of this workgroup: where their pieces begin, and how many there are (0: the last word is spoken).  Behind the step's last token the list may be an older step's, of
+    // more rows, whose pieces are not in this call's workspace: nothing there counts
     const int at = tok0 + lane * p.join_x, begins = at < p.rows ? p.parts[at] : 0, ends = at < p.rows ? p.parts[at + 1] : 0;
-    const int number = at >= p.rows || begins < 0 || used > p.rows ? 0 : (ends & INT_MAX) - begins;
+    const int number = at >= used || used > p.rows || begins < 0 ? 0 : (ends & INT_MAX) - begins;
     unsigned long long left = __builtin_amdgcn_ballot_w64(number > 0 || ((at >= used || used > p.rows) && at < p.rows));
     while (left) {
     const int which = __builtin_ctzll(left), tok = tok0 + which * p.join_x;

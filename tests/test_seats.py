@@ -538,6 +538,44 @@ def test_rows_of_another_step_become_nan(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,small,large", [((8, 2, 64), 64, 256), ((16, 8, 256), 3, 200), ((16, 1, 512), 5, 160)])
+def test_attention_with_more_rows_than_the_last_step(dev, heads, small, large):
+    """a step of many rows that leaves pieces, then one of few, replayed: attention of more rows behind it gives the step's tokens, and zeros"""
+    stored, content, own = [3000, 90], [0] * 5 + [1] * 2 + [-1], [40, 1, 90, 7, 300, 33, 2, 60]
+    s, pages = make(dev, stored, own, [0] * 8, 16, heads, content, rows=large, keys=400, spare=60)
+    cache, q = fill(s, pages, heads, 6, dev)
+    few = [1, 0, 1, 0, 1, 0, 0, 0]
+    new = torch.tensor(few, dtype=torch.int32, device=dev)
+    drop = torch.zeros_like(new)
+    step, attn = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(step):
+        s.step(new, drop, rows=small)
+    s.step(torch.zeros_like(new))                         # (on the host the last step has as many rows as the seats were built for)
+    sa.seats_attn(q, cache, s)
+    with torch.cuda.graph(attn):
+        recorded = sa.seats_attn(q, cache, s, return_lse=True)
+    many = torch.tensor([20, 1, 20, 18, 20, 20, 9, 20], dtype=torch.int32, device=dev)
+    for i in range(3):
+        s.step(many)                                      # pieces of 128 rows
+        assert s.took.tolist() == many.tolist()
+        drop.copy_(many)                                  # ... which go again
+        step.replay()
+        junk = torch.full((1 << 24,), float("nan"), device=dev)   # (what a workspace may hold)
+        del junk
+        attn.replay()
+        torch.cuda.synchronize()
+        begins = s._work[ss._layout(s._geo)["lists"][0][5] :][: large + 1].cpu().numpy()
+        assert ((begins[4:] & 0x7FFFFFFF) - begins[3:-1]).max() > 1   # (the older step's pieces are listed still)
+        own = [n + m for n, m in zip(own, few)]
+        assert s.took.tolist() == few and s.lens.tolist() == own
+        want, wlse, tol, ltol = reference(q, cache, s, stored, content, own, few, heads[2] ** -0.5)
+        for out, lse in (recorded, sa.seats_attn(q, cache, s, return_lse=True)):
+            close(out[:3], want, tol)
+            close(lse[:3], wlse, ltol)
+            assert (out[3:] == 0).all() and (lse[3:] == float("-inf")).all()
+
+
+@pytest.mark.gpu
 def test_several_head_geometries_in_one(dev):
     """a model's kinds of layers: what each gets is what seats of that kind alone give"""
     kinds = [((16, 8, 64), 0), ((16, 8, 64), 50), ((16, 8, 64), 1000), ((8, 1, 512), 0), ((40, 8, 128), 0), ((64, 1, 64), 0), ((128, 1, 64), 30), ((1, 1, 256), 0)]
