@@ -11,7 +11,7 @@
 // Kernels.  chunks: a chunk's largest logit, its weight, and how many logits and how much weight lie in each of 255 bins, a twelfth of T wide, below its largest one (bins at whole
 // multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
 // of the bins in question.  draw: the borders among those few, then the chunk by the chunks' weights and the token in it.  Rows without a filter need the first and the last.  Where
-// bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself: 8 rows of 262,144 equal logits, top-p: 1.2 ms.
+// bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself: 8 rows of 262,144 equal logits, top-p: 1.3 ms.
 // Bound by instructions of 64 bits beside HBM (320 rows of 262,144: 88 us, 61 at the rate of a copy) where rows are many, by the four launches' latencies where they are few (one row: 27 us).
 #include <hip/hip_runtime.h>
 
@@ -501,15 +501,39 @@ __global__ __launch_bounds__(LANES) void sample_gather_kernel(const Params p) {
     }
 }
 
+// What tokens are worth in a sum: weights of a list, or counts, in `whole`, whatever their unit is; of a row's up to 2^22 tokens 2^40ths of its largest weight in `whole` and what is left of them in
+// 2^40ths of that in `rest` (signed), so that a sum stays below 2^63 and is off by 2^-59 at most.  (Top-p below 1 leaves 2^-24 of the weight behind its border at least, which among 2^22 tokens is one of 2^-46 at the border:
+// with units of 2^-38 alone, tails of equal logits 20 T and more below the largest were rounded to few units or none.)
+typedef unsigned __int128 u128;
+constexpr int REST = 40;
+struct Worth {
+    u64 whole, rest;
+    static __device__ __forceinline__ Worth of(double w) {   // the last bits of w + 2^12 and of what that leaves + 2^-28, rounded there
+        const double up = w + 0x1p12, left = w - (up - 0x1p12);
+        return {(u64)(__double_as_longlong(up) - __double_as_longlong(0x1p12)), (u64)(__double_as_longlong(left + 0x1.8p-28) - __double_as_longlong(0x1.8p-28))};
+    }
+    __device__ __forceinline__ u128 all() const { return ((u128)whole << REST) + (u128)(__int128)(long long)rest; }
+};
+// the least whole number that is at least p times x; p below 1, x below 2^104
+__device__ __forceinline__ u128 share(float p, u128 x) {
+    const unsigned b = __float_as_uint(p), e = b >> 23, m = (b & 0x7fffff) | (e ? 0x800000 : 0);
+    const int down = 150 - (int)(e ? e : 1);   // p = m / 2^down
+    const u64 low = (u64)x, high = (u64)(x >> 64);
+    const u128 y = ((u128)(high * m + __umul64hi(low, m)) << 64) + (u128)(low * m);
+    return down < 127 ? (y + (((u128)1 << down) - 1)) >> down : (u128)(y != 0);
+}
+
 // The least number up to which (it counted in) those of `each` hold at least `need` in all; ~0: all of them hold less.  each(f) calls f(number, worth) for every one in question,
-// each lane for its share; `some`: a number next to them.  By 256 stretches of them (`stretch`, where there is one, never falls from one number to a later one: floats near zero differ in all of their bits, and lie
-// close together), then by eight bits from the first that differs among those that are left (bf16 has few values to a bin: what is left may differ in its index alone), until they
-// are few and counted against each other.
+// each lane for its share; worth() is what it counts (rests: there are some); `some`: a number next to them.  By 256 stretches of them (`stretch`, where there is one, never falls from one number to a later one: floats near
+// zero differ in all of their bits, and lie close together), then by eight bits from the first that differs among those that are left (bf16 has few values to a bin: what is left may differ in its index
+// alone), until they are few and counted against each other.
 constexpr int LEFT = 64;
+struct SearchRoom { u64 whole[256], rest[256], one[256], found[4]; int counts[256]; };   // found: the digit or number, how many of the few are placed, what is still needed
 template <class E, class S>
-__device__ __forceinline__ u64 search(u64 need, u64 some, bool stretches, u64* sums, u64* one, int* counts, u64* found, u64* room, E each, S stretch) {
+__device__ __forceinline__ u64 search(u128 need, u64 some, bool stretches, bool rests, SearchRoom& at, u64* room, E each, S stretch) {
     u64 known = 0, prefix = some;
     int line = -1;   // the stretch, once it is known
+    const auto sum_of = [&](int d) __attribute__((always_inline)) { return Worth{at.whole[d], at.rest[d]}.all(); };
 #pragma unroll 1
     while (true) {
         const bool by_stretch = stretches && line < 0;
@@ -518,7 +542,7 @@ __device__ __forceinline__ u64 search(u64 need, u64 some, bool stretches, u64* s
         int low = 0;
         if (!by_stretch) {
             u64 open = 0;
-            each([&](u64 c, u64) __attribute__((always_inline)) { open |= in(c) ? c ^ prefix : 0; });
+            each([&](u64 c, auto) __attribute__((always_inline)) { open |= in(c) ? c ^ prefix : 0; });
             open = over_all(open, room, [](u64 a, u64 b) { return a | b; });
             const int top = 63 - __builtin_clzll(open | 1);
             low = top > 7 ? top - 7 : 0;
@@ -526,67 +550,79 @@ __device__ __forceinline__ u64 search(u64 need, u64 some, bool stretches, u64* s
         }
         __syncthreads();
         if (threadIdx.x < 256) {
-            sums[threadIdx.x] = 0;
-            counts[threadIdx.x] = 0;
+            at.whole[threadIdx.x] = at.rest[threadIdx.x] = 0;
+            at.counts[threadIdx.x] = 0;
         }
         if (threadIdx.x == 0) {
-            found[0] = found[1] = ~0ull;
-            found[2] = 0;
+            at.found[0] = ~0ull;
+            at.found[1] = 0;
         }
         __syncthreads();
-        each([&](u64 c, u64 worth) __attribute__((always_inline)) {
+        each([&](u64 c, auto worth) __attribute__((always_inline)) {
             if (!in(c)) return;
             const int digit = by_stretch ? stretch(c) : (int)((c & bits) >> low);
-            atomicAdd(&sums[digit], worth);
-            atomicAdd(&counts[digit], 1);
-            one[digit] = c;   // (any of them)
+            const Worth w = worth();
+            atomicAdd(&at.whole[digit], w.whole);
+            if (rests) atomicAdd(&at.rest[digit], w.rest);
+            atomicAdd(&at.counts[digit], 1);
+            at.one[digit] = c;   // (any of them)
         });
         __syncthreads();
         if (threadIdx.x < 64) {   // four digits a lane
             const int d0 = 4 * threadIdx.x;
-            const u64 mine = sums[d0] + sums[d0 + 1] + sums[d0 + 2] + sums[d0 + 3];
-            u64 upto = mine;
+            const auto upto = [&](const u64 (&x)[256]) __attribute__((always_inline)) {
+                u64 y = x[d0] + x[d0 + 1] + x[d0 + 2] + x[d0 + 3];
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const u64 y = __shfl_up(upto, d);
-                if ((int)threadIdx.x >= d) upto += y;
-            }
-            u64 before = upto - mine;
-            if (before < need && upto >= need) {
+                for (int d = 1; d < 64; d <<= 1) {
+                    const u64 z = __shfl_up(y, d);
+                    if ((int)threadIdx.x >= d) y += z;
+                }
+                return y;
+            };
+            const u128 end = Worth{upto(at.whole), rests ? upto(at.rest) : 0}.all();
+            u128 before = end - sum_of(d0) - sum_of(d0 + 1) - sum_of(d0 + 2) - sum_of(d0 + 3);
+            if (before < need && end >= need) {
                 int d = d0;
-                while (before + sums[d] < need) before += sums[d++];
-                found[0] = d;
-                found[1] = need - before;
+                while (before + sum_of(d) < need) before += sum_of(d++);
+                at.found[0] = d;
+                at.found[2] = (u64)(need - before);
+                at.found[3] = (u64)((need - before) >> 64);
             }
         }
         __syncthreads();
-        const u64 digit = found[0];
+        const u64 digit = at.found[0];
         if (digit == ~0ull) return ~0ull;   // (of the first pass alone)
-        need = found[1];
-        const int left = counts[digit];
+        need = (u128)at.found[3] << 64 | at.found[2];
+        const int left = at.counts[digit];
         if (left > LEFT) {   // (no two numbers are equal: it ends)
-            prefix = one[digit];   // (its bits up to here are the number's)
+            prefix = at.one[digit];   // (its bits up to here are the number's)
             if (by_stretch) line = (int)digit;
             else known |= bits;
             continue;
         }
-        __syncthreads();   // (`one` and `sums` take the few)
-        each([&](u64 c, u64 worth) __attribute__((always_inline)) {
+        __syncthreads();   // (`one` and the sums take the few)
+        each([&](u64 c, auto worth) __attribute__((always_inline)) {
             if (!in(c) || digit != (u64)(by_stretch ? stretch(c) : (int)((c & bits) >> low))) return;
-            const int i = (int)atomicAdd(&found[2], 1);
-            one[i] = c;
-            sums[i] = worth;
+            const int i = (int)atomicAdd(&at.found[1], 1);
+            const Worth w = worth();
+            at.one[i] = c;
+            at.whole[i] = w.whole;
+            at.rest[i] = w.rest;
         });
         __syncthreads();
         if ((int)threadIdx.x < left) {
-            const u64 c = one[threadIdx.x];
-            u64 before = 0;
+            const u64 c = at.one[threadIdx.x];
+            Worth ahead = {0, 0};
 #pragma unroll 4
-            for (int i = 0; i < left; i++) before += one[i] < c ? sums[i] : 0;
-            if (before < need && before + sums[threadIdx.x] >= need) found[0] = c;
+            for (int i = 0; i < left; i++) {
+                ahead.whole += at.one[i] < c ? at.whole[i] : 0;
+                if (rests) ahead.rest += at.one[i] < c ? at.rest[i] : 0;
+            }
+            const u128 before = ahead.all();
+            if (before < need && before + sum_of(threadIdx.x) >= need) at.found[0] = c;
         }
         __syncthreads();
-        return found[0];
+        return at.found[0];
     }
 }
 
@@ -595,8 +631,9 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
     __shared__ u64 room[WAVES];
     __shared__ u64 listed[FILTERS ? LISTED : 1], worth[FILTERS ? LISTED : 1];   // numbers of the tokens in question, and their weights
     __shared__ u64 chunks[MOST_CHUNKS];
-    __shared__ u64 sums[256], one[256], found[3];
-    __shared__ int counts[256], begins[MOST_CHUNKS + 1], room_n[WAVES];
+    __shared__ SearchRoom looked;
+    __shared__ u64 found[2];
+    __shared__ int begins[MOST_CHUNKS + 1], room_n[WAVES];
     __shared__ float tops[MOST_CHUNKS];
     __shared__ double factor[MOST_CHUNKS], target[2], steps[STEPS];
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -687,8 +724,7 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
                         if (x[a] > -INFINITY) f(x[a], i0 + a * LANES);
                 }
             };
-            // (of a whole row up to 2^22 tokens: units of 2^-38 leave room for the sum)
-            const auto coarse = [&](float x) __attribute__((always_inline)) { return (by_row.of(x) + 256) >> 9; };
+            const auto fine = [&](float x) __attribute__((always_inline)) { return Worth::of(by_row.fits ? by_row.w.of(x) : weight(x, r.top, h.by_two)); };   // of a whole row
 #pragma unroll 1
             for (int mass = 0; mass < 2; mass++) {
                 if (mass ? !by_mass : !by_number) continue;
@@ -697,37 +733,42 @@ __global__ __launch_bounds__(LANES) void sample_draw_kernel(const Params p) {
 #pragma unroll 1
                         for (int i = tid; i < n; i += LANES) {
                             const u64 c = listed[i];
-                            if (mass ? c <= last && (h.few || bin(c) <= r.to) : bin(c) == r.kth) f(c, mass ? worth[i] : 1);
+                            if (mass ? c <= last && (h.few || bin(c) <= r.to) : bin(c) == r.kth) f(c, [&]() __attribute__((always_inline)) { return Worth{mass ? worth[i] : 1, 0}; });
                         }
                     } else
                         of_row([&](float x, int i) __attribute__((always_inline)) {
                             const u64 c = number(x, i);
-                            if (c <= last) f(c, mass ? coarse(x) : 1);
+                            if (c <= last) f(c, [&]() __attribute__((always_inline)) { return mass ? fine(x) : Worth{1, 0}; });
                         });
                 };
-                u64 need = list ? h.k - r.before_k : h.k;
-                if (mass) {
-                    u64 w = 0;
+                u128 need = (u128)(list ? h.k - r.before_k : h.k) << REST;
+                if (mass && list) {
                     double mine = r.sum;   // weight of the first k
-                    if (!list || r.kth < BINS || h.few) {
-                        if (list) {
+                    if (r.kth < BINS || h.few) {
+                        u64 w = 0;
 #pragma unroll 1
-                            for (int i = tid; i < n; i += LANES)
-                                if (listed[i] <= last && (h.few || bin(listed[i]) == r.kth)) w += worth[i];
-                        } else
-                            of_row([&](float x, int i) __attribute__((always_inline)) {
-                                if (number(x, i) <= last) w += coarse(x);
-                            });
-                        mine = (double)sum_all(w, room);
-                        if (list) mine = (h.few ? 0.0 : r.mass_k) + UNIT * mine;
+                        for (int i = tid; i < n; i += LANES)
+                            if (listed[i] <= last && (h.few || bin(listed[i]) == r.kth)) w += worth[i];
+                        mine = (h.few ? 0.0 : r.mass_k) + UNIT * (double)sum_all(w, room);
                     }
-                    const double least_of = list ? ceil(((double)h.p * mine - r.mass_from) * 0x1p47) : ceil((double)h.p * mine);
-                    need = least_of < 1.0 ? 1 : (u64)least_of;
+                    const double least_of = ceil(((double)h.p * mine - r.mass_from) * 0x1p47);
+                    need = (u128)(least_of < 1.0 ? 1 : (u64)least_of) << REST;
+                } else if (mass) {
+                    Worth w = {0, 0};
+                    of_row([&](float x, int i) __attribute__((always_inline)) {
+                        if (number(x, i) > last) return;
+                        const Worth y = fine(x);
+                        w.whole += y.whole;
+                        w.rest += y.rest;
+                    });
+                    w.whole = sum_all(w.whole, room);
+                    w.rest = sum_all(w.rest, room);
+                    need = share(h.p, w.all());
                 }
                 // (a list's stretches: of the bins that it comes from)
                 const float begin = (float)(r.grid + 1 - (h.few ? 0 : mass ? r.from : r.kth)), wide = 256.f / (h.few ? std::min(r.kth, BINS) + 1 : mass ? r.to - r.from + 1 : 1);
                 const auto stretch = [&](u64 c) __attribute__((always_inline)) { return (int)__builtin_amdgcn_fmed3f((begin - value(c) * h.scale) * wide, 0.f, 255.f); };
-                last = std::min(last, search(need, number(r.top, 0), list, sums, one, counts, found, room, each, stretch));
+                last = std::min(last, search(need, number(r.top, 0), list, !list && mass, looked, room, each, stretch));
             }
         }
         // what is kept, by chunk

@@ -257,3 +257,60 @@ def test_the_chance_of_an_unlikely_token(dev, dtype):
     x[:, :3] = -np.inf
     for how in (dict(), dict(top_k=20000 - 3), dict(top_p=1.0, min_p=1e-14), dict(top_k=19000, temperature=1.1)):
         check(dev, x, dtype, np.zeros(6), how)
+
+
+def reach(weights, p):
+    """the first n of these whole numbers (largest first) hold p of their sum: n, and how far that border lies from its neighbours, in weights of the token at it; exact"""
+    mass = np.cumsum(np.asarray(weights, object))
+    num, den = float(np.float32(p)).as_integer_ratio()
+    n = int(np.searchsorted(mass * den, num * mass[-1])) + 1
+    over, under = mass[n - 1] * den - num * mass[-1], num * mass[-1] - (mass[n - 2] * den if n > 1 else 0)
+    return n, float(min(over, under) / (weights[n - 1] * den))
+
+
+ONE = 1 << 110   # what a weight of 1 is as a whole number
+
+
+def weigh(z):
+    """exp(z) as 64 bits of precision and more give it"""
+    return int(np.ldexp(np.exp(np.longdouble(z)), 110))
+
+
+# Borders far below the largest logit.  One token of weight 1 is the vocabulary's last, those of the tail are the first by index, so the kept ones are tokens 0 .. n - 2 and the last: u just below and
+# just above what the n - 1 weigh tells n.  A tail token weighs 10^-13 (2^-43.3) and more of the whole.  What may move the border, in weights of such a token: weights are right to 2^-43 of
+# themselves, which moves a border by (1 - p) / weight (at most 2^21) times that, 2^-22; p of the sum is a number of 64 bits, 2^-53 of the whole, 2^-9.  `reach` says how far it lies from the next.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tail,temperature,top_k,top_p,vocab", [
+    (torch.float32, -26.0, 1.0, 0, 0.9999995, 262144), (torch.float32, -26.0, 1.0, 0, 0.999999, 262144), (torch.bfloat16, -26.0, 1.0, 0, 0.9999995, 262144), (torch.float32, -13.5, 0.5, 0, 0.9999995, 262144),
+    (torch.float32, -24.0, 1.0, 0, 0.9999995, 40000), (torch.float32, -26.5, 1.0, 0, 0.9999998, 151936), (torch.bfloat16, -30.0, 1.0, 0, 0.9999999, 1 << 22), (torch.float32, -28.0, 1.0, 0, 0.999999, 1 << 22),
+    (torch.float32, -22.5, 1.0, 0, 0.99999, 262144), (torch.bfloat16, -20.0, 1.0, 0, 0.9999, 262144), (torch.float32, -26.0, 1.0, 200000, 0.9999995, 262144), (torch.float32, -12.0, 1.0, 150001, 0.7, 262144)])
+def test_borders_of_top_p_far_below_the_largest(dev, dtype, tail, temperature, top_k, top_p, vocab):
+    w, every = weigh(np.longdouble(tail) / np.longdouble(temperature)), top_k or vocab
+    n, free = reach([ONE] + [w] * (every - 1), top_p)
+    assert 5000 < n < every - 5000 and free > 2.0**-7
+    x = torch.full((3, vocab), tail, dtype=dtype, device=dev)
+    x[:, -1] = 0.0
+    kept = ONE + (n - 1) * w
+    u = np.array([(2 * n - 3) * w / (2 * kept), (2 * n - 1) * w / (2 * kept), w / (2 * kept)])
+    token, prob = sa.sample_tokens(x, torch.from_numpy(u).to(dev), temperature=temperature, top_k=top_k, top_p=top_p, return_prob=True)
+    assert token.tolist() == [n - 2, vocab - 1, 0], (n, free)
+    for got, want in zip(prob.tolist(), (w / kept, ONE / kept, w / kept)):
+        assert abs(got - want) <= want * 2.0**-22
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_k,top_p", [(0, 0.9999995), (0, 0.9999998), (250000, 0.9999996)])
+def test_borders_of_top_p_in_a_falling_tail(dev, top_k, top_p):
+    """the same with a tail that falls by index from 24 to 30 below the largest: no two weights are equal"""
+    vocab = 262144
+    tail = np.linspace(-24, -30, vocab - 1).astype(np.float32)
+    assert (np.diff(tail) < 0).all()
+    weights = [ONE] + [weigh(z) for z in tail]
+    every = top_k or vocab
+    n, free = reach(weights[:every], top_p)
+    assert 5000 < n < every - 5000 and free > 2.0**-7
+    x = torch.from_numpy(np.concatenate([tail, np.zeros(1, np.float32)])).to(dev)[None].repeat(2, 1)
+    before = sum(weights[1:n])   # the kept ones of the tail
+    u = np.array([(2 * before - weights[n - 1]) / (2 * (ONE + before)), (2 * before + weights[n]) / (2 * (ONE + before))])
+    token = sa.sample_tokens(x, torch.from_numpy(u).to(dev), top_k=top_k, top_p=top_p)
+    assert token.tolist() == [n - 2, vocab - 1], (n, free)
