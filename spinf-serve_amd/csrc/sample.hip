@@ -128,8 +128,11 @@ struct Weights {   // of a chunk, by its largest logit
         magic = 0x1.8p52 - B;
         c0 = g * C0; c1 = g * C1; c2 = g * C2; c3 = g * C3;
     }
-    // (where the next number below the largest lies hundreds of T away, the exponent would not hold its weight; beyond 2^30 steps the whole number its place)
-    static __device__ __forceinline__ bool fits(float top, const How& h) { return h.plain && fabs(top * (h.by_two * STEPS)) < 0x1p30 && top - nextafterf(top, -INFINITY) <= 8.f * h.far; }
+    // (where the next number below the largest lies hundreds of T away, the exponent would not hold its weight; beyond 2^30 steps the whole number its place; where there is no number 60 T below the largest, masked logits
+    // would have no weight to be given)
+    static __device__ __forceinline__ bool fits(float top, const How& h) {
+        return h.plain && fabs(top * (h.by_two * STEPS)) < 0x1p30 && top - nextafterf(top, -INFINITY) <= 8.f * h.far && top - h.far > -INFINITY;
+    }
     // exp((x - top) / T) to 2^-44 of it; of what lies some 60 T and more below, and of NaN: less than 2^-70
     __device__ __forceinline__ double of(float x) const {
         const double t = fmaxf(x, low), whole = __builtin_fma(t, by_step, magic), f = __builtin_fma(t, by_step, magic - whole);

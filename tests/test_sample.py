@@ -144,6 +144,18 @@ def test_draws_from_extreme_logits(dev, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [20011, 9000])
+def test_logits_near_the_lowest(dev, vocab):
+    """the largest some T above the least finite number, masked ones beside them: 60 T below it there is no number"""
+    g = np.random.default_rng(5)
+    x = -np.finfo(np.float32).max * (1 - 0.01 * g.random((3, vocab)))
+    x[g.random((3, vocab)) < 0.5] = -np.inf
+    for t in (9e35, 2e35, 3e36):
+        for how in HOW:
+            check(dev, x, torch.float32, g.random(3), {**how, "temperature": t})
+
+
+@pytest.mark.gpu
 def test_settings_of_every_row(dev):
     g = np.random.default_rng(8)
     rows = 96
