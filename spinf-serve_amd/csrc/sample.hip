@@ -379,7 +379,7 @@ __global__ __launch_bounds__(LANES) void sample_rows_kernel(const Params p) {
             if (c0 == half && h.least > 0.f && !h.few) {   // (while the bins are on their way)
                 const double border = (double)r.top + log((double)h.least) / h.inv;
                 if (border == border && r.top < INFINITY) {
-                    float x = (float)fmin(fmax(border, -3e38), 3e38), up = x, down = x;
+                    float x = (float)fmin(fmax(border, -0x1.fffffep127), 0x1.fffffep127), up = x, down = x;
                     for (int i = 0; i < 2; i++) {
                         up = nextafterf(up, INFINITY);
                         down = nextafterf(down, -INFINITY);

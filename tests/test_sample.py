@@ -156,6 +156,17 @@ def test_logits_near_the_lowest(dev, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["infinite", "masked", "largest", "flat"])
+def test_draws_at_temperatures_of_any_size(dev, kind):
+    """the largest that 32 bits hold, and subnormal ones"""
+    g = np.random.default_rng(4)
+    x = logits(kind, 4, 20011, 7)
+    for t in (3.4e38, 1e-38, 1e-45):
+        for how in HOW:
+            check(dev, x, torch.float32, g.random(4), {**how, "temperature": t})
+
+
+@pytest.mark.gpu
 def test_settings_of_every_row(dev):
     g = np.random.default_rng(8)
     rows = 96
