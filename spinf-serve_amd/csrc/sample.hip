@@ -71,6 +71,7 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
         h.k = 1;
     }
     if (h.k == 1) h.best = true;
+    h.least = fminf(h.least, 1.f);   // (what weighs as much as the largest stays: under an infinite T that is all finite ones)
     h.filtered = h.k || h.p < 1.f || h.least > 0.f;
     h.few = h.k && h.k <= FEW;
     return h;

@@ -167,6 +167,16 @@ def test_draws_at_temperatures_of_any_size(dev, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["masked", "largest", "flat"])
+def test_equal_weights_under_an_infinite_temperature(dev, kind):
+    """all finite logits weigh the same: none is less likely than the likeliest, whatever min-p"""
+    g = np.random.default_rng(4)
+    x = logits(kind, 4, 20011, 7)
+    for how in HOW:
+        check(dev, x, torch.float32, g.random(4), {**how, "temperature": float("inf")})
+
+
+@pytest.mark.gpu
 def test_settings_of_every_row(dev):
     g = np.random.default_rng(8)
     rows = 96
