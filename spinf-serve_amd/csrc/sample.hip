@@ -62,7 +62,7 @@ __device__ __forceinline__ How settings(const Params& p, int row) {
     h.best = T == 0.f;
     h.inv = p.temperature ? 1.0 / (double)T : p.all_inv;
     h.by_two = h.inv * 1.4426950408889634;
-    h.scale = fminf(BINS_PER_UNIT / T, 3e38f);
+    h.scale = fminf(fmaxf(BINS_PER_UNIT / T, 0x1p-126f), 3e38f);   // (T infinite: an infinite logit times 0 would have no place)
     h.far = 60.f * T;
     h.plain = T < 1e36f;   // (far is finite)
     if (h.k <= 0 || h.k >= p.vocab) h.k = 0;

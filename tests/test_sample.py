@@ -158,12 +158,14 @@ def test_logits_near_the_lowest(dev, vocab):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["infinite", "masked", "largest", "flat"])
 def test_draws_at_temperatures_of_any_size(dev, kind):
-    """the largest that 32 bits hold, and subnormal ones"""
+    """the largest that 32 bits hold, an infinite one (all finite logits weigh the same), and subnormal ones"""
     g = np.random.default_rng(4)
     x = logits(kind, 4, 20011, 7)
-    for t in (3.4e38, 1e-38, 1e-45):
+    for t in (3.4e38, float("inf"), 1e-38, 1e-45):
         for how in HOW:
             check(dev, x, torch.float32, g.random(4), {**how, "temperature": t})
+    how = dict(temperature=np.array([np.inf, 1.0, np.inf, 3.4e38], np.float32), top_k=np.array([7, 0, 5000, 300], np.int32), top_p=np.array([1, 0.9, 0.7, 1], np.float32))
+    check(dev, x, torch.float32, g.random(4), how)
 
 
 @pytest.mark.gpu
