@@ -573,8 +573,12 @@ void rooms(const spinf_seats_args* a, const spinf_seats_kind& k, int64_t out[5])
     out[1] = (SEAT_SHARED_ROWS + 31) / 32 * A;
     out[2] = block ? by_block + 2 * (rows * group / 128 + A) : 0;
     out[3] = seats_last((int)group, k.d) && seats_last_pays(A, 0, k.hkv) ? A : 0;
-    // tokens x pieces: those of a set's blocks share the places; a token is in two sets at most
-    out[4] = 2 * rows + (32 / group + 1) * by_wave + (block ? (128 / group + 1) * by_block : 0);
+    // Partial rows: tokens x pieces.  A set's pieces are at most tiles / size + 1, its tokens at most a block's rows over `group` for each block, and blocks x tiles / size of all sets no more than
+    // the places: a term for the places, and one piece for each token of a set.  Tokens of seats that share their content's reading (up to SEAT_SHARED_ROWS rows each) are in two sets.  A
+    // seat of more rows is one set, and leaves pieces only where it has two and more: those are less than twice tiles / size, so its tokens have no term of their own (48 prompts of 100,805 rows in all, 16 heads on 8
+    // of 256: 13,619 partial rows; two to each row would be 3.4 GB of workspace).
+    const int64_t shared = std::min<int64_t>(rows, A * (SEAT_SHARED_ROWS / group));
+    out[4] = 2 * shared + (32 / group + 1) * by_wave + (block ? 2 * (128 / group + 1) * by_block : 0);
 }
 
 int check(const spinf_seats_args* a, const char* what) {

@@ -316,6 +316,39 @@ def test_lists_never_outgrow_their_rooms(dev):
                 assert all(n <= room for n, room in zip(counts, ss._rooms(s._geo, k)))
 
 
+def test_prompts_need_little_room_for_pieces(lib):
+    """a step whose rows are a few seats' whole prompts: partial rows go by the seats and the places, not by the rows"""
+    a, rooms = _lib.SeatsArgs(), (C.c_int64 * 5)()
+    a.seats, a.rows, a.page, a.keys, a.pool, a.longest, a.kinds = 48, 100805, 64, 4216, 3400, 470, 1
+    for hq, hkv, d in ((16, 8, 256), (24, 4, 256), (16, 1, 512), (32, 16, 128), (8, 8, 64)):
+        a.kind[0].hq, a.kind[0].hkv, a.kind[0].d = hq, hkv, d
+        assert lib.spinf_seats_rooms(C.byref(a), 0, rooms) == 0
+        assert rooms[4] < 30000   # (two to each row would be 201,610)
+
+
+@pytest.mark.gpu
+def test_lists_of_prompts_never_outgrow_their_rooms(dev):
+    """prompts of any length, on both sides of where a seat reads its content for itself, below long and short contents"""
+    rng = np.random.default_rng(9)
+    heads = [(16, 8, 256), (16, 1, 512), (8, 8, 64), (24, 4, 256, 1024), (96, 1, 64), (97, 1, 64, 64), (24, 12, 128)]
+    for i in range(12):
+        R, page, keys = int(rng.choice([1, 3, 24, 48, 300])), 64, 30000
+        stored = [int(rng.choice([33, 2000, 60000])), 470]
+        at = np.cumsum([0] + [-(-n // page) for n in stored])
+        s = sa.PagedSeats.build(R, 40000, page, keys, np.arange(1000 + 3 * R) + at[-1], contents=(stored, [np.arange(a, b) for a, b in zip(at[:-1], at[1:])]), heads=heads, device=dev)
+        for lengths in ([12], [12, 13], [1, 6, 7, 48, 49, 96, 97], [1, 1, 1, 3000], [500, 2000, 20000], [1, 12, 300]):
+            s.content.copy_(torch.from_numpy(np.sort(rng.integers(-1, 2, R)).astype(np.int32)))
+            for drop in (1 << 30, 0):   # (the second time below what the first one left)
+                s.step(torch.from_numpy(rng.choice(lengths, R).astype(np.int32)).to(dev), torch.full((R,), drop, dtype=torch.int32, device=dev))
+                rows = int(s.first[-1])
+                for k in range(len(heads)):
+                    lists, a, rooms = ss._layout(s._geo)["lists"][k], ss._numbers(s._geo), (C.c_int64 * 5)()
+                    counts = s._work[lists[4] : lists[4] + 5].tolist()
+                    a.rows = max(rows, 1)   # (what attention of as many rows as there are tokens has)
+                    assert _lib.load_library().spinf_seats_rooms(C.byref(a), k, rooms) == 0
+                    assert all(n <= room for n, room in zip(counts, rooms)), (heads[k], R, rows, counts, list(rooms))
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def fill(s, pages, heads, seed, device, order="heads", peaky=True):
     hq, hkv, d = heads
