@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .paged import _whole
 
 _SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32))
 
@@ -73,10 +74,10 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ret
     given, numbers = [], []
     for (name, _), x in zip(_SETTINGS, (temperature, top_k, top_p, min_p)):
         given.append(x if isinstance(x, torch.Tensor) else None)
-        n = 0.0 if isinstance(x, torch.Tensor) else float(x)
-        if not n >= 0.0 or (name == "top_k" and n != int(n)):
+        n = 0.0 if isinstance(x, torch.Tensor) else _whole(x, "sample_tokens: top_k") if name == "top_k" else float(x)
+        if not n >= 0:
             raise ValueError(f"sample_tokens: {name} {x}")
-        numbers.append(min(n, float(1 << 30)) if name == "top_k" else n)
+        numbers.append(float(min(n, 1 << 30)) if name == "top_k" else n)
     run = _sample if _lib.eager(logits, u, *given) else _sample_op
     token, prob = run(logits, u, *given, numbers, bool(return_prob))
     return (token, prob) if return_prob else token

@@ -21,6 +21,17 @@ def test_draws_refuse_what_they_do_not_take(lib):
             sa.sample_tokens(x, u, **how)
 
 
+def test_a_top_k_of_any_size(lib):
+    """a whole number, however large (more than there are: all); what is none is a ValueError as other settings are"""
+    x, u = torch.zeros((2, 8)), torch.zeros(2)
+    for k in (float("inf"), float("nan"), 2.5, -1, np.float32("inf")):
+        with pytest.raises(ValueError):
+            sa.sample_tokens(x, u, top_k=k)
+    for k in (3.0, np.int64(7), 1 << 40, 10**30):
+        with pytest.raises(RuntimeError):   # (no CPU path)
+            sa.sample_tokens(x, u, top_k=k)
+
+
 def test_the_c_entry_refuses_bad_arguments(lib):
     x = torch.zeros(64)
     need = C.c_int64()
