@@ -343,6 +343,11 @@ def eager(first, *tensors) -> bool:
     return True
 
 
+def lasting(key) -> bool:
+    """May a call's argument block be kept under this key?  Not where a number among its parts is a tensor: that may be written in place"""
+    return not any(isinstance(x, torch.Tensor) for x in key)
+
+
 def same_device(device, *tensors) -> None:
     """raises unless every tensor lies on `device`: a kernel that is handed an address of another memory faults"""
     for t in tensors:

@@ -281,6 +281,8 @@ class PagedBatch:
 
     def keep(self, key, args, device, *geometry):
         """notes an argument block with what it points into: the plan of `geometry`, if any, and the batch's own data"""
+        if not _lib.lasting(key):
+            return
         shared = [self._dev[1]] + ([self._plans[(*geometry, VARIANT)][3]] if geometry else [])
         if len(self._calls) > 256:
             self._calls.clear()

@@ -339,11 +339,12 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     if eager:
         a = _attn_block(*args)
         out, lse = _attn_run(a, q, k, v, return_lse)
-        if len(seats._calls) > 256:
-            seats._calls.clear()
-        for x in ("q", "k", "v", "out", "lse", "workspace"):
-            setattr(a, x, None)
-        seats._calls[key] = bytes(a)
+        if _lib.lasting(key):
+            if len(seats._calls) > 256:
+                seats._calls.clear()
+            for x in ("q", "k", "v", "out", "lse", "workspace"):
+                setattr(a, x, None)
+            seats._calls[key] = bytes(a)
     else:
         out, lse = _attn_op(*args, bool(return_lse))
     return (out, lse) if return_lse else out

@@ -833,6 +833,30 @@ def test_seats_and_their_tensors_refused_on_the_device(dev):
 
 
 @pytest.mark.gpu
+def test_numbers_that_are_written_in_place(dev):
+    """a scale, cap or window given as a tensor counts as what it holds at the call"""
+    heads, stored, content, own, new = (8, 2, 64), [100], [0, 0], [20, 30], [1, 1]
+    s, pages = make(dev, stored, own, new, 16, heads, content)
+    cache, q = fill(s, pages, heads, 1, dev)
+    need = -(-30 // 16)
+    batch = sa.PagedBatch.build([1], [30], [s.table[1, :need].tolist()], 16, dev)
+    for first, second in ((dict(scale=0.1), dict(scale=0.3)), (dict(softcap=5.0), dict(softcap=0.5))):
+        (name, x), y = *first.items(), *second.values()
+        given = torch.tensor(x)
+        for call in (lambda **how: sa.seats_attn(q, cache, s, **how), lambda **how: sa.paged_attn(q[:1], cache, batch, **how)):
+            given.fill_(x)
+            one = call(**{name: given})
+            given.fill_(y)
+            two = call(**{name: given})
+            assert torch.equal(one, call(**first)) and torch.equal(two, call(**second)) and not torch.equal(one, two)
+    given = torch.tensor(1)
+    one = sa.paged_attn(q[:1], cache, batch, window=given)
+    given.fill_(20)
+    two = sa.paged_attn(q[:1], cache, batch, window=given)
+    assert torch.equal(one, sa.paged_attn(q[:1], cache, batch, window=1)) and torch.equal(two, sa.paged_attn(q[:1], cache, batch, window=20)) and not torch.equal(one, two)
+
+
+@pytest.mark.gpu
 def test_the_example_of_answers_token_by_token(dev):
     import importlib.util
     import os
