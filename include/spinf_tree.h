@@ -495,7 +495,7 @@ int spinf_seats_attn_fwd(const spinf_seats_attn_args* args, void* stream);
  * Tokens drawn from logits [rows, vocab] (fp32: dtype 0, bf16: 1; rows ld elements apart) by given random numbers u [rows] in 0 .. 1 (fp32, or fp64 with u_f64); the reference draws
  * none.  Of each row: temperature T, top-k, top-p and min-p, [rows] device arrays or (NULL) one number for all.  Order: larger logits first, of equal ones the lower index; weight w = exp((x -
  * max) / T).  Kept are the first top_k of the order (below 1, or vocab and more: all), of these the shortest beginning with at least top_p of their weight (1 and more: all; the first in any
- * case), of these the tokens with w >= min_p of the largest weight.  token [rows] int64: the first by index up to which the kept weights add up to more than u times their sum (u at or
+ * case), of these the tokens with w >= min_p (above 1: 1) of the largest weight.  token [rows] int64: the first by index up to which the kept weights add up to more than u times their sum (u at or
  * above 1: the last kept one; below 0 or NaN: the first); prob [rows] fp32 or NULL: its share of the kept weights.  T 0: the first of the order.  Logits of -inf and NaN are never drawn; where one
  * is +inf, those that are share the weight.  token -1 and prob 0 where no logit is left, or T, top_p or min_p of the row is negative or NaN.
  * Weights are 64-bit, summed without rounding in units of 2^-47 of the largest of 8,192 neighbours: one of less than half a unit is none, also where u is 0 or 1.  Two launches, four where a filter is given; the workspace is the caller's, nothing is allocated. */

@@ -12,7 +12,9 @@
 // multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
 // of the bins in question.  draw: the borders among those few, then the chunk by the chunks' weights and the token in it.  Rows without a filter need the first and the last.  Where
 // bins tell too little (a border far below the largest logit, thousands of equal logits) the draw looks through the row itself: 8 rows of 262,144 equal logits, top-p: 1.3 ms.
-// Bound by instructions of 64 bits beside HBM (320 rows of 262,144: 88 us, 61 at the rate of a copy) where rows are many, by the four launches' latencies where they are few (one row: 27 us).
+// Where rows are many (320 of 262,144: 88 us, 61 at the rate of a copy) the chunks take 27 vector instructions a logit, nine of them of 64 bits, beside its bytes: they issue for 58 % of that kernel's time, the table of steps
+// keeps LDS busy for 16 % (half of it lanes that meet in a bank), waves wait for three quarters of theirs: a workgroup loads, then computes, and only others overlap it.  Where rows are few, the four launches'
+// latencies (one row: 27 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -46,7 +48,7 @@ struct Params {
     const void* logits; long ld; int vocab, rows, chunks; bool aligned;
     const void* u; bool u_f64;
     const float *temperature, *top_p, *min_p; const int* top_k;
-    float all_temperature, all_top_p, all_min_p; int all_top_k; double all_inv;   // (1 / T of all: a division of 64 bits is a tenth of a chunk's work)
+    float all_temperature, all_top_p, all_min_p; int all_top_k; double all_inv;   // (1 / T of all: a division of 64 bits was a tenth of a chunk's work)
     long* token; float* prob;
     Stat* stat; Row* row; int* hist_n; u64* hist_w; u64* kept; int* count; uint2* list;
 };
@@ -100,7 +102,7 @@ __device__ __forceinline__ double power(double t) {
     for (int k = 11; k >= 0; k--) y = __builtin_fma(y, f, c[k]);
     return __longlong_as_double(__double_as_longlong(y) + ((long long)(int)__double_as_longlong(whole) << 52));
 }
-// The same for a chunk's logits, where instructions of 64 bits are what bounds the kernel (each takes two of 32 bits).  With t = x / (T ln 2) in 256ths and B the whole number next to the
+// The same for a chunk's logits, where vector instructions are what takes longest beside the loads.  With t = x / (T ln 2) in 256ths and B the whole number next to the
 // largest logit's t: n = round(t) - B and what is left of t come of one product-and-sum each, exact but for the last bits; 2^(n / 256) by a table in LDS and the exponent, the rest by a
 // polynomial of degree 3 through the Chebyshev points of -1/2 .. 1/2 (off by 2^-45.7 at most), whose coefficients hold what the largest logit's own t is off from B: it weighs 1 to
 // 2^-44.  (320 rows of 262,144 logits: 90 us in all.  With differences from the largest logit, 32nds and degree 4 99, with the series above 120, with the library's exp 195.)

@@ -13,8 +13,10 @@
 // The lists' lengths are known on the GPU alone: grids have a bounded size and walk the lists.  A list without items costs 3 to 5 us of a launch.
 //
 // What bounds it.  24 answers below 301 tokens, 18 us: latency, three launches of one short item to a place each.  24 x 56 branches of one token on 470 + 9 keys, 77 us: the keys
-// alone would be 40 us, pieces written and read again are half as much.  48 answers below 65,536 tokens, 161 us (0.48 PFLOP/s), and 35 questions of 150 tokens in a window of 1,024, 169 us (0.52): the turns of a tile's products and its
-// softmax; the matrix unit is busy a third of the time, and at 256 dims two waves to a SIMD are all that fit: with 64 rows to a wave the accumulators spill, and eight waves
+// alone would be 40 us, pieces written and read again are half as much.  48 answers below 65,536 tokens, 161 us (0.48 PFLOP/s), and 35 questions of 150 tokens in a window of 1,024, 170 us (0.52): a
+// set's last block is mostly empty (288 and 300 rows are three blocks of 128: a third of all tiles are computed for 11 and 15 % of the rows), and a workgroup whose waves have no rows takes as long over a tile as a full one;
+// then the turns of a tile's products and its softmax.  The matrix unit is busy 30 % of the time; the same tiles and registers in paged_attn.hip's blocks, all of them full, keep it busy for 54 %.
+// At 256 dims two waves to a SIMD are all that fit: with 64 rows to a wave the accumulators spill, and eight waves
 // on the same tiles (four buffers) go in step, with nothing beside the softmax to feed the matrix unit: 146 for 129 us of the block kernel, 279 for 191.
 //
 // Keys that a row does not see leave no trace: as in paged_attn.hip, a workgroup that masked some tile and holds a result that is not finite looks whether masked tiles hold such

@@ -35,7 +35,8 @@ class PagedSeats:
       lens [seats]       own keys, the last step's new ones with them
       took, first        [seats] and [seats + 1]: the new tokens the last step gave each seat, and the row its first one is; first[-1]: rows in use
       table [seats, ceil(keys / page)], free [pool], left [1]: the seats' pages (behind a seat's keys: anything), the stack of free ones (its first left[0] entries)
-      slots [rows] int64, pos [rows]: the rows' places in the cache and positions, as qk_norm_rope_put takes them; -1 and 0 behind the last row
+      slots [rows] int64, pos [rows]: the rows' places in the cache and positions, as qk_norm_rope_put takes them; -1 and 0 behind the last row of as many as the last step had (behind those: an older
+                         step's; `step` returns its own)
 
     What `step` and `seats_attn` do is ordered as their streams are: calls that share seats follow each other.  A recorded graph reads and writes these tensors: they have to
     live as long as it is replayed."""
@@ -302,7 +303,7 @@ def seats_attn(q, cache: PagedCache, seats: PagedSeats, scale=None, window=None,
     Seats one after the other below the same content share its reading: put them next to each other.  fp32 throughout, but for the probabilities, each rounded to bf16 once for the
     product with its value, as in paged_attn (one token on few keys of its own: not rounded).  How keys are cut into pieces goes by all lengths of the step: the same step gives the same bits, a
     row beside other seats differs in the rounding of its sums.  What a row does not see may be anything, NaN and infinities too.
-    The rows are the last step's (its ``rows``); replayed behind a step of more tokens than q has rows, all of them are NaN.
+    The rows are the last step's (its ``rows``); replayed behind a step of more tokens than q has rows, all of them are NaN, behind one of fewer rows those after its tokens are zeros.
     (hq, key / value heads, d) and the window have to be among the seats' ``heads``.  The new tokens' own keys and values have to be in the cache (qk_norm_rope_put)."""
     k, v = cache.k, cache.v
     eager = _lib.eager(q, k, v)
