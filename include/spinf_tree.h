@@ -498,7 +498,8 @@ int spinf_seats_attn_fwd(const spinf_seats_attn_args* args, void* stream);
  * case), of these the tokens with w >= min_p (above 1: 1) of the largest weight.  token [rows] int64: the first by index up to which the kept weights add up to more than u times their sum (u at or
  * above 1: the last kept one; below 0 or NaN: the first); prob [rows] fp32 or NULL: its share of the kept weights.  T 0: the first of the order.  Logits of -inf and NaN are never drawn; where one
  * is +inf, those that are share the weight.  token -1 and prob 0 where no logit is left, or T, top_p or min_p of the row is negative or NaN.
- * Weights are 64-bit, summed without rounding in units of 2^-47 of the largest of 8,192 neighbours: one of less than half a unit is none, also where u is 0 or 1.  Two launches, four where a filter is given; the workspace is the caller's, nothing is allocated. */
+ * Weights are 64-bit, summed without rounding in units of 2^-47 of the largest of 8,192 neighbours: one of less than half a unit is none, also where u is 0 or 1.  (top_p's border: among at most 8,192 tokens in question, of the row's
+ * largest; among more, 2^-80 of it.)  Two launches, four where a filter is given; the workspace is the caller's, nothing is allocated. */
 typedef struct spinf_sample_args {
     const void* logits; int64_t ld, rows, vocab;
     const void* u; const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;

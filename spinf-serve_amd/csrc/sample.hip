@@ -6,7 +6,7 @@
 // drawn is the first, by index, up to which the kept weights add up to more than u times their sum.
 //
 // Where a border falls decides which token comes out, so weights are taken in 64 bits, and sums of them are sums of whole numbers: units of 2^-47 of the largest weight of a chunk
-// (8,192 logits), the same in any order.
+// (8,192 logits), the same in any order; where a border is looked for among listed tokens (8,192 at most), of the row's largest, and 2^-80 of it in a whole row.
 //
 // Kernels.  chunks: a chunk's largest logit, its weight, and how many logits and how much weight lie in each of 255 bins, a twelfth of T wide, below its largest one (bins at whole
 // multiples, so those of chunks fit together).  rows: the bins in which the k-th token and the border of p lie.  gather: weights of what is kept for certain, and the tokens
